@@ -171,6 +171,101 @@ NKIMOE_API int nkimoe_decode_attention(const void* qkv, const void* q_weight, co
                                        int64_t max_seq, float rope_theta, float eps, float scale, void* workspace,
                                        size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------- paged key-value cache
+ *
+ * A layer's cache is two pools k_pages / v_pages [num_pages, n_kv_heads,
+ * page_size, 128] (bf16, 16-byte aligned): the [n_kv_heads, page_size, 128]
+ * block of a page is contiguous, k_page_stride / v_page_stride elements lie
+ * between pages (multiples of 8).  page_size is 16, 32, 64, 128 or 256.  Row b
+ * of page_table (int32, table_stride apart) lists the max_pages pages of
+ * sequence b in order; -1 marks a page that is not held, and entries that a
+ * call does not need are not read.  A page that a call writes belongs to one
+ * sequence only (nkimoe_copy_pages makes one of a shared page).
+ *
+ * Visibility: the query at position p sees key s when s <= p and (window == 0
+ * or s > p - window or s < sinks): with a window the last `window` positions,
+ * p among them, and the first `sinks` ones.  Rotary angles are formed in 64
+ * bits (theta^(-i/64) * position), so far positions keep theirs.
+ *
+ * The workspace (status word, counters, scratch) must be zero-filled once
+ * before its first use; every call leaves its counters at zero, and any of
+ * these calls may share it on one stream.  Two launches that may run at the
+ * same time (two streams, two graphs) need a workspace each. */
+
+/* 0, or the id of the capture that `stream` is in (a workspace per captured
+ * graph is keyed by it). */
+NKIMOE_API int nkimoe_stream_capture_id(void* stream, unsigned long long* id);
+
+/* Prompt rows into the cache: the packed fused QKV rows qkv [T, (n_heads +
+ * 2*n_kv_heads) * 128] (bf16, before the q/k norms) of `batch` sequences get
+ * per-head q/k RMSNorm + rotate-half RoPE; the keys and values are stored in
+ * their pages and the queries written to q_out [T, n_heads * 128] (bf16, not
+ * overlapping qkv).  cu_seqlens int32 [batch + 1]: sequence b's rows are
+ * cu_seqlens[b] .. cu_seqlens[b+1] - 1; kv_lens int32 [batch]: its length with
+ * them, so its row i of n stands at position kv_lens[b] - n + i.  Rows from
+ * cu_seqlens[batch] on are left alone, in q_out too.  A row whose page is -1
+ * is not kept (a window has passed it); one outside the page table, or whose
+ * page id is not a page, is reported in *status (NKIMOE_DEV_BAD_INDEX).
+ * Reference: the q/k norms and RoPE of qwen_with_nki.py:330-350. */
+NKIMOE_API int nkimoe_qk_norm_rope_store(const void* qkv, const void* q_weight, const void* k_weight, int w_dtype,
+                                         const int32_t* cu_seqlens, const int32_t* kv_lens, void* k_pages,
+                                         void* v_pages, int64_t k_page_stride, int64_t v_page_stride,
+                                         int64_t num_pages, int64_t page_size, const int32_t* page_table,
+                                         int64_t table_stride, int64_t max_pages, void* q_out, int64_t T,
+                                         int64_t batch, int n_heads, int n_kv_heads, int head_dim, float rope_theta,
+                                         float eps, int* status, void* stream);
+
+NKIMOE_API size_t nkimoe_paged_decode_attention_workspace_bytes(int64_t batch, int n_heads, int n_kv_heads,
+                                                                int64_t max_pages, int64_t page_size);
+
+/* One decode step of grouped-query attention over the pages, fused as
+ * nkimoe_decode_attention is: sequence b's new token at p = positions[b *
+ * pos_stride] (int64, pos_stride 0 or 1) gets q/k RMSNorm + RoPE, its key and
+ * value are stored in their page, and query head h attends to the visible
+ * positions of kv head h / (n_heads / n_kv_heads).  out: bf16 [batch, n_heads
+ * * 128].  A negative position marks an idle row: nothing is stored, its
+ * output is zero; so is that of a position outside the page table, which is
+ * reported (NKIMOE_DEV_BAD_INDEX), as is a page that the query needs and that
+ * is not held (its positions count as invisible).  At most 16 query heads per
+ * kv head and 4096 sequences.
+ * Reference: nki_flash_attention_decode (nki_attention.py:252-373). */
+NKIMOE_API int nkimoe_paged_decode_attention(const void* qkv, const void* q_weight, const void* k_weight, int w_dtype,
+                                             const int64_t* positions, int64_t pos_stride, void* k_pages,
+                                             void* v_pages, int64_t k_page_stride, int64_t v_page_stride,
+                                             int64_t num_pages, int64_t page_size, const int32_t* page_table,
+                                             int64_t table_stride, int64_t max_pages, void* out, int64_t batch,
+                                             int n_heads, int n_kv_heads, int head_dim, float rope_theta, float eps,
+                                             float scale, int64_t window, int64_t sinks, void* workspace,
+                                             size_t workspace_bytes, void* stream);
+
+/* Copies page src[i] to page dst[i] (i < n) in each of `planes` pools of
+ * num_pages pages of page_bytes bytes (a multiple of 16), one behind the other
+ * at `pages`.  src and dst are HOST arrays, read before the call returns and
+ * checked there: ids in range, no page written twice, none both written and
+ * read (NKIMOE_ERR_INVALID_ARG, nothing copied).  A captured call keeps its
+ * ids.  No reference counterpart (the reference's cache is the runtime's). */
+NKIMOE_API int nkimoe_copy_pages(void* pages, int64_t planes, int64_t num_pages, int64_t page_bytes,
+                                 const int32_t* src, const int32_t* dst, int64_t n, void* stream);
+
+/* ---------------------------------------------------------------- token scores */
+
+NKIMOE_API size_t nkimoe_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top_n);
+
+/* Of each row of logits [rows, vocab] (fp32 or bf16, rows row_stride elements
+ * apart): the log probability of token tokens[r], the entropy of the row's
+ * distribution (nats) and its top_n (<= 32) most likely tokens with their log
+ * probabilities, equal logits in order of their id.  A negative token: none
+ * is given, its log probability comes out as 0; one >= vocab gives NaN.  A
+ * logit of -inf has probability zero; a row with a NaN, a +inf or nothing but
+ * -inf has no distribution: its results are NaN, its ids ordered with NaN
+ * above +inf.  Workspace: see the paged key-value cache; rows and vocab of any
+ * call may share it.
+ * Reference: the host-side logit comparison of main.py:296-378. */
+NKIMOE_API int nkimoe_token_logprobs(const void* logits, int dtype, int64_t row_stride, const int64_t* tokens,
+                                     int64_t rows, int64_t vocab, int top_n, float* logprob, float* entropy,
+                                     float* top_logprobs, int64_t* top_ids, void* workspace, size_t workspace_bytes,
+                                     void* stream);
+
 /* ---------------------------------------------------------------- decode projections */
 
 /* y[M, N] = x[M, K] . w[N, K]^T for decode batches, M <= 16 (bf16 in and out,

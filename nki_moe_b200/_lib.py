@@ -40,6 +40,15 @@ SIGNATURES = {
     "nkimoe_decode_attention_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i64]),
     "nkimoe_decode_attention": (_i, [_vp, _vp, _vp, _i, _vp, _i64, _vp, _vp, _vp, _i64, _i, _i, _i, _i64, _f, _f, _f,
                                      _vp, _sz, _vp]),
+    "nkimoe_stream_capture_id": (_i, [_vp, _c.POINTER(_c.c_ulonglong)]),
+    "nkimoe_qk_norm_rope_store": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64,
+                                       _vp, _i64, _i64, _i, _i, _i, _f, _f, _vp, _vp]),
+    "nkimoe_paged_decode_attention_workspace_bytes": (_sz, [_i64, _i, _i, _i64, _i64]),
+    "nkimoe_paged_decode_attention": (_i, [_vp, _vp, _vp, _i, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64,
+                                           _i64, _vp, _i64, _i, _i, _i, _f, _f, _f, _i64, _i64, _vp, _sz, _vp]),
+    "nkimoe_copy_pages": (_i, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "nkimoe_token_logprobs_workspace_bytes": (_sz, [_i64, _i64, _i]),
+    "nkimoe_token_logprobs": (_i, [_vp, _i, _i64, _vp, _i64, _i64, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "nkimoe_skinny_linear": (_i, [_vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "nkimoe_router_logits": (_i, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "nkimoe_topk_softmax": (_i, [_vp, _i64, _i64, _i64, _vp, _vp, _vp]),

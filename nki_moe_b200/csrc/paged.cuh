@@ -1,0 +1,130 @@
+// Shared by the kernels of the paged key-value cache: the cache's layout, the
+// rotary angles taken in 64 bits, and the q/k norms of half-warp heads.
+//
+// A layer's cache is two pools [num_pages, nkv, page_size, 128] (bf16; a
+// page's [nkv, page_size, 128] block is contiguous, the pages may be any
+// 8-element multiple apart), and row b of the page table lists the pages of
+// sequence b: position s lives in page table[b][s / page_size], row
+// s % page_size.  -1 marks a page that is not held.
+#pragma once
+
+#include <atomic>
+
+#include "kernels.h"
+#include "rope.cuh"
+
+namespace nkimoe {
+
+// Workspace of these kernels: a status word, counters that are zero between
+// calls, then scratch.  The first two have a fixed size, so calls of any of
+// the kernels and any shape may share one workspace on a stream.
+constexpr size_t kPagedStatusBytes = 256;
+constexpr int kPagedCounters = 1024;
+constexpr size_t kPagedScratch = kPagedStatusBytes + sizeof(int) * kPagedCounters;
+
+struct PagedCache {
+  __nv_bfloat16* k;
+  __nv_bfloat16* v;
+  long long k_stride, v_stride;  // elements between pages
+  const int* table;              // [B, max_pages]
+  long long table_stride;
+  int max_pages, num_pages, nkv;
+  int page_shift;  // log2 of the page size
+};
+
+// theta^(-i/64) / (2 pi): turns per position of each rotary frequency.  The
+// angle of a far position needs more bits than fp32 has (at position 10^5 an
+// fp32 angle is off by up to 4e-3 rad), so it is formed and reduced to a
+// fraction of a turn in 64 bits; the sine and cosine themselves are fp32.
+struct RopeTurns {
+  double f[kHeadDim / 2];
+};
+
+__device__ __forceinline__ float2 rope_cos_sin(double turns_per_pos, long long pos) {
+  double t = turns_per_pos * static_cast<double>(pos);
+  t -= rint(t);
+  float sn, cs;
+  sincospif(static_cast<float>(2.0 * t), &sn, &cs);
+  return make_float2(cs, sn);
+}
+
+// Whether the query at position p sees the key at position s.
+__device__ __forceinline__ bool key_visible(int s, int p, int window, int sinks) {
+  return s <= p && (window == 0 || s > p - window || s < sinks);
+}
+
+__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
+  const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
+  v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+  v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                    pack_bf16x2(v[6], v[7]));
+}
+
+// RMSNorm + rotate-half RoPE of one head held by a half-warp: lane l of the
+// sixteen owns elements [8l, 8l + 8), its rotate-half partner is lane l ^ 8.
+// `w` are the lane's norm weights, `cs` the cos / sin table of the position.
+__device__ __forceinline__ void norm_rope_half(const float (&x)[8], const float (&w)[8], const float2* cs, float eps,
+                                               int l, float (&o)[8]) {
+  float ss = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+  const float r = rsqrtf(ss * (1.f / kHeadDim) + eps);
+  float n[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) n[e] = x[e] * r * w[e];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float other = __shfl_xor_sync(0xffffffffu, n[e], 8);
+    const float2 t = cs[(l & 7) * 8 + e];
+    o[e] = fmaf(n[e], t.x, (l < 8 ? -other : other) * t.y);
+  }
+}
+
+__device__ __forceinline__ void load_weight8(const void* w, int w_dtype, int l, float (&o)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = head_wload(w, w_dtype, l * 8 + e);
+}
+
+// Lets a kernel take `bytes` of dynamic shared memory, once per device.
+template <auto kKernel>
+cudaError_t allow_smem(int bytes) {
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
+// ----------------------------------------------------------------- launches
+RopeTurns rope_turns(float theta);
+
+cudaError_t paged_store_launch(const __nv_bfloat16* qkv, const void* qw, const void* kw, int w_dtype,
+                               const int* cu_seqlens, const int* kv_lens, const PagedCache& cache,
+                               __nv_bfloat16* q_out, long long T, int B, int nq, float theta, float eps, int* status,
+                               cudaStream_t s);
+
+cudaError_t copy_pages_launch(void* pages, long long planes, long long plane_bytes, long long page_bytes,
+                              const int* src, const int* dst, long long n, cudaStream_t s);
+
+size_t paged_decode_workspace_bytes(long long B, int nq, int nkv, long long max_pages, int page_size);
+cudaError_t paged_decode_launch(const __nv_bfloat16* qkv, const void* qw, const void* kw, int w_dtype,
+                                const long long* positions, long long pos_stride, const PagedCache& cache,
+                                __nv_bfloat16* out, int B, int nq, float theta, float eps, float scale, int window,
+                                int sinks, void* workspace, cudaStream_t s);
+
+size_t token_logprobs_workspace_bytes(long long T, long long V, int top_n);
+cudaError_t token_logprobs_launch(const void* logits, int dtype, long long row_stride, const long long* tokens,
+                                  long long T, long long V, int top_n, float* logprob, float* entropy, float* top_lp,
+                                  long long* top_ids, void* workspace, cudaStream_t s);
+
+}  // namespace nkimoe

@@ -9,6 +9,7 @@ host buffers of :func:`moe_block_host`, whose block runs on the GPU.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 import weakref
@@ -25,7 +26,8 @@ __all__ = [
     "grouped_gemm", "swiglu", "aggregate", "read_status", "workspace", "sync_check_enabled", "router_split",
     "route", "dispatch", "segment_experts", "combine", "ep_dispatch", "decode_attention", "skinny_linear",
     "moe_block_add_rmsnorm", "moe_block_host", "kmajor_weights",
-    "release_captured_workspaces", "moe_block_rmsnorm",
+    "release_captured_workspaces", "moe_block_rmsnorm", "qk_norm_rope_store", "paged_decode_attention", "copy_pages",
+    "token_logprobs", "read_paged_status",
 ]
 
 _DT = {torch.float32: F32, torch.bfloat16: BF16, torch.int32: I32, torch.int64: I64}
@@ -245,6 +247,273 @@ def skinny_linear(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = N
         out = torch.empty(*x.shape[:-1], N, dtype=torch.bfloat16, device=x.device)
     call("nkimoe_skinny_linear", _p(x), _p(w), _p(out), M, N, K, _s(x))
     return out
+
+
+# ---------------------------------------------------------------- paged cache, token scores
+_paged_ws: dict = {}
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_PAGE_SIZES = (16, 32, 64, 128, 256)
+
+
+def _paged_workspace(dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+    """Zero-filled workspace of the paged-cache and token-score calls, one per
+    (device, stream).  A stream that is being captured gets one per capture,
+    allocated (and zeroed, as a node of the graph) in the graph's own memory,
+    so graphs that replay at the same time share none; only the latest
+    capture's is held here, the graph keeps the memory."""
+    capture = 0
+    if torch.cuda.is_current_stream_capturing():
+        cid = ctypes.c_ulonglong(0)
+        call("nkimoe_stream_capture_id", stream, ctypes.byref(cid))
+        capture = cid.value
+    key = (dev.index, stream, capture != 0)
+    with _ws_lock:
+        held = _paged_ws.get(key)
+        if held is None or held[0] != capture or held[1].numel() < nbytes:
+            held = (capture, torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=dev))
+            _paged_ws[key] = held
+        return held[1]
+
+
+def read_paged_status(device=None) -> None:
+    """Synchronises ``device`` and raises if a paged-cache call on it met a
+    position or page id out of range, or a page that it needed and that was
+    not held (the status is cleared)."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    index = torch.cuda.current_device() if dev.index is None else dev.index
+    torch.cuda.synchronize(index)
+    with _ws_lock:
+        held = [(k[1], v[1]) for k, v in _paged_ws.items() if k[0] == index]
+    bad = None
+    with torch.cuda.device(index):
+        for _, ws in held:
+            try:
+                call("nkimoe_read_status", ws.data_ptr(), _raw_stream(index), None)
+            except _lib.NKIMoEError as e:
+                bad = e
+    if bad is not None:
+        raise bad
+
+
+def _same_device(dev: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, expected {dev}")
+
+
+def _on_its_device(fn):
+    """Runs ``fn`` with its first argument's device as the current one (its
+    kernels launch there, on that device's current stream)."""
+    @functools.wraps(fn)
+    def run(*args, **kw):
+        t = args[0] if args else next(iter(kw.values()), None)
+        if isinstance(t, torch.Tensor) and t.is_cuda and t.device.index != torch._C._cuda_getDevice():
+            with torch.cuda.device(t.device):
+                return fn(*args, **kw)
+        return fn(*args, **kw)
+    return run
+
+
+def _norm_weights(q_weight: torch.Tensor, k_weight: torch.Tensor):
+    wdt = torch.float32 if q_weight.dtype == torch.float32 else torch.bfloat16
+    qw, kw = _contig(_cuda(q_weight, "q_weight"), wdt), _contig(_cuda(k_weight, "k_weight"), wdt)
+    if qw.numel() != 128 or kw.numel() != 128:
+        raise ValueError("q_weight and k_weight must have 128 elements")
+    return qw, kw, _DT[wdt]
+
+
+def _paged_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, n_kv_heads: int,
+                 batch: int):
+    """Checks one layer's pools and the page table of ``batch`` sequences and
+    returns their C arguments."""
+    for name, c in (("k_pages", k_pages), ("v_pages", v_pages)):
+        shape, st = c.shape, c.stride()
+        if not c.is_cuda or c.dtype != torch.bfloat16 or len(shape) != 4 or shape[1] != n_kv_heads or shape[3] != 128:
+            raise ValueError(f"{name} must be CUDA bf16 [pages, {n_kv_heads}, page_size, 128]")
+        if shape[2] not in _PAGE_SIZES:
+            raise ValueError(f"page size {shape[2]} (one of {_PAGE_SIZES})")
+        if shape[0] == 0 or st[3] != 1 or st[2] != 128 or (shape[1] > 1 and st[1] != 128 * shape[2]):
+            raise ValueError(f"{name}: the pages themselves must be contiguous")
+    if v_pages.shape != k_pages.shape:
+        raise ValueError("k_pages and v_pages differ in shape")
+    if not page_table.is_cuda or page_table.dtype != torch.int32 or page_table.dim() != 2 \
+            or page_table.shape[0] < batch or page_table.shape[1] == 0 or page_table.stride(1) != 1:
+        raise ValueError(f"page_table must be CUDA int32 [>= {batch}, pages per sequence] with contiguous rows")
+    page = n_kv_heads * k_pages.shape[2] * 128
+    kst, vst = (c.stride(0) if c.shape[0] > 1 else page for c in (k_pages, v_pages))
+    tst = page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1]
+    return (k_pages.data_ptr(), v_pages.data_ptr(), kst, vst, k_pages.shape[0], k_pages.shape[2],
+            page_table.data_ptr(), tst, page_table.shape[1])
+
+
+def _lengths(cu_seqlens: torch.Tensor, kv_lens: torch.Tensor) -> int:
+    for name, t in (("cu_seqlens", cu_seqlens), ("kv_lens", kv_lens)):
+        if not t.is_cuda or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous CUDA int32 vector")
+    if cu_seqlens.shape[0] != kv_lens.shape[0] + 1:
+        raise ValueError(f"cu_seqlens has {cu_seqlens.shape[0]} entries for {kv_lens.shape[0]} sequences")
+    return kv_lens.shape[0]
+
+
+@_on_its_device
+def qk_norm_rope_store(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cu_seqlens: torch.Tensor,
+                       kv_lens: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                       n_heads: int, n_kv_heads: int, theta: float = 1e6, eps: float = 1e-6,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """Prompt rows into a paged cache: per-head q/k RMSNorm + rotate-half RoPE
+    of the packed QKV rows, keys and values stored in their pages, queries
+    returned.
+
+    ``qkv``: ``[T, (n_heads + 2*n_kv_heads) * 128]`` bf16; ``cu_seqlens``:
+    int32 ``[B + 1]``, the first row of each sequence; ``kv_lens``: int32
+    ``[B]``, its length with the new rows (row ``i`` of ``n`` stands at
+    ``kv_len - n + i``); ``k_pages``/``v_pages``: one layer's ``[pages,
+    n_kv_heads, page_size, 128]`` bf16 pools, updated in place;
+    ``page_table``: int32 ``[B, pages per sequence]`` (-1: not kept).  Returns
+    the queries ``[T, n_heads, 128]`` bf16 (``out``, contiguous, if given);
+    rows from ``cu_seqlens[B]`` on are left as they were."""
+    _cuda(qkv, "qkv")
+    row = (n_heads + 2 * n_kv_heads) * 128
+    if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != row or not qkv.is_contiguous():
+        raise ValueError(f"qkv must be a contiguous bf16 [T, {row}] tensor")
+    T, dev = qkv.shape[0], qkv.device
+    B = _lengths(cu_seqlens, kv_lens)
+    qw, kw, wdt = _norm_weights(q_weight, k_weight)
+    cache = _paged_cache(k_pages, v_pages, page_table, n_kv_heads, B)
+    _same_device(dev, q_weight=qw, k_weight=kw, cu_seqlens=cu_seqlens, kv_lens=kv_lens, k_pages=k_pages,
+                 v_pages=v_pages, page_table=page_table)
+    if out is None:
+        out = torch.empty(T, n_heads, 128, dtype=torch.bfloat16, device=dev)
+    elif out.dtype != torch.bfloat16 or out.shape != (T, n_heads, 128) or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f"out must be a contiguous bf16 [{T}, {n_heads}, 128] tensor on {dev}")
+    s = _raw_stream(dev.index)
+    ws = _paged_workspace(dev, s, 0)
+    call("nkimoe_qk_norm_rope_store", qkv.data_ptr(), qw.data_ptr(), kw.data_ptr(), wdt,
+             cu_seqlens.data_ptr(), kv_lens.data_ptr(), *cache, out.data_ptr(), T, B, n_heads, n_kv_heads, 128,
+             theta, eps, ws.data_ptr(), s)
+    if sync_check_enabled():
+        read_status(ws)
+    return out
+
+
+@_on_its_device
+def paged_decode_attention(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                           positions: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                           page_table: torch.Tensor, n_heads: int, n_kv_heads: int, theta: float = 1e6,
+                           eps: float = 1e-6, scale: float | None = None, window: int = 0, sinks: int = 0,
+                           out: torch.Tensor | None = None) -> torch.Tensor:
+    """One decode step of grouped-query attention over a paged cache, fused
+    with the q/k RMSNorm + RoPE of the step's token and the store of its key
+    and value in its page (:func:`decode_attention` on pages).
+
+    ``qkv``: ``[B, (n_heads + 2*n_kv_heads) * 128]`` bf16 before the norms;
+    ``positions``: int64 ``[B]`` or ``[1]``, a negative one marks an idle row
+    (nothing is stored, its output is zero); ``k_pages``/``v_pages``/
+    ``page_table`` as in :func:`qk_norm_rope_store`.  With ``window > 0`` the
+    query at ``p`` sees the last ``window`` positions up to ``p`` and the first
+    ``sinks`` ones; pages that lie outside both need not be held.  Returns
+    ``[B, n_heads * 128]`` bf16."""
+    _cuda(qkv, "qkv")
+    row = (n_heads + 2 * n_kv_heads) * 128
+    if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != row or not qkv.is_contiguous():
+        raise ValueError(f"qkv must be a contiguous bf16 [B, {row}] tensor")
+    B, dev = qkv.shape[0], qkv.device
+    if not positions.is_cuda or positions.dtype != torch.int64 or not positions.is_contiguous():
+        raise ValueError("positions must be a contiguous CUDA int64 tensor")
+    n_pos = positions.numel()
+    if n_pos != B and n_pos != 1:
+        raise ValueError(f"positions has {n_pos} entries for {B} sequences")
+    qw, kw, wdt = _norm_weights(q_weight, k_weight)
+    cache = _paged_cache(k_pages, v_pages, page_table, n_kv_heads, B)
+    _same_device(dev, q_weight=qw, k_weight=kw, positions=positions, k_pages=k_pages, v_pages=v_pages,
+                 page_table=page_table)
+    if out is None:
+        out = torch.empty(B, n_heads * 128, dtype=torch.bfloat16, device=dev)
+    elif out.dtype != torch.bfloat16 or out.shape != (B, n_heads * 128) or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f"out must be a contiguous bf16 [{B}, {n_heads * 128}] tensor on {dev}")
+    s = _raw_stream(dev.index)
+    nbytes = size_call("nkimoe_paged_decode_attention_workspace_bytes", B, n_heads, n_kv_heads, cache[8], cache[5])
+    ws = _paged_workspace(dev, s, nbytes)
+    call("nkimoe_paged_decode_attention", qkv.data_ptr(), qw.data_ptr(), kw.data_ptr(), wdt,
+             positions.data_ptr(), 0 if n_pos == 1 else 1, *cache, out.data_ptr(), B, n_heads, n_kv_heads, 128, theta,
+             eps, 128 ** -0.5 if scale is None else scale, window, sinks, ws.data_ptr(), ws.numel(), s)
+    if sync_check_enabled():
+        read_status(ws)
+    return out
+
+
+def _page_ids(ids, name: str) -> torch.Tensor:
+    t = torch.as_tensor(ids)
+    if t.is_cuda or t.dim() != 1 or (t.numel() and t.dtype not in (torch.int32, torch.int64)):
+        raise ValueError(f"{name} must be a list or CPU vector of page ids (page bookkeeping is host data)")
+    if t.dtype == torch.int64 and t.numel() and (int(t.max()) > 0x7fffffff or int(t.min()) < -0x80000000):
+        raise ValueError(f"{name} holds ids that are not page ids")
+    return _contig(t, torch.int32)
+
+
+@_on_its_device
+def copy_pages(pages: torch.Tensor, src, dst) -> torch.Tensor:
+    """Copies page ``src[i]`` to page ``dst[i]`` in every plane of a pool, in
+    place: forks (the last page of a sequence that two continue) and
+    compactions, all layers' keys and values in one launch.
+
+    ``pages``: contiguous CUDA tensor ``[..., pages, n_kv_heads, page_size,
+    head_dim]`` of any type (a stack's pool is ``[layers, 2, pages, ...]``);
+    ``src``/``dst``: lists or CPU vectors.  Ids out of range, a page written
+    twice, or one that is both read and written are refused before anything
+    is copied.  Returns ``pages``."""
+    _cuda(pages, "pages")
+    if pages.dim() < 4 or not pages.is_contiguous():
+        raise ValueError("pages must be contiguous [..., pages, n_kv_heads, page_size, head_dim]")
+    src, dst = _page_ids(src, "src"), _page_ids(dst, "dst")
+    if src.numel() != dst.numel():
+        raise ValueError(f"{src.numel()} source pages for {dst.numel()} destinations")
+    if src.numel() == 0:
+        return pages
+    shape, dev = pages.shape, pages.device
+    page_bytes = shape[-1] * shape[-2] * shape[-3] * pages.element_size()
+    if pages.numel() == 0:
+        raise ValueError("pages is empty")
+    call("nkimoe_copy_pages", pages.data_ptr(), pages.numel() // (shape[-1] * shape[-2] * shape[-3] * shape[-4]),
+             shape[-4], page_bytes, src.data_ptr(), dst.data_ptr(), src.numel(), _raw_stream(dev.index))
+    return pages
+
+
+@_on_its_device
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0):
+    """Scores of given tokens under rows of logits, in one pass over them:
+    ``(logprob [T], entropy [T], top_logprobs [T, top_n], top_ids [T,
+    top_n])``, fp32 and int64.
+
+    ``logits``: ``[T, V]`` bf16 or fp32, rows at any stride; ``tokens``: int64
+    ``[T]`` (negative: none given, its logprob is 0; ``>= V``: NaN).  The
+    ``top_n`` (at most 32) most likely tokens come in order, equal logits by
+    the lower id.  -inf logits have probability zero; a row with a NaN, a +inf
+    or only -inf has no distribution and gives NaN."""
+    _cuda(logits, "logits")
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("logits must be fp32 or bf16 [T, V]")
+    T, V = logits.shape
+    if V == 0 or (V > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must have contiguous, non-empty rows")
+    if not tokens.is_cuda or tokens.dtype != torch.int64 or tokens.shape != (T,) or not tokens.is_contiguous():
+        raise ValueError(f"tokens must be a contiguous CUDA int64 [{T}] tensor")
+    if not 0 <= top_n <= min(32, V):
+        raise ValueError(f"top_n {top_n} is not in [0, min(32, {V})]")
+    dev = logits.device
+    _same_device(dev, tokens=tokens)
+    # one allocation for the two fp32 vectors, handed out as two tensors
+    lp, ent = torch.empty(2, T, dtype=torch.float32, device=dev)
+    top_lp = torch.empty(T, top_n, dtype=torch.float32, device=dev)
+    top_ids = torch.empty(T, top_n, dtype=torch.int64, device=dev)
+    if T == 0:
+        return lp, ent, top_lp, top_ids
+    s = _raw_stream(dev.index)
+    ws = _paged_workspace(dev, s, size_call("nkimoe_token_logprobs_workspace_bytes", T, V, top_n))
+    call("nkimoe_token_logprobs", logits.data_ptr(), _DT[logits.dtype], logits.stride(0) if T > 1 else V,
+             tokens.data_ptr(), T, V, top_n, lp.data_ptr(), ent.data_ptr(), top_lp.data_ptr(), top_ids.data_ptr(),
+             ws.data_ptr(), ws.numel(), s)
+    return lp, ent, top_lp, top_ids
 
 
 # ---------------------------------------------------------------- router

@@ -238,6 +238,31 @@ NKIMOE_API int nkimoe_paged_decode_attention(const void* qkv, const void* q_weig
                                              float scale, int64_t window, int64_t sinks, void* workspace,
                                              size_t workspace_bytes, void* stream);
 
+NKIMOE_API size_t nkimoe_paged_prefill_attention_workspace_bytes(int64_t T, int64_t batch, int n_heads,
+                                                                 int n_kv_heads, int64_t max_pages,
+                                                                 int64_t page_size);
+
+/* Causal attention of packed query rows q [T, n_heads, 128] (bf16, rows
+ * q_row_stride elements apart, normed and rotated: the q_out of
+ * nkimoe_qk_norm_rope_store) over the pages, which already hold the rows' own
+ * keys and values: whole prompts, or chunks of prompts over what the cache
+ * holds of them.  cu_seqlens, kv_lens as in nkimoe_qk_norm_rope_store; a
+ * sequence may have no rows.  out: bf16 [T, n_heads * 128]; rows from
+ * cu_seqlens[batch] on are left alone.  Lengths that make no sense (outside
+ * [0, T], decreasing, a kv_len below the rows or past the page table) are
+ * reported (NKIMOE_DEV_BAD_INDEX) and their rows left unwritten; a page that
+ * a row needs and that is not held is reported, and the rows that need it have
+ * no meaning.  Rows of the cache below kv_len must hold finite numbers; what
+ * lies behind, and pages that no row needs, may hold anything.
+ * Reference: the attention of qwen_with_nki.py:330-350. */
+NKIMOE_API int nkimoe_paged_prefill_attention(const void* q, int64_t q_row_stride, const void* k_pages,
+                                              const void* v_pages, int64_t k_page_stride, int64_t v_page_stride,
+                                              int64_t num_pages, int64_t page_size, const int32_t* page_table,
+                                              int64_t table_stride, int64_t max_pages, const int32_t* cu_seqlens,
+                                              const int32_t* kv_lens, void* out, int64_t T, int64_t batch,
+                                              int n_heads, int n_kv_heads, int head_dim, float scale, int64_t window,
+                                              int64_t sinks, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Copies page src[i] to page dst[i] (i < n) in each of `planes` pools of
  * num_pages pages of page_bytes bytes (a multiple of 16), one behind the other
  * at `pages`.  src and dst are HOST arrays, read before the call returns and

@@ -23,8 +23,8 @@ CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(REPO, "_build")
 LIB = os.path.join(PKG, "libnkimoe.so")
 SOURCES = ["norm.cu", "router.cu", "permute.cu", "pack.cu", "grouped_gemm.cu", "ep_peer.cu", "capi.cu",
-           "noalloc.cu", "attention.cu", "linear.cu", "paged_store.cu", "paged_copy.cu", "paged_decode.cu", "logprobs.cu",
-           "capi_paged.cu"]
+           "noalloc.cu", "attention.cu", "linear.cu", "paged_store.cu", "paged_copy.cu", "paged_decode.cu",
+           "paged_prefill.cu", "logprobs.cu", "capi_paged.cu"]
 HEADERS = ["common.cuh", "kernels.h", "rope.cuh", "permute_small.cuh", "paged.cuh"]
 
 

@@ -531,6 +531,8 @@ bool make_tmap_bf16(CUtensorMap* map, const void* base, long long rows, long lon
   return r == CUDA_SUCCESS;
 }
 
+void* tmap_encode_fn() { return reinterpret_cast<void*>(encode_fn()); }
+
 void set_last_error(const char* msg) { g_err = msg ? msg : ""; }
 
 namespace {

@@ -1,6 +1,6 @@
 // C ABI of the paged key-value cache and the token scores (include/nkimoe.h):
 // argument checks in front of the launches of paged_store.cu, paged_copy.cu,
-// paged_decode.cu and logprobs.cu.
+// paged_decode.cu, paged_prefill.cu and logprobs.cu.
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
@@ -82,6 +82,11 @@ int check_window(int64_t window, int64_t sinks) {
   return NKIMOE_OK;
 }
 
+int check_scale(float scale) {
+  NKI_REQUIRE(scale > 0.f && scale <= 3e38f, NKIMOE_ERR_INVALID_ARG, "scale must be positive and finite");
+  return NKIMOE_OK;
+}
+
 }  // namespace
 
 }  // namespace nkimoe
@@ -148,6 +153,7 @@ int nkimoe_paged_decode_attention(const void* qkv, const void* q_weight, const v
                                   void* stream) {
   NKI_CHECK(check_heads(n_heads, n_kv_heads, head_dim));
   NKI_CHECK(check_window(window, sinks));
+  NKI_CHECK(check_scale(scale));
   NKI_REQUIRE(batch >= 0 && (pos_stride == 0 || pos_stride == 1), NKIMOE_ERR_INVALID_ARG, "bad shape");
   NKI_REQUIRE(batch <= 4096, NKIMOE_ERR_UNSUPPORTED, "more than 4096 sequences");
   NKI_REQUIRE(w_dtype == NKIMOE_F32 || w_dtype == NKIMOE_BF16, NKIMOE_ERR_INVALID_ARG, "bad weight dtype");
@@ -170,6 +176,49 @@ int nkimoe_paged_decode_attention(const void* qkv, const void* q_weight, const v
                                static_cast<__nv_bfloat16*>(out), static_cast<int>(batch), n_heads, rope_theta, eps,
                                scale, static_cast<int>(window), static_cast<int>(sinks), workspace,
                                static_cast<cudaStream_t>(stream)));
+  return NKIMOE_OK;
+}
+
+size_t nkimoe_paged_prefill_attention_workspace_bytes(int64_t T, int64_t batch, int n_heads, int n_kv_heads,
+                                                      int64_t max_pages, int64_t page_size) {
+  if (T < 0 || batch < 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > 16 ||
+      max_pages <= 0 || page_size <= 0 || page_size > 256 || max_pages > (1LL << 30) / page_size ||
+      T > 0x7fffffffLL || batch > (1 << 24))
+    return 0;
+  return paged_prefill_workspace_bytes(T, batch, n_heads, n_kv_heads, max_pages, static_cast<int>(page_size));
+}
+
+int nkimoe_paged_prefill_attention(const void* q, int64_t q_row_stride, const void* k_pages, const void* v_pages,
+                                   int64_t k_page_stride, int64_t v_page_stride, int64_t num_pages, int64_t page_size,
+                                   const int32_t* page_table, int64_t table_stride, int64_t max_pages,
+                                   const int32_t* cu_seqlens, const int32_t* kv_lens, void* out, int64_t T,
+                                   int64_t batch, int n_heads, int n_kv_heads, int head_dim, float scale,
+                                   int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  NKI_CHECK(check_heads(n_heads, n_kv_heads, head_dim));
+  NKI_CHECK(check_window(window, sinks));
+  NKI_CHECK(check_scale(scale));
+  NKI_REQUIRE(T >= 0 && batch >= 0, NKIMOE_ERR_INVALID_ARG, "bad shape");
+  NKI_REQUIRE(T <= 0x7fffffffLL && batch <= (1 << 24), NKIMOE_ERR_UNSUPPORTED, "shape too large");
+  if (T == 0 || batch == 0) return NKIMOE_OK;
+  PagedCache c;
+  NKI_CHECK(check_cache(k_pages, v_pages, k_page_stride, v_page_stride, num_pages, page_size, page_table, table_stride,
+                        max_pages, n_kv_heads, &c));
+  NKI_REQUIRE((T + batch) * n_kv_heads < 0x7fff0000LL, NKIMOE_ERR_UNSUPPORTED, "shape too large");
+  NKI_REQUIRE(q && cu_seqlens && kv_lens && out && workspace, NKIMOE_ERR_INVALID_ARG, "null pointer");
+  NKI_REQUIRE(q_row_stride >= static_cast<int64_t>(n_heads) * 128 && q_row_stride % 8 == 0, NKIMOE_ERR_INVALID_ARG,
+              "query rows must be multiples of 8 elements apart and not overlap");
+  NKI_REQUIRE(q_row_stride < (1LL << 38) && k_page_stride < (1LL << 38) && v_page_stride < (1LL << 38),
+              NKIMOE_ERR_UNSUPPORTED, "stride too large");
+  NKI_REQUIRE(aligned16(q) && aligned16(out) && aligned16(workspace) && aligned4(cu_seqlens) && aligned4(kv_lens),
+              NKIMOE_ERR_INVALID_ARG, "q, out and workspace must be 16-byte aligned, lengths 4-byte aligned");
+  const size_t need =
+      paged_prefill_workspace_bytes(T, batch, n_heads, n_kv_heads, max_pages, static_cast<int>(page_size));
+  NKI_REQUIRE(workspace_bytes >= need, NKIMOE_ERR_WORKSPACE, "workspace %zu bytes < %zu", workspace_bytes, need);
+  NKI_CUDA(paged_prefill_launch(static_cast<const __nv_bfloat16*>(q), q_row_stride, cu_seqlens, kv_lens, c,
+                                static_cast<__nv_bfloat16*>(out), T, static_cast<int>(batch), n_heads, scale,
+                                static_cast<int>(window), static_cast<int>(sinks), workspace,
+                                static_cast<cudaStream_t>(stream)));
   return NKIMOE_OK;
 }
 

@@ -322,6 +322,9 @@ cudaError_t grouped_gemm_launch(int variant, const CUtensorMap& tmap_act, const 
 int grouped_gemm_box_rows_act(int variant);
 int grouped_gemm_box_rows_w(int variant);
 
+// The driver's cuTensorMapEncodeTiled (PFN_cuTensorMapEncodeTiled_v12000), or null.
+void* tmap_encode_fn();
+
 int device_sm_count();
 
 // Sets the calling thread's message returned by nkimoe_last_error().

@@ -122,6 +122,11 @@ cudaError_t paged_decode_launch(const __nv_bfloat16* qkv, const void* qw, const 
                                 __nv_bfloat16* out, int B, int nq, float theta, float eps, float scale, int window,
                                 int sinks, void* workspace, cudaStream_t s);
 
+size_t paged_prefill_workspace_bytes(long long T, long long B, int nq, int nkv, long long max_pages, int page_size);
+cudaError_t paged_prefill_launch(const __nv_bfloat16* q, long long q_stride, const int* cu_seqlens,
+                                 const int* kv_lens, const PagedCache& cache, __nv_bfloat16* out, long long T, int B,
+                                 int nq, float scale, int window, int sinks, void* workspace, cudaStream_t s);
+
 size_t token_logprobs_workspace_bytes(long long T, long long V, int top_n);
 cudaError_t token_logprobs_launch(const void* logits, int dtype, long long row_stride, const long long* tokens,
                                   long long T, long long V, int top_n, float* logprob, float* entropy, float* top_lp,

@@ -26,8 +26,8 @@ __all__ = [
     "grouped_gemm", "swiglu", "aggregate", "read_status", "workspace", "sync_check_enabled", "router_split",
     "route", "dispatch", "segment_experts", "combine", "ep_dispatch", "decode_attention", "skinny_linear",
     "moe_block_add_rmsnorm", "moe_block_host", "kmajor_weights",
-    "release_captured_workspaces", "moe_block_rmsnorm", "qk_norm_rope_store", "paged_decode_attention", "copy_pages",
-    "token_logprobs", "read_paged_status",
+    "release_captured_workspaces", "moe_block_rmsnorm", "qk_norm_rope_store", "paged_decode_attention",
+    "paged_prefill_attention", "copy_pages", "token_logprobs", "read_paged_status",
 ]
 
 _DT = {torch.float32: F32, torch.bfloat16: BF16, torch.int32: I32, torch.int64: I64}
@@ -437,6 +437,46 @@ def paged_decode_attention(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: 
     call("nkimoe_paged_decode_attention", qkv.data_ptr(), qw.data_ptr(), kw.data_ptr(), wdt,
              positions.data_ptr(), 0 if n_pos == 1 else 1, *cache, out.data_ptr(), B, n_heads, n_kv_heads, 128, theta,
              eps, 128 ** -0.5 if scale is None else scale, window, sinks, ws.data_ptr(), ws.numel(), s)
+    if sync_check_enabled():
+        read_status(ws)
+    return out
+
+
+@_on_its_device
+def paged_prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                            cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, scale: float | None = None,
+                            window: int = 0, sinks: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of packed prompt rows over a paged cache that already
+    holds their keys and values: whole prompts, or chunks of prompts over what
+    the cache holds of them.
+
+    ``q``: ``[T, n_heads, 128]`` bf16, normed and rotated (what
+    :func:`qk_norm_rope_store` returns), rows at any stride that is a multiple
+    of 8; ``cu_seqlens``, ``kv_lens``, ``k_pages``, ``v_pages``,
+    ``page_table`` as there; ``window``, ``sinks`` as in
+    :func:`paged_decode_attention`.  Cached rows below ``kv_lens`` must be
+    finite.  Returns ``[T, n_heads * 128]`` bf16; rows from ``cu_seqlens[B]``
+    on are left as they were in ``out``."""
+    _cuda(q, "q")
+    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != 128 or q.stride(2) != 1 \
+            or (q.shape[1] > 1 and q.stride(1) != 128):
+        raise ValueError("q must be bf16 [T, n_heads, 128] with contiguous rows")
+    T, nq, _ = q.shape
+    dev = q.device
+    B = _lengths(cu_seqlens, kv_lens)
+    nkv = k_pages.shape[1] if k_pages.dim() == 4 else 0
+    cache = _paged_cache(k_pages, v_pages, page_table, nkv, B)
+    _same_device(dev, cu_seqlens=cu_seqlens, kv_lens=kv_lens, k_pages=k_pages, v_pages=v_pages, page_table=page_table)
+    if out is None:
+        out = torch.empty(T, nq * 128, dtype=torch.bfloat16, device=dev)
+    elif out.dtype != torch.bfloat16 or out.shape != (T, nq * 128) or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f"out must be a contiguous bf16 [{T}, {nq * 128}] tensor on {dev}")
+    s = _raw_stream(dev.index)
+    nbytes = size_call("nkimoe_paged_prefill_attention_workspace_bytes", T, B, nq, nkv, cache[8], cache[5])
+    ws = _paged_workspace(dev, s, nbytes)
+    call("nkimoe_paged_prefill_attention", q.data_ptr(), q.stride(0) if T > 1 else nq * 128, *cache,
+         cu_seqlens.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), T, B, nq, nkv, 128,
+         128 ** -0.5 if scale is None else scale, window, sinks, ws.data_ptr(), ws.numel(), s)
     if sync_check_enabled():
         read_status(ws)
     return out

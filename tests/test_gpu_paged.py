@@ -433,3 +433,183 @@ def test_copy_pages_refusals_copy_nothing():
     with pytest.raises(ValueError):
         ops.copy_pages(pages[:, ::2], [0], [1])
     assert torch.equal(pages, before)
+
+
+# ------------------------------------------------------------------ prompt attention
+def prefill_case(news, pasts, nq, nkv, ps, window=0, sinks=0, seed=0, behind=0, scale=None, strided=False, sharp=1.0):
+    """P enters its product as bf16 (2^-8 of each weight), so the sum may be off
+    by 2^-8 of the largest value, beside the bars of the decode step."""
+    B = len(news)
+    total = [n + p for n, p in zip(news, pasts)]
+
+    def needed(b, lo, hi):
+        if news[b] == 0:
+            return False
+        see = visible(total[b] - 1, total[b], 0, 0)
+        if window:
+            first = pasts[b]
+            s = torch.arange(total[b])
+            see = (s > first - window) | (s < sinks)
+        return bool(see[lo:hi].any())
+
+    c = Cache(total, nkv, ps, seed, needed)
+    cu = torch.zeros(B + 1, dtype=torch.int32)
+    cu[1:] = torch.tensor(news).cumsum(0)
+    T = int(cu[-1]) + behind
+    g = torch.Generator().manual_seed(seed + 1)
+    q = (sharp * 1.3 * torch.randn(T, nq + (2 * nkv if strided else 0), HD, generator=g)).bfloat16()
+    qd = q.cuda()[:, :nq]
+    q = q[:, :nq]
+    out = torch.full((T, nq * HD), 7.0, dtype=torch.bfloat16, device="cuda")
+    kd, vd = c.k.cuda(), c.v.cuda()
+    ops.paged_prefill_attention(qd, kd, vd, c.table.cuda(), cu.cuda(), torch.tensor(total, dtype=torch.int32).cuda(),
+                                window=window, sinks=sinks, scale=scale, out=out)
+    ops.read_paged_status()
+    assert (out[int(cu[-1]):] == 7).all()
+    grp = nq // nkv
+    for b in range(B):
+        if not news[b]:
+            continue
+        r = slice(int(cu[b]), int(cu[b + 1]))
+        k, v = c.rows(c.k, b, total[b]).nan_to_num(), c.rows(c.v, b, total[b]).nan_to_num()
+        qb = q[r].double().transpose(0, 1)
+        s = qb @ k.repeat_interleave(grp, 0).transpose(1, 2) * (scale or HD ** -0.5)
+        p = torch.arange(pasts[b], total[b])[:, None]
+        t = torch.arange(total[b])
+        see = t <= p
+        if window:
+            see &= (t > p - window) | (t < sinks)
+        s.masked_fill_(~see, -math.inf)
+        ref = (torch.softmax(s, -1) @ v.repeat_interleave(grp, 0)).transpose(0, 1)
+        near(out[r].view(-1, nq, HD), ref, float(v.abs().max()), atol=2 ** -8 + 2 ** -10 * max(1.0, sharp))
+        rel = (out[r].view(-1, nq, HD).double().cpu() - ref).norm() / ref.norm()
+        assert rel < 2 ** -8, f"sequence {b}: {rel:.2e}"
+    return out
+
+
+@pytest.mark.parametrize("ps", [16, 32, 64, 128, 256])
+def test_prefill_page_sizes_and_odd_lengths(ps):
+    prefill_case([1, 2, 16, 17, 33, 129, 300], [0] * 7, 32, 4, ps, seed=ps)
+
+
+@pytest.mark.parametrize("nq,nkv", [(8, 8), (16, 1), (12, 4), (7, 1), (40, 8), (18, 2), (1, 1), (28, 4)])
+def test_prefill_heads(nq, nkv):
+    prefill_case([5, 140, 261], [3, 0, 200], nq, nkv, 16, seed=nq)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (7, 0), (64, 4), (128, 0), (129, 5), (200, 130), (500, 4),
+                                          (5000, 9), (40, 1000)])
+def test_prefill_window_and_sinks(window, sinks):
+    prefill_case([300, 5, 64], [0, 777, 400], 16, 2, 16, window, sinks, seed=window)
+    prefill_case([130], [1000], 32, 4, 64, window, sinks, seed=window + 1)
+
+
+def test_prefill_chunk_over_a_long_cache_is_cut_into_parts():
+    prefill_case([16], [9000], 32, 4, 64, seed=60)
+    prefill_case([1, 40, 3], [5000, 3000, 10], 16, 2, 128, seed=61)
+    prefill_case([33], [6000], 8, 1, 16, 3000, 200, seed=62)
+
+
+def test_prefill_sequences_without_rows_rows_behind_and_strided_queries():
+    prefill_case([0, 5, 0, 0, 33, 0], [10, 0, 0, 40, 7, 0], 16, 2, 32, seed=63, behind=11, strided=True)
+    prefill_case([20], [0], 8, 2, 16, seed=64, scale=0.5)
+
+
+def test_prefill_many_short_sequences():
+    prefill_case([1 + (7 * i) % 11 for i in range(60)], [(13 * i) % 90 for i in range(60)], 8, 2, 16, seed=65)
+
+
+def test_prefill_scores_that_rise_along_the_keys():
+    """The running maximum has to be raised often, by much."""
+    prefill_case([260], [300], 8, 2, 16, seed=66, sharp=6.0)
+    nq, nkv, ps, n = 8, 1, 64, 700
+    c = Cache([n], nkv, ps, 67)
+    ramp = torch.arange(n).float()
+    for s in range(n):
+        c.k[int(c.table[0, s // ps]), :, s % ps] = 0
+        c.k[int(c.table[0, s // ps]), :, s % ps, 0] = ramp[s] * 0.5
+    q = torch.zeros(n, nq, HD).bfloat16()
+    q[:, :, 0] = 4.0
+    out = ops.paged_prefill_attention(q.cuda(), c.k.cuda(), c.v.cuda(), c.table.cuda(),
+                                      torch.tensor([0, n], dtype=torch.int32).cuda(),
+                                      torch.tensor([n], dtype=torch.int32).cuda())
+    k, v = c.rows(c.k, 0, n), c.rows(c.v, 0, n)
+    s = torch.einsum("thd,xd->htx", q.double(), k[0]) * HD ** -0.5
+    s.masked_fill_(torch.ones(n, n).triu(1).bool(), -math.inf)
+    ref = torch.einsum("htx,xd->thd", torch.softmax(s, -1), v[0])
+    near(out.view(n, nq, HD), ref, float(v.abs().max()), atol=2 ** -8 + 2 ** -9)
+
+
+def test_prefill_equals_decode_of_the_last_token():
+    """The two kernels on the same cache, the store between them."""
+    nq, nkv, ps, lens = 32, 4, 16, [1, 37, 400]
+    c = Cache(lens, nkv, ps, 68)
+    g = torch.Generator().manual_seed(68)
+    qkv = torch.randn(sum(lens), (nq + 2 * nkv) * HD, generator=g).bfloat16().cuda()
+    qw, kw = (w.cuda() for w in weights(68))
+    k, v, table = c.k.cuda(), c.v.cuda(), c.table.cuda()
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32).cuda()
+    kv = torch.tensor(lens, dtype=torch.int32).cuda()
+    q = ops.qk_norm_rope_store(qkv, qw, kw, cu, kv, k, v, table, nq, nkv)
+    o = ops.paged_prefill_attention(q, k, v, table, cu, kv)
+    last = (cu[1:] - 1).long()
+    k2, v2 = k.clone(), v.clone()
+    d = ops.paged_decode_attention(qkv[last], qw, kw, (kv - 1).long(), k2, v2, table, nq, nkv)
+    ops.read_paged_status()
+    assert torch.equal(k.view(torch.int16), k2.view(torch.int16)) and torch.equal(v.view(torch.int16), v2.view(torch.int16))
+    assert (o[last].float() - d.float()).abs().max() <= 2 ** -5
+
+
+def test_prefill_two_streams_and_graphs():
+    nq, nkv, ps = 16, 2, 64
+    cases = []
+    for seed in (70, 71):
+        c = Cache([3000, 50], nkv, ps, seed)
+        g = torch.Generator().manual_seed(seed)
+        q = torch.randn(40, nq, HD, generator=g).bfloat16().cuda()
+        cu = torch.tensor([0, 30, 40], dtype=torch.int32).cuda()
+        args = (q, c.k.cuda(), c.v.cuda(), c.table.cuda(), cu, torch.tensor([3000, 50], dtype=torch.int32).cuda())
+        cases.append((args, ops.paged_prefill_attention(*args)))
+    torch.cuda.synchronize()
+    side, graphs = torch.cuda.Stream(), []
+    for args, want in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            out = ops.paged_prefill_attention(*args)
+        graphs.append((g, out, want))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(10):
+        for (g, _, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        here = ops.paged_prefill_attention(*cases[0][0])
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for _, out, want in graphs) and torch.equal(here, cases[0][1])
+    ops.read_paged_status()
+
+
+def test_prefill_reports_lengths_and_pages(monkeypatch):
+    monkeypatch.setenv("NKIMOE_SYNC_CHECK", "0")
+    nq, nkv, ps = 8, 2, 16
+    c = Cache([40, 30], nkv, ps, 72)
+    q = torch.randn(70, nq, HD).bfloat16().cuda()
+    k, v, table = c.k.cuda(), c.v.cuda(), c.table.cuda()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    good = ops.paged_prefill_attention(q, k, v, table, i32(0, 40, 70), i32(40, 30))
+    ops.read_paged_status()
+    for cu, kv in ((i32(0, 40, 71), i32(40, 31)), (i32(0, 40, 30), i32(40, 30)), (i32(-3, 40, 70), i32(43, 30)),
+                   (i32(0, 40, 70), i32(39, 30)), (i32(0, 40, 70), i32(40, 3000)), (i32(0, 0, 70), i32(-5, 70))):
+        ops.paged_prefill_attention(q, k, v, table, cu, kv)
+        with pytest.raises(NKIMoEError):
+            ops.read_paged_status()
+    wide = torch.cat([table, table[:, :1], table[:, :1]], 1)
+    ops.paged_prefill_attention(q, k, v, wide[[0, 0, 0]], i32(0, 70, 0, 70), i32(70, 0, 70))  # overlapping
+    with pytest.raises(NKIMoEError):
+        ops.read_paged_status()
+    for bad in (-1, 1000):
+        t2 = table.clone()
+        t2[1, 0] = bad
+        out = ops.paged_prefill_attention(q, k, v, t2, i32(0, 40, 70), i32(40, 30))
+        with pytest.raises(NKIMoEError):
+            ops.read_paged_status()
+        assert torch.equal(out[:40], good[:40])

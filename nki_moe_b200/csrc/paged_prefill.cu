@@ -46,15 +46,20 @@ namespace {
 constexpr int kPfBlock = 128;                  // key positions per block
 constexpr int kPfRows = 128;                   // MMA rows per tile
 constexpr int kPfThreads = 384;
-constexpr int kPfRing = 5;                     // stages of 32 KB
-constexpr uint32_t kPfTileBytes = kPfRows * kHeadDim * 2;  // 32 KB: a Q tile, a K block or a V block
-constexpr uint32_t kPfHalf = kPfTileBytes / 2;             // one 64-column half (128 rows x 128 bytes)
-constexpr size_t kPfSmem = 1024 + 2 * kPfTileBytes + kPfRing * kPfTileBytes;
-constexpr int kPfPartRow = 132;                // floats per partial row: o[128], m, l, pad
+constexpr int kPfRing = 4;                     // stages of 32 KB
+constexpr uint32_t kPfTileBytes = kPfRows * kHeadDim * 2;    // 32 KB: a Q tile
+constexpr uint32_t kPfTileHalf = kPfTileBytes / 2;           // one 64-column half (128 rows x 128 bytes)
+constexpr uint32_t kPfBlockBytes = kPfBlock * kHeadDim * 2;  // 32 KB: a K block or a V block
+constexpr uint32_t kPfBlockHalf = kPfBlockBytes / 2;
+constexpr size_t kPfSmem = 1024 + 2 * kPfTileBytes + kPfRing * kPfBlockBytes;
+// A part of a cut pair, per tile: o column by column [128][128 rows], then
+// the rows' m, then their l (a warp's rows are neighbours: coalesced)
+constexpr int kPfPartTile = (kHeadDim + 2) * kPfRows;
 constexpr int kPfMinBlocks = 4;                // key blocks of a part at least
 constexpr float kPfLog2e = 1.4426950408889634f;
+constexpr int kPfPoly = 0;                     // of 8 weights whose 2^x runs on the FMA pipe
 constexpr float kPfSlack = 8.f;                // log2 by which a block may exceed the running maximum
-// tensor memory columns: S (and P over its first half) of tile t at 128 t, O at 256 + 128 t
+// tensor memory columns: S of tile t at 128 t (P over its first half), O at 256 + 128 t
 constexpr uint32_t kPfTmemO = 256;
 
 struct PfUnit {
@@ -83,7 +88,7 @@ struct PfParams {
   int* slots;       // per unit entry: its first slot, or -1
   PfSplit* splits;  // [count of cut pairs]
   int* starts;      // [B + 1] pairs before each sequence
-  float* part;      // [slots * nkv, 256, kPfPartRow]
+  float* part;      // [slots * nkv, 2, kPfPartTile]
   PagedCache c;
   int T, B, nq, grp, tpt;  // tpt: tokens per tile
   int window, sinks;
@@ -219,15 +224,12 @@ __global__ void __launch_bounds__(kPlanThreads) paged_prefill_plan_kernel(const 
 }
 
 // ------------------------------------------------------------------ tensor memory, MMA with A from tensor memory
-__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -276,6 +278,56 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Two fp32 operations in one instruction (sm_100).
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x for a pair, x in [-127, 127], 0 at -127: x = n + f with n the nearest integer, 2^f
+// by the minimax polynomial of degree 3 on [-1/2, 1/2] (Remez; relative error
+// 7.5e-5, against 2^-9 = 2e-3 of the weights' rounding to bf16), n added to the
+// exponent (at n = -127 that leaves less than nothing: 0).  No MUFU.
+__device__ __forceinline__ float2 ex2_poly(uint64_t x) {
+  const uint64_t magic = pair2(12582912.f, 12582912.f);  // 1.5 * 2^23: the sum's low bits are n
+  const uint64_t r = add2(x, magic);
+  const uint64_t n = add2(r, pair2(-12582912.f, -12582912.f));
+  const uint64_t f = fma2(n, pair2(-1.f, -1.f), x);
+  uint64_t p = fma2(f, pair2(0.05517166853f, 0.05517166853f), pair2(0.24261112511f, 0.24261112511f));
+  p = fma2(p, f, pair2(0.69326096773f, 0.69326096773f));
+  p = fma2(p, f, pair2(0.99992805719f, 0.99992805719f));
+  const float2 pf = split2(p), rf = split2(r);
+  return make_float2(__int_as_float(max(__float_as_int(pf.x) + (__float_as_int(rf.x) << 23), 0)),
+                     __int_as_float(max(__float_as_int(pf.y) + (__float_as_int(rf.y) << 23), 0)));
+}
+
+// The lowest n bits (none for n <= 0, all for n >= 32).
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+}
+
 // What the roles need to know of a unit.
 struct PfWork {
   int row0;    // first packed row of the pair
@@ -304,6 +356,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
                          const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ PfParams p) {
   extern __shared__ uint8_t pf_raw[];
   __shared__ PfCtl ctl;
+  __shared__ __align__(16) __nv_bfloat16 stg[8][32][40];  // per softmax warp: 32 output columns of its rows
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pf_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* sq = smem;
   uint8_t* ring = smem + 2 * kPfTileBytes;
@@ -337,8 +390,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   const uint32_t tmem = ctl.tmem_base;
   pdl_launch_dependents();
   pdl_wait();
-
+  // 384 x 168 registers at launch = 128 x 88 + 256 x 208
   if (warp == 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     // ---------------------------------------------------------------- units and loads (one thread)
     if (lane == 0) {
       const int page_rows = min(1 << p.c.page_shift, kPfBlock);  // rows per box
@@ -377,55 +431,65 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         mbar_arrive(&ctl.u_full[us]);
         if (w.tokens == 0) break;
         const bool two = w.tokens > p.tpt;
-        if (!mbar_wait(&ctl.q_empty, (u & 1) ^ 1u, &ctl.abort_flag, p.status)) {
-          ok = false;
-          break;
-        }
-        mbar_arrive_expect_tx(&ctl.q_full, two ? 2 * q_bytes : q_bytes);
-        for (int t = 0; t < (two ? 2 : 1); ++t)
-          for (int h = 0; h < 2; ++h)
-            tma_load_3d(sq + t * kPfTileBytes + h * kPfHalf, &tmap_q, &ctl.q_full, h * 64, w.j * p.grp,
-                        w.row0 + t * p.tpt);
-        q_issued = true;
         // positions that some query of the pair sees; a page outside is read as zeros
         const int last = w.pos0 + w.tokens - 1;
         const int start = p.window && w.pos0 >= p.window ? w.pos0 - p.window + 1 : 0;
         const int* table = p.c.table + w.b * p.c.table_stride;
-        for (int i = w.lo; ok && i < w.hi; ++i) {
+        int pages[8];
+        auto look_up = [&](int i) {
           const int k0 = bl.at(i) * kPfBlock;
-          int pages[8];
 #pragma unroll
           for (int g = 0; g < 8; ++g) {
             const int s0 = k0 + g * page_rows;
-            pages[g] = p.c.num_pages;  // past the last page: the load fills zeros
-            if (g * page_rows < kPfBlock && s0 <= last && (s0 + page_rows > start || s0 < p.sinks)) {
-              const int pg = table[s0 >> p.c.page_shift];
-              if (pg >= 0 && pg < p.c.num_pages) pages[g] = pg;
-              else atomicOr(p.status, kDevErrBadIndex);
+            pages[g] = -2;  // not needed
+            if (g * page_rows < kPfBlock && s0 <= last && (s0 + page_rows > start || s0 < p.sinks))
+              pages[g] = table[s0 >> p.c.page_shift];
+          }
+        };
+        auto load = [&](int i, bool is_v, const int (&pg)[8]) {
+          if (!mbar_wait(&ctl.kv_empty[stage], phase ^ 1u, &ctl.abort_flag, p.status)) return false;
+          const int k0 = bl.at(i) * kPfBlock;
+          uint8_t* dst = ring + stage * kPfBlockBytes;
+          mbar_arrive_expect_tx(&ctl.kv_full[stage], kPfBlockBytes);
+          const void* tm = is_v ? static_cast<const void*>(&tmap_v) : static_cast<const void*>(&tmap_k);
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            if (g * page_rows < kPfBlock) {
+              const int in_page = (k0 + g * page_rows) & ((1 << p.c.page_shift) - 1);
+              tma_load_4d(dst + g * page_rows * 128, tm, &ctl.kv_full[stage], 0, in_page, w.j, pg[g]);
+              tma_load_4d(dst + kPfBlockHalf + g * page_rows * 128, tm, &ctl.kv_full[stage], 64, in_page, w.j, pg[g]);
             }
           }
-          for (int kvsel = 0; kvsel < 2; ++kvsel) {
-            if (!mbar_wait(&ctl.kv_empty[stage], phase ^ 1u, &ctl.abort_flag, p.status)) {
-              ok = false;
-              break;
-            }
-            uint8_t* dst = ring + stage * kPfTileBytes;
-            mbar_arrive_expect_tx(&ctl.kv_full[stage], kPfTileBytes);
-            const void* tm = kvsel ? static_cast<const void*>(&tmap_v) : static_cast<const void*>(&tmap_k);
+          issued |= 1u << stage;
+          last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
+          if (++stage == kPfRing) {
+            stage = 0;
+            phase ^= 1u;
+          }
+          return true;
+        };
+        look_up(w.lo);
+        for (int i = w.lo; ok && i < w.hi; ++i) {
+          int pg[8];
 #pragma unroll
-            for (int g = 0; g < 8; ++g) {
-              if (g * page_rows < kPfBlock) {
-                const int in_page = (k0 + g * page_rows) & ((1 << p.c.page_shift) - 1);
-                tma_load_4d(dst + g * page_rows * 128, tm, &ctl.kv_full[stage], 0, in_page, w.j, pages[g]);
-                tma_load_4d(dst + kPfHalf + g * page_rows * 128, tm, &ctl.kv_full[stage], 64, in_page, w.j, pages[g]);
-              }
-            }
-            issued |= 1u << stage;
-            last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
-            if (++stage == kPfRing) {
-              stage = 0;
-              phase ^= 1u;
-            }
+          for (int g = 0; g < 8; ++g) {
+            const bool held = pages[g] >= 0 && pages[g] < p.c.num_pages;
+            if (!held && pages[g] != -2) atomicOr(p.status, kDevErrBadIndex);
+            pg[g] = held ? pages[g] : p.c.num_pages;  // past the last page: the load fills zeros
+          }
+          if (i + 1 < w.hi) look_up(i + 1);  // in flight while this block waits for its stages
+          ok = load(i, false, pg) && load(i, true, pg);
+          // the queries after the unit's first block, which goes out while the
+          // unit before still reads its own
+          if (ok && i == w.lo) {
+            ok = mbar_wait(&ctl.q_empty, (u & 1) ^ 1u, &ctl.abort_flag, p.status);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&ctl.q_full, two ? 2 * q_bytes : q_bytes);
+            for (int t = 0; t < (two ? 2 : 1); ++t)
+              for (int h = 0; h < 2; ++h)
+                tma_load_3d(sq + t * kPfTileBytes + h * kPfTileHalf, &tmap_q, &ctl.q_full, h * 64, w.j * p.grp,
+                            w.row0 + t * p.tpt);
+            q_issued = true;
           }
         }
         if (!ok) break;
@@ -447,101 +511,102 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMA issue
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    // ---------------------------------------------------------------- MMA issue (one thread)
     constexpr uint32_t idesc_s = umma_idesc_bf16_f32(kPfRows, kPfBlock);
     constexpr uint32_t idesc_o = umma_idesc_bf16_f32(kPfRows, kHeadDim) | (1u << 16);  // B is MN-major
+    const int page_rows = min(1 << p.c.page_shift, kPfBlock);
     int stage = 0;
-    uint32_t phase = 0, pphase[2] = {0, 0};  // pphase: of p_full, one phase per key block of the tile
+    uint32_t phase = 0, pphase = 0;  // pphase: bit t, of p_full
     bool ok = true, any = false;
-    auto wait = [&](uint64_t* bar, uint32_t ph) {
-      const bool got = mbar_wait(bar, ph, &ctl.abort_flag, p.status);
-      return __all_sync(0xffffffffu, got);
-    };
-    // S of tile t against the K block in `st`
-    auto issue_s = [&](int t, int st) {
-      if (lane == 0) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint64_t da = umma_desc_sw128(smem_u32(sq + t * kPfTileBytes + h * kPfHalf));
-          const uint64_t db = umma_desc_sw128(smem_u32(ring + st * kPfTileBytes + h * kPfHalf));
-#pragma unroll
-          for (int k = 0; k < 4; ++k) umma_bf16(tmem + t * 128, da + 2 * k, db + 2 * k, idesc_s, (h | k) != 0);
-        }
-        umma_commit(&ctl.s_full[t]);
+    auto wait = [&](uint64_t* bar, uint32_t ph) { return mbar_wait(bar, ph, &ctl.abort_flag, p.status); };
+    auto next_stage = [&] {
+      if (++stage == kPfRing) {
+        stage = 0;
+        phase ^= 1u;
       }
+    };
+    // S of tile t against the K block in the current stage
+    auto issue_s = [&](int t) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint64_t da = umma_desc_sw128(smem_u32(sq + t * kPfTileBytes + h * kPfTileHalf));
+        const uint64_t db = umma_desc_sw128(smem_u32(ring + stage * kPfBlockBytes + h * kPfBlockHalf));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_bf16(tmem + t * 128, da + 2 * k, db + 2 * k, idesc_s, (h | k) != 0);
+      }
+      umma_commit(&ctl.s_full[t]);
       any = true;
     };
-    for (int u = 0; ok; ++u) {
+    // one thread alone: a loop with warp collectives around each step took 1000
+    // cycles per tile and block for the hand-offs alone
+    for (int u = 0; lane == 0 && ok; ++u) {
       const int us = u & 1;
       if (!wait(&ctl.u_full[us], (u >> 1) & 1)) { ok = false; break; }
       const PfWork w = ctl.work[us];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl.u_empty[us]);
+      mbar_arrive(&ctl.u_empty[us]);
       if (w.tokens == 0) break;
       const int tiles = w.tokens > p.tpt ? 2 : 1;
       const Blocks bl = blocks_of(w.pos0, w.pos0 + w.tokens - 1, p.window, p.sinks);
       if (!wait(&ctl.q_full, u & 1) || !wait(&ctl.kv_full[stage], phase)) { ok = false; break; }
-      tcgen05_fence_after();
-      for (int t = 0; t < tiles; ++t) issue_s(t, stage);
-      if (lane == 0) {
-        umma_commit(&ctl.kv_empty[stage]);
-        if (w.hi - w.lo == 1) umma_commit(&ctl.q_empty);
-      }
-      if (++stage == kPfRing) { stage = 0; phase ^= 1u; }
+      for (int t = 0; t < tiles; ++t) issue_s(t);
+      umma_commit(&ctl.kv_empty[stage]);
+      if (w.hi - w.lo == 1) umma_commit(&ctl.q_empty);
+      next_stage();
       for (int i = w.lo; i < w.hi; ++i) {
         const int vs = stage;
         if (!wait(&ctl.kv_full[stage], phase)) { ok = false; break; }
-        if (++stage == kPfRing) { stage = 0; phase ^= 1u; }
-        // rows behind the sequence's end hold anything: their weights are 0,
-        // and 0 times a NaN would not be
+        next_stage();
+        // rows behind the sequence's end in its last page hold anything: their
+        // weights are 0, and 0 times a NaN would not be (further pages are
+        // loaded as zeros)
         const int live = w.kv - bl.at(i) * kPfBlock;
         if (live < kPfBlock) {
-          uint8_t* v = ring + vs * kPfTileBytes;
-          for (int x = live * 8 + lane; x < kPfBlock * 8; x += 32) {
+          uint8_t* v = ring + vs * kPfBlockBytes;
+          const int end = (live + page_rows - 1) & ~(page_rows - 1);
+          for (int x = live * 8; x < end * 8; ++x) {
             *reinterpret_cast<uint4*>(v + x * 16) = make_uint4(0u, 0u, 0u, 0u);
-            *reinterpret_cast<uint4*>(v + kPfHalf + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(v + kPfBlockHalf + x * 16) = make_uint4(0u, 0u, 0u, 0u);
           }
           fence_proxy_async_shared();
-          __syncwarp();
         }
+        // O += P V of block i, then, over P, S of block i + 1
         const bool more = i + 1 < w.hi;
         for (int t = 0; t < tiles; ++t) {
-          if (!wait(&ctl.p_full[t], pphase[t])) { ok = false; break; }
-          pphase[t] ^= 1u;
+          if (!wait(&ctl.p_full[t], (pphase >> t) & 1u)) { ok = false; break; }
+          pphase ^= 1u << t;
           tcgen05_fence_after();
-          if (lane == 0) {
-            const uint64_t dv = umma_desc_sw128_mn(smem_u32(ring + vs * kPfTileBytes), kPfHalf);
+          const uint64_t dv = umma_desc_sw128_mn(smem_u32(ring + vs * kPfBlockBytes), kPfBlockHalf);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)  // 16 positions: 2048 bytes of V, 8 columns of P
-              umma_bf16_ts(tmem + kPfTmemO + t * 128, tmem + t * 128 + 8 * k, dv + 128 * k, idesc_o,
-                           i > w.lo || k != 0);
-          }
+          for (int k = 0; k < 8; ++k)  // 16 positions: 2048 bytes of V, 8 columns of P
+            umma_bf16_ts(tmem + kPfTmemO + t * 128, tmem + t * 128 + 8 * k, dv + 128 * k, idesc_o, i > w.lo || k != 0);
           if (more) {
             if (t == 0 && !wait(&ctl.kv_full[stage], phase)) { ok = false; break; }
-            issue_s(t, stage);
-          } else if (lane == 0) {
+            issue_s(t);
+          } else {
             umma_commit(&ctl.o_full[t]);
           }
         }
         if (!ok) break;
-        if (lane == 0) umma_commit(&ctl.kv_empty[vs]);
+        umma_commit(&ctl.kv_empty[vs]);
         if (more) {
-          if (lane == 0) {
-            umma_commit(&ctl.kv_empty[stage]);
-            if (i + 2 == w.hi) umma_commit(&ctl.q_empty);
-          }
-          if (++stage == kPfRing) { stage = 0; phase ^= 1u; }
+          umma_commit(&ctl.kv_empty[stage]);
+          if (i + 2 == w.hi) umma_commit(&ctl.q_empty);
+          next_stage();
         }
       }
     }
-    if (!ok && any && lane == 0) {  // issued MMAs end before tensor memory is released
+    if (!ok && any) {  // issued MMAs end before tensor memory is released
       umma_commit(&ctl.drain);
       const long long t0 = clock64();
       while (!mbar_try_wait(&ctl.drain, 0) && clock64() - t0 < kWaitBudgetCycles / 8) {
       }
     }
     __syncwarp();
-  } else if (warp >= 4) {
+  } else if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---------------------------------------------------------------- softmax, one row per thread
     const int t = (warp - 4) >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
@@ -566,6 +631,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       const int pos = tile_pos + token;
       float m = -INFINITY, l = 0.f;
       bool ok = true;
+#pragma unroll 1
       for (int i = w.lo; i < w.hi; ++i) {
         const int k0 = bl.at(i) * kPfBlock;
         if (!wait(&ctl.s_full[t], sphase)) { ok = false; break; }
@@ -576,49 +642,64 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(ts + c * 32, s[c]);
         tmem_ld_wait();
         if (k0 + kPfBlock - 1 > tile_pos || (p.window && k0 <= tile_pos + p.tpt - 1 - p.window)) {
-          const int hi = pos - k0;                                       // columns up to hi,
-          const int lo = p.window ? hi - p.window + 1 : 0, sk = p.sinks - k0;  // from lo on or below sk
+          // visible columns of each 32: up to hi, from lo on or below sk
+          const int hi = pos - k0 + 1, lo = p.window ? hi - p.window : 0, sk = p.sinks - k0;
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (!(c <= hi && (c >= lo || c < sk))) s[c >> 5][c & 31] = 0xff800000u;
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t see = low_bits(hi - c * 32) & (~low_bits(lo - c * 32) | low_bits(sk - c * 32));
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (!((see >> x) & 1u)) s[c][x] = 0xff800000u;
+          }
         }
-        float mx = -INFINITY;
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four short chains
 #pragma unroll
-        for (int c = 0; c < 128; ++c) mx = fmaxf(mx, __uint_as_float(s[c >> 5][c & 31]));
-        mx *= p.scale_log2;
+        for (int c = 0; c < 128; c += 2)
+          mx4[(c >> 1) & 3] = max3(mx4[(c >> 1) & 3], __uint_as_float(s[c >> 5][c & 31]), __uint_as_float(s[c >> 5][(c & 31) + 1]));
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
         const bool raise = mx > m + kPfSlack;  // the first finite maximum too: m is -inf
         if (__any_sync(0xffffffffu, raise)) {
           const float mn = raise ? mx : m;
           if (i > w.lo) {
-            // every lane takes part; lanes that keep their maximum multiply by 1
+            // every lane takes part; lanes that keep their maximum multiply by
+            // 1.  All products so far are done: this block's S came after them.
             const float f = raise ? ex2(m - mn) : 1.f;
             l *= f;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t o[32];
-              tmem_ld_32x32b_x32(to + c * 32, o);
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {  // rolled: rare
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(to + c * 16, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-              tmem_st_32x32b_x32(to + c * 32, o);
+              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+              tmem_st_32x32b_x16(to + c * 16, o);
             }
           }
           m = mn;
         }
         const float ms = m == -INFINITY ? 0.f : m;
+        const uint64_t sc2 = pair2(p.scale_log2, p.scale_log2), ms2 = pair2(-ms, -ms);
+        uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t pk[32];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
 #pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            const int c = h * 64 + 2 * x;
-            const float a = ex2(fmaf(__uint_as_float(s[c >> 5][c & 31]), p.scale_log2, -ms));
-            const float b = ex2(fmaf(__uint_as_float(s[c >> 5][(c & 31) + 1]), p.scale_log2, -ms));
-            l += a + b;
-            pk[x] = pack_bf16x2(a, b);
+          for (int x = 0; x < 16; ++x) {
+            const uint64_t y = fma2(pair2(__uint_as_float(s[c][2 * x]), __uint_as_float(s[c][2 * x + 1])), sc2, ms2);
+            float2 e = split2(y);
+            if ((x & 7) < kPfPoly) {
+              e = ex2_poly(pair2(fmaxf(e.x, -127.f), fmaxf(e.y, -127.f)));
+            } else {
+              e.x = ex2(e.x);
+              e.y = ex2(e.y);
+            }
+            sum[x & 3] = add2(sum[x & 3], pair2(e.x, e.y));
+            pk[x] = pack_bf16x2(e.x, e.y);
           }
-          tmem_st_32x32b_x32(ts + h * 32, pk);
+          tmem_st_32x32b_x16(ts + c * 16, pk);
         }
+        const float2 sums = split2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+        l += sums.x + sums.y;
         tmem_st_wait();
         tcgen05_fence_before();
         __syncwarp();
@@ -629,31 +710,42 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       tcgen05_fence_after();
       const bool mine = token < p.tpt && t * p.tpt + token < w.tokens;
       const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-      const long long orow = w.row0 + t * p.tpt + token;
-      __nv_bfloat16* dst = p.out + (orow * p.nq + w.j * p.grp + head) * kHeadDim;
-      float* part = w.slot >= 0 ? p.part + (static_cast<long long>(w.slot) * 2 * kPfRows + t * kPfRows + row) * kPfPartRow : nullptr;
-#pragma unroll
+      const long long out_at =
+          mine ? ((static_cast<long long>(w.row0) + t * p.tpt + token) * p.nq + w.j * p.grp + head) * kHeadDim : -1;
+      float* part = w.slot >= 0 ? p.part + (static_cast<long long>(w.slot) * 2 + t) * kPfPartTile + row : nullptr;
+#pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
         __syncwarp();
         tmem_ld_32x32b_x32(to + c * 32, o);
         tmem_ld_wait();
-        if (!mine) {
-        } else if (part) {
+        if (part) {
 #pragma unroll
-          for (int x = 0; x < 32; x += 4)
-            __stcg(reinterpret_cast<uint4*>(part + c * 32 + x), make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]));
+          for (int x = 0; x < 32; ++x) __stcg(part + (c * 32 + x) * kPfRows, __uint_as_float(o[x]));
         } else {
+          // through shared memory: eight rows of 64 bytes per store instead of
+          // 32 rows of 16
 #pragma unroll
           for (int x = 0; x < 32; x += 8) {
             float f[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[x + e]) * inv;
-            *reinterpret_cast<uint4*>(dst + c * 32 + x) = pack8(f);
+            *reinterpret_cast<uint4*>(&stg[warp - 4][lane][x]) = pack8(f);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int r = k * 8 + (lane >> 2);
+            const long long at = __shfl_sync(0xffffffffu, out_at, r);
+            const uint4 v = *reinterpret_cast<const uint4*>(&stg[warp - 4][r][(lane & 3) * 8]);
+            if (at >= 0) *reinterpret_cast<uint4*>(p.out + at + c * 32 + (lane & 3) * 8) = v;
           }
         }
       }
-      if (part && mine) __stcg(reinterpret_cast<float2*>(part + kHeadDim), make_float2(m, l));
+      if (part) {
+        __stcg(part + kHeadDim * kPfRows, m);
+        __stcg(part + (kHeadDim + 1) * kPfRows, l);
+      }
       tcgen05_fence_before();  // the next unit's MMAs follow this thread's next arrival
     }
   }
@@ -665,50 +757,45 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   }
 }
 
-// Joins the parts of cut pairs: one warp per (pair, kv head, row), a lane per
-// four columns, the parts in order.
+// Joins the parts of cut pairs, in order: a CTA per (pair, kv head, 32 rows),
+// a lane per row, a warp per 16 columns.
 __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const __grid_constant__ PfParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int rows = 2 * kPfRows;
-  const long long total = static_cast<long long>(p.list->splits) * p.c.nkv * rows;
-  for (long long i = blockIdx.x * 8ll + (threadIdx.x >> 5); i < total; i += gridDim.x * 8ll) {
-    const int r = static_cast<int>(i % rows), j = static_cast<int>(i / rows % p.c.nkv);
-    const PfSplit sp = p.splits[i / rows / p.c.nkv];
-    const int tile = r >> 7, token = (r & 127) / p.grp, head = (r & 127) - token * p.grp;
+  const int lane = threadIdx.x & 31, col = (threadIdx.x >> 5) * 16;
+  const int total = p.list->splits * p.c.nkv * 8;
+  for (int i = blockIdx.x; i < total; i += gridDim.x) {
+    const int tile = (i >> 2) & 1, row = (i & 3) * 32 + lane, j = (i >> 3) % p.c.nkv;
+    const PfSplit sp = p.splits[(i >> 3) / p.c.nkv];
+    const int token = row / p.grp, head = row - token * p.grp;
     const int at = sp.pair * 2 * p.tpt + tile * p.tpt + token;  // row of the sequence
     const int start = p.cu[sp.b];
     if (token >= p.tpt || at >= p.cu[sp.b + 1] - start) continue;
-    const float* part = p.part + (static_cast<long long>(sp.slot * p.c.nkv + j) * rows + r) * kPfPartRow;
-    const long long stride = static_cast<long long>(p.c.nkv) * rows * kPfPartRow;
+    const float* part = p.part + (static_cast<long long>(sp.slot * p.c.nkv + j) * 2 + tile) * kPfPartTile + row;
+    const long long stride = static_cast<long long>(p.c.nkv) * 2 * kPfPartTile;
     float m = -INFINITY;
-    for (int s = lane; s < sp.nsplit; s += 32) m = fmaxf(m, __ldcg(part + s * stride + kHeadDim));
-    m = warp_max(m);
-    float l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s0 = 0; s0 < sp.nsplit; s0 += 4) {
-      float4 v[4];
-      float2 ml[4];
+    for (int s = 0; s < sp.nsplit; ++s) m = fmaxf(m, __ldcg(part + s * stride + kHeadDim * kPfRows));
+    float l = 0.f, o[16];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const bool in = s0 + x < sp.nsplit;
-        ml[x] = in ? __ldcg(reinterpret_cast<const float2*>(part + (s0 + x) * stride + kHeadDim)) : make_float2(-INFINITY, 0.f);
-        v[x] = in ? __ldcg(reinterpret_cast<const float4*>(part + (s0 + x) * stride + lane * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
+    for (int x = 0; x < 16; ++x) o[x] = 0.f;
+    for (int s = 0; s < sp.nsplit; ++s) {
+      const float* from = part + s * stride;
+      const float f = m == -INFINITY ? 0.f : exp2f(__ldcg(from + kHeadDim * kPfRows) - m);
+      l = fmaf(f, __ldcg(from + (kHeadDim + 1) * kPfRows), l);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float f = m == -INFINITY ? 0.f : exp2f(ml[x].x - m);
-        l = fmaf(f, ml[x].y, l);
-        o.x = fmaf(f, v[x].x, o.x);
-        o.y = fmaf(f, v[x].y, o.y);
-        o.z = fmaf(f, v[x].z, o.z);
-        o.w = fmaf(f, v[x].w, o.w);
-      }
+      for (int x = 0; x < 16; ++x) o[x] = fmaf(f, __ldcg(from + (col + x) * kPfRows), o[x]);
     }
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-    *reinterpret_cast<uint2*>(p.out + ((static_cast<long long>(start + at) * p.nq + j * p.grp + head) * kHeadDim + lane * 4)) =
-        make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+#pragma unroll
+    for (int x = 0; x < 16; ++x) o[x] *= inv;
+    __nv_bfloat16* dst = p.out + (static_cast<long long>(start + at) * p.nq + j * p.grp + head) * kHeadDim + col;
+    float h[8];
+#pragma unroll
+    for (int x = 0; x < 16; x += 8) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[e] = o[x + e];
+      *reinterpret_cast<uint4*>(dst + x) = pack8(h);
+    }
   }
 }
 
@@ -742,7 +829,7 @@ PfLayout pf_layout(long long T, long long B, int nkv, int grp, long long max_pag
   L.starts = at;
   at += round(sizeof(int) * (B + 1));
   L.part = at;
-  at += sizeof(float) * L.slots * nkv * 2 * kPfRows * kPfPartRow;
+  at += sizeof(float) * L.slots * nkv * 2 * kPfPartTile;
   L.total = at;
   return L;
 }

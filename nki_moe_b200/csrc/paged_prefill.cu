@@ -57,18 +57,24 @@ constexpr size_t kPfSmem = 1024 + 2 * kPfTileBytes + kPfRing * kPfBlockBytes;
 constexpr int kPfPartTile = (kHeadDim + 2) * kPfRows;
 constexpr int kPfMinBlocks = 4;                // key blocks of a part at least
 constexpr float kPfLog2e = 1.4426950408889634f;
-constexpr int kPfPoly = 0;                     // of 8 weights whose 2^x runs on the FMA pipe
 constexpr float kPfSlack = 8.f;                // log2 by which a block may exceed the running maximum
 // tensor memory columns: S of tile t at 128 t (P over its first half), O at 256 + 128 t
 constexpr uint32_t kPfTmemO = 256;
 
-struct PfUnit {
-  int b, pair, split, nsplit;
+// A unit, for each kv head.
+struct __align__(16) PfUnit {
+  int row0;    // first packed row of the pair
+  int pos0;    // its position
+  int tokens;  // rows of the pair (<= 2 tpt)
+  int kv;      // length of the sequence
+  int b;
+  int lo, hi;  // range of the pair's key blocks
+  int slot;    // of its partial result, or -1
 };
 
 struct PfList {  // in the workspace
   int count;     // entries; unit u is entry u / nkv, kv head u % nkv
-  int next;      // the counter that CTAs take units from
+  int next;      // the counter that CTAs take units from, after one each
   int splits;    // pairs that are cut into parts
   int pad;
 };
@@ -85,7 +91,6 @@ struct PfParams {
   int* status;
   PfList* list;
   PfUnit* units;
-  int* slots;       // per unit entry: its first slot, or -1
   PfSplit* splits;  // [count of cut pairs]
   int* starts;      // [B + 1] pairs before each sequence
   float* part;      // [slots * nkv, 2, kPfPartTile]
@@ -124,6 +129,7 @@ __device__ __forceinline__ int pf_rows(const PfParams& p, int b, int& kv, bool f
 }
 
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanStarts = 4096;  // sequences whose first pairs are also kept in shared memory
 
 // Exclusive scan over the CTA; `total` gets the sum.
 __device__ __forceinline__ int plan_scan(int v, int* warp_sums, int& total) {
@@ -153,6 +159,7 @@ __device__ __forceinline__ int plan_scan(int v, int* warp_sums, int& total) {
 __global__ void __launch_bounds__(kPlanThreads) paged_prefill_plan_kernel(const __grid_constant__ PfParams p) {
   __shared__ int warp_sums[32];
   __shared__ float warp_tot[32];
+  __shared__ int near_starts[kPlanStarts + 1];
   const int tid = threadIdx.x;
   const int per_pair = 2 * p.tpt;
   pdl_launch_dependents();
@@ -172,10 +179,10 @@ __global__ void __launch_bounds__(kPlanThreads) paged_prefill_plan_kernel(const 
     }
     int total;
     const int before = plan_scan(np, warp_sums, total);
-    if (b < p.B) p.starts[b] = pairs + before;
+    if (b < p.B) (b <= kPlanStarts ? near_starts : p.starts)[b] = pairs + before;
     pairs += total;
   }
-  if (tid == 0) p.starts[p.B] = pairs;
+  if (tid == 0) (p.B <= kPlanStarts ? near_starts : p.starts)[p.B] = pairs;
   if (pairs > p.max_pairs) {  // sequences that overlap: more rows than there are
     if (tid == 0) atomicOr(p.status, kDevErrBadIndex);
     pairs = p.max_pairs;
@@ -187,21 +194,26 @@ __global__ void __launch_bounds__(kPlanThreads) paged_prefill_plan_kernel(const 
   for (int w = 0; w < kPlanThreads / 32; ++w) blocks += warp_tot[w];
   const int most = max(kPfMinBlocks, static_cast<int>(blocks / p.sms) + 1);  // blocks of a unit
 
+  auto start_of = [&](int b) { return b <= kPlanStarts ? near_starts[b] : p.starts[b]; };
   int entries = 0, slots = 0, cut = 0;
   for (int i0 = 0; i0 < pairs; i0 += kPlanThreads) {
     const int i = i0 + tid;
-    int ns = 0, b = 0, pair = 0;
+    int ns = 0, b = 0, pair = 0, blocks = 0;
+    PfUnit un{};
     if (i < pairs) {
       int hi = p.B;
       while (hi - b > 1) {
         const int mid = (b + hi) >> 1;
-        if (p.starts[mid] <= i) b = mid; else hi = mid;
+        if (start_of(mid) <= i) b = mid; else hi = mid;
       }
-      int kv;
-      const int n = pf_rows(p, b, kv, false);
-      pair = p.starts[b + 1] - 1 - i;  // the sequence's last pair, the longest, first
-      const int lo = kv - n + pair * per_pair;
-      ns = (blocks_of(lo, min(lo + per_pair, kv) - 1, p.window, p.sinks).n + most - 1) / most;
+      const int n = pf_rows(p, b, un.kv, false);
+      pair = start_of(b + 1) - 1 - i;  // the sequence's last pair, the longest, first
+      un.b = b;
+      un.row0 = p.cu[b] + pair * per_pair;
+      un.pos0 = un.kv - n + pair * per_pair;
+      un.tokens = min(per_pair, n - pair * per_pair);
+      blocks = blocks_of(un.pos0, un.pos0 + un.tokens - 1, p.window, p.sinks).n;
+      ns = (blocks + most - 1) / most;
     }
     int total;
     // parts are given up where the list or the slots would not hold them
@@ -215,8 +227,10 @@ __global__ void __launch_bounds__(kPlanThreads) paged_prefill_plan_kernel(const 
     const int e = plan_scan(ns, warp_sums, total) + entries;
     entries += total;
     for (int s = 0; s < ns; ++s) {
-      p.units[e + s] = PfUnit{b, pair, s, ns};
-      p.slots[e + s] = ns > 1 ? slot : -1;
+      un.lo = static_cast<int>(static_cast<long long>(blocks) * s / ns);
+      un.hi = static_cast<int>(static_cast<long long>(blocks) * (s + 1) / ns);
+      un.slot = ns > 1 ? slot + s : -1;
+      p.units[e + s] = un;
     }
     if (ns > 1) p.splits[k] = PfSplit{b, pair, slot, ns};
   }
@@ -306,38 +320,14 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// 2^x for a pair, x in [-127, 127], 0 at -127: x = n + f with n the nearest integer, 2^f
-// by the minimax polynomial of degree 3 on [-1/2, 1/2] (Remez; relative error
-// 7.5e-5, against 2^-9 = 2e-3 of the weights' rounding to bf16), n added to the
-// exponent (at n = -127 that leaves less than nothing: 0).  No MUFU.
-__device__ __forceinline__ float2 ex2_poly(uint64_t x) {
-  const uint64_t magic = pair2(12582912.f, 12582912.f);  // 1.5 * 2^23: the sum's low bits are n
-  const uint64_t r = add2(x, magic);
-  const uint64_t n = add2(r, pair2(-12582912.f, -12582912.f));
-  const uint64_t f = fma2(n, pair2(-1.f, -1.f), x);
-  uint64_t p = fma2(f, pair2(0.05517166853f, 0.05517166853f), pair2(0.24261112511f, 0.24261112511f));
-  p = fma2(p, f, pair2(0.69326096773f, 0.69326096773f));
-  p = fma2(p, f, pair2(0.99992805719f, 0.99992805719f));
-  const float2 pf = split2(p), rf = split2(r);
-  return make_float2(__int_as_float(max(__float_as_int(pf.x) + (__float_as_int(rf.x) << 23), 0)),
-                     __int_as_float(max(__float_as_int(pf.y) + (__float_as_int(rf.y) << 23), 0)));
-}
-
 // The lowest n bits (none for n <= 0, all for n >= 32).
 __device__ __forceinline__ uint32_t low_bits(int n) {
   return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
 }
 
-// What the roles need to know of a unit.
-struct PfWork {
-  int row0;    // first packed row of the pair
-  int pos0;    // its position
-  int tokens;  // rows of the pair (<= 2 tpt), 0: no more units
-  int j;       // kv head
-  int kv;      // length of the sequence
-  int b;
-  int lo, hi;  // range of the pair's key blocks
-  int slot;    // of the partial result, or -1
+// What the roles need to know of a unit; tokens 0: there are no more.
+struct PfWork : PfUnit {
+  int j;  // kv head
 };
 
 struct PfCtl {
@@ -407,25 +397,15 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           ok = false;
           break;
         }
-        const int unit = atomicAdd(&p.list->next, 1);
+        const int unit = u == 0 ? blockIdx.x : atomicAdd(&p.list->next, 1) + gridDim.x;
         PfWork w{};
         Blocks bl{};
         if (unit < total) {
           const int e = unit / p.c.nkv;
-          const PfUnit pu = p.units[e];
-          const int per_pair = 2 * p.tpt;
-          int kv;
-          const int n = pf_rows(p, pu.b, kv, false);
-          w.b = pu.b;
-          w.kv = kv;
+          static_cast<PfUnit&>(w) = p.units[e];
           w.j = unit - e * p.c.nkv;
-          w.row0 = p.cu[pu.b] + pu.pair * per_pair;
-          w.pos0 = kv - n + pu.pair * per_pair;
-          w.tokens = min(per_pair, n - pu.pair * per_pair);
+          if (w.slot >= 0) w.slot = w.slot * p.c.nkv + w.j;
           bl = blocks_of(w.pos0, w.pos0 + w.tokens - 1, p.window, p.sinks);
-          w.lo = static_cast<int>(static_cast<long long>(bl.n) * pu.split / pu.nsplit);
-          w.hi = static_cast<int>(static_cast<long long>(bl.n) * (pu.split + 1) / pu.nsplit);
-          w.slot = pu.nsplit > 1 ? (p.slots[e] + pu.split) * p.c.nkv + w.j : -1;
         }
         ctl.work[us] = w;
         mbar_arrive(&ctl.u_full[us]);
@@ -638,12 +618,15 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         sphase ^= 1u;
         tcgen05_fence_after();
         uint32_t s[4][32];
+        bool half_only = false;  // no row of the tile sees the second 64 columns: their weights are 0
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(ts + c * 32, s[c]);
         tmem_ld_wait();
         if (k0 + kPfBlock - 1 > tile_pos || (p.window && k0 <= tile_pos + p.tpt - 1 - p.window)) {
           // visible columns of each 32: up to hi, from lo on or below sk
           const int hi = pos - k0 + 1, lo = p.window ? hi - p.window : 0, sk = p.sinks - k0;
+          // the last block of a pair is half unseen on average
+          half_only = tile_pos + p.tpt - k0 <= kPfBlock / 2;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const uint32_t see = low_bits(hi - c * 32) & (~low_bits(lo - c * 32) | low_bits(sk - c * 32));
@@ -680,23 +663,28 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         const float ms = m == -INFINITY ? 0.f : m;
         const uint64_t sc2 = pair2(p.scale_log2, p.scale_log2), ms2 = pair2(-ms, -ms);
         uint64_t sum[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        auto weigh = [&](int c) {
           uint32_t pk[16];
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
             const uint64_t y = fma2(pair2(__uint_as_float(s[c][2 * x]), __uint_as_float(s[c][2 * x + 1])), sc2, ms2);
             float2 e = split2(y);
-            if ((x & 7) < kPfPoly) {
-              e = ex2_poly(pair2(fmaxf(e.x, -127.f), fmaxf(e.y, -127.f)));
-            } else {
-              e.x = ex2(e.x);
-              e.y = ex2(e.y);
-            }
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
             sum[x & 3] = add2(sum[x & 3], pair2(e.x, e.y));
             pk[x] = pack_bf16x2(e.x, e.y);
           }
           tmem_st_32x32b_x16(ts + c * 16, pk);
+        };
+        weigh(0);
+        weigh(1);
+        if (half_only) {
+          const uint32_t none[16] = {};
+          tmem_st_32x32b_x16(ts + 32, none);
+          tmem_st_32x32b_x16(ts + 48, none);
+        } else {
+          weigh(2);
+          weigh(3);
         }
         const float2 sums = split2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
         l += sums.x + sums.y;
@@ -713,6 +701,13 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       const long long out_at =
           mine ? ((static_cast<long long>(w.row0) + t * p.tpt + token) * p.nq + w.j * p.grp + head) * kHeadDim : -1;
       float* part = w.slot >= 0 ? p.part + (static_cast<long long>(w.slot) * 2 + t) * kPfPartTile + row : nullptr;
+      // where this lane stores: row 8 k + lane / 4, columns 8 (lane % 4) of each 32
+      __nv_bfloat16* to_row[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const long long at = __shfl_sync(0xffffffffu, out_at, k * 8 + (lane >> 2));
+        to_row[k] = at >= 0 ? p.out + at + (lane & 3) * 8 : nullptr;
+      }
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
@@ -735,10 +730,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           __syncwarp();
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const int r = k * 8 + (lane >> 2);
-            const long long at = __shfl_sync(0xffffffffu, out_at, r);
-            const uint4 v = *reinterpret_cast<const uint4*>(&stg[warp - 4][r][(lane & 3) * 8]);
-            if (at >= 0) *reinterpret_cast<uint4*>(p.out + at + c * 32 + (lane & 3) * 8) = v;
+            const uint4 v = *reinterpret_cast<const uint4*>(&stg[warp - 4][k * 8 + (lane >> 2)][(lane & 3) * 8]);
+            if (to_row[k]) *reinterpret_cast<uint4*>(to_row[k] + c * 32) = v;
           }
         }
       }
@@ -802,7 +795,7 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const __grid_co
 // Sizes that the host can bound without the lengths.
 struct PfLayout {
   long long pairs, slots, entries;
-  size_t list, units, slot_of, splits, starts, part, total;
+  size_t list, units, splits, starts, part, total;
 };
 
 PfLayout pf_layout(long long T, long long B, int nkv, int grp, long long max_pages, int page_size) {
@@ -822,8 +815,6 @@ PfLayout pf_layout(long long T, long long B, int nkv, int grp, long long max_pag
   at += 256;
   L.units = at;
   at += round(sizeof(PfUnit) * L.entries);
-  L.slot_of = at;
-  at += round(sizeof(int) * L.entries);
   L.splits = at;
   at += round(sizeof(PfSplit) * (L.slots / 2 + 1));
   L.starts = at;
@@ -878,7 +869,6 @@ cudaError_t paged_prefill_launch(const __nv_bfloat16* q, long long q_stride, con
   p.status = reinterpret_cast<int*>(ws);
   p.list = reinterpret_cast<PfList*>(ws + L.list);
   p.units = reinterpret_cast<PfUnit*>(ws + L.units);
-  p.slots = reinterpret_cast<int*>(ws + L.slot_of);
   p.splits = reinterpret_cast<PfSplit*>(ws + L.splits);
   p.starts = reinterpret_cast<int*>(ws + L.starts);
   p.part = reinterpret_cast<float*>(ws + L.part);

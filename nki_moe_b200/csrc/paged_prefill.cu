@@ -30,11 +30,12 @@
 // P is rounded to bf16 (relative 2^-9 at most, the size of the output's own
 // rounding); sums and maxima are fp32.
 //
-// Work: a small kernel turns the lengths (device data) into a list of units,
-// (sequence, pair, range of key blocks), the longest of a sequence first;
-// CTAs take units from a counter.  A pair is cut into several ranges only
-// when there are too few pairs for the SMs; the parts are joined by a third
-// kernel.
+// Work: a small kernel turns the lengths (device data) into the list of pairs,
+// a sequence's longest first, with their counts of key blocks.  With pairs
+// enough, CTAs take whole ones from a counter.  Where one pair would be longer
+// than a CTA's share of all blocks (a chunk over a long cache), every CTA takes
+// an equal run of the list of blocks instead, the pairs that are cut leave
+// partial results, and a third kernel joins them.
 #include <cudaTypedefs.h>
 
 #include "paged.cuh"
@@ -73,15 +74,16 @@ struct __align__(16) PfUnit {
 };
 
 struct PfList {  // in the workspace
-  int count;     // entries; unit u is entry u / nkv, kv head u % nkv
-  int next;      // the counter that CTAs take units from, after one each
-  int splits;    // pairs that are cut into parts
-  int pad;
+  int pairs;
+  int next;   // the counter that CTAs take pairs from, after one each
+  int total;  // key blocks of all pairs and kv heads
+  int share;  // a CTA's run of them, or 0: CTAs take whole pairs
 };
 
-// A pair that is cut: its rows and its parts' slots (slot + split) * nkv + j.
+// What a CTA began and others went on with: the pair of a kv head whose parts
+// lie in slot 2 c + 1 of CTA c and the slots 0 of the CTAs after it.
 struct PfSplit {
-  int b, pair, slot, nsplit;
+  int pair, j, parts, pad;
 };
 
 struct PfParams {
@@ -90,14 +92,15 @@ struct PfParams {
   __nv_bfloat16* out;  // [T, nq * 128]
   int* status;
   PfList* list;
-  PfUnit* units;
-  PfSplit* splits;  // [count of cut pairs]
+  PfUnit* units;    // [pairs]
+  int* offs;        // [pairs + 1] key blocks before each pair
+  PfSplit* splits;  // [grid]
   int* starts;      // [B + 1] pairs before each sequence
-  float* part;      // [slots * nkv, 2, kPfPartTile]
+  float* part;      // [2 grid, 2, kPfPartTile]
   PagedCache c;
   int T, B, nq, grp, tpt;  // tpt: tokens per tile
   int window, sinks;
-  int sms, max_pairs, max_entries, max_slots;
+  int sms, max_pairs;
   float scale_log2;
 };
 
@@ -158,83 +161,66 @@ __device__ __forceinline__ int plan_scan(int v, int* warp_sums, int& total) {
 // One CTA: the list of units from the lengths.
 __global__ void __launch_bounds__(kPlanThreads) paged_prefill_plan_kernel(const __grid_constant__ PfParams p) {
   __shared__ int warp_sums[32];
-  __shared__ float warp_tot[32];
   __shared__ int near_starts[kPlanStarts + 1];
+  __shared__ int longest;
   const int tid = threadIdx.x;
   const int per_pair = 2 * p.tpt;
+  if (tid == 0) longest = 0;
   pdl_launch_dependents();
   pdl_wait();
   int pairs = 0;
-  float blocks = 0.f;  // all key blocks of all units, estimated from each sequence's first and last pair
   for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
     const int b = b0 + tid;
     int n = 0, kv = 0;
     if (b < p.B) n = pf_rows(p, b, kv, true);
-    const int np = (n + per_pair - 1) / per_pair;
-    if (np > 0) {
-      const int lo = kv - n;
-      const int a = blocks_of(lo, min(lo + per_pair, kv) - 1, p.window, p.sinks).n;
-      const int z = blocks_of(kv - 1 - (n - 1) % per_pair, kv - 1, p.window, p.sinks).n;
-      blocks += 0.5f * np * (a + z) * p.c.nkv;
-    }
     int total;
-    const int before = plan_scan(np, warp_sums, total);
-    if (b < p.B) (b <= kPlanStarts ? near_starts : p.starts)[b] = pairs + before;
-    pairs += total;
+    const int before = plan_scan((n + per_pair - 1) / per_pair, warp_sums, total);
+    if (b < p.B) (b <= kPlanStarts ? near_starts : p.starts)[b] = min(pairs + before, p.max_pairs);
+    pairs = min(pairs + total, p.max_pairs + 1);
   }
-  if (tid == 0) (p.B <= kPlanStarts ? near_starts : p.starts)[p.B] = pairs;
   if (pairs > p.max_pairs) {  // sequences that overlap: more rows than there are
     if (tid == 0) atomicOr(p.status, kDevErrBadIndex);
     pairs = p.max_pairs;
   }
-  blocks = warp_sum(blocks);
-  if ((tid & 31) == 0) warp_tot[tid >> 5] = blocks;
+  if (tid == 0) (p.B <= kPlanStarts ? near_starts : p.starts)[p.B] = pairs;
   __syncthreads();
-  blocks = 0.f;
-  for (int w = 0; w < kPlanThreads / 32; ++w) blocks += warp_tot[w];
-  const int most = max(kPfMinBlocks, static_cast<int>(blocks / p.sms) + 1);  // blocks of a unit
 
   auto start_of = [&](int b) { return b <= kPlanStarts ? near_starts[b] : p.starts[b]; };
-  int entries = 0, slots = 0, cut = 0;
+  long long blocks = 0;  // of the pairs so far
   for (int i0 = 0; i0 < pairs; i0 += kPlanThreads) {
     const int i = i0 + tid;
-    int ns = 0, b = 0, pair = 0, blocks = 0;
     PfUnit un{};
     if (i < pairs) {
-      int hi = p.B;
+      int b = 0, hi = p.B;
       while (hi - b > 1) {
         const int mid = (b + hi) >> 1;
         if (start_of(mid) <= i) b = mid; else hi = mid;
       }
       const int n = pf_rows(p, b, un.kv, false);
-      pair = start_of(b + 1) - 1 - i;  // the sequence's last pair, the longest, first
+      const int pair = (n + per_pair - 1) / per_pair - 1 - (i - start_of(b));  // a sequence's longest pair first
       un.b = b;
       un.row0 = p.cu[b] + pair * per_pair;
       un.pos0 = un.kv - n + pair * per_pair;
       un.tokens = min(per_pair, n - pair * per_pair);
-      blocks = blocks_of(un.pos0, un.pos0 + un.tokens - 1, p.window, p.sinks).n;
-      ns = (blocks + most - 1) / most;
+      un.hi = blocks_of(un.pos0, un.pos0 + un.tokens - 1, p.window, p.sinks).n;
+      un.slot = -1;
+      p.units[i] = un;
     }
+    const int most = __reduce_max_sync(0xffffffffu, un.hi);
+    if ((tid & 31) == 0) atomicMax(&longest, most);
     int total;
-    // parts are given up where the list or the slots would not hold them
-    int at = plan_scan(ns > 1 ? ns : 0, warp_sums, total);
-    const int room = min((p.max_slots - slots), p.max_entries - entries - (pairs - i0));
-    if (ns > 1 && at + ns > room) ns = 1;
-    const int slot = plan_scan(ns > 1 ? ns : 0, warp_sums, total) + slots;
-    slots += total;
-    const int k = plan_scan(ns > 1, warp_sums, total) + cut;
-    cut += total;
-    const int e = plan_scan(ns, warp_sums, total) + entries;
-    entries += total;
-    for (int s = 0; s < ns; ++s) {
-      un.lo = static_cast<int>(static_cast<long long>(blocks) * s / ns);
-      un.hi = static_cast<int>(static_cast<long long>(blocks) * (s + 1) / ns);
-      un.slot = ns > 1 ? slot + s : -1;
-      p.units[e + s] = un;
-    }
-    if (ns > 1) p.splits[k] = PfSplit{b, pair, slot, ns};
+    const int before = plan_scan(un.hi, warp_sums, total);
+    if (i < pairs) p.offs[i] = static_cast<int>(min(blocks + before, 0x7fffffffLL));
+    blocks += total;
   }
-  if (tid == 0) *p.list = PfList{entries, 0, cut, 0};
+  if (tid == 0) {
+    p.offs[pairs] = static_cast<int>(min(blocks, 0x7fffffffLL));
+    blocks *= p.c.nkv;
+    // a pair is cut only where one is longer than a CTA's share of the work
+    const long long share = max(static_cast<long long>(kPfMinBlocks), (blocks + p.sms - 1) / p.sms);
+    const bool cut = longest > share && blocks < (1LL << 30);
+    *p.list = PfList{pairs, 0, static_cast<int>(min(blocks, 1LL << 30)), cut ? static_cast<int>(share) : 0};
+  }
 }
 
 // ------------------------------------------------------------------ tensor memory, MMA with A from tensor memory
@@ -390,23 +376,46 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       int stage = 0, u = 0;
       uint32_t phase = 0, issued = 0, last_phase = 0;
       bool ok = true, q_issued = false;
-      const int total = p.list->count * p.c.nkv;
+      const PfList list = *p.list;
+      // a run of the list of key blocks (pair, kv head, block), or whole pairs
+      const int run_lo = min(list.total, static_cast<int>(blockIdx.x) * list.share);
+      const int run_hi = min(list.total, run_lo + list.share);
+      int at = run_lo, pair = 0;
+      if (list.share) {
+        p.splits[blockIdx.x].parts = 0;
+        for (int hi = list.pairs; hi - pair > 1;) {
+          const int mid = (pair + hi) >> 1;
+          if (p.offs[mid] * p.c.nkv <= at) pair = mid; else hi = mid;
+        }
+      }
       for (;; ++u) {
         const int us = u & 1;
         if (!mbar_wait(&ctl.u_empty[us], ((u >> 1) & 1) ^ 1u, &ctl.abort_flag, p.status)) {
           ok = false;
           break;
         }
-        const int unit = u == 0 ? blockIdx.x : atomicAdd(&p.list->next, 1) + gridDim.x;
         PfWork w{};
         Blocks bl{};
-        if (unit < total) {
-          const int e = unit / p.c.nkv;
-          static_cast<PfUnit&>(w) = p.units[e];
-          w.j = unit - e * p.c.nkv;
-          if (w.slot >= 0) w.slot = w.slot * p.c.nkv + w.j;
-          bl = blocks_of(w.pos0, w.pos0 + w.tokens - 1, p.window, p.sinks);
+        if (list.share == 0) {
+          const int unit = u == 0 ? blockIdx.x : atomicAdd(&p.list->next, 1) + gridDim.x;
+          if (unit < list.pairs * p.c.nkv) {
+            static_cast<PfUnit&>(w) = p.units[unit / p.c.nkv];
+            w.j = unit % p.c.nkv;
+          }
+        } else if (at < run_hi) {
+          static_cast<PfUnit&>(w) = p.units[pair];
+          const int base = p.offs[pair] * p.c.nkv, n = w.hi;
+          w.j = (at - base) / n;
+          const int item = base + w.j * n;  // the list's first block of (pair, kv head)
+          w.lo = at - item;
+          w.hi = min(n, run_hi - item);
+          const int first = item / list.share, parts = (item + n - 1) / list.share - first + 1;
+          if (parts > 1) w.slot = 2 * static_cast<int>(blockIdx.x) + (item < run_lo ? 0 : 1);
+          if (parts > 1 && item >= run_lo) p.splits[blockIdx.x] = PfSplit{pair, w.j, parts, 0};
+          at = item + w.hi;
+          if (w.hi == n && w.j == p.c.nkv - 1) ++pair;
         }
+        if (w.tokens) bl = blocks_of(w.pos0, w.pos0 + w.tokens - 1, p.window, p.sinks);
         ctl.work[us] = w;
         mbar_arrive(&ctl.u_full[us]);
         if (w.tokens == 0) break;
@@ -750,52 +759,52 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   }
 }
 
-// Joins the parts of cut pairs, in order: a CTA per (pair, kv head, 32 rows),
-// a lane per row, a warp per 16 columns.
+// Joins the parts of a cut pair, in order: a CTA per (pair and kv head, 32
+// rows), a lane per row, a warp per 16 columns.
 __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const __grid_constant__ PfParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31, col = (threadIdx.x >> 5) * 16;
-  const int total = p.list->splits * p.c.nkv * 8;
-  for (int i = blockIdx.x; i < total; i += gridDim.x) {
-    const int tile = (i >> 2) & 1, row = (i & 3) * 32 + lane, j = (i >> 3) % p.c.nkv;
-    const PfSplit sp = p.splits[(i >> 3) / p.c.nkv];
-    const int token = row / p.grp, head = row - token * p.grp;
-    const int at = sp.pair * 2 * p.tpt + tile * p.tpt + token;  // row of the sequence
-    const int start = p.cu[sp.b];
-    if (token >= p.tpt || at >= p.cu[sp.b + 1] - start) continue;
-    const float* part = p.part + (static_cast<long long>(sp.slot * p.c.nkv + j) * 2 + tile) * kPfPartTile + row;
-    const long long stride = static_cast<long long>(p.c.nkv) * 2 * kPfPartTile;
-    float m = -INFINITY;
-    for (int s = 0; s < sp.nsplit; ++s) m = fmaxf(m, __ldcg(part + s * stride + kHeadDim * kPfRows));
-    float l = 0.f, o[16];
+  if (p.list->share == 0) return;
+  const int cta = blockIdx.x >> 3, tile = (blockIdx.x >> 2) & 1;
+  const int lane = threadIdx.x & 31, col = (threadIdx.x >> 5) * 16, row = (blockIdx.x & 3) * 32 + lane;
+  const PfSplit sp = p.splits[cta];
+  if (sp.parts == 0) return;
+  const PfUnit un = p.units[sp.pair];
+  const int token = row / p.grp, head = row - token * p.grp;
+  if (token >= p.tpt || tile * p.tpt + token >= un.tokens) return;
+  auto part_of = [&](int s) {
+    const int slot = 2 * (cta + s) + (s == 0);
+    return p.part + (static_cast<long long>(slot) * 2 + tile) * kPfPartTile + row;
+  };
+  float m = -INFINITY;
+  for (int s = 0; s < sp.parts; ++s) m = fmaxf(m, __ldcg(part_of(s) + kHeadDim * kPfRows));
+  float l = 0.f, o[16];
 #pragma unroll
-    for (int x = 0; x < 16; ++x) o[x] = 0.f;
-    for (int s = 0; s < sp.nsplit; ++s) {
-      const float* from = part + s * stride;
-      const float f = m == -INFINITY ? 0.f : exp2f(__ldcg(from + kHeadDim * kPfRows) - m);
-      l = fmaf(f, __ldcg(from + (kHeadDim + 1) * kPfRows), l);
+  for (int x = 0; x < 16; ++x) o[x] = 0.f;
+  for (int s = 0; s < sp.parts; ++s) {
+    const float* from = part_of(s);
+    const float f = m == -INFINITY ? 0.f : exp2f(__ldcg(from + kHeadDim * kPfRows) - m);
+    l = fmaf(f, __ldcg(from + (kHeadDim + 1) * kPfRows), l);
 #pragma unroll
-      for (int x = 0; x < 16; ++x) o[x] = fmaf(f, __ldcg(from + (col + x) * kPfRows), o[x]);
-    }
-    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+    for (int x = 0; x < 16; ++x) o[x] = fmaf(f, __ldcg(from + (col + x) * kPfRows), o[x]);
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+  __nv_bfloat16* dst =
+      p.out + ((static_cast<long long>(un.row0) + tile * p.tpt + token) * p.nq + sp.j * p.grp + head) * kHeadDim + col;
 #pragma unroll
-    for (int x = 0; x < 16; ++x) o[x] *= inv;
-    __nv_bfloat16* dst = p.out + (static_cast<long long>(start + at) * p.nq + j * p.grp + head) * kHeadDim + col;
+  for (int x = 0; x < 16; x += 8) {
     float h[8];
 #pragma unroll
-    for (int x = 0; x < 16; x += 8) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) h[e] = o[x + e];
-      *reinterpret_cast<uint4*>(dst + x) = pack8(h);
-    }
+    for (int e = 0; e < 8; ++e) h[e] = o[x + e] * inv;
+    *reinterpret_cast<uint4*>(dst + x) = pack8(h);
   }
 }
 
 // Sizes that the host can bound without the lengths.
 struct PfLayout {
-  long long pairs, slots, entries;
-  size_t list, units, splits, starts, part, total;
+  long long pairs, grid;  // grid: of the main kernel
+  bool may_cut;
+  size_t list, units, offs, splits, starts, part, total;
 };
 
 PfLayout pf_layout(long long T, long long B, int nkv, int grp, long long max_pages, int page_size) {
@@ -803,24 +812,24 @@ PfLayout pf_layout(long long T, long long B, int nkv, int grp, long long max_pag
   const int tpt = kPfRows / grp;
   L.pairs = T / (2 * tpt) + B;
   const long long blocks = (max_pages * page_size + kPfBlock - 1) / kPfBlock;
-  const long long sms = device_sm_count();
-  // parts of all cut pairs: about one per SM and kv head share, twice that with the rounding
-  long long slots = blocks > kPfMinBlocks ? 2 * sms / nkv + 16 : 0;
-  const long long most = L.pairs * ((blocks + kPfMinBlocks - 1) / kPfMinBlocks);
-  L.slots = slots < most ? slots : most;
-  L.entries = L.pairs + L.slots;
+  const long long most = L.pairs * nkv * ((blocks + kPfMinBlocks - 1) / kPfMinBlocks);  // runs at least
+  L.grid = device_sm_count();
+  if (most < L.grid) L.grid = most;
+  L.may_cut = blocks > kPfMinBlocks;
   auto round = [](size_t n) { return (n + 255) & ~static_cast<size_t>(255); };
   size_t at = kPagedScratch;
   L.list = at;
   at += 256;
   L.units = at;
-  at += round(sizeof(PfUnit) * L.entries);
+  at += round(sizeof(PfUnit) * L.pairs);
+  L.offs = at;
+  at += round(sizeof(int) * (L.pairs + 1));
   L.splits = at;
-  at += round(sizeof(PfSplit) * (L.slots / 2 + 1));
+  at += round(sizeof(PfSplit) * L.grid);
   L.starts = at;
   at += round(sizeof(int) * (B + 1));
   L.part = at;
-  at += sizeof(float) * L.slots * nkv * 2 * kPfPartTile;
+  if (L.may_cut) at += sizeof(float) * 2 * L.grid * 2 * kPfPartTile;
   L.total = at;
   return L;
 }
@@ -869,6 +878,7 @@ cudaError_t paged_prefill_launch(const __nv_bfloat16* q, long long q_stride, con
   p.status = reinterpret_cast<int*>(ws);
   p.list = reinterpret_cast<PfList*>(ws + L.list);
   p.units = reinterpret_cast<PfUnit*>(ws + L.units);
+  p.offs = reinterpret_cast<int*>(ws + L.offs);
   p.splits = reinterpret_cast<PfSplit*>(ws + L.splits);
   p.starts = reinterpret_cast<int*>(ws + L.starts);
   p.part = reinterpret_cast<float*>(ws + L.part);
@@ -880,20 +890,16 @@ cudaError_t paged_prefill_launch(const __nv_bfloat16* q, long long q_stride, con
   p.tpt = tpt;
   p.window = window;
   p.sinks = sinks;
-  p.sms = device_sm_count();
+  p.sms = static_cast<int>(L.grid);
   p.max_pairs = static_cast<int>(L.pairs);
-  p.max_entries = static_cast<int>(L.entries);
-  p.max_slots = static_cast<int>(L.slots);
   p.scale_log2 = scale * kPfLog2e;
   cudaError_t e = launch_pdl(paged_prefill_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p);
   if (e != cudaSuccess) return e;
   e = allow_smem<paged_prefill_kernel>(static_cast<int>(kPfSmem));
   if (e != cudaSuccess) return e;
-  const long long units = L.entries * nkv;
-  const int grid = static_cast<int>(units < p.sms ? units : p.sms);
-  e = launch_pdl(paged_prefill_kernel, dim3(grid), dim3(kPfThreads), kPfSmem, s, mq, mk, mv, p);
-  if (e != cudaSuccess || L.slots == 0) return e;
-  return launch_pdl(paged_prefill_join_kernel, dim3(2 * p.sms), dim3(256), 0, s, p);
+  e = launch_pdl(paged_prefill_kernel, dim3(p.sms), dim3(kPfThreads), kPfSmem, s, mq, mk, mv, p);
+  if (e != cudaSuccess || !L.may_cut) return e;
+  return launch_pdl(paged_prefill_join_kernel, dim3(8 * p.sms), dim3(256), 0, s, p);
 }
 
 }  // namespace nkimoe

@@ -18,14 +18,14 @@ namespace nkimoe {
 
 namespace {
 
-constexpr int kLpThreads = 512;
+constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
-constexpr int kLpElems = 32;                        // elements per thread and chunk
-constexpr int kLpChunk = kLpThreads * kLpElems;     // 16384
+constexpr int kLpVecs = 4;                          // 16-byte vectors per thread and chunk
+constexpr int kLpChunkBytes = kLpThreads * kLpVecs * 16;  // 16 KB: 8192 bf16 or 4096 fp32 logits
 constexpr int kLpTopMax = 32;
-constexpr int kLpCand = 1024;                       // candidates a chunk may add before the slow path
 constexpr int kLpSplits = 32;                       // CTAs per row at most
-static_assert(kLpSplits <= 32 && 4 * 148 <= kPagedCounters, "one lane and one counter each");
+constexpr int kLpSplitRows = 4 * 148;               // rows from which on one CTA takes a whole row
+static_assert(kLpSplits <= 32 && kLpSplitRows <= kPagedCounters, "one lane and one counter each");
 // a CTA's part of a row in the workspace: m, s, t, count, then keys and ids
 constexpr int kLpPart = 4 + 2 * kLpTopMax;
 
@@ -39,7 +39,7 @@ struct LpParams {
   long long* top_ids;
   int* counters;  // [T], zero between calls
   float* part;    // [T, splits, kLpPart]
-  int V, top, splits, per_split;  // per_split: elements of a split, a multiple of the chunk
+  int V, top, splits, per_split;  // per_split: elements of a split, whole chunks
 };
 
 // Integers that order as the values do: NaN above +inf, -0 equal to +0.
@@ -49,6 +49,12 @@ __device__ __forceinline__ int order_key(float x) {
   return b < 0 ? b ^ 0x7fffffff : b;
 }
 __device__ __forceinline__ float key_value(int k) { return __int_as_float(k < 0 ? k ^ 0x7fffffff : k); }
+
+__device__ __forceinline__ float ex2_ftz(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 
 // Running maximum, sum and shifted first moment of a set of logits.
 struct Stat {
@@ -69,199 +75,217 @@ __device__ __forceinline__ void stat_join(Stat& a, const Stat& b) {
 }
 
 template <typename T>
-__device__ __forceinline__ float to_f(T v);
-template <>
-__device__ __forceinline__ float to_f<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+struct LpVec {
+  static constexpr int VE = 16 / sizeof(T);                 // elements per vector
+  static constexpr int NE = kLpVecs * VE;                   // per thread and chunk: 32 or 16
+  static constexpr int Chunk = kLpThreads * NE;             // per CTA and chunk
+};
 
-// A thread's elements of a chunk: vector v of the thread covers VE = 16 bytes
-// at element base + (v * threads + tid) * VE, the base rounded down to a
+__device__ __forceinline__ float lp_float(float v) { return v; }
+__device__ __forceinline__ float lp_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// A thread's vectors of a chunk, as loaded: vector v of the thread covers 16
+// bytes at element base + (v * threads + tid) * VE, the base being on a
 // 16-byte boundary.  Whole vectors are loaded as such; a vector that crosses
 // the row's ends is read element by element, and what lies outside is -inf.
 template <typename T>
-__device__ __forceinline__ void load_chunk(const T* row, long long base, int lo, int hi, float (&x)[kLpElems]) {
-  constexpr int VE = 16 / sizeof(T);
-  constexpr int NV = kLpElems / VE;
+__device__ __forceinline__ void load_chunk(const T* row, long long base, int lo, int hi, uint4 (&raw)[kLpVecs]) {
+  constexpr int VE = LpVec<T>::VE;
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
+  for (int v = 0; v < kLpVecs; ++v) {
     const long long e0 = base + static_cast<long long>(v * kLpThreads + threadIdx.x) * VE;
     if (e0 >= lo && e0 + VE <= hi) {
-      const uint4 u = __ldcs(reinterpret_cast<const uint4*>(row + e0));
-      if constexpr (sizeof(T) == 2) {
-        float f[8];
-        unpack8(u, f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[v * VE + e] = f[e];
-      } else {
-        x[v * VE] = __uint_as_float(u.x);
-        x[v * VE + 1] = __uint_as_float(u.y);
-        x[v * VE + 2] = __uint_as_float(u.z);
-        x[v * VE + 3] = __uint_as_float(u.w);
-      }
+      raw[v] = __ldcs(reinterpret_cast<const uint4*>(row + e0));
     } else {
+      uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < VE; ++e)
-        x[v * VE + e] = e0 + e >= lo && e0 + e < hi ? to_f<T>(row[e0 + e]) : -INFINITY;
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 2) {
+          const long long e = e0 + 2 * i;
+          const float a = e >= lo && e < hi ? lp_float(row[e]) : -INFINITY;
+          const float b = e + 1 >= lo && e + 1 < hi ? lp_float(row[e + 1]) : -INFINITY;
+          w[i] = pack_bf16x2(a, b);
+        } else {
+          w[i] = __float_as_uint(e0 + i >= lo && e0 + i < hi ? lp_float(row[e0 + i]) : -INFINITY);
+        }
+      }
+      raw[v] = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
 }
 
-struct TopShared {
-  int key[kLpCand + kLpTopMax];  // candidates, then the best so far
-  int id[kLpCand + kLpTopMax];
-  int best_key[kLpTopMax];
-  int best_id[kLpTopMax];
-  int count, have;
-  int red_key[kLpWarps], red_id[kLpWarps];
-};
+// Vector v of a chunk as fp32.
+template <typename T>
+__device__ __forceinline__ void unpack_vec(const uint4& raw, float (&x)[LpVec<T>::VE]) {
+  if constexpr (sizeof(T) == 2) {
+    unpack8(raw, x);
+  } else {
+    x[0] = __uint_as_float(raw.x);
+    x[1] = __uint_as_float(raw.y);
+    x[2] = __uint_as_float(raw.z);
+    x[3] = __uint_as_float(raw.w);
+  }
+}
 
 // a before b: the greater key, equal ones by the lower id
 __device__ __forceinline__ bool before(int ka, int ia, int kb, int ib) { return ka > kb || (ka == kb && ia < ib); }
 
-// The best `top` of the n entries in sh.key / sh.id, in order, into sh.best_*:
-// an entry's place is the number of entries before it.
-__device__ __forceinline__ void take_best(TopShared& sh, int n, int top) {
-  for (int i = threadIdx.x; i < n; i += kLpThreads) {
-    const int k = sh.key[i], id = sh.id[i];
-    int place = 0;
-    for (int j = 0; j < n && place < top; ++j) place += before(sh.key[j], sh.id[j], k, id);
-    if (place < top) {
-      sh.best_key[place] = k;
-      sh.best_id[place] = id;
+// A warp's best 32 so far, the lane-th best in each lane (INT_MIN: none; the
+// ids are all different, so no two entries are equal).
+struct WarpTop {
+  int key, id;
+
+  __device__ __forceinline__ void clear(int lane) {
+    key = INT_MIN;
+    id = INT_MAX - lane;
+  }
+
+  // Of a pair of lanes, d apart, the one with the bit clear (`up`: set) takes
+  // the entry that comes first.
+  __device__ __forceinline__ void exchange(int d, bool up, int lane) {
+    const int pk = __shfl_xor_sync(0xffffffffu, key, d), pi = __shfl_xor_sync(0xffffffffu, id, d);
+    if (before(pk, pi, key, id) == (((lane & d) == 0) != up)) {
+      key = pk;
+      id = pi;
     }
   }
-  if (threadIdx.x == 0) sh.have = min(n, top);
-  __syncthreads();
+
+  // Sorts any 32 entries (bitonic).
+  __device__ __forceinline__ void sort(int lane) {
+#pragma unroll
+    for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll
+      for (int d = n >> 1; d > 0; d >>= 1) exchange(d, n < 32 && (lane & n), lane);
+  }
+
+  // The first 32 of two sorted lists, sorted.
+  __device__ __forceinline__ void merge(const WarpTop& o, int lane) {
+    const int pk = __shfl_sync(0xffffffffu, o.key, 31 - lane), pi = __shfl_sync(0xffffffffu, o.id, 31 - lane);
+    if (before(pk, pi, key, id)) {
+      key = pk;
+      id = pi;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) exchange(d, false, lane);
+  }
+
+  __device__ __forceinline__ void insert(int k, int i, int lane) {
+    const int at = __popc(__ballot_sync(0xffffffffu, before(key, id, k, i)));
+    const int pk = __shfl_up_sync(0xffffffffu, key, 1), pi = __shfl_up_sync(0xffffffffu, id, 1);
+    if (lane > at) {
+      key = pk;
+      id = pi;
+    } else if (lane == at) {
+      key = k;
+      id = i;
+    }
+  }
+};
+
+struct TopShared {
+  int2 list[kLpWarps][32];
+  int2 cand[kLpWarps][64];  // a warp's candidates that are not in its list yet
+  uint4 spread[kLpWarps][kLpVecs];
+  int floor;                // `top` elements of the row are known to be at or above this key
+};
+
+// The CTA's best 32 of the warps' lists, in warp 0.
+__device__ __forceinline__ void join_warps(TopShared& sh, WarpTop& best, int warp, int lane) {
+#pragma unroll
+  for (int d = 1; d < kLpWarps; d <<= 1) {
+    sh.list[warp][lane] = make_int2(best.key, best.id);
+    __syncthreads();
+    if ((warp & (2 * d - 1)) == 0) {
+      const int2 o = sh.list[warp + d][lane];
+      best.merge(WarpTop{o.x, o.y}, lane);
+    }
+    __syncthreads();
+  }
 }
 
-// Joins a chunk (this thread's x, first element ids as load_chunk lays them
-// out) into the row's best `top`.  Called by the whole CTA.
+// Joins a warp's part of a chunk (its lanes' vectors, their largest values mx)
+// into the warp's best.  The warps do this each for itself; what one has found
+// lets the others pass over more (sh.floor).  Most chunks of a row hold
+// nothing: one comparison and one vote.
 template <typename T>
-__device__ __forceinline__ void top_chunk(TopShared& sh, const float (&x)[kLpElems], long long base, int lo, int hi,
-                                          int top) {
-  constexpr int VE = 16 / sizeof(T);
-  auto id_of = [&](int i) {
-    return static_cast<int>(base + static_cast<long long>((i / VE) * kLpThreads + threadIdx.x) * VE + (i % VE));
-  };
-  int mk = INT_MIN;  // INT_MIN is no value's key: -inf has 0x807fffff
-#pragma unroll
-  for (int i = 0; i < kLpElems; ++i) {
-    const int id = id_of(i);
-    if (id >= lo && id < hi) mk = max(mk, order_key(x[i]));
-  }
-  const int have = sh.have;
+__device__ __forceinline__ void warp_top(TopShared& sh, WarpTop& best, const uint4 (&raw)[kLpVecs], float mx, bool nan,
+                                         long long base, int lo, int hi, int top, int lane) {
+  constexpr int VE = LpVec<T>::VE;
+  // the lane's greatest key (what lies outside the row counts as -inf here,
+  // which only lowers the bound)
+  const int mk = nan ? 0x7fffffff : order_key(mx);
+  const int worst = __shfl_sync(0xffffffffu, best.key, top - 1);
   int least;  // keys from here on are candidates
-  if (have == top) {
-    // later elements lose ties against the ones already held
-    least = sh.best_key[top - 1] == 0x7fffffff ? 0x7fffffff : sh.best_key[top - 1] + 1;
+  if (worst != INT_MIN) {
+    least = worst == 0x7fffffff ? worst : worst + 1;  // later elements lose ties against the ones held
   } else {
-    // the top-th largest of the threads' maxima has `top` elements at or above
-    // it; its upper 16 bits, found bit by bit, serve as well
-    unsigned v = 0;
-    const unsigned u = static_cast<unsigned>(mk) ^ 0x80000000u;
-    for (int bit = 31; bit >= 16; --bit) {
-      const unsigned cand = v | (1u << bit);
-      if (__syncthreads_count(u >= cand) >= top) v = cand;
-    }
-    least = static_cast<int>(v ^ 0x80000000u);
-    if (least == INT_MIN) least = INT_MIN + 1;  // fewer than `top` threads have a value: all values
-  }
-  if (mk >= least) {
+    // the top-th largest of the lanes' maxima has `top` elements at or above it
+    int place = 0;
 #pragma unroll
-    for (int i = 0; i < kLpElems; ++i) {
-      const int id = id_of(i), k = order_key(x[i]);
-      if (id >= lo && id < hi && k >= least) {
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < kLpCand) {
-          sh.key[at] = k;
-          sh.id[at] = id;
-        }
-      }
+    for (int o = 0; o < 32; ++o) {
+      const int k = __shfl_sync(0xffffffffu, mk, o);
+      place += k > mk || (k == mk && o < lane);
     }
+    least = __shfl_sync(0xffffffffu, mk, __ffs(__ballot_sync(0xffffffffu, place == top - 1)) - 1);
   }
-  __syncthreads();
-  const int n = sh.count;
-  __syncthreads();
-  if (n == 0) return;
-  if (threadIdx.x == 0) sh.count = 0;
-  if (n <= kLpCand) {
-    if (threadIdx.x < have) {
-      sh.key[n + threadIdx.x] = sh.best_key[threadIdx.x];
-      sh.id[n + threadIdx.x] = sh.best_id[threadIdx.x];
-    }
-    __syncthreads();
-    take_best(sh, n + have, top);
-    return;
-  }
-  // More candidates than fit (many equal values): the chunk's best one after
-  // another, each the first that comes after the one before it.
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int pk = INT_MAX, pid = -1;
-  int got = 0;
-  for (; got < top; ++got) {
-    int bk = INT_MIN, bid = INT_MAX;
+  least = max(least, *const_cast<volatile int*>(&sh.floor));
+  unsigned lanes = __ballot_sync(0xffffffffu, mk >= least);
+  if (lanes == 0) return;
+  int2* const cand = sh.cand[threadIdx.x >> 5];
+  uint4* const spread = sh.spread[threadIdx.x >> 5];
+  int n = 0;
+  while (lanes) {  // one lane's elements at a time, spread over the warp
+    const int src = __ffs(lanes) - 1;
+    lanes &= lanes - 1;
+    if (lane == src) {
 #pragma unroll
-    for (int i = 0; i < kLpElems; ++i) {
-      const int id = id_of(i), k = order_key(x[i]);
-      if (id >= lo && id < hi && before(pk, pid, k, id) && before(k, id, bk, bid)) {
-        bk = k;
-        bid = id;
-      }
+      for (int v = 0; v < kLpVecs; ++v) spread[v] = raw[v];
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const int ok = __shfl_xor_sync(0xffffffffu, bk, o), oid = __shfl_xor_sync(0xffffffffu, bid, o);
-      if (before(ok, oid, bk, bid)) {
-        bk = ok;
-        bid = oid;
-      }
+    __syncwarp();
+    float x = 0.f;
+    if (lane < LpVec<T>::NE) x = lp_float(reinterpret_cast<const T*>(spread)[lane]);
+    const int k = order_key(x);
+    const int tid = (threadIdx.x & ~31) + src;
+    const long long id = base + static_cast<long long>((lane / VE) * kLpThreads + tid) * VE + lane % VE;
+    const bool in = lane < LpVec<T>::NE && id >= lo && id < hi && k >= least;
+    const unsigned hit = __ballot_sync(0xffffffffu, in);
+    if (in) cand[n + __popc(hit & ((1u << lane) - 1u))] = make_int2(k, static_cast<int>(id));
+    n += __popc(hit);
+    __syncwarp();
+    if (n < 32 && lanes) continue;
+    if (n <= 4) {  // a few: each to its place
+      for (int i = 0; i < n; ++i) best.insert(cand[i].x, cand[i].y, lane);
+      n = 0;
     }
-    if (lane == 0) {
-      sh.red_key[warp] = bk;
-      sh.red_id[warp] = bid;
+    while (n >= 32 || (n > 0 && lanes == 0)) {  // many (the first chunk): sorted and merged, 32 at a time
+      const int2 c = lane < n ? cand[lane] : make_int2(INT_MIN, INT_MAX - 32 - lane);
+      WarpTop more{c.x, c.y};
+      more.sort(lane);
+      best.merge(more, lane);
+      const int2 rest = cand[32 + lane];
+      __syncwarp();
+      cand[lane] = rest;
+      __syncwarp();
+      n = max(n - 32, 0);
     }
-    __syncthreads();
-    bk = INT_MIN;
-    bid = INT_MAX;
-    for (int w = 0; w < kLpWarps; ++w)
-      if (before(sh.red_key[w], sh.red_id[w], bk, bid)) {
-        bk = sh.red_key[w];
-        bid = sh.red_id[w];
-      }
-    __syncthreads();
-    if (bk == INT_MIN) break;
-    if (threadIdx.x == 0) {
-      sh.key[got] = bk;
-      sh.id[got] = bid;
-    }
-    pk = bk;
-    pid = bid;
   }
-  if (threadIdx.x < have) {
-    sh.key[got + threadIdx.x] = sh.best_key[threadIdx.x];
-    sh.id[got + threadIdx.x] = sh.best_id[threadIdx.x];
-  }
-  __syncthreads();
-  take_best(sh, got + have, top);
+  const int now = __shfl_sync(0xffffffffu, best.key, top - 1);
+  if (lane == 0 && now > worst) atomicMax(&sh.floor, now);
 }
 
 // CTA (split, row): elements [split * per_split, ...) of the row in chunks of
-// 16384 held in registers; the last CTA of a row joins the splits' parts.
+// 16 KB held in registers, the next chunk in flight; the last CTA of a row joins the splits' parts.
 //
 // Bound by HBM over many rows (the logits read once).
 template <typename T, bool kTop>
-__global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpParams p) {
+__global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const LpParams p) {
   __shared__ TopShared sh;
   __shared__ Stat warp_stat[kLpWarps];
   __shared__ int s_last;
   const int split = blockIdx.x % p.splits;
   const long long r = blockIdx.x / p.splits;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (kTop && threadIdx.x == 0) {
-    sh.count = 0;
-    sh.have = 0;
-  }
+  if (kTop && threadIdx.x == 0) sh.floor = INT_MIN;
   pdl_launch_dependents();
   pdl_wait();
   const T* row = static_cast<const T*>(p.x) + r * p.row_stride;
@@ -272,28 +296,51 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpP
   __syncthreads();
 
   Stat st{-INFINITY, 0.f, 0.f};
-  for (long long base = first; base < hi; base += kLpChunk) {
-    float x[kLpElems];
-    load_chunk<T>(row, base, lo, hi, x);
+  WarpTop best;
+  best.clear(lane);
+  uint4 raw[kLpVecs], next[kLpVecs];
+  if (first < hi) load_chunk<T>(row, first, lo, hi, next);
+  for (long long base = first; base < hi; base += LpVec<T>::Chunk) {
+#pragma unroll
+    for (int v = 0; v < kLpVecs; ++v) raw[v] = next[v];
+    // the next chunk is in flight while this one is worked on
+    if (base + LpVec<T>::Chunk < hi) load_chunk<T>(row, base + LpVec<T>::Chunk, lo, hi, next);
+    constexpr int VE = LpVec<T>::VE;
+    float x[VE];
     float mx = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kLpElems; ++i) mx = fmaxf(mx, x[i]);
+    for (int v = 0; v < kLpVecs; ++v) {
+      unpack_vec<T>(raw[v], x);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) mx = fmaxf(mx, x[e]);
+    }
     Stat c{mx, 0.f, 0.f};
     if (mx == -INFINITY) {  // nothing, or only -inf and NaN: a NaN has to show
 #pragma unroll
-      for (int i = 0; i < kLpElems; ++i)
-        if (x[i] != x[i]) c.s = x[i];
-    } else {
+      for (int v = 0; v < kLpVecs; ++v) {
+        unpack_vec<T>(raw[v], x);
 #pragma unroll
-      for (int i = 0; i < kLpElems; ++i) {
-        const float d = x[i] - mx;
-        const float e = exp2f(d * 1.4426950408889634f);
-        c.s += e;
-        c.t = fmaf(e, fmaxf(d, -200.f), c.t);  // e is 0 there, and 0 * -inf would not be
+        for (int e = 0; e < VE; ++e)
+          if (x[e] != x[e]) c.s = x[e];
       }
+    } else {
+      float s4[4] = {0.f, 0.f, 0.f, 0.f}, t4[4] = {0.f, 0.f, 0.f, 0.f};  // short chains
+#pragma unroll
+      for (int v = 0; v < kLpVecs; ++v) {
+        unpack_vec<T>(raw[v], x);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          const float d = x[i] - mx;
+          const float e = ex2_ftz(d * 1.4426950408889634f);
+          s4[i & 3] += e;
+          t4[i & 3] = fmaf(e, fmaxf(d, -200.f), t4[i & 3]);  // e is 0 there, and 0 * -inf would not be
+        }
+      }
+      c.s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      c.t = (t4[0] + t4[1]) + (t4[2] + t4[3]);
     }
     stat_join(st, c);
-    if constexpr (kTop) top_chunk<T>(sh, x, base, lo, hi, p.top);
+    if constexpr (kTop) warp_top<T>(sh, best, raw, mx, c.s != c.s, base, lo, hi, p.top, lane);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -305,6 +352,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpP
   }
   if (lane == 0) warp_stat[warp] = st;
   __syncthreads();
+  if constexpr (kTop) join_warps(sh, best, warp, lane);
   if (warp == 0) {
     st = lane < kLpWarps ? warp_stat[lane] : Stat{-INFINITY, 0.f, 0.f};
 #pragma unroll
@@ -319,11 +367,10 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpP
 
   if (p.splits > 1) {
     float* part = p.part + (r * p.splits + split) * kLpPart;
-    const int have = kTop ? sh.have : 0;
-    if (threadIdx.x == 0) __stcg(reinterpret_cast<float4*>(part), make_float4(st.m, st.s, st.t, __int_as_float(have)));
-    if (kTop && threadIdx.x < have) {
-      __stcg(reinterpret_cast<int*>(part) + 4 + threadIdx.x, sh.best_key[threadIdx.x]);
-      __stcg(reinterpret_cast<int*>(part) + 4 + kLpTopMax + threadIdx.x, sh.best_id[threadIdx.x]);
+    if (threadIdx.x == 0) __stcg(reinterpret_cast<float4*>(part), make_float4(st.m, st.s, st.t, 0.f));
+    if (kTop && threadIdx.x < p.top) {  // lane < top of warp 0
+      __stcg(reinterpret_cast<int*>(part) + 4 + lane, best.key);
+      __stcg(reinterpret_cast<int*>(part) + 4 + kLpTopMax + lane, best.id);
     }
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -332,19 +379,26 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpP
       if (s_last) {
         __threadfence();
         p.counters[r] = 0;
-        if (kTop) sh.count = 0;
       }
     }
     __syncthreads();
     if (!s_last) return;
     const float* parts = p.part + r * p.splits * kLpPart;
+    if constexpr (kTop) {  // the splits' lists, spread over the warps
+      best.clear(lane);
+      for (int sp = warp; sp < p.splits; sp += kLpWarps) {
+        const int* ip = reinterpret_cast<const int*>(parts + sp * kLpPart) + 4 + lane;
+        WarpTop o;
+        o.clear(lane);
+        if (lane < p.top) o = WarpTop{__ldcg(ip), __ldcg(ip + kLpTopMax)};
+        best.merge(o, lane);
+      }
+    }
     if (warp == 0) {
       st = Stat{-INFINITY, 0.f, 0.f};
-      int n = 0;
       if (lane < p.splits) {
         const float4 v = __ldcg(reinterpret_cast<const float4*>(parts + lane * kLpPart));
         st = Stat{v.x, v.y, v.z};
-        n = __float_as_int(v.w);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
@@ -354,26 +408,8 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpP
         b.t = __shfl_xor_sync(0xffffffffu, st.t, o);
         stat_join(st, b);
       }
-      if (kTop) {  // where each split's entries go
-        int at = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int v = __shfl_up_sync(0xffffffffu, at, o);
-          if (lane >= o) at += v;
-        }
-        if (lane == 31) sh.count = at;
-        at -= n;
-        const int* ip = reinterpret_cast<const int*>(parts + lane * kLpPart);
-        for (int i = 0; i < n; ++i) {
-          sh.key[at + i] = __ldcg(ip + 4 + i);
-          sh.id[at + i] = __ldcg(ip + 4 + kLpTopMax + i);
-        }
-      }
     }
-    if constexpr (kTop) {
-      __syncthreads();
-      take_best(sh, sh.count, p.top);
-    }
+    if constexpr (kTop) join_warps(sh, best, warp, lane);
   }
 
   if (threadIdx.x == 0) {
@@ -381,7 +417,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpP
     const long long tok = p.tokens[r];
     float lp = 0.f;  // a negative token: none is given
     if (tok >= p.V) lp = __int_as_float(0x7fc00000);
-    else if (tok >= 0) lp = (to_f<T>(row[tok]) - st.m) - ls;
+    else if (tok >= 0) lp = (lp_float(row[tok]) - st.m) - ls;
     p.logprob[r] = lp;
     p.entropy[r] = ls - st.t / st.s;
     warp_stat[0] = Stat{st.m, ls, 0.f};
@@ -389,23 +425,26 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LpP
   if constexpr (kTop) {
     __syncthreads();
     if (threadIdx.x < p.top) {
-      const int k = sh.best_key[threadIdx.x];
+      const int k = best.key;
       const float v = k == 0x7fffffff ? __int_as_float(0x7fc00000) : key_value(k);
       p.top_lp[r * p.top + threadIdx.x] = (v - warp_stat[0].m) - warp_stat[0].s;
-      p.top_ids[r * p.top + threadIdx.x] = sh.best_id[threadIdx.x];
+      p.top_ids[r * p.top + threadIdx.x] = best.id;
     }
   }
 }
 
 // Chunks of a row: up to 7 places of the first lie before the row (it starts
 // at the 16-byte boundary at or below the row's).
-long long lp_chunks(long long V) { return (V + 7 + kLpChunk - 1) / kLpChunk; }
+long long lp_chunks(long long V, int dtype) {
+  const int chunk = kLpChunkBytes / (dtype == kF32 ? 4 : 2);
+  return (V + 7 + chunk - 1) / chunk;
+}
 
-// CTAs per row: enough for about two waves of resident CTAs, and no more than
-// the row has chunks.
-int lp_splits(long long T, long long V) {
-  const long long chunks = lp_chunks(V);
-  long long n = (4LL * 148 + T - 1) / T;
+// CTAs per row: one wave of resident CTAs (4 per SM) in all, and no more than the
+// row has chunks.
+int lp_splits(long long T, long long V, int dtype) {
+  const long long chunks = lp_chunks(V, dtype);
+  long long n = (kLpSplitRows + T - 1) / T;
   if (n > chunks) n = chunks;
   if (n > kLpSplits) n = kLpSplits;
   return static_cast<int>(n < 1 ? 1 : n);
@@ -422,7 +461,8 @@ cudaError_t lp_launch(const LpParams& p, long long rows, cudaStream_t s) {
 
 size_t token_logprobs_workspace_bytes(long long T, long long V, int top_n) {
   (void)top_n;
-  const int splits = T > 0 ? lp_splits(T, V) : 1;
+  // the wider type has the more chunks
+  const int splits = T > 0 ? lp_splits(T, V, kF32) : 1;
   return kPagedScratch + (splits > 1 ? sizeof(float) * T * splits * kLpPart : 0);
 }
 
@@ -442,10 +482,10 @@ cudaError_t token_logprobs_launch(const void* logits, int dtype, long long row_s
   p.part = reinterpret_cast<float*>(ws + kPagedScratch);
   p.V = static_cast<int>(V);
   p.top = top_n;
-  const long long chunks = lp_chunks(V);
-  const long long per = (chunks + lp_splits(T, V) - 1) / lp_splits(T, V);
+  const long long chunks = lp_chunks(V, dtype), most = lp_splits(T, V, dtype);
+  const long long per = (chunks + most - 1) / most;
   p.splits = static_cast<int>((chunks + per - 1) / per);
-  p.per_split = static_cast<int>(per) * kLpChunk;
+  p.per_split = static_cast<int>(per * (kLpChunkBytes / (dtype == kF32 ? 4 : 2)));
   return dtype == kF32 ? lp_launch<float>(p, T, s) : lp_launch<__nv_bfloat16>(p, T, s);
 }
 

@@ -39,6 +39,7 @@ struct LpParams {
   long long* top_ids;
   int* counters;  // [T], zero between calls
   float* part;    // [T, splits, kLpPart]
+  long long rows;
   int V, top, splits, per_split;  // per_split: elements of a split, whole chunks
 };
 
@@ -50,28 +51,37 @@ __device__ __forceinline__ int order_key(float x) {
 }
 __device__ __forceinline__ float key_value(int k) { return __int_as_float(k < 0 ? k ^ 0x7fffffff : k); }
 
-__device__ __forceinline__ float ex2_ftz(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 // Running maximum, sum and shifted first moment of a set of logits.
 struct Stat {
   float m, s, t;
 };
 
-__device__ __forceinline__ void stat_join(Stat& a, const Stat& b) {
+// The factor that moves sums from maximum `from` to `to` (>= from), and the
+// distance itself; a side without a finite value (m = -inf, s = 0) moves
+// nothing where both are -inf, its distance would be inf - inf.
+__device__ __forceinline__ void stat_move(Stat& a, float to) {
+  const float d = a.m == to ? 0.f : a.m - to;
+  const float f = ex2(d * 1.4426950408889634f);
+  // f is 0 from -200 on; d itself times a sum could overflow, and 0 * inf would not be 0
+  a.t = f * fmaf(fmaxf(d, -200.f), a.s, a.t);
+  a.s *= f;
+  a.m = to;
+}
+
+__device__ __forceinline__ void stat_join(Stat& a, Stat b) {
   const float m = fmaxf(a.m, b.m);
-  // a side without a finite value (m = -inf, s = 0) moves nothing; its shift
-  // would be inf - inf
-  const float da = a.m == m ? 0.f : a.m - m, db = b.m == m ? 0.f : b.m - m;
-  const float fa = expf(da), fb = expf(db);
-  // e^{d} is 0 from -200 on; d itself times a sum could overflow, and 0 * inf would not be 0
-  const float ca = fmaxf(da, -200.f), cb = fmaxf(db, -200.f);
-  a.t = fa * fmaf(ca, a.s, a.t) + fb * fmaf(cb, b.s, b.t);
-  a.s = fa * a.s + fb * b.s;
-  a.m = m;
+  stat_move(a, m);
+  stat_move(b, m);
+  a.s += b.s;
+  a.t += b.t;
+}
+
+// The stat of the whole warp, in every lane.
+__device__ __forceinline__ Stat stat_warp(Stat a) {
+  stat_move(a, warp_max(a.m));
+  a.s = warp_sum(a.s);
+  a.t = warp_sum(a.t);
+  return a;
 }
 
 template <typename T>
@@ -91,6 +101,12 @@ __device__ __forceinline__ float lp_float(__nv_bfloat16 v) { return __bfloat162f
 template <typename T>
 __device__ __forceinline__ void load_chunk(const T* row, long long base, int lo, int hi, uint4 (&raw)[kLpVecs]) {
   constexpr int VE = LpVec<T>::VE;
+  if (base >= lo && base + LpVec<T>::Chunk <= hi) {
+    const uint4* at = reinterpret_cast<const uint4*>(row + base) + threadIdx.x;
+#pragma unroll
+    for (int v = 0; v < kLpVecs; ++v) raw[v] = __ldcs(at + v * kLpThreads);
+    return;
+  }
 #pragma unroll
   for (int v = 0; v < kLpVecs; ++v) {
     const long long e0 = base + static_cast<long long>(v * kLpThreads + threadIdx.x) * VE;
@@ -125,6 +141,60 @@ __device__ __forceinline__ void unpack_vec(const uint4& raw, float (&x)[LpVec<T>
     x[2] = __uint_as_float(raw.z);
     x[3] = __uint_as_float(raw.w);
   }
+}
+
+// Maxima that let a NaN through, of two bf16 or of fp32.
+__device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// The largest value of a thread's vectors (NaN if one is).
+template <typename T>
+__device__ __forceinline__ float max_of(const uint4 (&raw)[kLpVecs]) {
+  if constexpr (sizeof(T) == 2) {
+    uint32_t m = max_nan_bf16x2(max_nan_bf16x2(raw[0].x, raw[0].y), max_nan_bf16x2(raw[0].z, raw[0].w));
+#pragma unroll
+    for (int v = 1; v < kLpVecs; ++v)
+      m = max_nan_bf16x2(m, max_nan_bf16x2(max_nan_bf16x2(raw[v].x, raw[v].y), max_nan_bf16x2(raw[v].z, raw[v].w)));
+    const float2 f = unpack_bf16x2(m);
+    return max_nan(f.x, f.y);
+  } else {
+    float m = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < kLpVecs; ++v)
+      m = max_nan(m, max_nan(max_nan(__uint_as_float(raw[v].x), __uint_as_float(raw[v].y)),
+                             max_nan(__uint_as_float(raw[v].z), __uint_as_float(raw[v].w))));
+    return m;
+  }
+}
+
+// A pair of neighbouring elements as fp32, -inf raised to the type's lowest
+// finite value (so that 0 times its distance from the maximum is 0).
+template <typename T, int P>
+__device__ __forceinline__ uint64_t pair_of(const uint4& u) {
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t w = max_nan_bf16x2(P == 0 ? u.x : P == 1 ? u.y : P == 2 ? u.z : u.w, 0xff7fff7fu);
+    return pair2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  } else {
+    const float low = __uint_as_float(0xff7fffffu);
+    return pair2(max_nan(__uint_as_float(P == 0 ? u.x : u.z), low), max_nan(__uint_as_float(P == 0 ? u.y : u.w), low));
+  }
+}
+
+// Adds a pair's e^d and e^d d to the sums.
+__device__ __forceinline__ void add_pair(uint64_t x, uint64_t neg_max, uint64_t& s, uint64_t& t) {
+  const uint64_t d = add2(x, neg_max);
+  const float2 y = split2(mul2(d, pair2(1.4426950408889634f, 1.4426950408889634f)));
+  const uint64_t e = pair2(ex2(y.x), ex2(y.y));
+  s = add2(s, e);
+  t = fma2(e, d, t);
 }
 
 // a before b: the greater key, equal ones by the lower id
@@ -208,12 +278,12 @@ __device__ __forceinline__ void join_warps(TopShared& sh, WarpTop& best, int war
 // lets the others pass over more (sh.floor).  Most chunks of a row hold
 // nothing: one comparison and one vote.
 template <typename T>
-__device__ __forceinline__ void warp_top(TopShared& sh, WarpTop& best, const uint4 (&raw)[kLpVecs], float mx, bool nan,
+__device__ __forceinline__ void warp_top(TopShared& sh, WarpTop& best, const uint4 (&raw)[kLpVecs], float mx,
                                          long long base, int lo, int hi, int top, int lane) {
   constexpr int VE = LpVec<T>::VE;
   // the lane's greatest key (what lies outside the row counts as -inf here,
   // which only lowers the bound)
-  const int mk = nan ? 0x7fffffff : order_key(mx);
+  const int mk = order_key(mx);
   const int worst = __shfl_sync(0xffffffffu, best.key, top - 1);
   int least;  // keys from here on are candidates
   if (worst != INT_MIN) {
@@ -274,17 +344,18 @@ __device__ __forceinline__ void warp_top(TopShared& sh, WarpTop& best, const uin
 }
 
 // CTA (split, row): elements [split * per_split, ...) of the row in chunks of
-// 16 KB held in registers, the next chunk in flight; the last CTA of a row joins the splits' parts.
+// 16 KB held in registers, the next chunk in flight; the last CTA of a row
+// joins the splits' parts.
 //
 // Bound by HBM over many rows (the logits read once).
 template <typename T, bool kTop>
-__global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const LpParams p) {
+__global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LpParams p) {
   __shared__ TopShared sh;
   __shared__ Stat warp_stat[kLpWarps];
   __shared__ int s_last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int split = blockIdx.x % p.splits;
   const long long r = blockIdx.x / p.splits;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (kTop && threadIdx.x == 0) sh.floor = INT_MIN;
   pdl_launch_dependents();
   pdl_wait();
@@ -293,77 +364,65 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const LpP
   const long long first = static_cast<long long>(split) * p.per_split - mis;  // a 16-byte boundary
   const int lo = static_cast<int>(max(first, 0LL));
   const int hi = static_cast<int>(min(first + p.per_split, static_cast<long long>(p.V)));
-  __syncthreads();
+  uint4 raw[kLpVecs], next[kLpVecs];
+  if (first < hi) load_chunk<T>(row, first, lo, hi, next);
+  // the given token's logit, long before it is needed
+  long long tok = -1;
+  float x_tok = 0.f;
+  if (threadIdx.x == 0) {
+    tok = p.tokens[r];
+    if (tok >= 0 && tok < p.V) x_tok = lp_float(row[tok]);
+  }
+  if (kTop) __syncthreads();
 
   Stat st{-INFINITY, 0.f, 0.f};
   WarpTop best;
   best.clear(lane);
-  uint4 raw[kLpVecs], next[kLpVecs];
-  if (first < hi) load_chunk<T>(row, first, lo, hi, next);
   for (long long base = first; base < hi; base += LpVec<T>::Chunk) {
 #pragma unroll
     for (int v = 0; v < kLpVecs; ++v) raw[v] = next[v];
-    // the next chunk is in flight while this one is worked on
     if (base + LpVec<T>::Chunk < hi) load_chunk<T>(row, base + LpVec<T>::Chunk, lo, hi, next);
-    constexpr int VE = LpVec<T>::VE;
-    float x[VE];
-    float mx = -INFINITY;
-#pragma unroll
-    for (int v = 0; v < kLpVecs; ++v) {
-      unpack_vec<T>(raw[v], x);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) mx = fmaxf(mx, x[e]);
-    }
+    const float mx = max_of<T>(raw);
     Stat c{mx, 0.f, 0.f};
-    if (mx == -INFINITY) {  // nothing, or only -inf and NaN: a NaN has to show
+    if (mx > __uint_as_float(0xff7fffffu) && mx < 1e37f) {
+      uint64_t s2[2] = {0, 0}, t2[2] = {0, 0};  // short chains
+      const uint64_t nm = pair2(-mx, -mx);
 #pragma unroll
       for (int v = 0; v < kLpVecs; ++v) {
-        unpack_vec<T>(raw[v], x);
-#pragma unroll
-        for (int e = 0; e < VE; ++e)
-          if (x[e] != x[e]) c.s = x[e];
-      }
-    } else {
-      float s4[4] = {0.f, 0.f, 0.f, 0.f}, t4[4] = {0.f, 0.f, 0.f, 0.f};  // short chains
-#pragma unroll
-      for (int v = 0; v < kLpVecs; ++v) {
-        unpack_vec<T>(raw[v], x);
-#pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          const float d = x[i] - mx;
-          const float e = ex2_ftz(d * 1.4426950408889634f);
-          s4[i & 3] += e;
-          t4[i & 3] = fmaf(e, fmaxf(d, -200.f), t4[i & 3]);  // e is 0 there, and 0 * -inf would not be
+        add_pair(pair_of<T, 0>(raw[v]), nm, s2[0], t2[0]);
+        add_pair(pair_of<T, 1>(raw[v]), nm, s2[1], t2[1]);
+        if constexpr (sizeof(T) == 2) {
+          add_pair(pair_of<T, 2>(raw[v]), nm, s2[0], t2[0]);
+          add_pair(pair_of<T, 3>(raw[v]), nm, s2[1], t2[1]);
         }
       }
-      c.s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
-      c.t = (t4[0] + t4[1]) + (t4[2] + t4[3]);
+      const float2 s = split2(add2(s2[0], s2[1])), t = split2(add2(t2[0], t2[1]));
+      c.s = s.x + s.y;
+      c.t = t.x + t.y;
+    } else if (mx != -INFINITY) {
+      // a NaN, an infinity, or values whose distance from the maximum may overflow
+#pragma unroll 1
+      for (int v = 0; v < kLpVecs; ++v) {
+        float x[LpVec<T>::VE];
+        unpack_vec<T>(v == 0 ? raw[0] : v == 1 ? raw[1] : v == 2 ? raw[2] : raw[3], x);
+#pragma unroll
+        for (int i = 0; i < LpVec<T>::VE; ++i) {
+          const float d = x[i] - mx;
+          const float e = ex2(d * 1.4426950408889634f);
+          c.s += e;
+          c.t = fmaf(e, fmaxf(d, -200.f), c.t);  // e is 0 there
+        }
+      }
+      if (mx != mx) c.m = -INFINITY;  // the sums hold the NaN
     }
     stat_join(st, c);
-    if constexpr (kTop) warp_top<T>(sh, best, raw, mx, c.s != c.s, base, lo, hi, p.top, lane);
+    if constexpr (kTop) warp_top<T>(sh, best, raw, mx, base, lo, hi, p.top, lane);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stat b;
-    b.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-    b.t = __shfl_xor_sync(0xffffffffu, st.t, o);
-    stat_join(st, b);
-  }
+  st = stat_warp(st);
   if (lane == 0) warp_stat[warp] = st;
   __syncthreads();
   if constexpr (kTop) join_warps(sh, best, warp, lane);
-  if (warp == 0) {
-    st = lane < kLpWarps ? warp_stat[lane] : Stat{-INFINITY, 0.f, 0.f};
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      Stat b;
-      b.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-      b.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-      b.t = __shfl_xor_sync(0xffffffffu, st.t, o);
-      stat_join(st, b);
-    }
-  }
+  if (warp == 0) st = stat_warp(lane < kLpWarps ? warp_stat[lane] : Stat{-INFINITY, 0.f, 0.f});
 
   if (p.splits > 1) {
     float* part = p.part + (r * p.splits + split) * kLpPart;
@@ -400,35 +459,24 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const LpP
         const float4 v = __ldcg(reinterpret_cast<const float4*>(parts + lane * kLpPart));
         st = Stat{v.x, v.y, v.z};
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        Stat b;
-        b.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-        b.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-        b.t = __shfl_xor_sync(0xffffffffu, st.t, o);
-        stat_join(st, b);
-      }
+      st = stat_warp(st);
     }
     if constexpr (kTop) join_warps(sh, best, warp, lane);
   }
 
-  if (threadIdx.x == 0) {
+  if (warp == 0) {
     const float ls = logf(st.s);
-    const long long tok = p.tokens[r];
-    float lp = 0.f;  // a negative token: none is given
-    if (tok >= p.V) lp = __int_as_float(0x7fc00000);
-    else if (tok >= 0) lp = (lp_float(row[tok]) - st.m) - ls;
-    p.logprob[r] = lp;
-    p.entropy[r] = ls - st.t / st.s;
-    warp_stat[0] = Stat{st.m, ls, 0.f};
-  }
-  if constexpr (kTop) {
-    __syncthreads();
-    if (threadIdx.x < p.top) {
-      const int k = best.key;
-      const float v = k == 0x7fffffff ? __int_as_float(0x7fc00000) : key_value(k);
-      p.top_lp[r * p.top + threadIdx.x] = (v - warp_stat[0].m) - warp_stat[0].s;
-      p.top_ids[r * p.top + threadIdx.x] = best.id;
+    if (lane == 0) {
+      float lp = 0.f;  // a negative token: none is given
+      if (tok >= p.V) lp = __int_as_float(0x7fc00000);
+      else if (tok >= 0) lp = (x_tok - st.m) - ls;
+      p.logprob[r] = lp;
+      p.entropy[r] = ls - st.t / st.s;
+    }
+    if (kTop && lane < p.top) {
+      const float v = best.key == 0x7fffffff ? __int_as_float(0x7fc00000) : key_value(best.key);
+      p.top_lp[r * p.top + lane] = (v - st.m) - ls;
+      p.top_ids[r * p.top + lane] = best.id;
     }
   }
 }
@@ -451,8 +499,8 @@ int lp_splits(long long T, long long V, int dtype) {
 }
 
 template <typename T>
-cudaError_t lp_launch(const LpParams& p, long long rows, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>(rows * p.splits));
+cudaError_t lp_launch(const LpParams& p, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>(p.rows * p.splits));
   return p.top ? launch_pdl(token_logprobs_kernel<T, true>, grid, dim3(kLpThreads), 0, s, p)
                : launch_pdl(token_logprobs_kernel<T, false>, grid, dim3(kLpThreads), 0, s, p);
 }
@@ -480,13 +528,14 @@ cudaError_t token_logprobs_launch(const void* logits, int dtype, long long row_s
   char* ws = static_cast<char*>(workspace);
   p.counters = reinterpret_cast<int*>(ws + kPagedStatusBytes);
   p.part = reinterpret_cast<float*>(ws + kPagedScratch);
+  p.rows = T;
   p.V = static_cast<int>(V);
   p.top = top_n;
   const long long chunks = lp_chunks(V, dtype), most = lp_splits(T, V, dtype);
   const long long per = (chunks + most - 1) / most;
   p.splits = static_cast<int>((chunks + per - 1) / per);
   p.per_split = static_cast<int>(per * (kLpChunkBytes / (dtype == kF32 ? 4 : 2)));
-  return dtype == kF32 ? lp_launch<float>(p, T, s) : lp_launch<__nv_bfloat16>(p, T, s);
+  return dtype == kF32 ? lp_launch<float>(p, s) : lp_launch<__nv_bfloat16>(p, s);
 }
 
 }  // namespace nkimoe

@@ -19,7 +19,7 @@ namespace nkimoe {
 // calls, then scratch.  The first two have a fixed size, so calls of any of
 // the kernels and any shape may share one workspace on a stream.
 constexpr size_t kPagedStatusBytes = 256;
-constexpr int kPagedCounters = 1024;
+constexpr int kPagedCounters = 8192;
 constexpr size_t kPagedScratch = kPagedStatusBytes + sizeof(int) * kPagedCounters;
 
 struct PagedCache {
@@ -62,6 +62,40 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
 __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
   return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
                     pack_bf16x2(v[6], v[7]));
+}
+
+// Two fp32 operations in one instruction (sm_100).
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x to 2 ulp, subnormal results as 0 (ex2 of the hardware).
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 // RMSNorm + rotate-half RoPE of one head held by a half-warp: lane l of the

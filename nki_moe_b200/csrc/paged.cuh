@@ -98,31 +98,77 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-// RMSNorm + rotate-half RoPE of one head held by a half-warp: lane l of the
-// sixteen owns elements [8l, 8l + 8), its rotate-half partner is lane l ^ 8.
-// `w` are the lane's norm weights, `cs` the cos / sin table of the position.
-__device__ __forceinline__ void norm_rope_half(const float (&x)[8], const float (&w)[8], const float2* cs, float eps,
-                                               int l, float (&o)[8]) {
-  float ss = 0.f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-  for (int d = 8; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-  const float r = rsqrtf(ss * (1.f / kHeadDim) + eps);
-  float n[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) n[e] = x[e] * r * w[e];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float other = __shfl_xor_sync(0xffffffffu, n[e], 8);
-    const float2 t = cs[(l & 7) * 8 + e];
-    o[e] = fmaf(n[e], t.x, (l < 8 ? -other : other) * t.y);
-  }
+// A head held by a half-warp: lane l of the sixteen owns elements [4l, 4l + 4)
+// and their rotate-half partners [64 + 4l, 64 + 4l + 4), each as two pairs, so
+// the rotation needs no other lane.
+struct HeadPart {
+  uint64_t a[2], b[2];
+};
+
+__device__ __forceinline__ uint64_t pair_of_bf16x2(uint32_t u) {
+  return pair2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ __forceinline__ HeadPart part_of_rows(const uint2& lo, const uint2& hi) {
+  return HeadPart{{pair_of_bf16x2(lo.x), pair_of_bf16x2(lo.y)}, {pair_of_bf16x2(hi.x), pair_of_bf16x2(hi.y)}};
+}
+__device__ __forceinline__ uint32_t bf16x2_of_pair(uint64_t v) {
+  const float2 f = split2(v);
+  return pack_bf16x2(f.x, f.y);
+}
+__device__ __forceinline__ uint2 row_of_pairs(const uint64_t (&v)[2]) {
+  return make_uint2(bf16x2_of_pair(v[0]), bf16x2_of_pair(v[1]));
 }
 
-__device__ __forceinline__ void load_weight8(const void* w, int w_dtype, int l, float (&o)[8]) {
+// The lane's norm weights.
+__device__ __forceinline__ HeadPart load_weight_part(const void* w, int w_dtype, int l) {
+  float f[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) o[e] = head_wload(w, w_dtype, l * 8 + e);
+  for (int e = 0; e < 4; ++e) {
+    f[e] = head_wload(w, w_dtype, l * 4 + e);
+    f[4 + e] = head_wload(w, w_dtype, 64 + l * 4 + e);
+  }
+  return HeadPart{{pair2(f[0], f[1]), pair2(f[2], f[3])}, {pair2(f[4], f[5]), pair2(f[6], f[7])}};
+}
+
+// cos, sin and -sin of frequencies 4l .. 4l + 3, as two pairs each.
+struct TurnPart {
+  uint64_t c[2], s[2], ms[2];
+};
+__device__ __forceinline__ TurnPart turn_part(const float2* tab, int l) {
+  TurnPart t;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const float2 x = tab[l * 4 + 2 * e], y = tab[l * 4 + 2 * e + 1];
+    t.c[e] = pair2(x.x, y.x);
+    t.s[e] = pair2(x.y, y.y);
+    t.ms[e] = pair2(-x.y, -y.y);
+  }
+  return t;
+}
+
+// RMSNorm of the head times the weights, then rotate-half RoPE, times `scale`:
+// the rotation is linear, so the norm's factor comes last.  All 32 lanes of
+// the warp call it.
+__device__ __forceinline__ HeadPart norm_rope_part(const HeadPart& x, const HeadPart& w, const TurnPart& t, float eps,
+                                                   float scale = 1.f) {
+  uint64_t sq = mul2(x.a[0], x.a[0]);
+  sq = fma2(x.a[1], x.a[1], sq);
+  sq = fma2(x.b[0], x.b[0], sq);
+  sq = fma2(x.b[1], x.b[1], sq);
+  const float2 q = split2(sq);
+  float ss = q.x + q.y;
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+  const float r = rsqrtf(ss * (1.f / kHeadDim) + eps) * scale;
+  const uint64_t r2 = pair2(r, r);
+  HeadPart o;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const uint64_t a = mul2(x.a[e], w.a[e]), b = mul2(x.b[e], w.b[e]);
+    o.a[e] = mul2(fma2(b, t.ms[e], mul2(a, t.c[e])), r2);
+    o.b[e] = mul2(fma2(a, t.s[e], mul2(b, t.c[e])), r2);
+  }
+  return o;
 }
 
 // Lets a kernel take `bytes` of dynamic shared memory, once per device.

@@ -109,7 +109,7 @@ template <bool kWide>  // 9 to 16 heads per kv head
 struct PdShared {
   __nv_bfloat16 stage[kPdWarps][kPdStages][kPdStage];
   __nv_bfloat16 q[kWide ? 2 : 1][16][kPdQRow];  // narrow: rows 0-7 hi, 8-15 lo; wide: hi, lo
-  __nv_bfloat16 knew[kHeadDim], vnew[kHeadDim];
+  __align__(16) __nv_bfloat16 knew[kHeadDim], vnew[kHeadDim];
   float2 tab[kHeadDim / 2];
   float ml[kPdWarps][16][2];
   int warp_sum[kPdWarps];
@@ -252,34 +252,48 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
       const int l = lane & 15, half = tid >> 4;
       const __nv_bfloat16* row = p.qkv + static_cast<long long>(b) * (p.nq + 2 * nkv) * D;
       constexpr int kHalves = kPdThreads / 16;
-      float w[8];
-      load_weight8(p.qw, p.w_dtype, l, w);
+      const TurnPart turn = turn_part(sh.tab, l);
+      HeadPart w = load_weight_part(p.qw, p.w_dtype, l);
       for (int h0 = 0; h0 < (kWide ? 16 : 8); h0 += kHalves) {
         const int h = h0 + half;
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, o[8];
-        if (h < grp) unpack8(*reinterpret_cast<const uint4*>(row + static_cast<long long>(j * grp + h) * D + l * 8), x);
-        norm_rope_half(x, w, sh.tab, p.eps, l, o);
-        float rest[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          o[e] = h < grp ? o[e] * p.scale_log2 : 0.f;
-          rest[e] = o[e] - __bfloat162float(__float2bfloat16_rn(o[e]));
+        uint2 lo = make_uint2(0u, 0u), hi = lo;
+        if (h < grp) {
+          const uint2* from = reinterpret_cast<const uint2*>(row + static_cast<long long>(j * grp + h) * D) + l;
+          lo = from[0];
+          hi = from[16];
         }
-        *reinterpret_cast<uint4*>(&sh.q[0][h][l * 8]) = pack8(o);
-        *reinterpret_cast<uint4*>(kWide ? &sh.q[kWide ? 1 : 0][h][l * 8] : &sh.q[0][h + 8][l * 8]) = pack8(rest);
+        const HeadPart o = norm_rope_part(part_of_rows(lo, hi), w, turn, p.eps, p.scale_log2);  // 0 for no head
+        const uint2 ha = row_of_pairs(o.a), hb = row_of_pairs(o.b);
+        const uint64_t minus = pair2(-1.f, -1.f);
+        const HeadPart top = part_of_rows(ha, hb);
+        const HeadPart rest{{fma2(top.a[0], minus, o.a[0]), fma2(top.a[1], minus, o.a[1])},
+                            {fma2(top.b[0], minus, o.b[0]), fma2(top.b[1], minus, o.b[1])}};
+        uint2* q_hi = reinterpret_cast<uint2*>(&sh.q[0][h][0]);
+        uint2* q_lo = reinterpret_cast<uint2*>(kWide ? &sh.q[kWide ? 1 : 0][h][0] : &sh.q[0][h + 8][0]);
+        q_hi[l] = ha;
+        q_hi[16 + l] = hb;
+        q_lo[l] = row_of_pairs(rest.a);
+        q_lo[16 + l] = row_of_pairs(rest.b);
       }
       if (owns_new && warp == kPdWarps - 1) {
-        const uint4 u = *reinterpret_cast<const uint4*>(row + static_cast<long long>(p.nq + (lane < 16 ? 0 : nkv) + j) * D + l * 8);
-        float x[8], o[8];
-        load_weight8(p.kw, p.w_dtype, l, w);
-        unpack8(u, x);
-        norm_rope_half(x, w, sh.tab, p.eps, l, o);
-        const uint4 put = lane < 16 ? pack8(o) : u;  // the value bit for bit
-        *reinterpret_cast<uint4*>((lane < 16 ? sh.knew : sh.vnew) + l * 8) = put;
+        const uint2* from =
+            reinterpret_cast<const uint2*>(row + static_cast<long long>(p.nq + (lane < 16 ? 0 : nkv) + j) * D) + l;
+        uint2 lo = from[0], hi = from[16];
+        w = load_weight_part(p.kw, p.w_dtype, l);
+        const HeadPart o = norm_rope_part(part_of_rows(lo, hi), w, turn, p.eps);
+        if (lane < 16) {  // the value goes bit for bit
+          lo = row_of_pairs(o.a);
+          hi = row_of_pairs(o.b);
+        }
+        uint2* keep = reinterpret_cast<uint2*>(lane < 16 ? sh.knew : sh.vnew);
+        keep[l] = lo;
+        keep[16 + l] = hi;
         const int pg = table[pos >> p.c.page_shift];
         if (pg >= 0 && pg < p.c.num_pages) {
-          const long long off = ((static_cast<long long>(j) << p.c.page_shift) + (pos & page_mask)) * D + l * 8;
-          *reinterpret_cast<uint4*>((lane < 16 ? p.c.k + pg * p.c.k_stride : p.c.v + pg * p.c.v_stride) + off) = put;
+          const long long off = ((static_cast<long long>(j) << p.c.page_shift) + (pos & page_mask)) * D;
+          uint2* dst = reinterpret_cast<uint2*>((lane < 16 ? p.c.k + pg * p.c.k_stride : p.c.v + pg * p.c.v_stride) + off);
+          dst[l] = lo;
+          dst[16 + l] = hi;
         }
       }
     }

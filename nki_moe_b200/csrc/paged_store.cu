@@ -13,7 +13,7 @@ namespace nkimoe {
 namespace {
 
 constexpr int kStoreThreads = 256;
-constexpr int kStoreHalves = kStoreThreads / 16;
+constexpr int kStoreFew = 4 * 148;  // rows that get a CTA each
 
 struct StoreParams {
   const __nv_bfloat16* qkv;  // [T, (nq + 2 nkv) * 128]
@@ -25,6 +25,7 @@ struct StoreParams {
   int* status;
   PagedCache c;
   RopeTurns turns;
+  long long T;
   int w_dtype, B, nq;
   float eps;
 };
@@ -44,67 +45,87 @@ __device__ __forceinline__ int sequence_of(const int* cu, int B, int t, int lane
   return lo;
 }
 
-// One CTA per row; a half-warp per head (16-byte pieces).  The row's loads go
-// out before the position is known, so the two latencies overlap.
+// kWarps warps share a row, a half-warp a head; a warp needs no other's work
+// but the norm weights in shared memory.  Its first heads' loads go out before
+// the row's position is known, so the two latencies overlap.
 //
 // Bound by HBM: (nq + 2 nkv) * 256 bytes read and as many written per row.
-__global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const __grid_constant__ StoreParams p) {
+template <int kWarps>
+__global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_store_kernel(const __grid_constant__ StoreParams p) {
   constexpr int D = kHeadDim;
-  constexpr int kAhead = 3;  // heads per half-warp in flight: 48 heads in one pass
-  __shared__ float2 tab[D / 2];
-  const int lane = threadIdx.x & 31, l = threadIdx.x & 15, half = threadIdx.x >> 4;
-  const long long t = blockIdx.x;
+  constexpr int kHalves = 2 * kWarps;                     // heads of a row at a time
+  constexpr int kAhead = kWarps >= 4 ? 3 : 5;             // heads per half-warp in flight
+  __shared__ __align__(16) float wtab[2][D];
+  __shared__ __align__(16) float2 tab[kStoreThreads / 32][D / 2];
+  const int lane = threadIdx.x & 31, l = threadIdx.x & 15, warp = threadIdx.x >> 5;
+  const int half = (warp % kWarps) * 2 + (lane >> 4);
+  const long long t = static_cast<long long>(blockIdx.x) * (kStoreThreads / 32 / kWarps) + warp / kWarps;
   const int nh = p.nq + 2 * p.c.nkv;
   pdl_launch_dependents();
   pdl_wait();
-  const uint4* row = reinterpret_cast<const uint4*>(p.qkv + t * nh * D);
-  uint4 raw[kAhead];
+  const uint2* row = reinterpret_cast<const uint2*>(p.qkv + t * nh * D) + l;  // head h: row[32 h], row[32 h + 16]
+  uint2 raw[kAhead][2];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
-    const int h = half + i * kStoreHalves;
-    if (h < nh) raw[i] = __ldcs(row + h * 16 + l);
+    const int h = half + i * kHalves;
+    if (h < nh && t < p.T) {
+      raw[i][0] = __ldcs(row + h * 32);
+      raw[i][1] = __ldcs(row + h * 32 + 16);
+    }
   }
-  if (t >= p.cu[p.B]) return;  // rows behind the last sequence
+  wtab[threadIdx.x >> 7][threadIdx.x & 127] = head_wload(threadIdx.x < D ? p.qw : p.kw, p.w_dtype, threadIdx.x & 127);
+  __syncthreads();
+  if (t >= p.T || t >= p.cu[p.B]) return;  // behind the last sequence
   const int b = sequence_of(p.cu, p.B, static_cast<int>(t), lane);
   const int start = p.cu[b], end = p.cu[b + 1];
   const int pos = p.kv_lens[b] - end + static_cast<int>(t);
   const int slot = pos >> p.c.page_shift;
   if (t < start || t >= end || pos < 0 || slot >= p.c.max_pages) {
-    if (threadIdx.x == 0) atomicOr(p.status, kDevErrBadIndex);
+    if (lane == 0) atomicOr(p.status, kDevErrBadIndex);
     return;
   }
   const int page = p.c.table[b * p.c.table_stride + slot];
   const bool held = page >= 0 && page < p.c.num_pages;
-  if (!held && page != -1 && threadIdx.x == 0) atomicOr(p.status, kDevErrBadIndex);
-  if (threadIdx.x < D / 2) tab[threadIdx.x] = rope_cos_sin(p.turns.f[threadIdx.x], pos);
-  float qw[8], kw[8];
-  load_weight8(p.qw, p.w_dtype, l, qw);
-  load_weight8(p.kw, p.w_dtype, l, kw);
-  __syncthreads();
-  const int in_page = pos & ((1 << p.c.page_shift) - 1);
+  if (!held && page != -1 && lane == 0) atomicOr(p.status, kDevErrBadIndex);
+  tab[warp][lane] = rope_cos_sin(p.turns.f[lane], pos);
+  tab[warp][lane + 32] = rope_cos_sin(p.turns.f[lane + 32], pos);
+  __syncwarp();
+  const TurnPart turn = turn_part(tab[warp], l);
+  // where the row's heads go, this lane's part
+  const int in_page = pos & ((1 << p.c.page_shift) - 1), head_shift = p.c.page_shift + 5;  // in 8-byte pieces
+  uint2* const q_dst = reinterpret_cast<uint2*>(p.q_out + t * p.nq * D) + l;
+  uint2* const k_dst = reinterpret_cast<uint2*>(p.c.k + (held ? page * p.c.k_stride + in_page * D : 0)) + l;
+  uint2* const v_dst = reinterpret_cast<uint2*>(p.c.v + (held ? page * p.c.v_stride + in_page * D : 0)) + l;
   // a half-warp past the last head runs along with the other (the norm
   // shuffles within the whole warp) and stores nothing
-  for (int h0 = 0; h0 < nh; h0 += kAhead * kStoreHalves) {
+  for (int h0 = 0; h0 < nh; h0 += kAhead * kHalves) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int h = h0 + half + i * kStoreHalves;
+      const int h = h0 + half + i * kHalves;
       if ((h & ~1) >= nh) break;
-      uint4 u = make_uint4(0u, 0u, 0u, 0u);
-      if (h < nh) u = h0 == 0 ? raw[i] : __ldcs(row + h * 16 + l);
-      const bool is_q = h < p.nq, is_k = !is_q && h < p.nq + p.c.nkv;
-      float x[8], w[8], o[8];
-      unpack8(u, x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = is_q ? qw[e] : kw[e];
-      norm_rope_half(x, w, tab, p.eps, l, o);
-      if (h >= nh) continue;
-      if (is_q) {
-        *reinterpret_cast<uint4*>(p.q_out + (t * p.nq + h) * D + l * 8) = pack8(o);
-      } else if (held) {
-        const int j = is_k ? h - p.nq : h - p.nq - p.c.nkv;
-        __nv_bfloat16* dst = is_k ? p.c.k + page * p.c.k_stride : p.c.v + page * p.c.v_stride;
-        dst += ((static_cast<long long>(j) << p.c.page_shift) + in_page) * D + l * 8;
-        *reinterpret_cast<uint4*>(dst) = is_k ? pack8(o) : u;  // the value bit for bit
+      uint2 lo = raw[i][0], hi = raw[i][1];
+      if (h + kAhead * kHalves < nh) {
+        raw[i][0] = __ldcs(row + (h + kAhead * kHalves) * 32);
+        raw[i][1] = __ldcs(row + (h + kAhead * kHalves) * 32 + 16);
+      }
+      const bool is_q = h < p.nq, is_v = h >= p.nq + p.c.nkv;
+      if (!__all_sync(0xffffffffu, is_v)) {
+        HeadPart w;
+        const float* wt = wtab[is_q ? 0 : 1] + l * 4;
+        *reinterpret_cast<ulonglong2*>(w.a) = *reinterpret_cast<const ulonglong2*>(wt);
+        *reinterpret_cast<ulonglong2*>(w.b) = *reinterpret_cast<const ulonglong2*>(wt + 64);
+        const HeadPart o = norm_rope_part(part_of_rows(lo, hi), w, turn, p.eps);
+        if (!is_v) {  // a value goes bit for bit
+          lo = row_of_pairs(o.a);
+          hi = row_of_pairs(o.b);
+        }
+      }
+      if (h < nh && (is_q || held)) {
+        uint2* const dst = is_q ? q_dst + h * 32
+                           : is_v ? v_dst + (static_cast<long long>(h - p.nq - p.c.nkv) << head_shift)
+                                  : k_dst + (static_cast<long long>(h - p.nq) << head_shift);
+        dst[0] = lo;
+        dst[16] = hi;
       }
     }
   }
@@ -135,10 +156,16 @@ cudaError_t paged_store_launch(const __nv_bfloat16* qkv, const void* qw, const v
   p.c = cache;
   p.turns = rope_turns(theta);
   p.w_dtype = w_dtype;
+  p.T = T;
   p.B = B;
   p.nq = nq;
   p.eps = eps;
-  return launch_pdl(paged_store_kernel, dim3(static_cast<unsigned>(T)), dim3(kStoreThreads), 0, s, p);
+  // few rows: a CTA's eight warps on each; many: a warp each, so that the lookups
+  // and the sines of a row are done once (8192 rows of 32 + 2 * 4 heads: 37 us,
+  // with two warps 46, with eight 42)
+  if (T <= kStoreFew)
+    return launch_pdl(paged_store_kernel<8>, dim3(static_cast<unsigned>(T)), dim3(kStoreThreads), 0, s, p);
+  return launch_pdl(paged_store_kernel<1>, dim3(static_cast<unsigned>((T + 7) / 8)), dim3(kStoreThreads), 0, s, p);
 }
 
 }  // namespace nkimoe

@@ -162,7 +162,7 @@ int nkimoe_paged_decode_attention(const void* qkv, const void* q_weight, const v
   PagedCache c;
   NKI_CHECK(check_cache(k_pages, v_pages, k_page_stride, v_page_stride, num_pages, page_size, page_table, table_stride,
                         max_pages, n_kv_heads, &c));
-  NKI_REQUIRE(batch * n_kv_heads * ((max_pages * page_size + 63) / 64) < 0x7fff0000LL, NKIMOE_ERR_UNSUPPORTED,
+  NKI_REQUIRE(batch * n_kv_heads * ((max_pages * page_size + 63) / 64 + 6) < 0x7fff0000LL, NKIMOE_ERR_UNSUPPORTED,
               "batch and page table too large");
   NKI_REQUIRE(qkv && q_weight && k_weight && positions && out && workspace, NKIMOE_ERR_INVALID_ARG, "null pointer");
   NKI_REQUIRE(aligned16(qkv) && aligned16(out) && aligned16(workspace) &&

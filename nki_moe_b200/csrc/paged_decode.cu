@@ -11,7 +11,8 @@
 // qwen_with_nki.py:330-350 (per-head q/k norms, then RoPE).
 //
 // Split: the batch's visible positions, in granules of 64, form one list over
-// (sequence, kv head, granule), and every CTA takes an equal run of it, so a
+// (sequence, kv head, granule), each (sequence, kv head) preceded by places
+// that stand for its own cost, and every CTA takes an equal run of it, so a
 // batch of any mix of lengths loads all SMs alike and the launch needs no
 // length on the host.  A (sequence, kv head) whose granules fall to several
 // CTAs leaves one partial (m, l, o) per CTA; the last of them to finish
@@ -38,6 +39,7 @@ constexpr int kPdRow = kHeadDim;                // elements per staged row (swiz
 constexpr int kPdStage = 2 * kPdTile * kPdRow;  // elements per stage: K and V
 constexpr int kPdPart = 132;                    // floats per partial and head: o[128], m, l, pad
 constexpr int kPdCtasPerSm = 2;
+constexpr int kPdItem = 6;                      // granules that beginning and ending an item costs
 constexpr float kPdLog2e = 1.4426950408889634f;
 constexpr int kPdMaxBatch = 4096;
 constexpr int kPdQRow = kHeadDim + 8;           // padded query row (conflict-free ldmatrix)
@@ -137,7 +139,7 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
     int n = 0;
     if (b < p.B) {
       const int pos = pd_position(p, b, blockIdx.x == 0);
-      if (pos >= 0) n = granules_of(pos, p.window, p.sinks).n * nkv;
+      if (pos >= 0) n = (granules_of(pos, p.window, p.sinks).n + kPdItem) * nkv;
     }
     int incl = n;
 #pragma unroll
@@ -179,12 +181,14 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
     }
     const int pos = pd_position(p, b, false);
     const Granules gr = granules_of(pos, p.window, p.sinks);
-    const int j = (at - before[b]) / gr.n;
-    const int item = before[b] + j * gr.n;  // the list's first granule of (b, j)
-    const int g_lo = at - item, g_hi = min(gr.n, run_hi - item);
+    const int j = (at - before[b]) / (gr.n + kPdItem);
+    // the list's first granule of (b, j), behind the places that stand for its own cost
+    const int item = before[b] + j * (gr.n + kPdItem) + kPdItem;
+    const int g_lo = max(at - item, 0), g_hi = min(gr.n, run_hi - item);
+    at = item + gr.n;
+    if (g_hi <= 0) break;  // the run ends before the item's granules
     const int first_cta = item / share, parts = (item + gr.n - 1) / share - first_cta + 1;
     const int* table = p.c.table + b * p.c.table_stride;
-    at = item + g_hi;
 
     // this warp's tiles: 16 positions of each granule; lane i looks up the
     // page of the warp's tile i (of the next 32)

@@ -255,6 +255,12 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 _PAGE_SIZES = (16, 32, 64, 128, 256)
 
 
+@functools.lru_cache(maxsize=512)
+def _paged_ws_bytes(device_index: int, name: str, *args) -> int:
+    """A workspace size (a function of the sizes and the device's SM count)."""
+    return size_call(name, *args)
+
+
 def _paged_workspace(dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     """Zero-filled workspace of the paged-cache and token-score calls, one per
     (device, stream).  A stream that is being captured gets one per capture,
@@ -267,11 +273,12 @@ def _paged_workspace(dev: torch.device, stream: int, nbytes: int) -> torch.Tenso
         call("nkimoe_stream_capture_id", stream, ctypes.byref(cid))
         capture = cid.value
     key = (dev.index, stream, capture != 0)
+    held = _paged_ws.get(key)
+    if held is not None and held[0] == capture and held[1].numel() >= nbytes:
+        return held[1]
     with _ws_lock:
-        held = _paged_ws.get(key)
-        if held is None or held[0] != capture or held[1].numel() < nbytes:
-            held = (capture, torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=dev))
-            _paged_ws[key] = held
+        held = (capture, torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=dev))
+        _paged_ws[key] = held
         return held[1]
 
 
@@ -283,10 +290,10 @@ def read_paged_status(device=None) -> None:
     index = torch.cuda.current_device() if dev.index is None else dev.index
     torch.cuda.synchronize(index)
     with _ws_lock:
-        held = [(k[1], v[1]) for k, v in _paged_ws.items() if k[0] == index]
+        held = [v[1] for k, v in _paged_ws.items() if k[0] == index]
     bad = None
     with torch.cuda.device(index):
-        for _, ws in held:
+        for ws in held:
             try:
                 call("nkimoe_read_status", ws.data_ptr(), _raw_stream(index), None)
             except _lib.NKIMoEError as e:
@@ -295,23 +302,23 @@ def read_paged_status(device=None) -> None:
         raise bad
 
 
-def _same_device(dev: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, expected {dev}")
-
-
 def _on_its_device(fn):
     """Runs ``fn`` with its first argument's device as the current one (its
     kernels launch there, on that device's current stream)."""
     @functools.wraps(fn)
     def run(*args, **kw):
         t = args[0] if args else next(iter(kw.values()), None)
-        if isinstance(t, torch.Tensor) and t.is_cuda and t.device.index != torch._C._cuda_getDevice():
+        if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() != torch._C._cuda_getDevice():
             with torch.cuda.device(t.device):
                 return fn(*args, **kw)
         return fn(*args, **kw)
     return run
+
+
+def _same_device(index: int, **tensors) -> None:
+    for name, t in tensors.items():
+        if t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
 
 
 def _norm_weights(q_weight: torch.Tensor, k_weight: torch.Tensor):
@@ -322,28 +329,39 @@ def _norm_weights(q_weight: torch.Tensor, k_weight: torch.Tensor):
     return qw, kw, _DT[wdt]
 
 
+def _page_stride(c: torch.Tensor, name: str, n_kv_heads: int) -> int:
+    """Checks one pool and returns the elements between its pages."""
+    shape = c.shape
+    if not c.is_cuda or c.dtype != torch.bfloat16 or len(shape) != 4 or shape[1] != n_kv_heads or shape[3] != 128:
+        raise ValueError(f"{name} must be CUDA bf16 [pages, {n_kv_heads}, page_size, 128]")
+    if shape[2] not in _PAGE_SIZES:
+        raise ValueError(f"page size {shape[2]} (one of {_PAGE_SIZES})")
+    if shape[0] == 0:
+        raise ValueError(f"{name} has no pages")
+    page = n_kv_heads * shape[2] * 128
+    if c.is_contiguous():
+        return page
+    st = c.stride()
+    if st[3] != 1 or st[2] != 128 or (n_kv_heads > 1 and st[1] != 128 * shape[2]):
+        raise ValueError(f"{name}: the pages themselves must be contiguous")
+    return st[0] if shape[0] > 1 else page
+
+
 def _paged_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, n_kv_heads: int,
                  batch: int):
     """Checks one layer's pools and the page table of ``batch`` sequences and
     returns their C arguments."""
-    for name, c in (("k_pages", k_pages), ("v_pages", v_pages)):
-        shape, st = c.shape, c.stride()
-        if not c.is_cuda or c.dtype != torch.bfloat16 or len(shape) != 4 or shape[1] != n_kv_heads or shape[3] != 128:
-            raise ValueError(f"{name} must be CUDA bf16 [pages, {n_kv_heads}, page_size, 128]")
-        if shape[2] not in _PAGE_SIZES:
-            raise ValueError(f"page size {shape[2]} (one of {_PAGE_SIZES})")
-        if shape[0] == 0 or st[3] != 1 or st[2] != 128 or (shape[1] > 1 and st[1] != 128 * shape[2]):
-            raise ValueError(f"{name}: the pages themselves must be contiguous")
-    if v_pages.shape != k_pages.shape:
+    kst, vst = _page_stride(k_pages, "k_pages", n_kv_heads), _page_stride(v_pages, "v_pages", n_kv_heads)
+    shape = k_pages.shape
+    if v_pages.shape != shape:
         raise ValueError("k_pages and v_pages differ in shape")
-    if not page_table.is_cuda or page_table.dtype != torch.int32 or page_table.dim() != 2 \
-            or page_table.shape[0] < batch or page_table.shape[1] == 0 or page_table.stride(1) != 1:
-        raise ValueError(f"page_table must be CUDA int32 [>= {batch}, pages per sequence] with contiguous rows")
-    page = n_kv_heads * k_pages.shape[2] * 128
-    kst, vst = (c.stride(0) if c.shape[0] > 1 else page for c in (k_pages, v_pages))
-    tst = page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1]
-    return (k_pages.data_ptr(), v_pages.data_ptr(), kst, vst, k_pages.shape[0], k_pages.shape[2],
-            page_table.data_ptr(), tst, page_table.shape[1])
+    if not page_table.is_cuda or page_table.dtype != torch.int32 or page_table.dim() != 2:
+        raise ValueError("page_table must be CUDA int32 [sequences, pages per sequence]")
+    rows, width = page_table.shape
+    if rows < batch or width == 0 or (width > 1 and page_table.stride(1) != 1):
+        raise ValueError(f"page_table must have contiguous rows for {batch} sequences")
+    return (k_pages.data_ptr(), v_pages.data_ptr(), kst, vst, shape[0], shape[2], page_table.data_ptr(),
+            page_table.stride(0) if rows > 1 else width, width)
 
 
 def _lengths(cu_seqlens: torch.Tensor, kv_lens: torch.Tensor) -> int:
@@ -353,6 +371,14 @@ def _lengths(cu_seqlens: torch.Tensor, kv_lens: torch.Tensor) -> int:
     if cu_seqlens.shape[0] != kv_lens.shape[0] + 1:
         raise ValueError(f"cu_seqlens has {cu_seqlens.shape[0]} entries for {kv_lens.shape[0]} sequences")
     return kv_lens.shape[0]
+
+
+def _rows_out(out: torch.Tensor | None, shape: tuple, dev: torch.device) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    if out.dtype != torch.bfloat16 or out.shape != shape or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f"out must be a contiguous bf16 {list(shape)} tensor on {dev}")
+    return out
 
 
 @_on_its_device
@@ -380,12 +406,9 @@ def qk_norm_rope_store(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torc
     B = _lengths(cu_seqlens, kv_lens)
     qw, kw, wdt = _norm_weights(q_weight, k_weight)
     cache = _paged_cache(k_pages, v_pages, page_table, n_kv_heads, B)
-    _same_device(dev, q_weight=qw, k_weight=kw, cu_seqlens=cu_seqlens, kv_lens=kv_lens, k_pages=k_pages,
+    _same_device(dev.index, q_weight=qw, k_weight=kw, cu_seqlens=cu_seqlens, kv_lens=kv_lens, k_pages=k_pages,
                  v_pages=v_pages, page_table=page_table)
-    if out is None:
-        out = torch.empty(T, n_heads, 128, dtype=torch.bfloat16, device=dev)
-    elif out.dtype != torch.bfloat16 or out.shape != (T, n_heads, 128) or not out.is_contiguous() or out.device != dev:
-        raise ValueError(f"out must be a contiguous bf16 [{T}, {n_heads}, 128] tensor on {dev}")
+    out = _rows_out(out, (T, n_heads, 128), dev)
     s = _raw_stream(dev.index)
     ws = _paged_workspace(dev, s, 0)
     call("nkimoe_qk_norm_rope_store", qkv.data_ptr(), qw.data_ptr(), kw.data_ptr(), wdt,
@@ -425,14 +448,12 @@ def paged_decode_attention(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: 
         raise ValueError(f"positions has {n_pos} entries for {B} sequences")
     qw, kw, wdt = _norm_weights(q_weight, k_weight)
     cache = _paged_cache(k_pages, v_pages, page_table, n_kv_heads, B)
-    _same_device(dev, q_weight=qw, k_weight=kw, positions=positions, k_pages=k_pages, v_pages=v_pages,
+    _same_device(dev.index, q_weight=qw, k_weight=kw, positions=positions, k_pages=k_pages, v_pages=v_pages,
                  page_table=page_table)
-    if out is None:
-        out = torch.empty(B, n_heads * 128, dtype=torch.bfloat16, device=dev)
-    elif out.dtype != torch.bfloat16 or out.shape != (B, n_heads * 128) or not out.is_contiguous() or out.device != dev:
-        raise ValueError(f"out must be a contiguous bf16 [{B}, {n_heads * 128}] tensor on {dev}")
+    out = _rows_out(out, (B, n_heads * 128), dev)
     s = _raw_stream(dev.index)
-    nbytes = size_call("nkimoe_paged_decode_attention_workspace_bytes", B, n_heads, n_kv_heads, cache[8], cache[5])
+    nbytes = _paged_ws_bytes(dev.index, "nkimoe_paged_decode_attention_workspace_bytes", B, n_heads, n_kv_heads,
+                             cache[8], cache[5])
     ws = _paged_workspace(dev, s, nbytes)
     call("nkimoe_paged_decode_attention", qkv.data_ptr(), qw.data_ptr(), kw.data_ptr(), wdt,
              positions.data_ptr(), 0 if n_pos == 1 else 1, *cache, out.data_ptr(), B, n_heads, n_kv_heads, 128, theta,
@@ -466,13 +487,11 @@ def paged_prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     B = _lengths(cu_seqlens, kv_lens)
     nkv = k_pages.shape[1] if k_pages.dim() == 4 else 0
     cache = _paged_cache(k_pages, v_pages, page_table, nkv, B)
-    _same_device(dev, cu_seqlens=cu_seqlens, kv_lens=kv_lens, k_pages=k_pages, v_pages=v_pages, page_table=page_table)
-    if out is None:
-        out = torch.empty(T, nq * 128, dtype=torch.bfloat16, device=dev)
-    elif out.dtype != torch.bfloat16 or out.shape != (T, nq * 128) or not out.is_contiguous() or out.device != dev:
-        raise ValueError(f"out must be a contiguous bf16 [{T}, {nq * 128}] tensor on {dev}")
+    _same_device(dev.index, cu_seqlens=cu_seqlens, kv_lens=kv_lens, k_pages=k_pages, v_pages=v_pages, page_table=page_table)
+    out = _rows_out(out, (T, nq * 128), dev)
     s = _raw_stream(dev.index)
-    nbytes = size_call("nkimoe_paged_prefill_attention_workspace_bytes", T, B, nq, nkv, cache[8], cache[5])
+    nbytes = _paged_ws_bytes(dev.index, "nkimoe_paged_prefill_attention_workspace_bytes", T, B, nq, nkv, cache[8],
+                             cache[5])
     ws = _paged_workspace(dev, s, nbytes)
     call("nkimoe_paged_prefill_attention", q.data_ptr(), q.stride(0) if T > 1 else nq * 128, *cache,
          cu_seqlens.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), T, B, nq, nkv, 128,
@@ -541,15 +560,15 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0):
     if not 0 <= top_n <= min(32, V):
         raise ValueError(f"top_n {top_n} is not in [0, min(32, {V})]")
     dev = logits.device
-    _same_device(dev, tokens=tokens)
-    # one allocation for the two fp32 vectors, handed out as two tensors
-    lp, ent = torch.empty(2, T, dtype=torch.float32, device=dev)
+    _same_device(dev.index, tokens=tokens)
+    lp = torch.empty(T, dtype=torch.float32, device=dev)
+    ent = torch.empty(T, dtype=torch.float32, device=dev)
     top_lp = torch.empty(T, top_n, dtype=torch.float32, device=dev)
     top_ids = torch.empty(T, top_n, dtype=torch.int64, device=dev)
     if T == 0:
         return lp, ent, top_lp, top_ids
     s = _raw_stream(dev.index)
-    ws = _paged_workspace(dev, s, size_call("nkimoe_token_logprobs_workspace_bytes", T, V, top_n))
+    ws = _paged_workspace(dev, s, _paged_ws_bytes(dev.index, "nkimoe_token_logprobs_workspace_bytes", T, V, top_n))
     call("nkimoe_token_logprobs", logits.data_ptr(), _DT[logits.dtype], logits.stride(0) if T > 1 else V,
              tokens.data_ptr(), T, V, top_n, lp.data_ptr(), ent.data_ptr(), top_lp.data_ptr(), top_ids.data_ptr(),
              ws.data_ptr(), ws.numel(), s)

@@ -18,6 +18,13 @@ the whole MoE block (``nkimoe_moe_block``).  The dense projections (QKV, O,
 LM head) are plain cuBLAS GEMMs through torch and prefill attention is torch's
 scaled-dot-product attention; neither is part of the MoE hot path.
 
+Serving from a paged cache (:mod:`nki_moe_b200.paged`; sequences of their own
+lengths, shared prompts, windows): :meth:`Qwen3MoEStack.prefill_paged`,
+:meth:`~Qwen3MoEStack.decode_paged`, :meth:`~Qwen3MoEStack.generate_paged` and
+:meth:`~Qwen3MoEStack.score` run the library's own attention for prompts too
+(``nkimoe_qk_norm_rope_store``, ``nkimoe_paged_prefill_attention``,
+``nkimoe_paged_decode_attention``, ``nkimoe_token_logprobs``).
+
 Decode keeps every shape static (a KV cache of ``max_seq`` positions, the
 current position in a device tensor that the attention kernel reads), so one
 decode step over all layers is captured into a single CUDA graph.
@@ -33,6 +40,7 @@ import torch
 import torch.nn.functional as F
 
 from . import ops
+from .paged import PagedKVCache
 
 
 @dataclass
@@ -97,6 +105,7 @@ class Qwen3MoEStack:
         self._graph = None
         self._graph_batch = None
         self._graph_out = None
+        self._paged = None  # the captured paged decode step: its cache, batch, buffers and graph
         # the skinny linear kernel takes N % 16 == 0 and K % 32 == 0
         H, hd = cfg.hidden_size, cfg.head_dim
         nq, nkv = cfg.num_attention_heads, cfg.num_key_value_heads
@@ -349,6 +358,184 @@ class Qwen3MoEStack:
 
     def release_graph(self):
         self._graph = self._graph_out = None
+        self._paged = None
+
+    # ------------------------------------------------------------ paged cache
+    def paged_cache(self, num_pages: int, page_size: int = 64, max_seq: int | None = None, window: int = 0,
+                    sinks: int = 0) -> PagedKVCache:
+        """A paged cache of this stack's layers (``max_seq``: the longest
+        sequence, the stack's by default)."""
+        c = self.cfg
+        return PagedKVCache(c.num_hidden_layers, c.num_key_value_heads, num_pages, page_size, max_seq or self.max_seq,
+                            window, sinks, self.device)
+
+    def _prompt_hidden(self, cache: PagedKVCache, seqs, prompts) -> torch.Tensor:
+        """Runs the layers on new tokens of the sequences, packed, and returns
+        the final norm's rows ``[T, H]``."""
+        c = self.cfg
+        lens = [int(p.numel()) for p in prompts]
+        if len(prompts) != len(seqs) or not seqs or min(lens) == 0:
+            raise ValueError("one prompt, not empty, for each sequence")
+        if any(lyr.ep is not None for lyr in self.layers) and sum(lens) > self.max_batch * self.max_seq:
+            raise ValueError(f"{sum(lens)} tokens exceed the expert-parallel exchange "
+                             f"({self.max_batch} x {self.max_seq})")
+        cache.extend(seqs, lens)
+        cu = torch.zeros(len(seqs) + 1, dtype=torch.int32)
+        cu[1:] = torch.tensor(lens).cumsum(0)
+        cu = cu.to(self.device)
+        kv = torch.tensor([cache.length(q) for q in seqs], dtype=torch.int32).to(self.device)
+        table = cache.table(seqs).to(self.device)
+        ids = torch.cat([p.reshape(-1).to(self.device) for p in prompts])
+        h = F.embedding(ids, self.embed)
+
+        def attention(li, lyr, xn):
+            k, v = cache.layer(li)
+            q = ops.qk_norm_rope_store(F.linear(xn, lyr.qkv_w), lyr.q_norm, lyr.k_norm, cu, kv, k, v, table,
+                                       c.num_attention_heads, c.num_key_value_heads, c.rope_theta, c.rms_norm_eps)
+            return ops.paged_prefill_attention(q, k, v, table, cu, kv, window=cache.window, sinks=cache.sinks)
+
+        return self._layers(h, attention)
+
+    @torch.inference_mode()
+    def prefill_paged(self, cache: PagedKVCache, seqs, prompts) -> torch.Tensor:
+        """Appends ``prompts[i]`` (token ids, any lengths) to sequence
+        ``seqs[i]`` of the cache, which may hold the beginning already (a
+        prompt in chunks, or one that continues a fork).  Returns the logits
+        of each prompt's last token ``[len(seqs), V]``."""
+        hn = self._prompt_hidden(cache, seqs, prompts)
+        last = torch.tensor([int(p.numel()) for p in prompts]).cumsum(0) - 1
+        logits = F.linear(hn[last.to(self.device)], self.lm_head)
+        for q in seqs:
+            cache.trim(q)
+        return logits
+
+    def _paged_body(self, cache: PagedKVCache, tokens, positions, table) -> torch.Tensor:
+        c = self.cfg
+        B = tokens.shape[0]
+        linear = ops.skinny_linear if B <= 16 and self._skinny_ok else F.linear
+
+        def attention(li, lyr, xn):
+            k, v = cache.layer(li)
+            return ops.paged_decode_attention(linear(xn, lyr.qkv_w), lyr.q_norm, lyr.k_norm, positions, k, v, table,
+                                              c.num_attention_heads, c.num_key_value_heads, c.rope_theta,
+                                              c.rms_norm_eps, window=cache.window, sinks=cache.sinks)
+
+        hn = self._layers(F.embedding(tokens, self.embed), attention, linear, decode=True)
+        return linear(hn, self.lm_head)
+
+    @torch.inference_mode()
+    def decode_paged(self, cache: PagedKVCache, seqs, tokens: torch.Tensor, graph: bool = True) -> torch.Tensor:
+        """One decode step: ``tokens[i]`` appended to sequence ``seqs[i]``.
+        Returns logits ``[len(seqs), V]`` (a tensor of its own).  With
+        ``graph`` the step is captured once per cache and batch size; lengths
+        and pages are device data."""
+        B = len(seqs)
+        if tokens.numel() != B:
+            raise ValueError(f"{tokens.numel()} tokens for {B} sequences")
+        if any(lyr.ep is not None for lyr in self.layers) and B > self.max_batch:
+            raise ValueError(f"batch {B} exceeds the expert-parallel exchange ({self.max_batch})")
+        cache.extend(seqs, [1] * B)
+        positions = torch.tensor([cache.length(q) - 1 for q in seqs])
+        table = cache.table(seqs)
+        step = self._paged
+        if not graph:
+            out = self._paged_body(cache, tokens.reshape(-1).to(self.device), positions.to(self.device),
+                                   table.to(self.device))
+        else:
+            if step is None or step["cache"] is not cache or step["B"] != B:
+                step = {"cache": cache, "B": B,
+                        "tokens": torch.zeros(B, dtype=torch.int64, device=self.device),
+                        "positions": torch.zeros(B, dtype=torch.int64, device=self.device),
+                        "table": torch.zeros(B, cache.max_pages, dtype=torch.int32, device=self.device)}
+            step["tokens"].copy_(tokens.reshape(-1))
+            step["positions"].copy_(positions)
+            step["table"].copy_(table)
+            if "graph" not in step:
+                s = torch.cuda.Stream(device=self.device)
+                s.wait_stream(torch.cuda.current_stream(self.device))
+                # warm up on the capture stream; what this writes the replay writes again
+                with torch.cuda.stream(s):
+                    self._paged_body(cache, step["tokens"], step["positions"], step["table"])
+                torch.cuda.current_stream(self.device).wait_stream(s)
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=s):
+                    step["out"] = self._paged_body(cache, step["tokens"], step["positions"], step["table"])
+                step["graph"] = g
+                self._paged = step
+            step["graph"].replay()
+            out = step["out"].clone()
+        for q in seqs:
+            cache.trim(q)
+        return out
+
+    @torch.inference_mode()
+    def generate_paged(self, prompts, max_new_tokens: int, samples: int = 1, temperature: float = 0.0,
+                       top_logprobs: int | None = None, page_size: int = 64, window: int = 0, sinks: int = 0,
+                       generator: torch.Generator | None = None, cache: PagedKVCache | None = None,
+                       graph: bool = True):
+        """Generation for prompts of any lengths, ``samples`` continuations of
+        each from one prefill (the prompt's pages are shared).
+
+        Greedy with ``temperature`` 0, else sampled (``generator`` on the
+        stack's device).  With ``window`` the model attends to the last
+        ``window`` tokens and the first ``sinks`` ones.  Returns ``(tokens
+        [len(prompts), samples, max_new_tokens], scores)``; ``scores`` is None
+        or, with ``top_logprobs`` alternatives, a dict of ``logprob`` and
+        ``entropy`` ``[.., max_new_tokens]`` and ``top_logprobs``/``top_ids``
+        ``[.., max_new_tokens, top_logprobs]``."""
+        if samples < 1 or max_new_tokens < 1:
+            raise ValueError("samples and max_new_tokens must be positive")
+        n, ends = len(prompts), [int(p.numel()) + max_new_tokens for p in prompts]
+        if cache is None:
+            pages = sum(-(-e // page_size) * samples for e in ends)
+            cache = self.paged_cache(pages, page_size, max(ends), window, sinks)
+        seqs = [cache.add() for _ in prompts]
+        try:
+            logits = self.prefill_paged(cache, seqs, prompts)
+            seqs = [q for first in seqs for q in [first] + [cache.fork(first) for _ in range(samples - 1)]]
+            logits = logits.repeat_interleave(samples, 0)
+            out, scores = [], []
+            for i in range(max_new_tokens):
+                if temperature > 0:
+                    # the largest of logits + Gumbel noise is a sample of the softmax
+                    noise = torch.empty_like(logits, dtype=torch.float32).exponential_(generator=generator).log()
+                    tok = (logits.float() / temperature - noise).argmax(-1)
+                else:
+                    tok = logits.argmax(-1)
+                out.append(tok)
+                if top_logprobs is not None:
+                    scores.append(ops.token_logprobs(logits, tok, top_logprobs))
+                if i + 1 < max_new_tokens:
+                    logits = self.decode_paged(cache, seqs, tok, graph)
+        finally:
+            for q in seqs:
+                if q in cache:
+                    cache.free(q)
+        tokens = torch.stack(out, 1).view(n, samples, max_new_tokens)
+        if top_logprobs is None:
+            return tokens, None
+        lp, ent, tlp, tid = (torch.stack(x, 1) for x in zip(*scores))
+        shape = (n, samples, max_new_tokens)
+        return tokens, {"logprob": lp.view(shape), "entropy": ent.view(shape), "top_logprobs": tlp.view(*shape, -1),
+                        "top_ids": tid.view(*shape, -1)}
+
+    @torch.inference_mode()
+    def score(self, prompts, top_n: int = 0, page_size: int = 64, window: int = 0, sinks: int = 0,
+              chunk: int = 2048):
+        """Scores of given texts: for each prompt a tuple ``(logprob [n - 1],
+        entropy [n - 1], top_logprobs [n - 1, top_n], top_ids)`` of its tokens
+        from the second on, each under what comes before it.  The logits are
+        formed ``chunk`` rows at a time."""
+        lens = [int(p.numel()) for p in prompts]
+        cache = self.paged_cache(sum(-(-n // page_size) for n in lens), page_size, max(lens), window, sinks)
+        hn = self._prompt_hidden(cache, [cache.add() for _ in prompts], prompts)
+        # a prompt's last row predicts nothing that is given
+        given = torch.cat([torch.cat([p.reshape(-1)[1:].to(self.device), p.new_full((1,), -1).to(self.device)])
+                           for p in prompts]).to(torch.int64)
+        parts = [ops.token_logprobs(F.linear(hn[r:r + chunk], self.lm_head), given[r:r + chunk], top_n)
+                 for r in range(0, hn.shape[0], chunk)]
+        whole = [torch.cat(x) for x in zip(*parts)]
+        return [tuple(t[:n - 1] for t in rows) for n, rows in zip(lens, zip(*(w.split(lens) for w in whole)))]
 
     # ------------------------------------------------------------ generate
     @torch.inference_mode()

@@ -1,0 +1,163 @@
+"""The decoder stack on its paged cache, against HF ``Qwen3MoeForCausalLM``
+(bars: see ``test_gpu_stack.py``): prompts of different lengths, chunks,
+forks, windows, graph and eager steps, scores."""
+
+import pytest
+import torch
+
+from tests.test_gpu_stack import NORM_BAR, QUANTILE, _check, tiny_hf
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+
+
+@pytest.fixture(scope="module")
+def pair():
+    from nki_moe_b200.qwen_stack import Qwen3MoEStack
+
+    hf = tiny_hf()
+    return hf, Qwen3MoEStack.from_hf(hf, max_batch=4, max_seq=256)
+
+
+def ids(n, seed):
+    return torch.randint(0, 1024, (n,), generator=torch.Generator().manual_seed(seed))
+
+
+def hf_logits(hf, tokens, window=0, sinks=0):
+    """All logits of one text; with a window through an explicit mask."""
+    mask = None
+    if window:
+        n = len(tokens)
+        p, s = torch.arange(n)[:, None], torch.arange(n)
+        see = (s <= p) & ((s > p - window) | (s < sinks))
+        mask = torch.zeros(1, 1, n, n).masked_fill(~see, torch.finfo(torch.float32).min)
+    with torch.no_grad():
+        return hf(tokens[None], attention_mask=mask).logits[0]
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_prompts_of_different_lengths_then_steps(pair, graph):
+    hf, st = pair
+    texts = [ids(n + 6, n) for n in (1, 17, 40, 100, 130)]
+    cache = st.paged_cache(40, page_size=16)
+    seqs = [cache.add() for _ in texts]
+    got = [st.prefill_paged(cache, seqs, [t[:-6] for t in texts])]
+    for i in range(6, 0, -1):
+        step = torch.stack([t[-i] for t in texts]).cuda()
+        got.append(st.decode_paged(cache, seqs, step, graph=graph))
+    got = torch.stack(got, 1)
+    ref = torch.stack([hf_logits(hf, t)[-7:] for t in texts])
+    _check(got.reshape(-1, 1024), ref.reshape(-1, 1024))
+    st.release_graph()
+
+
+def test_a_prompt_in_chunks_equals_the_whole(pair):
+    hf, st = pair
+    text = ids(150, 3)
+    cache = st.paged_cache(20, page_size=32)
+    seq = cache.add()
+    got = [st.prefill_paged(cache, [seq], [text[a:b]])[0] for a, b in ((0, 1), (1, 33), (33, 100), (100, 150))]
+    ref = hf_logits(hf, text)
+    _check(torch.stack(got), ref[[0, 32, 99, 149]])
+
+
+@pytest.mark.parametrize("window,sinks", [(40, 4), (16, 0)])
+def test_window_and_first_tokens(pair, window, sinks):
+    hf, st = pair
+    texts = [ids(n, n) for n in (150, 90)]
+    cache = st.paged_cache(30, page_size=16, window=window, sinks=sinks)
+    seqs = [cache.add() for _ in texts]
+    got = [st.prefill_paged(cache, seqs, [t[:-8] for t in texts])]
+    held = 30 - cache.free_pages
+    assert held <= 2 * (window // 16 + 3)  # the rest was given back
+    for i in range(8, 0, -1):
+        got.append(st.decode_paged(cache, seqs, torch.stack([t[-i] for t in texts])))
+    got = torch.stack(got, 1)
+    ref = torch.stack([hf_logits(hf, t, window, sinks)[-9:] for t in texts])
+    _check(got.reshape(-1, 1024), ref.reshape(-1, 1024))
+    st.release_graph()
+
+
+def test_forks_go_their_own_ways_and_compaction_keeps_them(pair):
+    hf, st = pair
+    prompt, ways = ids(37, 5), [ids(6, 50 + i) for i in range(3)]
+    cache = st.paged_cache(40, page_size=16)
+    hole = cache.add()
+    cache.extend([hole], [64])
+    first = cache.add()
+    st.prefill_paged(cache, [first], [prompt])
+    seqs = [first, cache.fork(first), cache.fork(first)]
+    assert cache.free_pages == 40 - 4 - 3
+    got = []
+    for i in range(6):
+        got.append(st.decode_paged(cache, seqs, torch.stack([w[i] for w in ways])))
+        if i == 2:
+            cache.free(hole)
+            assert cache.compact()
+    ref = torch.stack([hf_logits(hf, torch.cat([prompt, w]))[-6:] for w in ways])
+    _check(torch.stack(got, 1).reshape(-1, 1024), ref.reshape(-1, 1024))
+    st.release_graph()
+
+
+def test_generate_samples_and_scores(pair):
+    _, st = pair
+    prompts = [ids(20, 6), ids(51, 7)]
+    tok, sc = st.generate_paged(prompts, 8, samples=2, top_logprobs=5, page_size=16)
+    assert tok.shape == (2, 2, 8) and torch.equal(tok[:, 0], tok[:, 1])  # greedy: the samples are alike
+    assert torch.equal(sc["top_ids"][..., 0], tok) and torch.equal(sc["top_logprobs"][..., 0], sc["logprob"])
+    assert sc["top_ids"].shape == (2, 2, 8, 5) and (sc["entropy"] >= 0).all()
+    eager, none = st.generate_paged(prompts, 8, page_size=16, graph=False)
+    assert none is None and torch.equal(eager[:, 0], tok[:, 0])
+
+    def sampled(seed):
+        return st.generate_paged(prompts, 8, samples=3, temperature=1.0,
+                                 generator=torch.Generator(device="cuda").manual_seed(seed))[0]
+
+    a, b, c = sampled(1), sampled(1), sampled(2)
+    assert torch.equal(a, b) and not torch.equal(a, c) and not torch.equal(a[:, 0], a[:, 1])
+    cache = st.paged_cache(8, page_size=16)
+    st.generate_paged([prompts[0]], 4, samples=2, cache=cache)
+    assert cache.free_pages == 8
+    with pytest.raises(RuntimeError):
+        st.generate_paged(prompts * 2, 4, samples=2, cache=cache)
+    assert cache.free_pages == 8
+    st.release_graph()
+
+
+def test_score_of_given_texts(pair):
+    hf, st = pair
+    texts = [ids(n, 60 + n) for n in (1, 2, 70, 120)]
+    got = st.score(texts, top_n=3, page_size=16, chunk=50)
+    for text, (lp, ent, tlp, tid) in zip(texts, got):
+        n = len(text) - 1
+        assert lp.shape == ent.shape == (n,) and tlp.shape == tid.shape == (n, 3)
+        if not n:
+            continue
+        logits = hf_logits(hf, text)[:-1]
+        ref = torch.log_softmax(logits.double(), -1).gather(-1, text[1:, None])[:, 0]
+        # logits are within NORM_BAR of the largest at 95% of the positions, a
+        # log probability within twice that
+        bar = 2 * NORM_BAR * logits.abs().amax(-1)
+        assert ((lp.cpu() - ref).abs() <= bar).float().mean() >= QUANTILE or n < 20
+
+
+def test_refusals(pair):
+    _, st = pair
+    cache = st.paged_cache(4, page_size=16)
+    a, b = cache.add(), cache.add()
+    for seqs, prompts in (([a], []), ([], []), ([a], [ids(0, 1)]), ([a, a], [ids(3, 1)] * 2), ([77], [ids(3, 1)])):
+        with pytest.raises(ValueError):
+            st.prefill_paged(cache, seqs, prompts)
+    st.prefill_paged(cache, [a, b], [ids(5, 1), ids(9, 2)])
+    with pytest.raises(ValueError):
+        st.decode_paged(cache, [a, b], torch.tensor([1]))
+    with pytest.raises(ValueError):
+        st.decode_paged(cache, [a, a], torch.tensor([1, 2]))
+    with pytest.raises(RuntimeError):
+        st.prefill_paged(cache, [a], [ids(60, 3)])
+    assert cache.length(a) == 5 and cache.free_pages == 2

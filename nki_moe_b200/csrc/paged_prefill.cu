@@ -341,132 +341,119 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   // 384 x 168 registers at launch = 128 x 88 + 256 x 208
   if (warp == 0) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    // ---------------------------------------------------------------- units and loads (one thread)
-    if (lane == 0) {
-      const int page_rows = min(1 << p.c.page_shift, kPfBlock);  // rows per box
-      const uint32_t q_bytes = 2u * p.grp * p.tpt * 128u;        // both halves of one tile's box
-      int stage = 0, u = 0;
-      uint32_t phase = 0, issued = 0, last_phase = 0;
-      bool ok = true, q_issued = false;
-      const PfList list = *p.list;
-      // a run of the list of key blocks (pair, kv head, block), or whole pairs
-      const int run_lo = min(list.total, static_cast<int>(blockIdx.x) * list.share);
-      const int run_hi = min(list.total, run_lo + list.share);
-      int at = run_lo, pair = 0;
-      if (list.share) {
-        p.splits[blockIdx.x].parts = 0;
-        for (int hi = list.pairs; hi - pair > 1;) {
-          const int mid = (pair + hi) >> 1;
-          if (p.offs[mid] * p.c.nkv <= at) pair = mid; else hi = mid;
-        }
+    // ---------------------------------------------------------------- units and loads
+    // Lane (v, h, g) loads half h of page g of a K (v = 0) or V block: one
+    // thread's bookkeeping for all of them took 2000 cycles per block.
+    const int v_lane = lane >> 4, h_lane = (lane >> 3) & 1, g_lane = lane & 7;
+    const int page_rows = min(1 << p.c.page_shift, kPfBlock);  // rows per box
+    const bool loads = g_lane * page_rows < kPfBlock;
+    const void* const tm = v_lane ? static_cast<const void*>(&tmap_v) : static_cast<const void*>(&tmap_k);
+    const int box_at = h_lane * static_cast<int>(kPfBlockHalf) + g_lane * page_rows * 128;
+    const uint32_t q_bytes = 2u * p.grp * p.tpt * 128u;  // both halves of one tile's box
+    auto wait = [&](uint64_t* bar, uint32_t ph) {
+      const bool got = mbar_wait(bar, ph, &ctl.abort_flag, p.status);
+      return __all_sync(0xffffffffu, got);
+    };
+    int stage = 0;
+    uint32_t phase = 0, issued = 0, last_phase = 0;
+    bool ok = true, q_issued = false;
+    const PfList list = *p.list;
+    // a run of the list of key blocks (pair, kv head, block), or whole pairs
+    const int run_lo = min(list.total, static_cast<int>(blockIdx.x) * list.share);
+    const int run_hi = min(list.total, run_lo + list.share);
+    int at = run_lo, pair = 0, unit = blockIdx.x;
+    if (list.share) {
+      if (lane == 0) p.splits[blockIdx.x].parts = 0;
+      for (int hi = list.pairs; hi - pair > 1;) {
+        const int mid = (pair + hi) >> 1;
+        if (p.offs[mid] * p.c.nkv <= at) pair = mid; else hi = mid;
       }
-      for (;; ++u) {
-        const int us = u & 1;
-        if (!mbar_wait(&ctl.u_empty[us], ((u >> 1) & 1) ^ 1u, &ctl.abort_flag, p.status)) {
-          ok = false;
-          break;
+    }
+    for (int u = 0; ok; ++u) {
+      const int us = u & 1;
+      if (!wait(&ctl.u_empty[us], ((u >> 1) & 1) ^ 1u)) { ok = false; break; }
+      PfWork w{};
+      if (list.share == 0) {
+        if (unit < list.pairs * p.c.nkv) {
+          static_cast<PfUnit&>(w) = p.units[unit / p.c.nkv];
+          w.j = unit % p.c.nkv;
+          // the one after it, long before it is needed
+          if (lane == 0) unit = atomicAdd(&p.list->next, 1) + gridDim.x;
         }
-        PfWork w{};
-        Blocks bl{};
-        if (list.share == 0) {
-          const int unit = u == 0 ? blockIdx.x : atomicAdd(&p.list->next, 1) + gridDim.x;
-          if (unit < list.pairs * p.c.nkv) {
-            static_cast<PfUnit&>(w) = p.units[unit / p.c.nkv];
-            w.j = unit % p.c.nkv;
-          }
-        } else if (at < run_hi) {
-          static_cast<PfUnit&>(w) = p.units[pair];
-          const int base = p.offs[pair] * p.c.nkv, n = w.hi;
-          w.j = (at - base) / n;
-          const int item = base + w.j * n;  // the list's first block of (pair, kv head)
-          w.lo = at - item;
-          w.hi = min(n, run_hi - item);
-          const int first = item / list.share, parts = (item + n - 1) / list.share - first + 1;
-          if (parts > 1) w.slot = 2 * static_cast<int>(blockIdx.x) + (item < run_lo ? 0 : 1);
-          if (parts > 1 && item >= run_lo) p.splits[blockIdx.x] = PfSplit{pair, w.j, parts, 0};
-          at = item + w.hi;
-          if (w.hi == n && w.j == p.c.nkv - 1) ++pair;
-        }
-        if (w.tokens) bl = blocks_of(w.pos0, w.pos0 + w.tokens - 1, p.window, p.sinks);
+      } else if (at < run_hi) {
+        static_cast<PfUnit&>(w) = p.units[pair];
+        const int base = p.offs[pair] * p.c.nkv, n = w.hi;
+        w.j = (at - base) / n;
+        const int item = base + w.j * n;  // the list's first block of (pair, kv head)
+        w.lo = at - item;
+        w.hi = min(n, run_hi - item);
+        const int first = item / list.share, parts = (item + n - 1) / list.share - first + 1;
+        if (parts > 1) w.slot = 2 * static_cast<int>(blockIdx.x) + (item < run_lo ? 0 : 1);
+        if (parts > 1 && item >= run_lo && lane == 0) p.splits[blockIdx.x] = PfSplit{pair, w.j, parts, 0};
+        at = item + w.hi;
+        if (w.hi == n && w.j == p.c.nkv - 1) ++pair;
+      }
+      if (lane == 0) {
         ctl.work[us] = w;
         mbar_arrive(&ctl.u_full[us]);
-        if (w.tokens == 0) break;
-        const bool two = w.tokens > p.tpt;
-        // positions that some query of the pair sees; a page outside is read as zeros
-        const int last = w.pos0 + w.tokens - 1;
-        const int start = p.window && w.pos0 >= p.window ? w.pos0 - p.window + 1 : 0;
-        const int* table = p.c.table + w.b * p.c.table_stride;
-        int pages[8];
-        auto look_up = [&](int i) {
-          const int k0 = bl.at(i) * kPfBlock;
+      }
+      if (w.tokens == 0) break;
+      const Blocks bl = blocks_of(w.pos0, w.pos0 + w.tokens - 1, p.window, p.sinks);
+      // positions that some query of the pair sees; a page outside is read as zeros
+      const int last = w.pos0 + w.tokens - 1;
+      const int start = p.window && w.pos0 >= p.window ? w.pos0 - p.window + 1 : 0;
+      const int* table = p.c.table + w.b * p.c.table_stride;
+      auto look_up = [&](int i) {
+        const int s0 = bl.at(i) * kPfBlock + g_lane * page_rows;
+        const bool need = loads && s0 <= last && (s0 + page_rows > start || s0 < p.sinks);
+        return need ? table[s0 >> p.c.page_shift] : -2;
+      };
+      int next = look_up(w.lo);
+      for (int i = w.lo; ok && i < w.hi; ++i) {
+        const bool held = next >= 0 && next < p.c.num_pages;
+        if (!held && next != -2) atomicOr(p.status, kDevErrBadIndex);
+        const int page = held ? next : p.c.num_pages;  // past the last page: the load fills zeros
+        const int in_page = (bl.at(i) * kPfBlock + g_lane * page_rows) & ((1 << p.c.page_shift) - 1);
+        if (i + 1 < w.hi) next = look_up(i + 1);  // in flight while this block waits for its stages
 #pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            const int s0 = k0 + g * page_rows;
-            pages[g] = -2;  // not needed
-            if (g * page_rows < kPfBlock && s0 <= last && (s0 + page_rows > start || s0 < p.sinks))
-              pages[g] = table[s0 >> p.c.page_shift];
-          }
-        };
-        auto load = [&](int i, bool is_v, const int (&pg)[8]) {
-          if (!mbar_wait(&ctl.kv_empty[stage], phase ^ 1u, &ctl.abort_flag, p.status)) return false;
-          const int k0 = bl.at(i) * kPfBlock;
-          uint8_t* dst = ring + stage * kPfBlockBytes;
-          mbar_arrive_expect_tx(&ctl.kv_full[stage], kPfBlockBytes);
-          const void* tm = is_v ? static_cast<const void*>(&tmap_v) : static_cast<const void*>(&tmap_k);
-#pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            if (g * page_rows < kPfBlock) {
-              const int in_page = (k0 + g * page_rows) & ((1 << p.c.page_shift) - 1);
-              tma_load_4d(dst + g * page_rows * 128, tm, &ctl.kv_full[stage], 0, in_page, w.j, pg[g]);
-              tma_load_4d(dst + kPfBlockHalf + g * page_rows * 128, tm, &ctl.kv_full[stage], 64, in_page, w.j, pg[g]);
-            }
-          }
+        for (int v = 0; v < 2; ++v) {
+          if (!wait(&ctl.kv_empty[stage], phase ^ 1u)) { ok = false; break; }
+          if (lane == 0) mbar_arrive_expect_tx(&ctl.kv_full[stage], kPfBlockBytes);
+          __syncwarp();
+          if (loads && v_lane == v)
+            tma_load_4d(ring + stage * kPfBlockBytes + box_at, tm, &ctl.kv_full[stage], h_lane * 64, in_page, w.j, page);
           issued |= 1u << stage;
           last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
           if (++stage == kPfRing) {
             stage = 0;
             phase ^= 1u;
           }
-          return true;
-        };
-        look_up(w.lo);
-        for (int i = w.lo; ok && i < w.hi; ++i) {
-          int pg[8];
-#pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            const bool held = pages[g] >= 0 && pages[g] < p.c.num_pages;
-            if (!held && pages[g] != -2) atomicOr(p.status, kDevErrBadIndex);
-            pg[g] = held ? pages[g] : p.c.num_pages;  // past the last page: the load fills zeros
-          }
-          if (i + 1 < w.hi) look_up(i + 1);  // in flight while this block waits for its stages
-          ok = load(i, false, pg) && load(i, true, pg);
-          // the queries after the unit's first block, which goes out while the
-          // unit before still reads its own
-          if (ok && i == w.lo) {
-            ok = mbar_wait(&ctl.q_empty, (u & 1) ^ 1u, &ctl.abort_flag, p.status);
-            if (!ok) break;
-            mbar_arrive_expect_tx(&ctl.q_full, two ? 2 * q_bytes : q_bytes);
-            for (int t = 0; t < (two ? 2 : 1); ++t)
-              for (int h = 0; h < 2; ++h)
-                tma_load_3d(sq + t * kPfTileBytes + h * kPfTileHalf, &tmap_q, &ctl.q_full, h * 64, w.j * p.grp,
-                            w.row0 + t * p.tpt);
-            q_issued = true;
+        }
+        // the queries after the unit's first block, which goes out while the
+        // unit before still reads its own
+        if (ok && i == w.lo) {
+          if (!wait(&ctl.q_empty, (u & 1) ^ 1u)) { ok = false; break; }
+          const int tiles = w.tokens > p.tpt ? 2 : 1;
+          if (lane == 0) mbar_arrive_expect_tx(&ctl.q_full, tiles * q_bytes);
+          __syncwarp();
+          if (lane < 2 * tiles)
+            tma_load_3d(sq + (lane >> 1) * kPfTileBytes + (lane & 1) * kPfTileHalf, &tmap_q, &ctl.q_full, (lane & 1) * 64,
+                        w.j * p.grp, w.row0 + (lane >> 1) * p.tpt);
+          q_issued = true;
+        }
+      }
+      unit = __shfl_sync(0xffffffffu, unit, 0);
+    }
+    if (!ok && lane == 0) {  // let the copies in flight land before the CTA exits
+      for (int s = 0; s < kPfRing; ++s)
+        if ((issued >> s) & 1u) {
+          const long long t0 = clock64();
+          while (!mbar_try_wait(&ctl.kv_full[s], (last_phase >> s) & 1u) && clock64() - t0 < kWaitBudgetCycles / 8) {
           }
         }
-        if (!ok) break;
-      }
-      if (!ok) {  // let the copies in flight land before the CTA exits
-        for (int s = 0; s < kPfRing; ++s)
-          if ((issued >> s) & 1u) {
-            const long long t0 = clock64();
-            while (!mbar_try_wait(&ctl.kv_full[s], (last_phase >> s) & 1u) && clock64() - t0 < kWaitBudgetCycles / 8) {
-            }
-          }
-        if (q_issued) {
-          // the last unit whose Q was issued: u itself, or the one before it
-          const long long t0 = clock64();
-          while (clock64() - t0 < kWaitBudgetCycles / 64) {
-          }
+      if (q_issued) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < kWaitBudgetCycles / 64) {
         }
       }
     }

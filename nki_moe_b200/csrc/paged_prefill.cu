@@ -53,8 +53,8 @@ constexpr uint32_t kPfTileHalf = kPfTileBytes / 2;           // one 64-column ha
 constexpr uint32_t kPfBlockBytes = kPfBlock * kHeadDim * 2;  // 32 KB: a K block or a V block
 constexpr uint32_t kPfBlockHalf = kPfBlockBytes / 2;
 constexpr size_t kPfSmem = 1024 + 2 * kPfTileBytes + kPfRing * kPfBlockBytes;
-// A part of a cut pair, per tile: o column by column [128][128 rows], then
-// the rows' m, then their l (a warp's rows are neighbours: coalesced)
+// A part of a cut pair, per tile: o four columns at a time [32][128 rows][4],
+// then the rows' m, then their l (a warp's rows are neighbours: coalesced)
 constexpr int kPfPartTile = (kHeadDim + 2) * kPfRows;
 constexpr int kPfMinBlocks = 4;                // key blocks of a part at least
 constexpr float kPfLog2e = 1.4426950408889634f;
@@ -668,7 +668,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
       const long long out_at =
           mine ? ((static_cast<long long>(w.row0) + t * p.tpt + token) * p.nq + w.j * p.grp + head) * kHeadDim : -1;
-      float* part = w.slot >= 0 ? p.part + (static_cast<long long>(w.slot) * 2 + t) * kPfPartTile + row : nullptr;
+      float* part = w.slot >= 0 ? p.part + (static_cast<long long>(w.slot) * 2 + t) * kPfPartTile : nullptr;
       // where this lane stores: row 8 k + lane / 4, columns 8 (lane % 4) of each 32
       __nv_bfloat16* to_row[4];
 #pragma unroll
@@ -684,7 +684,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         tmem_ld_wait();
         if (part) {
 #pragma unroll
-          for (int x = 0; x < 32; ++x) __stcg(part + (c * 32 + x) * kPfRows, __uint_as_float(o[x]));
+          for (int x = 0; x < 32; x += 4)
+            __stcg(reinterpret_cast<uint4*>(part) + (c * 8 + x / 4) * kPfRows + row,
+                   make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]));
         } else {
           // through shared memory: eight rows of 64 bytes per store instead of
           // 32 rows of 16
@@ -704,8 +706,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         }
       }
       if (part) {
-        __stcg(part + kHeadDim * kPfRows, m);
-        __stcg(part + (kHeadDim + 1) * kPfRows, l);
+        __stcg(part + kHeadDim * kPfRows + row, m);
+        __stcg(part + (kHeadDim + 1) * kPfRows + row, l);
       }
       tcgen05_fence_before();  // the next unit's MMAs follow this thread's next arrival
     }
@@ -733,19 +735,27 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const __grid_co
   if (token >= p.tpt || tile * p.tpt + token >= un.tokens) return;
   auto part_of = [&](int s) {
     const int slot = 2 * (cta + s) + (s == 0);
-    return p.part + (static_cast<long long>(slot) * 2 + tile) * kPfPartTile + row;
+    return p.part + (static_cast<long long>(slot) * 2 + tile) * kPfPartTile;
   };
   float m = -INFINITY;
-  for (int s = 0; s < sp.parts; ++s) m = fmaxf(m, __ldcg(part_of(s) + kHeadDim * kPfRows));
+  for (int s = 0; s < sp.parts; ++s) m = fmaxf(m, __ldcg(part_of(s) + kHeadDim * kPfRows + row));
   float l = 0.f, o[16];
 #pragma unroll
   for (int x = 0; x < 16; ++x) o[x] = 0.f;
   for (int s = 0; s < sp.parts; ++s) {
     const float* from = part_of(s);
-    const float f = m == -INFINITY ? 0.f : exp2f(__ldcg(from + kHeadDim * kPfRows) - m);
-    l = fmaf(f, __ldcg(from + (kHeadDim + 1) * kPfRows), l);
+    float4 v[4];
 #pragma unroll
-    for (int x = 0; x < 16; ++x) o[x] = fmaf(f, __ldcg(from + (col + x) * kPfRows), o[x]);
+    for (int x = 0; x < 4; ++x) v[x] = __ldcg(reinterpret_cast<const float4*>(from) + (col / 4 + x) * kPfRows + row);
+    const float f = m == -INFINITY ? 0.f : exp2f(__ldcg(from + kHeadDim * kPfRows + row) - m);
+    l = fmaf(f, __ldcg(from + (kHeadDim + 1) * kPfRows + row), l);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      o[4 * x] = fmaf(f, v[x].x, o[4 * x]);
+      o[4 * x + 1] = fmaf(f, v[x].y, o[4 * x + 1]);
+      o[4 * x + 2] = fmaf(f, v[x].z, o[4 * x + 2]);
+      o[4 * x + 3] = fmaf(f, v[x].w, o[4 * x + 3]);
+    }
   }
   const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
   __nv_bfloat16* dst =

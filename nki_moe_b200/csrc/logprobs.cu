@@ -347,7 +347,11 @@ __device__ __forceinline__ void warp_top(TopShared& sh, WarpTop& best, const uin
 // 16 KB held in registers, the next chunk in flight; the last CTA of a row
 // joins the splits' parts.
 //
-// Bound by HBM over many rows (the logits read once).
+// Bound by HBM over many rows (the logits read once), by issue next to it:
+// measured 2000 rows of 151936 bf16 with 5 alternatives 139 us = 4.36 TB/s =
+// 0.67 of the measured copy; 8 rows with 20 alternatives 14.7 us (one chunk per
+// CTA, then the join).  With the CTA's best tokens kept in common, a barrier per
+// chunk, 2000 rows took 500 us.
 template <typename T, bool kTop>
 __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LpParams p) {
   __shared__ TopShared sh;

@@ -24,6 +24,8 @@ struct CopyParams {
 };
 
 // CTA (piece, plane, pair).  Bound by HBM: each page read once, written once.
+// Measured: 300 pages of 64 KB in 48 planes 287 us = 6.6 TB/s = the measured
+// copy; 8 pages of 16 KB in 96 planes 4.6 us.
 template <int N>
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyParams<N> p) {
   pdl_launch_dependents();

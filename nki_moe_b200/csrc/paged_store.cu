@@ -49,7 +49,9 @@ __device__ __forceinline__ int sequence_of(const int* cu, int B, int t, int lane
 // but the norm weights in shared memory.  Its first heads' loads go out before
 // the row's position is known, so the two latencies overlap.
 //
-// Bound by HBM: (nq + 2 nkv) * 256 bytes read and as many written per row.
+// Bound by HBM and by issue: (nq + 2 nkv) * 256 bytes read and as many written
+// per row.  Measured: 8192 rows of 32 + 2 * 4 heads 36 us = 4.65 TB/s = 0.71 of
+// the measured copy; 15 rows 3.6 us.
 template <int kWarps>
 __global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_store_kernel(const __grid_constant__ StoreParams p) {
   constexpr int D = kHeadDim;

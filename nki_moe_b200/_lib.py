@@ -137,7 +137,7 @@ def load() -> ctypes.CDLL:
 
 
 def call(name: str, *args) -> int:
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != OK:
         msg = lib.nkimoe_last_error().decode(errors="replace")

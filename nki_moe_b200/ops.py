@@ -315,18 +315,20 @@ def _on_its_device(fn):
     return run
 
 
-def _same_device(index: int, **tensors) -> None:
-    for name, t in tensors.items():
+def _same_device(index: int, names: str, *tensors: torch.Tensor) -> None:
+    for i, t in enumerate(tensors):
         if t.get_device() != index:
-            raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
+            raise ValueError(f"{names.split()[i]} is on {t.device}, expected cuda:{index}")
 
 
 def _norm_weights(q_weight: torch.Tensor, k_weight: torch.Tensor):
-    wdt = torch.float32 if q_weight.dtype == torch.float32 else torch.bfloat16
-    qw, kw = _contig(_cuda(q_weight, "q_weight"), wdt), _contig(_cuda(k_weight, "k_weight"), wdt)
-    if qw.numel() != 128 or kw.numel() != 128:
+    wdt = q_weight.dtype
+    if wdt != torch.bfloat16 or k_weight.dtype != wdt or not q_weight.is_contiguous() or not k_weight.is_contiguous():
+        wdt = torch.float32 if wdt == torch.float32 else torch.bfloat16
+        q_weight, k_weight = _contig(_cuda(q_weight, "q_weight"), wdt), _contig(_cuda(k_weight, "k_weight"), wdt)
+    if q_weight.numel() != 128 or k_weight.numel() != 128:
         raise ValueError("q_weight and k_weight must have 128 elements")
-    return qw, kw, _DT[wdt]
+    return q_weight, k_weight, _DT[wdt]
 
 
 def _page_stride(c: torch.Tensor, name: str, n_kv_heads: int) -> int:
@@ -351,11 +353,16 @@ def _paged_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch
                  batch: int):
     """Checks one layer's pools and the page table of ``batch`` sequences and
     returns their C arguments."""
-    kst, vst = _page_stride(k_pages, "k_pages", n_kv_heads), _page_stride(v_pages, "v_pages", n_kv_heads)
     shape = k_pages.shape
-    if v_pages.shape != shape:
-        raise ValueError("k_pages and v_pages differ in shape")
-    if not page_table.is_cuda or page_table.dtype != torch.int32 or page_table.dim() != 2:
+    if len(shape) == 4 and shape == v_pages.shape and shape[1] == n_kv_heads and shape[3] == 128 and shape[0] \
+            and shape[2] in _PAGE_SIZES and k_pages.dtype == v_pages.dtype == torch.bfloat16 \
+            and k_pages.is_contiguous() and v_pages.is_contiguous():
+        kst = vst = n_kv_heads * shape[2] * 128
+    else:
+        kst, vst = _page_stride(k_pages, "k_pages", n_kv_heads), _page_stride(v_pages, "v_pages", n_kv_heads)
+        if v_pages.shape != shape:
+            raise ValueError("k_pages and v_pages differ in shape")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2:
         raise ValueError("page_table must be CUDA int32 [sequences, pages per sequence]")
     rows, width = page_table.shape
     if rows < batch or width == 0 or (width > 1 and page_table.stride(1) != 1):
@@ -373,9 +380,11 @@ def _lengths(cu_seqlens: torch.Tensor, kv_lens: torch.Tensor) -> int:
     return kv_lens.shape[0]
 
 
-def _rows_out(out: torch.Tensor | None, shape: tuple, dev: torch.device) -> torch.Tensor:
+def _rows_out(out: torch.Tensor | None, shape: tuple, like: torch.Tensor) -> torch.Tensor:
+    """``out`` checked, or a new bf16 tensor on the device of ``like`` (bf16)."""
     if out is None:
-        return torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        return like.new_empty(shape)
+    dev = like.device
     if out.dtype != torch.bfloat16 or out.shape != shape or not out.is_contiguous() or out.device != dev:
         raise ValueError(f"out must be a contiguous bf16 {list(shape)} tensor on {dev}")
     return out
@@ -406,15 +415,15 @@ def qk_norm_rope_store(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torc
     B = _lengths(cu_seqlens, kv_lens)
     qw, kw, wdt = _norm_weights(q_weight, k_weight)
     cache = _paged_cache(k_pages, v_pages, page_table, n_kv_heads, B)
-    _same_device(dev.index, q_weight=qw, k_weight=kw, cu_seqlens=cu_seqlens, kv_lens=kv_lens, k_pages=k_pages,
-                 v_pages=v_pages, page_table=page_table)
-    out = _rows_out(out, (T, n_heads, 128), dev)
+    _same_device(dev.index, "q_weight k_weight cu_seqlens kv_lens k_pages v_pages page_table", qw, kw, cu_seqlens,
+                 kv_lens, k_pages, v_pages, page_table)
+    out = _rows_out(out, (T, n_heads, 128), qkv)
     s = _raw_stream(dev.index)
     ws = _paged_workspace(dev, s, 0)
     call("nkimoe_qk_norm_rope_store", qkv.data_ptr(), qw.data_ptr(), kw.data_ptr(), wdt,
              cu_seqlens.data_ptr(), kv_lens.data_ptr(), *cache, out.data_ptr(), T, B, n_heads, n_kv_heads, 128,
              theta, eps, ws.data_ptr(), s)
-    if sync_check_enabled():
+    if "NKIMOE_SYNC_CHECK" in os.environ and sync_check_enabled():
         read_status(ws)
     return out
 
@@ -448,9 +457,9 @@ def paged_decode_attention(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: 
         raise ValueError(f"positions has {n_pos} entries for {B} sequences")
     qw, kw, wdt = _norm_weights(q_weight, k_weight)
     cache = _paged_cache(k_pages, v_pages, page_table, n_kv_heads, B)
-    _same_device(dev.index, q_weight=qw, k_weight=kw, positions=positions, k_pages=k_pages, v_pages=v_pages,
-                 page_table=page_table)
-    out = _rows_out(out, (B, n_heads * 128), dev)
+    _same_device(dev.index, "q_weight k_weight positions k_pages v_pages page_table", qw, kw, positions, k_pages,
+                 v_pages, page_table)
+    out = _rows_out(out, (B, n_heads * 128), qkv)
     s = _raw_stream(dev.index)
     nbytes = _paged_ws_bytes(dev.index, "nkimoe_paged_decode_attention_workspace_bytes", B, n_heads, n_kv_heads,
                              cache[8], cache[5])
@@ -458,7 +467,7 @@ def paged_decode_attention(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: 
     call("nkimoe_paged_decode_attention", qkv.data_ptr(), qw.data_ptr(), kw.data_ptr(), wdt,
              positions.data_ptr(), 0 if n_pos == 1 else 1, *cache, out.data_ptr(), B, n_heads, n_kv_heads, 128, theta,
              eps, 128 ** -0.5 if scale is None else scale, window, sinks, ws.data_ptr(), ws.numel(), s)
-    if sync_check_enabled():
+    if "NKIMOE_SYNC_CHECK" in os.environ and sync_check_enabled():
         read_status(ws)
     return out
 
@@ -487,8 +496,9 @@ def paged_prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     B = _lengths(cu_seqlens, kv_lens)
     nkv = k_pages.shape[1] if k_pages.dim() == 4 else 0
     cache = _paged_cache(k_pages, v_pages, page_table, nkv, B)
-    _same_device(dev.index, cu_seqlens=cu_seqlens, kv_lens=kv_lens, k_pages=k_pages, v_pages=v_pages, page_table=page_table)
-    out = _rows_out(out, (T, nq * 128), dev)
+    _same_device(dev.index, "cu_seqlens kv_lens k_pages v_pages page_table", cu_seqlens, kv_lens, k_pages, v_pages,
+                 page_table)
+    out = _rows_out(out, (T, nq * 128), q)
     s = _raw_stream(dev.index)
     nbytes = _paged_ws_bytes(dev.index, "nkimoe_paged_prefill_attention_workspace_bytes", T, B, nq, nkv, cache[8],
                              cache[5])
@@ -496,7 +506,7 @@ def paged_prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     call("nkimoe_paged_prefill_attention", q.data_ptr(), q.stride(0) if T > 1 else nq * 128, *cache,
          cu_seqlens.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), T, B, nq, nkv, 128,
          128 ** -0.5 if scale is None else scale, window, sinks, ws.data_ptr(), ws.numel(), s)
-    if sync_check_enabled():
+    if "NKIMOE_SYNC_CHECK" in os.environ and sync_check_enabled():
         read_status(ws)
     return out
 
@@ -560,11 +570,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0):
     if not 0 <= top_n <= min(32, V):
         raise ValueError(f"top_n {top_n} is not in [0, min(32, {V})]")
     dev = logits.device
-    _same_device(dev.index, tokens=tokens)
+    _same_device(dev.index, "tokens", tokens)
     lp = torch.empty(T, dtype=torch.float32, device=dev)
     ent = torch.empty(T, dtype=torch.float32, device=dev)
     top_lp = torch.empty(T, top_n, dtype=torch.float32, device=dev)
-    top_ids = torch.empty(T, top_n, dtype=torch.int64, device=dev)
+    top_ids = tokens.new_empty((T, top_n))
     if T == 0:
         return lp, ent, top_lp, top_ids
     s = _raw_stream(dev.index)

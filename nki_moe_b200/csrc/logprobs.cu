@@ -252,11 +252,13 @@ struct WarpTop {
   }
 };
 
+constexpr int kLpShow = 32 / kLpWarps;  // keys that each warp shows the others
+
 struct TopShared {
   int2 list[kLpWarps][32];
   int2 cand[kLpWarps][64];  // a warp's candidates that are not in its list yet
-  uint4 spread[kLpWarps][kLpVecs];
-  int floor;                // `top` elements of the row are known to be at or above this key
+  int seen[32];             // keys of elements seen, kLpShow of each warp
+  int4 copy[kLpWarps][8];
 };
 
 // The CTA's best 32 of the warps' lists, in warp 0.
@@ -273,65 +275,122 @@ __device__ __forceinline__ void join_warps(TopShared& sh, WarpTop& best, int war
   }
 }
 
-// Joins a warp's part of a chunk (its lanes' vectors, their largest values mx)
-// into the warp's best.  The warps do this each for itself; what one has found
-// lets the others pass over more (sh.floor).  Most chunks of a row hold
-// nothing: one comparison and one vote.
-template <typename T>
-__device__ __forceinline__ void warp_top(TopShared& sh, WarpTop& best, const uint4 (&raw)[kLpVecs], float mx,
-                                         long long base, int lo, int hi, int top, int lane) {
-  constexpr int VE = LpVec<T>::VE;
-  // the lane's greatest key (what lies outside the row counts as -inf here,
-  // which only lowers the bound)
-  const int mk = order_key(mx);
-  const int worst = __shfl_sync(0xffffffffu, best.key, top - 1);
-  int least;  // keys from here on are candidates
-  if (worst != INT_MIN) {
-    least = worst == 0x7fffffff ? worst : worst + 1;  // later elements lose ties against the ones held
-  } else {
-    // the top-th largest of the lanes' maxima has `top` elements at or above it
-    int place = 0;
-#pragma unroll
-    for (int o = 0; o < 32; ++o) {
-      const int k = __shfl_sync(0xffffffffu, mk, o);
-      place += k > mk || (k == mk && o < lane);
+// The n-th largest of the keys that the warps show, as one warp finds them (an
+// older state of some only lowers it): `n` elements reach it.  A few places by
+// one maximum each, more by the keys' ranks (8000 rows of 32000 with 5
+// alternatives 140 us against 144, 2000 rows of 151936 with 20 148 against 169).
+__device__ __forceinline__ int nth_seen(TopShared& sh, int n, int warp, int lane) {
+  int mine = *static_cast<volatile int*>(&sh.seen[lane]);
+  if (n <= 8) {
+    for (;;) {
+      const int v = __reduce_max_sync(0xffffffffu, mine);
+      n -= __popc(__ballot_sync(0xffffffffu, mine == v));
+      if (n <= 0) return v;
+      if (mine == v) mine = INT_MIN;
     }
-    least = __shfl_sync(0xffffffffu, mk, __ffs(__ballot_sync(0xffffffffu, place == top - 1)) - 1);
   }
-  least = max(least, *const_cast<volatile int*>(&sh.floor));
-  unsigned lanes = __ballot_sync(0xffffffffu, mk >= least);
-  if (lanes == 0) return;
-  int2* const cand = sh.cand[threadIdx.x >> 5];
-  uint4* const spread = sh.spread[threadIdx.x >> 5];
-  int n = 0;
-  while (lanes) {  // one lane's elements at a time, spread over the warp
-    const int src = __ffs(lanes) - 1;
-    lanes &= lanes - 1;
-    if (lane == src) {
+  reinterpret_cast<int*>(sh.copy[warp])[lane] = mine;  // one state for all lanes
+  __syncwarp();
+  int above = 0;
 #pragma unroll
-      for (int v = 0; v < kLpVecs; ++v) spread[v] = raw[v];
+  for (int i = 0; i < 8; ++i) {
+    const int4 o = sh.copy[warp][i];
+    above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+  }
+  return __reduce_min_sync(0xffffffffu, above < n ? mine : INT_MAX);
+}
+
+// Which of a thread's elements may reach the key `least`: bit i for word i
+// (bf16: its low half, bit 16 + i its high half).  NaNs always may, and so may
+// bf16 values right below a key that is not one of theirs.
+template <typename T>
+__device__ __forceinline__ unsigned may_reach(const uint4 (&raw)[kLpVecs], int least) {
+  unsigned bits = 0;
+  if constexpr (sizeof(T) == 2) {
+    const unsigned h = (least >= 0 ? least : least ^ 0x7fff0000) >> 16 & 0xffff;
+    const unsigned t = h << 16 | h;
+#pragma unroll
+    for (int v = 0; v < kLpVecs; ++v) {
+      const uint32_t w[4] = {raw[v].x, raw[v].y, raw[v].z, raw[v].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t m;
+        asm("set.geu.u32.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(w[i]), "r"(t));
+        bits |= m & (0x00010001u << (4 * v + i));
+      }
     }
-    __syncwarp();
-    float x = 0.f;
-    if (lane < LpVec<T>::NE) x = lp_float(reinterpret_cast<const T*>(spread)[lane]);
+  } else {
+    const float t = key_value(least);
+#pragma unroll
+    for (int v = 0; v < kLpVecs; ++v) {
+      const uint32_t w[4] = {raw[v].x, raw[v].y, raw[v].z, raw[v].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bits |= __uint_as_float(w[i]) < t ? 0u : 1u << (4 * v + i);
+    }
+  }
+  return bits;
+}
+
+// Word w (0 .. 15) of a thread's vectors, by selection.
+__device__ __forceinline__ uint32_t word_of(const uint4 (&raw)[kLpVecs], int w) {
+  const bool a = w & 8, b = w & 4, c = w & 2, d = w & 1;
+  const uint32_t x = a ? (b ? raw[3].x : raw[2].x) : (b ? raw[1].x : raw[0].x);
+  const uint32_t y = a ? (b ? raw[3].y : raw[2].y) : (b ? raw[1].y : raw[0].y);
+  const uint32_t z = a ? (b ? raw[3].z : raw[2].z) : (b ? raw[1].z : raw[0].z);
+  const uint32_t u = a ? (b ? raw[3].w : raw[2].w) : (b ? raw[1].w : raw[0].w);
+  return c ? (d ? u : z) : (d ? y : x);
+}
+
+// Joins a warp's part of a chunk (its lanes' vectors, their largest values mx)
+// into the warp's best.  Most chunks of a row hold nothing: one comparison and
+// one vote.  Where one may, the bound is drawn up to what the CTA's warps have
+// seen by then; elements of this warp's own come after all that its list holds,
+// so they lose ties there.  In the row's first chunk the warps show the largest
+// values of eight lanes each and wait for one another.
+template <typename T>
+__device__ __forceinline__ void warp_top(TopShared& sh, WarpTop& best, const uint4 (&raw)[kLpVecs], float mx, int& least,
+                                         long long base, bool first, int lo, int hi, int top, int warp, int lane) {
+  constexpr int VE = LpVec<T>::VE;
+  const int mk = order_key(mx);  // (what lies outside the row counts as -inf, which only lowers the bound)
+  if (first) {
+    int k = mk;
+#pragma unroll
+    for (int d = 1; d < 32 / kLpShow; d <<= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, d));
+    if (lane % (32 / kLpShow) == 0) sh.seen[threadIdx.x / (32 / kLpShow)] = k;
+    __syncthreads();
+  } else if (!__any_sync(0xffffffffu, mk >= least)) {
+    return;
+  }
+  const int worst = __shfl_sync(0xffffffffu, best.key, top - 1);
+  least = max(max(least, nth_seen(sh, top, warp, lane)), worst == 0x7fffffff || worst == INT_MIN ? worst : worst + 1);
+  unsigned mine = mk >= least ? may_reach<T>(raw, least) : 0;
+  if (!__any_sync(0xffffffffu, mine != 0)) return;
+  int2* const cand = sh.cand[warp];
+  int n = 0;
+  for (bool more = true; more;) {  // an element of every lane that has one left
+    const int bit = __ffs(mine) - 1, w = bit & 15;
+    const uint32_t word = word_of(raw, w);
+    const float x = sizeof(T) == 4 ? __uint_as_float(word) : __uint_as_float(bit & 16 ? word & 0xffff0000u : word << 16);
     const int k = order_key(x);
-    const int tid = (threadIdx.x & ~31) + src;
-    const long long id = base + static_cast<long long>((lane / VE) * kLpThreads + tid) * VE + lane % VE;
-    const bool in = lane < LpVec<T>::NE && id >= lo && id < hi && k >= least;
+    const int e = sizeof(T) == 4 ? w : 2 * w + (bit >> 4 & 1);
+    const long long id = base + static_cast<long long>((e / VE) * kLpThreads + threadIdx.x) * VE + e % VE;
+    const bool in = mine != 0 && id >= lo && id < hi && k >= least;
     const unsigned hit = __ballot_sync(0xffffffffu, in);
     if (in) cand[n + __popc(hit & ((1u << lane) - 1u))] = make_int2(k, static_cast<int>(id));
     n += __popc(hit);
+    mine &= mine - 1;
+    more = __any_sync(0xffffffffu, mine != 0);
     __syncwarp();
-    if (n < 32 && lanes) continue;
-    if (n <= 4) {  // a few: each to its place
+    if (n < 32 && more) continue;
+    if (n <= 8) {  // a few: each to its place
       for (int i = 0; i < n; ++i) best.insert(cand[i].x, cand[i].y, lane);
       n = 0;
     }
-    while (n >= 32 || (n > 0 && lanes == 0)) {  // many (the first chunk): sorted and merged, 32 at a time
+    while (n >= 32 || (n > 0 && !more)) {  // many: sorted and merged, 32 at a time
       const int2 c = lane < n ? cand[lane] : make_int2(INT_MIN, INT_MAX - 32 - lane);
-      WarpTop more{c.x, c.y};
-      more.sort(lane);
-      best.merge(more, lane);
+      WarpTop o{c.x, c.y};
+      o.sort(lane);
+      best.merge(o, lane);
       const int2 rest = cand[32 + lane];
       __syncwarp();
       cand[lane] = rest;
@@ -339,19 +398,27 @@ __device__ __forceinline__ void warp_top(TopShared& sh, WarpTop& best, const uin
       n = max(n - 32, 0);
     }
   }
-  const int now = __shfl_sync(0xffffffffu, best.key, top - 1);
-  if (lane == 0 && now > worst) atomicMax(&sh.floor, now);
+  // (the lanes' largest values of the first chunk may be others than the list's first)
+  if (lane < kLpShow) {
+    volatile int* at = &sh.seen[warp * kLpShow + lane];
+    *at = best.key;
+  }
 }
 
 // CTA (split, row): elements [split * per_split, ...) of the row in chunks of
 // 16 KB held in registers, the next chunk in flight; the last CTA of a row
 // joins the splits' parts.
 //
-// Bound by HBM over many rows (the logits read once), by issue next to it:
-// measured 2000 rows of 151936 bf16 with 5 alternatives 139 us = 4.36 TB/s =
-// 0.67 of the measured copy; 8 rows with 20 alternatives 14.7 us (one chunk per
-// CTA, then the join).  With the CTA's best tokens kept in common, a barrier per
-// chunk, 2000 rows took 500 us.
+// Bound by HBM over many rows (the logits read once), by the exponentials next
+// to it: measured 2000 rows of 151936 bf16 99.5 us without alternatives (6.11
+// TB/s = 0.93 of the measured copy), 122 us with 5 and 148 us with 20: a warp that
+// finds a candidate keeps its next loads waiting.  8 rows with 20 alternatives
+// 8.8 us (one chunk per CTA, then the join).  What was slower with 5
+// alternatives: the CTA's best tokens kept in common, a barrier per chunk, 500
+// us; the warps' lists made one after 1, 2, 4, 8 ... chunks, 137 us; a lane's
+// elements spread over its warp, one such lane at a time, 124 us (8000 rows of
+// 32000: 158 against 140).  Chunks copied to shared memory two ahead: 121 us,
+// but 108 without alternatives and 155 for the shorter rows.
 template <typename T, bool kTop>
 __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LpParams p) {
   __shared__ TopShared sh;
@@ -360,7 +427,6 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LpP
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int split = blockIdx.x % p.splits;
   const long long r = blockIdx.x / p.splits;
-  if (kTop && threadIdx.x == 0) sh.floor = INT_MIN;
   pdl_launch_dependents();
   pdl_wait();
   const T* row = static_cast<const T*>(p.x) + r * p.row_stride;
@@ -377,11 +443,11 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LpP
     tok = p.tokens[r];
     if (tok >= 0 && tok < p.V) x_tok = lp_float(row[tok]);
   }
-  if (kTop) __syncthreads();
 
   Stat st{-INFINITY, 0.f, 0.f};
   WarpTop best;
   best.clear(lane);
+  int least = INT_MIN;
   for (long long base = first; base < hi; base += LpVec<T>::Chunk) {
 #pragma unroll
     for (int v = 0; v < kLpVecs; ++v) raw[v] = next[v];
@@ -420,7 +486,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LpP
       if (mx != mx) c.m = -INFINITY;  // the sums hold the NaN
     }
     stat_join(st, c);
-    if constexpr (kTop) warp_top<T>(sh, best, raw, mx, base, lo, hi, p.top, lane);
+    if constexpr (kTop) {
+      warp_top<T>(sh, best, raw, mx, least, base, base == first, lo, hi, p.top, warp, lane);
+    }
   }
   st = stat_warp(st);
   if (lane == 0) warp_stat[warp] = st;

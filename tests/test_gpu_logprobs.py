@@ -139,3 +139,23 @@ def test_calls_on_two_streams_and_in_graphs():
     for (_, got), w in zip(graphs, want):
         assert all(torch.equal(a, b) for a, b in zip(got, w))
     assert all(torch.equal(a, b) for a, b in zip(eager, want[0]))
+
+
+@pytest.mark.parametrize("dtype,n", [(torch.float32, 20), (torch.bfloat16, 5), (torch.bfloat16, 32)])
+def test_orders_within_whole_rows(dtype, n):
+    """Rows that one CTA reads in several chunks: rising, falling, few different values,
+    all below zero, all of the best in one warp's or one lane's places, the best last."""
+    T, V = 600, 25003
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn(T, V, generator=g, device="cuda")
+    at = torch.arange(V, device="cuda")
+    x[0:100] = x[0:100].sort(-1).values
+    x[100:200] = x[100:200].sort(-1, descending=True).values
+    x[200:300] = (2 * x[200:300]).round()
+    x[300:400] = -5 - x[300:400].abs()
+    x[400:450] += 20.0 * ((at // 256) % 8 == 3)
+    x[450:500] += 20.0 * ((at // 8) % 256 == 77)
+    x[500:550, -40:] += 10
+    x[550:600] = -torch.inf
+    x[550:600, ::911] = 0.5
+    check(x.to(dtype), torch.randint(V, (T,), generator=g, device="cuda"), n)

@@ -572,8 +572,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0):
     dev = logits.device
     _same_device(dev.index, "tokens", tokens)
     lp = torch.empty(T, dtype=torch.float32, device=dev)
-    ent = torch.empty(T, dtype=torch.float32, device=dev)
-    top_lp = torch.empty(T, top_n, dtype=torch.float32, device=dev)
+    ent = torch.empty_like(lp)
+    top_lp = lp.new_empty((T, top_n))
     top_ids = tokens.new_empty((T, top_n))
     if T == 0:
         return lp, ent, top_lp, top_ids

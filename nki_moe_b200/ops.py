@@ -285,7 +285,9 @@ def _paged_workspace(dev: torch.device, stream: int, nbytes: int) -> torch.Tenso
 def read_paged_status(device=None) -> None:
     """Synchronises ``device`` and raises if a paged-cache call on it met a
     position or page id out of range, or a page that it needed and that was
-    not held (the status is cleared)."""
+    not held (the status is cleared).  Of calls in CUDA graphs it sees the
+    last replay of the graph captured last on each stream: a replay begins by
+    clearing its own status."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     index = torch.cuda.current_device() if dev.index is None else dev.index
     torch.cuda.synchronize(index)

@@ -198,7 +198,7 @@ class PagedKVCache(PageTables):
 
     def __init__(self, num_layers: int, n_kv_heads: int, num_pages: int, page_size: int = 64, max_seq: int = 4096,
                  window: int = 0, sinks: int = 0, device="cuda"):
-        super().__init__(num_pages, page_size, -(-max_seq // page_size), window, sinks)
+        super().__init__(num_pages, page_size, -(-max_seq // page_size) if page_size > 0 else 1, window, sinks)
         self.device = torch.device(device)
         self.pool = torch.empty(num_layers, 2, num_pages, n_kv_heads, page_size, 128, dtype=torch.bfloat16,
                                 device=self.device)

@@ -478,17 +478,22 @@ class Qwen3MoEStack:
 
         Greedy with ``temperature`` 0, else sampled (``generator`` on the
         stack's device).  With ``window`` the model attends to the last
-        ``window`` tokens and the first ``sinks`` ones.  Returns ``(tokens
+        ``window`` tokens and the first ``sinks`` ones; a ``cache`` that is given
+        brings its own page size and window.  Returns ``(tokens
         [len(prompts), samples, max_new_tokens], scores)``; ``scores`` is None
         or, with ``top_logprobs`` alternatives, a dict of ``logprob`` and
         ``entropy`` ``[.., max_new_tokens]`` and ``top_logprobs``/``top_ids``
         ``[.., max_new_tokens, top_logprobs]``."""
         if samples < 1 or max_new_tokens < 1:
             raise ValueError("samples and max_new_tokens must be positive")
-        n, ends = len(prompts), [int(p.numel()) + max_new_tokens for p in prompts]
+        n, ends, own = len(prompts), [int(p.numel()) + max_new_tokens for p in prompts], cache is None
+        if n == 0:
+            raise ValueError("no prompts")
         if cache is None:
-            pages = sum(-(-e // page_size) * samples for e in ends)
+            pages = sum(-(-e // max(page_size, 1)) * samples for e in ends)
             cache = self.paged_cache(pages, page_size, max(ends), window, sinks)
+        elif (window or sinks) and (window, sinks) != (cache.window, cache.sinks):
+            raise ValueError(f"the cache has window {cache.window} and sinks {cache.sinks}, not {window} and {sinks}")
         seqs = [cache.add() for _ in prompts]
         try:
             logits = self.prefill_paged(cache, seqs, prompts)
@@ -511,6 +516,8 @@ class Qwen3MoEStack:
             for q in seqs:
                 if q in cache:
                     cache.free(q)
+            if own and self._paged is not None and self._paged["cache"] is cache:
+                self._paged = None  # nobody else can use this cache: its pools go with the captured step
         tokens = torch.stack(out, 1).view(n, samples, max_new_tokens)
         if top_logprobs is None:
             return tokens, None
@@ -527,7 +534,11 @@ class Qwen3MoEStack:
         from the second on, each under what comes before it.  The logits are
         formed ``chunk`` rows at a time."""
         lens = [int(p.numel()) for p in prompts]
-        cache = self.paged_cache(sum(-(-n // page_size) for n in lens), page_size, max(lens), window, sinks)
+        if not lens or min(lens) == 0:
+            raise ValueError("prompts must not be empty")
+        if chunk < 1:
+            raise ValueError(f"chunk {chunk} is not positive")
+        cache = self.paged_cache(sum(-(-n // max(page_size, 1)) for n in lens), page_size, max(lens), window, sinks)
         hn = self._prompt_hidden(cache, [cache.add() for _ in prompts], prompts)
         # a prompt's last row predicts nothing that is given
         given = torch.cat([torch.cat([p.reshape(-1)[1:].to(self.device), p.new_full((1,), -1).to(self.device)])

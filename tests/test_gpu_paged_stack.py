@@ -161,3 +161,36 @@ def test_refusals(pair):
     with pytest.raises(RuntimeError):
         st.prefill_paged(cache, [a], [ids(60, 3)])
     assert cache.length(a) == 5 and cache.free_pages == 2
+
+
+def test_generation_keeps_no_cache_of_its_own(pair):
+    """The captured step of a cache that nobody else can reach ends with the call; a
+    given cache keeps its step, its pages come back, and its window is not overruled."""
+    _, st = pair
+    prompts = [ids(20, 1), ids(33, 2)]
+    st.release_graph()
+    mine, _ = st.generate_paged(prompts, 4, page_size=16)
+    assert st._paged is None
+    cache = st.paged_cache(12, page_size=16, window=64, sinks=2)
+    given, _ = st.generate_paged(prompts, 4, cache=cache)  # nothing is outside the window yet
+    assert st._paged["cache"] is cache and cache.free_pages == 12
+    assert torch.equal(mine, given)
+    again, _ = st.generate_paged(prompts, 4, cache=cache, window=64, sinks=2)
+    assert torch.equal(mine, again)
+    for kw in (dict(window=32), dict(window=64, sinks=4), dict(sinks=2)):
+        with pytest.raises(ValueError):
+            st.generate_paged(prompts, 4, cache=cache, **kw)
+    assert cache.free_pages == 12
+    for size in (0, -16, 24):
+        with pytest.raises(ValueError):
+            st.generate_paged(prompts, 4, page_size=size)
+        with pytest.raises(ValueError):
+            st.score(prompts, page_size=size)
+    for none in ([], [ids(0, 1)]):
+        with pytest.raises(ValueError):
+            st.generate_paged(none, 4)
+        with pytest.raises(ValueError):
+            st.score(none)
+    with pytest.raises(ValueError):
+        st.score(prompts, chunk=-1)
+    st.release_graph()

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from nki_moe_b200 import _lib, ops
-from nki_moe_b200.paged import CacheFull, PageTables
+from nki_moe_b200.paged import CacheFull, PagedKVCache, PageTables
 
 
 def test_extend_takes_the_lowest_pages_and_counts_lengths():
@@ -248,3 +248,9 @@ def test_entry_points_refuse_cpu_tensors():
         ops.copy_pages(pages, [0], [1])
     with pytest.raises(ValueError):
         ops.token_logprobs(x, torch.zeros(2, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("size", [0, -16, 24, 512])
+def test_a_cache_refuses_other_page_sizes(size):
+    with pytest.raises(ValueError):
+        PagedKVCache(1, 1, 4, size, 64, device="cpu")

@@ -101,10 +101,13 @@ def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
 
 def release_captured_workspaces() -> int:
     """Drop the replaced workspaces kept for captured CUDA graphs (call after
-    those graphs are destroyed).  Returns how many were released."""
+    those graphs are destroyed), and what the paged calls hold of the last
+    graph's memory.  Returns how many replaced ones were released."""
     with _ws_lock:
         n = len(_ws_retired)
         _ws_retired.clear()
+        for key in [k for k in _paged_ws if k[2]]:
+            del _paged_ws[key]
     return n
 
 

@@ -13,9 +13,10 @@
 // tokens wide.  A CTA works on two such tiles at a time ("pair") against the
 // same key blocks of 128 positions:
 //
-//   warp 0      one thread: takes work units, loads Q (TMA, rows gathered by
-//               a 3-D box over heads and tokens) and the K / V blocks page by
-//               page (4-D boxes, 128-byte swizzle) into a ring of 32 KB stages
+//   warp 0      takes work units, loads Q (TMA, rows gathered by a 3-D box over
+//               heads and tokens) and the K blocks page by page (4-D boxes,
+//               128-byte swizzle) into a ring of 32 KB stages
+//   warp 2      loads the V blocks
 //   warp 1      issues the MMAs: S = Q K^T into tensor memory, then
 //               O += P V with P read from tensor memory and V as the
 //               transposed (MN-major) operand
@@ -34,7 +35,7 @@
 // -> weights -> product -> next scores, about 3500 cycles per block and pair
 // against 2100 of MMAs (P lies over S, so a tile's next scores wait for its
 // product).  Measured: 8192 causal tokens, 32 heads over 4: 447 us = 1.23
-// PFLOP/s = 0.73 of the measured cuBLAS rate; 8 x 512 tokens 39 us; 945 rows in
+// PFLOP/s = 0.73 of the measured cuBLAS rate; 8 x 512 tokens 37 us; 945 rows in
 // four chunks over 9001 cached positions, window 4096: 83 us.
 // Other shapes of the pipeline were slower (8192 tokens): key blocks of 64 with
 // two score buffers per tile 891 us (an MMA of N = 64 takes as long as one of
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       mbar_init(&ctl.p_full[t], 4);  // one arrival per softmax warp
       mbar_init(&ctl.o_full[t], 1);
       mbar_init(&ctl.u_full[t], 1);
-      mbar_init(&ctl.u_empty[t], 1 + 8);  // the MMA warp and the softmax warps
+      mbar_init(&ctl.u_empty[t], 2 + 8);  // the MMA warp, the warp that loads V, the softmax warps
     }
     mbar_init(&ctl.drain, 1);
     ctl.abort_flag = 0;
@@ -352,22 +353,25 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
   // 384 x 168 registers at launch = 128 x 88 + 256 x 208
-  if (warp == 0) {
+  if (warp == 0 || warp == 2) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     // ---------------------------------------------------------------- units and loads
-    // Lane (v, h, g) loads half h of page g of a K (v = 0) or V block: one
-    // thread's bookkeeping for all of them took 2000 cycles per block.
-    const int v_lane = lane >> 4, h_lane = (lane >> 3) & 1, g_lane = lane & 7;
+    // Lane (h, g) loads half h of page g of a block.  A box takes its warp 110
+    // cycles (a block of 16-position pages 1800), so K and V have a warp each and
+    // the first queries go out before the page ids are there: 8 x 512 tokens 39.0
+    // -> 37.8 us.
+    const int v = warp >> 1;
+    const int h_lane = (lane >> 3) & 1, g_lane = lane & 7;
     const int page_rows = min(1 << p.c.page_shift, kPfBlock);  // rows per box
-    const bool loads = g_lane * page_rows < kPfBlock;
-    const void* const tm = v_lane ? static_cast<const void*>(&tmap_v) : static_cast<const void*>(&tmap_k);
+    const bool loads = lane < 16 && g_lane * page_rows < kPfBlock;
+    const void* const tm = v ? static_cast<const void*>(&tmap_v) : static_cast<const void*>(&tmap_k);
     const int box_at = h_lane * static_cast<int>(kPfBlockHalf) + g_lane * page_rows * 128;
     const uint32_t q_bytes = 2u * p.grp * p.tpt * 128u;  // both halves of one tile's box
     auto wait = [&](uint64_t* bar, uint32_t ph) {
       const bool got = mbar_wait(bar, ph, &ctl.abort_flag, p.status);
       return __all_sync(0xffffffffu, got);
     };
-    int stage = 0;
+    int stage = v;  // K blocks in the even stages, V blocks in the odd ones
     uint32_t phase = 0, issued = 0, last_phase = 0;
     bool ok = true, q_issued = false;
     const PfList list = *p.list;
@@ -375,40 +379,58 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     const int run_lo = min(list.total, static_cast<int>(blockIdx.x) * list.share);
     const int run_hi = min(list.total, run_lo + list.share);
     int at = run_lo, pair = 0, unit = blockIdx.x;
-    if (list.share) {
+    if (v == 0 && list.share) {
       if (lane == 0) p.splits[blockIdx.x].parts = 0;
       for (int hi = list.pairs; hi - pair > 1;) {
         const int mid = (pair + hi) >> 1;
         if (p.offs[mid] * p.c.nkv <= at) pair = mid; else hi = mid;
       }
     }
+    auto load_q = [&](const PfWork& w, int u) {
+      if (!wait(&ctl.q_empty, (u & 1) ^ 1u)) return false;
+      const int tiles = w.tokens > p.tpt ? 2 : 1;
+      if (lane == 0) mbar_arrive_expect_tx(&ctl.q_full, tiles * q_bytes);
+      __syncwarp();
+      if (lane < 2 * tiles)
+        tma_load_3d(sq + (lane >> 1) * kPfTileBytes + (lane & 1) * kPfTileHalf, &tmap_q, &ctl.q_full, (lane & 1) * 64,
+                    w.j * p.grp, w.row0 + (lane >> 1) * p.tpt);
+      q_issued = true;
+      return true;
+    };
     for (int u = 0; ok; ++u) {
       const int us = u & 1;
-      if (!wait(&ctl.u_empty[us], ((u >> 1) & 1) ^ 1u)) { ok = false; break; }
       PfWork w{};
-      if (list.share == 0) {
-        if (unit < list.pairs * p.c.nkv) {
-          static_cast<PfUnit&>(w) = p.units[unit / p.c.nkv];
-          w.j = unit % p.c.nkv;
-          // the one after it, long before it is needed
-          if (lane == 0) unit = atomicAdd(&p.list->next, 1) + gridDim.x;
+      if (v) {
+        if (!wait(&ctl.u_full[us], (u >> 1) & 1)) { ok = false; break; }
+        w = ctl.work[us];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.u_empty[us]);
+      } else {
+        if (!wait(&ctl.u_empty[us], ((u >> 1) & 1) ^ 1u)) { ok = false; break; }
+        if (list.share == 0) {
+          if (unit < list.pairs * p.c.nkv) {
+            static_cast<PfUnit&>(w) = p.units[unit / p.c.nkv];
+            w.j = unit % p.c.nkv;
+            // the one after it, long before it is needed
+            if (lane == 0) unit = atomicAdd(&p.list->next, 1) + gridDim.x;
+          }
+        } else if (at < run_hi) {
+          static_cast<PfUnit&>(w) = p.units[pair];
+          const int base = p.offs[pair] * p.c.nkv, n = w.hi;
+          w.j = (at - base) / n;
+          const int item = base + w.j * n;  // the list's first block of (pair, kv head)
+          w.lo = at - item;
+          w.hi = min(n, run_hi - item);
+          const int first = item / list.share, parts = (item + n - 1) / list.share - first + 1;
+          if (parts > 1) w.slot = 2 * static_cast<int>(blockIdx.x) + (item < run_lo ? 0 : 1);
+          if (parts > 1 && item >= run_lo && lane == 0) p.splits[blockIdx.x] = PfSplit{pair, w.j, parts, 0};
+          at = item + w.hi;
+          if (w.hi == n && w.j == p.c.nkv - 1) ++pair;
         }
-      } else if (at < run_hi) {
-        static_cast<PfUnit&>(w) = p.units[pair];
-        const int base = p.offs[pair] * p.c.nkv, n = w.hi;
-        w.j = (at - base) / n;
-        const int item = base + w.j * n;  // the list's first block of (pair, kv head)
-        w.lo = at - item;
-        w.hi = min(n, run_hi - item);
-        const int first = item / list.share, parts = (item + n - 1) / list.share - first + 1;
-        if (parts > 1) w.slot = 2 * static_cast<int>(blockIdx.x) + (item < run_lo ? 0 : 1);
-        if (parts > 1 && item >= run_lo && lane == 0) p.splits[blockIdx.x] = PfSplit{pair, w.j, parts, 0};
-        at = item + w.hi;
-        if (w.hi == n && w.j == p.c.nkv - 1) ++pair;
-      }
-      if (lane == 0) {
-        ctl.work[us] = w;
-        mbar_arrive(&ctl.u_full[us]);
+        if (lane == 0) {
+          ctl.work[us] = w;
+          mbar_arrive(&ctl.u_full[us]);
+        }
       }
       if (w.tokens == 0) break;
       const Blocks bl = blocks_of(w.pos0, w.pos0 + w.tokens - 1, p.window, p.sinks);
@@ -421,39 +443,28 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         const bool need = loads && s0 <= last && (s0 + page_rows > start || s0 < p.sinks);
         return need ? table[s0 >> p.c.page_shift] : -2;
       };
+      if (v == 0 && u == 0 && !load_q(w, u)) { ok = false; break; }
       int next = look_up(w.lo);
       for (int i = w.lo; ok && i < w.hi; ++i) {
         const bool held = next >= 0 && next < p.c.num_pages;
         if (!held && next != -2) atomicOr(p.status, kDevErrBadIndex);
         const int page = held ? next : p.c.num_pages;  // past the last page: the load fills zeros
         const int in_page = (bl.at(i) * kPfBlock + g_lane * page_rows) & ((1 << p.c.page_shift) - 1);
-        if (i + 1 < w.hi) next = look_up(i + 1);  // in flight while this block waits for its stages
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          if (!wait(&ctl.kv_empty[stage], phase ^ 1u)) { ok = false; break; }
-          if (lane == 0) mbar_arrive_expect_tx(&ctl.kv_full[stage], kPfBlockBytes);
-          __syncwarp();
-          if (loads && v_lane == v)
-            tma_load_4d(ring + stage * kPfBlockBytes + box_at, tm, &ctl.kv_full[stage], h_lane * 64, in_page, w.j, page);
-          issued |= 1u << stage;
-          last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
-          if (++stage == kPfRing) {
-            stage = 0;
-            phase ^= 1u;
-          }
+        if (i + 1 < w.hi) next = look_up(i + 1);  // in flight while this block waits for its stage
+        if (!wait(&ctl.kv_empty[stage], phase ^ 1u)) { ok = false; break; }
+        if (lane == 0) mbar_arrive_expect_tx(&ctl.kv_full[stage], kPfBlockBytes);
+        __syncwarp();
+        if (loads) tma_load_4d(ring + stage * kPfBlockBytes + box_at, tm, &ctl.kv_full[stage], h_lane * 64, in_page, w.j, page);
+        issued |= 1u << stage;
+        last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
+        stage += 2;
+        if (stage >= kPfRing) {
+          stage = v;
+          phase ^= 1u;
         }
-        // the queries after the unit's first block, which goes out while the
+        // later units' queries after their first block, which goes out while the
         // unit before still reads its own
-        if (ok && i == w.lo) {
-          if (!wait(&ctl.q_empty, (u & 1) ^ 1u)) { ok = false; break; }
-          const int tiles = w.tokens > p.tpt ? 2 : 1;
-          if (lane == 0) mbar_arrive_expect_tx(&ctl.q_full, tiles * q_bytes);
-          __syncwarp();
-          if (lane < 2 * tiles)
-            tma_load_3d(sq + (lane >> 1) * kPfTileBytes + (lane & 1) * kPfTileHalf, &tmap_q, &ctl.q_full, (lane & 1) * 64,
-                        w.j * p.grp, w.row0 + (lane >> 1) * p.tpt);
-          q_issued = true;
-        }
+        if (v == 0 && u > 0 && i == w.lo && !load_q(w, u)) { ok = false; break; }
       }
       unit = __shfl_sync(0xffffffffu, unit, 0);
     }
@@ -564,7 +575,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp < 4) {
+  } else if (warp == 3) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -689,33 +700,36 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         const long long at = __shfl_sync(0xffffffffu, out_at, k * 8 + (lane >> 2));
         to_row[k] = at >= 0 ? p.out + at + (lane & 3) * 8 : nullptr;
       }
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        uint32_t o[32];
-        __syncwarp();
-        tmem_ld_32x32b_x32(to + c * 32, o);
-        tmem_ld_wait();
-        if (part) {
+      uint32_t o[4][32];  // all at once: 8 x 512 tokens 37.8 -> 37.4 us against 32 columns at a time
+      __syncwarp();
 #pragma unroll
-          for (int x = 0; x < 32; x += 4)
-            __stcg(reinterpret_cast<uint4*>(part) + (c * 8 + x / 4) * kPfRows + row,
-                   make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]));
-        } else {
-          // through shared memory: eight rows of 64 bytes per store instead of
-          // 32 rows of 16
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(to + c * 32, o[c]);
+      tmem_ld_wait();
+      if (part) {
+#pragma unroll
+        for (int x = 0; x < 128; x += 4)
+          __stcg(reinterpret_cast<uint4*>(part) + (x / 4) * kPfRows + row,
+                 make_uint4(o[x >> 5][x & 31], o[x >> 5][(x & 31) + 1], o[x >> 5][(x & 31) + 2], o[x >> 5][(x & 31) + 3]));
+      } else {
+        // through shared memory: eight rows of 64 bytes per store instead of
+        // 32 rows of 16
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
 #pragma unroll
           for (int x = 0; x < 32; x += 8) {
             float f[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[x + e]) * inv;
+            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[c][x + e]) * inv;
             *reinterpret_cast<uint4*>(&stg[warp - 4][lane][x]) = pack8(f);
           }
           __syncwarp();
+          uint4 v[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint4 v = *reinterpret_cast<const uint4*>(&stg[warp - 4][k * 8 + (lane >> 2)][(lane & 3) * 8]);
-            if (to_row[k]) *reinterpret_cast<uint4*>(to_row[k] + c * 32) = v;
-          }
+          for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const uint4*>(&stg[warp - 4][k * 8 + (lane >> 2)][(lane & 3) * 8]);
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (to_row[k]) *reinterpret_cast<uint4*>(to_row[k] + c * 32) = v[k];
         }
       }
       if (part) {

@@ -34,15 +34,18 @@
 // Bound by the tensor core and, more, by each tile's chain: scores -> softmax
 // -> weights -> product -> next scores, about 3500 cycles per block and pair
 // against 2100 of MMAs (P lies over S, so a tile's next scores wait for its
-// product).  Measured: 8192 causal tokens, 32 heads over 4: 447 us = 1.23
-// PFLOP/s = 0.73 of the measured cuBLAS rate; 8 x 512 tokens 37 us; 945 rows in
+// product).  Measured: 8192 causal tokens, 32 heads over 4: 441 us = 1.24
+// PFLOP/s = 0.74 of the measured cuBLAS rate; 8 x 512 tokens 37 us; 945 rows in
 // four chunks over 9001 cached positions, window 4096: 83 us.
 // Other shapes of the pipeline were slower (8192 tokens): key blocks of 64 with
 // two score buffers per tile 891 us (an MMA of N = 64 takes as long as one of
 // 128: it is bound by reading Q), one tile with two score buffers and its own
 // P columns 581 us (twice the K / V traffic through shared memory), two softmax
 // threads per row 500 us, a share of the exponentials as polynomials on the FMA
-// pipe 500 us, weights handed over in two parts 450 us.
+// pipe 500 us, weights handed over in two parts 450 us.  One score buffer that
+// the tiles use in turn, P in columns of its own and a thread per tile for the
+// MMAs: 415 us, but 8 x 512 tokens 39 us (with the unit's first scores in O's
+// columns 426 and 42 us), and as much again in barriers to keep right.
 //
 // Work: a small kernel turns the lengths (device data) into the list of pairs,
 // a sequence's longest first, with their counts of key blocks.  With pairs

@@ -171,6 +171,67 @@ __device__ __forceinline__ HeadPart norm_rope_part(const HeadPart& x, const Head
   return o;
 }
 
+// Keys are kept rounded, so a sum in fp32 that falls on the other side of the
+// middle between two bf16 values stays wrong for good.  key_near_tie says which
+// of the lane's rotated pairs (bit e: elements 4l + e and 64 + 4l + e) lie that
+// near to a middle, by 2^-23 of the pair's length, which the rotation keeps: one
+// head in 60 has one.  Those are formed again by key_in_64_bits.  Of 361 values in
+// 12 million that fp32 alone rounds to the other side 2 are left (none with
+// 2^-22, 61 with 2^-24).
+__device__ __forceinline__ uint32_t key_near_tie(const HeadPart& o) {
+  uint32_t near = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float2 a = split2(o.a[i]), b = split2(o.b[i]);
+    const float av[2] = {a.x, a.y}, bv[2] = {b.x, b.y};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float e = (fabsf(av[k]) + fabsf(bv[k])) * 0x1p-23f;
+      const float am = __uint_as_float((__float_as_uint(av[k]) & 0xffff0000u) | 0x8000u);
+      const float bm = __uint_as_float((__float_as_uint(bv[k]) & 0xffff0000u) | 0x8000u);
+      if (fabsf(av[k] - am) < e || fabsf(bv[k] - bm) < e) near |= 1u << (2 * i + k);
+    }
+  }
+  return near;
+}
+
+// The pairs of `which` (any lane's) of a head, from its bf16 elements lo and hi
+// into its rounded key klo and khi; a half-warp per head, all 32 lanes call it.
+// w: the lane's first weight, of 128 in fp32.
+__device__ __noinline__ static void key_in_64_bits(uint32_t which, uint2 lo, uint2 hi, const float* w,
+                                                   const double* turns, int l, int pos, float eps, uint2& klo,
+                                                   uint2& khi) {
+  const uint32_t words[4] = {lo.x, lo.y, hi.x, hi.y};
+  double ss = 0.0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const double x = __uint_as_float(words[i] << 16), y = __uint_as_float(words[i] & 0xffff0000u);
+    ss += x * x + y * y;
+  }
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+  const double r = rsqrt(ss * (1.0 / kHeadDim) + static_cast<double>(eps));
+  which = __reduce_or_sync(0xffffffffu, which);
+#pragma unroll 1
+  for (int e = 0; e < 4; ++e) {
+    if (!((which >> e) & 1u)) continue;
+    const bool second = e & 2;
+    const uint32_t sh = e & 1 ? 16 : 0, keep = e & 1 ? 0xffffu : 0xffff0000u;
+    const uint32_t ua = second ? lo.y : lo.x, ub = second ? hi.y : hi.x;
+    const double a = static_cast<double>(__uint_as_float(ua >> sh << 16)) * w[e];
+    const double b = static_cast<double>(__uint_as_float(ub >> sh << 16)) * w[64 + e];
+    double t = turns[4 * l + e] * static_cast<double>(pos), sn, cs;
+    t -= rint(t);
+    sincospi(2.0 * t, &sn, &cs);
+    const uint32_t ra = __bfloat16_as_ushort(__float2bfloat16_rn(static_cast<float>((a * cs - b * sn) * r)));
+    const uint32_t rb = __bfloat16_as_ushort(__float2bfloat16_rn(static_cast<float>((b * cs + a * sn) * r)));
+    uint32_t& wa = second ? klo.y : klo.x;
+    uint32_t& wb = second ? khi.y : khi.x;
+    wa = (wa & keep) | ra << sh;
+    wb = (wb & keep) | rb << sh;
+  }
+}
+
 // Lets a kernel take `bytes` of dynamic shared memory, once per device.
 template <auto kKernel>
 cudaError_t allow_smem(int bytes) {

@@ -120,6 +120,7 @@ struct PdShared {
   __nv_bfloat16 q[kWide ? 2 : 1][16][kPdQRow];  // narrow: rows 0-7 hi, 8-15 lo; wide: hi, lo
   __align__(16) __nv_bfloat16 knew[kHeadDim], vnew[kHeadDim];
   float2 tab[kHeadDim / 2];
+  float kw[kHeadDim];  // key norm weights, for a key that is done again
   float ml[kPdWarps][16][2];
   int warp_sum[kPdWarps];
   int last;
@@ -292,9 +293,16 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
         uint2 lo = from[0], hi = from[16];
         w = load_weight_part(p.kw, p.w_dtype, l);
         const HeadPart o = norm_rope_part(part_of_rows(lo, hi), w, turn, p.eps);
+        uint2 klo = row_of_pairs(o.a), khi = row_of_pairs(o.b);
+        const uint32_t which = lane < 16 ? key_near_tie(o) : 0u;
+        if (__any_sync(0xffffffffu, which != 0)) {
+          for (int i = lane; i < D; i += 32) sh.kw[i] = head_wload(p.kw, p.w_dtype, i);
+          __syncwarp();
+          key_in_64_bits(which, lo, hi, sh.kw + 4 * l, p.turns.f, l, pos, p.eps, klo, khi);
+        }
         if (lane < 16) {  // the value goes bit for bit
-          lo = row_of_pairs(o.a);
-          hi = row_of_pairs(o.b);
+          lo = klo;
+          hi = khi;
         }
         uint2* keep = reinterpret_cast<uint2*>(lane < 16 ? sh.knew : sh.vnew);
         keep[l] = lo;

@@ -50,8 +50,9 @@ __device__ __forceinline__ int sequence_of(const int* cu, int B, int t, int lane
 // the row's position is known, so the two latencies overlap.
 //
 // Bound by HBM and by issue: (nq + 2 nkv) * 256 bytes read and as many written
-// per row.  Measured: 8192 rows of 32 + 2 * 4 heads 36 us = 4.65 TB/s = 0.71 of
-// the measured copy; 15 rows 3.6 us.
+// per row.  Measured: 8192 rows of 32 + 2 * 4 heads 41 us = 4.1 TB/s = 0.63 of
+// the measured copy; 15 rows 5.1 us.  Of that 4 us and 1.5 us are the keys formed
+// again in 64 bits, nearly all of it the first fetch of that code by each SM.
 template <int kWarps>
 __global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_store_kernel(const __grid_constant__ StoreParams p) {
   constexpr int D = kHeadDim;
@@ -100,6 +101,7 @@ __global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_stor
   uint2* const v_dst = reinterpret_cast<uint2*>(p.c.v + (held ? page * p.c.v_stride + in_page * D : 0)) + l;
   // a half-warp past the last head runs along with the other (the norm
   // shuffles within the whole warp) and stores nothing
+  uint32_t again = 0;  // which pairs of keys to form again: four bits per turn (modulo 8)
   for (int h0 = 0; h0 < nh; h0 += kAhead * kHalves) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
@@ -120,6 +122,7 @@ __global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_stor
         if (!is_v) {  // a value goes bit for bit
           lo = row_of_pairs(o.a);
           hi = row_of_pairs(o.b);
+          if (!is_q) again |= key_near_tie(o) << (4 * ((h0 / kHalves + i) & 7));
         }
       }
       if (h < nh && (is_q || held)) {
@@ -129,6 +132,30 @@ __global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_stor
         dst[0] = lo;
         dst[16] = hi;
       }
+    }
+  }
+  again = __reduce_or_sync(0xffffffffu, again);
+  if (again == 0 || !held) return;
+  for (int turn_no = p.nq / kHalves; turn_no * kHalves < p.nq + p.c.nkv; ++turn_no) {
+    const uint32_t which = again >> (4 * (turn_no & 7)) & 15u;
+    if (which == 0) continue;
+    const int h = half + turn_no * kHalves;
+    const bool is_k = h >= p.nq && h < p.nq + p.c.nkv;
+    uint2 lo = make_uint2(0u, 0u), hi = lo;
+    if (is_k) {
+      lo = row[h * 32];
+      hi = row[h * 32 + 16];
+    }
+    uint2* const dst = k_dst + (static_cast<long long>(is_k ? h - p.nq : 0) << head_shift);
+    uint2 klo = lo, khi = hi;
+    if (is_k) {  // as this lane stored them
+      klo = dst[0];
+      khi = dst[16];
+    }
+    key_in_64_bits(which, lo, hi, wtab[1] + l * 4, p.turns.f, l, pos, p.eps, klo, khi);
+    if (is_k) {
+      dst[0] = klo;
+      dst[16] = khi;
     }
   }
 }
@@ -163,8 +190,8 @@ cudaError_t paged_store_launch(const __nv_bfloat16* qkv, const void* qw, const v
   p.nq = nq;
   p.eps = eps;
   // few rows: a CTA's eight warps on each; many: a warp each, so that the lookups
-  // and the sines of a row are done once (8192 rows of 32 + 2 * 4 heads: 37 us,
-  // with two warps 46, with eight 42)
+  // and the sines of a row are done once (8192 rows of 32 + 2 * 4 heads, before keys
+  // were formed again: 37 us, with two warps 46, with eight 42)
   if (T <= kStoreFew)
     return launch_pdl(paged_store_kernel<8>, dim3(static_cast<unsigned>(T)), dim3(kStoreThreads), 0, s, p);
   return launch_pdl(paged_store_kernel<1>, dim3(static_cast<unsigned>((T + 7) / 8)), dim3(kStoreThreads), 0, s, p);

@@ -613,3 +613,29 @@ def test_prefill_reports_lengths_and_pages(monkeypatch):
         with pytest.raises(NKIMoEError):
             ops.read_paged_status()
         assert torch.equal(out[:40], good[:40])
+
+
+def test_kept_keys_are_the_rounded_ones():
+    """Keys against the formula in 64 bits, rounded once: fp32 alone puts about 3 of 10^5
+    values on the other side of the middle between two bf16 values; those near one are
+    formed again, so at most 1 of 10^6 may differ (and 2, so that one value is no failure)."""
+    for B, new, past, nq, nkv, ps, seed in ((3, 701, 20000, 12, 4, 64, 1), (2, 150, 5, 24, 8, 16, 2), (1, 4001, 0, 6, 2, 256, 3)):
+        total = [past + new + b for b in range(B)]
+        c = Cache(total, nkv, ps, seed)
+        g = torch.Generator().manual_seed(seed)
+        T = B * new
+        qkv = torch.randn(T, (nq + 2 * nkv) * HD, generator=g).bfloat16()
+        w = (1 + 0.2 * torch.randn(HD, generator=g)).bfloat16()
+        kd, vd = c.k.cuda(), c.v.cuda()
+        cu = torch.arange(B + 1, dtype=torch.int32) * new
+        ops.qk_norm_rope_store(qkv.cuda(), w.cuda(), w.cuda(), cu.cuda(), torch.tensor(total, dtype=torch.int32).cuda(),
+                               kd, vd, c.table.cuda(), nq, nkv)
+        x = qkv.view(T, -1, HD)[:, nq:nq + nkv].double()
+        x = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + 1e-6) * w.double()
+        pos = torch.cat([torch.arange(t - new, t) for t in total]).double()
+        ang = pos[:, None, None] * 1e6 ** (-torch.arange(HD // 2, dtype=torch.float64) / (HD // 2))
+        a, b = x[..., :HD // 2], x[..., HD // 2:]
+        ref = torch.cat([a * ang.cos() - b * ang.sin(), b * ang.cos() + a * ang.sin()], -1).float().bfloat16()
+        got = torch.cat([c.rows(kd.cpu(), i, t)[:, t - new:].transpose(0, 1) for i, t in enumerate(total)])
+        bad = int((got.double() != ref.double()).sum())
+        assert bad <= 2 + 1e-6 * ref.numel(), f"{bad} of {ref.numel()}"

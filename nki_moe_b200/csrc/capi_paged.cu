@@ -237,14 +237,26 @@ int nkimoe_copy_pages(void* pages, int64_t planes, int64_t num_pages, int64_t pa
                 "pair %lld: page %d -> %d of %lld", (long long)i, src[i], dst[i], (long long)num_pages);
   // the copies run at the same time: a page that is written must be written
   // once and read by none
+  // (1566 pairs in a pool of 3151: 2 us by a mark per page, 145 us by sorting,
+  // which is left for pools so large that clearing the marks would cost more)
   try {
-    std::vector<int32_t> to(dst, dst + n), from(src, src + n);
-    std::sort(to.begin(), to.end());
-    for (int64_t i = 1; i < n; ++i)
-      NKI_REQUIRE(to[i] != to[i - 1], NKIMOE_ERR_INVALID_ARG, "page %d is written twice", to[i]);
-    for (int32_t f : from)
-      NKI_REQUIRE(!std::binary_search(to.begin(), to.end(), f), NKIMOE_ERR_INVALID_ARG,
-                  "page %d is both read and written", f);
+    if (num_pages <= 256 * n + (1 << 16)) {
+      std::vector<char> written(static_cast<size_t>(num_pages), 0);
+      for (int64_t i = 0; i < n; ++i) {
+        NKI_REQUIRE(!written[dst[i]], NKIMOE_ERR_INVALID_ARG, "page %d is written twice", dst[i]);
+        written[dst[i]] = 1;
+      }
+      for (int64_t i = 0; i < n; ++i)
+        NKI_REQUIRE(!written[src[i]], NKIMOE_ERR_INVALID_ARG, "page %d is both read and written", src[i]);
+    } else {
+      std::vector<int32_t> to(dst, dst + n);
+      std::sort(to.begin(), to.end());
+      for (int64_t i = 1; i < n; ++i)
+        NKI_REQUIRE(to[i] != to[i - 1], NKIMOE_ERR_INVALID_ARG, "page %d is written twice", to[i]);
+      for (int64_t i = 0; i < n; ++i)
+        NKI_REQUIRE(!std::binary_search(to.begin(), to.end(), src[i]), NKIMOE_ERR_INVALID_ARG,
+                    "page %d is both read and written", src[i]);
+    }
   } catch (...) {
     return fail(NKIMOE_ERR_INVALID_ARG, "out of host memory");
   }

@@ -8,6 +8,7 @@ host buffers of :func:`moe_block_host`, whose block runs on the GPU.
 
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 import os
@@ -517,6 +518,12 @@ def paged_prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
 
 
 def _page_ids(ids, name: str) -> torch.Tensor:
+    if isinstance(ids, (list, tuple)):
+        try:
+            ids = array.array("i", ids)
+        except (TypeError, OverflowError) as e:
+            raise ValueError(f"{name} holds what is no page id: {e}") from None
+        return torch.frombuffer(ids, dtype=torch.int32) if len(ids) else torch.empty(0, dtype=torch.int32)
     t = torch.as_tensor(ids)
     if t.is_cuda or t.dim() != 1 or (t.numel() and t.dtype not in (torch.int32, torch.int64)):
         raise ValueError(f"{name} must be a list or CPU vector of page ids (page bookkeeping is host data)")

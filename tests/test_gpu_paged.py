@@ -639,3 +639,18 @@ def test_kept_keys_are_the_rounded_ones():
         got = torch.cat([c.rows(kd.cpu(), i, t)[:, t - new:].transpose(0, 1) for i, t in enumerate(total)])
         bad = int((got.double() != ref.double()).sum())
         assert bad <= 2 + 1e-6 * ref.numel(), f"{bad} of {ref.numel()}"
+
+
+@pytest.mark.parametrize("pool,n", [(2000, 900), (70000, 3)])
+def test_copy_pages_takes_lists_tuples_and_vectors(pool, n):
+    g = torch.Generator().manual_seed(n)
+    at = torch.randperm(pool, generator=g)[:2 * n]
+    want = torch.randn(pool, 1, 16, 8, generator=g).bfloat16().cuda()
+    start = want.clone()
+    want[at[n:].cuda()] = want[at[:n].cuda()]
+    for form in (list, tuple, torch.tensor, lambda x: torch.tensor(x, dtype=torch.int32)):
+        got = start.clone()
+        ops.copy_pages(got, form(at[:n].tolist()), form(at[n:].tolist()))
+        assert torch.equal(got, want)
+    ops.copy_pages(got, [], ())
+    assert torch.equal(got, want)

@@ -254,3 +254,13 @@ def test_entry_points_refuse_cpu_tensors():
 def test_a_cache_refuses_other_page_sizes(size):
     with pytest.raises(ValueError):
         PagedKVCache(1, 1, 4, size, 64, device="cpu")
+
+
+@pytest.mark.parametrize("pool", [5, 70000, 2 ** 30])
+def test_pages_written_twice_or_read_and_written_are_refused_in_pools_of_any_size(pool):
+    def ids(*x):
+        return (ctypes.c_int32 * len(x))(*x)
+
+    last = pool - 1
+    for src, dst in (((0, 1), (2, 2)), ((0, last), (last, 3)), ((last,), (last,)), ((pool,), (0,)), ((0,), (-1,))):
+        assert code("nkimoe_copy_pages", SOME, 2, pool, 4096, ids(*src), ids(*dst), len(src), NULL) == _lib.ERR_INVALID_ARG

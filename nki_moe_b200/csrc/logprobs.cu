@@ -257,7 +257,8 @@ constexpr int kLpShow = 32 / kLpWarps;  // keys that each warp shows the others
 struct TopShared {
   int2 list[kLpWarps][32];
   int2 cand[kLpWarps][64];  // a warp's candidates that are not in its list yet
-  int seen[32];             // keys of elements seen, kLpShow of each warp
+  int first[32];            // the first chunk's largest keys of eight lanes each
+  int seen[32];             // keys of elements seen, kLpShow of each warp (INT_MIN: none yet)
   int4 copy[kLpWarps][8];
 };
 
@@ -275,12 +276,16 @@ __device__ __forceinline__ void join_warps(TopShared& sh, WarpTop& best, int war
   }
 }
 
-// The n-th largest of the keys that the warps show, as one warp finds them (an
-// older state of some only lowers it): `n` elements reach it.  A few places by
-// one maximum each, more by the keys' ranks (8000 rows of 32000 with 5
-// alternatives 140 us against 144, 2000 rows of 151936 with 20 148 against 169).
-__device__ __forceinline__ int nth_seen(TopShared& sh, int n, int warp, int lane) {
-  int mine = *static_cast<volatile int*>(&sh.seen[lane]);
+// The n-th largest of 32 keys that the warps show (`keys`: sh.first or sh.seen),
+// as one warp finds them: `n` elements reach it.  The warps write sh.seen while
+// others read it, so a reader may find any mix of older and newer keys; the
+// keys of a mix are still those of different elements, since an element has one
+// slot for good (show_best), and an older key only lowers the bound.
+// A few places by one maximum each, more by the keys' ranks (8000 rows of 32000
+// with 5 alternatives 140 us against 144, 2000 rows of 151936 with 20 148
+// against 169).
+__device__ __forceinline__ int nth_shown(TopShared& sh, const volatile int* keys, int n, int warp, int lane) {
+  int mine = keys[lane];
   if (n <= 8) {
     for (;;) {
       const int v = __reduce_max_sync(0xffffffffu, mine);
@@ -298,6 +303,34 @@ __device__ __forceinline__ int nth_seen(TopShared& sh, int n, int warp, int lane
     above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
   }
   return __reduce_min_sync(0xffffffffu, above < n ? mine : INT_MAX);
+}
+
+// Shows the keys of the warp's best kLpShow elements in its slots of sh.seen; lane
+// i < kLpShow holds the id of what slot i shows (negative: nothing).  What is
+// among the best stays in its slot, what has come in takes the slot of what has
+// dropped out.  What has dropped out never comes back (the best only get better),
+// so no element is ever in two slots, at whatever times they are read.
+__device__ __forceinline__ void show_best(TopShared& sh, const WarpTop& best, int& shown, int warp, int lane) {
+  bool stays = false, known = false;  // this lane's slot, this lane's place in the list
+#pragma unroll
+  for (int i = 0; i < kLpShow; ++i) {
+    stays |= __shfl_sync(0xffffffffu, best.id, i) == shown;
+    known |= __shfl_sync(0xffffffffu, shown, i) == best.id;
+  }
+  const unsigned slots = __ballot_sync(0xffffffffu, lane < kLpShow && !stays);
+  unsigned places = __ballot_sync(0xffffffffu, lane < kLpShow && !known && best.key != INT_MIN);
+  if (places == 0) return;
+  // the i-th free slot takes the i-th new element
+  const int turn = __popc(slots & ((1u << lane) - 1u));
+#pragma unroll
+  for (int i = 0; i + 1 < kLpShow; ++i)
+    if (i < turn) places &= places - 1;
+  const int from = places ? __ffs(places) - 1 : 0;
+  const int key = __shfl_sync(0xffffffffu, best.key, from), id = __shfl_sync(0xffffffffu, best.id, from);
+  if ((slots >> lane & 1u) && places) {
+    shown = id;
+    *static_cast<volatile int*>(&sh.seen[warp * kLpShow + lane]) = key;
+  }
 }
 
 // Which of a thread's elements may reach the key `least`: bit i for word i
@@ -346,23 +379,28 @@ __device__ __forceinline__ uint32_t word_of(const uint4 (&raw)[kLpVecs], int w) 
 // one vote.  Where one may, the bound is drawn up to what the CTA's warps have
 // seen by then; elements of this warp's own come after all that its list holds,
 // so they lose ties there.  In the row's first chunk the warps show the largest
-// values of eight lanes each and wait for one another.
+// values of eight lanes each and wait for one another; that bound stays in `least`.
 template <typename T>
-__device__ __forceinline__ void warp_top(TopShared& sh, WarpTop& best, const uint4 (&raw)[kLpVecs], float mx, int& least,
-                                         long long base, bool first, int lo, int hi, int top, int warp, int lane) {
+__device__ __forceinline__ void warp_top(TopShared& sh, WarpTop& best, int& shown, const uint4 (&raw)[kLpVecs], float mx,
+                                         int& least, long long base, bool first, int lo, int hi, int top, int warp,
+                                         int lane) {
   constexpr int VE = LpVec<T>::VE;
   const int mk = order_key(mx);  // (what lies outside the row counts as -inf, which only lowers the bound)
   if (first) {
     int k = mk;
 #pragma unroll
     for (int d = 1; d < 32 / kLpShow; d <<= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, d));
-    if (lane % (32 / kLpShow) == 0) sh.seen[threadIdx.x / (32 / kLpShow)] = k;
+    if (lane % (32 / kLpShow) == 0) {
+      sh.first[threadIdx.x / (32 / kLpShow)] = k;
+      sh.seen[threadIdx.x / (32 / kLpShow)] = INT_MIN;
+    }
     __syncthreads();
   } else if (!__any_sync(0xffffffffu, mk >= least)) {
     return;
   }
   const int worst = __shfl_sync(0xffffffffu, best.key, top - 1);
-  least = max(max(least, nth_seen(sh, top, warp, lane)), worst == 0x7fffffff || worst == INT_MIN ? worst : worst + 1);
+  least = max(max(least, nth_shown(sh, first ? sh.first : sh.seen, top, warp, lane)),
+              worst == 0x7fffffff || worst == INT_MIN ? worst : worst + 1);
   unsigned mine = mk >= least ? may_reach<T>(raw, least) : 0;
   if (!__any_sync(0xffffffffu, mine != 0)) return;
   int2* const cand = sh.cand[warp];
@@ -398,11 +436,7 @@ __device__ __forceinline__ void warp_top(TopShared& sh, WarpTop& best, const uin
       n = max(n - 32, 0);
     }
   }
-  // (the lanes' largest values of the first chunk may be others than the list's first)
-  if (lane < kLpShow) {
-    volatile int* at = &sh.seen[warp * kLpShow + lane];
-    *at = best.key;
-  }
+  show_best(sh, best, shown, warp, lane);
 }
 
 // CTA (split, row): elements [split * per_split, ...) of the row in chunks of
@@ -447,7 +481,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LpP
   Stat st{-INFINITY, 0.f, 0.f};
   WarpTop best;
   best.clear(lane);
-  int least = INT_MIN;
+  int least = INT_MIN, shown = -1;
   for (long long base = first; base < hi; base += LpVec<T>::Chunk) {
 #pragma unroll
     for (int v = 0; v < kLpVecs; ++v) raw[v] = next[v];
@@ -487,7 +521,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LpP
     }
     stat_join(st, c);
     if constexpr (kTop) {
-      warp_top<T>(sh, best, raw, mx, least, base, base == first, lo, hi, p.top, warp, lane);
+      warp_top<T>(sh, best, shown, raw, mx, least, base, base == first, lo, hi, p.top, warp, lane);
     }
   }
   st = stat_warp(st);

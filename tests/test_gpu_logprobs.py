@@ -159,3 +159,15 @@ def test_orders_within_whole_rows(dtype, n):
     x[550:600] = -torch.inf
     x[550:600, ::911] = 0.5
     check(x.to(dtype), torch.randint(V, (T,), generator=g, device="cuda"), n)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 6, 17, 32])
+def test_alternatives_of_rows_whose_best_keep_changing(dtype, n):
+    """Every chunk of the row holds new best tokens of every warp, so what the warps
+    show each other changes all the time."""
+    T, V = 640, 40003
+    g = torch.Generator(device="cuda").manual_seed(7 + n)
+    x = torch.randn(T, V, generator=g, device="cuda") + torch.arange(V, device="cuda") / 1000
+    x[::3] = (4 * x[::3]).round() / 4  # and ties among them
+    check(x.to(dtype), torch.randint(V, (T,), generator=g, device="cuda"), n)

@@ -175,8 +175,13 @@ __device__ __forceinline__ float max_of(const uint4 (&raw)[kLpVecs]) {
   }
 }
 
+// Maxima below this take the short way through the sums: the distance of the
+// lowest finite value from them is still finite in both types (from 1.02e31 on
+// fp32's, from 1.3e36 on bf16's rounds to -inf, and 0 times that is NaN).
+constexpr float kLpFar = 1e30f;
+
 // A pair of neighbouring elements as fp32, -inf raised to the type's lowest
-// finite value (so that 0 times its distance from the maximum is 0).
+// finite value (so that 0 times its distance from a maximum below kLpFar is 0).
 template <typename T, int P>
 __device__ __forceinline__ uint64_t pair_of(const uint4& u) {
   if constexpr (sizeof(T) == 2) {
@@ -488,7 +493,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LpP
     if (base + LpVec<T>::Chunk < hi) load_chunk<T>(row, base + LpVec<T>::Chunk, lo, hi, next);
     const float mx = max_of<T>(raw);
     Stat c{mx, 0.f, 0.f};
-    if (mx > __uint_as_float(0xff7fffffu) && mx < 1e37f) {
+    if (mx > __uint_as_float(0xff7fffffu) && mx < kLpFar) {
       uint64_t s2[2] = {0, 0}, t2[2] = {0, 0};  // short chains
       const uint64_t nm = pair2(-mx, -mx);
 #pragma unroll

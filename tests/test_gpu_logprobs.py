@@ -171,3 +171,33 @@ def test_alternatives_of_rows_whose_best_keep_changing(dtype, n):
     x = torch.randn(T, V, generator=g, device="cuda") + torch.arange(V, device="cuda") / 1000
     x[::3] = (4 * x[::3]).round() / 4  # and ties among them
     check(x.to(dtype), torch.randint(V, (T,), generator=g, device="cuda"), n)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [500, 8192, 20011])
+@pytest.mark.parametrize("n", [0, 5])
+def test_large_maxima(dtype, V, n):
+    """A logit far above the others, of any size that the type holds, with and without
+    excluded tokens next to it: all the weight lies on it, or half where there are two.
+    Results are fp32: what lies further out than the type reaches, the log probability of a
+    token masked with the lowest value under a maximum of 3e38, is -inf, as its rounding is."""
+    tops = [1e29, 9e29, 1e31, 2e31, 1e32, 1e36, 1.5e36, 9e36, 1.1e37, 1e38, 3e38]
+    x = torch.zeros(4 * len(tops), V, device="cuda")
+    for i, m in enumerate(tops):
+        x[4 * i:4 * i + 4, V // 3] = m
+        x[4 * i + 1, ::7] = -torch.inf
+        x[4 * i + 2, V - 2] = m
+        x[4 * i + 3, 1::2] = torch.finfo(dtype).min
+        x[4 * i:4 * i + 4, V // 3] = m
+    x, tok = x.to(dtype), torch.arange(4 * len(tops), device="cuda") % V
+    lp, ent, tlp, tid = (t.cpu() for t in ops.token_logprobs(x, tok, n))
+    ref = torch.log_softmax(x.double().cpu(), -1)
+    p = ref.exp()
+    ids = torch.sort(x.cpu().double(), dim=-1, descending=True, stable=True).indices[:, :n]
+    assert torch.equal(tid, ids)
+    for got, want in ((lp, ref.gather(-1, tok.cpu()[:, None])[:, 0]), (tlp, ref.gather(-1, ids))):
+        want = want.float().double()
+        far = torch.isinf(want)
+        assert torch.equal(got.double()[far], want[far])
+        assert ((got.double() - want).abs()[~far] <= LP + 2 ** -22 * want.abs()[~far]).all()
+    assert ((ent.double() + (p * torch.where(p > 0, ref, torch.zeros_like(ref))).sum(-1)).abs() <= ENT).all()

@@ -175,13 +175,14 @@ __device__ __forceinline__ float max_of(const uint4 (&raw)[kLpVecs]) {
   }
 }
 
-// Maxima below this take the short way through the sums: the distance of the
-// lowest finite value from them is still finite in both types (from 1.02e31 on
-// fp32's, from 1.3e36 on bf16's rounds to -inf, and 0 times that is NaN).
+// Maxima between -this and this take the short way through the sums, which
+// raises -inf to the lowest finite value.  Above, that value's distance from the
+// maximum would round to -inf (from 1.02e31 on in fp32, from 1.3e36 on in bf16),
+// and 0 times that is NaN; below, it would come near the maximum itself and count.
 constexpr float kLpFar = 1e30f;
 
 // A pair of neighbouring elements as fp32, -inf raised to the type's lowest
-// finite value (so that 0 times its distance from a maximum below kLpFar is 0).
+// finite value (so that 0 times its distance from a maximum within kLpFar is 0).
 template <typename T, int P>
 __device__ __forceinline__ uint64_t pair_of(const uint4& u) {
   if constexpr (sizeof(T) == 2) {
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LpP
     if (base + LpVec<T>::Chunk < hi) load_chunk<T>(row, base + LpVec<T>::Chunk, lo, hi, next);
     const float mx = max_of<T>(raw);
     Stat c{mx, 0.f, 0.f};
-    if (mx > __uint_as_float(0xff7fffffu) && mx < kLpFar) {
+    if (fabsf(mx) < kLpFar) {
       uint64_t s2[2] = {0, 0}, t2[2] = {0, 0};  // short chains
       const uint64_t nm = pair2(-mx, -mx);
 #pragma unroll
@@ -509,7 +510,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LpP
       c.s = s.x + s.y;
       c.t = t.x + t.y;
     } else if (mx != -INFINITY) {
-      // a NaN, an infinity, or values whose distance from the maximum may overflow
+      // a NaN, +inf, or a maximum so far out that -inf has to stay what it is
 #pragma unroll 1
       for (int v = 0; v < kLpVecs; ++v) {
         float x[LpVec<T>::VE];

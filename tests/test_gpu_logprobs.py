@@ -201,3 +201,20 @@ def test_large_maxima(dtype, V, n):
         assert torch.equal(got.double()[far], want[far])
         assert ((got.double() - want).abs()[~far] <= LP + 2 ** -22 * want.abs()[~far]).all()
     assert ((ent.double() + (p * torch.where(p > 0, ref, torch.zeros_like(ref))).sum(-1)).abs() <= ENT).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [5, 500, 8192, 20011])
+def test_rows_of_the_lowest_values(dtype, V):
+    """Rows whose largest logit is the type's lowest finite value, or next to it: the tokens
+    that share it are equally likely, excluded ones and places outside the row count for nothing."""
+    low = torch.finfo(dtype).min
+    x = torch.full((6, V), low, device="cuda", dtype=dtype)
+    x[1, ::2] = -torch.inf
+    x[2, :] = -torch.inf
+    x[2, V - 1] = low
+    x[3, 1] = torch.tensor(low, dtype=dtype) * (1 - torch.finfo(dtype).eps)
+    x[4] = -1e31
+    x[5, 2:4] = -2e30
+    for top_n in (0, min(V, 7)):
+        check(x, torch.tensor([0, 1, V - 1, 1, 2, 3], device="cuda"), top_n)

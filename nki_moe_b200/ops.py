@@ -257,6 +257,7 @@ def skinny_linear(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = N
 _paged_ws: dict = {}
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _PAGE_SIZES = (16, 32, 64, 128, 256)
+_STATUS_BYTES = 4  # the status word at the head of a workspace
 
 
 @functools.lru_cache(maxsize=512)
@@ -270,7 +271,8 @@ def _paged_workspace(dev: torch.device, stream: int, nbytes: int) -> torch.Tenso
     (device, stream).  A stream that is being captured gets one per capture,
     allocated (and zeroed, as a node of the graph) in the graph's own memory,
     so graphs that replay at the same time share none; only the latest
-    capture's is held here, the graph keeps the memory."""
+    capture's is held here, the graph keeps the memory.  A larger workspace
+    takes over the status of the one that it replaces."""
     capture = 0
     if torch.cuda.is_current_stream_capturing():
         cid = ctypes.c_ulonglong(0)
@@ -281,9 +283,14 @@ def _paged_workspace(dev: torch.device, stream: int, nbytes: int) -> torch.Tenso
     if held is not None and held[0] == capture and held[1].numel() >= nbytes:
         return held[1]
     with _ws_lock:
-        held = (capture, torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=dev))
-        _paged_ws[key] = held
-        return held[1]
+        held = _paged_ws.get(key)  # again: another thread may have been here
+        if held is not None and held[0] == capture and held[1].numel() >= nbytes:
+            return held[1]
+        ws = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=dev)
+        if held is not None and held[0] == capture:  # a smaller one: what it has reported goes on
+            ws[:_STATUS_BYTES].copy_(held[1][:_STATUS_BYTES])
+        _paged_ws[key] = (capture, ws)
+        return ws
 
 
 def read_paged_status(device=None) -> None:

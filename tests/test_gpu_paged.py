@@ -654,3 +654,46 @@ def test_copy_pages_takes_lists_tuples_and_vectors(pool, n):
         assert torch.equal(got, want)
     ops.copy_pages(got, [], ())
     assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------ status
+def test_reports_survive_a_larger_workspace(monkeypatch):
+    """A bad row is reported after a later, larger call of the stream too, in a captured graph as well."""
+    monkeypatch.setenv("NKIMOE_SYNC_CHECK", "0")
+    nq, nkv = 4, 2
+    pages = torch.zeros(64, nkv, 256, HD, dtype=torch.bfloat16, device="cuda")
+    qkv = torch.randn(8, (nq + 2 * nkv) * HD, device="cuda").bfloat16()
+    w = torch.ones(HD, dtype=torch.bfloat16, device="cuda")
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    cu, table = i32(0, 8), torch.arange(64, dtype=torch.int32, device="cuda")[None]
+    logits, tokens = torch.randn(8, 60000, device="cuda"), torch.zeros(8, dtype=torch.int64, device="cuda")
+    lens, far = i32(9000), i32(100_000)
+
+    def calls(kv):
+        q = ops.qk_norm_rope_store(qkv, w, w, cu, kv, pages, pages, table, nq, nkv)  # 100000 has no place
+        ops.paged_prefill_attention(q, pages, pages, table, cu, lens)
+        ops.token_logprobs(logits, tokens, 5)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    fresh = [k for k in ops._paged_ws if k[1] == side.cuda_stream]
+    for k in fresh:  # as on a stream that no call has used
+        del ops._paged_ws[k]
+    with torch.cuda.stream(side):
+        calls(far)
+    with pytest.raises(NKIMoEError):
+        ops.read_paged_status()
+    ops.read_paged_status()
+    with torch.cuda.stream(side):
+        calls(lens)
+    ops.read_paged_status()
+    kv = lens.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        calls(kv)
+    g.replay()
+    ops.read_paged_status()
+    kv.copy_(far)
+    g.replay()
+    with pytest.raises(NKIMoEError):
+        ops.read_paged_status()

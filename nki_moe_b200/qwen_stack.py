@@ -128,7 +128,8 @@ class Qwen3MoEStack:
         ``E / P`` experts, and runs each layer's MoE as a peer-memory
         expert-parallel block over its own sequences (``max_batch`` of them,
         up to ``max_seq`` tokens each).  Every rank must run the same calls
-        (prefill, decode steps) in the same order."""
+        (prefill, decode steps) in the same order; the batches of the paged
+        calls may differ."""
         dev = torch.device(device)
         g = torch.Generator(device=dev).manual_seed(seed)
         H, hd = cfg.hidden_size, cfg.head_dim
@@ -428,7 +429,9 @@ class Qwen3MoEStack:
         """One decode step: ``tokens[i]`` appended to sequence ``seqs[i]``.
         Returns logits ``[len(seqs), V]`` (a tensor of its own).  With
         ``graph`` the step is captured once per cache and batch size; lengths
-        and pages are device data."""
+        and pages are device data.  The call that captures runs the step
+        itself and the capture runs nothing, so that every call runs each
+        layer's expert-parallel exchange once, whatever a rank's batch does."""
         B = len(seqs)
         if tokens.numel() != B:
             raise ValueError(f"{tokens.numel()} tokens for {B} sequences")
@@ -450,20 +453,22 @@ class Qwen3MoEStack:
             step["tokens"].copy_(tokens.reshape(-1))
             step["positions"].copy_(positions)
             step["table"].copy_(table)
-            if "graph" not in step:
+            if "graph" in step:
+                step["graph"].replay()
+                out = step["out"].clone()
+            else:
                 s = torch.cuda.Stream(device=self.device)
                 s.wait_stream(torch.cuda.current_stream(self.device))
-                # warm up on the capture stream; what this writes the replay writes again
+                # this call's step, on the capture stream (workspaces are sized outside the capture)
                 with torch.cuda.stream(s):
-                    self._paged_body(cache, step["tokens"], step["positions"], step["table"])
+                    out = self._paged_body(cache, step["tokens"], step["positions"], step["table"])
                 torch.cuda.current_stream(self.device).wait_stream(s)
+                out = out.clone()
                 g = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(g, stream=s):
                     step["out"] = self._paged_body(cache, step["tokens"], step["positions"], step["table"])
                 step["graph"] = g
                 self._paged = step
-            step["graph"].replay()
-            out = step["out"].clone()
         for q in seqs:
             cache.trim(q)
         return out

@@ -194,3 +194,40 @@ def test_generation_keeps_no_cache_of_its_own(pair):
     with pytest.raises(ValueError):
         st.score(prompts, chunk=-1)
     st.release_graph()
+
+
+class _Counted:
+    """An expert block in the place of a layer's exchange: what runs on the device is counted there."""
+
+    def __init__(self, lyr, top_k):
+        from nki_moe_b200 import ops
+
+        self.count = torch.zeros(1, dtype=torch.int64, device="cuda")
+        self.block = lambda x: ops.moe_block(x, lyr.router_w, lyr.experts, top_k, router_w_split=lyr.router_split)
+
+    def __call__(self, x):
+        self.count.add_(1)
+        return self.block(x)
+
+    def close(self):
+        pass
+
+
+def test_a_call_runs_each_exchange_once():
+    """Ranks of an expert-parallel stack stay in step whatever their batches do: a call runs
+    each layer's exchange once, whether it captures a step, replays one or neither."""
+    from nki_moe_b200.qwen_stack import Qwen3MoEStack
+
+    st = Qwen3MoEStack.from_hf(tiny_hf(), max_batch=4, max_seq=256)
+    for lyr in st.layers:
+        lyr.ep, lyr.ep_decode = _Counted(lyr, st.cfg.num_experts_per_tok), _Counted(lyr, st.cfg.num_experts_per_tok)
+    cache = st.paged_cache(20, page_size=16)
+    seqs = [cache.add() for _ in range(4)]
+    calls = 0
+    st.prefill_paged(cache, seqs, [ids(5, 1)] * 4)
+    for B, graph in ((4, True), (4, True), (3, True), (4, True), (2, False), (3, True), (1, True), (1, True)):
+        st.decode_paged(cache, seqs[:B], ids(B, calls), graph=graph)
+        calls += 1
+        for lyr in st.layers:
+            assert int(lyr.ep_decode.count) == calls and int(lyr.ep.count) == 1
+    st.close()

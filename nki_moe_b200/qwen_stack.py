@@ -34,6 +34,8 @@ from __future__ import annotations
 
 import math
 import time
+import weakref
+from collections import OrderedDict
 from dataclasses import dataclass
 
 import torch
@@ -89,6 +91,8 @@ class _Layer:
 class Qwen3MoEStack:
     """bf16 Qwen3-MoE causal LM: prefill, static-shape decode, greedy generate."""
 
+    PAGED_STEPS = 32  # captured paged steps (batch sizes) that are kept of each cache
+
     def __init__(self, cfg: Qwen3MoEConfig, embed: torch.Tensor, layers: list[_Layer], final_norm: torch.Tensor,
                  lm_head: torch.Tensor, max_batch: int, max_seq: int):
         self.cfg = cfg
@@ -105,7 +109,12 @@ class Qwen3MoEStack:
         self._graph = None
         self._graph_batch = None
         self._graph_out = None
-        self._paged = None  # the captured paged decode step: its cache, batch, buffers and graph
+        # the captured paged decode steps: of each cache in use, its buffers and graph by batch size, the
+        # last used last (a cache that is gone takes its steps along); and which was used last
+        self._paged_steps: weakref.WeakKeyDictionary[PagedKVCache, OrderedDict] = weakref.WeakKeyDictionary()
+        self._paged_last = None
+        # the steps share their capture stream's workspaces, so one begins when the one before has ended
+        self._paged_stream = self._paged_done = None
         # the skinny linear kernel takes N % 16 == 0 and K % 32 == 0
         H, hd = cfg.hidden_size, cfg.head_dim
         nq, nkv = cfg.num_attention_heads, cfg.num_key_value_heads
@@ -359,7 +368,21 @@ class Qwen3MoEStack:
 
     def release_graph(self):
         self._graph = self._graph_out = None
-        self._paged = None
+        for cache in list(self._paged_steps):
+            self._drop_steps(cache)
+
+    def _drop_steps(self, cache: PagedKVCache):
+        """Ends the captured steps of a cache."""
+        self._paged_steps.pop(cache, None)
+
+    @property
+    def _paged(self):
+        """The captured paged step that was used last and its cache, or None."""
+        if self._paged_last is None:
+            return None
+        cache, B = self._paged_last[0](), self._paged_last[1]
+        step = None if cache is None else self._paged_steps.get(cache, {}).get(B)
+        return None if step is None else {"cache": cache, "B": B, **step}
 
     # ------------------------------------------------------------ paged cache
     def paged_cache(self, num_pages: int, page_size: int = 64, max_seq: int | None = None, window: int = 0,
@@ -428,8 +451,9 @@ class Qwen3MoEStack:
     def decode_paged(self, cache: PagedKVCache, seqs, tokens: torch.Tensor, graph: bool = True) -> torch.Tensor:
         """One decode step: ``tokens[i]`` appended to sequence ``seqs[i]``.
         Returns logits ``[len(seqs), V]`` (a tensor of its own).  With
-        ``graph`` the step is captured once per cache and batch size; lengths
-        and pages are device data.  The call that captures runs the step
+        ``graph`` the step is captured once per cache and batch size (the
+        ``PAGED_STEPS`` sizes used last are kept); lengths and pages are device
+        data.  The call that captures runs the step
         itself and the capture runs nothing, so that every call runs each
         layer's expert-parallel exchange once, whatever a rank's batch does."""
         B = len(seqs)
@@ -440,14 +464,18 @@ class Qwen3MoEStack:
         cache.extend(seqs, [1] * B)
         positions = torch.tensor([cache.length(q) - 1 for q in seqs])
         table = cache.table(seqs)
-        step = self._paged
         if not graph:
             out = self._paged_body(cache, tokens.reshape(-1).to(self.device), positions.to(self.device),
                                    table.to(self.device))
         else:
-            if step is None or step["cache"] is not cache or step["B"] != B:
-                step = {"cache": cache, "B": B,
-                        "tokens": torch.zeros(B, dtype=torch.int64, device=self.device),
+            here = torch.cuda.current_stream(self.device)
+            if self._paged_done is None:
+                self._paged_stream, self._paged_done = torch.cuda.Stream(device=self.device), torch.cuda.Event()
+            here.wait_event(self._paged_done)
+            steps = self._paged_steps.setdefault(cache, OrderedDict())
+            step = steps.get(B)
+            if step is None:
+                step = {"tokens": torch.zeros(B, dtype=torch.int64, device=self.device),
                         "positions": torch.zeros(B, dtype=torch.int64, device=self.device),
                         "table": torch.zeros(B, cache.max_pages, dtype=torch.int32, device=self.device)}
             step["tokens"].copy_(tokens.reshape(-1))
@@ -456,19 +484,26 @@ class Qwen3MoEStack:
             if "graph" in step:
                 step["graph"].replay()
                 out = step["out"].clone()
+                steps.move_to_end(B)
             else:
-                s = torch.cuda.Stream(device=self.device)
-                s.wait_stream(torch.cuda.current_stream(self.device))
+                s = self._paged_stream
+                s.wait_stream(here)
                 # this call's step, on the capture stream (workspaces are sized outside the capture)
-                with torch.cuda.stream(s):
-                    out = self._paged_body(cache, step["tokens"], step["positions"], step["table"])
-                torch.cuda.current_stream(self.device).wait_stream(s)
+                try:
+                    with torch.cuda.stream(s):
+                        out = self._paged_body(cache, step["tokens"], step["positions"], step["table"])
+                finally:
+                    here.wait_stream(s)
                 out = out.clone()
                 g = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(g, stream=s):
                     step["out"] = self._paged_body(cache, step["tokens"], step["positions"], step["table"])
                 step["graph"] = g
-                self._paged = step
+                steps[B] = step
+                if len(steps) > self.PAGED_STEPS:
+                    steps.popitem(last=False)
+            self._paged_done.record(here)
+            self._paged_last = (weakref.ref(cache), B)
         for q in seqs:
             cache.trim(q)
         return out
@@ -521,8 +556,8 @@ class Qwen3MoEStack:
             for q in seqs:
                 if q in cache:
                     cache.free(q)
-            if own and self._paged is not None and self._paged["cache"] is cache:
-                self._paged = None  # nobody else can use this cache: its pools go with the captured step
+            if own:
+                self._drop_steps(cache)  # nobody else can use this cache
         tokens = torch.stack(out, 1).view(n, samples, max_new_tokens)
         if top_logprobs is None:
             return tokens, None

@@ -231,3 +231,68 @@ def test_a_call_runs_each_exchange_once():
         for lyr in st.layers:
             assert int(lyr.ep_decode.count) == calls and int(lyr.ep.count) == 1
     st.close()
+
+
+def test_steps_of_several_batch_sizes_and_caches_are_kept(pair):
+    """A batch that grows and shrinks replays the steps that it captured before, with the
+    logits of steps that were never captured."""
+    _, st = pair
+    st.release_graph()
+    caches = [st.paged_cache(40, page_size=16) for _ in range(4)]  # 0, 1 with graphs; 2, 3 without
+    prompts = [ids(n, 80 + n) for n in (5, 20, 33)]
+    seqs = []
+    for c in caches:
+        seqs.append([c.add() for _ in prompts])
+        st.prefill_paged(c, seqs[-1], prompts)
+    graphs = {}
+    for i, (c, B) in enumerate(((0, 2), (0, 3), (1, 2), (0, 2), (1, 3), (0, 3), (0, 1), (1, 2), (0, 2), (1, 3), (0, 1))):
+        tok = ids(B, i)
+        got = st.decode_paged(caches[c], seqs[c][:B], tok)
+        want = st.decode_paged(caches[c + 2], seqs[c + 2][:B], tok, graph=False)
+        assert torch.equal(got, want), (c, B)
+        assert graphs.setdefault((c, B), st._paged["graph"]) is st._paged["graph"]
+    assert len({id(g) for g in graphs.values()}) == len(graphs) == 5
+    st.release_graph()
+    assert st._paged is None
+
+
+def test_the_steps_used_last_are_kept_and_those_of_a_cache_end_with_it(pair, monkeypatch):
+    _, st = pair
+    st.release_graph()
+    monkeypatch.setattr(type(st), "PAGED_STEPS", 2)
+    cache = st.paged_cache(20, page_size=16)
+    seqs = [cache.add() for _ in range(3)]
+    st.prefill_paged(cache, seqs, [ids(4, i) for i in range(3)])
+    for B, kept in ((1, [1]), (2, [1, 2]), (1, [2, 1]), (3, [1, 3]), (3, [1, 3]), (2, [3, 2])):
+        st.decode_paged(cache, seqs[:B], ids(B, B))
+        assert list(st._paged_steps[cache]) == kept
+    del cache
+    assert len(st._paged_steps) == 0 and st._paged is None
+
+
+def test_two_caches_on_two_streams(pair):
+    _, st = pair
+    st.release_graph()
+    prompts = [ids(n, 90 + n) for n in (30, 9)]
+
+    def start(c):
+        seqs = [c.add() for _ in prompts]
+        st.prefill_paged(c, seqs, prompts)
+        return seqs
+
+    caches = [st.paged_cache(20, page_size=16) for _ in range(2)]
+    seqs = [start(c) for c in caches]
+    toks = [ids(2, i).cuda() for i in range(24)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for i, tok in enumerate(toks):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(st.decode_paged(caches[i % 2], seqs[i % 2], tok))
+    torch.cuda.synchronize()
+    for k in range(2):
+        cache = st.paged_cache(20, page_size=16)
+        mine = start(cache)
+        for i in range(k, 24, 2):
+            assert torch.equal(got[i], st.decode_paged(cache, mine, toks[i], graph=False)), i
+    st.release_graph()

@@ -255,6 +255,7 @@ def skinny_linear(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = N
 
 # ---------------------------------------------------------------- paged cache, token scores
 _paged_ws: dict = {}
+_paged_sinks: list = []  # weak references to status words of graphs' owners
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _PAGE_SIZES = (16, 32, 64, 128, 256)
 _STATUS_BYTES = 4  # the status word at the head of a workspace
@@ -293,17 +294,44 @@ def _paged_workspace(dev: torch.device, stream: int, nbytes: int) -> torch.Tenso
         return ws
 
 
+def _status_sink(device: torch.device) -> torch.Tensor:
+    """A status word that collects what the replays of its owner's graphs report
+    (:func:`_end_of_capture`); :func:`read_paged_status` reads it while it lives."""
+    sink = torch.zeros(1, dtype=torch.int32, device=device)
+    with _ws_lock:
+        _paged_sinks[:] = [r for r in _paged_sinks if r() is not None] + [weakref.ref(sink)]
+    return sink
+
+
+def _end_of_capture(sink: torch.Tensor) -> list:
+    """Called last in a capture on the current stream, by the owner of the
+    graph: each replay ends by adding its paged calls' status to ``sink``.
+    Returns the workspaces that the capture uses; the owner holds them as long
+    as the graph, this module no longer than a next capture needs them."""
+    key = (sink.device.index, torch.cuda.current_stream(sink.device).cuda_stream)
+    with _ws_lock:
+        held = [table[key] for table in (_ws, _attn_ws) if key in table]
+        paged = _paged_ws.pop(key + (True,), None)
+    if paged is not None:
+        sink.bitwise_or_(paged[1][:_STATUS_BYTES].view(torch.int32))
+        held.append(paged[1])
+    return held
+
+
 def read_paged_status(device=None) -> None:
     """Synchronises ``device`` and raises if a paged-cache call on it met a
     position or page id out of range, or a page that it needed and that was
-    not held (the status is cleared).  Of calls in CUDA graphs it sees the
-    last replay of the graph captured last on each stream: a replay begins by
-    clearing its own status."""
+    not held (the status is cleared).  Of calls in a caller's own CUDA graphs it
+    sees the last replay of the graph captured last on each stream: a replay
+    begins by clearing its own status.  The decoder stack's captured steps
+    collect theirs, and every one is seen."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     index = torch.cuda.current_device() if dev.index is None else dev.index
     torch.cuda.synchronize(index)
     with _ws_lock:
         held = [v[1] for k, v in _paged_ws.items() if k[0] == index]
+        sinks = [r() for r in _paged_sinks]
+        held += [t for t in sinks if t is not None and t.get_device() == index]
     bad = None
     with torch.cuda.device(index):
         for ws in held:

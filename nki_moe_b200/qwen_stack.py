@@ -114,7 +114,7 @@ class Qwen3MoEStack:
         self._paged_steps: weakref.WeakKeyDictionary[PagedKVCache, OrderedDict] = weakref.WeakKeyDictionary()
         self._paged_last = None
         # the steps share their capture stream's workspaces, so one begins when the one before has ended
-        self._paged_stream = self._paged_done = None
+        self._paged_stream = self._paged_done = self._paged_status = None
         # the skinny linear kernel takes N % 16 == 0 and K % 32 == 0
         H, hd = cfg.hidden_size, cfg.head_dim
         nq, nkv = cfg.num_attention_heads, cfg.num_key_value_heads
@@ -471,6 +471,7 @@ class Qwen3MoEStack:
             here = torch.cuda.current_stream(self.device)
             if self._paged_done is None:
                 self._paged_stream, self._paged_done = torch.cuda.Stream(device=self.device), torch.cuda.Event()
+                self._paged_status = ops._status_sink(self.device)
             here.wait_event(self._paged_done)
             steps = self._paged_steps.setdefault(cache, OrderedDict())
             step = steps.get(B)
@@ -498,6 +499,7 @@ class Qwen3MoEStack:
                 g = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(g, stream=s):
                     step["out"] = self._paged_body(cache, step["tokens"], step["positions"], step["table"])
+                    step["workspaces"] = ops._end_of_capture(self._paged_status)
                 step["graph"] = g
                 steps[B] = step
                 if len(steps) > self.PAGED_STEPS:

@@ -296,3 +296,44 @@ def test_two_caches_on_two_streams(pair):
         for i in range(k, 24, 2):
             assert torch.equal(got[i], st.decode_paged(cache, mine, toks[i], graph=False)), i
     st.release_graph()
+
+
+def test_captured_steps_leave_nothing_behind(pair):
+    """What a captured step held goes with it; what it had reported does not."""
+    import gc
+
+    from nki_moe_b200 import ops
+    from nki_moe_b200._lib import NKIMoEError
+
+    _, st = pair
+    st.release_graph()
+    ops.release_captured_workspaces()
+    prompts = [ids(20, 1), ids(33, 2)]
+
+    def use():
+        st.generate_paged(prompts, 3, page_size=16)
+        gc.collect()  # what other tests left in cycles
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        return torch.cuda.memory_allocated(), torch.cuda.memory_reserved()
+
+    for _ in range(3):
+        use()
+    before = use()
+    for _ in range(4):
+        assert use() == before
+    assert not [k for k in ops._paged_ws if k[2]]
+    ops.read_paged_status()
+    cache = st.paged_cache(8, page_size=16)
+    seq = cache.add()
+    st.prefill_paged(cache, [seq], [prompts[1]])
+    st.decode_paged(cache, [seq], ids(1, 1))
+    st.decode_paged(cache, [seq], ids(1, 2))
+    page, cache._seqs[seq].pages[1] = cache._seqs[seq].pages[1], 10 ** 6  # no such page
+    st.decode_paged(cache, [seq], ids(1, 3))
+    cache._seqs[seq].pages[1] = page
+    st.decode_paged(cache, [seq], ids(1, 4))  # a good one after it
+    st.release_graph()
+    with pytest.raises(NKIMoEError):
+        ops.read_paged_status()
+    ops.read_paged_status()

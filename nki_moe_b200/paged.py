@@ -146,6 +146,19 @@ class PageTables:
                 s.pages.append(self._take())
         return copies
 
+    def take_back(self, seqs, lengths) -> None:
+        """Puts ``seqs[i]`` back to ``lengths[i]`` positions, as it had before an
+        :meth:`extend` whose positions were not written after all.  The pages
+        behind are given back; one that was made private stays so."""
+        seqs, lengths = list(seqs), list(lengths)
+        if len(seqs) != len(lengths) or any(not 0 <= n <= self.length(q) for q, n in zip(seqs, lengths)):
+            raise ValueError("one length, no larger than the sequence's, for each sequence")
+        for q, n in zip(seqs, lengths):
+            s = self._seqs[q]
+            while len(s.pages) > -(-n // self.page_size):
+                self._drop(s.pages.pop())
+            s.length = n
+
     def _take(self) -> int:
         page = heapq.heappop(self._free)
         self._refs[page] = 1

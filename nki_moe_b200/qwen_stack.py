@@ -32,6 +32,7 @@ decode step over all layers is captured into a single CUDA graph.
 
 from __future__ import annotations
 
+import contextlib
 import math
 import time
 import weakref
@@ -43,6 +44,25 @@ import torch.nn.functional as F
 
 from . import ops
 from .paged import PagedKVCache
+
+
+@contextlib.contextmanager
+def _appending(cache: PagedKVCache, seqs, counts):
+    """Extends the sequences; where what follows fails, they get their lengths back."""
+    seqs = list(seqs)
+    lengths = [cache.length(q) for q in seqs]
+    cache.extend(seqs, counts)
+    try:
+        yield
+    except BaseException:
+        cache.take_back(seqs, lengths)
+        raise
+
+
+def _token_ids(t: torch.Tensor) -> torch.Tensor:
+    if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
+        raise ValueError(f"token ids must be whole numbers, not {t.dtype}")
+    return t.reshape(-1)
 
 
 @dataclass
@@ -394,22 +414,15 @@ class Qwen3MoEStack:
                             window, sinks, self.device)
 
     def _prompt_hidden(self, cache: PagedKVCache, seqs, prompts) -> torch.Tensor:
-        """Runs the layers on new tokens of the sequences, packed, and returns
-        the final norm's rows ``[T, H]``."""
+        """Runs the layers on new tokens of the sequences, which the cache has
+        been extended by, packed, and returns the final norm's rows ``[T, H]``."""
         c = self.cfg
-        lens = [int(p.numel()) for p in prompts]
-        if len(prompts) != len(seqs) or not seqs or min(lens) == 0:
-            raise ValueError("one prompt, not empty, for each sequence")
-        if any(lyr.ep is not None for lyr in self.layers) and sum(lens) > self.max_batch * self.max_seq:
-            raise ValueError(f"{sum(lens)} tokens exceed the expert-parallel exchange "
-                             f"({self.max_batch} x {self.max_seq})")
-        cache.extend(seqs, lens)
         cu = torch.zeros(len(seqs) + 1, dtype=torch.int32)
-        cu[1:] = torch.tensor(lens).cumsum(0)
+        cu[1:] = torch.tensor([p.numel() for p in prompts]).cumsum(0)
         cu = cu.to(self.device)
         kv = torch.tensor([cache.length(q) for q in seqs], dtype=torch.int32).to(self.device)
         table = cache.table(seqs).to(self.device)
-        ids = torch.cat([p.reshape(-1).to(self.device) for p in prompts])
+        ids = torch.cat([_token_ids(p).to(self.device, torch.int64) for p in prompts])
         h = F.embedding(ids, self.embed)
 
         def attention(li, lyr, xn):
@@ -420,15 +433,28 @@ class Qwen3MoEStack:
 
         return self._layers(h, attention)
 
+    def _prompt_lengths(self, seqs, prompts) -> list[int]:
+        """The prompts' lengths, checked."""
+        lens = [int(_token_ids(p).numel()) for p in prompts]
+        if len(prompts) != len(seqs) or not seqs or min(lens) == 0:
+            raise ValueError("one prompt, not empty, for each sequence")
+        if any(lyr.ep is not None for lyr in self.layers) and sum(lens) > self.max_batch * self.max_seq:
+            raise ValueError(f"{sum(lens)} tokens exceed the expert-parallel exchange "
+                             f"({self.max_batch} x {self.max_seq})")
+        return lens
+
     @torch.inference_mode()
     def prefill_paged(self, cache: PagedKVCache, seqs, prompts) -> torch.Tensor:
         """Appends ``prompts[i]`` (token ids, any lengths) to sequence
         ``seqs[i]`` of the cache, which may hold the beginning already (a
         prompt in chunks, or one that continues a fork).  Returns the logits
-        of each prompt's last token ``[len(seqs), V]``."""
-        hn = self._prompt_hidden(cache, seqs, prompts)
-        last = torch.tensor([int(p.numel()) for p in prompts]).cumsum(0) - 1
-        logits = F.linear(hn[last.to(self.device)], self.lm_head)
+        of each prompt's last token ``[len(seqs), V]``.  Where the call fails,
+        the sequences keep their lengths."""
+        lens = self._prompt_lengths(seqs, prompts)
+        with _appending(cache, seqs, lens):
+            hn = self._prompt_hidden(cache, seqs, prompts)
+            last = torch.tensor(lens).cumsum(0) - 1
+            logits = F.linear(hn[last.to(self.device)], self.lm_head)
         for q in seqs:
             cache.trim(q)
         return logits
@@ -455,59 +481,67 @@ class Qwen3MoEStack:
         ``PAGED_STEPS`` sizes used last are kept); lengths and pages are device
         data.  The call that captures runs the step
         itself and the capture runs nothing, so that every call runs each
-        layer's expert-parallel exchange once, whatever a rank's batch does."""
+        layer's expert-parallel exchange once, whatever a rank's batch does.
+        Where the call fails, the sequences keep their lengths."""
         B = len(seqs)
         if tokens.numel() != B:
             raise ValueError(f"{tokens.numel()} tokens for {B} sequences")
         if any(lyr.ep is not None for lyr in self.layers) and B > self.max_batch:
             raise ValueError(f"batch {B} exceeds the expert-parallel exchange ({self.max_batch})")
-        cache.extend(seqs, [1] * B)
-        positions = torch.tensor([cache.length(q) - 1 for q in seqs])
-        table = cache.table(seqs)
-        if not graph:
-            out = self._paged_body(cache, tokens.reshape(-1).to(self.device), positions.to(self.device),
-                                   table.to(self.device))
-        else:
-            here = torch.cuda.current_stream(self.device)
-            if self._paged_done is None:
-                self._paged_stream, self._paged_done = torch.cuda.Stream(device=self.device), torch.cuda.Event()
-                self._paged_status = ops._status_sink(self.device)
-            here.wait_event(self._paged_done)
-            steps = self._paged_steps.setdefault(cache, OrderedDict())
-            step = steps.get(B)
-            if step is None:
-                step = {"tokens": torch.zeros(B, dtype=torch.int64, device=self.device),
-                        "positions": torch.zeros(B, dtype=torch.int64, device=self.device),
-                        "table": torch.zeros(B, cache.max_pages, dtype=torch.int32, device=self.device)}
-            step["tokens"].copy_(tokens.reshape(-1))
-            step["positions"].copy_(positions)
-            step["table"].copy_(table)
-            if "graph" in step:
-                step["graph"].replay()
-                out = step["out"].clone()
-                steps.move_to_end(B)
+        tokens = _token_ids(tokens)
+        with _appending(cache, seqs, [1] * B):
+            positions = torch.tensor([cache.length(q) - 1 for q in seqs])
+            table = cache.table(seqs)
+            if graph:
+                out = self._paged_step(cache, tokens, positions, table)
             else:
-                s = self._paged_stream
-                s.wait_stream(here)
-                # this call's step, on the capture stream (workspaces are sized outside the capture)
-                try:
-                    with torch.cuda.stream(s):
-                        out = self._paged_body(cache, step["tokens"], step["positions"], step["table"])
-                finally:
-                    here.wait_stream(s)
-                out = out.clone()
-                g = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(g, stream=s):
-                    step["out"] = self._paged_body(cache, step["tokens"], step["positions"], step["table"])
-                    step["workspaces"] = ops._end_of_capture(self._paged_status)
-                step["graph"] = g
-                steps[B] = step
-                if len(steps) > self.PAGED_STEPS:
-                    steps.popitem(last=False)
-            self._paged_done.record(here)
-            self._paged_last = (weakref.ref(cache), B)
+                out = self._paged_body(cache, tokens.to(self.device, torch.int64), positions.to(self.device),
+                                       table.to(self.device))
         for q in seqs:
             cache.trim(q)
+        return out
+
+    def _paged_step(self, cache: PagedKVCache, tokens, positions, table) -> torch.Tensor:
+        """The step's replay, or the step itself and its capture."""
+        B = tokens.numel()
+        here = torch.cuda.current_stream(self.device)
+        if self._paged_done is None:
+            self._paged_stream, self._paged_done = torch.cuda.Stream(device=self.device), torch.cuda.Event()
+            self._paged_status = ops._status_sink(self.device)
+        here.wait_event(self._paged_done)
+        steps = self._paged_steps.setdefault(cache, OrderedDict())
+        step = steps.get(B)
+        if step is None:
+            step = {"tokens": torch.zeros(B, dtype=torch.int64, device=self.device),
+                    "positions": torch.zeros(B, dtype=torch.int64, device=self.device),
+                    "table": torch.zeros(B, cache.max_pages, dtype=torch.int32, device=self.device)}
+        step["tokens"].copy_(tokens)
+        step["positions"].copy_(positions)
+        step["table"].copy_(table)
+        if "graph" in step:
+            step["graph"].replay()
+            out = step["out"].clone()
+            steps.move_to_end(B)
+        else:
+            s = self._paged_stream
+            s.wait_stream(here)
+            # this call's step, on the capture stream (workspaces are sized outside the capture)
+            try:
+                with torch.cuda.stream(s):
+                    out = self._paged_body(cache, step["tokens"], step["positions"], step["table"])
+            finally:
+                here.wait_stream(s)
+            out = out.clone()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                step["out"] = self._paged_body(cache, step["tokens"], step["positions"], step["table"])
+                step["workspaces"] = ops._end_of_capture(self._paged_status)
+            step["graph"] = g
+            steps[B] = step
+            if len(steps) > self.PAGED_STEPS:
+                steps.popitem(last=False)
+        self._paged_done.record(here)
+        self._paged_last = (weakref.ref(cache), B)
         return out
 
     @torch.inference_mode()
@@ -581,7 +615,9 @@ class Qwen3MoEStack:
         if chunk < 1:
             raise ValueError(f"chunk {chunk} is not positive")
         cache = self.paged_cache(sum(-(-n // max(page_size, 1)) for n in lens), page_size, max(lens), window, sinks)
-        hn = self._prompt_hidden(cache, [cache.add() for _ in prompts], prompts)
+        seqs = [cache.add() for _ in prompts]
+        cache.extend(seqs, self._prompt_lengths(seqs, prompts))
+        hn = self._prompt_hidden(cache, seqs, prompts)
         # a prompt's last row predicts nothing that is given
         given = torch.cat([torch.cat([p.reshape(-1)[1:].to(self.device), p.new_full((1,), -1).to(self.device)])
                            for p in prompts]).to(torch.int64)

@@ -337,3 +337,38 @@ def test_captured_steps_leave_nothing_behind(pair):
     with pytest.raises(NKIMoEError):
         ops.read_paged_status()
     ops.read_paged_status()
+
+
+def test_a_call_that_fails_leaves_the_lengths(pair, monkeypatch):
+    """Nothing counts as held that was not stored: a prompt or a step that fails on the way
+    can be given again."""
+    hf, st = pair
+    text = ids(60, 9)
+    cache = st.paged_cache(12, page_size=16)
+    seq = cache.add()
+    st.prefill_paged(cache, [seq], [text[:20]])
+    other = cache.fork(seq)
+    free = cache.free_pages
+
+    def fails(*a, **kw):
+        raise RuntimeError("out of memory")
+
+    for name in ("_layers", "_paged_body"):
+        with monkeypatch.context() as m:
+            m.setattr(st, name, fails)
+            for graph in (False, True):
+                with pytest.raises(RuntimeError, match="out of memory"):
+                    if name == "_layers":
+                        st.prefill_paged(cache, [seq, other], [text[20:57], text[20:30]])
+                    st.decode_paged(cache, [other, seq], text[20:22], graph=graph)
+    for bad in (torch.rand(3), torch.zeros(3, dtype=torch.bool)):
+        with pytest.raises(ValueError):
+            st.prefill_paged(cache, [seq], [bad])
+        for graph in (False, True):
+            with pytest.raises(ValueError):
+                st.decode_paged(cache, [seq], bad[:1], graph=graph)
+    assert cache.length(seq) == cache.length(other) == 20 and cache.free_pages >= free - 1  # a copied page may stay
+    got = [st.prefill_paged(cache, [seq], [text[20:57]])[0]] + [st.decode_paged(cache, [seq], text[i:i + 1])[0]
+                                                                for i in range(57, 60)]
+    _check(torch.stack(got), hf_logits(hf, text)[56:60])
+    st.release_graph()

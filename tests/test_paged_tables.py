@@ -147,6 +147,26 @@ def test_random_use_against_a_model_of_contents():
     assert t.free_pages == 40
 
 
+def test_take_back_undoes_an_extension():
+    t = PageTables(8, 16, 4)
+    a, b = t.add(), t.add()
+    t.extend([a, b], [20, 16])
+    c = t.fork(a)
+    t.extend([a, b], [40, 1])  # a copies its last page
+    assert t.pages(a) == [0, 3, 4, 5] and t.pages(b) == [2, 6] and t.free_pages == 1
+    t.take_back([a, b], [20, 16])
+    assert t.pages(a) == [0, 3] and t.length(a) == 20 and t.pages(b) == [2] and t.length(b) == 16
+    assert t.pages(c) == [0, 1] and t.free_pages == 4
+    t.take_back([b, c], [0, 20])
+    assert t.pages(b) == [] and t.length(b) == 0 and t.free_pages == 5
+    for seqs, lengths in (([a], [21]), ([a], [-1]), ([99], [0]), ([a], []), ([a, b], [20, 1])):
+        with pytest.raises(ValueError):
+            t.take_back(seqs, lengths)
+    assert t.length(a) == 20 and t.free_pages == 5
+    t.extend([b], [64])
+    assert t.free_pages == 1
+
+
 # ------------------------------------------------------------------ refusals
 NULL = ctypes.c_void_p(0)
 SOME = ctypes.c_void_p(4096)  # never dereferenced: the checks come first

@@ -490,7 +490,7 @@ class Qwen3MoEStack:
             raise ValueError(f"batch {B} exceeds the expert-parallel exchange ({self.max_batch})")
         tokens = _token_ids(tokens)
         with _appending(cache, seqs, [1] * B):
-            positions = torch.tensor([cache.length(q) - 1 for q in seqs])
+            positions = torch.tensor([cache.length(q) - 1 for q in seqs], dtype=torch.int64)
             table = cache.table(seqs)
             if graph:
                 out = self._paged_step(cache, tokens, positions, table)

@@ -372,3 +372,12 @@ def test_a_call_that_fails_leaves_the_lengths(pair, monkeypatch):
                                                                 for i in range(57, 60)]
     _check(torch.stack(got), hf_logits(hf, text)[56:60])
     st.release_graph()
+
+
+def test_a_step_of_no_sequences(pair):
+    _, st = pair
+    cache = st.paged_cache(4, page_size=16)
+    for graph in (False, True, True):
+        assert st.decode_paged(cache, [], ids(0, 1), graph=graph).shape == (0, 1024)
+    assert cache.free_pages == 4
+    st.release_graph()

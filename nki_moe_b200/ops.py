@@ -344,11 +344,11 @@ def read_paged_status(device=None) -> None:
 
 
 def _on_its_device(fn):
-    """Runs ``fn`` with its first argument's device as the current one (its
+    """Runs ``fn`` with the device of its first CUDA tensor as the current one (its
     kernels launch there, on that device's current stream)."""
     @functools.wraps(fn)
     def run(*args, **kw):
-        t = args[0] if args else next(iter(kw.values()), None)
+        t = args[0] if args else next((v for v in kw.values() if isinstance(v, torch.Tensor) and v.is_cuda), None)
         if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() != torch._C._cuda_getDevice():
             with torch.cuda.device(t.device):
                 return fn(*args, **kw)

@@ -284,3 +284,35 @@ def test_pages_written_twice_or_read_and_written_are_refused_in_pools_of_any_siz
     last = pool - 1
     for src, dst in (((0, 1), (2, 2)), ((0, last), (last, 3)), ((last,), (last,)), ((pool,), (0,)), ((0,), (-1,))):
         assert code("nkimoe_copy_pages", SOME, 2, pool, 4096, ids(*src), ids(*dst), len(src), NULL) == _lib.ERR_INVALID_ARG
+
+
+def test_calls_run_on_the_device_of_their_tensors_in_any_order_of_arguments(monkeypatch):
+    class OnSecond(torch.Tensor):
+        is_cuda = True
+        device = torch.device("cuda", 1)
+
+        def get_device(self):
+            return 1
+
+    entered = []
+
+    class Device:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            entered.append(self.device)
+
+        def __exit__(self, *exc):
+            return False
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    t = torch.zeros(2).as_subclass(OnSecond)
+    fn = ops._on_its_device(lambda *args, **kw: len(args) + len(kw))
+    for args, kw in (((t, 3), {}), ((), {"qkv": t, "n_heads": 8}), ((), {"n_heads": 8, "qkv": t, "out": None}),
+                     ((), {"out": None, "qkv": t}), ((), {"src": torch.zeros(1), "pages": t})):
+        entered.clear()
+        assert fn(*args, **kw) == len(args) + len(kw) and entered == [torch.device("cuda", 1)], kw
+    entered.clear()
+    assert fn(n_heads=8) == 1 and fn(torch.zeros(1), 2) == 2 and not entered

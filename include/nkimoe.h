@@ -223,7 +223,7 @@ NKIMOE_API size_t nkimoe_paged_decode_attention_workspace_bytes(int64_t batch, i
  * pos_stride] (int64, pos_stride 0 or 1) gets q/k RMSNorm + RoPE, its key and
  * value are stored in their page, and query head h attends to the visible
  * positions of kv head h / (n_heads / n_kv_heads).  out: bf16 [batch, n_heads
- * * 128].  A negative position marks an idle row: nothing is stored, its
+ * * 128], not overlapping qkv.  A negative position marks an idle row: nothing is stored, its
  * output is zero; so is that of a position outside the page table, which is
  * reported (NKIMOE_DEV_BAD_INDEX), as is a page that the query needs and that
  * is not held (its positions count as invisible).  At most 16 query heads per
@@ -247,8 +247,9 @@ NKIMOE_API size_t nkimoe_paged_prefill_attention_workspace_bytes(int64_t T, int6
  * nkimoe_qk_norm_rope_store) over the pages, which already hold the rows' own
  * keys and values: whole prompts, or chunks of prompts over what the cache
  * holds of them.  cu_seqlens, kv_lens as in nkimoe_qk_norm_rope_store; a
- * sequence may have no rows.  out: bf16 [T, n_heads * 128]; rows from
- * cu_seqlens[batch] on are left alone.  Lengths that make no sense (outside
+ * sequence may have no rows.  out: bf16 [T, n_heads * 128], not overlapping q
+ * unless it is q itself (dense rows); rows from cu_seqlens[batch] on are left
+ * alone.  Lengths that make no sense (outside
  * [0, T], decreasing, a kv_len below the rows or past the page table) are
  * reported (NKIMOE_DEV_BAD_INDEX) and their rows left unwritten; a page that
  * a row needs and that is not held is reported, and the rows that need it have

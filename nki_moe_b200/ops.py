@@ -421,13 +421,20 @@ def _lengths(cu_seqlens: torch.Tensor, kv_lens: torch.Tensor) -> int:
     return kv_lens.shape[0]
 
 
-def _rows_out(out: torch.Tensor | None, shape: tuple, like: torch.Tensor) -> torch.Tensor:
-    """``out`` checked, or a new bf16 tensor on the device of ``like`` (bf16)."""
+def _rows_out(out: torch.Tensor | None, shape: tuple, like: torch.Tensor, in_place: bool = False) -> torch.Tensor:
+    """``out`` checked against the rows ``like`` (bf16) that the call reads, or
+    a new tensor on their device.  A call writes some rows while it still
+    reads others, so the two must lie apart, or with ``in_place`` be the same."""
     if out is None:
         return like.new_empty(shape)
     dev = like.device
     if out.dtype != torch.bfloat16 or out.shape != shape or not out.is_contiguous() or out.device != dev:
         raise ValueError(f"out must be a contiguous bf16 {list(shape)} tensor on {dev}")
+    if out.numel() and like.numel():
+        a, b = out.data_ptr(), like.data_ptr()
+        last = sum((n - 1) * st for n, st in zip(like.shape, like.stride()))
+        if a < b + 2 * (last + 1) and b < a + 2 * out.numel() and not (in_place and a == b and like.is_contiguous()):
+            raise ValueError("out must not overlap the rows that the call reads")
     return out
 
 
@@ -446,8 +453,8 @@ def qk_norm_rope_store(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torc
     ``kv_len - n + i``); ``k_pages``/``v_pages``: one layer's ``[pages,
     n_kv_heads, page_size, 128]`` bf16 pools, updated in place;
     ``page_table``: int32 ``[B, pages per sequence]`` (-1: not kept).  Returns
-    the queries ``[T, n_heads, 128]`` bf16 (``out``, contiguous, if given);
-    rows from ``cu_seqlens[B]`` on are left as they were."""
+    the queries ``[T, n_heads, 128]`` bf16 (``out``, contiguous and apart from
+    ``qkv``, if given); rows from ``cu_seqlens[B]`` on are left as they were."""
     _cuda(qkv, "qkv")
     row = (n_heads + 2 * n_kv_heads) * 128
     if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != row or not qkv.is_contiguous():
@@ -485,7 +492,8 @@ def paged_decode_attention(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: 
     ``page_table`` as in :func:`qk_norm_rope_store`.  With ``window > 0`` the
     query at ``p`` sees the last ``window`` positions up to ``p`` and the first
     ``sinks`` ones; pages that lie outside both need not be held.  Returns
-    ``[B, n_heads * 128]`` bf16."""
+    ``[B, n_heads * 128]`` bf16 (``out``, contiguous and apart from ``qkv``, if
+    given)."""
     _cuda(qkv, "qkv")
     row = (n_heads + 2 * n_kv_heads) * 128
     if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != row or not qkv.is_contiguous():
@@ -527,7 +535,8 @@ def paged_prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     ``page_table`` as there; ``window``, ``sinks`` as in
     :func:`paged_decode_attention`.  Cached rows below ``kv_lens`` must be
     finite.  Returns ``[T, n_heads * 128]`` bf16; rows from ``cu_seqlens[B]``
-    on are left as they were in ``out``."""
+    on are left as they were in ``out`` (apart from ``q``, or a contiguous ``q``
+    itself in its place)."""
     _cuda(q, "q")
     if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != 128 or q.stride(2) != 1 \
             or (q.shape[1] > 1 and q.stride(1) != 128):
@@ -539,7 +548,7 @@ def paged_prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     cache = _paged_cache(k_pages, v_pages, page_table, nkv, B)
     _same_device(dev.index, "cu_seqlens kv_lens k_pages v_pages page_table", cu_seqlens, kv_lens, k_pages, v_pages,
                  page_table)
-    out = _rows_out(out, (T, nq * 128), q)
+    out = _rows_out(out, (T, nq * 128), q, in_place=True)
     s = _raw_stream(dev.index)
     nbytes = _paged_ws_bytes(dev.index, "nkimoe_paged_prefill_attention_workspace_bytes", T, B, nq, nkv, cache[8],
                              cache[5])

@@ -697,3 +697,53 @@ def test_reports_survive_a_larger_workspace(monkeypatch):
     g.replay()
     with pytest.raises(NKIMoEError):
         ops.read_paged_status()
+
+
+def test_outputs_lie_apart_from_what_is_read():
+    nq, nkv, B = 8, 2, 5
+    args = step_inputs([70, 33, 50, 1, 17], nq, nkv, 16, 33)
+    qkv, qw, kw, pos, k, v, table = args[:7]
+    want = ops.paged_decode_attention(*args)
+    row = (nq + 2 * nkv) * HD
+    buf = torch.empty(B * row + B * nq * HD, dtype=torch.bfloat16, device="cuda")
+    buf[:B * row] = qkv.reshape(-1)
+    rows = buf[:B * row].view(B, row)
+    cu = torch.arange(B + 1, dtype=torch.int32, device="cuda")
+    kv = (pos + 1).int()
+    for at in (0, 64, 2 * row, B * row - 8):
+        out = buf[at:at + B * nq * HD].view(B, nq * HD)
+        with pytest.raises(ValueError):
+            ops.paged_decode_attention(rows, *args[1:], out=out)
+        with pytest.raises(ValueError):
+            ops.qk_norm_rope_store(rows, qw, kw, cu, kv, k, v, table, nq, nkv, out=out.view(B, nq, HD))
+    out = buf[B * row:].view(B, nq * HD)  # right behind
+    assert ops.paged_decode_attention(rows, *args[1:], out=out) is out and torch.equal(out, want)
+    q = ops.qk_norm_rope_store(rows, qw, kw, cu, kv, k, v, table, nq, nkv, out=out.view(B, nq, HD))
+    want = ops.paged_prefill_attention(q, k, v, table, cu, kv)
+    for at in (8, nq * HD):
+        with pytest.raises(ValueError):
+            ops.paged_prefill_attention(buf[:B * nq * HD].view(B, nq, HD), k, v, table, cu, kv,
+                                        out=buf[at:at + B * nq * HD].view(B, nq * HD))
+    apart = torch.empty(B, 2 * nq, HD, dtype=torch.bfloat16, device="cuda")
+    apart[:, :nq] = q
+    with pytest.raises(ValueError):  # rows with gaps cannot be written in place
+        ops.paged_prefill_attention(apart[:, :nq], k, v, table, cu, kv,
+                                    out=apart.view(-1)[:B * nq * HD].view(B, nq * HD))
+    got = ops.paged_prefill_attention(q, k, v, table, cu, kv, out=q.view(B, nq * HD))
+    assert got.data_ptr() == q.data_ptr() and torch.equal(got, want)
+    ops.read_paged_status()
+
+
+@pytest.mark.parametrize("new,past,window", [(700, 0, 0), (45, 9000, 0), (300, 4000, 600)])
+def test_prefill_over_its_own_queries(new, past, window):
+    """Whole pairs and cut ones, into the queries' own rows."""
+    nq, nkv, ps = 16, 2, 64
+    c = Cache([past + new, past + new + 7], nkv, ps, 90)
+    g = torch.Generator().manual_seed(new)
+    q = torch.randn(2 * new, nq, HD, generator=g).bfloat16().cuda()
+    args = (c.k.cuda(), c.v.cuda(), c.table.cuda(), torch.tensor([0, new, 2 * new], dtype=torch.int32).cuda(),
+            torch.tensor([past + new, past + new + 7], dtype=torch.int32).cuda())
+    want = ops.paged_prefill_attention(q, *args, window=window, sinks=4 if window else 0)
+    ops.paged_prefill_attention(q, *args, window=window, sinks=4 if window else 0, out=q.view(2 * new, nq * HD))
+    assert torch.equal(q.view(2 * new, nq * HD), want)
+    ops.read_paged_status()

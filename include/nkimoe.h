@@ -177,8 +177,8 @@ NKIMOE_API int nkimoe_decode_attention(const void* qkv, const void* q_weight, co
  * page_size, 128] (bf16, 16-byte aligned): the [n_kv_heads, page_size, 128]
  * block of a page is contiguous, k_page_stride / v_page_stride elements lie
  * between pages (multiples of 8).  page_size is 16, 32, 64, 128 or 256.  Row b
- * of page_table (int32, table_stride apart) lists the max_pages pages of
- * sequence b in order; -1 marks a page that is not held, and entries that a
+ * of page_table (int32, table_stride apart) lists the max_pages pages (at most
+ * 2^30 positions, for the prompt attention fewer) of sequence b in order; -1 marks a page that is not held, and entries that a
  * call does not need are not read.  A page that a call writes belongs to one
  * sequence only (nkimoe_copy_pages makes one of a shared page).
  *

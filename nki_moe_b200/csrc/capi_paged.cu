@@ -205,6 +205,8 @@ int nkimoe_paged_prefill_attention(const void* q, int64_t q_row_stride, const vo
   NKI_CHECK(check_cache(k_pages, v_pages, k_page_stride, v_page_stride, num_pages, page_size, page_table, table_stride,
                         max_pages, n_kv_heads, &c));
   NKI_REQUIRE((T + batch) * n_kv_heads < 0x7fff0000LL, NKIMOE_ERR_UNSUPPORTED, "shape too large");
+  // the key blocks (of 128 positions) of 256 pairs are added up in 32 bits
+  NKI_REQUIRE(max_pages * page_size < (1LL << 30), NKIMOE_ERR_UNSUPPORTED, "page tables of 2^30 positions or more");
   NKI_REQUIRE(q && cu_seqlens && kv_lens && out && workspace, NKIMOE_ERR_INVALID_ARG, "null pointer");
   NKI_REQUIRE(q_row_stride >= static_cast<int64_t>(n_heads) * 128 && q_row_stride % 8 == 0, NKIMOE_ERR_INVALID_ARG,
               "query rows must be multiples of 8 elements apart and not overlap");

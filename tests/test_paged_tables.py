@@ -316,3 +316,13 @@ def test_calls_run_on_the_device_of_their_tensors_in_any_order_of_arguments(monk
         assert fn(*args, **kw) == len(args) + len(kw) and entered == [torch.device("cuda", 1)], kw
     entered.clear()
     assert fn(n_heads=8) == 1 and fn(torch.zeros(1), 2) == 2 and not entered
+
+
+def test_prompt_tables_of_2_30_positions_are_refused():
+    """The key blocks of 256 pairs are added up in 32 bits: 2^23 of each would be 2^31."""
+    uns = _lib.ERR_UNSUPPORTED
+    for ps, most in ((256, 2 ** 22), (16, 2 ** 26)):
+        kw = dict(ps=ps, ts=most, ks=ps * 512, vs=ps * 512, wsb=0)
+        assert code("nkimoe_paged_prefill_attention", *prefill_args(mp=most, **kw)) == uns
+        # one page less is a matter of the workspace alone
+        assert code("nkimoe_paged_prefill_attention", *prefill_args(mp=most - 1, **kw)) == _lib.ERR_WORKSPACE

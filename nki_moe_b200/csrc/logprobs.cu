@@ -288,7 +288,7 @@ __device__ __forceinline__ void join_warps(TopShared& sh, WarpTop& best, int war
 // keys of a mix are still those of different elements, since an element has one
 // slot for good (show_best), and an older key only lowers the bound.
 // A few places by one maximum each, more by the keys' ranks (8000 rows of 32000
-// with 5 alternatives 140 us against 144, 2000 rows of 151936 with 20 148
+// with 5 alternatives 145 us against 151, 2000 rows of 151936 with 20 155
 // against 169).
 __device__ __forceinline__ int nth_shown(TopShared& sh, const volatile int* keys, int n, int warp, int lane) {
   int mine = keys[lane];
@@ -451,14 +451,18 @@ __device__ __forceinline__ void warp_top(TopShared& sh, WarpTop& best, int& show
 //
 // Bound by HBM over many rows (the logits read once), by the exponentials next
 // to it: measured 2000 rows of 151936 bf16 99.5 us without alternatives (6.11
-// TB/s = 0.93 of the measured copy), 122 us with 5 and 148 us with 20: a warp that
-// finds a candidate keeps its next loads waiting.  8 rows with 20 alternatives
-// 8.8 us (one chunk per CTA, then the join).  What was slower with 5
-// alternatives: the CTA's best tokens kept in common, a barrier per chunk, 500
-// us; the warps' lists made one after 1, 2, 4, 8 ... chunks, 137 us; a lane's
-// elements spread over its warp, one such lane at a time, 124 us (8000 rows of
-// 32000: 158 against 140).  Chunks copied to shared memory two ahead: 121 us,
-// but 108 without alternatives and 155 for the shorter rows.
+// TB/s = 0.93 of the measured copy), 124 us with 5 and 154 us with 20: a warp that
+// finds a candidate keeps its next loads waiting.  Back to back for seconds, at
+// the power cap, 5 alternatives take 135 us.  1000 rows in fp32: 92 us, with 5
+// alternatives 104 us.  8 rows with 20 alternatives 8.8 us, in fp32 11 us (one
+// chunk per CTA, then the join).
+// What was slower with 5 alternatives (when they took 122 us, 8000 rows of 32000
+// 140 us; that an element keeps its slot in what the warps show has added 2 and 5
+// us): the CTA's best tokens kept in common, a barrier per chunk, 500 us; the
+// warps' lists made one after 1, 2, 4, 8 ... chunks, 137 us; a lane's elements
+// spread over its warp, one such lane at a time, 124 us (8000 rows: 158).  Chunks
+// copied to shared memory two ahead: 121 us, but 108 without alternatives and 155
+// for the shorter rows.
 template <typename T, bool kTop>
 __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LpParams p) {
   __shared__ TopShared sh;

@@ -172,7 +172,8 @@ __device__ __forceinline__ HeadPart norm_rope_part(const HeadPart& x, const Head
 }
 
 // Keys are kept rounded, so a sum in fp32 that falls on the other side of the
-// middle between two bf16 values stays wrong for good.  key_near_tie says which
+// middle between two bf16 values stays one bf16 step off for good (more than half
+// a step from the formula's value).  key_near_tie says which
 // of the lane's rotated pairs (bit e: elements 4l + e and 64 + 4l + e) lie that
 // near to a middle, by 2^-23 of the pair's length, which the rotation keeps: one
 // head in 60 has one.  Those are formed again by key_in_64_bits.  Of 361 values in

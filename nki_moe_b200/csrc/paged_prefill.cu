@@ -34,10 +34,12 @@
 // Bound by the tensor core and, more, by each tile's chain: scores -> softmax
 // -> weights -> product -> next scores, about 3500 cycles per block and pair
 // against 2100 of MMAs (P lies over S, so a tile's next scores wait for its
-// product).  Measured: 8192 causal tokens, 32 heads over 4: 441 us = 1.24
-// PFLOP/s = 0.74 of the measured cuBLAS rate; 8 x 512 tokens 37 us; 945 rows in
-// four chunks over 9001 cached positions, window 4096: 83 us.
-// Other shapes of the pipeline were slower (8192 tokens): key blocks of 64 with
+// product).  Measured: 8192 causal tokens, 32 heads over 4, 441 to 451 us in runs
+// of some 40 ms at 1965 MHz = 1.22 to 1.25 PFLOP/s = 0.73 to 0.75 of the measured
+// cuBLAS burst; back to back for seconds, 1670 MHz at the power cap, 511 us = 1.08
+// PFLOP/s = 0.77 of the sustained one.  8 x 512 tokens 37 to 38 us either way; 945
+// rows in four chunks over 9001 cached positions, window 4096: 83 to 88 us.
+// Other shapes of the pipeline were slower (8192 tokens, short runs): key blocks of 64 with
 // two score buffers per tile 891 us (an MMA of N = 64 takes as long as one of
 // 128: it is bound by reading Q), one tile with two score buffers and its own
 // P columns 581 us (twice the K / V traffic through shared memory), two softmax

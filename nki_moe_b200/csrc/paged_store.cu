@@ -49,9 +49,11 @@ __device__ __forceinline__ int sequence_of(const int* cu, int B, int t, int lane
 // but the norm weights in shared memory.  Its first heads' loads go out before
 // the row's position is known, so the two latencies overlap.
 //
-// Bound by HBM and by issue: (nq + 2 nkv) * 256 bytes read and as many written
-// per row.  Measured: 8192 rows of 32 + 2 * 4 heads 41 us = 4.1 TB/s = 0.63 of
-// the measured copy; 15 rows 5.1 us.  Of that 4 us and 1.5 us are the keys formed
+// (nq + 2 nkv) * 256 bytes are read and as many written per row.  Measured: 8192
+// rows of 32 + 2 * 4 heads 41 us, 4.1 TB/s read and written = 0.63 of the measured
+// copy, while the profile shows DRAM at 33 % (half of the traffic ends in L2) and
+// issue at 64 %: neither is full, a row's chain of lookups, sines and packing is
+// what it waits for.  15 rows 5.1 us.  Of that 4 us and 1.5 us are the keys formed
 // again in 64 bits (their check alone 0.3 us).
 template <int kWarps>
 __global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_store_kernel(const __grid_constant__ StoreParams p) {

@@ -306,8 +306,8 @@ def _status_sink(device: torch.device) -> torch.Tensor:
 def _end_of_capture(sink: torch.Tensor) -> list:
     """Called last in a capture on the current stream, by the owner of the
     graph: each replay ends by adding its paged calls' status to ``sink``.
-    Returns the workspaces that the capture uses; the owner holds them as long
-    as the graph, this module no longer than a next capture needs them."""
+    Returns the workspaces that the capture uses, which the owner holds as long
+    as the graph."""
     key = (sink.device.index, torch.cuda.current_stream(sink.device).cuda_stream)
     with _ws_lock:
         held = [table[key] for table in (_ws, _attn_ws) if key in table]

@@ -59,10 +59,15 @@ def _appending(cache: PagedKVCache, seqs, counts):
         raise
 
 
-def _token_ids(t: torch.Tensor) -> torch.Tensor:
+def _token_ids(t: torch.Tensor, vocab: int) -> torch.Tensor:
+    """``t`` as a vector, checked: its type, and on the host its range (on the
+    device that would wait for it)."""
     if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
         raise ValueError(f"token ids must be whole numbers, not {t.dtype}")
-    return t.reshape(-1)
+    t = t.reshape(-1)
+    if not t.is_cuda and t.numel() and not (0 <= int(t.min()) and int(t.max()) < vocab):
+        raise ValueError(f"token ids must be in [0, {vocab})")
+    return t
 
 
 @dataclass
@@ -422,7 +427,7 @@ class Qwen3MoEStack:
         cu = cu.to(self.device)
         kv = torch.tensor([cache.length(q) for q in seqs], dtype=torch.int32).to(self.device)
         table = cache.table(seqs).to(self.device)
-        ids = torch.cat([_token_ids(p).to(self.device, torch.int64) for p in prompts])
+        ids = torch.cat([p.reshape(-1).to(self.device, torch.int64) for p in prompts])
         h = F.embedding(ids, self.embed)
 
         def attention(li, lyr, xn):
@@ -435,7 +440,7 @@ class Qwen3MoEStack:
 
     def _prompt_lengths(self, seqs, prompts) -> list[int]:
         """The prompts' lengths, checked."""
-        lens = [int(_token_ids(p).numel()) for p in prompts]
+        lens = [int(_token_ids(p, self.cfg.vocab_size).numel()) for p in prompts]
         if len(prompts) != len(seqs) or not seqs or min(lens) == 0:
             raise ValueError("one prompt, not empty, for each sequence")
         if any(lyr.ep is not None for lyr in self.layers) and sum(lens) > self.max_batch * self.max_seq:
@@ -488,7 +493,7 @@ class Qwen3MoEStack:
             raise ValueError(f"{tokens.numel()} tokens for {B} sequences")
         if any(lyr.ep is not None for lyr in self.layers) and B > self.max_batch:
             raise ValueError(f"batch {B} exceeds the expert-parallel exchange ({self.max_batch})")
-        tokens = _token_ids(tokens)
+        tokens = _token_ids(tokens, self.cfg.vocab_size)
         with _appending(cache, seqs, [1] * B):
             positions = torch.tensor([cache.length(q) - 1 for q in seqs], dtype=torch.int64)
             table = cache.table(seqs)

@@ -326,3 +326,15 @@ def test_prompt_tables_of_2_30_positions_are_refused():
         assert code("nkimoe_paged_prefill_attention", *prefill_args(mp=most, **kw)) == uns
         # one page less is a matter of the workspace alone
         assert code("nkimoe_paged_prefill_attention", *prefill_args(mp=most - 1, **kw)) == _lib.ERR_WORKSPACE
+
+
+def test_token_ids_on_the_host_are_checked():
+    from nki_moe_b200.qwen_stack import _token_ids
+
+    for ok in (torch.tensor([[0, 99]]), torch.tensor([5], dtype=torch.int32), torch.zeros(0, dtype=torch.int64),
+               torch.tensor([99], dtype=torch.uint8)):
+        assert _token_ids(ok, 100).shape == (ok.numel(),)
+    for bad in (torch.tensor([3, 100]), torch.tensor([-1]), torch.tensor([2 ** 40]), torch.rand(2),
+                torch.zeros(2, dtype=torch.bool), torch.zeros(1, dtype=torch.complex64)):
+        with pytest.raises(ValueError):
+            _token_ids(bad, 100)

@@ -49,6 +49,7 @@ extern "C" {
 #define NKIMOE_BF16 1
 #define NKIMOE_I32 2
 #define NKIMOE_I64 3
+#define NKIMOE_F64 4
 
 /* weight layouts accepted by the packing entry points */
 #define NKIMOE_LAYOUT_NXD 0        /* gate_up [E,H,2I], down [E,I,H] (qwen.py:164-226)          */
@@ -272,6 +273,54 @@ NKIMOE_API int nkimoe_paged_prefill_attention(const void* q, int64_t q_row_strid
  * ids.  No reference counterpart (the reference's cache is the runtime's). */
 NKIMOE_API int nkimoe_copy_pages(void* pages, int64_t planes, int64_t num_pages, int64_t page_bytes,
                                  const int32_t* src, const int32_t* dst, int64_t n, void* stream);
+
+/* The end of a step with drafted tokens.  Sequence b brought the nodes
+ * cu_seqlens[b] .. cu_seqlens[b+1] - 1 of a tree (int64 tokens, int32 parents:
+ * indexes among its nodes; node 0 is the root, its current token; at most 64),
+ * which lie in places kv_lens[b] - n + i of its cache, and a token was drawn
+ * after each (int64 sampled).  From the root on the path goes to the lowest
+ * child (of a higher index than its parent) whose token equals what was drawn,
+ * until there is none.  counts int32 [batch]: the path's nodes; of a
+ * sequence's n entries in path (int32 [T]) and new_tokens (int64 [T]) the
+ * first counts[b] get the path's nodes and what was drawn after them, the
+ * others -1, as do rows of no sequence.  The rows of the path's nodes move to
+ * places kv_lens[b] - n + k, in each of `planes` pools [num_pages, n_kv_heads,
+ * page_size, row_bytes] (16-byte multiples), one behind the other at `pages`.
+ * Lengths that make no sense, more than 64 nodes, or a row to be moved whose
+ * page is not held are reported (NKIMOE_DEV_BAD_INDEX); such a sequence's
+ * count is 0, such a row stays.  At most 65535 sequences.  No reference counterpart (it
+ * decodes one token a step). */
+NKIMOE_API int nkimoe_accept_drafts(const int64_t* tokens, const int64_t* sampled, const int32_t* parents,
+                                    const int32_t* cu_seqlens, const int32_t* kv_lens, void* pages, int64_t planes,
+                                    int64_t num_pages, int64_t n_kv_heads, int64_t page_size, int64_t row_bytes,
+                                    const int32_t* page_table, int64_t table_stride, int64_t max_pages,
+                                    int32_t* counts, int32_t* path, int64_t* new_tokens, int64_t T, int64_t batch,
+                                    int* status, void* stream);
+
+/* ---------------------------------------------------------------- sampling */
+
+/* A token from each row of logits [rows, vocab] (fp32 or bf16, rows row_stride
+ * elements apart, vocab at most 2^18), given a random number of [0, 1) per row
+ * (uniforms, NKIMOE_F32 or NKIMOE_F64).  The distribution is softmax(x /
+ * temperature) restricted, in the order of falling logits (equal ones by the
+ * lower id), to the first top_k tokens (0: all), of those to the fewest that
+ * hold top_p of their sum (1: all, at least one), and to probabilities of at
+ * least min_p times the largest; tokens[r] (int64) is the first id whose
+ * running sum over the kept ids, in rising order, exceeds the random number
+ * times the whole, logprob[r] the logarithm of its probability in the
+ * restricted distribution.  temperature 0: the largest logit, the lowest id of
+ * equal ones, logprob 0.  Each setting is a device array with an entry per row,
+ * or, where that is NULL, the one value after it.  In arrays a top_k below 1, a
+ * top_p that is not below 1 and a min_p that is not above 0 restrict nothing.
+ * Weights and sums are fp64.  A logit of -inf is never drawn; a row with a NaN,
+ * a +inf, nothing but -inf, or a negative or NaN temperature has no
+ * distribution: token -1, logprob NaN.
+ * No reference counterpart (sampling is its runtime's). */
+NKIMOE_API int nkimoe_sample_tokens(const void* logits, int dtype, int64_t row_stride, const void* uniforms,
+                                    int u_dtype, const float* temperature, double temperature_all,
+                                    const int32_t* top_k, int64_t top_k_all, const float* top_p, double top_p_all,
+                                    const float* min_p, double min_p_all, int64_t rows, int64_t vocab,
+                                    int64_t* tokens, float* logprob, void* stream);
 
 /* ---------------------------------------------------------------- token scores */
 

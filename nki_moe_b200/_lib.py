@@ -22,11 +22,12 @@ ERR_WORKSPACE = 3
 ERR_CUDA = 4
 ERR_DEVICE = 5
 
-F32, BF16, I32, I64 = 0, 1, 2, 3
+F32, BF16, I32, I64, F64 = 0, 1, 2, 3, 4
 LAYOUT_NXD, LAYOUT_HF = 0, 1
 
 _c = ctypes
 _vp, _i, _i64, _f, _sz = _c.c_void_p, _c.c_int, _c.c_int64, _c.c_float, _c.c_size_t
+_d = _c.c_double
 
 # name -> (restype, argtypes); the list is the C ABI this package binds.
 SIGNATURES = {
@@ -50,6 +51,10 @@ SIGNATURES = {
     "nkimoe_paged_prefill_attention": (_i, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
                                             _i64, _i64, _i, _i, _i, _f, _i64, _i64, _vp, _sz, _vp]),
     "nkimoe_copy_pages": (_i, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "nkimoe_accept_drafts": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
+                                  _vp, _i64, _i64, _vp, _vp]),
+    "nkimoe_sample_tokens": (_i, [_vp, _i, _i64, _vp, _i, _vp, _d, _vp, _i64, _vp, _d, _vp, _d, _i64, _i64, _vp, _vp,
+                                  _vp]),
     "nkimoe_token_logprobs_workspace_bytes": (_sz, [_i64, _i64, _i]),
     "nkimoe_token_logprobs": (_i, [_vp, _i, _i64, _vp, _i64, _i64, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "nkimoe_skinny_linear": (_i, [_vp, _vp, _vp, _i64, _i64, _i64, _vp]),

@@ -1,6 +1,6 @@
 // C ABI of the paged key-value cache and the token scores (include/nkimoe.h):
 // argument checks in front of the launches of paged_store.cu, paged_copy.cu,
-// paged_decode.cu, paged_prefill.cu and logprobs.cu.
+// paged_decode.cu, paged_prefill.cu, accept.cu, logprobs.cu and sample.cu.
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
@@ -290,6 +290,73 @@ int nkimoe_token_logprobs(const void* logits, int dtype, int64_t row_stride, con
   NKI_CUDA(token_logprobs_launch(logits, dtype, row_stride, reinterpret_cast<const long long*>(tokens), rows, vocab,
                                  top_n, logprob, entropy, top_logprobs, reinterpret_cast<long long*>(top_ids),
                                  workspace, static_cast<cudaStream_t>(stream)));
+  return NKIMOE_OK;
+}
+
+int nkimoe_sample_tokens(const void* logits, int dtype, int64_t row_stride, const void* uniforms, int u_dtype,
+                         const float* temperature, double temperature_all, const int32_t* top_k, int64_t top_k_all,
+                         const float* top_p, double top_p_all, const float* min_p, double min_p_all, int64_t rows,
+                         int64_t vocab, int64_t* tokens, float* logprob, void* stream) {
+  NKI_REQUIRE(rows >= 0 && vocab > 0 && row_stride >= 0, NKIMOE_ERR_INVALID_ARG, "bad shape");
+  NKI_REQUIRE(dtype == NKIMOE_F32 || dtype == NKIMOE_BF16, NKIMOE_ERR_UNSUPPORTED, "logits must be fp32 or bf16");
+  NKI_REQUIRE(u_dtype == NKIMOE_F32 || u_dtype == NKIMOE_F64, NKIMOE_ERR_UNSUPPORTED, "uniforms must be fp32 or fp64");
+  NKI_REQUIRE(vocab <= (1LL << 18) && rows <= (1LL << 25), NKIMOE_ERR_UNSUPPORTED, "vocab over 2^18 or rows over 2^25");
+  NKI_REQUIRE(temperature || (temperature_all >= 0.0 && temperature_all < 1e300), NKIMOE_ERR_INVALID_ARG,
+              "temperature must be finite and not negative");
+  NKI_REQUIRE(top_p || (top_p_all >= 0.0 && top_p_all <= 1.0), NKIMOE_ERR_INVALID_ARG, "top_p must be in [0, 1]");
+  NKI_REQUIRE(min_p || (min_p_all >= 0.0 && min_p_all <= 1.0), NKIMOE_ERR_INVALID_ARG, "min_p must be in [0, 1]");
+  NKI_REQUIRE(top_k || top_k_all >= 0, NKIMOE_ERR_INVALID_ARG, "top_k must not be negative");
+  if (rows == 0) return NKIMOE_OK;
+  NKI_REQUIRE(logits && uniforms && tokens && logprob, NKIMOE_ERR_INVALID_ARG, "null pointer");
+  NKI_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (dtype == NKIMOE_F32 ? 3 : 1)) == 0 &&
+                  (reinterpret_cast<uintptr_t>(uniforms) & (u_dtype == NKIMOE_F32 ? 3 : 7)) == 0 &&
+                  (reinterpret_cast<uintptr_t>(tokens) & 7) == 0 && aligned4(logprob) && aligned4(temperature) &&
+                  aligned4(top_k) && aligned4(top_p) && aligned4(min_p),
+              NKIMOE_ERR_INVALID_ARG, "pointers must be aligned to their type");
+  SampleSettings set;
+  set.temperature = temperature;
+  set.top_k = top_k;
+  set.top_p = top_p;
+  set.min_p = min_p;
+  set.temperature_all = temperature_all;
+  set.top_k_all = top_k_all;
+  set.top_p_all = top_p_all;
+  set.min_p_all = min_p_all;
+  NKI_CUDA(sample_tokens_launch(logits, dtype, row_stride, uniforms, u_dtype == NKIMOE_F64, set, rows, vocab,
+                                reinterpret_cast<long long*>(tokens), logprob, static_cast<cudaStream_t>(stream)));
+  return NKIMOE_OK;
+}
+
+int nkimoe_accept_drafts(const int64_t* tokens, const int64_t* sampled, const int32_t* parents,
+                         const int32_t* cu_seqlens, const int32_t* kv_lens, void* pages, int64_t planes,
+                         int64_t num_pages, int64_t n_kv_heads, int64_t page_size, int64_t row_bytes,
+                         const int32_t* page_table, int64_t table_stride, int64_t max_pages, int32_t* counts,
+                         int32_t* path, int64_t* new_tokens, int64_t T, int64_t batch, int* status, void* stream) {
+  NKI_REQUIRE(T >= 0 && batch >= 0 && planes > 0 && num_pages > 0 && n_kv_heads > 0 && page_size > 0 && row_bytes > 0 &&
+                  max_pages > 0,
+              NKIMOE_ERR_INVALID_ARG, "bad shape");
+  NKI_REQUIRE(row_bytes % 16 == 0, NKIMOE_ERR_UNSUPPORTED, "rows must be multiples of 16 bytes (%lld)",
+              (long long)row_bytes);
+  NKI_REQUIRE(batch <= 65535 && T <= 0x7fffffffLL && planes <= (1 << 20) && num_pages <= 0x7fffffffLL &&
+                  n_kv_heads <= 65535 && page_size <= (1 << 20) && row_bytes <= (1 << 14) &&
+                  n_kv_heads * page_size * row_bytes <= (1LL << 30),
+              NKIMOE_ERR_UNSUPPORTED, "shape too large");
+  NKI_REQUIRE(max_pages <= (1LL << 30) / page_size, NKIMOE_ERR_UNSUPPORTED, "sequences over 2^30 positions");
+  NKI_REQUIRE(table_stride >= max_pages, NKIMOE_ERR_INVALID_ARG, "page table rows overlap");
+  if (T == 0 || batch == 0) return NKIMOE_OK;
+  NKI_REQUIRE(tokens && sampled && parents && cu_seqlens && kv_lens && pages && page_table && counts && path &&
+                  new_tokens && status,
+              NKIMOE_ERR_INVALID_ARG, "null pointer");
+  NKI_REQUIRE(aligned16(pages) && ((reinterpret_cast<uintptr_t>(tokens) | reinterpret_cast<uintptr_t>(sampled) |
+                                    reinterpret_cast<uintptr_t>(new_tokens)) & 7) == 0 &&
+                  aligned4(parents) && aligned4(cu_seqlens) && aligned4(kv_lens) && aligned4(page_table) &&
+                  aligned4(counts) && aligned4(path) && aligned4(status),
+              NKIMOE_ERR_INVALID_ARG, "pages must be 16-byte aligned, the others to their type");
+  NKI_CUDA(accept_drafts_launch(reinterpret_cast<const long long*>(tokens), reinterpret_cast<const long long*>(sampled),
+                                parents, cu_seqlens, kv_lens, pages, planes, num_pages, static_cast<int>(n_kv_heads),
+                                static_cast<int>(page_size), static_cast<int>(row_bytes), page_table, table_stride,
+                                static_cast<int>(max_pages), counts, path, reinterpret_cast<long long*>(new_tokens), T,
+                                static_cast<int>(batch), status, static_cast<cudaStream_t>(stream)));
   return NKIMOE_OK;
 }
 

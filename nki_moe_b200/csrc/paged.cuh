@@ -274,4 +274,24 @@ cudaError_t token_logprobs_launch(const void* logits, int dtype, long long row_s
                                   long long T, long long V, int top_n, float* logprob, float* entropy, float* top_lp,
                                   long long* top_ids, void* workspace, cudaStream_t s);
 
+// A sampling step's settings: one per row, or (null) one for all.
+struct SampleSettings {
+  const float* temperature;
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  double temperature_all, top_p_all, min_p_all;
+  long long top_k_all;
+};
+cudaError_t sample_tokens_launch(const void* logits, int dtype, long long row_stride, const void* uniforms, bool u_f64,
+                                 const SampleSettings& set, long long rows, long long V, long long* tokens,
+                                 float* logprob, cudaStream_t s);
+
+constexpr int kTreeNodes = 64;  // nodes of a sequence's tree at most
+cudaError_t accept_drafts_launch(const long long* tokens, const long long* sampled, const int* parents, const int* cu_seqlens,
+                                 const int* kv_lens, void* pages, long long planes, long long num_pages, int n_heads,
+                                 int page_size, int row_bytes, const int* table, long long table_stride, int max_pages,
+                                 int* counts, int* path, long long* new_tokens, long long T, int B, int* status,
+                                 cudaStream_t s);
+
 }  // namespace nkimoe

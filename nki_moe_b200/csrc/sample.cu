@@ -1,0 +1,683 @@
+// Draws a token from every row of logits: softmax of x / temperature,
+// restricted to the first top_k tokens (in the order of falling logits, equal
+// ones by the lower id), of those to the fewest that hold top_p of their sum,
+// and to weights of at least min_p times the largest; then the first id whose
+// running sum over the kept ids, in rising order, exceeds u times the whole.
+//
+//   d_i = x_i - max x,  w_i = 2^(d_i log2(e) / temperature)
+//   token = min { i kept : sum_{j <= i, kept} w_j > u S },  log p = log w - log S
+//
+// The random number u is the caller's.  Which token comes out depends on sums
+// over up to V weights next to a border, so the sums have to be better than
+// fp32: a border lies within 2^-24 S of u S for one row in a hundred when 10^5
+// tokens are kept.  Weights and sums are fp64; where the order of addition
+// would depend on timing (histograms) they are added as integers.
+//
+// A cluster of CTAs holds a row in shared memory, each a slice, so the logits
+// are read from HBM once and every later pass is local.  top_k and top_p are
+// found alike: a histogram over 1024 distances from the maximum (1/32 of a
+// binary order each) of counts or of weights, the bin where the sum passes the
+// border, then that bin's tokens sorted by the cluster's first CTA.  A bin of
+// more tokens than the sort takes is split further, by its own smallest and
+// largest (logit, id).
+//
+// Reference: the sampling of the reference's runtime is not vendored; no
+// kernel of its own.
+#include <cooperative_groups.h>
+
+#include "paged.cuh"
+
+namespace nkimoe {
+
+namespace cg = cooperative_groups;
+
+namespace {
+
+constexpr int kSmThreads = 512;
+constexpr int kSmWarps = kSmThreads / 32;
+constexpr int kSmBins = 1024;
+constexpr int kSmBinsPerOctave = 32;
+constexpr int kSmList = 2048;        // tokens that the last sort takes
+constexpr int kSmCluster = 8;        // CTAs per row at most
+constexpr int kSmSlice = 96 * 1024;  // bytes of a row per CTA that two CTAs per SM leave room for
+constexpr int kSmMaxVocab = 1 << 18;
+static_assert(2 * kSmThreads == kSmBins, "two bins per thread");
+
+using u64 = unsigned long long;
+
+struct SmParams {
+  const void* x;
+  long long row_stride;
+  const void* u;
+  const float* temperature;  // per row, or null: the value below
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  long long* tokens;
+  float* logprob;
+  double temperature_all, top_p_all, min_p_all;
+  long long top_k_all;
+  int V, slice;  // slice: elements per CTA, whole 16-byte vectors
+  int u_f64;
+};
+
+struct SmShared {
+  float max_of[kSmCluster];
+  double sum_of[kSmCluster];
+  u64 lo_of[kSmCluster], hi_of[kSmCluster];
+  // what the first CTA tells all
+  int bin;        // -1: no border
+  double above;   // counts or weights before the bin
+  double target;
+  u64 lo, hi;     // the range that is split, as (order, id)
+  u64 border;     // the last kept (order, id)
+  int listed;     // the first CTA's: tokens in its list
+  int pick;
+  double warp_d[kSmWarps];
+  u64 warp_lo[kSmWarps], warp_hi[kSmWarps];
+  float warp_f[kSmWarps];
+  union {
+    struct {
+      unsigned a[kSmBins];  // counts, or the upper halves of weights
+      unsigned b[kSmBins];  // the lower halves
+    } hist;
+    u64 list[kSmList];
+  };
+};
+
+// Integers that rise as the values fall; -0 equal to +0.
+__device__ __forceinline__ unsigned falling(float x) {
+  const unsigned b = __float_as_uint(x + 0.0f);
+  return ~(b & 0x80000000u ? ~b : b | 0x80000000u);
+}
+__device__ __forceinline__ float falling_value(unsigned o) {
+  const unsigned b = ~o;
+  return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+}
+
+// 2^t for t <= 1, 0 from -1022 on: t = n + f with |f| <= 1/2, 2^f by its Taylor
+// series about 0 (the first term left out is 0.35^12 / 12! = 2^-47), 2^n by the exponent.
+__device__ __forceinline__ double pow2(double t) {
+  const double big = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is rint(t)
+  const double s = t + big;
+  const int n = __double2loint(s);
+  const double f = (t - (s - big)) * 0.69314718055994530942;
+  double y = 1.0 / 39916800.0;
+  y = fma(y, f, 1.0 / 3628800.0);
+  y = fma(y, f, 1.0 / 362880.0);
+  y = fma(y, f, 1.0 / 40320.0);
+  y = fma(y, f, 1.0 / 5040.0);
+  y = fma(y, f, 1.0 / 720.0);
+  y = fma(y, f, 1.0 / 120.0);
+  y = fma(y, f, 1.0 / 24.0);
+  y = fma(y, f, 1.0 / 6.0);
+  y = fma(y, f, 0.5);
+  y = fma(y, f, 1.0);
+  y = fma(y, f, 1.0);
+  return t < -1022.0 ? 0.0 : __hiloint2double(__double2hiint(y) + (n << 20), __double2loint(y));
+}
+
+__device__ __forceinline__ float sm_float(float v) { return v; }
+__device__ __forceinline__ float sm_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// One row's settings and what is known of it.
+struct SmRow {
+  double c;    // log2(e) / temperature
+  double max;  // the largest logit
+  float maxf;
+  float bins;  // bins per unit of x
+  double min_weight;
+  u64 border;  // the last (order, id) that is kept so far
+
+  __device__ __forceinline__ double exponent(float x) const { return (static_cast<double>(x) - max) * c; }
+  __device__ __forceinline__ int bin(float x) const {
+    return __float2int_rn(fminf(fminf(maxf - x, 3e38f) * bins, kSmBins - 1.f));
+  }
+};
+
+// The CTA's part of the row.
+template <typename T>
+struct SmSlice {
+  static constexpr int VE = 16 / sizeof(T);
+  const uint4* data;
+  int vecs;
+  int id0;  // of the first element (a vector may begin before the row: -inf there)
+
+  __device__ __forceinline__ void get(int v, float (&x)[VE]) const {
+    const uint4 u = data[v];
+    if constexpr (sizeof(T) == 2) {
+      unpack8(u, x);
+    } else {
+      x[0] = __uint_as_float(u.x);
+      x[1] = __uint_as_float(u.y);
+      x[2] = __uint_as_float(u.z);
+      x[3] = __uint_as_float(u.w);
+    }
+  }
+  // f(logit, id) for every finite logit up to the row's border
+  template <typename F>
+  __device__ __forceinline__ void each(u64 border, F f) const {
+    const float least = border == ~0ull ? -INFINITY : falling_value(static_cast<unsigned>(border >> 32));
+    for (int v = threadIdx.x; v < vecs; v += kSmThreads) {
+      float x[VE];
+      get(v, x);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        if (x[i] == -INFINITY || x[i] < least) continue;
+        const int id = id0 + v * VE + i;
+        if (x[i] == least && ((static_cast<u64>(falling(x[i])) << 32) | static_cast<unsigned>(id)) > border) continue;
+        f(x[i], id);
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ u64 composite(float x, int id) {
+  return (static_cast<u64>(falling(x)) << 32) | static_cast<unsigned>(id);
+}
+
+// Running sums over the CTA's threads in order, each thread's before it and with
+// it (the one is bit for bit the other of the thread before); `total` gets the whole.
+struct SmSums {
+  double before, upto;
+};
+__device__ __forceinline__ SmSums sm_scan(double v, double* warp_d, double& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double w = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += w;
+  }
+  double prev = __shfl_up_sync(0xffffffffu, v, 1);
+  if (lane == 0) prev = 0.0;
+  __syncthreads();  // warp_d is free
+  if (lane == 31) warp_d[warp] = v;
+  __syncthreads();
+  double base = 0.0;
+  total = 0.0;
+  for (int w = 0; w < kSmWarps; ++w) {
+    if (w == warp) base = total;
+    total += warp_d[w];
+  }
+  return SmSums{base + prev, base + v};
+}
+
+// Whether this thread is the first whose running sums pass `need` (0 < need <=
+// the whole, so there is one).
+__device__ __forceinline__ bool sm_passes(const SmSums& s, double need, int* pick) {
+  if (threadIdx.x == 0) *pick = kSmThreads;
+  __syncthreads();
+  if (s.before < need && need <= s.upto) atomicMin(pick, static_cast<int>(threadIdx.x));
+  __syncthreads();
+  return *pick == static_cast<int>(threadIdx.x);
+}
+
+// Finds the last (order, id) that is kept when tokens are taken in order until
+// their count reaches k (kMass false; `limit` is k) or their weight reaches
+// `limit` times the whole (kMass).  Only tokens up to row.border take part, and
+// row.border is what comes out.  All CTAs of the cluster call it and take the
+// same way through it.
+template <typename T, bool kMass>
+__device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const SmSlice<T>& sl, SmRow& row, double limit) {
+  const int tid = threadIdx.x, ranks = cl.num_blocks();
+  const bool first = cl.block_rank() == 0;
+  SmShared& lead = *cl.map_shared_rank(&sh, 0);
+  bool split = false;  // the range is [lo, hi], not yet: one bin of distances
+  u64 lo = 0, hi = 0, width = 0;
+  double top = 0.0;  // split: exponent of the range's largest weight
+  int bin = 0;
+
+  auto member = [&](float x, u64 key) { return split ? key >= lo && key <= hi : row.bin(x) == bin; };
+
+  for (int level = 0;; ++level) {
+    // ---- histogram of the range
+    for (int i = tid; i < kSmBins; i += kSmThreads) sh.hist.a[i] = sh.hist.b[i] = 0;
+    if (first && tid == 0) sh.listed = 0;
+    __syncthreads();
+    sl.each(row.border, [&](float x, int id) {
+      int at;
+      double y = 0.0;  // exponent of the weight relative to the bin
+      if (split) {
+        const u64 key = composite(x, id);
+        if (key < lo || key > hi) return;
+        at = static_cast<int>((key - lo) / width);
+        if (kMass) y = row.exponent(x) - top;
+      } else {
+        at = row.bin(x);
+        if (kMass) y = row.exponent(x) + at * (1.0 / kSmBinsPerOctave);
+      }
+      if constexpr (kMass) {
+        // in units of 2^-31, at most 2^32 - 1; the halves of 65536 weights add up in 32 bits
+        const double q = pow2(y) * 2147483648.0;
+        const unsigned w = q >= 4294967295.0 ? 0xffffffffu : __double2uint_rn(q);
+        atomicAdd(&sh.hist.a[at], w >> 16);
+        atomicAdd(&sh.hist.b[at], w & 0xffffu);
+      } else {
+        atomicAdd(&sh.hist.a[at], 1u);
+      }
+    });
+    cl.sync();
+    // ---- the first CTA joins the histograms and finds the bin
+    if (first) {
+      double v[2] = {0.0, 0.0};
+      for (int r = 0; r < ranks; ++r) {
+        const SmShared& o = *cl.map_shared_rank(&sh, r);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = 2 * tid + e;
+          v[e] += kMass ? fma(static_cast<double>(o.hist.a[i]), 65536.0, static_cast<double>(o.hist.b[i]))
+                        : static_cast<double>(o.hist.a[i]);
+        }
+      }
+      if constexpr (kMass) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          v[e] *= pow2(split ? top : (2 * tid + e) * (-1.0 / kSmBinsPerOctave)) * (1.0 / 2147483648.0);
+      }
+      double total;
+      const SmSums sums = sm_scan(v[0] + v[1], sh.warp_d, total);
+      if (level == 0 && tid == 0) {
+        sh.target = kMass ? fmax(limit * total, 1e-300) : limit;
+        sh.above = 0.0;
+        sh.bin = -1;
+      }
+      __syncthreads();
+      const double above = sh.above;
+      // what is left to reach; the sums of a split range differ from its bin's by their rounding
+      double need = sh.target - above;
+      const bool none = !kMass && level == 0 && total <= limit;
+      if (level > 0) need = fmin(fmax(need, 1e-300), total * (1.0 - 0x1p-50));
+      const bool here = sm_passes(sums, need, &sh.pick);
+      if (!none && here) {
+        const bool second = sums.before + v[0] < need && v[1] > 0.0;
+        const int at = 2 * tid + second;
+        const double ab = above + sums.before + (second ? v[0] : 0.0);
+        for (int r = 0; r < ranks; ++r) {
+          SmShared& o = *cl.map_shared_rank(&sh, r);
+          o.bin = at;
+          o.above = ab;
+        }
+      } else if (none && tid == 0) {
+        for (int r = 0; r < ranks; ++r) cl.map_shared_rank(&sh, r)->bin = -1;
+      }
+    }
+    cl.sync();
+    bin = sh.bin;
+    if (bin < 0) return;  // fewer than k
+    if (split) {
+      lo += width * bin;
+      hi = min(hi, lo + width - 1);
+    }
+    // ---- the bin's tokens to the first CTA
+    sl.each(row.border, [&](float x, int id) {
+      const u64 key = composite(x, id);
+      if (!member(x, key)) return;
+      const int at = atomicAdd(&lead.listed, 1);
+      if (at < kSmList) lead.list[at] = key;
+    });
+    cl.sync();
+    const int n = lead.listed;
+    if (n <= kSmList) {
+      if (first) {
+        int m = 32;
+        while (m < n) m <<= 1;
+        for (int i = n + tid; i < m; i += kSmThreads) sh.list[i] = ~0ull;
+        __syncthreads();
+        for (int size = 2; size <= m; size <<= 1)
+          for (int d = size >> 1; d > 0; d >>= 1) {
+            for (int i = tid; i < m / 2; i += kSmThreads) {
+              const int a = 2 * i - (i & (d - 1)), b = a + d;
+              const u64 ka = sh.list[a], kb = sh.list[b];
+              if ((ka > kb) == ((a & size) == 0)) {
+                sh.list[a] = kb;
+                sh.list[b] = ka;
+              }
+            }
+            __syncthreads();
+          }
+        // in order until the border is reached
+        constexpr int kEach = kSmList / kSmThreads;
+        double v[kEach], sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+          const int i = tid * kEach + e;
+          v[e] = i >= n ? 0.0 : kMass ? pow2(row.exponent(falling_value(static_cast<unsigned>(sh.list[i] >> 32)))) : 1.0;
+          sum += v[e];
+        }
+        double total;
+        const SmSums sums = sm_scan(sum, sh.warp_d, total);
+        const double need = fmin(fmax(sh.target - sh.above, 1e-300), total * (1.0 - 0x1p-50));
+        if (sm_passes(sums, need, &sh.pick)) {
+          double before = sums.before;
+          int at = tid * kEach;
+#pragma unroll
+          for (int e = 0; e + 1 < kEach; ++e)
+            if (at == tid * kEach + e && before + v[e] < need) {
+              before += v[e];
+              ++at;
+            }
+          const u64 border = sh.list[min(at, n - 1)];
+          for (int r = 0; r < ranks; ++r) cl.map_shared_rank(&sh, r)->border = border;
+        }
+      }
+      cl.sync();
+      row.border = sh.border;
+      return;
+    }
+    // ---- too many: the range from the smallest to the largest of them is split
+    u64 least = ~0ull, most = 0;
+    sl.each(row.border, [&](float x, int id) {
+      const u64 key = composite(x, id);
+      if (!member(x, key)) return;
+      least = min(least, key);
+      most = max(most, key);
+    });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    }
+    if ((tid & 31) == 0) {
+      sh.warp_lo[tid >> 5] = least;
+      sh.warp_hi[tid >> 5] = most;
+    }
+    __syncthreads();
+    if (tid < ranks) {
+      for (int w = 0; w < kSmWarps; ++w) {
+        least = min(least, sh.warp_lo[w]);
+        most = max(most, sh.warp_hi[w]);
+      }
+      SmShared& o = *cl.map_shared_rank(&sh, tid);
+      o.lo_of[cl.block_rank()] = least;
+      o.hi_of[cl.block_rank()] = most;
+    }
+    cl.sync();
+    lo = ~0ull;
+    hi = 0;
+    for (int r = 0; r < ranks; ++r) {
+      lo = min(lo, sh.lo_of[r]);
+      hi = max(hi, sh.hi_of[r]);
+    }
+    width = (hi - lo) / kSmBins + 1;
+    top = row.exponent(falling_value(static_cast<unsigned>(lo >> 32)));
+    split = true;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __grid_constant__ SmParams p) {
+  constexpr int VE = 16 / sizeof(T);
+  extern __shared__ __align__(16) uint8_t sm_raw[];
+  __shared__ SmShared sh;
+  const cg::cluster_group cl = cg::this_cluster();
+  const int ranks = cl.num_blocks(), rank = cl.block_rank();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const long long r = blockIdx.x / ranks;
+  uint4* const data = reinterpret_cast<uint4*>(sm_raw);
+  cl.barrier_arrive();  // no CTA is written to before it runs
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // ---- the slice, from the 16-byte boundary at or below the row's first element on
+  const T* const x = static_cast<const T*>(p.x) + r * p.row_stride;
+  const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  SmSlice<T> sl;
+  sl.data = data;
+  sl.id0 = rank * p.slice - mis;
+  sl.vecs = min(p.slice, max(0, p.V - sl.id0) + VE - 1) / VE;
+  for (int v = tid; v < sl.vecs; v += kSmThreads) {
+    const int id = sl.id0 + v * VE;
+    if (id >= 0 && id + VE <= p.V) {
+      cp_async_16(smem_u32(data + v), x + id, 16);
+    } else {
+      T* at = reinterpret_cast<T*>(data + v);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) at[i] = id + i >= 0 && id + i < p.V ? x[id + i] : static_cast<T>(-INFINITY);
+    }
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  const double temperature = p.temperature ? static_cast<double>(p.temperature[r]) : p.temperature_all;
+  const long long top_k = p.top_k ? p.top_k[r] : p.top_k_all;
+  const double top_p = p.top_p ? static_cast<double>(p.top_p[r]) : p.top_p_all;
+  const double min_p = p.min_p ? static_cast<double>(p.min_p[r]) : p.min_p_all;
+  const double u = p.u_f64 ? static_cast<const double*>(p.u)[r] : static_cast<double>(static_cast<const float*>(p.u)[r]);
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+  // ---- the largest logit (a NaN comes through)
+  float mx = -INFINITY;
+  bool nan = false;
+  for (int v = tid; v < sl.vecs; v += kSmThreads) {  // what this thread copied
+    float e[VE];
+    sl.get(v, e);
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      nan |= e[i] != e[i];
+      mx = fmaxf(mx, e[i]);
+    }
+  }
+  mx = warp_max(mx);
+  if (__any_sync(0xffffffffu, nan)) mx = __int_as_float(0x7fc00000);
+  if (lane == 0) sh.warp_f[warp] = mx;
+  __syncthreads();
+  cl.barrier_wait();
+  if (tid < ranks) {
+    mx = -INFINITY;
+    for (int w = 0; w < kSmWarps; ++w) mx = mx != mx || sh.warp_f[w] != sh.warp_f[w] ? __int_as_float(0x7fc00000) : fmaxf(mx, sh.warp_f[w]);
+    cl.map_shared_rank(&sh, tid)->max_of[rank] = mx;
+  }
+  cl.sync();
+  mx = -INFINITY;
+  for (int q = 0; q < ranks; ++q) mx = mx != mx || sh.max_of[q] != sh.max_of[q] ? __int_as_float(0x7fc00000) : fmaxf(mx, sh.max_of[q]);
+  if (!(fabsf(mx) < INFINITY) || !(temperature >= 0.0)) {  // no distribution
+    if (rank == 0 && tid == 0) {
+      p.tokens[r] = -1;
+      p.logprob[r] = __int_as_float(0x7fc00000);
+    }
+    return;
+  }
+
+  if (temperature == 0.0 || top_k == 1) {  // the largest, the lowest id of equal ones
+    int id = 0x7fffffff;
+    sl.each(~0ull, [&](float e, int i) {
+      if (e == mx) id = min(id, i);
+    });
+    id = __reduce_min_sync(0xffffffffu, id);
+    if (lane == 0) sh.warp_lo[warp] = static_cast<u64>(id);
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 0; w < kSmWarps; ++w) id = min(id, static_cast<int>(sh.warp_lo[w]));
+      cl.map_shared_rank(&sh, 0)->lo_of[rank] = static_cast<u64>(id);
+    }
+    cl.sync();
+    if (rank == 0 && tid == 0) {
+      for (int q = 0; q < ranks; ++q) id = min(id, static_cast<int>(sh.lo_of[q]));
+      p.tokens[r] = id;
+      p.logprob[r] = 0.f;
+    }
+    return;
+  }
+
+  SmRow row;
+  row.c = 1.4426950408889634074 / temperature;
+  row.max = static_cast<double>(mx);
+  row.maxf = mx;
+  row.bins = static_cast<float>(fmin(row.c * kSmBinsPerOctave, 1e30));
+  row.min_weight = min_p > 0.0 ? fmin(min_p, 1.0) : 0.0;
+  row.border = ~0ull;
+  if (top_k > 0 && top_k < p.V) sm_select<T, false>(cl, sh, sl, row, static_cast<double>(top_k));
+  if (top_p < 1.0) sm_select<T, true>(cl, sh, sl, row, top_p);
+
+  // ---- the kept weights' sums, a warp's vectors being neighbours
+  const float least = row.border == ~0ull ? -INFINITY : falling_value(static_cast<unsigned>(row.border >> 32));
+  const int per = (sl.vecs + kSmWarps - 1) / kSmWarps;
+  const int v_lo = min(sl.vecs, warp * per), v_hi = min(sl.vecs, v_lo + per);
+  auto weight = [&](float e, int id) {
+    if (e == -INFINITY || e < least || (e == least && composite(e, id) > row.border)) return 0.0;
+    const double w = pow2(row.exponent(e));
+    return w >= row.min_weight ? w : 0.0;
+  };
+  double sum = 0.0;
+  for (int v = v_lo + lane; v < v_hi; v += 32) {
+    float e[VE];
+    sl.get(v, e);
+#pragma unroll
+    for (int i = 0; i < VE; ++i) sum += weight(e[i], sl.id0 + v * VE + i);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  __syncthreads();
+  if (lane == 0) sh.warp_d[warp] = sum;
+  __syncthreads();
+  if (tid < ranks) {
+    double all = 0.0;
+    for (int w = 0; w < kSmWarps; ++w) all += sh.warp_d[w];
+    cl.map_shared_rank(&sh, tid)->sum_of[rank] = all;
+  }
+  cl.sync();
+
+  // ---- the CTA, the warp and the token where the running sum passes u S
+  double whole = 0.0;
+  for (int q = 0; q < ranks; ++q) whole += sh.sum_of[q];
+  const double goal = u * whole;
+  double before = 0.0, at = 0.0;
+  int here = -1;
+  for (int q = 0; q < ranks; ++q) {
+    if (sh.sum_of[q] > 0.0) {
+      here = q;
+      before = at;
+      if (at + sh.sum_of[q] > goal) break;
+    }
+    at += sh.sum_of[q];
+  }
+  if (here != rank) return;
+  at = before;
+  here = -1;
+  for (int w = 0; w < kSmWarps; ++w) {
+    if (sh.warp_d[w] > 0.0) {
+      here = w;
+      before = at;
+      if (at + sh.warp_d[w] > goal) break;
+    }
+    at += sh.warp_d[w];
+  }
+  if (here != warp) return;
+  int token = -1;      // the last kept one so far, in every lane
+  double weight_of = 0.0;
+  for (int v0 = v_lo; v0 < v_hi; v0 += 32) {
+    const int v = v0 + lane;
+    double w[VE], mine = 0.0;
+    int last = -1;
+    double last_w = 0.0;
+    if (v < v_hi) {
+      float e[VE];
+      sl.get(v, e);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        w[i] = weight(e[i], sl.id0 + v * VE + i);
+        mine += w[i];
+        if (w[i] > 0.0) {
+          last = sl.id0 + v * VE + i;
+          last_w = w[i];
+        }
+      }
+    }
+    double upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    const unsigned over = __ballot_sync(0xffffffffu, mine > 0.0 && before + upto > goal);
+    if (over) {
+      const int from = __ffs(over) - 1;
+      if (lane == from) {
+        double s = before + (upto - mine);
+        int pick = last;
+        double pick_w = last_w;
+        bool found = false;
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          s += w[i];
+          if (!found && w[i] > 0.0 && s > goal) {
+            found = true;
+            pick = sl.id0 + v * VE + i;
+            pick_w = w[i];
+          }
+        }
+        token = pick;
+        weight_of = pick_w;
+      }
+      token = __shfl_sync(0xffffffffu, token, from);
+      weight_of = __shfl_sync(0xffffffffu, weight_of, from);
+      break;
+    }
+    const unsigned some = __ballot_sync(0xffffffffu, last >= 0);
+    if (some) {
+      const int from = 31 - __clz(some);
+      token = __shfl_sync(0xffffffffu, last, from);
+      weight_of = __shfl_sync(0xffffffffu, last_w, from);
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  if (lane == 0) {
+    p.tokens[r] = token;
+    p.logprob[r] = static_cast<float>(log(weight_of / whole));
+  }
+}
+
+template <typename T>
+cudaError_t sm_launch(const SmParams& params, long long rows, cudaStream_t s) {
+  constexpr int VE = 16 / sizeof(T);
+  SmParams p = params;
+  // as few CTAs per row as hold it at two per SM; more where rows are few
+  const long long vecs = (static_cast<long long>(p.V) + VE - 1 + VE - 1) / VE;  // a row may begin inside a vector
+  int ranks = 1;
+  while (ranks < kSmCluster && ((vecs + ranks - 1) / ranks) * 16 > kSmSlice) ranks *= 2;
+  while (ranks < kSmCluster && rows * ranks < device_sm_count() && vecs > 64 * ranks) ranks *= 2;
+  p.slice = static_cast<int>((vecs + ranks - 1) / ranks) * VE;
+  const size_t smem = static_cast<size_t>(p.slice) * sizeof(T);
+  constexpr int kMost = kSmMaxVocab * sizeof(T) / kSmCluster;
+  cudaError_t e = allow_smem<sample_tokens_kernel<T>>((kMost > kSmSlice ? kMost : kSmSlice) + 64);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * ranks));
+  cfg.blockDim = dim3(kSmThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T>, p);
+}
+
+}  // namespace
+
+cudaError_t sample_tokens_launch(const void* logits, int dtype, long long row_stride, const void* uniforms, bool u_f64,
+                                 const SampleSettings& set, long long rows, long long V, long long* tokens,
+                                 float* logprob, cudaStream_t s) {
+  SmParams p{};
+  p.x = logits;
+  p.row_stride = row_stride;
+  p.u = uniforms;
+  p.u_f64 = u_f64;
+  p.temperature = set.temperature;
+  p.top_k = set.top_k;
+  p.top_p = set.top_p;
+  p.min_p = set.min_p;
+  p.temperature_all = set.temperature_all;
+  p.top_k_all = set.top_k_all;
+  p.top_p_all = set.top_p_all;
+  p.min_p_all = set.min_p_all;
+  p.tokens = tokens;
+  p.logprob = logprob;
+  p.V = static_cast<int>(V);
+  return dtype == kF32 ? sm_launch<float>(p, rows, s) : sm_launch<__nv_bfloat16>(p, rows, s);
+}
+
+}  // namespace nkimoe

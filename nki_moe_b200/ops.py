@@ -19,7 +19,7 @@ from collections import OrderedDict
 import torch
 
 from . import _lib
-from ._lib import BF16, F32, I32, I64, LAYOUT_HF, LAYOUT_NXD, call, size_call
+from ._lib import BF16, F32, F64, I32, I64, LAYOUT_HF, LAYOUT_NXD, call, size_call
 
 __all__ = [
     "rmsnorm", "add_rmsnorm", "qk_norm_rope", "router_logits", "topk_softmax", "permute",
@@ -29,6 +29,7 @@ __all__ = [
     "moe_block_add_rmsnorm", "moe_block_host", "kmajor_weights",
     "release_captured_workspaces", "moe_block_rmsnorm", "qk_norm_rope_store", "paged_decode_attention",
     "paged_prefill_attention", "copy_pages", "token_logprobs", "read_paged_status",
+    "accept_drafts", "sample_tokens",
 ]
 
 _DT = {torch.float32: F32, torch.bfloat16: BF16, torch.int32: I32, torch.int64: I64}
@@ -639,6 +640,111 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0):
              tokens.data_ptr(), T, V, top_n, lp.data_ptr(), ent.data_ptr(), top_lp.data_ptr(), top_ids.data_ptr(),
              ws.data_ptr(), ws.numel(), s)
     return lp, ent, top_lp, top_ids
+
+
+def _setting(value, name: str, dtype: torch.dtype, rows: int, dev: int):
+    """A sampling setting as the C pair (array of a value per row, value for all)."""
+    if not isinstance(value, torch.Tensor):
+        return None, value
+    if value.dtype != dtype or value.shape != (rows,) or not value.is_contiguous() or value.get_device() != dev:
+        raise ValueError(f"{name} must be a number or a contiguous {dtype} [{rows}] tensor on cuda:{dev}")
+    return value.data_ptr(), 0
+
+
+@_on_its_device
+def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """A token from every row of logits, and the logarithm of its probability:
+    ``(tokens [T] int64, logprob [T] fp32)``.
+
+    ``logits``: ``[T, V]`` bf16 or fp32, rows at any stride, V at most 2^18;
+    ``uniforms``: ``[T]`` fp32 or fp64, a random number of [0, 1) per row.  The
+    distribution is ``softmax(logits / temperature)`` restricted, in the order of
+    falling logits (equal ones by the lower id), to the first ``top_k`` tokens (0:
+    all), of those to the fewest that hold ``top_p`` of their sum (at least one),
+    and to probabilities of at least ``min_p`` times the largest.  The token is
+    the first id whose running sum over the kept ids, in rising order, exceeds
+    ``uniforms`` times the whole.  ``temperature`` 0: the largest logit, the
+    lowest id of equal ones, logprob 0.
+
+    Each setting is a number or a tensor ``[T]`` with one per row (fp32; ``top_k``
+    int32), in which ``top_k < 1``, ``top_p >= 1`` and ``min_p <= 0`` restrict
+    nothing.  -inf logits are never drawn; a row with a NaN, a +inf or only -inf,
+    or with a negative or NaN temperature, has no distribution and gives -1 and
+    NaN."""
+    _cuda(logits, "logits")
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("logits must be fp32 or bf16 [T, V]")
+    T, V = logits.shape
+    if V == 0 or (V > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must have contiguous, non-empty rows")
+    dev = logits.get_device()
+    if not uniforms.is_cuda or uniforms.dtype not in (torch.float32, torch.float64) or uniforms.shape != (T,) \
+            or not uniforms.is_contiguous():
+        raise ValueError(f"uniforms must be a contiguous CUDA fp32 or fp64 [{T}] tensor")
+    _same_device(dev, "uniforms", uniforms)
+    settings = (*_setting(temperature, "temperature", torch.float32, T, dev),
+                *_setting(top_k, "top_k", torch.int32, T, dev), *_setting(top_p, "top_p", torch.float32, T, dev),
+                *_setting(min_p, "min_p", torch.float32, T, dev))
+    tokens = torch.empty(T, dtype=torch.int64, device=logits.device)
+    lp = torch.empty(T, dtype=torch.float32, device=logits.device)
+    call("nkimoe_sample_tokens", logits.data_ptr(), _DT[logits.dtype], logits.stride(0) if T > 1 else V,
+         uniforms.data_ptr(), F32 if uniforms.dtype == torch.float32 else F64, *settings, T, V, tokens.data_ptr(),
+         lp.data_ptr(), _raw_stream(dev))
+    return tokens, lp
+
+
+def _node_ids(t: torch.Tensor, name: str, dtype: torch.dtype, T: int) -> None:
+    if not t.is_cuda or t.dtype != dtype or t.shape != (T,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous CUDA {dtype} [{T}] tensor")
+
+
+@_on_its_device
+def accept_drafts(tokens: torch.Tensor, sampled: torch.Tensor, parents: torch.Tensor, cu_seqlens: torch.Tensor,
+                  kv_lens: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor):
+    """The end of a step with drafted tokens: ``(counts [B] int32, path [T] int32,
+    new_tokens [T] int64)``, and the kept drafts' keys and values in place.
+
+    Packed trees (see :func:`paged_tree_attention`): ``tokens`` int64 ``[T]``, node
+    0 of a sequence being its current token, ``sampled`` int64 ``[T]`` what was
+    drawn after every node, ``parents``, ``cu_seqlens``, ``kv_lens`` as there.  The
+    path begins at node 0 and goes on to the lowest child whose token is what was
+    drawn, until there is none; of a sequence's rows in ``path`` and ``new_tokens``
+    the first ``counts[b]`` hold its nodes and what was drawn after them, the
+    others -1.  In ``pages`` (a pool ``[..., pages, n_kv_heads, page_size,
+    head_dim]``, contiguous, any type) the rows of the path's nodes move to the
+    places right behind what the cache held before, so that the sequence goes on
+    from ``kv_len - n + counts[b]`` positions."""
+    _cuda(tokens, "tokens")
+    T, dev = tokens.numel(), tokens.device
+    _node_ids(tokens, "tokens", torch.int64, T)
+    _node_ids(sampled, "sampled", torch.int64, T)
+    _node_ids(parents, "parents", torch.int32, T)
+    B = _lengths(cu_seqlens, kv_lens)
+    shape = pages.shape
+    if not pages.is_cuda or len(shape) < 4 or not pages.is_contiguous() or pages.numel() == 0:
+        raise ValueError("pages must be contiguous CUDA [..., pages, n_kv_heads, page_size, head_dim]")
+    if not page_table.is_cuda or page_table.dtype != torch.int32 or page_table.dim() != 2:
+        raise ValueError("page_table must be CUDA int32 [sequences, pages per sequence]")
+    rows, width = page_table.shape
+    if rows < B or width == 0 or (width > 1 and page_table.stride(1) != 1):
+        raise ValueError(f"page_table must have contiguous rows for {B} sequences")
+    _same_device(dev.index, "sampled parents cu_seqlens kv_lens pages page_table", sampled, parents, cu_seqlens, kv_lens,
+                 pages, page_table)
+    counts = torch.empty(B, dtype=torch.int32, device=dev)
+    path = torch.empty(T, dtype=torch.int32, device=dev)
+    new = torch.empty(T, dtype=torch.int64, device=dev)
+    if B == 0 or T == 0:
+        return counts.zero_(), path.fill_(-1), new.fill_(-1)
+    s = _raw_stream(dev.index)
+    ws = _paged_workspace(dev, s, 0)
+    call("nkimoe_accept_drafts", tokens.data_ptr(), sampled.data_ptr(), parents.data_ptr(), cu_seqlens.data_ptr(),
+         kv_lens.data_ptr(), pages.data_ptr(), pages.numel() // (shape[-1] * shape[-2] * shape[-3] * shape[-4]),
+         shape[-4], shape[-3], shape[-2], shape[-1] * pages.element_size(), page_table.data_ptr(),
+         page_table.stride(0) if rows > 1 else width, width, counts.data_ptr(), path.data_ptr(), new.data_ptr(), T, B,
+         ws.data_ptr(), s)
+    if "NKIMOE_SYNC_CHECK" in os.environ and sync_check_enabled():
+        read_status(ws)
+    return counts, path, new
 
 
 # ---------------------------------------------------------------- router

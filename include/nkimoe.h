@@ -265,6 +265,36 @@ NKIMOE_API int nkimoe_paged_prefill_attention(const void* q, int64_t q_row_strid
                                               int n_heads, int n_kv_heads, int head_dim, float scale, int64_t window,
                                               int64_t sinks, void* workspace, size_t workspace_bytes, void* stream);
 
+NKIMOE_API size_t nkimoe_paged_tree_attention_workspace_bytes(int64_t T, int64_t batch, int n_heads, int n_kv_heads,
+                                                              int64_t max_pages, int64_t page_size);
+
+/* Trees of drafted tokens over the pages, fused as the decode step is: the
+ * packed rows qkv [T, (n_heads + 2*n_kv_heads) * 128] (bf16, before the q/k
+ * norms) are nodes, cu_seqlens and kv_lens as in nkimoe_qk_norm_rope_store.
+ * Node i of a sequence's n (at most 64) lies in place kv_len - n + i of its
+ * cache and stands at position kv_len - n + its depth; parents int32 [T] is its
+ * parent's index among the sequence's nodes, which is below its own, or -1.
+ * The rows get q/k RMSNorm + RoPE at their positions, keys and values are
+ * stored in their places' pages, and a node attends to the places before the
+ * tree that its position sees (window, sinks), and of its ancestors and itself
+ * to those whose positions it sees.  out: bf16 [T, n_heads * 128], not
+ * overlapping qkv; rows from cu_seqlens[batch] on are left alone.  A parent
+ * that is not below its child counts as -1 and is reported
+ * (NKIMOE_DEV_BAD_INDEX), as are lengths that make no sense or more than 64
+ * nodes, whose rows are left unwritten, and a page that a node needs and that
+ * is not held.  Rows of the cache before the tree, and the nodes' own, must be
+ * finite.  At most 16 query heads per kv head.
+ * Reference: the attention of qwen_with_nki.py:330-350, which sees one token or
+ * a causal prompt. */
+NKIMOE_API int nkimoe_paged_tree_attention(const void* qkv, const void* q_weight, const void* k_weight, int w_dtype,
+                                           const int32_t* parents, const int32_t* cu_seqlens, const int32_t* kv_lens,
+                                           void* k_pages, void* v_pages, int64_t k_page_stride, int64_t v_page_stride,
+                                           int64_t num_pages, int64_t page_size, const int32_t* page_table,
+                                           int64_t table_stride, int64_t max_pages, void* out, int64_t T,
+                                           int64_t batch, int n_heads, int n_kv_heads, int head_dim, float rope_theta,
+                                           float eps, float scale, int64_t window, int64_t sinks, void* workspace,
+                                           size_t workspace_bytes, void* stream);
+
 /* Copies page src[i] to page dst[i] (i < n) in each of `planes` pools of
  * num_pages pages of page_bytes bytes (a multiple of 16), one behind the other
  * at `pages`.  src and dst are HOST arrays, read before the call returns and

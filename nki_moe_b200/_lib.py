@@ -51,6 +51,9 @@ SIGNATURES = {
     "nkimoe_paged_prefill_attention": (_i, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
                                             _i64, _i64, _i, _i, _i, _f, _i64, _i64, _vp, _sz, _vp]),
     "nkimoe_copy_pages": (_i, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "nkimoe_paged_tree_attention_workspace_bytes": (_sz, [_i64, _i64, _i, _i, _i64, _i64]),
+    "nkimoe_paged_tree_attention": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64,
+                                         _i64, _vp, _i64, _i64, _i, _i, _i, _f, _f, _f, _i64, _i64, _vp, _sz, _vp]),
     "nkimoe_accept_drafts": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
                                   _vp, _i64, _i64, _vp, _vp]),
     "nkimoe_sample_tokens": (_i, [_vp, _i, _i64, _vp, _i, _vp, _d, _vp, _i64, _vp, _d, _vp, _d, _i64, _i64, _vp, _vp,

@@ -24,8 +24,8 @@ BUILD = os.path.join(REPO, "_build")
 LIB = os.path.join(PKG, "libnkimoe.so")
 SOURCES = ["norm.cu", "router.cu", "permute.cu", "pack.cu", "grouped_gemm.cu", "ep_peer.cu", "capi.cu",
            "noalloc.cu", "attention.cu", "linear.cu", "paged_store.cu", "paged_copy.cu", "paged_decode.cu",
-           "paged_prefill.cu", "logprobs.cu", "sample.cu", "accept.cu", "capi_paged.cu"]
-HEADERS = ["common.cuh", "kernels.h", "rope.cuh", "permute_small.cuh", "paged.cuh"]
+           "paged_prefill.cu", "paged_tree.cu", "logprobs.cu", "sample.cu", "accept.cu", "capi_paged.cu"]
+HEADERS = ["common.cuh", "kernels.h", "rope.cuh", "permute_small.cuh", "paged.cuh", "paged_mma.cuh", "paged_tree.cuh"]
 
 
 def nvcc() -> str:

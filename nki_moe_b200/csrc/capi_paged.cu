@@ -1,6 +1,6 @@
 // C ABI of the paged key-value cache and the token scores (include/nkimoe.h):
 // argument checks in front of the launches of paged_store.cu, paged_copy.cu,
-// paged_decode.cu, paged_prefill.cu, accept.cu, logprobs.cu and sample.cu.
+// paged_decode.cu, paged_prefill.cu, paged_tree.cu, accept.cu, logprobs.cu and sample.cu.
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
@@ -221,6 +221,53 @@ int nkimoe_paged_prefill_attention(const void* q, int64_t q_row_stride, const vo
                                 static_cast<__nv_bfloat16*>(out), T, static_cast<int>(batch), n_heads, scale,
                                 static_cast<int>(window), static_cast<int>(sinks), workspace,
                                 static_cast<cudaStream_t>(stream)));
+  return NKIMOE_OK;
+}
+
+size_t nkimoe_paged_tree_attention_workspace_bytes(int64_t T, int64_t batch, int n_heads, int n_kv_heads,
+                                                   int64_t max_pages, int64_t page_size) {
+  if (T < 0 || batch < 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > 16 ||
+      max_pages <= 0 || page_size <= 0 || page_size > 256 || max_pages > (1LL << 30) / page_size || T > (1 << 24) ||
+      batch > (1 << 20))
+    return 0;
+  return paged_tree_workspace_bytes(T, batch, n_heads, n_kv_heads, max_pages, static_cast<int>(page_size));
+}
+
+int nkimoe_paged_tree_attention(const void* qkv, const void* q_weight, const void* k_weight, int w_dtype,
+                                const int32_t* parents, const int32_t* cu_seqlens, const int32_t* kv_lens, void* k_pages,
+                                void* v_pages, int64_t k_page_stride, int64_t v_page_stride, int64_t num_pages,
+                                int64_t page_size, const int32_t* page_table, int64_t table_stride, int64_t max_pages,
+                                void* out, int64_t T, int64_t batch, int n_heads, int n_kv_heads, int head_dim,
+                                float rope_theta, float eps, float scale, int64_t window, int64_t sinks,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  NKI_CHECK(check_heads(n_heads, n_kv_heads, head_dim));
+  NKI_CHECK(check_window(window, sinks));
+  NKI_CHECK(check_scale(scale));
+  NKI_REQUIRE(T >= 0 && batch >= 0, NKIMOE_ERR_INVALID_ARG, "bad shape");
+  NKI_REQUIRE(T <= (1 << 24) && batch <= (1 << 20), NKIMOE_ERR_UNSUPPORTED, "shape too large");
+  NKI_REQUIRE(w_dtype == NKIMOE_F32 || w_dtype == NKIMOE_BF16, NKIMOE_ERR_INVALID_ARG, "bad weight dtype");
+  NKI_REQUIRE(rope_theta > 0.f, NKIMOE_ERR_INVALID_ARG, "rope_theta must be positive");
+  if (T == 0 || batch == 0) return NKIMOE_OK;
+  PagedCache c;
+  NKI_CHECK(check_cache(k_pages, v_pages, k_page_stride, v_page_stride, num_pages, page_size, page_table, table_stride,
+                        max_pages, n_kv_heads, &c));
+  // the places of all units are counted in 32 bits
+  const int64_t units = (kTreeNodes * (n_heads / n_kv_heads) + 127) / 128;
+  NKI_REQUIRE(batch * units * n_kv_heads * ((max_pages * page_size + 127) / 128 + 2) < 0x7fff0000LL,
+              NKIMOE_ERR_UNSUPPORTED, "batch and page table too large");
+  NKI_REQUIRE(k_page_stride < (1LL << 38) && v_page_stride < (1LL << 38), NKIMOE_ERR_UNSUPPORTED, "stride too large");
+  NKI_REQUIRE(qkv && q_weight && k_weight && parents && cu_seqlens && kv_lens && out && workspace,
+              NKIMOE_ERR_INVALID_ARG, "null pointer");
+  NKI_REQUIRE(aligned16(qkv) && aligned16(out) && aligned16(workspace) && aligned4(parents) && aligned4(cu_seqlens) &&
+                  aligned4(kv_lens),
+              NKIMOE_ERR_INVALID_ARG, "qkv, out and workspace must be 16-byte aligned, parents and lengths 4-byte aligned");
+  const size_t need =
+      paged_tree_workspace_bytes(T, batch, n_heads, n_kv_heads, max_pages, static_cast<int>(page_size));
+  NKI_REQUIRE(workspace_bytes >= need, NKIMOE_ERR_WORKSPACE, "workspace %zu bytes < %zu", workspace_bytes, need);
+  NKI_CUDA(paged_tree_launch(static_cast<const __nv_bfloat16*>(qkv), q_weight, k_weight, w_dtype, parents, cu_seqlens,
+                             kv_lens, c, static_cast<__nv_bfloat16*>(out), T, static_cast<int>(batch), n_heads,
+                             rope_theta, eps, scale, static_cast<int>(window), static_cast<int>(sinks), workspace,
+                             static_cast<cudaStream_t>(stream)));
   return NKIMOE_OK;
 }
 

@@ -288,6 +288,12 @@ cudaError_t sample_tokens_launch(const void* logits, int dtype, long long row_st
                                  float* logprob, cudaStream_t s);
 
 constexpr int kTreeNodes = 64;  // nodes of a sequence's tree at most
+size_t paged_tree_workspace_bytes(long long T, long long B, int nq, int nkv, long long max_pages, int page_size);
+cudaError_t paged_tree_launch(const __nv_bfloat16* qkv, const void* qw, const void* kw, int w_dtype,
+                              const int* parents, const int* cu_seqlens, const int* kv_lens, const PagedCache& cache,
+                              __nv_bfloat16* out, long long T, int B, int nq, float theta, float eps, float scale,
+                              int window, int sinks, void* workspace, cudaStream_t s);
+
 cudaError_t accept_drafts_launch(const long long* tokens, const long long* sampled, const int* parents, const int* cu_seqlens,
                                  const int* kv_lens, void* pages, long long planes, long long num_pages, int n_heads,
                                  int page_size, int row_bytes, const int* table, long long table_stride, int max_pages,

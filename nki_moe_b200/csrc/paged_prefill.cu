@@ -55,31 +55,19 @@
 // than a CTA's share of all blocks (a chunk over a long cache), every CTA takes
 // an equal run of the list of blocks instead, the pairs that are cut leave
 // partial results, and a third kernel joins them.
-#include <cudaTypedefs.h>
-
-#include "paged.cuh"
+#include "paged_mma.cuh"
 
 namespace nkimoe {
 
 namespace {
 
-constexpr int kPfBlock = 128;                  // key positions per block
-constexpr int kPfRows = 128;                   // MMA rows per tile
 constexpr int kPfThreads = 384;
 constexpr int kPfRing = 4;                     // stages of 32 KB
-constexpr uint32_t kPfTileBytes = kPfRows * kHeadDim * 2;    // 32 KB: a Q tile
-constexpr uint32_t kPfTileHalf = kPfTileBytes / 2;           // one 64-column half (128 rows x 128 bytes)
-constexpr uint32_t kPfBlockBytes = kPfBlock * kHeadDim * 2;  // 32 KB: a K block or a V block
-constexpr uint32_t kPfBlockHalf = kPfBlockBytes / 2;
 constexpr size_t kPfSmem = 1024 + 2 * kPfTileBytes + kPfRing * kPfBlockBytes;
 // A part of a cut pair, per tile: o four columns at a time [32][128 rows][4],
 // then the rows' m, then their l (a warp's rows are neighbours: coalesced)
 constexpr int kPfPartTile = (kHeadDim + 2) * kPfRows;
 constexpr int kPfMinBlocks = 4;                // key blocks of a part at least
-constexpr float kPfLog2e = 1.4426950408889634f;
-constexpr float kPfSlack = 8.f;                // log2 by which a block may exceed the running maximum
-// tensor memory columns: S of tile t at 128 t (P over its first half), O at 256 + 128 t
-constexpr uint32_t kPfTmemO = 256;
 
 // A unit, for each kv head.
 struct __align__(16) PfUnit {
@@ -122,21 +110,6 @@ struct PfParams {
   int sms, max_pairs;
   float scale_log2;
 };
-
-// The key blocks of queries at positions [lo, hi]: those of the first `sinks`
-// positions, then from the first block of lo's window on.
-struct Blocks {
-  int sink, first, n;
-  __device__ __forceinline__ int at(int i) const { return i < sink ? i : i - sink + first; }
-};
-__device__ __forceinline__ Blocks blocks_of(int lo, int hi, int window, int sinks) {
-  Blocks r;
-  const int start = window && lo >= window ? lo - window + 1 : 0;
-  r.first = start / kPfBlock;
-  r.sink = start > 0 ? min((min(sinks, start) + kPfBlock - 1) / kPfBlock, r.first) : 0;
-  r.n = r.sink + hi / kPfBlock - r.first + 1;
-  return r;
-}
 
 // New rows of sequence b, 0 where its lengths make no sense (flagged).
 __device__ __forceinline__ int pf_rows(const PfParams& p, int b, int& kv, bool flag) {
@@ -240,66 +213,6 @@ __global__ void __launch_bounds__(kPlanThreads) paged_prefill_plan_kernel(const 
     const bool cut = longest > share && blocks < (1LL << 30);
     *p.list = PfList{pairs, 0, static_cast<int>(min(blocks, 1LL << 30)), cut ? static_cast<int>(share) : 0};
   }
-}
-
-// ------------------------------------------------------------------ tensor memory, MMA with A from tensor memory
-__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// D += A B with A (bf16 pairs, one row per lane) in tensor memory
-__device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                             uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate));
-}
-
-// Descriptor of a 128-byte-swizzled MN-major operand: blocks of 64 columns
-// (leading byte offset: the distance of two blocks), 8 rows of K every 1024 bytes.
-__device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t smem_addr, uint32_t block_bytes) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
-  d |= static_cast<uint64_t>(block_bytes >> 4) << 16;
-  d |= static_cast<uint64_t>(1024u >> 4) << 32;
-  d |= static_cast<uint64_t>(1u) << 46;
-  d |= static_cast<uint64_t>(2u) << 61;
-  return d;
-}
-
-__device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, uint64_t* bar, int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::
-          "r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
-__device__ __forceinline__ void tma_load_4d(void* dst, const void* tmap, uint64_t* bar, int c0, int c1, int c2,
-                                            int c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
-      "[%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-      : "memory");
-}
-
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
-// The lowest n bits (none for n <= 0, all for n >= 32).
-__device__ __forceinline__ uint32_t low_bits(int n) {
-  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
 }
 
 // What the roles need to know of a unit; tokens 0: there are no more.
@@ -848,28 +761,9 @@ cudaError_t paged_prefill_launch(const __nv_bfloat16* q, long long q_stride, con
   if (!encode) return cudaErrorNotSupported;
   const int nkv = cache.nkv, grp = nq / nkv, tpt = kPfRows / grp, page = 1 << cache.page_shift;
   CUtensorMap mq, mk, mv;
-  {
-    const cuuint64_t dims[3] = {kHeadDim, static_cast<cuuint64_t>(nq), static_cast<cuuint64_t>(T)};
-    const cuuint64_t strides[2] = {kHeadDim * 2, static_cast<cuuint64_t>(q_stride) * 2};
-    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(grp), static_cast<cuuint32_t>(tpt)};
-    const cuuint32_t one[3] = {1, 1, 1};
-    if (encode(&mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<__nv_bfloat16*>(q), dims, strides, box, one,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return cudaErrorInvalidValue;
-  }
-  for (int i = 0; i < 2; ++i) {
-    const cuuint64_t dims[4] = {kHeadDim, static_cast<cuuint64_t>(page), static_cast<cuuint64_t>(nkv),
-                                static_cast<cuuint64_t>(cache.num_pages)};
-    const cuuint64_t strides[3] = {kHeadDim * 2, static_cast<cuuint64_t>(page) * kHeadDim * 2,
-                                   static_cast<cuuint64_t>(i ? cache.v_stride : cache.k_stride) * 2};
-    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(page < kPfBlock ? page : kPfBlock), 1, 1};
-    const cuuint32_t one[4] = {1, 1, 1, 1};
-    if (encode(i ? &mv : &mk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, i ? cache.v : cache.k, dims, strides, box, one,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return cudaErrorInvalidValue;
-  }
+  if (!tmap_of_rows(encode, &mq, q, nq, T, q_stride, grp, tpt) || !tmap_of_pages(encode, &mk, cache, false) ||
+      !tmap_of_pages(encode, &mv, cache, true))
+    return cudaErrorInvalidValue;
   const PfLayout L = pf_layout(T, B, nkv, grp, cache.max_pages, page);
   char* ws = static_cast<char*>(workspace);
   PfParams p;

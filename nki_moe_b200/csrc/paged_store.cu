@@ -6,7 +6,9 @@
 // attention; the reference's caches are the runtime's own (not vendored).
 #include <math.h>
 
-#include "paged.cuh"
+#include <type_traits>
+
+#include "paged_tree.cuh"
 
 namespace nkimoe {
 
@@ -28,6 +30,13 @@ struct StoreParams {
   long long T;
   int w_dtype, B, nq;
   float eps;
+};
+
+// The rows are nodes of trees: a row's place is where it is stored, its depth
+// makes its position.
+struct TreeStoreParams : StoreParams {
+  const int* parents;
+  TrPlan plan;
 };
 
 // The sequence whose rows hold row t: the number of starts cu[1..B) that are
@@ -55,8 +64,9 @@ __device__ __forceinline__ int sequence_of(const int* cu, int B, int t, int lane
 // issue at 64 %: neither is full, a row's chain of lookups, sines and packing is
 // what it waits for.  15 rows 5.1 us.  Of that 4 us and 1.5 us are the keys formed
 // again in 64 bits (their check alone 0.3 us).
-template <int kWarps>
-__global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_store_kernel(const __grid_constant__ StoreParams p) {
+template <int kWarps, typename Params>
+__global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_store_kernel(const __grid_constant__ Params p) {
+  constexpr bool kTree = std::is_same<Params, TreeStoreParams>::value;
   constexpr int D = kHeadDim;
   constexpr int kHalves = 2 * kWarps;                     // heads of a row at a time
   constexpr int kAhead = kWarps >= 4 ? 3 : 5;             // heads per half-warp in flight
@@ -64,10 +74,17 @@ __global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_stor
   __shared__ __align__(16) float2 tab[kStoreThreads / 32][D / 2];
   const int lane = threadIdx.x & 31, l = threadIdx.x & 15, warp = threadIdx.x >> 5;
   const int half = (warp % kWarps) * 2 + (lane >> 4);
-  const long long t = static_cast<long long>(blockIdx.x) * (kStoreThreads / 32 / kWarps) + warp / kWarps;
+  // of trees the first CTA makes the list of what the attention does
+  const long long t = static_cast<long long>(blockIdx.x - kTree) * (kStoreThreads / 32 / kWarps) + warp / kWarps;
   const int nh = p.nq + 2 * p.c.nkv;
   pdl_launch_dependents();
   pdl_wait();
+  if constexpr (kTree) {
+    if (blockIdx.x == 0) {
+      tree_plan<kStoreThreads>(p.plan, p.c, p.cu, p.kv_lens, p.T, p.B, p.status);
+      return;
+    }
+  }
   const uint2* row = reinterpret_cast<const uint2*>(p.qkv + t * nh * D) + l;  // head h: row[32 h], row[32 h + 16]
   uint2 raw[kAhead][2];
 #pragma unroll
@@ -83,11 +100,24 @@ __global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_stor
   if (t >= p.T || t >= p.cu[p.B]) return;  // behind the last sequence
   const int b = sequence_of(p.cu, p.B, static_cast<int>(t), lane);
   const int start = p.cu[b], end = p.cu[b + 1];
-  const int pos = p.kv_lens[b] - end + static_cast<int>(t);
-  const int slot = pos >> p.c.page_shift;
-  if (t < start || t >= end || pos < 0 || slot >= p.c.max_pages) {
+  const int place = p.kv_lens[b] - end + static_cast<int>(t);
+  const int slot = place >> p.c.page_shift;
+  if (t < start || t >= end || place < 0 || slot >= p.c.max_pages) {
     if (lane == 0) atomicOr(p.status, kDevErrBadIndex);
     return;
+  }
+  int pos = place;
+  bool keep_lo = false;  // of the queries
+  if constexpr (kTree) {
+    const int n = end - start, i = static_cast<int>(t) - start;
+    if (n > kTreeNodes || place < i) {  // the list holds no unit of such a sequence
+      if (lane == 0) atomicOr(p.status, kDevErrBadIndex);
+      return;
+    }
+    const TrRow line = tree_line(p.parents + start, n, i, place - i, p.plan.window, p.plan.sinks, lane, p.status);
+    pos = line.pos;
+    keep_lo = n - i / (2 * p.plan.tpt) * (2 * p.plan.tpt) <= p.plan.tpt;  // a unit of one tile
+    if (lane == 0 && warp % kWarps == 0) p.plan.rows[t] = line;
   }
   const int page = p.c.table[b * p.c.table_stride + slot];
   const bool held = page >= 0 && page < p.c.num_pages;
@@ -97,7 +127,7 @@ __global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_stor
   __syncwarp();
   const TurnPart turn = turn_part(tab[warp], l);
   // where the row's heads go, this lane's part
-  const int in_page = pos & ((1 << p.c.page_shift) - 1), head_shift = p.c.page_shift + 5;  // in 8-byte pieces
+  const int in_page = place & ((1 << p.c.page_shift) - 1), head_shift = p.c.page_shift + 5;  // in 8-byte pieces
   uint2* const q_dst = reinterpret_cast<uint2*>(p.q_out + t * p.nq * D) + l;
   uint2* const k_dst = reinterpret_cast<uint2*>(p.c.k + (held ? page * p.c.k_stride + in_page * D : 0)) + l;
   uint2* const v_dst = reinterpret_cast<uint2*>(p.c.v + (held ? page * p.c.v_stride + in_page * D : 0)) + l;
@@ -124,6 +154,17 @@ __global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_stor
         if (!is_v) {  // a value goes bit for bit
           lo = row_of_pairs(o.a);
           hi = row_of_pairs(o.b);
+          if constexpr (kTree) {
+            if (is_q && keep_lo && h < nh) {
+              const uint64_t minus = pair2(-1.f, -1.f);
+              const HeadPart top = part_of_rows(lo, hi);
+              const uint64_t ra[2] = {fma2(top.a[0], minus, o.a[0]), fma2(top.a[1], minus, o.a[1])};
+              const uint64_t rb[2] = {fma2(top.b[0], minus, o.b[0]), fma2(top.b[1], minus, o.b[1])};
+              uint2* const rest = reinterpret_cast<uint2*>(p.plan.q_lo + t * p.nq * D) + l + h * 32;
+              rest[0] = row_of_pairs(ra);
+              rest[16] = row_of_pairs(rb);
+            }
+          }
           if (!is_q) again |= key_near_tie(o) << (4 * ((h0 / kHalves + i) & 7));
         }
       }
@@ -172,10 +213,9 @@ RopeTurns rope_turns(float theta) {
   return r;
 }
 
-cudaError_t paged_store_launch(const __nv_bfloat16* qkv, const void* qw, const void* kw, int w_dtype,
-                               const int* cu_seqlens, const int* kv_lens, const PagedCache& cache,
-                               __nv_bfloat16* q_out, long long T, int B, int nq, float theta, float eps, int* status,
-                               cudaStream_t s) {
+static StoreParams store_params(const __nv_bfloat16* qkv, const void* qw, const void* kw, int w_dtype,
+                                const int* cu_seqlens, const int* kv_lens, const PagedCache& cache,
+                                __nv_bfloat16* q_out, long long T, int B, int nq, float theta, float eps, int* status) {
   StoreParams p;
   p.qkv = qkv;
   p.qw = qw;
@@ -191,12 +231,36 @@ cudaError_t paged_store_launch(const __nv_bfloat16* qkv, const void* qw, const v
   p.B = B;
   p.nq = nq;
   p.eps = eps;
+  return p;
+}
+
+cudaError_t paged_store_launch(const __nv_bfloat16* qkv, const void* qw, const void* kw, int w_dtype,
+                               const int* cu_seqlens, const int* kv_lens, const PagedCache& cache,
+                               __nv_bfloat16* q_out, long long T, int B, int nq, float theta, float eps, int* status,
+                               cudaStream_t s) {
+  const StoreParams p =
+      store_params(qkv, qw, kw, w_dtype, cu_seqlens, kv_lens, cache, q_out, T, B, nq, theta, eps, status);
   // few rows: a CTA's eight warps on each; many: a warp each, so that the lookups
   // and the sines of a row are done once (8192 rows of 32 + 2 * 4 heads, before keys
   // were formed again: 37 us, with two warps 46, with eight 42)
   if (T <= kStoreFew)
-    return launch_pdl(paged_store_kernel<8>, dim3(static_cast<unsigned>(T)), dim3(kStoreThreads), 0, s, p);
-  return launch_pdl(paged_store_kernel<1>, dim3(static_cast<unsigned>((T + 7) / 8)), dim3(kStoreThreads), 0, s, p);
+    return launch_pdl(paged_store_kernel<8, StoreParams>, dim3(static_cast<unsigned>(T)), dim3(kStoreThreads), 0, s, p);
+  return launch_pdl(paged_store_kernel<1, StoreParams>, dim3(static_cast<unsigned>((T + 7) / 8)), dim3(kStoreThreads), 0, s,
+                    p);
+}
+
+cudaError_t paged_tree_store_launch(const __nv_bfloat16* qkv, const void* qw, const void* kw, int w_dtype,
+                                    const int* parents, const int* cu_seqlens, const int* kv_lens,
+                                    const PagedCache& cache, __nv_bfloat16* q_out, long long T, int B, int nq,
+                                    float theta, float eps, const TrPlan& plan, int* status, cudaStream_t s) {
+  TreeStoreParams p;
+  static_cast<StoreParams&>(p) = store_params(qkv, qw, kw, w_dtype, cu_seqlens, kv_lens, cache, q_out, T, B, nq, theta, eps, status);
+  p.parents = parents;
+  p.plan = plan;
+  if (T <= kStoreFew)
+    return launch_pdl(paged_store_kernel<8, TreeStoreParams>, dim3(static_cast<unsigned>(T + 1)), dim3(kStoreThreads), 0, s, p);
+  return launch_pdl(paged_store_kernel<1, TreeStoreParams>, dim3(static_cast<unsigned>((T + 7) / 8 + 1)), dim3(kStoreThreads),
+                    0, s, p);
 }
 
 }  // namespace nkimoe

@@ -29,7 +29,7 @@ __all__ = [
     "moe_block_add_rmsnorm", "moe_block_host", "kmajor_weights",
     "release_captured_workspaces", "moe_block_rmsnorm", "qk_norm_rope_store", "paged_decode_attention",
     "paged_prefill_attention", "copy_pages", "token_logprobs", "read_paged_status",
-    "accept_drafts", "sample_tokens",
+    "paged_tree_attention", "accept_drafts", "sample_tokens",
 ]
 
 _DT = {torch.float32: F32, torch.bfloat16: BF16, torch.int32: I32, torch.int64: I64}
@@ -556,6 +556,54 @@ def paged_prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     ws = _paged_workspace(dev, s, nbytes)
     call("nkimoe_paged_prefill_attention", q.data_ptr(), q.stride(0) if T > 1 else nq * 128, *cache,
          cu_seqlens.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), T, B, nq, nkv, 128,
+         128 ** -0.5 if scale is None else scale, window, sinks, ws.data_ptr(), ws.numel(), s)
+    if "NKIMOE_SYNC_CHECK" in os.environ and sync_check_enabled():
+        read_status(ws)
+    return out
+
+
+@_on_its_device
+def paged_tree_attention(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, parents: torch.Tensor,
+                         cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, k_pages: torch.Tensor,
+                         v_pages: torch.Tensor, page_table: torch.Tensor, n_heads: int, n_kv_heads: int,
+                         theta: float = 1e6, eps: float = 1e-6, scale: float | None = None, window: int = 0,
+                         sinks: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """One step of grouped-query attention for a tree of drafted tokens per
+    sequence over a paged cache, fused with the q/k RMSNorm + RoPE of the nodes
+    and the store of their keys and values (:func:`paged_decode_attention` for
+    more than one token).
+
+    ``qkv``: ``[T, (n_heads + 2*n_kv_heads) * 128]`` bf16 before the norms, the
+    sequences' nodes packed; ``cu_seqlens``, ``kv_lens``, ``k_pages``,
+    ``v_pages``, ``page_table`` as in :func:`qk_norm_rope_store`: node ``i`` of
+    ``n`` (at most 64) lies in place ``kv_len - n + i`` of the cache.
+    ``parents``: int32 ``[T]``, the index of a node's parent among its
+    sequence's nodes (below its own) or -1; a node's position, for RoPE and the
+    window, is ``kv_len - n`` and its depth.  A node sees what was in the cache
+    before the tree, its ancestors and itself, within ``window`` and ``sinks``
+    as in :func:`paged_decode_attention`.  Cached rows below ``kv_lens`` and the
+    nodes' own must be finite.  Returns ``[T, n_heads * 128]`` bf16 (``out``,
+    contiguous and apart from ``qkv``, if given); rows from ``cu_seqlens[B]`` on
+    are left as they were.  :func:`accept_drafts` keeps the path that is agreed
+    with."""
+    _cuda(qkv, "qkv")
+    row = (n_heads + 2 * n_kv_heads) * 128
+    if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != row or not qkv.is_contiguous():
+        raise ValueError(f"qkv must be a contiguous bf16 [T, {row}] tensor")
+    T, dev = qkv.shape[0], qkv.device
+    _node_ids(parents, "parents", torch.int32, T)
+    B = _lengths(cu_seqlens, kv_lens)
+    qw, kw, wdt = _norm_weights(q_weight, k_weight)
+    cache = _paged_cache(k_pages, v_pages, page_table, n_kv_heads, B)
+    _same_device(dev.index, "q_weight k_weight parents cu_seqlens kv_lens k_pages v_pages page_table", qw, kw, parents,
+                 cu_seqlens, kv_lens, k_pages, v_pages, page_table)
+    out = _rows_out(out, (T, n_heads * 128), qkv)
+    s = _raw_stream(dev.index)
+    nbytes = _paged_ws_bytes(dev.index, "nkimoe_paged_tree_attention_workspace_bytes", T, B, n_heads, n_kv_heads,
+                             cache[8], cache[5])
+    ws = _paged_workspace(dev, s, nbytes)
+    call("nkimoe_paged_tree_attention", qkv.data_ptr(), qw.data_ptr(), kw.data_ptr(), wdt, parents.data_ptr(),
+         cu_seqlens.data_ptr(), kv_lens.data_ptr(), *cache, out.data_ptr(), T, B, n_heads, n_kv_heads, 128, theta, eps,
          128 ** -0.5 if scale is None else scale, window, sinks, ws.data_ptr(), ws.numel(), s)
     if "NKIMOE_SYNC_CHECK" in os.environ and sync_check_enabled():
         read_status(ws)

@@ -251,9 +251,9 @@ int nkimoe_paged_tree_attention(const void* qkv, const void* q_weight, const voi
   PagedCache c;
   NKI_CHECK(check_cache(k_pages, v_pages, k_page_stride, v_page_stride, num_pages, page_size, page_table, table_stride,
                         max_pages, n_kv_heads, &c));
-  // the places of all units are counted in 32 bits
-  const int64_t units = (kTreeNodes * (n_heads / n_kv_heads) + 127) / 128;
-  NKI_REQUIRE(batch * units * n_kv_heads * ((max_pages * page_size + 127) / 128 + 2) < 0x7fff0000LL,
+  // the places of all tiles are counted in 32 bits
+  const int64_t tiles = (kTreeNodes + 128 / (n_heads / n_kv_heads) - 1) / (128 / (n_heads / n_kv_heads));
+  NKI_REQUIRE(batch * tiles * n_kv_heads * ((max_pages * page_size + 127) / 128 + 2) < 0x7fff0000LL,
               NKIMOE_ERR_UNSUPPORTED, "batch and page table too large");
   NKI_REQUIRE(k_page_stride < (1LL << 38) && v_page_stride < (1LL << 38), NKIMOE_ERR_UNSUPPORTED, "stride too large");
   NKI_REQUIRE(qkv && q_weight && k_weight && parents && cu_seqlens && kv_lens && out && workspace,

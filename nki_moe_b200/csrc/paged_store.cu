@@ -35,8 +35,7 @@ struct StoreParams {
 // The rows are nodes of trees: a row's place is where it is stored, its depth
 // makes its position.
 struct TreeStoreParams : StoreParams {
-  const int* parents;
-  TrPlan plan;
+  TreeOut tree;
 };
 
 // The sequence whose rows hold row t: the number of starts cu[1..B) that are
@@ -74,17 +73,13 @@ __global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_stor
   __shared__ __align__(16) float2 tab[kStoreThreads / 32][D / 2];
   const int lane = threadIdx.x & 31, l = threadIdx.x & 15, warp = threadIdx.x >> 5;
   const int half = (warp % kWarps) * 2 + (lane >> 4);
-  // of trees the first CTA makes the list of what the attention does
-  const long long t = static_cast<long long>(blockIdx.x - kTree) * (kStoreThreads / 32 / kWarps) + warp / kWarps;
+  const long long t = static_cast<long long>(blockIdx.x) * (kStoreThreads / 32 / kWarps) + warp / kWarps;
   const int nh = p.nq + 2 * p.c.nkv;
-  pdl_launch_dependents();
+  // the attention of trees reads what lies before them at once: it may start only
+  // when all that came before this kernel has ended
+  if (!kTree) pdl_launch_dependents();
   pdl_wait();
-  if constexpr (kTree) {
-    if (blockIdx.x == 0) {
-      tree_plan<kStoreThreads>(p.plan, p.c, p.cu, p.kv_lens, p.T, p.B, p.status);
-      return;
-    }
-  }
+  if (kTree) pdl_launch_dependents();
   const uint2* row = reinterpret_cast<const uint2*>(p.qkv + t * nh * D) + l;  // head h: row[32 h], row[32 h + 16]
   uint2 raw[kAhead][2];
 #pragma unroll
@@ -107,17 +102,15 @@ __global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_stor
     return;
   }
   int pos = place;
-  bool keep_lo = false;  // of the queries
   if constexpr (kTree) {
     const int n = end - start, i = static_cast<int>(t) - start;
-    if (n > kTreeNodes || place < i) {  // the list holds no unit of such a sequence
+    if (n > kTreeNodes || place < i) {  // the attention leaves such a sequence out
       if (lane == 0) atomicOr(p.status, kDevErrBadIndex);
       return;
     }
-    const TrRow line = tree_line(p.parents + start, n, i, place - i, p.plan.window, p.plan.sinks, lane, p.status);
+    const TrRow line = tree_line(p.tree.parents + start, n, i, place - i, p.tree.window, p.tree.sinks, lane, p.status);
     pos = line.pos;
-    keep_lo = n - i / (2 * p.plan.tpt) * (2 * p.plan.tpt) <= p.plan.tpt;  // a unit of one tile
-    if (lane == 0 && warp % kWarps == 0) p.plan.rows[t] = line;
+    if (lane == 0 && warp % kWarps == 0) p.tree.rows[t] = line;
   }
   const int page = p.c.table[b * p.c.table_stride + slot];
   const bool held = page >= 0 && page < p.c.num_pages;
@@ -155,12 +148,12 @@ __global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_stor
           lo = row_of_pairs(o.a);
           hi = row_of_pairs(o.b);
           if constexpr (kTree) {
-            if (is_q && keep_lo && h < nh) {
+            if (is_q && h < nh) {
               const uint64_t minus = pair2(-1.f, -1.f);
               const HeadPart top = part_of_rows(lo, hi);
               const uint64_t ra[2] = {fma2(top.a[0], minus, o.a[0]), fma2(top.a[1], minus, o.a[1])};
               const uint64_t rb[2] = {fma2(top.b[0], minus, o.b[0]), fma2(top.b[1], minus, o.b[1])};
-              uint2* const rest = reinterpret_cast<uint2*>(p.plan.q_lo + t * p.nq * D) + l + h * 32;
+              uint2* const rest = reinterpret_cast<uint2*>(p.tree.q_lo + t * p.nq * D) + l + h * 32;
               rest[0] = row_of_pairs(ra);
               rest[16] = row_of_pairs(rb);
             }
@@ -250,17 +243,17 @@ cudaError_t paged_store_launch(const __nv_bfloat16* qkv, const void* qw, const v
 }
 
 cudaError_t paged_tree_store_launch(const __nv_bfloat16* qkv, const void* qw, const void* kw, int w_dtype,
-                                    const int* parents, const int* cu_seqlens, const int* kv_lens,
-                                    const PagedCache& cache, __nv_bfloat16* q_out, long long T, int B, int nq,
-                                    float theta, float eps, const TrPlan& plan, int* status, cudaStream_t s) {
+                                    const int* cu_seqlens, const int* kv_lens, const PagedCache& cache,
+                                    __nv_bfloat16* q_out, long long T, int B, int nq, float theta, float eps,
+                                    const TreeOut& tree, int* status, cudaStream_t s) {
   TreeStoreParams p;
-  static_cast<StoreParams&>(p) = store_params(qkv, qw, kw, w_dtype, cu_seqlens, kv_lens, cache, q_out, T, B, nq, theta, eps, status);
-  p.parents = parents;
-  p.plan = plan;
+  static_cast<StoreParams&>(p) =
+      store_params(qkv, qw, kw, w_dtype, cu_seqlens, kv_lens, cache, q_out, T, B, nq, theta, eps, status);
+  p.tree = tree;
   if (T <= kStoreFew)
-    return launch_pdl(paged_store_kernel<8, TreeStoreParams>, dim3(static_cast<unsigned>(T + 1)), dim3(kStoreThreads), 0, s, p);
-  return launch_pdl(paged_store_kernel<1, TreeStoreParams>, dim3(static_cast<unsigned>((T + 7) / 8 + 1)), dim3(kStoreThreads),
-                    0, s, p);
+    return launch_pdl(paged_store_kernel<8, TreeStoreParams>, dim3(static_cast<unsigned>(T)), dim3(kStoreThreads), 0, s, p);
+  return launch_pdl(paged_store_kernel<1, TreeStoreParams>, dim3(static_cast<unsigned>((T + 7) / 8)), dim3(kStoreThreads), 0,
+                    s, p);
 }
 
 }  // namespace nkimoe

@@ -8,31 +8,32 @@
 // its ancestors and itself.  A node's place in the cache is where its row stands
 // in the tree, its position the length before the tree and its depth.
 //
-// Two launches come before: the store (paged_store.cu) norms and turns the rows,
-// puts keys and values in their pages and the queries in the workspace, works out
-// every node's line of ancestors as 64 bits, and one CTA of it makes the list of
-// units; a kernel after it joins what was cut.
+// The store before it (paged_store.cu) norms and turns the rows, puts keys and
+// values in their pages and the queries in the workspace, and works out every
+// node's line of ancestors as 64 bits; a kernel after it joins what was cut.
 //
 // Tile: 128 MMA rows are floor(128 / group) nodes times the `group` query heads
-// of one kv head.  A unit is up to two tiles of a sequence's nodes, for one kv
-// head, against key blocks of 128 places.  Warps as in paged_prefill.cu: one
-// loads Q and K, one V, one thread issues the MMAs, and a warpgroup per tile
-// takes S from tensor memory and leaves P there.  With two tiles both work on
-// the same block; with one (trees of up to 128 / group nodes) the two warpgroups
-// take the blocks in turn, each with its own maximum, sum and O, which are joined
-// at the unit's end: a block's chain (scores, softmax, product) takes longer than
-// its bytes take to come from HBM, two chains at a time do not.
+// of one kv head, against key blocks of 128 places.  One warp loads Q and K, one
+// V, one thread issues the MMAs, and two warpgroups take S from tensor memory,
+// a thread per row, and leave P there.  The warpgroups take a tile's blocks in
+// turn, each with its own maximum, sum and O, which are joined at its end: a
+// block's chain (scores, softmax, product, 4000 cycles) takes longer than its
+// bytes take to come from HBM (2800), two chains at a time do not.
 //
-// Arithmetic: bf16 operands, sums, maxima and O in fp32.  In a unit of one tile
-// queries and weights enter the MMAs as a sum of two bf16 (hi + lo, 2^-17), as in
-// the decode step: the second query tile and the columns of S beside P are free
-// for the lo parts there, and their MMAs fit into the time that a block's bytes
-// take.  In a unit of two tiles both are rounded to bf16 (2^-9, random over the
-// terms of a sum), as in the prompt attention.
+// Arithmetic: bf16 operands, sums, maxima and O in fp32.  Queries enter as a sum
+// of two bf16 (hi + lo, 2^-17) by a second MMA into the same scores; weights are
+// rounded to bf16 (2^-9 at most, random over the terms of a sum).  With the
+// queries rounded too the output's error against 64 bits is 1.8 times that of its
+// own rounding, so 1.4 times; weights as hi + lo bring it to 1.0, but take 2500
+// cycles more per block (37 sequences of 16 nodes over 16 K: 290 us, so 228, and
+// with rounded queries 201).
 //
-// Work: the blocks of all (unit, kv head) form one list, and every CTA takes an
-// equal run of it, so sequences of any mix of lengths load all SMs alike and the
-// launch needs no length on the host.
+// Work: the blocks of all (sequence, kv head, tile) form one list, and every CTA
+// takes an equal run of it, so sequences of any mix of lengths load all SMs alike
+// and the launch needs no length on the host.  Each CTA finds its run from the
+// lengths itself, and loads its first keys, while the store still runs: the
+// store lets this kernel start only once all that came before it has ended, so
+// what the store does not write may be read at once.
 #include "paged_tree.cuh"
 
 namespace nkimoe {
@@ -40,41 +41,49 @@ namespace nkimoe {
 namespace {
 
 constexpr int kTrThreads = 384;
-constexpr int kTrRing = 4;  // stages of 32 KB: K blocks in the even ones, V blocks in the odd ones
-constexpr size_t kTrSmem = 1024 + 2 * kPfTileBytes + kTrRing * kPfBlockBytes;
-// A part of a cut unit, per tile: o four columns at a time [32][128 rows][4],
-// then the rows' m, then their l (a warp's rows are neighbours: coalesced)
-constexpr int kTrPartTile = (kHeadDim + 2) * kPfRows;
+constexpr int kTrK = 3, kTrV = 2;  // stages of 32 KB: K blocks, V blocks
+constexpr int kTrItem = 1;         // key blocks that beginning and ending an item (sequence, kv head, tile) costs
+constexpr int kTrMinRun = 3;       // places of a CTA's run at least: a block for each warpgroup
+// A part of a cut item: o four columns at a time [32][128 rows][4], then the
+// rows' m, then their l (a warp's rows are neighbours: coalesced)
+constexpr int kTrPart = (kHeadDim + 2) * kPfRows;
+constexpr int kTrJoinRows = 8;     // rows per CTA of the join
 
-// What a CTA began and others went on with: the unit of a kv head whose parts
-// lie in slot 2 c + 1 of CTA c and the slots 0 of the CTAs after it.
+// What a CTA began and others went on with: the item whose parts lie in slot
+// 2 c + 1 of CTA c and the slots 0 of the CTAs after it.
 struct TrSplit {
-  int unit, j, parts, pad;
+  int row0, tokens, j, parts;
 };
 
 struct TrParams {
+  const int* cu;       // [B + 1]
+  const int* kv_lens;  // [B]
   __nv_bfloat16* out;  // [T, nq * 128]
   int* status;
-  const TrRow* rows;    // [T]
-  const TrList* list;
-  const TrUnit* units;
-  const int* offs;
-  TrSplit* splits;  // [grid]
-  float* part;      // [2 grid, 2, kTrPartTile]
+  const TrRow* rows;  // [T]
+  TrSplit* splits;    // [grid]
+  float* part;        // [2 grid, kTrPart]
   PagedCache c;
-  int nq, grp, tpt;  // tpt: nodes per tile
+  int T, B, nq, grp, tpt;  // tpt: nodes per tile
   int window, sinks;
   float scale_log2;
 };
 
-// What the roles need to know of a unit; tokens 0: there are no more.
-struct TrWork : TrUnit {
-  int j;  // kv head
+// What the roles need to know of an item; tokens 0: there are no more.
+struct TrWork {
+  int row0;    // first packed row of the tile
+  int tokens;  // its nodes
+  int past;    // places before the tree
+  int kv;      // places with it
+  int b, j;    // sequence, kv head
+  int lo, hi;  // range of key blocks
+  int slot;    // of the partial result, or -1
 };
 
 struct TrCtl {
   uint64_t q_full, q_empty;
-  uint64_t kv_full[kTrRing], kv_empty[kTrRing];
+  uint64_t k_full[kTrK], k_empty[kTrK];
+  uint64_t v_full[kTrV], v_empty[kTrV];
   uint64_t s_full[2], p_full[2], o_full[2];
   uint64_t u_full[2], u_empty[2];
   uint64_t ml_full, ml_empty;  // the softmax warps have left their maxima and sums; have read them and both O
@@ -82,27 +91,146 @@ struct TrCtl {
   TrWork work[2];
   uint32_t tmem_base;
   int abort_flag;
-  float2 ml[2][kPfRows];  // one tile: maximum and sum of both warpgroups
+  float2 ml[2][kPfRows];  // maximum and sum of both warpgroups
+};
+
+struct TrShared {  // on a 1024-byte boundary: the tiles are swizzled
+  uint8_t q[2][kPfTileBytes];  // hi, lo
+  uint8_t k[kTrK][kPfBlockBytes];
+  uint8_t v[kTrV][kPfBlockBytes];
+  TrCtl ctl;
+};
+static_assert(sizeof(TrShared) <= 227 * 1024, "shared memory of an SM");
+
+// A sequence's nodes and lengths; n 0: none, or they make no sense (flagged).
+struct TrSeq {
+  int row0, n, kv, blocks;
+};
+__device__ __forceinline__ TrSeq tr_sequence(const TrParams& p, int b, bool flag) {
+  TrSeq s{0, 0, 0, 0};
+  if (b >= p.B) return s;
+  s.row0 = p.cu[b];
+  s.n = p.cu[b + 1] - s.row0;
+  s.kv = p.kv_lens[b];
+  if (s.n == 0) return s;
+  if (s.row0 < 0 || s.n < 0 || s.row0 + s.n > p.T || s.n > kTreeNodes || s.kv < s.n ||
+      s.kv > static_cast<long long>(p.c.max_pages) << p.c.page_shift) {
+    if (flag) atomicOr(p.status, kDevErrBadIndex);
+    s.n = 0;
+    return s;
+  }
+  s.blocks = blocks_of(s.kv - s.n, s.kv - 1, p.window, p.sinks).n;
+  return s;
+}
+
+// The run of one CTA through the list of blocks (sequence, kv head, tile, block),
+// each item preceded by kTrItem places for its own cost; a warp walks it.
+struct TrRun {
+  int share, run_lo, run_hi;
+  int at;    // place in the list
+  int base;  // place of the first of sequence b
+  int b;
+  TrSeq mine;  // of sequence 32 * (b / 32) + lane
+
+  __device__ __forceinline__ int tiles(const TrParams& p, const TrSeq& s) const { return (s.n + p.tpt - 1) / p.tpt; }
+  __device__ __forceinline__ int places(const TrParams& p, const TrSeq& s) const {
+    return tiles(p, s) * p.c.nkv * (s.blocks + kTrItem);
+  }
+  __device__ __forceinline__ TrSeq of(int b) const {
+    const int l = b & 31;
+    return TrSeq{__shfl_sync(0xffffffffu, mine.row0, l), __shfl_sync(0xffffffffu, mine.n, l),
+                 __shfl_sync(0xffffffffu, mine.kv, l), __shfl_sync(0xffffffffu, mine.blocks, l)};
+  }
+
+  __device__ __forceinline__ void begin(const TrParams& p, int lane) {
+    int total = 0;
+    for (int c = 0; c < p.B; c += 32) {
+      mine = tr_sequence(p, c + lane, blockIdx.x == 0);
+      total += __reduce_add_sync(0xffffffffu, places(p, mine));
+    }
+    share = max(kTrMinRun, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+    run_lo = min(total, static_cast<int>(blockIdx.x) * share);
+    run_hi = min(total, run_lo + share);
+    at = run_lo;
+    base = b = 0;
+    if (at >= run_hi) return;
+    // the sequence of place `at`
+    for (int c = 0;; c += 32) {
+      if (p.B > 32) mine = tr_sequence(p, c + lane, false);
+      int incl = places(p, mine);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += x;
+      }
+      const int all = __shfl_sync(0xffffffffu, incl, 31);
+      if (base + all <= at) {
+        base += all;
+        continue;
+      }
+      const int l = __ffs(__ballot_sync(0xffffffffu, base + incl > at)) - 1;
+      b = c + l;
+      const int before = __shfl_sync(0xffffffffu, incl, l > 0 ? l - 1 : 0);
+      if (l > 0) base += before;
+      return;
+    }
+  }
+
+  // The run's next item, or one without nodes.
+  __device__ __forceinline__ TrWork next(const TrParams& p, int lane) {
+    TrWork w{};
+    if (at >= run_hi) return w;
+    TrSeq s = of(b);
+    while (at >= base + places(p, s)) {  // (there is a next one: at < run_hi <= the whole list)
+      base += places(p, s);
+      ++b;
+      if ((b & 31) == 0) mine = tr_sequence(p, b + lane, false);
+      s = of(b);
+    }
+    const int n = s.blocks, tls = tiles(p, s);
+    const int q = (at - base) / (n + kTrItem);
+    const int item = base + q * (n + kTrItem) + kTrItem;  // the list's first block of the item
+    const int tile = q % tls;
+    w.lo = max(at - item, 0);
+    w.hi = min(n, run_hi - item);
+    at = item + n;
+    if (w.hi <= 0) return TrWork{};  // the run ends before the item's blocks
+    w.row0 = s.row0 + tile * p.tpt;
+    w.tokens = min(p.tpt, s.n - tile * p.tpt);
+    w.past = s.kv - s.n;
+    w.kv = s.kv;
+    w.b = b;
+    w.j = q / tls;
+    const int first = item / share, parts = (item + n - 1) / share - first + 1;
+    w.slot = parts > 1 ? 2 * static_cast<int>(blockIdx.x) + (item < run_lo ? 0 : 1) : -1;
+    if (parts > 1 && item >= run_lo && lane == 0) p.splits[blockIdx.x] = TrSplit{w.row0, w.tokens, w.j, parts};
+    return w;
+  }
 };
 
 __global__ void __launch_bounds__(kTrThreads, 1)
-    paged_tree_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                      const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_lo,
+    paged_tree_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_lo,
+                      const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                       const __grid_constant__ TrParams p) {
-  extern __shared__ uint8_t tr_raw[];
-  __shared__ TrCtl ctl;
-  __shared__ __align__(16) __nv_bfloat16 stg[8][32][40];  // per softmax warp: 32 output columns of its rows
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tr_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* sq = smem;
-  uint8_t* ring = smem + 2 * kPfTileBytes;
+  extern __shared__ __align__(1024) uint8_t tr_raw[];
+  TrShared& sh = *reinterpret_cast<TrShared*>(tr_raw);
+  TrCtl& ctl = sh.ctl;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (smem_u32(tr_raw) & 1023u) {  // never: the kernel has no other shared memory
+    if (threadIdx.x == 0) atomicOr(p.status, kDevErrTmem);
+    return;
+  }
 
   if (threadIdx.x == 0) {
     mbar_init(&ctl.q_full, 1);
     mbar_init(&ctl.q_empty, 1);
-    for (int s = 0; s < kTrRing; ++s) {
-      mbar_init(&ctl.kv_full[s], 1);
-      mbar_init(&ctl.kv_empty[s], 1);
+    for (int s = 0; s < kTrK; ++s) {
+      mbar_init(&ctl.k_full[s], 1);
+      mbar_init(&ctl.k_empty[s], 1);
+    }
+    for (int s = 0; s < kTrV; ++s) {
+      mbar_init(&ctl.v_full[s], 1);
+      mbar_init(&ctl.v_empty[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&ctl.s_full[t], 1);
@@ -128,40 +256,42 @@ __global__ void __launch_bounds__(kTrThreads, 1)
   tcgen05_fence_after();
   const uint32_t tmem = ctl.tmem_base;
   pdl_launch_dependents();
-  pdl_wait();
   // 384 x 168 registers at launch = 128 x 88 + 256 x 208
   if (warp == 0 || warp == 2) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    // ---------------------------------------------------------------- units and loads
+    // ---------------------------------------------------------------- items and loads
     // Lane (h, g) loads half h of page g of a block.
     const int v = warp >> 1;
+    const int stages = v ? kTrV : kTrK;
+    uint8_t* const ring = v ? &sh.v[0][0] : &sh.k[0][0];
+    uint64_t* const full = v ? ctl.v_full : ctl.k_full;
+    uint64_t* const empty = v ? ctl.v_empty : ctl.k_empty;
     const int h_lane = (lane >> 3) & 1, g_lane = lane & 7;
     const int page_rows = min(1 << p.c.page_shift, kPfBlock);  // rows per box
     const bool loads = lane < 16 && g_lane * page_rows < kPfBlock;
     const void* const tm = v ? static_cast<const void*>(&tmap_v) : static_cast<const void*>(&tmap_k);
     const int box_at = h_lane * static_cast<int>(kPfBlockHalf) + g_lane * page_rows * 128;
-    const uint32_t q_bytes = 2u * p.grp * p.tpt * 128u;  // both halves of one tile's box
+    const uint32_t q_bytes = 2u * p.grp * p.tpt * 128u;  // both halves of the tile's box
     auto wait = [&](uint64_t* bar, uint32_t ph) {
       const bool got = mbar_wait(bar, ph, &ctl.abort_flag, p.status);
       return __all_sync(0xffffffffu, got);
     };
-    int stage = v;
+    int stage = 0;
     uint32_t phase = 0, issued = 0, last_phase = 0, tail_phase = 0;
     bool ok = true, q_issued = false;
-    const TrList list = *p.list;
-    const int run_lo = min(list.total, static_cast<int>(blockIdx.x) * list.share);
-    const int run_hi = min(list.total, run_lo + list.share);
-    int at = run_lo, unit = 0;
+    bool stored = false;  // the store before this kernel has ended
+    auto after_store = [&] {
+      if (!stored) pdl_wait();
+      stored = true;
+    };
+    TrRun run;
     if (v == 0) {
       if (lane == 0) p.splits[blockIdx.x].parts = 0;
-      for (int hi = list.units; hi - unit > 1;) {
-        const int mid = (unit + hi) >> 1;
-        if (p.offs[mid] <= at) unit = mid; else hi = mid;
-      }
+      run.begin(p, lane);
     }
     for (int u = 0; ok; ++u) {
       const int us = u & 1;
-      TrWork w{};
+      TrWork w;
       if (v) {
         if (!wait(&ctl.u_full[us], (u >> 1) & 1)) { ok = false; break; }
         w = ctl.work[us];
@@ -169,24 +299,7 @@ __global__ void __launch_bounds__(kTrThreads, 1)
         if (lane == 0) mbar_arrive(&ctl.u_empty[us]);
       } else {
         if (!wait(&ctl.u_empty[us], ((u >> 1) & 1) ^ 1u)) { ok = false; break; }
-        if (at < run_hi) {
-          static_cast<TrUnit&>(w) = p.units[unit];
-          const int n = w.hi, base = p.offs[unit];
-          w.j = (at - base) / (n + kTrItem);
-          // the list's first block of (unit, kv head), behind the places for its own cost
-          const int item = base + w.j * (n + kTrItem) + kTrItem;
-          w.lo = max(at - item, 0);
-          w.hi = min(n, run_hi - item);
-          const int first = item / list.share, parts = (item + n - 1) / list.share - first + 1;
-          if (w.hi <= 0) {
-            w.tokens = 0;  // the run ends before the item's blocks
-          } else {
-            if (parts > 1) w.slot = 2 * static_cast<int>(blockIdx.x) + (item < run_lo ? 0 : 1);
-            if (parts > 1 && item >= run_lo && lane == 0) p.splits[blockIdx.x] = TrSplit{unit, w.j, parts, 0};
-          }
-          at = item + w.hi;
-          if (w.hi == n && w.j == p.c.nkv - 1) ++unit;
-        }
+        w = run.next(p, lane);
         if (lane == 0) {
           ctl.work[us] = w;
           mbar_arrive(&ctl.u_full[us]);
@@ -204,17 +317,6 @@ __global__ void __launch_bounds__(kTrThreads, 1)
         return need ? table[s0 >> p.c.page_shift] : -2;
       };
       int next = look_up(w.lo);
-      if (v == 0) {
-        if (!wait(&ctl.q_empty, (u & 1) ^ 1u)) { ok = false; break; }
-        // two tiles, or one tile's hi and lo parts
-        const bool lo = w.tokens <= p.tpt && lane > 1;
-        if (lane == 0) mbar_arrive_expect_tx(&ctl.q_full, 2 * q_bytes);
-        __syncwarp();
-        if (lane < 4)
-          tma_load_3d(sq + (lane >> 1) * kPfTileBytes + (lane & 1) * kPfTileHalf, lo ? &tmap_lo : &tmap_q, &ctl.q_full,
-                      (lane & 1) * 64, w.j * p.grp, w.row0 + (lo ? 0 : (lane >> 1) * p.tpt));
-        q_issued = true;
-      }
       for (int i = w.lo; ok && i < w.hi; ++i) {
         const bool held = next >= 0 && next < p.c.num_pages;
         if (!held && next != -2) atomicOr(p.status, kDevErrBadIndex);
@@ -222,13 +324,14 @@ __global__ void __launch_bounds__(kTrThreads, 1)
         const int k0 = bl.at(i) * kPfBlock;
         const int in_page = (k0 + g_lane * page_rows) & ((1 << p.c.page_shift) - 1);
         if (i + 1 < w.hi) next = look_up(i + 1);  // in flight while this block waits for its stage
-        if (!wait(&ctl.kv_empty[stage], phase ^ 1u)) { ok = false; break; }
+        if (!wait(&empty[stage], phase ^ 1u)) { ok = false; break; }
+        if (k0 + kPfBlock > w.past) after_store();  // the tree's own rows are in the block
         // rows behind the sequence's end in its last page hold anything: their
         // weights are 0, and 0 times a NaN would not be, so this warp clears
         // them once the block is there (further pages are loaded as zeros)
         const int live = w.kv - k0;
         const bool clear = v == 1 && live < kPfBlock && (live & (page_rows - 1)) != 0;
-        uint64_t* const bar = clear ? &ctl.tail : &ctl.kv_full[stage];
+        uint64_t* const bar = clear ? &ctl.tail : &full[stage];
         if (lane == 0) mbar_arrive_expect_tx(bar, kPfBlockBytes);
         __syncwarp();
         uint8_t* const to = ring + stage * kPfBlockBytes;
@@ -243,22 +346,34 @@ __global__ void __launch_bounds__(kTrThreads, 1)
           }
           fence_proxy_async_shared();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl.kv_full[stage]);
+          if (lane == 0) mbar_arrive(&full[stage]);
         }
         issued |= 1u << stage;
         last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
-        stage += 2;
-        if (stage >= kTrRing) {
-          stage = v;
+        if (++stage == stages) {
+          stage = 0;
           phase ^= 1u;
+        }
+        // the item's queries after its first keys, which may go out before the store
+        // has ended, and while the item before still reads its own queries
+        if (v == 0 && i == w.lo) {
+          if (!wait(&ctl.q_empty, (u & 1) ^ 1u)) { ok = false; break; }
+          after_store();
+          if (lane == 0) mbar_arrive_expect_tx(&ctl.q_full, 2 * q_bytes);
+          __syncwarp();
+          if (lane < 4)
+            tma_load_3d(sh.q[lane >> 1] + (lane & 1) * kPfTileHalf, lane < 2 ? &tmap_q : &tmap_lo, &ctl.q_full,
+                        (lane & 1) * 64, w.j * p.grp, w.row0);
+          q_issued = true;
         }
       }
     }
+    after_store();
     if (!ok && lane == 0) {  // let the copies in flight land before the CTA exits
-      for (int s = 0; s < kTrRing; ++s)
+      for (int s = 0; s < stages; ++s)
         if ((issued >> s) & 1u) {
           const long long t0 = clock64();
-          while (!mbar_try_wait(&ctl.kv_full[s], (last_phase >> s) & 1u) && clock64() - t0 < kWaitBudgetCycles / 8) {
+          while (!mbar_try_wait(&full[s], (last_phase >> s) & 1u) && clock64() - t0 < kWaitBudgetCycles / 8) {
           }
         }
       if (q_issued || v) {
@@ -273,46 +388,29 @@ __global__ void __launch_bounds__(kTrThreads, 1)
     // ---------------------------------------------------------------- MMA issue (one thread)
     constexpr uint32_t idesc_s = umma_idesc_bf16_f32(kPfRows, kPfBlock);
     constexpr uint32_t idesc_o = umma_idesc_bf16_f32(kPfRows, kHeadDim) | (1u << 16);  // B is MN-major
-    uint32_t ks = 0, vs = 0, pphase = 0;  // K and V blocks taken so far; pphase: bit t, of p_full
+    int ks = 0, vs = 0;
+    uint32_t kphase = 0, vphase = 0, pphase = 0;  // pphase: bit t, of p_full
     bool ok = true, any = false;
     auto wait = [&](uint64_t* bar, uint32_t ph) { return mbar_wait(bar, ph, &ctl.abort_flag, p.status); };
-    auto k_stage = [&] { return 2 * (ks & 1); };
-    auto v_stage = [&] { return 2 * (vs & 1) + 1; };
-    auto k_here = [&] { return wait(&ctl.kv_full[k_stage()], (ks >> 1) & 1); };
-    auto v_here = [&] { return wait(&ctl.kv_full[v_stage()], (vs >> 1) & 1); };
-    // S of tile t against the K block in the current stage, with the queries of slots q_lo .. q_hi
-    auto issue_s = [&](int t, int q_lo, int q_hi) {
-      for (int q = q_lo; q <= q_hi; ++q) {
+    // S of warpgroup t against the next K block
+    auto issue_s = [&](int t) {
+      if (!wait(&ctl.k_full[ks], kphase)) return false;
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint64_t da = umma_desc_sw128(smem_u32(sq + q * kPfTileBytes + h * kPfTileHalf));
-          const uint64_t db = umma_desc_sw128(smem_u32(ring + k_stage() * kPfBlockBytes + h * kPfBlockHalf));
+          const uint64_t da = umma_desc_sw128(smem_u32(sh.q[q] + h * kPfTileHalf));
+          const uint64_t db = umma_desc_sw128(smem_u32(sh.k[ks] + h * kPfBlockHalf));
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_bf16(tmem + t * 128, da + 2 * k, db + 2 * k, idesc_s, q > q_lo || (h | k) != 0);
+          for (int k = 0; k < 4; ++k) umma_bf16(tmem + t * 128, da + 2 * k, db + 2 * k, idesc_s, (q | h | k) != 0);
         }
-      }
       umma_commit(&ctl.s_full[t]);
+      umma_commit(&ctl.k_empty[ks]);
       any = true;
-    };
-    auto k_done = [&] {
-      umma_commit(&ctl.kv_empty[k_stage()]);
-      ++ks;
-    };
-    // O += P V of tile t; lo: P's lo part lies behind it
-    auto issue_o = [&](int t, bool more, bool lo) {
-      const uint64_t dv = umma_desc_sw128_mn(smem_u32(ring + v_stage() * kPfBlockBytes), kPfBlockHalf);
-#pragma unroll
-      for (int k = 0; k < 8; ++k)  // 16 positions: 2048 bytes of V, 8 columns of P
-        umma_bf16_ts(tmem + kPfTmemO + t * 128, tmem + t * 128 + 8 * k, dv + 128 * k, idesc_o, more || k != 0);
-      if (lo)
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          umma_bf16_ts(tmem + kPfTmemO + t * 128, tmem + t * 128 + 64 + 8 * k, dv + 128 * k, idesc_o, 1);
-    };
-    auto p_here = [&](int t) {
-      if (!wait(&ctl.p_full[t], (pphase >> t) & 1u)) return false;
-      pphase ^= 1u << t;
-      tcgen05_fence_after();
+      if (++ks == kTrK) {
+        ks = 0;
+        kphase ^= 1u;
+      }
       return true;
     };
     for (int u = 0; lane == 0 && ok; ++u) {
@@ -321,56 +419,28 @@ __global__ void __launch_bounds__(kTrThreads, 1)
       const int tokens = ctl.work[us].tokens, n = ctl.work[us].hi - ctl.work[us].lo;
       mbar_arrive(&ctl.u_empty[us]);
       if (tokens == 0) break;
-      if (!wait(&ctl.q_full, u & 1) || !k_here()) { ok = false; break; }
-      if (tokens <= p.tpt) {
-        // one tile: block i is warpgroup i % 2's
-        issue_s(0, 0, 1);
-        k_done();
-        if (n > 1) {
-          if (!k_here()) { ok = false; break; }
-          issue_s(1, 0, 1);
-          k_done();
+      // block i is warpgroup i % 2's
+      if (!wait(&ctl.q_full, u & 1) || !issue_s(0) || (n > 1 && !issue_s(1))) { ok = false; break; }
+      if (n <= 2) umma_commit(&ctl.q_empty);
+      for (int i = 0; i < n; ++i) {
+        const int t = i & 1;
+        if (!wait(&ctl.v_full[vs], vphase) || !wait(&ctl.p_full[t], (pphase >> t) & 1u)) { ok = false; break; }
+        pphase ^= 1u << t;
+        tcgen05_fence_after();
+        const uint64_t dv = umma_desc_sw128_mn(smem_u32(sh.v[vs]), kPfBlockHalf);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)  // 16 positions: 2048 bytes of V, 8 columns of P
+          umma_bf16_ts(tmem + kPfTmemO + t * 128, tmem + t * 128 + 8 * k, dv + 128 * k, idesc_o, i > 1 || k != 0);
+        umma_commit(&ctl.v_empty[vs]);
+        if (++vs == kTrV) {
+          vs = 0;
+          vphase ^= 1u;
         }
-        if (n <= 2) umma_commit(&ctl.q_empty);
-        for (int i = 0; i < n; ++i) {
-          const int t = i & 1;
-          if (!v_here() || !p_here(t)) { ok = false; break; }
-          issue_o(t, i > 1, true);
-          umma_commit(&ctl.kv_empty[v_stage()]);
-          ++vs;
-          if (i + 2 < n) {  // over P, which the product before it has read
-            if (!k_here()) { ok = false; break; }
-            issue_s(t, 0, 1);
-            k_done();
-            if (i + 3 == n) umma_commit(&ctl.q_empty);
-          } else {
-            umma_commit(&ctl.o_full[t]);
-          }
-        }
-        continue;
-      }
-      for (int t = 0; t < 2; ++t) issue_s(t, t, t);
-      k_done();
-      if (n == 1) umma_commit(&ctl.q_empty);
-      for (int i = 0; ok && i < n; ++i) {
-        if (!v_here()) { ok = false; break; }
-        const bool more = i + 1 < n;
-        for (int t = 0; t < 2; ++t) {
-          if (!p_here(t)) { ok = false; break; }
-          issue_o(t, i > 0, false);
-          if (more) {
-            if (t == 0 && !k_here()) { ok = false; break; }
-            issue_s(t, t, t);
-          } else {
-            umma_commit(&ctl.o_full[t]);
-          }
-        }
-        if (!ok) break;
-        umma_commit(&ctl.kv_empty[v_stage()]);
-        ++vs;
-        if (more) {
-          k_done();
-          if (i + 2 == n) umma_commit(&ctl.q_empty);
+        if (i + 2 < n) {  // over P, which the product before it has read
+          if (!issue_s(t)) { ok = false; break; }
+          if (i + 3 == n) umma_commit(&ctl.q_empty);
+        } else {
+          umma_commit(&ctl.o_full[t]);
         }
       }
     }
@@ -381,8 +451,10 @@ __global__ void __launch_bounds__(kTrThreads, 1)
       }
     }
     __syncwarp();
+    pdl_wait();
   } else if (warp == 3) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    pdl_wait();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---------------------------------------------------------------- softmax, one row per thread
@@ -396,6 +468,7 @@ __global__ void __launch_bounds__(kTrThreads, 1)
       const bool got = mbar_wait(bar, ph, &ctl.abort_flag, p.status);
       return __all_sync(0xffffffffu, got);
     };
+    pdl_wait();
     for (int u = 0;; ++u) {
       const int us = u & 1;
       if (!wait(&ctl.u_full[us], (u >> 1) & 1)) break;
@@ -403,17 +476,15 @@ __global__ void __launch_bounds__(kTrThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl.u_empty[us]);
       if (w.tokens == 0) break;
-      const bool single = w.tokens <= p.tpt;  // one tile, whose blocks the warpgroups share
-      const int node = (single ? 0 : g * p.tpt) + token;
-      const bool mine = token < p.tpt && node < w.tokens;
+      const bool mine = token < w.tokens;
       TrRow info{0, w.past, 0};
-      if (mine) info = p.rows[w.row0 + node];
+      if (mine) info = p.rows[w.row0 + token];
       const Blocks bl = blocks_of(w.past, w.kv - 1, p.window, p.sinks);
       float m = -INFINITY, l = 0.f;
       bool ok = true;
-      const int first = w.lo + (single ? g : 0), step = single ? 2 : 1;
+      const int first = w.lo + g;
 #pragma unroll 1
-      for (int i = first; i < w.hi; i += step) {
+      for (int i = first; i < w.hi; i += 2) {
         const int k0 = bl.at(i) * kPfBlock;
         if (!wait(&ctl.s_full[g], sphase)) { ok = false; break; }
         sphase ^= 1u;
@@ -466,24 +537,18 @@ __global__ void __launch_bounds__(kTrThreads, 1)
         const float ms = m == -INFINITY ? 0.f : m;
         const uint64_t sc2 = pair2(p.scale_log2, p.scale_log2), ms2 = pair2(-ms, -ms);
         uint64_t sum[4] = {0, 0, 0, 0};
-        auto weigh = [&](int c) {  // 16 columns at a time: registers
+        auto weigh = [&](int c) {
+          uint32_t pk[16];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t pk[8], lo[8];
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              const uint64_t y = fma2(pair2(__uint_as_float(s[c][16 * h + 2 * x]), __uint_as_float(s[c][16 * h + 2 * x + 1])), sc2, ms2);
-              float2 e = split2(y);
-              e.x = ex2(e.x);
-              e.y = ex2(e.y);
-              const uint64_t w2 = pair2(e.x, e.y);
-              sum[x & 3] = add2(sum[x & 3], w2);
-              pk[x] = pack_bf16x2(e.x, e.y);
-              if (single) lo[x] = bf16x2_of_pair(fma2(pair_of_bf16x2(pk[x]), pair2(-1.f, -1.f), w2));
-            }
-            tmem_st_32x32b_x8(ts + c * 16 + h * 8, pk);
-            if (single) tmem_st_32x32b_x8(ts + 64 + c * 16 + h * 8, lo);
+          for (int x = 0; x < 16; ++x) {
+            const uint64_t y = fma2(pair2(__uint_as_float(s[c][2 * x]), __uint_as_float(s[c][2 * x + 1])), sc2, ms2);
+            float2 e = split2(y);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            sum[x & 3] = add2(sum[x & 3], pair2(e.x, e.y));
+            pk[x] = pack_bf16x2(e.x, e.y);
           }
+          tmem_st_32x32b_x16(ts + c * 16, pk);
         };
         weigh(0);
         weigh(1);
@@ -491,10 +556,6 @@ __global__ void __launch_bounds__(kTrThreads, 1)
           const uint32_t none[16] = {};
           tmem_st_32x32b_x16(ts + 32, none);
           tmem_st_32x32b_x16(ts + 48, none);
-          if (single) {
-            tmem_st_32x32b_x16(ts + 96, none);
-            tmem_st_32x32b_x16(ts + 112, none);
-          }
         } else {
           weigh(2);
           weigh(3);
@@ -511,18 +572,8 @@ __global__ void __launch_bounds__(kTrThreads, 1)
         if (!wait(&ctl.o_full[g], ophase)) break;
         ophase ^= 1u;
       }
-      // where this lane stores: row 8 k + lane / 4, columns 8 (lane % 4) of each 32
-      const long long out_at =
-          mine ? ((static_cast<long long>(w.row0) + node) * p.nq + w.j * p.grp + head) * kHeadDim : -1;
-      __nv_bfloat16* to_row[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const long long at = __shfl_sync(0xffffffffu, out_at, k * 8 + (lane >> 2));
-        to_row[k] = at >= 0 ? p.out + at + (lane & 3) * 8 : nullptr;
-      }
-      float* part = w.slot >= 0 ? p.part + (static_cast<long long>(w.slot) * 2 + (single ? 0 : g)) * kTrPartTile : nullptr;
       float own = 1.f, other = 0.f;  // what this warpgroup's O and the other's are multiplied by
-      const bool joined = single && w.hi - w.lo > 1;
+      const bool joined = w.hi - w.lo > 1;
       if (joined) {
         ctl.ml[g][row] = make_float2(m, l);
         __syncwarp();
@@ -536,12 +587,17 @@ __global__ void __launch_bounds__(kTrThreads, 1)
         m = mn;
       }
       tcgen05_fence_after();
-      const float inv = part ? 1.f : l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-      own *= inv;
-      other *= inv;
-      // columns [64 g, 64 g + 64) of a joined tile, all of a tile of its own; nothing for the second warpgroup of one block
-      const int c_lo = joined ? 2 * g : 0, c_hi = joined ? 2 * g + 2 : single && g ? 0 : 4;
-      const uint32_t to_other = joined ? tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (1 - g) * 128 + kPfTmemO : to;
+      float* const part = w.slot >= 0 ? p.part + static_cast<long long>(w.slot) * kTrPart : nullptr;
+      if (!part) {
+        const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+        own *= inv;
+        other *= inv;
+      }
+      // columns [64 g, 64 g + 64) of both O, or all of the one
+      const int c_lo = joined ? 2 * g : 0, c_hi = joined ? 2 * g + 2 : g ? 0 : 4;
+      const uint32_t to_other = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (1 - g) * 128 + kPfTmemO;
+      __nv_bfloat16* const dst =
+          p.out + ((static_cast<long long>(w.row0) + token) * p.nq + w.j * p.grp + head) * kHeadDim;
       __syncwarp();
 #pragma unroll 1
       for (int c = c_lo; c < c_hi; ++c) {
@@ -554,35 +610,28 @@ __global__ void __launch_bounds__(kTrThreads, 1)
           const float a = __uint_as_float(o[x]) * own;
           o[x] = __float_as_uint(joined ? fmaf(__uint_as_float(q[x]), other, a) : a);
         }
-        if (part) {
+        if (mine && part) {
 #pragma unroll
           for (int x = 0; x < 32; x += 4)
             __stcg(reinterpret_cast<uint4*>(part) + (c * 8 + x / 4) * kPfRows + row, make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]));
-        } else {
-          // through shared memory: eight rows of 64 bytes per store instead of 32 rows of 16
+        } else if (mine) {
 #pragma unroll
           for (int x = 0; x < 32; x += 8) {
             float f[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[x + e]);
-            *reinterpret_cast<uint4*>(&stg[warp - 4][lane][x]) = pack8(f);
+            *reinterpret_cast<uint4*>(dst + c * 32 + x) = pack8(f);
           }
-          __syncwarp();
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint4 v = *reinterpret_cast<const uint4*>(&stg[warp - 4][k * 8 + (lane >> 2)][(lane & 3) * 8]);
-            if (to_row[k]) *reinterpret_cast<uint4*>(to_row[k] + c * 32) = v;
-          }
-          __syncwarp();
         }
+        __syncwarp();  // before the next load from tensor memory
       }
-      if (part && c_lo == 0 && c_hi > 0) {
+      if (part && mine && c_lo == 0 && c_hi > 0) {
         __stcg(part + kHeadDim * kPfRows + row, m);
         __stcg(part + (kHeadDim + 1) * kPfRows + row, l);
       }
-      tcgen05_fence_before();  // the next unit's MMAs follow this thread's next arrival
-      if (joined) {  // the next unit's MMAs and maxima wait until both warpgroups have read both
-        __syncwarp();
+      __syncwarp();
+      tcgen05_fence_before();  // the next item's MMAs follow this thread's next arrival
+      if (joined) {  // they, and the next maxima, wait until both warpgroups have read both
         if (lane == 0) mbar_arrive(&ctl.ml_empty);
         if (!wait(&ctl.ml_empty, jphase)) break;
         jphase ^= 1u;
@@ -597,79 +646,74 @@ __global__ void __launch_bounds__(kTrThreads, 1)
   }
 }
 
-// Joins the parts of a cut unit, in order: a CTA per (unit and kv head, 32
-// rows), a lane per row, a warp per 16 columns.
-__global__ void __launch_bounds__(256) paged_tree_join_kernel(const __grid_constant__ TrParams p) {
+// Joins the parts of a cut item, in order: a CTA per (item, 8 rows), a thread per
+// row and four columns, eight parts in flight.
+__global__ void __launch_bounds__(32 * kTrJoinRows) paged_tree_join_kernel(const __grid_constant__ TrParams p) {
+  constexpr int kSlices = kPfRows / kTrJoinRows, kAhead = 8;
+  const int cta = blockIdx.x / kSlices;
+  const int row = (blockIdx.x % kSlices) * kTrJoinRows + threadIdx.x % kTrJoinRows, col4 = threadIdx.x / kTrJoinRows;
   pdl_launch_dependents();
   pdl_wait();
-  const int cta = blockIdx.x >> 3, tile = (blockIdx.x >> 2) & 1;
-  const int lane = threadIdx.x & 31, col = (threadIdx.x >> 5) * 16, row = (blockIdx.x & 3) * 32 + lane;
   const TrSplit sp = p.splits[cta];
-  if (sp.parts == 0) return;
-  const TrUnit un = p.units[sp.unit];
   const int token = row / p.grp, head = row - token * p.grp;
-  if (token >= p.tpt || tile * p.tpt + token >= un.tokens) return;
-  auto part_of = [&](int s) {
-    const int slot = 2 * (cta + s) + (s == 0);
-    return p.part + (static_cast<long long>(slot) * 2 + tile) * kTrPartTile;
-  };
-  float m = -INFINITY;
-  for (int s = 0; s < sp.parts; ++s) m = fmaxf(m, __ldcg(part_of(s) + kHeadDim * kPfRows + row));
-  float l = 0.f, o[16];
+  if (sp.parts == 0 || token >= sp.tokens) return;
+  auto part_of = [&](int s) { return p.part + static_cast<long long>(2 * (cta + s) + (s == 0)) * kTrPart; };
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < sp.parts; s0 += kAhead) {
+    float4 v[kAhead];
+    float pm[kAhead], pl[kAhead];
 #pragma unroll
-  for (int x = 0; x < 16; ++x) o[x] = 0.f;
-  for (int s = 0; s < sp.parts; ++s) {
-    const float* from = part_of(s);
-    float4 v[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) v[x] = __ldcg(reinterpret_cast<const float4*>(from) + (col / 4 + x) * kPfRows + row);
-    const float f = m == -INFINITY ? 0.f : exp2f(__ldcg(from + kHeadDim * kPfRows + row) - m);
-    l = fmaf(f, __ldcg(from + (kHeadDim + 1) * kPfRows + row), l);
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      o[4 * x] = fmaf(f, v[x].x, o[4 * x]);
-      o[4 * x + 1] = fmaf(f, v[x].y, o[4 * x + 1]);
-      o[4 * x + 2] = fmaf(f, v[x].z, o[4 * x + 2]);
-      o[4 * x + 3] = fmaf(f, v[x].w, o[4 * x + 3]);
+    for (int e = 0; e < kAhead; ++e) {
+      const bool here = s0 + e < sp.parts;
+      const float* from = part_of(here ? s0 + e : s0);
+      v[e] = __ldcg(reinterpret_cast<const float4*>(from) + col4 * kPfRows + row);
+      pm[e] = here ? __ldcg(from + kHeadDim * kPfRows + row) : -INFINITY;
+      pl[e] = __ldcg(from + (kHeadDim + 1) * kPfRows + row);
     }
+    float mn = m;
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) mn = fmaxf(mn, pm[e]);
+    const float f0 = m == -INFINITY ? 0.f : exp2f(m - mn);
+    l *= f0;
+    o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      const float f = pm[e] == -INFINITY ? 0.f : exp2f(pm[e] - mn);
+      if (f == 0.f) continue;  // a part that sees nothing, or far less than the others
+      l = fmaf(f, pl[e], l);
+      o.x = fmaf(f, v[e].x, o.x);
+      o.y = fmaf(f, v[e].y, o.y);
+      o.z = fmaf(f, v[e].z, o.z);
+      o.w = fmaf(f, v[e].w, o.w);
+    }
+    m = mn;
   }
   const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
   __nv_bfloat16* dst =
-      p.out + ((static_cast<long long>(un.row0) + tile * p.tpt + token) * p.nq + sp.j * p.grp + head) * kHeadDim + col;
-#pragma unroll
-  for (int x = 0; x < 16; x += 8) {
-    float h[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = o[x + e] * inv;
-    *reinterpret_cast<uint4*>(dst + x) = pack8(h);
-  }
+      p.out + ((static_cast<long long>(sp.row0) + token) * p.nq + sp.j * p.grp + head) * kHeadDim + 4 * col4;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
 }
 
 // Sizes that the host can bound without the lengths.
 struct TrLayout {
-  long long units, grid;  // grid: of the main kernel
-  size_t rows, list, units_at, offs, splits, q, q_lo, part, total;
+  long long grid;  // of the main kernel
+  size_t rows, splits, q, q_lo, part, total;
 };
 
 TrLayout tr_layout(long long T, long long B, int nq, int nkv, long long max_pages, int page_size) {
   TrLayout L;
   const int tpt = kPfRows / (nq / nkv);
-  L.units = T / (2 * tpt) + (B < T ? B : T);
+  const long long tiles = T / tpt + (B < T ? B : T);
   const long long blocks = (max_pages * page_size + kPfBlock - 1) / kPfBlock;
   // places at most, and so runs at most
-  const long long most = (L.units * nkv * (blocks + 1 + kTrItem) + kTrMinBlocks + kTrItem - 1) / (kTrMinBlocks + kTrItem);
+  const long long most = (tiles * nkv * (blocks + 1 + kTrItem) + kTrMinRun - 1) / kTrMinRun;
   L.grid = device_sm_count();
   if (most < L.grid) L.grid = most;
   auto round = [](size_t n) { return (n + 255) & ~static_cast<size_t>(255); };
   size_t at = kPagedScratch;
-  L.list = at;
-  at += 256;
   L.rows = at;
   at += round(sizeof(TrRow) * T);
-  L.units_at = at;
-  at += round(sizeof(TrUnit) * L.units);
-  L.offs = at;
-  at += round(sizeof(int) * (L.units + 1));
   L.splits = at;
   at += round(sizeof(TrSplit) * L.grid);
   L.q = at;
@@ -677,7 +721,7 @@ TrLayout tr_layout(long long T, long long B, int nq, int nkv, long long max_page
   L.q_lo = at;
   at += round(sizeof(__nv_bfloat16) * T * nq * kHeadDim);
   L.part = at;
-  at += sizeof(float) * 2 * L.grid * 2 * kTrPartTile;
+  at += sizeof(float) * 2 * L.grid * kTrPart;
   L.total = at;
   return L;
 }
@@ -697,49 +741,45 @@ cudaError_t paged_tree_launch(const __nv_bfloat16* qkv, const void* qw, const vo
   const int nkv = cache.nkv, grp = nq / nkv, tpt = kPfRows / grp;
   const TrLayout L = tr_layout(T, B, nq, nkv, cache.max_pages, 1 << cache.page_shift);
   char* ws = static_cast<char*>(workspace);
-  int* status = reinterpret_cast<int*>(ws);
-  __nv_bfloat16* q = reinterpret_cast<__nv_bfloat16*>(ws + L.q);
-  __nv_bfloat16* q_lo = reinterpret_cast<__nv_bfloat16*>(ws + L.q_lo);
-  CUtensorMap mq, mk, mv, ml;
-  if (!tmap_of_rows(encode, &mq, q, nq, T, static_cast<long long>(nq) * kHeadDim, grp, tpt) ||
-      !tmap_of_rows(encode, &ml, q_lo, nq, T, static_cast<long long>(nq) * kHeadDim, grp, tpt) ||
-      !tmap_of_pages(encode, &mk, cache, false) || !tmap_of_pages(encode, &mv, cache, true))
-    return cudaErrorInvalidValue;
-  TrPlan plan;
-  plan.q_lo = q_lo;
-  plan.rows = reinterpret_cast<TrRow*>(ws + L.rows);
-  plan.list = reinterpret_cast<TrList*>(ws + L.list);
-  plan.units = reinterpret_cast<TrUnit*>(ws + L.units_at);
-  plan.offs = reinterpret_cast<int*>(ws + L.offs);
-  plan.window = window;
-  plan.sinks = sinks;
-  plan.tpt = tpt;
-  plan.sms = static_cast<int>(L.grid);
-  plan.max_units = static_cast<int>(L.units);
-  cudaError_t e = paged_tree_store_launch(qkv, qw, kw, w_dtype, parents, cu_seqlens, kv_lens, cache, q, T, B, nq, theta,
-                                          eps, plan, status, s);
-  if (e != cudaSuccess) return e;
   TrParams p;
+  p.cu = cu_seqlens;
+  p.kv_lens = kv_lens;
   p.out = out;
-  p.status = status;
-  p.rows = plan.rows;
-  p.list = plan.list;
-  p.units = plan.units;
-  p.offs = plan.offs;
+  p.status = reinterpret_cast<int*>(ws);
+  p.rows = reinterpret_cast<TrRow*>(ws + L.rows);
   p.splits = reinterpret_cast<TrSplit*>(ws + L.splits);
   p.part = reinterpret_cast<float*>(ws + L.part);
   p.c = cache;
+  p.T = static_cast<int>(T);
+  p.B = B;
   p.nq = nq;
   p.grp = grp;
   p.tpt = tpt;
   p.window = window;
   p.sinks = sinks;
   p.scale_log2 = scale * kPfLog2e;
-  e = allow_smem<paged_tree_kernel>(static_cast<int>(kTrSmem));
+  TreeOut tree;
+  tree.parents = parents;
+  tree.rows = reinterpret_cast<TrRow*>(ws + L.rows);
+  tree.q_lo = reinterpret_cast<__nv_bfloat16*>(ws + L.q_lo);
+  tree.window = window;
+  tree.sinks = sinks;
+  __nv_bfloat16* q = reinterpret_cast<__nv_bfloat16*>(ws + L.q);
+  const long long q_row = static_cast<long long>(nq) * kHeadDim;
+  CUtensorMap mq, ml, mk, mv;
+  if (!tmap_of_rows(encode, &mq, q, nq, T, q_row, grp, tpt) || !tmap_of_rows(encode, &ml, tree.q_lo, nq, T, q_row, grp, tpt) ||
+      !tmap_of_pages(encode, &mk, cache, false) || !tmap_of_pages(encode, &mv, cache, true))
+    return cudaErrorInvalidValue;
+  cudaError_t e = paged_tree_store_launch(qkv, qw, kw, w_dtype, cu_seqlens, kv_lens, cache, q, T, B, nq, theta, eps,
+                                          tree, p.status, s);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(paged_tree_kernel, dim3(static_cast<unsigned>(L.grid)), dim3(kTrThreads), kTrSmem, s, mq, mk, mv, ml, p);
+  e = allow_smem<paged_tree_kernel>(static_cast<int>(sizeof(TrShared)));
   if (e != cudaSuccess) return e;
-  return launch_pdl(paged_tree_join_kernel, dim3(static_cast<unsigned>(8 * L.grid)), dim3(256), 0, s, p);
+  e = launch_pdl(paged_tree_kernel, dim3(static_cast<unsigned>(L.grid)), dim3(kTrThreads), sizeof(TrShared), s, mq, ml,
+                 mk, mv, p);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(paged_tree_join_kernel, dim3(static_cast<unsigned>(L.grid * (kPfRows / kTrJoinRows))),
+                    dim3(32 * kTrJoinRows), 0, s, p);
 }
 
 }  // namespace nkimoe

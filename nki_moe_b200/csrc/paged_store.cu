@@ -250,8 +250,14 @@ cudaError_t paged_tree_store_launch(const __nv_bfloat16* qkv, const void* qw, co
   static_cast<StoreParams&>(p) =
       store_params(qkv, qw, kw, w_dtype, cu_seqlens, kv_lens, cache, q_out, T, B, nq, theta, eps, status);
   p.tree = tree;
-  if (T <= kStoreFew)
+  // steps are hundreds of rows: eight warps on each as long as all CTAs run at
+  // once, then four (the whole step, 16 trees of 49 to 64 nodes = 913 rows: with
+  // four 115 us, two 122, eight 120, one 127; 8 trees of 8: 20, 23, 19 us)
+  if (T <= kStoreFew / 2)
     return launch_pdl(paged_store_kernel<8, TreeStoreParams>, dim3(static_cast<unsigned>(T)), dim3(kStoreThreads), 0, s, p);
+  if (T <= 4 * kStoreFew)
+    return launch_pdl(paged_store_kernel<4, TreeStoreParams>, dim3(static_cast<unsigned>((T + 1) / 2)), dim3(kStoreThreads), 0,
+                      s, p);
   return launch_pdl(paged_store_kernel<1, TreeStoreParams>, dim3(static_cast<unsigned>((T + 7) / 8)), dim3(kStoreThreads), 0,
                     s, p);
 }

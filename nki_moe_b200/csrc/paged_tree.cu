@@ -14,7 +14,7 @@
 //
 // Tile: 128 MMA rows are floor(128 / group) nodes times the `group` query heads
 // of one kv head, against key blocks of 128 places.  One warp loads Q and K, one
-// V, one thread issues the MMAs, and two warpgroups take S from tensor memory,
+// V, one thread each issues the MMAs of scores and of products, and two warpgroups take S from tensor memory,
 // a thread per row, and leave P there.  The warpgroups take a tile's blocks in
 // turn, each with its own maximum, sum and O, which are joined at its end: a
 // block's chain (scores, softmax, product, 4000 cycles) takes longer than its
@@ -42,7 +42,7 @@ namespace {
 
 constexpr int kTrThreads = 384;
 constexpr int kTrK = 3, kTrV = 2;  // stages of 32 KB: K blocks, V blocks
-constexpr int kTrItem = 1;         // key blocks that beginning and ending an item (sequence, kv head, tile) costs
+constexpr int kTrItem = 2;         // key blocks that beginning and ending an item (sequence, kv head, tile) costs
 constexpr int kTrMinRun = 3;       // places of a CTA's run at least: a block for each warpgroup
 // A part of a cut item: o four columns at a time [32][128 rows][4], then the
 // rows' m, then their l (a warp's rows are neighbours: coalesced)
@@ -84,10 +84,10 @@ struct TrCtl {
   uint64_t q_full, q_empty;
   uint64_t k_full[kTrK], k_empty[kTrK];
   uint64_t v_full[kTrV], v_empty[kTrV];
-  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t s_full[2], p_full[2], pv_done[2], o_full[2];
   uint64_t u_full[2], u_empty[2];
   uint64_t ml_full, ml_empty;  // the softmax warps have left their maxima and sums; have read them and both O
-  uint64_t tail, drain;
+  uint64_t tail, drain[2];
   TrWork work[2];
   uint32_t tmem_base;
   int abort_flag;
@@ -235,14 +235,16 @@ __global__ void __launch_bounds__(kTrThreads, 1)
     for (int t = 0; t < 2; ++t) {
       mbar_init(&ctl.s_full[t], 1);
       mbar_init(&ctl.p_full[t], 4);  // one arrival per softmax warp
+      mbar_init(&ctl.pv_done[t], 1);
       mbar_init(&ctl.o_full[t], 1);
       mbar_init(&ctl.u_full[t], 1);
-      mbar_init(&ctl.u_empty[t], 2 + 8);  // the MMA warp, the warp that loads V, the softmax warps
+      mbar_init(&ctl.u_empty[t], 3 + 8);  // the MMA warps, the warp that loads V, the softmax warps
     }
     mbar_init(&ctl.ml_full, 8);
     mbar_init(&ctl.ml_empty, 8);
     mbar_init(&ctl.tail, 1);
-    mbar_init(&ctl.drain, 1);
+    mbar_init(&ctl.drain[0], 1);
+    mbar_init(&ctl.drain[1], 1);
     ctl.abort_flag = 0;
     fence_barrier_init();
     prefetch_tmap(&tmap_q);
@@ -385,43 +387,66 @@ __global__ void __launch_bounds__(kTrThreads, 1)
     __syncwarp();
   } else if (warp == 1) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    // ---------------------------------------------------------------- MMA issue (one thread)
+    // ---------------------------------------------------------------- scores (one thread)
     constexpr uint32_t idesc_s = umma_idesc_bf16_f32(kPfRows, kPfBlock);
-    constexpr uint32_t idesc_o = umma_idesc_bf16_f32(kPfRows, kHeadDim) | (1u << 16);  // B is MN-major
-    int ks = 0, vs = 0;
-    uint32_t kphase = 0, vphase = 0, pphase = 0;  // pphase: bit t, of p_full
+    int ks = 0;
+    uint32_t kphase = 0, dphase = 3;  // dphase: bit t, of pv_done (nothing to wait for at first)
     bool ok = true, any = false;
     auto wait = [&](uint64_t* bar, uint32_t ph) { return mbar_wait(bar, ph, &ctl.abort_flag, p.status); };
-    // S of warpgroup t against the next K block
-    auto issue_s = [&](int t) {
-      if (!wait(&ctl.k_full[ks], kphase)) return false;
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint64_t da = umma_desc_sw128(smem_u32(sh.q[q] + h * kPfTileHalf));
-          const uint64_t db = umma_desc_sw128(smem_u32(sh.k[ks] + h * kPfBlockHalf));
-#pragma unroll
-          for (int k = 0; k < 4; ++k) umma_bf16(tmem + t * 128, da + 2 * k, db + 2 * k, idesc_s, (q | h | k) != 0);
-        }
-      umma_commit(&ctl.s_full[t]);
-      umma_commit(&ctl.k_empty[ks]);
-      any = true;
-      if (++ks == kTrK) {
-        ks = 0;
-        kphase ^= 1u;
-      }
-      return true;
-    };
     for (int u = 0; lane == 0 && ok; ++u) {
       const int us = u & 1;
       if (!wait(&ctl.u_full[us], (u >> 1) & 1)) { ok = false; break; }
       const int tokens = ctl.work[us].tokens, n = ctl.work[us].hi - ctl.work[us].lo;
       mbar_arrive(&ctl.u_empty[us]);
       if (tokens == 0) break;
-      // block i is warpgroup i % 2's
-      if (!wait(&ctl.q_full, u & 1) || !issue_s(0) || (n > 1 && !issue_s(1))) { ok = false; break; }
-      if (n <= 2) umma_commit(&ctl.q_empty);
+      if (!wait(&ctl.q_full, u & 1)) { ok = false; break; }
+      for (int i = 0; i < n; ++i) {  // block i is warpgroup i % 2's
+        const int t = i & 1;
+        // over P, which the product of the warpgroup's block before has read
+        if (!wait(&ctl.pv_done[t], (dphase >> t) & 1u) || !wait(&ctl.k_full[ks], kphase)) { ok = false; break; }
+        dphase ^= 1u << t;
+        tcgen05_fence_after();
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint64_t da = umma_desc_sw128(smem_u32(sh.q[q] + h * kPfTileHalf));
+            const uint64_t db = umma_desc_sw128(smem_u32(sh.k[ks] + h * kPfBlockHalf));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) umma_bf16(tmem + t * 128, da + 2 * k, db + 2 * k, idesc_s, (q | h | k) != 0);
+          }
+        any = true;
+        umma_commit(&ctl.s_full[t]);
+        umma_commit(&ctl.k_empty[ks]);
+        if (++ks == kTrK) {
+          ks = 0;
+          kphase ^= 1u;
+        }
+      }
+      if (ok) umma_commit(&ctl.q_empty);
+    }
+    if (!ok && any) {  // issued MMAs end before tensor memory is released
+      umma_commit(&ctl.drain[0]);
+      const long long t0 = clock64();
+      while (!mbar_try_wait(&ctl.drain[0], 0) && clock64() - t0 < kWaitBudgetCycles / 8) {
+      }
+    }
+    __syncwarp();
+    pdl_wait();
+  } else if (warp == 3) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    // ---------------------------------------------------------------- products (one thread)
+    constexpr uint32_t idesc_o = umma_idesc_bf16_f32(kPfRows, kHeadDim) | (1u << 16);  // B is MN-major
+    int vs = 0;
+    uint32_t vphase = 0, pphase = 0;  // pphase: bit t, of p_full
+    bool ok = true, any = false;
+    auto wait = [&](uint64_t* bar, uint32_t ph) { return mbar_wait(bar, ph, &ctl.abort_flag, p.status); };
+    for (int u = 0; lane == 0 && ok; ++u) {
+      const int us = u & 1;
+      if (!wait(&ctl.u_full[us], (u >> 1) & 1)) { ok = false; break; }
+      const int tokens = ctl.work[us].tokens, n = ctl.work[us].hi - ctl.work[us].lo;
+      mbar_arrive(&ctl.u_empty[us]);
+      if (tokens == 0) break;
       for (int i = 0; i < n; ++i) {
         const int t = i & 1;
         if (!wait(&ctl.v_full[vs], vphase) || !wait(&ctl.p_full[t], (pphase >> t) & 1u)) { ok = false; break; }
@@ -431,29 +456,23 @@ __global__ void __launch_bounds__(kTrThreads, 1)
 #pragma unroll
         for (int k = 0; k < 8; ++k)  // 16 positions: 2048 bytes of V, 8 columns of P
           umma_bf16_ts(tmem + kPfTmemO + t * 128, tmem + t * 128 + 8 * k, dv + 128 * k, idesc_o, i > 1 || k != 0);
+        any = true;
+        umma_commit(&ctl.pv_done[t]);
         umma_commit(&ctl.v_empty[vs]);
+        if (i + 2 >= n) umma_commit(&ctl.o_full[t]);
         if (++vs == kTrV) {
           vs = 0;
           vphase ^= 1u;
         }
-        if (i + 2 < n) {  // over P, which the product before it has read
-          if (!issue_s(t)) { ok = false; break; }
-          if (i + 3 == n) umma_commit(&ctl.q_empty);
-        } else {
-          umma_commit(&ctl.o_full[t]);
-        }
       }
     }
-    if (!ok && any) {  // issued MMAs end before tensor memory is released
-      umma_commit(&ctl.drain);
+    if (!ok && any) {
+      umma_commit(&ctl.drain[1]);
       const long long t0 = clock64();
-      while (!mbar_try_wait(&ctl.drain, 0) && clock64() - t0 < kWaitBudgetCycles / 8) {
+      while (!mbar_try_wait(&ctl.drain[1], 0) && clock64() - t0 < kWaitBudgetCycles / 8) {
       }
     }
     __syncwarp();
-    pdl_wait();
-  } else if (warp == 3) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     pdl_wait();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -647,51 +666,93 @@ __global__ void __launch_bounds__(kTrThreads, 1)
 }
 
 // Joins the parts of a cut item, in order: a CTA per (item, 8 rows), a thread per
-// row and four columns, eight parts in flight.
+// row and four columns, eight parts in flight once their factors are known.
+// (One sequence over all SMs, 37 parts each: 8.4 us with a running maximum over
+// the parts; with a few CTAs that take slices in turn the ragged batch takes 6 us
+// more.)
 __global__ void __launch_bounds__(32 * kTrJoinRows) paged_tree_join_kernel(const __grid_constant__ TrParams p) {
-  constexpr int kSlices = kPfRows / kTrJoinRows, kAhead = 8;
-  const int cta = blockIdx.x / kSlices;
-  const int row = (blockIdx.x % kSlices) * kTrJoinRows + threadIdx.x % kTrJoinRows, col4 = threadIdx.x / kTrJoinRows;
+  constexpr int kSlices = kPfRows / kTrJoinRows, kAhead = 8, kFew = 4;
+  extern __shared__ float2 factor[];  // [parts][rows]: maximum and sum, then the weight and the sum's share
+  __shared__ float whole[kTrJoinRows];
+  const int cta = blockIdx.x / kSlices, row0 = (blockIdx.x % kSlices) * kTrJoinRows;
+  const int r = threadIdx.x % kTrJoinRows, col4 = threadIdx.x / kTrJoinRows, row = row0 + r;
   pdl_launch_dependents();
   pdl_wait();
   const TrSplit sp = p.splits[cta];
-  const int token = row / p.grp, head = row - token * p.grp;
-  if (sp.parts == 0 || token >= sp.tokens) return;
+  if (sp.parts == 0 || row0 >= sp.tokens * p.grp) return;
   auto part_of = [&](int s) { return p.part + static_cast<long long>(2 * (cta + s) + (s == 0)) * kTrPart; };
-  float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = 0; s0 < sp.parts; s0 += kAhead) {
-    float4 v[kAhead];
-    float pm[kAhead], pl[kAhead];
+  const int token = row / p.grp, head = row - token * p.grp;
+  __nv_bfloat16* const dst =
+      p.out + ((static_cast<long long>(sp.row0) + token) * p.nq + sp.j * p.grp + head) * kHeadDim + 4 * col4;
+  if (sp.parts <= kFew) {  // all at once
+    if (token >= sp.tokens) return;
+    float4 v[kFew];
+    float2 ml[kFew];
 #pragma unroll
-    for (int e = 0; e < kAhead; ++e) {
-      const bool here = s0 + e < sp.parts;
-      const float* from = part_of(here ? s0 + e : s0);
+    for (int e = 0; e < kFew; ++e) {
+      if (e >= sp.parts) break;
+      const float* from = part_of(e);
       v[e] = __ldcg(reinterpret_cast<const float4*>(from) + col4 * kPfRows + row);
-      pm[e] = here ? __ldcg(from + kHeadDim * kPfRows + row) : -INFINITY;
-      pl[e] = __ldcg(from + (kHeadDim + 1) * kPfRows + row);
+      ml[e] = make_float2(__ldcg(from + kHeadDim * kPfRows + row), __ldcg(from + (kHeadDim + 1) * kPfRows + row));
     }
-    float mn = m;
+    float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int e = 0; e < kAhead; ++e) mn = fmaxf(mn, pm[e]);
-    const float f0 = m == -INFINITY ? 0.f : exp2f(m - mn);
-    l *= f0;
-    o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+    for (int e = 0; e < kFew; ++e)
+      if (e < sp.parts) m = fmaxf(m, ml[e].x);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int e = 0; e < kAhead; ++e) {
-      const float f = pm[e] == -INFINITY ? 0.f : exp2f(pm[e] - mn);
-      if (f == 0.f) continue;  // a part that sees nothing, or far less than the others
-      l = fmaf(f, pl[e], l);
+    for (int e = 0; e < kFew; ++e) {
+      if (e >= sp.parts) break;
+      const float f = ml[e].x == -INFINITY ? 0.f : exp2f(ml[e].x - m);
+      l = fmaf(f, ml[e].y, l);
       o.x = fmaf(f, v[e].x, o.x);
       o.y = fmaf(f, v[e].y, o.y);
       o.z = fmaf(f, v[e].z, o.z);
       o.w = fmaf(f, v[e].w, o.w);
     }
-    m = mn;
+    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+    return;
   }
-  const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-  __nv_bfloat16* dst =
-      p.out + ((static_cast<long long>(sp.row0) + token) * p.nq + sp.j * p.grp + head) * kHeadDim + 4 * col4;
+  for (int s = col4; s < sp.parts; s += 32) {
+    const float* from = part_of(s) + kHeadDim * kPfRows + row;
+    factor[s * kTrJoinRows + r] = make_float2(__ldcg(from), __ldcg(from + kPfRows));
+  }
+  // the first parts, long before their factors are known
+  float4 v[kAhead];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e)
+      if (s0 + e < sp.parts) v[e] = __ldcg(reinterpret_cast<const float4*>(part_of(s0 + e)) + col4 * kPfRows + row);
+  };
+  load(0);
+  __syncthreads();
+  if (col4 == 0) {
+    float m = -INFINITY, l = 0.f;
+    for (int s = 0; s < sp.parts; ++s) m = fmaxf(m, factor[s * kTrJoinRows + r].x);
+    for (int s = 0; s < sp.parts; ++s) {
+      float2& f = factor[s * kTrJoinRows + r];
+      f.x = f.x == -INFINITY ? 0.f : exp2f(f.x - m);
+      l = fmaf(f.x, f.y, l);
+    }
+    whole[r] = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+  }
+  __syncthreads();
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < sp.parts; s0 += kAhead) {
+    if (s0 > 0) load(s0);
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      if (s0 + e >= sp.parts) break;
+      const float f = factor[(s0 + e) * kTrJoinRows + r].x;
+      o.x = fmaf(f, v[e].x, o.x);
+      o.y = fmaf(f, v[e].y, o.y);
+      o.z = fmaf(f, v[e].z, o.z);
+      o.w = fmaf(f, v[e].w, o.w);
+    }
+  }
+  if (token >= sp.tokens) return;
+  const float inv = whole[r];
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
 }
 
@@ -779,7 +840,7 @@ cudaError_t paged_tree_launch(const __nv_bfloat16* qkv, const void* qw, const vo
                  mk, mv, p);
   if (e != cudaSuccess) return e;
   return launch_pdl(paged_tree_join_kernel, dim3(static_cast<unsigned>(L.grid * (kPfRows / kTrJoinRows))),
-                    dim3(32 * kTrJoinRows), 0, s, p);
+                    dim3(32 * kTrJoinRows), sizeof(float2) * kTrJoinRows * L.grid, s, p);
 }
 
 }  // namespace nkimoe

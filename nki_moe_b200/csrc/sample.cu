@@ -14,12 +14,18 @@
 // would depend on timing (histograms) they are added as integers.
 //
 // A cluster of CTAs holds a row in shared memory, each a slice, so the logits
-// are read from HBM once and every later pass is local.  top_k and top_p are
-// found alike: a histogram over 1024 distances from the maximum (1/32 of a
-// binary order each) of counts or of weights, the bin where the sum passes the
-// border, then that bin's tokens sorted by the cluster's first CTA.  A bin of
-// more tokens than the sort takes is split further, by its own smallest and
-// largest (logit, id).
+// are read from HBM once and every later pass is local.  What top_k and top_p
+// keep is found from histograms:
+//
+//   bf16  of the values themselves.  Of each sign the 2048 values of the 16 binary
+//         orders below the largest magnitude that matters have a bin, so counts
+//         alone give every sum exactly (a weight per bin), and equal logits are
+//         cut by counting them in order.  What lies nearer to zero is summed by
+//         itself; a border among it is found as in fp32.
+//   fp32  over 1024 distances from the maximum (1/32 of a binary order each), of
+//         counts or of weights; the border's bin is sorted by the cluster's first
+//         CTA, or, with more tokens than that takes, split further by its own
+//         smallest and largest (logit, id).
 //
 // Reference: the sampling of the reference's runtime is not vendored; no
 // kernel of its own.
@@ -40,6 +46,7 @@ constexpr int kSmBinsPerOctave = 32;
 constexpr int kSmList = 2048;        // tokens that the last sort takes
 constexpr int kSmCluster = 8;        // CTAs per row at most
 constexpr int kSmSlice = 96 * 1024;  // bytes of a row per CTA that two CTAs per SM leave room for
+constexpr int kSmValues = 2048;      // values of a sign that have a bin
 constexpr int kSmMaxVocab = 1 << 18;
 static_assert(2 * kSmThreads == kSmBins, "two bins per thread");
 
@@ -62,9 +69,12 @@ struct SmParams {
 };
 
 struct SmShared {
-  float max_of[kSmCluster];
+  float max_of[kSmCluster], min_of[kSmCluster];
   double sum_of[kSmCluster];
   u64 lo_of[kSmCluster], hi_of[kSmCluster];
+  int count_of[kSmCluster];
+  double zone_of[kSmCluster];  // weight of the logits near zero, and how many they are
+  int zones_of[kSmCluster];
   // what the first CTA tells all
   int bin;        // -1: no border
   double above;   // counts or weights before the bin
@@ -73,17 +83,27 @@ struct SmShared {
   u64 border;     // the last kept (order, id)
   int listed;     // the first CTA's: tokens in its list
   int pick;
+  int state;      // of the border among values: one of kSm...
+  float edge;     // its value
+  int ties;       // how many tokens of this value are kept
+  int last_k, last_p;  // places of the borders in the list of values
+  int ties_k, ties_p;
+  double sum_k;
   double warp_d[kSmWarps];
   u64 warp_lo[kSmWarps], warp_hi[kSmWarps];
-  float warp_f[kSmWarps];
+  int warp_n[kSmWarps];
+  float warp_f[kSmWarps], warp_g[kSmWarps];
   union {
     struct {
       unsigned a[kSmBins];  // counts, or the upper halves of weights
       unsigned b[kSmBins];  // the lower halves
     } hist;
     u64 list[kSmList];
+    unsigned values[2 * kSmValues];  // counts by magnitude, then of negative values
+    double weights[kSmValues];       // by magnitude, of the maximum's sign
   };
 };
+enum SmState { kSmAll, kSmEdge, kSmTies, kSmSearch };
 
 // Integers that rise as the values fall; -0 equal to +0.
 __device__ __forceinline__ unsigned falling(float x) {
@@ -119,6 +139,23 @@ __device__ __forceinline__ double pow2(double t) {
 
 __device__ __forceinline__ float sm_float(float v) { return v; }
 __device__ __forceinline__ float sm_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Maxima that let a NaN through, and minima that pass one over.
+__device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t min_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 // One row's settings and what is known of it.
 struct SmRow {
@@ -161,12 +198,16 @@ struct SmSlice {
     for (int v = threadIdx.x; v < vecs; v += kSmThreads) {
       float x[VE];
       get(v, x);
+      float most = x[0];
+#pragma unroll
+      for (int i = 1; i < VE; ++i) most = fmaxf(most, x[i]);
+      if (most < least || most == -INFINITY) continue;
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
-        if (x[i] == -INFINITY || x[i] < least) continue;
         const int id = id0 + v * VE + i;
-        if (x[i] == least && ((static_cast<u64>(falling(x[i])) << 32) | static_cast<unsigned>(id)) > border) continue;
-        f(x[i], id);
+        if (x[i] > least || (x[i] == least && x[i] != -INFINITY &&
+                             ((static_cast<u64>(falling(x[i])) << 32) | static_cast<unsigned>(id)) <= border))
+          f(x[i], id);
       }
     }
   }
@@ -404,6 +445,257 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const SmSli
   }
 }
 
+// The window of magnitudes that have a bin: [lo, lo + kSmValues).
+struct SmWindow {
+  int lo;
+  __device__ __forceinline__ int place(unsigned b) const { return static_cast<int>(b & 0x7fffu) - lo; }
+  __device__ __forceinline__ float value(int mag, bool negative) const {
+    return __uint_as_float(static_cast<unsigned>(mag) << 16 | (negative ? 0x80000000u : 0u));
+  }
+};
+
+// The border of top_k and top_p among bf16 logits: row.border.  Values in
+// falling order are the positive ones by falling magnitude, what is nearer to
+// zero (the zone), the negative ones by rising magnitude.  Weights below 2^-64
+// count as 0.  All CTAs of the cluster call it and take the same way through it;
+// false: the border lies in the zone and has to be searched.
+__device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const SmSlice<__nv_bfloat16>& sl, SmRow& row,
+                          const SmWindow& win, double top_k, double top_p) {
+  constexpr int kEach = 2 * kSmValues / kSmThreads;  // bins per thread
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ranks = cl.num_blocks(), rank = cl.block_rank();
+  for (int i = tid; i < 2 * kSmValues / 4; i += kSmThreads) reinterpret_cast<uint4*>(sh.values)[i] = make_uint4(0u, 0u, 0u, 0u);
+  __syncthreads();
+  double zone = 0.0;
+  int zones = 0;
+  for (int v = tid; v < sl.vecs; v += kSmThreads) {
+    const uint4 u = sl.data[v];
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const unsigned b = h ? w[i] >> 16 : w[i] & 0xffffu;
+        const int at = win.place(b);
+        if (static_cast<unsigned>(at) < kSmValues) {
+          atomicAdd(&sh.values[at | (b >> 4 & 0x800u)], 1u);
+        } else if (at < 0) {
+          zone += pow2(row.exponent(__uint_as_float(b << 16)));
+          ++zones;
+        }  // else: -inf, or too far below the maximum to weigh anything
+      }
+  }
+  zones = __reduce_add_sync(0xffffffffu, zones);
+  if (zones > 0) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) zone += __shfl_xor_sync(0xffffffffu, zone, o);
+  }
+  if (lane == 0) {
+    sh.warp_d[warp] = zone;
+    sh.warp_n[warp] = zones;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    zone = 0.0;
+    zones = 0;
+    for (int w = 0; w < kSmWarps; ++w) {
+      zone += sh.warp_d[w];
+      zones += sh.warp_n[w];
+    }
+    SmShared& o = *cl.map_shared_rank(&sh, 0);
+    o.zone_of[rank] = zone;
+    o.zones_of[rank] = zones;
+  }
+  cl.sync();
+  if (rank == 0) {
+    // thread t: places 8 t .. 8 t + 7 of the list; the zone follows the last positive one
+    unsigned n[kEach + 1];
+    double w[kEach + 1];
+    const bool negative = tid >= kSmThreads / 2;
+    const int at0 = negative ? kEach * tid : kSmValues - kEach * (tid + 1);  // lowest address of its bins
+#pragma unroll
+    for (int e = 0; e <= kEach; ++e) {
+      n[e] = 0;
+      w[e] = 0.0;
+    }
+    for (int r = 0; r < ranks; ++r) {
+      const uint4* from = reinterpret_cast<const uint4*>(cl.map_shared_rank(&sh, r)->values + at0);
+#pragma unroll
+      for (int e = 0; e < kEach; e += 4) {
+        const uint4 c = from[e / 4];
+        n[e] += c.x;
+        n[e + 1] += c.y;
+        n[e + 2] += c.z;
+        n[e + 3] += c.w;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kEach / 2; ++e) {  // of positive values in falling order
+      const unsigned a = n[e], b = n[kEach - 1 - e];
+      n[e] = negative ? a : b;
+      n[kEach - 1 - e] = negative ? b : a;
+    }
+    const bool has_zone = tid == kSmThreads / 2 - 1;
+    if (win.lo == 0) {  // -0 is 0: the first negative bin joins the last positive one
+      __syncthreads();
+      if (tid == kSmThreads / 2) {
+        sh.pick = static_cast<int>(n[0]);
+        n[0] = 0;
+      }
+      __syncthreads();
+      if (has_zone) n[kEach - 1] += static_cast<unsigned>(sh.pick);
+    }
+    double mass = 0.0, zone_w = 0.0;
+    unsigned count = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int mag = win.lo + (negative ? at0 + e - kSmValues : at0 + kEach - 1 - e);
+      if (n[e] != 0) w[e] = pow2(row.exponent(win.value(mag, negative)));
+      mass += n[e] * w[e];
+      count += n[e];
+    }
+    if (has_zone) {
+      for (int r = 0; r < ranks; ++r) {
+        zone_w += sh.zone_of[r];
+        n[kEach] += static_cast<unsigned>(sh.zones_of[r]);
+      }
+      mass += zone_w;
+      count += n[kEach];
+    }
+    auto mass_of = [&](int e) { return e == kEach ? zone_w : n[e] * w[e]; };
+    double all, total;
+    const SmSums counts = sm_scan(static_cast<double>(count), sh.warp_d, all);
+    const SmSums sums = sm_scan(mass, sh.warp_d, total);
+    const int none = 0x7fffffff;
+    if (tid == 0) {
+      sh.last_k = sh.last_p = none;
+      sh.sum_k = total;
+    }
+    __syncthreads();
+    if (top_k > 0.0 && top_k < all && sm_passes(counts, top_k, &sh.pick)) {
+      double c = counts.before, m = sums.before;
+      bool found = false;
+#pragma unroll
+      for (int e = 0; e <= kEach; ++e) {
+        if (found) continue;
+        if (c + n[e] >= top_k) {
+          found = true;
+          sh.last_k = tid * (kEach + 1) + e;
+          sh.ties_k = static_cast<int>(top_k - c);
+          sh.sum_k = m + (top_k - c) * w[e];
+          continue;
+        }
+        c += n[e];
+        m += mass_of(e);
+      }
+    }
+    __syncthreads();
+    const bool zone_k = sh.last_k == (kSmThreads / 2 - 1) * (kEach + 1) + kEach;
+    if (top_p < 1.0 && !zone_k) {
+      const double need = fmin(fmax(top_p * sh.sum_k, 1e-300), total * (1.0 - 0x1p-50));
+      if (sm_passes(sums, need, &sh.pick)) {
+        double m = sums.before;
+        bool found = false;
+#pragma unroll
+        for (int e = 0; e <= kEach; ++e) {
+          if (found || n[e] == 0) continue;
+          found = m + mass_of(e) >= need;
+          // (by rounding it may be none: then it is the thread's last)
+          sh.last_p = tid * (kEach + 1) + e;
+          sh.ties_p = w[e] > 0.0 ? static_cast<int>(fmin(fmax(ceil((need - m) / w[e]), 1.0), static_cast<double>(n[e]))) : 1;
+          m += mass_of(e);
+        }
+      }
+    }
+    __syncthreads();
+    const int last = min(sh.last_k, sh.last_p);
+    const int zone_at = (kSmThreads / 2 - 1) * (kEach + 1) + kEach;
+    if (last == none || last == zone_at || last / (kEach + 1) == tid) {
+      if (last / (kEach + 1) == tid || (tid == 0 && (last == none || last == zone_at))) {
+        int state = last == none ? kSmAll : kSmSearch, ties = 0;
+        float edge = 0.f;
+        if (last != none && last != zone_at) {
+          const int e = last % (kEach + 1);
+          int mag = 0;
+          unsigned held = 0;
+#pragma unroll
+          for (int i = 0; i < kEach; ++i)
+            if (i == e) {
+              mag = win.lo + (negative ? at0 + i - kSmValues : at0 + kEach - 1 - i);
+              held = n[i];
+            }
+          edge = win.value(mag, negative);
+          ties = static_cast<int>(held);
+          if (last == sh.last_k) ties = min(ties, sh.ties_k);
+          if (last == sh.last_p) ties = min(ties, sh.ties_p);
+          state = ties < static_cast<int>(held) ? kSmTies : kSmEdge;
+        }
+        for (int r = 0; r < ranks; ++r) {
+          SmShared& o = *cl.map_shared_rank(&sh, r);
+          o.state = state;
+          o.edge = edge;
+          o.ties = ties;
+        }
+      }
+    }
+  }
+  cl.sync();
+  if (sh.state == kSmSearch) return false;
+  if (sh.state == kSmAll) return true;
+  const float edge = sh.edge;
+  row.border = composite(edge, 0x7fffffff);
+  if (sh.state == kSmEdge) return true;
+  // ---- equal logits at the border: the id of the last that is kept
+  const int ties = sh.ties;
+  const int per = (sl.vecs + kSmWarps - 1) / kSmWarps;
+  const int v_lo = min(sl.vecs, warp * per), v_hi = min(sl.vecs, v_lo + per);
+  auto ties_in = [&](int v) {
+    float x[8];
+    sl.get(v, x);
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c += x[i] == edge;
+    return c;
+  };
+  int c = 0;
+  for (int v = v_lo + lane; v < v_hi; v += 32) c += ties_in(v);
+  c = __reduce_add_sync(0xffffffffu, c);
+  if (lane == 0) sh.warp_n[warp] = c;
+  __syncthreads();
+  if (tid < ranks) {
+    c = 0;
+    for (int w = 0; w < kSmWarps; ++w) c += sh.warp_n[w];
+    cl.map_shared_rank(&sh, tid)->count_of[rank] = c;
+  }
+  cl.sync();
+  int before = 0;
+  for (int r = 0; r < rank; ++r) before += sh.count_of[r];
+  if (before < ties && before + sh.count_of[rank] >= ties) {  // in this CTA's slice
+    int from = 0;
+    while (before + sh.warp_n[from] < ties) before += sh.warp_n[from++];
+    // a warp's vectors are at most as many as the CTA has threads
+    const int first = min(sl.vecs, from * per), v = first + tid;
+    const int mine = v < min(sl.vecs, first + per) ? ties_in(v) : 0;
+    double all;
+    const SmSums sums = sm_scan(static_cast<double>(mine), sh.warp_d, all);
+    const double need = ties - before;
+    if (mine > 0 && sums.before < need && need <= sums.upto) {
+      float x[8];
+      sl.get(v, x);
+      int left = static_cast<int>(need - sums.before), id = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (x[i] == edge && left > 0) {
+          id = sl.id0 + v * 8 + i;
+          --left;
+        }
+      for (int r = 0; r < ranks; ++r) cl.map_shared_rank(&sh, r)->border = composite(edge, id);
+    }
+  }
+  cl.sync();
+  row.border = sh.border;
+  return true;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __grid_constant__ SmParams p) {
   constexpr int VE = 16 / sizeof(T);
@@ -444,30 +736,46 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 
   // ---- the largest logit (a NaN comes through)
-  float mx = -INFINITY;
-  bool nan = false;
+  float mx = -INFINITY, mn = INFINITY;  // (the smallest matters where it is finite)
   for (int v = tid; v < sl.vecs; v += kSmThreads) {  // what this thread copied
-    float e[VE];
-    sl.get(v, e);
+    if constexpr (sizeof(T) == 2) {
+      const uint4 d = data[v];
+      const float2 f = unpack_bf16x2(max_nan_bf16x2(max_nan_bf16x2(d.x, d.y), max_nan_bf16x2(d.z, d.w)));
+      const float2 g = unpack_bf16x2(min_bf16x2(min_bf16x2(d.x, d.y), min_bf16x2(d.z, d.w)));
+      mx = max_nan(mx, max_nan(f.x, f.y));
+      mn = fminf(mn, fminf(g.x, g.y));
+    } else {
+      float e[VE];
+      sl.get(v, e);
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      nan |= e[i] != e[i];
-      mx = fmaxf(mx, e[i]);
+      for (int i = 0; i < VE; ++i) mx = max_nan(mx, e[i]);
     }
   }
-  mx = warp_max(mx);
-  if (__any_sync(0xffffffffu, nan)) mx = __int_as_float(0x7fc00000);
-  if (lane == 0) sh.warp_f[warp] = mx;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+  }
+  if (lane == 0) {
+    sh.warp_f[warp] = mx;
+    sh.warp_g[warp] = mn;
+  }
   __syncthreads();
   cl.barrier_wait();
   if (tid < ranks) {
-    mx = -INFINITY;
-    for (int w = 0; w < kSmWarps; ++w) mx = mx != mx || sh.warp_f[w] != sh.warp_f[w] ? __int_as_float(0x7fc00000) : fmaxf(mx, sh.warp_f[w]);
-    cl.map_shared_rank(&sh, tid)->max_of[rank] = mx;
+    for (int w = 0; w < kSmWarps; ++w) {
+      mx = max_nan(mx, sh.warp_f[w]);
+      mn = fminf(mn, sh.warp_g[w]);
+    }
+    SmShared& o = *cl.map_shared_rank(&sh, tid);
+    o.max_of[rank] = mx;
+    o.min_of[rank] = mn;
   }
   cl.sync();
-  mx = -INFINITY;
-  for (int q = 0; q < ranks; ++q) mx = mx != mx || sh.max_of[q] != sh.max_of[q] ? __int_as_float(0x7fc00000) : fmaxf(mx, sh.max_of[q]);
+  for (int q = 0; q < ranks; ++q) {
+    mx = max_nan(mx, sh.max_of[q]);
+    mn = fminf(mn, sh.min_of[q]);
+  }
   if (!(fabsf(mx) < INFINITY) || !(temperature >= 0.0)) {  // no distribution
     if (rank == 0 && tid == 0) {
       p.tokens[r] = -1;
@@ -504,25 +812,64 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   row.bins = static_cast<float>(fmin(row.c * kSmBinsPerOctave, 1e30));
   row.min_weight = min_p > 0.0 ? fmin(min_p, 1.0) : 0.0;
   row.border = ~0ull;
-  if (top_k > 0 && top_k < p.V) sm_select<T, false>(cl, sh, sl, row, static_cast<double>(top_k));
-  if (top_p < 1.0) sm_select<T, true>(cl, sh, sl, row, top_p);
+  const bool by_k = top_k > 0 && top_k < p.V, by_p = top_p < 1.0;
+  SmWindow win{0};
+  if constexpr (sizeof(T) == 2) {
+    // magnitudes up to the largest of a logit that weighs 2^-64 or more
+    const float low = fmaxf(mn, static_cast<float>(row.max - fmin(64.0 / row.c, 1e38)));
+    const int top = static_cast<int>((__float_as_uint(mx) & 0x7fffffffu) >> 16);
+    const int down = low < 0.f ? min(static_cast<int>((__float_as_uint(low) & 0x7fffffffu) >> 16) + 1, 0x7f7f) : 0;
+    win.lo = max(0, max(top, down) - kSmValues + 1);
+    if ((by_k || by_p) && !sm_values(cl, sh, sl, row, win, by_k ? static_cast<double>(top_k) : 0.0, top_p)) {
+      row.border = ~0ull;
+      if (by_k) sm_select<T, false>(cl, sh, sl, row, static_cast<double>(top_k));
+      if (by_p) sm_select<T, true>(cl, sh, sl, row, top_p);
+    }
+  } else {
+    if (by_k) sm_select<T, false>(cl, sh, sl, row, static_cast<double>(top_k));
+    if (by_p) sm_select<T, true>(cl, sh, sl, row, top_p);
+  }
 
   // ---- the kept weights' sums, a warp's vectors being neighbours
   const float least = row.border == ~0ull ? -INFINITY : falling_value(static_cast<unsigned>(row.border >> 32));
-  const int per = (sl.vecs + kSmWarps - 1) / kSmWarps;
-  const int v_lo = min(sl.vecs, warp * per), v_hi = min(sl.vecs, v_lo + per);
+  // bf16 weights of the maximum's sign come from a table
+  const unsigned sign = __float_as_uint(mx) >> 31;
+  if constexpr (sizeof(T) == 2) {
+    __syncthreads();
+    for (int i = tid; i < kSmValues; i += kSmThreads) {
+      const float x = win.value(win.lo + i, sign);
+      const double w = x <= mx && x >= least ? pow2(row.exponent(x)) : 0.0;
+      sh.weights[i] = w >= row.min_weight ? w : 0.0;
+    }
+    __syncthreads();
+  }
   auto weight = [&](float e, int id) {
     if (e == -INFINITY || e < least || (e == least && composite(e, id) > row.border)) return 0.0;
+    if constexpr (sizeof(T) == 2) {
+      const unsigned b = __float_as_uint(e);
+      const int at = win.place(b >> 16);
+      if (b >> 31 == sign && static_cast<unsigned>(at) < kSmValues) return sh.weights[at];
+    }
     const double w = pow2(row.exponent(e));
     return w >= row.min_weight ? w : 0.0;
   };
-  double sum = 0.0;
-  for (int v = v_lo + lane; v < v_hi; v += 32) {
+  auto weigh = [&](int v) {  // a vector
     float e[VE];
     sl.get(v, e);
+    float most = e[0];
 #pragma unroll
-    for (int i = 0; i < VE; ++i) sum += weight(e[i], sl.id0 + v * VE + i);
-  }
+    for (int i = 1; i < VE; ++i) most = fmaxf(most, e[i]);
+    double sum = 0.0;
+    if (most >= least && most > -INFINITY) {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) sum += weight(e[i], sl.id0 + v * VE + i);
+    }
+    return sum;
+  };
+  const int per = (sl.vecs + kSmWarps - 1) / kSmWarps;
+  const int v_lo = min(sl.vecs, warp * per), v_hi = min(sl.vecs, v_lo + per);
+  double sum = 0.0;
+  for (int v = v_lo + lane; v < v_hi; v += 32) sum += weigh(v);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   __syncthreads();
@@ -560,66 +907,42 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     }
     at += sh.warp_d[w];
   }
-  if (here != warp) return;
-  int token = -1;      // the last kept one so far, in every lane
-  double weight_of = 0.0;
-  for (int v0 = v_lo; v0 < v_hi; v0 += 32) {
-    const int v = v0 + lane;
-    double w[VE], mine = 0.0;
-    int last = -1;
-    double last_w = 0.0;
-    if (v < v_hi) {
+  // that warp's vectors, at most 513, two for each thread
+  __syncthreads();
+  const int first = min(sl.vecs, here * per) + 2 * tid, end = min(sl.vecs, here * per + per);
+  double mine = 0.0;
+  for (int v = first; v < min(end, first + 2); ++v) mine += weigh(v);
+  double all;
+  const SmSums sums = sm_scan(mine, sh.warp_d, all);
+  // the first that passes; by rounding, or outside of [0, 1), there may be none: the last that is kept
+  if (tid == 0) {
+    sh.pick = -1;
+    sh.listed = kSmThreads;
+  }
+  __syncthreads();
+  if (mine > 0.0) {
+    atomicMax(&sh.pick, tid);
+    if (before + sums.upto > goal) atomicMin(&sh.listed, tid);
+  }
+  __syncthreads();
+  const bool passed = sh.listed < kSmThreads;
+  if (tid == (passed ? sh.listed : sh.pick)) {
+    double s = before + sums.before, weight_of = 0.0;
+    int token = -1;
+    for (int v = first; v < min(end, first + 2); ++v) {
       float e[VE];
       sl.get(v, e);
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
-        w[i] = weight(e[i], sl.id0 + v * VE + i);
-        mine += w[i];
-        if (w[i] > 0.0) {
-          last = sl.id0 + v * VE + i;
-          last_w = w[i];
+        const double w = weight(e[i], sl.id0 + v * VE + i);
+        // the first that passes, or the last
+        if (w > 0.0 && (token < 0 || !passed || !(s > goal))) {
+          token = sl.id0 + v * VE + i;
+          weight_of = w;
         }
+        s += w;
       }
     }
-    double upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double y = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += y;
-    }
-    const unsigned over = __ballot_sync(0xffffffffu, mine > 0.0 && before + upto > goal);
-    if (over) {
-      const int from = __ffs(over) - 1;
-      if (lane == from) {
-        double s = before + (upto - mine);
-        int pick = last;
-        double pick_w = last_w;
-        bool found = false;
-#pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          s += w[i];
-          if (!found && w[i] > 0.0 && s > goal) {
-            found = true;
-            pick = sl.id0 + v * VE + i;
-            pick_w = w[i];
-          }
-        }
-        token = pick;
-        weight_of = pick_w;
-      }
-      token = __shfl_sync(0xffffffffu, token, from);
-      weight_of = __shfl_sync(0xffffffffu, weight_of, from);
-      break;
-    }
-    const unsigned some = __ballot_sync(0xffffffffu, last >= 0);
-    if (some) {
-      const int from = 31 - __clz(some);
-      token = __shfl_sync(0xffffffffu, last, from);
-      weight_of = __shfl_sync(0xffffffffu, last_w, from);
-    }
-    before += __shfl_sync(0xffffffffu, upto, 31);
-  }
-  if (lane == 0) {
     p.tokens[r] = token;
     p.logprob[r] = static_cast<float>(log(weight_of / whole));
   }

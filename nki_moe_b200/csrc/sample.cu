@@ -70,7 +70,7 @@ struct SmParams {
 
 struct SmShared {
   float max_of[kSmCluster], min_of[kSmCluster];
-  double sum_of[kSmCluster];
+  u64 sum_of[kSmCluster];
   u64 lo_of[kSmCluster], hi_of[kSmCluster];
   int count_of[kSmCluster];
   double zone_of[kSmCluster];  // weight of the logits near zero, and how many they are
@@ -100,7 +100,7 @@ struct SmShared {
     } hist;
     u64 list[kSmList];
     unsigned values[2 * kSmValues];  // counts by magnitude, then of negative values
-    double weights[kSmValues];       // by magnitude, of the maximum's sign
+    u64 weights[kSmValues];           // by magnitude, of the maximum's sign
   };
 };
 enum SmState { kSmAll, kSmEdge, kSmTies, kSmSearch };
@@ -151,6 +151,12 @@ __device__ __forceinline__ uint32_t min_bf16x2(uint32_t a, uint32_t b) {
   asm("min.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+// -inf as +inf, for minima of what is finite.
+__device__ __forceinline__ uint32_t finite_or_high(uint32_t w) {
+  uint32_t m;
+  asm("set.eq.u32.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(w), "r"(0xff80ff80u));
+  return w & ~(m & 0x80008000u);
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -164,13 +170,32 @@ struct SmRow {
   float maxf;
   float bins;  // bins per unit of x
   double min_weight;
-  u64 border;  // the last (order, id) that is kept so far
+  // what is kept so far: logits above `least`, and equal ones up to an id
+  float least;
+  int last_id;
 
+  __device__ __forceinline__ bool keeps(float x, int id) const { return x > least || (x == least && id <= last_id); }
+  __device__ __forceinline__ void keep_all() {
+    least = -INFINITY;  // and no equal one: what lies before the row has negative ids
+    last_id = -0x7fffffff - 1;
+  }
+  __device__ __forceinline__ void keep_to(u64 border) {
+    least = falling_value(static_cast<unsigned>(border >> 32));
+    last_id = static_cast<int>(border & 0xffffffffu);
+  }
   __device__ __forceinline__ double exponent(float x) const { return (static_cast<double>(x) - max) * c; }
   __device__ __forceinline__ int bin(float x) const {
     return __float2int_rn(fminf(fminf(maxf - x, 3e38f) * bins, kSmBins - 1.f));
   }
 };
+
+// The warp's sum, in every lane.
+template <typename N>
+__device__ __forceinline__ N sm_sum(N v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
 
 // The CTA's part of the row.
 template <typename T>
@@ -193,21 +218,14 @@ struct SmSlice {
   }
   // f(logit, id) for every finite logit up to the row's border
   template <typename F>
-  __device__ __forceinline__ void each(u64 border, F f) const {
-    const float least = border == ~0ull ? -INFINITY : falling_value(static_cast<unsigned>(border >> 32));
+  __device__ __forceinline__ void each(const SmRow& row, F f) const {
     for (int v = threadIdx.x; v < vecs; v += kSmThreads) {
       float x[VE];
       get(v, x);
-      float most = x[0];
-#pragma unroll
-      for (int i = 1; i < VE; ++i) most = fmaxf(most, x[i]);
-      if (most < least || most == -INFINITY) continue;
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
         const int id = id0 + v * VE + i;
-        if (x[i] > least || (x[i] == least && x[i] != -INFINITY &&
-                             ((static_cast<u64>(falling(x[i])) << 32) | static_cast<unsigned>(id)) <= border))
-          f(x[i], id);
+        if (row.keeps(x[i], id)) f(x[i], id);
       }
     }
   }
@@ -219,33 +237,41 @@ __device__ __forceinline__ u64 composite(float x, int id) {
 
 // Running sums over the CTA's threads in order, each thread's before it and with
 // it (the one is bit for bit the other of the thread before); `total` gets the whole.
+template <typename N>
 struct SmSums {
-  double before, upto;
+  N before, upto;
 };
-__device__ __forceinline__ SmSums sm_scan(double v, double* warp_d, double& total) {
+template <typename N>
+__device__ __forceinline__ SmSums<N> sm_scan(N v, N* warp_sum, N& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const double w = __shfl_up_sync(0xffffffffu, v, o);
+    const N w = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += w;
   }
-  double prev = __shfl_up_sync(0xffffffffu, v, 1);
-  if (lane == 0) prev = 0.0;
-  __syncthreads();  // warp_d is free
-  if (lane == 31) warp_d[warp] = v;
+  N prev = __shfl_up_sync(0xffffffffu, v, 1);
+  if (lane == 0) prev = 0;
+  __syncthreads();  // warp_sum is free
+  if (lane == 31) warp_sum[warp] = v;
   __syncthreads();
-  double base = 0.0;
-  total = 0.0;
-  for (int w = 0; w < kSmWarps; ++w) {
-    if (w == warp) base = total;
-    total += warp_d[w];
+  N all = lane < kSmWarps ? warp_sum[lane] : N(0);
+#pragma unroll
+  for (int o = 1; o < kSmWarps; o <<= 1) {
+    const N w = __shfl_up_sync(0xffffffffu, all, o);
+    if (lane >= o) all += w;
   }
-  return SmSums{base + prev, base + v};
+  total = __shfl_sync(0xffffffffu, all, kSmWarps - 1);
+  N base = __shfl_sync(0xffffffffu, all, warp > 0 ? warp - 1 : 0);
+  if (warp == 0) base = 0;
+  N upto = base + v;
+  const N at_end = __shfl_sync(0xffffffffu, all, warp);
+  if (lane == 31) upto = at_end;  // as the next warp has it
+  return SmSums<N>{base + prev, upto};
 }
 
 // Whether this thread is the first whose running sums pass `need` (0 < need <=
 // the whole, so there is one).
-__device__ __forceinline__ bool sm_passes(const SmSums& s, double need, int* pick) {
+__device__ __forceinline__ bool sm_passes(const SmSums<double>& s, double need, int* pick) {
   if (threadIdx.x == 0) *pick = kSmThreads;
   __syncthreads();
   if (s.before < need && need <= s.upto) atomicMin(pick, static_cast<int>(threadIdx.x));
@@ -255,8 +281,8 @@ __device__ __forceinline__ bool sm_passes(const SmSums& s, double need, int* pic
 
 // Finds the last (order, id) that is kept when tokens are taken in order until
 // their count reaches k (kMass false; `limit` is k) or their weight reaches
-// `limit` times the whole (kMass).  Only tokens up to row.border take part, and
-// row.border is what comes out.  All CTAs of the cluster call it and take the
+// `limit` times the whole (kMass).  Only tokens that row keeps take part, and
+// what it keeps is what comes out.  All CTAs of the cluster call it and take the
 // same way through it.
 template <typename T, bool kMass>
 __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const SmSlice<T>& sl, SmRow& row, double limit) {
@@ -275,7 +301,7 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const SmSli
     for (int i = tid; i < kSmBins; i += kSmThreads) sh.hist.a[i] = sh.hist.b[i] = 0;
     if (first && tid == 0) sh.listed = 0;
     __syncthreads();
-    sl.each(row.border, [&](float x, int id) {
+    sl.each(row, [&](float x, int id) {
       int at;
       double y = 0.0;  // exponent of the weight relative to the bin
       if (split) {
@@ -316,7 +342,7 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const SmSli
           v[e] *= pow2(split ? top : (2 * tid + e) * (-1.0 / kSmBinsPerOctave)) * (1.0 / 2147483648.0);
       }
       double total;
-      const SmSums sums = sm_scan(v[0] + v[1], sh.warp_d, total);
+      const SmSums<double> sums = sm_scan(v[0] + v[1], sh.warp_d, total);
       if (level == 0 && tid == 0) {
         sh.target = kMass ? fmax(limit * total, 1e-300) : limit;
         sh.above = 0.0;
@@ -350,7 +376,7 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const SmSli
       hi = min(hi, lo + width - 1);
     }
     // ---- the bin's tokens to the first CTA
-    sl.each(row.border, [&](float x, int id) {
+    sl.each(row, [&](float x, int id) {
       const u64 key = composite(x, id);
       if (!member(x, key)) return;
       const int at = atomicAdd(&lead.listed, 1);
@@ -386,7 +412,7 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const SmSli
           sum += v[e];
         }
         double total;
-        const SmSums sums = sm_scan(sum, sh.warp_d, total);
+        const SmSums<double> sums = sm_scan(sum, sh.warp_d, total);
         const double need = fmin(fmax(sh.target - sh.above, 1e-300), total * (1.0 - 0x1p-50));
         if (sm_passes(sums, need, &sh.pick)) {
           double before = sums.before;
@@ -402,12 +428,12 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const SmSli
         }
       }
       cl.sync();
-      row.border = sh.border;
+      row.keep_to(sh.border);
       return;
     }
     // ---- too many: the range from the smallest to the largest of them is split
     u64 least = ~0ull, most = 0;
-    sl.each(row.border, [&](float x, int id) {
+    sl.each(row, [&](float x, int id) {
       const u64 key = composite(x, id);
       if (!member(x, key)) return;
       least = min(least, key);
@@ -460,7 +486,7 @@ struct SmWindow {
 // count as 0.  All CTAs of the cluster call it and take the same way through it;
 // false: the border lies in the zone and has to be searched.
 __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const SmSlice<__nv_bfloat16>& sl, SmRow& row,
-                          const SmWindow& win, double top_k, double top_p) {
+                          const SmWindow& win, int top_k, double top_p) {
   constexpr int kEach = 2 * kSmValues / kSmThreads;  // bins per thread
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ranks = cl.num_blocks(), rank = cl.block_rank();
   for (int i = tid; i < 2 * kSmValues / 4; i += kSmThreads) reinterpret_cast<uint4*>(sh.values)[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -485,25 +511,20 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const SmSli
       }
   }
   zones = __reduce_add_sync(0xffffffffu, zones);
-  if (zones > 0) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) zone += __shfl_xor_sync(0xffffffffu, zone, o);
-  }
+  if (zones > 0) zone = sm_sum(zone);
   if (lane == 0) {
     sh.warp_d[warp] = zone;
     sh.warp_n[warp] = zones;
   }
   __syncthreads();
-  if (tid == 0) {
-    zone = 0.0;
-    zones = 0;
-    for (int w = 0; w < kSmWarps; ++w) {
-      zone += sh.warp_d[w];
-      zones += sh.warp_n[w];
+  if (warp == 0) {
+    zones = __reduce_add_sync(0xffffffffu, lane < kSmWarps ? sh.warp_n[lane] : 0);
+    zone = zones > 0 ? sm_sum(lane < kSmWarps ? sh.warp_d[lane] : 0.0) : 0.0;
+    if (lane == 0) {
+      SmShared& o = *cl.map_shared_rank(&sh, 0);
+      o.zone_of[rank] = zone;
+      o.zones_of[rank] = zones;
     }
-    SmShared& o = *cl.map_shared_rank(&sh, 0);
-    o.zone_of[rank] = zone;
-    o.zones_of[rank] = zones;
   }
   cl.sync();
   if (rank == 0) {
@@ -517,15 +538,25 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const SmSli
       n[e] = 0;
       w[e] = 0.0;
     }
-    for (int r = 0; r < ranks; ++r) {
-      const uint4* from = reinterpret_cast<const uint4*>(cl.map_shared_rank(&sh, r)->values + at0);
+    static_assert(kEach == 8, "two vectors of counts");
+    for (int r0 = 0; r0 < ranks; r0 += 4) {  // eight loads in flight
+      uint4 c[4][2];
 #pragma unroll
-      for (int e = 0; e < kEach; e += 4) {
-        const uint4 c = from[e / 4];
-        n[e] += c.x;
-        n[e + 1] += c.y;
-        n[e + 2] += c.z;
-        n[e + 3] += c.w;
+      for (int r = 0; r < 4; ++r) {
+        const uint4* from = reinterpret_cast<const uint4*>(cl.map_shared_rank(&sh, min(r0 + r, ranks - 1))->values + at0);
+        c[r][0] = from[0];
+        c[r][1] = from[1];
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (r0 + r >= ranks) break;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          n[4 * e] += c[r][e].x;
+          n[4 * e + 1] += c[r][e].y;
+          n[4 * e + 2] += c[r][e].z;
+          n[4 * e + 3] += c[r][e].w;
+        }
       }
     }
 #pragma unroll
@@ -549,7 +580,7 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const SmSli
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       const int mag = win.lo + (negative ? at0 + e - kSmValues : at0 + kEach - 1 - e);
-      if (n[e] != 0) w[e] = pow2(row.exponent(win.value(mag, negative)));
+      w[e] = n[e] != 0 ? pow2(row.exponent(win.value(mag, negative))) : 0.0;  // (a value above the maximum has none)
       mass += n[e] * w[e];
       count += n[e];
     }
@@ -562,29 +593,32 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const SmSli
       count += n[kEach];
     }
     auto mass_of = [&](int e) { return e == kEach ? zone_w : n[e] * w[e]; };
-    double all, total;
-    const SmSums counts = sm_scan(static_cast<double>(count), sh.warp_d, all);
-    const SmSums sums = sm_scan(mass, sh.warp_d, total);
+    double total;
+    int all;
+    const SmSums<int> counts = sm_scan(static_cast<int>(count), sh.warp_n, all);
+    const SmSums<double> sums = sm_scan(mass, sh.warp_d, total);
     const int none = 0x7fffffff;
     if (tid == 0) {
       sh.last_k = sh.last_p = none;
       sh.sum_k = total;
     }
     __syncthreads();
-    if (top_k > 0.0 && top_k < all && sm_passes(counts, top_k, &sh.pick)) {
-      double c = counts.before, m = sums.before;
+    // (one thread: counts are exact)
+    if (top_k > 0 && top_k < all && counts.before < top_k && top_k <= counts.upto) {
+      int c = counts.before;
+      double m = sums.before;
       bool found = false;
 #pragma unroll
       for (int e = 0; e <= kEach; ++e) {
         if (found) continue;
-        if (c + n[e] >= top_k) {
+        if (c + static_cast<int>(n[e]) >= top_k) {
           found = true;
           sh.last_k = tid * (kEach + 1) + e;
-          sh.ties_k = static_cast<int>(top_k - c);
+          sh.ties_k = top_k - c;
           sh.sum_k = m + (top_k - c) * w[e];
           continue;
         }
-        c += n[e];
+        c += static_cast<int>(n[e]);
         m += mass_of(e);
       }
     }
@@ -642,7 +676,8 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const SmSli
   if (sh.state == kSmSearch) return false;
   if (sh.state == kSmAll) return true;
   const float edge = sh.edge;
-  row.border = composite(edge, 0x7fffffff);
+  row.least = edge;
+  row.last_id = 0x7fffffff;
   if (sh.state == kSmEdge) return true;
   // ---- equal logits at the border: the id of the last that is kept
   const int ties = sh.ties;
@@ -661,10 +696,9 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const SmSli
   c = __reduce_add_sync(0xffffffffu, c);
   if (lane == 0) sh.warp_n[warp] = c;
   __syncthreads();
-  if (tid < ranks) {
-    c = 0;
-    for (int w = 0; w < kSmWarps; ++w) c += sh.warp_n[w];
-    cl.map_shared_rank(&sh, tid)->count_of[rank] = c;
+  if (warp == 0) {
+    c = __reduce_add_sync(0xffffffffu, lane < kSmWarps ? sh.warp_n[lane] : 0);
+    if (lane < ranks) cl.map_shared_rank(&sh, lane)->count_of[rank] = c;
   }
   cl.sync();
   int before = 0;
@@ -675,13 +709,13 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const SmSli
     // a warp's vectors are at most as many as the CTA has threads
     const int first = min(sl.vecs, from * per), v = first + tid;
     const int mine = v < min(sl.vecs, first + per) ? ties_in(v) : 0;
-    double all;
-    const SmSums sums = sm_scan(static_cast<double>(mine), sh.warp_d, all);
-    const double need = ties - before;
+    int all;
+    const SmSums<int> sums = sm_scan(mine, sh.warp_n, all);
+    const int need = ties - before;
     if (mine > 0 && sums.before < need && need <= sums.upto) {
       float x[8];
       sl.get(v, x);
-      int left = static_cast<int>(need - sums.before), id = 0;
+      int left = need - sums.before, id = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (x[i] == edge && left > 0) {
@@ -692,7 +726,7 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const SmSli
     }
   }
   cl.sync();
-  row.border = sh.border;
+  row.keep_to(sh.border);
   return true;
 }
 
@@ -741,7 +775,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     if constexpr (sizeof(T) == 2) {
       const uint4 d = data[v];
       const float2 f = unpack_bf16x2(max_nan_bf16x2(max_nan_bf16x2(d.x, d.y), max_nan_bf16x2(d.z, d.w)));
-      const float2 g = unpack_bf16x2(min_bf16x2(min_bf16x2(d.x, d.y), min_bf16x2(d.z, d.w)));
+      const float2 g = unpack_bf16x2(min_bf16x2(min_bf16x2(finite_or_high(d.x), finite_or_high(d.y)),
+                                                min_bf16x2(finite_or_high(d.z), finite_or_high(d.w))));
       mx = max_nan(mx, max_nan(f.x, f.y));
       mn = fminf(mn, fminf(g.x, g.y));
     } else {
@@ -786,9 +821,13 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
 
   if (temperature == 0.0 || top_k == 1) {  // the largest, the lowest id of equal ones
     int id = 0x7fffffff;
-    sl.each(~0ull, [&](float e, int i) {
-      if (e == mx) id = min(id, i);
-    });
+    for (int v = tid; v < sl.vecs; v += kSmThreads) {
+      float e[VE];
+      sl.get(v, e);
+#pragma unroll
+      for (int i = 0; i < VE; ++i)
+        if (e[i] == mx) id = min(id, sl.id0 + v * VE + i);
+    }
     id = __reduce_min_sync(0xffffffffu, id);
     if (lane == 0) sh.warp_lo[warp] = static_cast<u64>(id);
     __syncthreads();
@@ -811,7 +850,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   row.maxf = mx;
   row.bins = static_cast<float>(fmin(row.c * kSmBinsPerOctave, 1e30));
   row.min_weight = min_p > 0.0 ? fmin(min_p, 1.0) : 0.0;
-  row.border = ~0ull;
+  row.keep_all();
   const bool by_k = top_k > 0 && top_k < p.V, by_p = top_p < 1.0;
   SmWindow win{0};
   if constexpr (sizeof(T) == 2) {
@@ -820,8 +859,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     const int top = static_cast<int>((__float_as_uint(mx) & 0x7fffffffu) >> 16);
     const int down = low < 0.f ? min(static_cast<int>((__float_as_uint(low) & 0x7fffffffu) >> 16) + 1, 0x7f7f) : 0;
     win.lo = max(0, max(top, down) - kSmValues + 1);
-    if ((by_k || by_p) && !sm_values(cl, sh, sl, row, win, by_k ? static_cast<double>(top_k) : 0.0, top_p)) {
-      row.border = ~0ull;
+    if ((by_k || by_p) && !sm_values(cl, sh, sl, row, win, by_k ? static_cast<int>(top_k) : 0, top_p)) {
+      row.keep_all();
       if (by_k) sm_select<T, false>(cl, sh, sl, row, static_cast<double>(top_k));
       if (by_p) sm_select<T, true>(cl, sh, sl, row, top_p);
     }
@@ -830,66 +869,99 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     if (by_p) sm_select<T, true>(cl, sh, sl, row, top_p);
   }
 
-  // ---- the kept weights' sums, a warp's vectors being neighbours
-  const float least = row.border == ~0ull ? -INFINITY : falling_value(static_cast<unsigned>(row.border >> 32));
-  // bf16 weights of the maximum's sign come from a table
+  // ---- the kept weights' sums, a warp's vectors being neighbours: whole numbers
+  // of 2^-44 of the largest weight, so 2^18 of them fit 64 bits and add up alike
+  // in any order.  bf16 weights of the maximum's sign come from a table.
   const unsigned sign = __float_as_uint(mx) >> 31;
+  auto fixed = [&](double w) {  // w <= 1: the sum's low 52 bits
+    const u64 bits = static_cast<u64>(__double_as_longlong(fma(w, 0x1p44, 0x1p52))) & ((1ull << 52) - 1);
+    return w >= row.min_weight ? bits : 0ull;
+  };
   if constexpr (sizeof(T) == 2) {
     __syncthreads();
-    for (int i = tid; i < kSmValues; i += kSmThreads) {
-      const float x = win.value(win.lo + i, sign);
-      const double w = x <= mx && x >= least ? pow2(row.exponent(x)) : 0.0;
-      sh.weights[i] = w >= row.min_weight ? w : 0.0;
+#pragma unroll
+    for (int i = 0; i < kSmValues / kSmThreads; ++i) {
+      const int at = tid + i * kSmThreads;
+      const float x = win.value(win.lo + at, sign);
+      const u64 w = fixed(pow2(row.exponent(fminf(x, mx))));
+      sh.weights[at] = x >= row.least ? w : 0ull;
     }
     __syncthreads();
   }
-  auto weight = [&](float e, int id) {
-    if (e == -INFINITY || e < least || (e == least && composite(e, id) > row.border)) return 0.0;
-    if constexpr (sizeof(T) == 2) {
-      const unsigned b = __float_as_uint(e);
-      const int at = win.place(b >> 16);
-      if (b >> 31 == sign && static_cast<unsigned>(at) < kSmValues) return sh.weights[at];
-    }
-    const double w = pow2(row.exponent(e));
-    return w >= row.min_weight ? w : 0.0;
-  };
-  auto weigh = [&](int v) {  // a vector
+  auto weigh = [&](int v, u64 (&w)[VE]) {  // the weights of a vector
     float e[VE];
     sl.get(v, e);
-    float most = e[0];
+    const int id = sl.id0 + v * VE;
+    if constexpr (sizeof(T) == 2) {
+      bool rest = false;
 #pragma unroll
-    for (int i = 1; i < VE; ++i) most = fmaxf(most, e[i]);
-    double sum = 0.0;
-    if (most >= least && most > -INFINITY) {
+      for (int i = 0; i < VE; ++i) {
+        const unsigned b = __float_as_uint(e[i]);
+        const int at = win.place(b >> 16);
+        const bool kept = row.keeps(e[i], id + i), here = b >> 31 == sign && static_cast<unsigned>(at) < kSmValues;
+        w[i] = 0;
+        if (kept && here) w[i] = sh.weights[at];
+        rest |= kept && !here;
+      }
+      if (rest) {
 #pragma unroll
-      for (int i = 0; i < VE; ++i) sum += weight(e[i], sl.id0 + v * VE + i);
+        for (int i = 0; i < VE; ++i) {
+          const unsigned b = __float_as_uint(e[i]);
+          const bool here = b >> 31 == sign && static_cast<unsigned>(win.place(b >> 16)) < kSmValues;
+          const u64 x = fixed(pow2(row.exponent(e[i])));
+          if (row.keeps(e[i], id + i) && !here) w[i] = x;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        const u64 x = fixed(pow2(row.exponent(e[i])));
+        w[i] = row.keeps(e[i], id + i) ? x : 0ull;
+      }
+    }
+  };
+  auto some = [&](int v) {  // whether any of a vector is kept
+    const uint4 d = data[v];
+    if constexpr (sizeof(T) == 2) {
+      const float2 f = unpack_bf16x2(max_nan_bf16x2(max_nan_bf16x2(d.x, d.y), max_nan_bf16x2(d.z, d.w)));
+      return fmaxf(f.x, f.y) >= row.least;
+    } else {
+      return fmaxf(fmaxf(__uint_as_float(d.x), __uint_as_float(d.y)), fmaxf(__uint_as_float(d.z), __uint_as_float(d.w))) >= row.least;
+    }
+  };
+  auto sum_of = [&](int v) {
+    u64 w[VE], sum = 0;
+    if (some(v)) {
+      weigh(v, w);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) sum += w[i];
     }
     return sum;
   };
   const int per = (sl.vecs + kSmWarps - 1) / kSmWarps;
   const int v_lo = min(sl.vecs, warp * per), v_hi = min(sl.vecs, v_lo + per);
-  double sum = 0.0;
-  for (int v = v_lo + lane; v < v_hi; v += 32) sum += weigh(v);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  u64 sum = 0;
+  for (int v = v_lo + lane; v < v_hi; v += 32) sum += sum_of(v);
+  sum = sm_sum(sum);
   __syncthreads();
-  if (lane == 0) sh.warp_d[warp] = sum;
+  if (lane == 0) sh.warp_lo[warp] = sum;
   __syncthreads();
-  if (tid < ranks) {
-    double all = 0.0;
-    for (int w = 0; w < kSmWarps; ++w) all += sh.warp_d[w];
-    cl.map_shared_rank(&sh, tid)->sum_of[rank] = all;
+  if (warp == 0) {
+    const u64 all = sm_sum(lane < kSmWarps ? sh.warp_lo[lane] : 0ull);
+    if (lane < ranks) cl.map_shared_rank(&sh, lane)->sum_of[rank] = all;
   }
   cl.sync();
 
-  // ---- the CTA, the warp and the token where the running sum passes u S
-  double whole = 0.0;
+  // ---- the CTA, the warp and the token where the running sum passes u S; outside
+  // of [0, 1) there may be none: the last that is kept
+  u64 whole = 0;
   for (int q = 0; q < ranks; ++q) whole += sh.sum_of[q];
-  const double goal = u * whole;
-  double before = 0.0, at = 0.0;
+  const double part = u * static_cast<double>(whole);
+  const u64 goal = part >= static_cast<double>(whole) || part != part ? whole : part > 0.0 ? static_cast<u64>(part) : 0ull;
+  u64 before = 0, at = 0;
   int here = -1;
   for (int q = 0; q < ranks; ++q) {
-    if (sh.sum_of[q] > 0.0) {
+    if (sh.sum_of[q] > 0) {
       here = q;
       before = at;
       if (at + sh.sum_of[q] > goal) break;
@@ -900,51 +972,52 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   at = before;
   here = -1;
   for (int w = 0; w < kSmWarps; ++w) {
-    if (sh.warp_d[w] > 0.0) {
+    if (sh.warp_lo[w] > 0) {
       here = w;
       before = at;
-      if (at + sh.warp_d[w] > goal) break;
+      if (at + sh.warp_lo[w] > goal) break;
     }
-    at += sh.warp_d[w];
+    at += sh.warp_lo[w];
   }
   // that warp's vectors, at most 513, two for each thread
-  __syncthreads();
   const int first = min(sl.vecs, here * per) + 2 * tid, end = min(sl.vecs, here * per + per);
-  double mine = 0.0;
-  for (int v = first; v < min(end, first + 2); ++v) mine += weigh(v);
-  double all;
-  const SmSums sums = sm_scan(mine, sh.warp_d, all);
-  // the first that passes; by rounding, or outside of [0, 1), there may be none: the last that is kept
+  u64 mine = 0;
+  for (int v = first; v < min(end, first + 2); ++v) mine += sum_of(v);
+  u64 all;
+  const SmSums<u64> sums = sm_scan(mine, sh.warp_hi, all);
   if (tid == 0) {
     sh.pick = -1;
     sh.listed = kSmThreads;
   }
   __syncthreads();
-  if (mine > 0.0) {
+  if (mine > 0) {
     atomicMax(&sh.pick, tid);
     if (before + sums.upto > goal) atomicMin(&sh.listed, tid);
   }
   __syncthreads();
   const bool passed = sh.listed < kSmThreads;
   if (tid == (passed ? sh.listed : sh.pick)) {
-    double s = before + sums.before, weight_of = 0.0;
+    u64 s = before + sums.before;
     int token = -1;
+    float x = 0.f;
     for (int v = first; v < min(end, first + 2); ++v) {
+      u64 w[VE];
       float e[VE];
+      weigh(v, w);
       sl.get(v, e);
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
-        const double w = weight(e[i], sl.id0 + v * VE + i);
         // the first that passes, or the last
-        if (w > 0.0 && (token < 0 || !passed || !(s > goal))) {
+        if (w[i] > 0 && (token < 0 || !passed || s <= goal)) {
           token = sl.id0 + v * VE + i;
-          weight_of = w;
+          x = e[i];
         }
-        s += w;
+        s += w[i];
       }
     }
     p.tokens[r] = token;
-    p.logprob[r] = static_cast<float>(log(weight_of / whole));
+    // the weight itself, not its whole number
+    p.logprob[r] = static_cast<float>(row.exponent(x) * 0.69314718055994530942 - log(static_cast<double>(whole) * 0x1p-44));
   }
 }
 

@@ -1,10 +1,11 @@
 """Sampling on the GPU against its definition in 64 bits.
 
-Tokens have to be equal: weights and sums are fp64 in the kernel, histograms hold
-weights to 2^-32, so a border may be off by some 2^-32 of the sum, and no random
-number here lies that near to one (checked: ``margin``).  A log probability is one
-rounding to fp32 (2^-24 of its value) of what 64 bits give, whose own error (2^-46 of
-the ratio under the logarithm, sums of 2^18 weights) stays below 1e-12.
+Tokens have to be equal: the weights that a draw adds up are whole numbers of 2^-44 of
+the largest, each off by 2^-45 at most, whose errors in a sum of V are V / 2 of them at
+the very most and the square root of V in earnest (2^-36 for 2^18); histograms hold weights to 2^-32 each; and
+no random number here lies nearer to a border than 2^-31 of the sum (checked:
+``margin``).  A log probability is one rounding to fp32 (2^-24 of its value) of the
+weight's logarithm less that of the sum, which is off by V 2^-45 at most.
 """
 
 import math
@@ -68,7 +69,7 @@ def check(logits, u, t=1.0, k=0, p=1.0, m=0.0, exact_margin=True):
         if math.isnan(want_lp):
             assert math.isnan(float(lp[i]))
         else:
-            assert abs(float(lp[i]) - want_lp) <= 2 ** -24 * abs(want_lp) + 1e-12
+            assert abs(float(lp[i]) - want_lp) <= 2 ** -24 * abs(want_lp) + logits.shape[1] * 2 ** -45 + 1e-12
     return token
 
 

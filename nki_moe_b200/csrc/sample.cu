@@ -13,9 +13,10 @@
 // tokens are kept.  Weights and sums are fp64; where the order of addition
 // would depend on timing (histograms) they are added as integers.
 //
-// A cluster of CTAs holds a row in shared memory, each a slice, so the logits
-// are read from HBM once and every later pass is local.  What top_k and top_p
-// keep is found from histograms:
+// Few rows: a cluster of CTAs holds a row in shared memory, each a slice, so that
+// all SMs work on them.  Many rows: a CTA takes a whole row, from the L2 after its
+// first pass, so that nothing waits for other CTAs.  What top_k and top_p keep is
+// found from histograms:
 //
 //   bf16  of the values themselves.  Of each sign the 2048 values of the 16 binary
 //         orders below the largest magnitude that matters have a bin, so counts
@@ -31,6 +32,8 @@
 // kernel of its own.
 #include <cooperative_groups.h>
 
+#include <cstddef>
+
 #include "paged.cuh"
 
 namespace nkimoe {
@@ -45,7 +48,8 @@ constexpr int kSmBins = 1024;
 constexpr int kSmBinsPerOctave = 32;
 constexpr int kSmList = 2048;        // tokens that the last sort takes
 constexpr int kSmCluster = 8;        // CTAs per row at most
-constexpr int kSmSlice = 96 * 1024;  // bytes of a row per CTA that two CTAs per SM leave room for
+constexpr int kSmSlice = 76 * 1024;  // bytes of a row per CTA that two CTAs per SM leave room for
+constexpr int kSmWholeRows = 148;    // rows from which on a CTA takes a whole one
 constexpr int kSmValues = 2048;      // values of a sign that have a bin
 constexpr int kSmMaxVocab = 1 << 18;
 static_assert(2 * kSmThreads == kSmBins, "two bins per thread");
@@ -75,6 +79,7 @@ struct SmShared {
   int count_of[kSmCluster];
   double zone_of[kSmCluster];  // weight of the logits near zero, and how many they are
   int zones_of[kSmCluster];
+  double mass_of[kSmCluster];
   // what the first CTA tells all
   int bin;        // -1: no border
   double above;   // counts or weights before the bin
@@ -83,27 +88,26 @@ struct SmShared {
   u64 border;     // the last kept (order, id)
   int listed;     // the first CTA's: tokens in its list
   int pick;
-  int state;      // of the border among values: one of kSm...
-  float edge;     // its value
-  int ties;       // how many tokens of this value are kept
-  int last_k, last_p;  // places of the borders in the list of values
-  int ties_k, ties_p;
+  // the borders of top_k and top_p among values: place in the list of values (-1:
+  // none), how many of its tokens are kept, of how many
+  int place_of[2], ties_of[2], held_of[2];
   double sum_k;
   double warp_d[kSmWarps];
   u64 warp_lo[kSmWarps], warp_hi[kSmWarps];
   int warp_n[kSmWarps];
   float warp_f[kSmWarps], warp_g[kSmWarps];
-  union {
+  union __align__(16) {
     struct {
       unsigned a[kSmBins];  // counts, or the upper halves of weights
       unsigned b[kSmBins];  // the lower halves
     } hist;
     u64 list[kSmList];
     unsigned values[2 * kSmValues];  // counts by magnitude, then of negative values
-    u64 weights[kSmValues];           // by magnitude, of the maximum's sign
+    u64 weights[2 * kSmValues];      // as the counts
   };
 };
-enum SmState { kSmAll, kSmEdge, kSmTies, kSmSearch };
+
+static_assert(offsetof(SmShared, values) % 16 == 0, "cleared by vectors");
 
 // Integers that rise as the values fall; -0 equal to +0.
 __device__ __forceinline__ unsigned falling(float x) {
@@ -197,16 +201,33 @@ __device__ __forceinline__ N sm_sum(N v) {
   return v;
 }
 
-// The CTA's part of the row.
-template <typename T>
+// The CTA's part of the row: a slice in shared memory, or (kWhole) the row itself.
+template <typename T, bool kWhole>
 struct SmSlice {
   static constexpr int VE = 16 / sizeof(T);
+  static constexpr int kAhead = kWhole ? 4 : 1;  // vectors in flight per thread
   const uint4* data;
   int vecs;
   int id0;  // of the first element (a vector may begin before the row: -inf there)
+  int V;
 
-  __device__ __forceinline__ void get(int v, float (&x)[VE]) const {
-    const uint4 u = data[v];
+  // A vector of the row in global memory; what lies outside of the row is -inf.
+  static __device__ __forceinline__ uint4 fetch(const uint4* at, int id, int V) {
+    if (id >= 0 && id + VE <= V) return __ldg(at);
+    union {
+      T e[VE];
+      uint4 u;
+    } x;
+    const T* row = reinterpret_cast<const T*>(at);
+#pragma unroll
+    for (int i = 0; i < VE; ++i) x.e[i] = id + i >= 0 && id + i < V ? row[i] : static_cast<T>(-INFINITY);
+    return x.u;
+  }
+  __device__ __forceinline__ uint4 raw(int v) const {
+    if constexpr (kWhole) return fetch(data + v, id0 + v * VE, V);
+    return data[v];
+  }
+  static __device__ __forceinline__ void unpack(const uint4& u, float (&x)[VE]) {
     if constexpr (sizeof(T) == 2) {
       unpack8(u, x);
     } else {
@@ -216,18 +237,31 @@ struct SmSlice {
       x[3] = __uint_as_float(u.w);
     }
   }
+  // f(vector, its number) for the vectors lo + at, lo + at + step, ... below hi
+  template <typename F>
+  __device__ __forceinline__ void vectors(int lo, int hi, int at, int step, F f) const {
+    for (int v = lo + at; v < hi; v += kAhead * step) {
+      uint4 u[kAhead];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a)
+        if (v + a * step < hi) u[a] = raw(v + a * step);
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a)
+        if (v + a * step < hi) f(u[a], v + a * step);
+    }
+  }
   // f(logit, id) for every finite logit up to the row's border
   template <typename F>
   __device__ __forceinline__ void each(const SmRow& row, F f) const {
-    for (int v = threadIdx.x; v < vecs; v += kSmThreads) {
+    vectors(0, vecs, threadIdx.x, kSmThreads, [&](const uint4& u, int v) {
       float x[VE];
-      get(v, x);
+      unpack(u, x);
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
         const int id = id0 + v * VE + i;
         if (row.keeps(x[i], id)) f(x[i], id);
       }
-    }
+    });
   }
 };
 
@@ -284,8 +318,8 @@ __device__ __forceinline__ bool sm_passes(const SmSums<double>& s, double need, 
 // `limit` times the whole (kMass).  Only tokens that row keeps take part, and
 // what it keeps is what comes out.  All CTAs of the cluster call it and take the
 // same way through it.
-template <typename T, bool kMass>
-__device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const SmSlice<T>& sl, SmRow& row, double limit) {
+template <bool kMass, typename Slice>
+__device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const Slice& sl, SmRow& row, double limit) {
   const int tid = threadIdx.x, ranks = cl.num_blocks();
   const bool first = cl.block_rank() == 0;
   SmShared& lead = *cl.map_shared_rank(&sh, 0);
@@ -475,26 +509,32 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const SmSli
 struct SmWindow {
   int lo;
   __device__ __forceinline__ int place(unsigned b) const { return static_cast<int>(b & 0x7fffu) - lo; }
-  __device__ __forceinline__ float value(int mag, bool negative) const {
-    return __uint_as_float(static_cast<unsigned>(mag) << 16 | (negative ? 0x80000000u : 0u));
+  __device__ __forceinline__ bool has(int at) const { return static_cast<unsigned>(at) < kSmValues; }
+  // the bin of bits b whose magnitude has place `at`
+  __device__ __forceinline__ int bin(unsigned b, int at) const { return at | (b >> 4 & kSmValues); }
+  __device__ __forceinline__ float value(int bin) const {
+    return __uint_as_float(static_cast<unsigned>(lo + (bin & (kSmValues - 1))) << 16 | (bin & kSmValues ? 0x80000000u : 0u));
   }
 };
+// Bins in falling order of their values: the positive ones by falling magnitude,
+// then the negative ones by rising magnitude.
+__device__ __forceinline__ int sm_bin_at(int place) { return place < kSmValues ? kSmValues - 1 - place : place; }
+constexpr int kSmZone = 2 * kSmValues;  // the place of what is nearer to zero than the window
 
-// The border of top_k and top_p among bf16 logits: row.border.  Values in
-// falling order are the positive ones by falling magnitude, what is nearer to
-// zero (the zone), the negative ones by rising magnitude.  Weights below 2^-64
-// count as 0.  All CTAs of the cluster call it and take the same way through it;
-// false: the border lies in the zone and has to be searched.
-__device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const SmSlice<__nv_bfloat16>& sl, SmRow& row,
-                          const SmWindow& win, int top_k, double top_p) {
-  constexpr int kEach = 2 * kSmValues / kSmThreads;  // bins per thread
+// The border of top_k (0: none) and top_p (1: none) among bf16 logits, into what
+// row keeps.  In order stand the positive values, the zone (what is nearer to zero
+// than the window), the negative ones; each CTA of the cluster has a share of the
+// bins.  Weights below 2^-64 count as 0.  All CTAs of the cluster call it and take
+// the same way through it; false: the border lies in the zone and has to be searched.
+template <typename Slice>
+__device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice& sl, SmRow& row, const SmWindow& win,
+                          int top_k, double top_p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ranks = cl.num_blocks(), rank = cl.block_rank();
   for (int i = tid; i < 2 * kSmValues / 4; i += kSmThreads) reinterpret_cast<uint4*>(sh.values)[i] = make_uint4(0u, 0u, 0u, 0u);
   __syncthreads();
   double zone = 0.0;
   int zones = 0;
-  for (int v = tid; v < sl.vecs; v += kSmThreads) {
-    const uint4 u = sl.data[v];
+  sl.vectors(0, sl.vecs, tid, kSmThreads, [&](const uint4& u, int) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -502,226 +542,208 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const SmSli
       for (int h = 0; h < 2; ++h) {
         const unsigned b = h ? w[i] >> 16 : w[i] & 0xffffu;
         const int at = win.place(b);
-        if (static_cast<unsigned>(at) < kSmValues) {
-          atomicAdd(&sh.values[at | (b >> 4 & 0x800u)], 1u);
+        if (win.has(at)) {
+          atomicAdd(&sh.values[win.bin(b, at)], 1u);
         } else if (at < 0) {
           zone += pow2(row.exponent(__uint_as_float(b << 16)));
           ++zones;
         }  // else: -inf, or too far below the maximum to weigh anything
       }
-  }
+  });
   zones = __reduce_add_sync(0xffffffffu, zones);
   if (zones > 0) zone = sm_sum(zone);
   if (lane == 0) {
     sh.warp_d[warp] = zone;
     sh.warp_n[warp] = zones;
   }
+  if (tid < 2) sh.place_of[tid] = -1;
   __syncthreads();
   if (warp == 0) {
     zones = __reduce_add_sync(0xffffffffu, lane < kSmWarps ? sh.warp_n[lane] : 0);
     zone = zones > 0 ? sm_sum(lane < kSmWarps ? sh.warp_d[lane] : 0.0) : 0.0;
-    if (lane == 0) {
-      SmShared& o = *cl.map_shared_rank(&sh, 0);
+    if (lane < ranks) {
+      SmShared& o = *cl.map_shared_rank(&sh, lane);
       o.zone_of[rank] = zone;
       o.zones_of[rank] = zones;
     }
   }
   cl.sync();
-  if (rank == 0) {
-    // thread t: places 8 t .. 8 t + 7 of the list; the zone follows the last positive one
-    unsigned n[kEach + 1];
-    double w[kEach + 1];
-    const bool negative = tid >= kSmThreads / 2;
-    const int at0 = negative ? kEach * tid : kSmValues - kEach * (tid + 1);  // lowest address of its bins
+  // ---- this CTA's share of the bins: a thread's are neighbours in the order
+  constexpr int kMost = 2 * kSmValues / kSmThreads;  // bins per thread of a whole row's CTA
+  const int shift = __ffs(kMost / ranks) - 1, each = 1 << shift, share = 2 * kSmValues / ranks;  // (1, 2, 4 or 8 CTAs)
+  const int place0 = rank * share + tid * each;
+  int n[kMost + 1];
+  double w[kMost + 1], mass[kMost + 1];
 #pragma unroll
-    for (int e = 0; e <= kEach; ++e) {
-      n[e] = 0;
-      w[e] = 0.0;
-    }
-    static_assert(kEach == 8, "two vectors of counts");
-    for (int r0 = 0; r0 < ranks; r0 += 4) {  // eight loads in flight
-      uint4 c[4][2];
+  for (int e = 0; e <= kMost; ++e) n[e] = 0;
+  {
+    unsigned got[kMost];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint4* from = reinterpret_cast<const uint4*>(cl.map_shared_rank(&sh, min(r0 + r, ranks - 1))->values + at0);
-        c[r][0] = from[0];
-        c[r][1] = from[1];
-      }
+    for (int i = 0; i < kMost; ++i)  // all loads in flight
+      got[i] = cl.map_shared_rank(&sh, i >> shift)->values[sm_bin_at(place0 + (i & (each - 1)))];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (r0 + r >= ranks) break;
+    for (int e = 0; e < kMost; ++e)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          n[4 * e] += c[r][e].x;
-          n[4 * e + 1] += c[r][e].y;
-          n[4 * e + 2] += c[r][e].z;
-          n[4 * e + 3] += c[r][e].w;
-        }
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < kEach / 2; ++e) {  // of positive values in falling order
-      const unsigned a = n[e], b = n[kEach - 1 - e];
-      n[e] = negative ? a : b;
-      n[kEach - 1 - e] = negative ? b : a;
-    }
-    const bool has_zone = tid == kSmThreads / 2 - 1;
-    if (win.lo == 0) {  // -0 is 0: the first negative bin joins the last positive one
-      __syncthreads();
-      if (tid == kSmThreads / 2) {
-        sh.pick = static_cast<int>(n[0]);
-        n[0] = 0;
-      }
-      __syncthreads();
-      if (has_zone) n[kEach - 1] += static_cast<unsigned>(sh.pick);
-    }
-    double mass = 0.0, zone_w = 0.0;
-    unsigned count = 0;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int mag = win.lo + (negative ? at0 + e - kSmValues : at0 + kEach - 1 - e);
-      w[e] = n[e] != 0 ? pow2(row.exponent(win.value(mag, negative))) : 0.0;  // (a value above the maximum has none)
-      mass += n[e] * w[e];
-      count += n[e];
-    }
-    if (has_zone) {
+      for (int i = 0; i < kMost; ++i)
+        if ((i & (each - 1)) == e) n[e] += static_cast<int>(got[i]);
+  }
+  if (win.lo == 0) {  // -0 is 0: the first negative bin joins the last positive one
+    const bool gets = place0 + each == kSmValues, gives = place0 == kSmValues;
+    if (gets)
       for (int r = 0; r < ranks; ++r) {
-        zone_w += sh.zone_of[r];
-        n[kEach] += static_cast<unsigned>(sh.zones_of[r]);
+        const int more = static_cast<int>(cl.map_shared_rank(&sh, r)->values[kSmValues]);
+#pragma unroll
+        for (int e = 0; e < kMost; ++e)
+          if (e == each - 1) n[e] += more;
       }
-      mass += zone_w;
-      count += n[kEach];
+    if (gives) n[0] = 0;
+  }
+  int count = 0;
+  double sum = 0.0;
+#pragma unroll
+  for (int e = 0; e < kMost; ++e) {
+    w[e] = pow2(row.exponent(fminf(win.value(sm_bin_at(place0 + (e < each ? e : 0))), row.maxf)));
+    mass[e] = n[e] * w[e];
+    count += n[e];
+    sum += mass[e];
+  }
+  w[kMost] = mass[kMost] = 0.0;
+  if (place0 + each == kSmValues) {  // the zone follows the last positive bin
+    for (int r = 0; r < ranks; ++r) {
+      mass[kMost] += sh.zone_of[r];
+      n[kMost] += sh.zones_of[r];
     }
-    auto mass_of = [&](int e) { return e == kEach ? zone_w : n[e] * w[e]; };
-    double total;
-    int all;
-    const SmSums<int> counts = sm_scan(static_cast<int>(count), sh.warp_n, all);
-    const SmSums<double> sums = sm_scan(mass, sh.warp_d, total);
-    const int none = 0x7fffffff;
-    if (tid == 0) {
-      sh.last_k = sh.last_p = none;
-      sh.sum_k = total;
+    count += n[kMost];
+    sum += mass[kMost];
+  }
+  double mine;
+  int held;
+  SmSums<int> counts = sm_scan(count, sh.warp_n, held);
+  SmSums<double> sums = sm_scan(sum, sh.warp_d, mine);
+  if (tid < ranks) {
+    SmShared& o = *cl.map_shared_rank(&sh, tid);
+    o.count_of[rank] = held;
+    o.mass_of[rank] = mine;
+  }
+  cl.sync();
+  int all = 0, count_before = 0;
+  double total = 0.0, mass_before = 0.0;
+  for (int r = 0; r < ranks; ++r) {
+    if (r == rank) {
+      count_before = all;
+      mass_before = total;
     }
-    __syncthreads();
-    // (one thread: counts are exact)
-    if (top_k > 0 && top_k < all && counts.before < top_k && top_k <= counts.upto) {
+    all += sh.count_of[r];
+    total += sh.mass_of[r];
+  }
+  const double mass_after = mass_before + mine;
+  counts.before += count_before;
+  counts.upto += count_before;
+  sums.before += mass_before;
+  sums.upto += mass_before;
+  // tells all CTAs border i: of a thread's bin e the first `ties` tokens are kept
+  auto tell = [&](int i, int e, int ties, int of, double kept) {
+    for (int r = 0; r < ranks; ++r) {
+      SmShared& o = *cl.map_shared_rank(&sh, r);
+      o.place_of[i] = e == kMost ? kSmZone : place0 + e;
+      o.ties_of[i] = ties;
+      o.held_of[i] = of;
+      o.sum_k = kept;
+    }
+  };
+  double kept = total;
+  if (top_k > 0 && top_k < all) {
+    if (counts.before < top_k && top_k <= counts.upto) {  // one thread
       int c = counts.before;
       double m = sums.before;
       bool found = false;
 #pragma unroll
-      for (int e = 0; e <= kEach; ++e) {
+      for (int e = 0; e <= kMost; ++e) {
         if (found) continue;
-        if (c + static_cast<int>(n[e]) >= top_k) {
-          found = true;
-          sh.last_k = tid * (kEach + 1) + e;
-          sh.ties_k = top_k - c;
-          sh.sum_k = m + (top_k - c) * w[e];
-          continue;
-        }
-        c += static_cast<int>(n[e]);
-        m += mass_of(e);
+        found = c + n[e] >= top_k;
+        if (found) tell(0, e, top_k - c, n[e], m + (top_k - c) * w[e]);
+        c += n[e];
+        m += mass[e];
       }
     }
-    __syncthreads();
-    const bool zone_k = sh.last_k == (kSmThreads / 2 - 1) * (kEach + 1) + kEach;
-    if (top_p < 1.0 && !zone_k) {
-      const double need = fmin(fmax(top_p * sh.sum_k, 1e-300), total * (1.0 - 0x1p-50));
-      if (sm_passes(sums, need, &sh.pick)) {
-        double m = sums.before;
-        bool found = false;
-#pragma unroll
-        for (int e = 0; e <= kEach; ++e) {
-          if (found || n[e] == 0) continue;
-          found = m + mass_of(e) >= need;
-          // (by rounding it may be none: then it is the thread's last)
-          sh.last_p = tid * (kEach + 1) + e;
-          sh.ties_p = w[e] > 0.0 ? static_cast<int>(fmin(fmax(ceil((need - m) / w[e]), 1.0), static_cast<double>(n[e]))) : 1;
-          m += mass_of(e);
-        }
-      }
-    }
-    __syncthreads();
-    const int last = min(sh.last_k, sh.last_p);
-    const int zone_at = (kSmThreads / 2 - 1) * (kEach + 1) + kEach;
-    if (last == none || last == zone_at || last / (kEach + 1) == tid) {
-      if (last / (kEach + 1) == tid || (tid == 0 && (last == none || last == zone_at))) {
-        int state = last == none ? kSmAll : kSmSearch, ties = 0;
-        float edge = 0.f;
-        if (last != none && last != zone_at) {
-          const int e = last % (kEach + 1);
-          int mag = 0;
-          unsigned held = 0;
-#pragma unroll
-          for (int i = 0; i < kEach; ++i)
-            if (i == e) {
-              mag = win.lo + (negative ? at0 + i - kSmValues : at0 + kEach - 1 - i);
-              held = n[i];
-            }
-          edge = win.value(mag, negative);
-          ties = static_cast<int>(held);
-          if (last == sh.last_k) ties = min(ties, sh.ties_k);
-          if (last == sh.last_p) ties = min(ties, sh.ties_p);
-          state = ties < static_cast<int>(held) ? kSmTies : kSmEdge;
-        }
-        for (int r = 0; r < ranks; ++r) {
-          SmShared& o = *cl.map_shared_rank(&sh, r);
-          o.state = state;
-          o.edge = edge;
-          o.ties = ties;
-        }
-      }
-    }
+    cl.sync();
+    if (sh.place_of[0] == kSmZone) return false;
+    kept = sh.sum_k;
   }
-  cl.sync();
-  if (sh.state == kSmSearch) return false;
-  if (sh.state == kSmAll) return true;
-  const float edge = sh.edge;
+  if (top_p < 1.0) {
+    const double need = fmin(fmax(top_p * kept, 1e-300), total * (1.0 - 0x1p-50));
+    if (mass_before < need && need <= mass_after && sm_passes(sums, need, &sh.pick)) {
+      double m = sums.before;
+      bool found = false;
+#pragma unroll
+      for (int e = 0; e <= kMost; ++e) {
+        if (found || n[e] == 0) continue;
+        found = m + mass[e] >= need;
+        // (by rounding it may be none: then it is the thread's last)
+        const double ties = w[e] > 0.0 ? fmin(fmax(ceil((need - m) / w[e]), 1.0), static_cast<double>(n[e])) : 1.0;
+        tell(1, e, static_cast<int>(ties), n[e], kept);
+        m += mass[e];
+      }
+    }
+    cl.sync();
+    if (sh.place_of[1] == kSmZone) return false;
+  }
+  // ---- the first of the two
+  const int pk = sh.place_of[0], pp = sh.place_of[1];
+  if (pk < 0 && pp < 0) return true;
+  const int i = pk < 0 || (pp >= 0 && pp < pk) ? 1 : 0;
+  const int ties = pk == pp ? min(sh.ties_of[0], sh.ties_of[1]) : sh.ties_of[i];
+  const float edge = win.value(sm_bin_at(sh.place_of[i]));
   row.least = edge;
   row.last_id = 0x7fffffff;
-  if (sh.state == kSmEdge) return true;
+  if (ties == sh.held_of[i]) return true;
   // ---- equal logits at the border: the id of the last that is kept
-  const int ties = sh.ties;
   const int per = (sl.vecs + kSmWarps - 1) / kSmWarps;
   const int v_lo = min(sl.vecs, warp * per), v_hi = min(sl.vecs, v_lo + per);
-  auto ties_in = [&](int v) {
+  auto equal = [&](const uint4& u) {
     float x[8];
-    sl.get(v, x);
+    Slice::unpack(u, x);
     int c = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) c += x[i] == edge;
     return c;
   };
   int c = 0;
-  for (int v = v_lo + lane; v < v_hi; v += 32) c += ties_in(v);
+  sl.vectors(v_lo, v_hi, lane, 32, [&](const uint4& u, int) { c += equal(u); });
   c = __reduce_add_sync(0xffffffffu, c);
+  __syncthreads();
   if (lane == 0) sh.warp_n[warp] = c;
   __syncthreads();
   if (warp == 0) {
     c = __reduce_add_sync(0xffffffffu, lane < kSmWarps ? sh.warp_n[lane] : 0);
-    if (lane < ranks) cl.map_shared_rank(&sh, lane)->count_of[rank] = c;
+    if (lane < ranks) cl.map_shared_rank(&sh, lane)->zones_of[rank] = c;
   }
   cl.sync();
   int before = 0;
-  for (int r = 0; r < rank; ++r) before += sh.count_of[r];
-  if (before < ties && before + sh.count_of[rank] >= ties) {  // in this CTA's slice
+  for (int r = 0; r < rank; ++r) before += sh.zones_of[r];
+  if (before < ties && before + sh.zones_of[rank] >= ties) {  // in this CTA's slice
     int from = 0;
     while (before + sh.warp_n[from] < ties) before += sh.warp_n[from++];
-    // a warp's vectors are at most as many as the CTA has threads
-    const int first = min(sl.vecs, from * per), v = first + tid;
-    const int mine = v < min(sl.vecs, first + per) ? ties_in(v) : 0;
-    int all;
-    const SmSums<int> sums = sm_scan(mine, sh.warp_n, all);
+    // that warp's vectors, neighbours for each thread
+    const int most = (per + kSmThreads - 1) / kSmThreads;
+    const int first = min(sl.vecs, from * per) + most * tid, end = min(sl.vecs, from * per + per);
+    int mine = 0;
+    for (int v = first; v < min(end, first + most); ++v) mine += equal(sl.raw(v));
+    int sum_all;
+    const SmSums<int> sums = sm_scan(mine, sh.warp_n, sum_all);
     const int need = ties - before;
     if (mine > 0 && sums.before < need && need <= sums.upto) {
-      float x[8];
-      sl.get(v, x);
       int left = need - sums.before, id = 0;
+      for (int v = first; v < min(end, first + most); ++v) {
+        float x[8];
+        Slice::unpack(sl.raw(v), x);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (x[i] == edge && left > 0) {
-          id = sl.id0 + v * 8 + i;
-          --left;
-        }
+        for (int i = 0; i < 8; ++i)
+          if (x[i] == edge && left > 0) {
+            id = sl.id0 + v * 8 + i;
+            --left;
+          }
+      }
       for (int r = 0; r < ranks; ++r) cl.map_shared_rank(&sh, r)->border = composite(edge, id);
     }
   }
@@ -730,16 +752,17 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const SmSli
   return true;
 }
 
-template <typename T>
+// Grid: kWhole a CTA per row, else a cluster per row.
+template <typename T, bool kWhole>
 __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __grid_constant__ SmParams p) {
-  constexpr int VE = 16 / sizeof(T);
+  using Slice = SmSlice<T, kWhole>;
+  constexpr int VE = Slice::VE;
   extern __shared__ __align__(16) uint8_t sm_raw[];
-  __shared__ SmShared sh;
+  __shared__ __align__(16) SmShared sh;
   const cg::cluster_group cl = cg::this_cluster();
   const int ranks = cl.num_blocks(), rank = cl.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long r = blockIdx.x / ranks;
-  uint4* const data = reinterpret_cast<uint4*>(sm_raw);
   cl.barrier_arrive();  // no CTA is written to before it runs
   pdl_launch_dependents();
   pdl_wait();
@@ -747,33 +770,35 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   // ---- the slice, from the 16-byte boundary at or below the row's first element on
   const T* const x = static_cast<const T*>(p.x) + r * p.row_stride;
   const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  SmSlice<T> sl;
-  sl.data = data;
+  const uint4* const row0 = reinterpret_cast<const uint4*>(x - mis);
+  Slice sl;
+  sl.V = p.V;
   sl.id0 = rank * p.slice - mis;
   sl.vecs = min(p.slice, max(0, p.V - sl.id0) + VE - 1) / VE;
-  for (int v = tid; v < sl.vecs; v += kSmThreads) {
-    const int id = sl.id0 + v * VE;
-    if (id >= 0 && id + VE <= p.V) {
-      cp_async_16(smem_u32(data + v), x + id, 16);
-    } else {
-      T* at = reinterpret_cast<T*>(data + v);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) at[i] = id + i >= 0 && id + i < p.V ? x[id + i] : static_cast<T>(-INFINITY);
+  if constexpr (kWhole) {
+    sl.data = row0;
+  } else {
+    uint4* const data = reinterpret_cast<uint4*>(sm_raw);
+    sl.data = data;
+    const uint4* const from = row0 + rank * (p.slice / VE);
+    for (int v = tid; v < sl.vecs; v += kSmThreads) {
+      const int id = sl.id0 + v * VE;
+      if (id >= 0 && id + VE <= p.V) cp_async_16(smem_u32(data + v), from + v, 16);
+      else data[v] = Slice::fetch(from + v, id, p.V);
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  asm volatile("cp.async.commit_group;" ::: "memory");
   const double temperature = p.temperature ? static_cast<double>(p.temperature[r]) : p.temperature_all;
   const long long top_k = p.top_k ? p.top_k[r] : p.top_k_all;
   const double top_p = p.top_p ? static_cast<double>(p.top_p[r]) : p.top_p_all;
   const double min_p = p.min_p ? static_cast<double>(p.min_p[r]) : p.min_p_all;
   const double u = p.u_f64 ? static_cast<const double*>(p.u)[r] : static_cast<double>(static_cast<const float*>(p.u)[r]);
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if constexpr (!kWhole) asm volatile("cp.async.wait_group 0;" ::: "memory");
 
-  // ---- the largest logit (a NaN comes through)
-  float mx = -INFINITY, mn = INFINITY;  // (the smallest matters where it is finite)
-  for (int v = tid; v < sl.vecs; v += kSmThreads) {  // what this thread copied
+  // ---- the largest logit (a NaN comes through), and of bf16 the smallest finite one
+  float mx = -INFINITY, mn = INFINITY;
+  sl.vectors(0, sl.vecs, tid, kSmThreads, [&](const uint4& d, int) {  // what this thread copied
     if constexpr (sizeof(T) == 2) {
-      const uint4 d = data[v];
       const float2 f = unpack_bf16x2(max_nan_bf16x2(max_nan_bf16x2(d.x, d.y), max_nan_bf16x2(d.z, d.w)));
       const float2 g = unpack_bf16x2(min_bf16x2(min_bf16x2(finite_or_high(d.x), finite_or_high(d.y)),
                                                 min_bf16x2(finite_or_high(d.z), finite_or_high(d.w))));
@@ -781,32 +806,38 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
       mn = fminf(mn, fminf(g.x, g.y));
     } else {
       float e[VE];
-      sl.get(v, e);
+      Slice::unpack(d, e);
 #pragma unroll
       for (int i = 0; i < VE; ++i) mx = max_nan(mx, e[i]);
     }
-  }
+  });
+  auto join = [&] {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-  }
+    for (int o = 16; o > 0; o >>= 1) {
+      mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      if (sizeof(T) == 2) mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    }
+  };
+  join();
   if (lane == 0) {
     sh.warp_f[warp] = mx;
     sh.warp_g[warp] = mn;
   }
   __syncthreads();
   cl.barrier_wait();
-  if (tid < ranks) {
-    for (int w = 0; w < kSmWarps; ++w) {
-      mx = max_nan(mx, sh.warp_f[w]);
-      mn = fminf(mn, sh.warp_g[w]);
+  if (warp == 0) {
+    mx = lane < kSmWarps ? sh.warp_f[lane] : -INFINITY;
+    mn = lane < kSmWarps ? sh.warp_g[lane] : INFINITY;
+    join();
+    if (lane < ranks) {
+      SmShared& o = *cl.map_shared_rank(&sh, lane);
+      o.max_of[rank] = mx;
+      o.min_of[rank] = mn;
     }
-    SmShared& o = *cl.map_shared_rank(&sh, tid);
-    o.max_of[rank] = mx;
-    o.min_of[rank] = mn;
   }
   cl.sync();
+  mx = -INFINITY;
+  mn = INFINITY;
   for (int q = 0; q < ranks; ++q) {
     mx = max_nan(mx, sh.max_of[q]);
     mn = fminf(mn, sh.min_of[q]);
@@ -821,23 +852,23 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
 
   if (temperature == 0.0 || top_k == 1) {  // the largest, the lowest id of equal ones
     int id = 0x7fffffff;
-    for (int v = tid; v < sl.vecs; v += kSmThreads) {
+    sl.vectors(0, sl.vecs, tid, kSmThreads, [&](const uint4& d, int v) {
       float e[VE];
-      sl.get(v, e);
+      Slice::unpack(d, e);
 #pragma unroll
       for (int i = 0; i < VE; ++i)
         if (e[i] == mx) id = min(id, sl.id0 + v * VE + i);
-    }
+    });
     id = __reduce_min_sync(0xffffffffu, id);
-    if (lane == 0) sh.warp_lo[warp] = static_cast<u64>(id);
+    if (lane == 0) sh.warp_n[warp] = id;
     __syncthreads();
-    if (tid == 0) {
-      for (int w = 0; w < kSmWarps; ++w) id = min(id, static_cast<int>(sh.warp_lo[w]));
-      cl.map_shared_rank(&sh, 0)->lo_of[rank] = static_cast<u64>(id);
+    if (warp == 0) {
+      id = __reduce_min_sync(0xffffffffu, lane < kSmWarps ? sh.warp_n[lane] : 0x7fffffff);
+      if (lane == 0) cl.map_shared_rank(&sh, 0)->count_of[rank] = id;
     }
     cl.sync();
     if (rank == 0 && tid == 0) {
-      for (int q = 0; q < ranks; ++q) id = min(id, static_cast<int>(sh.lo_of[q]));
+      for (int q = 0; q < ranks; ++q) id = min(id, sh.count_of[q]);
       p.tokens[r] = id;
       p.logprob[r] = 0.f;
     }
@@ -853,63 +884,57 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   row.keep_all();
   const bool by_k = top_k > 0 && top_k < p.V, by_p = top_p < 1.0;
   SmWindow win{0};
+  bool search = by_k || by_p;
   if constexpr (sizeof(T) == 2) {
     // magnitudes up to the largest of a logit that weighs 2^-64 or more
     const float low = fmaxf(mn, static_cast<float>(row.max - fmin(64.0 / row.c, 1e38)));
     const int top = static_cast<int>((__float_as_uint(mx) & 0x7fffffffu) >> 16);
     const int down = low < 0.f ? min(static_cast<int>((__float_as_uint(low) & 0x7fffffffu) >> 16) + 1, 0x7f7f) : 0;
     win.lo = max(0, max(top, down) - kSmValues + 1);
-    if ((by_k || by_p) && !sm_values(cl, sh, sl, row, win, by_k ? static_cast<int>(top_k) : 0, top_p)) {
-      row.keep_all();
-      if (by_k) sm_select<T, false>(cl, sh, sl, row, static_cast<double>(top_k));
-      if (by_p) sm_select<T, true>(cl, sh, sl, row, top_p);
-    }
-  } else {
-    if (by_k) sm_select<T, false>(cl, sh, sl, row, static_cast<double>(top_k));
-    if (by_p) sm_select<T, true>(cl, sh, sl, row, top_p);
+    if (search && sm_values(cl, sh, sl, row, win, by_k ? static_cast<int>(top_k) : 0, top_p)) search = false;
+  }
+  if (search) {
+    row.keep_all();
+    if (by_k) sm_select<false>(cl, sh, sl, row, static_cast<double>(top_k));
+    if (by_p) sm_select<true>(cl, sh, sl, row, top_p);
   }
 
   // ---- the kept weights' sums, a warp's vectors being neighbours: whole numbers
   // of 2^-44 of the largest weight, so 2^18 of them fit 64 bits and add up alike
-  // in any order.  bf16 weights of the maximum's sign come from a table.
-  const unsigned sign = __float_as_uint(mx) >> 31;
+  // in any order.  bf16 weights come from a table.
   auto fixed = [&](double w) {  // w <= 1: the sum's low 52 bits
     const u64 bits = static_cast<u64>(__double_as_longlong(fma(w, 0x1p44, 0x1p52))) & ((1ull << 52) - 1);
     return w >= row.min_weight ? bits : 0ull;
   };
   if constexpr (sizeof(T) == 2) {
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kSmValues / kSmThreads; ++i) {
-      const int at = tid + i * kSmThreads;
-      const float x = win.value(win.lo + at, sign);
-      const u64 w = fixed(pow2(row.exponent(fminf(x, mx))));
-      sh.weights[at] = x >= row.least ? w : 0ull;
+#pragma unroll 4
+    for (int i = tid; i < 2 * kSmValues; i += kSmThreads) {
+      const float x = win.value(i);
+      sh.weights[i] = x >= row.least ? fixed(pow2(row.exponent(fminf(x, mx)))) : 0ull;
     }
     __syncthreads();
   }
-  auto weigh = [&](int v, u64 (&w)[VE]) {  // the weights of a vector
+  auto weigh = [&](const uint4& d, int v, u64 (&w)[VE]) {  // the weights of a vector
     float e[VE];
-    sl.get(v, e);
+    Slice::unpack(d, e);
     const int id = sl.id0 + v * VE;
     if constexpr (sizeof(T) == 2) {
       bool rest = false;
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
-        const unsigned b = __float_as_uint(e[i]);
-        const int at = win.place(b >> 16);
-        const bool kept = row.keeps(e[i], id + i), here = b >> 31 == sign && static_cast<unsigned>(at) < kSmValues;
+        const unsigned b = __float_as_uint(e[i]) >> 16;
+        const int at = win.place(b);
+        const bool kept = row.keeps(e[i], id + i);
         w[i] = 0;
-        if (kept && here) w[i] = sh.weights[at];
-        rest |= kept && !here;
+        if (kept && win.has(at)) w[i] = sh.weights[win.bin(b, at)];
+        rest |= kept && !win.has(at);
       }
-      if (rest) {
+      if (rest) {  // near zero, or far below
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
-          const unsigned b = __float_as_uint(e[i]);
-          const bool here = b >> 31 == sign && static_cast<unsigned>(win.place(b >> 16)) < kSmValues;
           const u64 x = fixed(pow2(row.exponent(e[i])));
-          if (row.keeps(e[i], id + i) && !here) w[i] = x;
+          if (row.keeps(e[i], id + i) && !win.has(win.place(__float_as_uint(e[i]) >> 16))) w[i] = x;
         }
       }
     } else {
@@ -920,8 +945,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
       }
     }
   };
-  auto some = [&](int v) {  // whether any of a vector is kept
-    const uint4 d = data[v];
+  auto some = [&](const uint4& d) {  // whether any of a vector may be kept
     if constexpr (sizeof(T) == 2) {
       const float2 f = unpack_bf16x2(max_nan_bf16x2(max_nan_bf16x2(d.x, d.y), max_nan_bf16x2(d.z, d.w)));
       return fmaxf(f.x, f.y) >= row.least;
@@ -929,10 +953,10 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
       return fmaxf(fmaxf(__uint_as_float(d.x), __uint_as_float(d.y)), fmaxf(__uint_as_float(d.z), __uint_as_float(d.w))) >= row.least;
     }
   };
-  auto sum_of = [&](int v) {
+  auto sum_of = [&](const uint4& d, int v) {
     u64 w[VE], sum = 0;
-    if (some(v)) {
-      weigh(v, w);
+    if (some(d)) {
+      weigh(d, v, w);
 #pragma unroll
       for (int i = 0; i < VE; ++i) sum += w[i];
     }
@@ -941,7 +965,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   const int per = (sl.vecs + kSmWarps - 1) / kSmWarps;
   const int v_lo = min(sl.vecs, warp * per), v_hi = min(sl.vecs, v_lo + per);
   u64 sum = 0;
-  for (int v = v_lo + lane; v < v_hi; v += 32) sum += sum_of(v);
+  sl.vectors(v_lo, v_hi, lane, 32, [&](const uint4& d, int v) { sum += sum_of(d, v); });
   sum = sm_sum(sum);
   __syncthreads();
   if (lane == 0) sh.warp_lo[warp] = sum;
@@ -979,10 +1003,11 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     }
     at += sh.warp_lo[w];
   }
-  // that warp's vectors, at most 513, two for each thread
-  const int first = min(sl.vecs, here * per) + 2 * tid, end = min(sl.vecs, here * per + per);
+  // that warp's vectors, neighbours for each thread
+  const int most = (per + kSmThreads - 1) / kSmThreads;
+  const int first = min(sl.vecs, here * per) + most * tid, end = min(sl.vecs, here * per + per);
   u64 mine = 0;
-  for (int v = first; v < min(end, first + 2); ++v) mine += sum_of(v);
+  for (int v = first; v < min(end, first + most); ++v) mine += sum_of(sl.raw(v), v);
   u64 all;
   const SmSums<u64> sums = sm_scan(mine, sh.warp_hi, all);
   if (tid == 0) {
@@ -1000,11 +1025,12 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     u64 s = before + sums.before;
     int token = -1;
     float x = 0.f;
-    for (int v = first; v < min(end, first + 2); ++v) {
+    for (int v = first; v < min(end, first + most); ++v) {
       u64 w[VE];
       float e[VE];
-      weigh(v, w);
-      sl.get(v, e);
+      const uint4 d = sl.raw(v);
+      weigh(d, v, w);
+      Slice::unpack(d, e);
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
         // the first that passes, or the last
@@ -1025,15 +1051,17 @@ template <typename T>
 cudaError_t sm_launch(const SmParams& params, long long rows, cudaStream_t s) {
   constexpr int VE = 16 / sizeof(T);
   SmParams p = params;
-  // as few CTAs per row as hold it at two per SM; more where rows are few
   const long long vecs = (static_cast<long long>(p.V) + VE - 1 + VE - 1) / VE;  // a row may begin inside a vector
+  // rows enough for two on every SM: a CTA each
+  const bool whole = rows >= kSmWholeRows;
+  // else as few CTAs per row as hold it at two per SM; more where rows are few
   int ranks = 1;
-  while (ranks < kSmCluster && ((vecs + ranks - 1) / ranks) * 16 > kSmSlice) ranks *= 2;
-  while (ranks < kSmCluster && rows * ranks < device_sm_count() && vecs > 64 * ranks) ranks *= 2;
+  while (!whole && ranks < kSmCluster && ((vecs + ranks - 1) / ranks) * 16 > kSmSlice) ranks *= 2;
+  while (!whole && ranks < kSmCluster && rows * ranks < device_sm_count() && vecs > 64 * ranks) ranks *= 2;
   p.slice = static_cast<int>((vecs + ranks - 1) / ranks) * VE;
-  const size_t smem = static_cast<size_t>(p.slice) * sizeof(T);
+  const size_t smem = whole ? 0 : static_cast<size_t>(p.slice) * sizeof(T);
   constexpr int kMost = kSmMaxVocab * sizeof(T) / kSmCluster;
-  cudaError_t e = allow_smem<sample_tokens_kernel<T>>((kMost > kSmSlice ? kMost : kSmSlice) + 64);
+  cudaError_t e = allow_smem<sample_tokens_kernel<T, false>>((kMost > kSmSlice ? kMost : kSmSlice) + 64);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * ranks));
@@ -1049,7 +1077,8 @@ cudaError_t sm_launch(const SmParams& params, long long rows, cudaStream_t s) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T>, p);
+  return whole ? cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T, true>, p)
+               : cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T, false>, p);
 }
 
 }  // namespace

@@ -155,12 +155,6 @@ __device__ __forceinline__ uint32_t min_bf16x2(uint32_t a, uint32_t b) {
   asm("min.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// -inf as +inf, for minima of what is finite.
-__device__ __forceinline__ uint32_t finite_or_high(uint32_t w) {
-  uint32_t m;
-  asm("set.eq.u32.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(w), "r"(0xff80ff80u));
-  return w & ~(m & 0x80008000u);
-}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -515,6 +509,18 @@ struct SmWindow {
   __device__ __forceinline__ float value(int bin) const {
     return __uint_as_float(static_cast<unsigned>(lo + (bin & (kSmValues - 1))) << 16 | (bin & kSmValues ? 0x80000000u : 0u));
   }
+  // Byte offsets of the bins (kBytes each) of a word's two logits, the place clamped
+  // from above (what lies behind the window counts as its last bin); `below` gets a
+  // negative number where one lies nearer to zero than the window.
+  template <int kBytes>
+  __device__ __forceinline__ void offsets(uint32_t w, unsigned& first, unsigned& second, int& below) const {
+    constexpr int kShift = kBytes == 8 ? 3 : 2;
+    constexpr unsigned kMags = 0x7fffu << kShift, kSign = kSmValues * kBytes;  // the sign's bit: 13 or 14
+    const int a = static_cast<int>(w << kShift & kMags) - (lo << kShift), c = static_cast<int>(w >> (16 - kShift) & kMags) - (lo << kShift);
+    below = min(below, min(a, c));
+    first = static_cast<unsigned>(min(a, (kSmValues - 1) * kBytes)) | (w >> (4 - kShift) & kSign);
+    second = static_cast<unsigned>(min(c, (kSmValues - 1) * kBytes)) | (w >> (20 - kShift) & kSign);
+  }
 };
 // Bins in falling order of their values: the positive ones by falling magnitude,
 // then the negative ones by rising magnitude.
@@ -536,19 +542,29 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
   int zones = 0;
   sl.vectors(0, sl.vecs, tid, kSmThreads, [&](const uint4& u, int) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    unsigned at[8];
+    int below = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i) win.offsets<4>(w[i], at[2 * i], at[2 * i + 1], below);
+    if (below >= 0) {
+      // -inf, and what is too far below the maximum to weigh anything, add to the
+      // last negative bin, which no other logit is in
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const unsigned b = h ? w[i] >> 16 : w[i] & 0xffffu;
-        const int at = win.place(b);
-        if (win.has(at)) {
-          atomicAdd(&sh.values[win.bin(b, at)], 1u);
-        } else if (at < 0) {
+      for (int i = 0; i < 8; ++i) atomicAdd(reinterpret_cast<unsigned*>(reinterpret_cast<char*>(sh.values) + at[i]), 1u);
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t x = i < 2 ? u.x : i < 4 ? u.y : i < 6 ? u.z : u.w;
+        const unsigned b = i & 1 ? x >> 16 : x & 0xffffu;
+        const int place = win.place(b);
+        if (place >= 0) {
+          atomicAdd(&sh.values[win.bin(b, min(place, kSmValues - 1))], 1u);
+        } else {
           zone += pow2(row.exponent(__uint_as_float(b << 16)));
           ++zones;
-        }  // else: -inf, or too far below the maximum to weigh anything
+        }
       }
+    }
   });
   zones = __reduce_add_sync(0xffffffffu, zones);
   if (zones > 0) zone = sm_sum(zone);
@@ -586,6 +602,11 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
 #pragma unroll
       for (int i = 0; i < kMost; ++i)
         if ((i & (each - 1)) == e) n[e] += static_cast<int>(got[i]);
+  }
+  if (place0 + each == 2 * kSmValues) {  // the last negative bin holds what does not count
+#pragma unroll
+    for (int e = 0; e < kMost; ++e)
+      if (e == each - 1) n[e] = 0;
   }
   if (win.lo == 0) {  // -0 is 0: the first negative bin joins the last positive one
     const bool gets = place0 + each == kSmValues, gives = place0 == kSmValues;
@@ -752,6 +773,34 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
   return true;
 }
 
+// A weight (at most 1) in whole numbers of 2^-44, none below min_weight: the sum's
+// low 52 bits.
+__device__ __forceinline__ u64 sm_fixed(double w, double min_weight) {
+  const u64 bits = static_cast<u64>(__double_as_longlong(fma(w, 0x1p44, 0x1p52))) & ((1ull << 52) - 1);
+  return w >= min_weight ? bits : 0ull;
+}
+
+// The sum of a vector's kept weights, each formed for itself; id: of its first.
+template <typename T>
+__device__ __forceinline__ u64 sm_weigh_here(const uint4& d, int id, const SmRow& row) {
+  constexpr int VE = 16 / sizeof(T);
+  float e[VE];
+  SmSlice<T, false>::unpack(d, e);
+  u64 sum = 0;
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    const u64 x = sm_fixed(pow2(row.exponent(e[i])), row.min_weight);
+    sum += row.keeps(e[i], id + i) ? x : 0ull;
+  }
+  return sum;
+}
+__device__ __noinline__ u64 sm_weigh_rare(uint4 d, int id, SmRow row) { return sm_weigh_here<__nv_bfloat16>(d, id, row); }
+template <typename T>
+__device__ __forceinline__ u64 sm_weigh(const uint4& d, int id, const SmRow& row) {
+  if constexpr (sizeof(T) == 2) return sm_weigh_rare(d, id, row);  // near zero, or equal logits that are cut
+  else return sm_weigh_here<T>(d, id, row);
+}
+
 // Grid: kWhole a CTA per row, else a cluster per row.
 template <typename T, bool kWhole>
 __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __grid_constant__ SmParams p) {
@@ -795,22 +844,25 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   const double u = p.u_f64 ? static_cast<const double*>(p.u)[r] : static_cast<double>(static_cast<const float*>(p.u)[r]);
   if constexpr (!kWhole) asm volatile("cp.async.wait_group 0;" ::: "memory");
 
-  // ---- the largest logit (a NaN comes through), and of bf16 the smallest finite one
+  // ---- the largest logit (a NaN comes through), and of bf16 the smallest
   float mx = -INFINITY, mn = INFINITY;
-  sl.vectors(0, sl.vecs, tid, kSmThreads, [&](const uint4& d, int) {  // what this thread copied
-    if constexpr (sizeof(T) == 2) {
-      const float2 f = unpack_bf16x2(max_nan_bf16x2(max_nan_bf16x2(d.x, d.y), max_nan_bf16x2(d.z, d.w)));
-      const float2 g = unpack_bf16x2(min_bf16x2(min_bf16x2(finite_or_high(d.x), finite_or_high(d.y)),
-                                                min_bf16x2(finite_or_high(d.z), finite_or_high(d.w))));
-      mx = max_nan(mx, max_nan(f.x, f.y));
-      mn = fminf(mn, fminf(g.x, g.y));
-    } else {
+  if constexpr (sizeof(T) == 2) {
+    uint32_t high = 0xff80ff80u, low = 0x7f807f80u;
+    sl.vectors(0, sl.vecs, tid, kSmThreads, [&](const uint4& d, int) {  // what this thread copied
+      high = max_nan_bf16x2(high, max_nan_bf16x2(max_nan_bf16x2(d.x, d.y), max_nan_bf16x2(d.z, d.w)));
+      low = min_bf16x2(low, min_bf16x2(min_bf16x2(d.x, d.y), min_bf16x2(d.z, d.w)));
+    });
+    const float2 f = unpack_bf16x2(high), g = unpack_bf16x2(low);
+    mx = max_nan(f.x, f.y);
+    mn = fminf(g.x, g.y);
+  } else {
+    sl.vectors(0, sl.vecs, tid, kSmThreads, [&](const uint4& d, int) {
       float e[VE];
       Slice::unpack(d, e);
 #pragma unroll
       for (int i = 0; i < VE; ++i) mx = max_nan(mx, e[i]);
-    }
-  });
+    });
+  }
   auto join = [&] {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -884,14 +936,16 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   row.keep_all();
   const bool by_k = top_k > 0 && top_k < p.V, by_p = top_p < 1.0;
   SmWindow win{0};
-  bool search = by_k || by_p;
+  bool search = by_k || by_p, plain = true;  // plain: the table holds all weights but the zone's
   if constexpr (sizeof(T) == 2) {
-    // magnitudes up to the largest of a logit that weighs 2^-64 or more
+    // magnitudes up to beyond the largest of a negative logit that weighs 2^-64 or
+    // more: the last negative bin is left to those that weigh nothing
     const float low = fmaxf(mn, static_cast<float>(row.max - fmin(64.0 / row.c, 1e38)));
     const int top = static_cast<int>((__float_as_uint(mx) & 0x7fffffffu) >> 16);
-    const int down = low < 0.f ? min(static_cast<int>((__float_as_uint(low) & 0x7fffffffu) >> 16) + 1, 0x7f7f) : 0;
-    win.lo = max(0, max(top, down) - kSmValues + 1);
-    if (search && sm_values(cl, sh, sl, row, win, by_k ? static_cast<int>(top_k) : 0, top_p)) search = false;
+    const int down = low < 0.f ? static_cast<int>((__float_as_uint(low) & 0x7fffffffu) >> 16) + 1 : 0;
+    plain = down <= 0x7f7f && 64.0 / row.c < 1e38;
+    win.lo = max(0, min(max(top, down), 0x7f7f) - kSmValues + 1);
+    if (search && plain && sm_values(cl, sh, sl, row, win, by_k ? static_cast<int>(top_k) : 0, top_p)) search = false;
   }
   if (search) {
     row.keep_all();
@@ -902,49 +956,15 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   // ---- the kept weights' sums, a warp's vectors being neighbours: whole numbers
   // of 2^-44 of the largest weight, so 2^18 of them fit 64 bits and add up alike
   // in any order.  bf16 weights come from a table.
-  auto fixed = [&](double w) {  // w <= 1: the sum's low 52 bits
-    const u64 bits = static_cast<u64>(__double_as_longlong(fma(w, 0x1p44, 0x1p52))) & ((1ull << 52) - 1);
-    return w >= row.min_weight ? bits : 0ull;
-  };
   if constexpr (sizeof(T) == 2) {
     __syncthreads();
 #pragma unroll 4
     for (int i = tid; i < 2 * kSmValues; i += kSmThreads) {
       const float x = win.value(i);
-      sh.weights[i] = x >= row.least ? fixed(pow2(row.exponent(fminf(x, mx)))) : 0ull;
+      sh.weights[i] = x >= row.least && x <= mx && i != 2 * kSmValues - 1 ? sm_fixed(pow2(row.exponent(fminf(x, mx))), row.min_weight) : 0ull;
     }
     __syncthreads();
   }
-  auto weigh = [&](const uint4& d, int v, u64 (&w)[VE]) {  // the weights of a vector
-    float e[VE];
-    Slice::unpack(d, e);
-    const int id = sl.id0 + v * VE;
-    if constexpr (sizeof(T) == 2) {
-      bool rest = false;
-#pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        const unsigned b = __float_as_uint(e[i]) >> 16;
-        const int at = win.place(b);
-        const bool kept = row.keeps(e[i], id + i);
-        w[i] = 0;
-        if (kept && win.has(at)) w[i] = sh.weights[win.bin(b, at)];
-        rest |= kept && !win.has(at);
-      }
-      if (rest) {  // near zero, or far below
-#pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          const u64 x = fixed(pow2(row.exponent(e[i])));
-          if (row.keeps(e[i], id + i) && !win.has(win.place(__float_as_uint(e[i]) >> 16))) w[i] = x;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        const u64 x = fixed(pow2(row.exponent(e[i])));
-        w[i] = row.keeps(e[i], id + i) ? x : 0ull;
-      }
-    }
-  };
   auto some = [&](const uint4& d) {  // whether any of a vector may be kept
     if constexpr (sizeof(T) == 2) {
       const float2 f = unpack_bf16x2(max_nan_bf16x2(max_nan_bf16x2(d.x, d.y), max_nan_bf16x2(d.z, d.w)));
@@ -953,14 +973,39 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
       return fmaxf(fmaxf(__uint_as_float(d.x), __uint_as_float(d.y)), fmaxf(__uint_as_float(d.z), __uint_as_float(d.w))) >= row.least;
     }
   };
+  const uint32_t edge2 = pack_bf16x2(row.least, row.least);  // (bf16 only)
   auto sum_of = [&](const uint4& d, int v) {
-    u64 w[VE], sum = 0;
-    if (some(d)) {
-      weigh(d, v, w);
+    u64 sum = 0;
+    if (!some(d)) return sum;
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t x[4] = {d.x, d.y, d.z, d.w};
+      unsigned at[8];
+      int below = plain ? 0 : -1;
 #pragma unroll
-      for (int i = 0; i < VE; ++i) sum += w[i];
+      for (int i = 0; i < 4; ++i) win.offsets<8>(x[i], at[2 * i], at[2 * i + 1], below);
+      const int id = sl.id0 + v * VE;
+      bool ties = false;  // cut within this vector
+      if (id + VE - 1 > row.last_id && row.least > -INFINITY) {  // behind the last equal logit that is kept, if not before its vector's end
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t q;
+          asm("set.eq.u32.bf16x2 %0, %1, %2;" : "=r"(q) : "r"(x[i]), "r"(edge2));
+          m |= q;
+        }
+        ties = m != 0;
+      }
+      if (below >= 0 && !ties) {
+        u64 even = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          sum += *reinterpret_cast<const u64*>(reinterpret_cast<const char*>(sh.weights) + at[i]);
+          even += *reinterpret_cast<const u64*>(reinterpret_cast<const char*>(sh.weights) + at[i + 1]);
+        }
+        return sum + even;
+      }
     }
-    return sum;
+    return sm_weigh<T>(d, sl.id0 + v * VE, row);
   };
   const int per = (sl.vecs + kSmWarps - 1) / kSmWarps;
   const int v_lo = min(sl.vecs, warp * per), v_hi = min(sl.vecs, v_lo + per);
@@ -1026,19 +1071,21 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     int token = -1;
     float x = 0.f;
     for (int v = first; v < min(end, first + most); ++v) {
-      u64 w[VE];
       float e[VE];
-      const uint4 d = sl.raw(v);
-      weigh(d, v, w);
-      Slice::unpack(d, e);
-#pragma unroll
+      Slice::unpack(sl.raw(v), e);
+#pragma unroll 1
       for (int i = 0; i < VE; ++i) {
+        float y = e[0];
+#pragma unroll
+        for (int j = 1; j < VE; ++j) y = i == j ? e[j] : y;
+        const int id = sl.id0 + v * VE + i;
+        const u64 w = row.keeps(y, id) ? sm_fixed(pow2(row.exponent(y)), row.min_weight) : 0ull;
         // the first that passes, or the last
-        if (w[i] > 0 && (token < 0 || !passed || s <= goal)) {
-          token = sl.id0 + v * VE + i;
-          x = e[i];
+        if (w > 0 && (token < 0 || !passed || s <= goal)) {
+          token = id;
+          x = y;
         }
-        s += w[i];
+        s += w;
       }
     }
     p.tokens[r] = token;

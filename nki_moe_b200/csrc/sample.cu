@@ -51,6 +51,7 @@ constexpr int kSmCluster = 8;        // CTAs per row at most
 constexpr int kSmSlice = 76 * 1024;  // bytes of a row per CTA that two CTAs per SM leave room for
 constexpr int kSmWholeRows = 148;    // rows from which on a CTA takes a whole one
 constexpr int kSmValues = 2048;      // values of a sign that have a bin
+constexpr int kSmNear = 512;         // logits nearer to zero that a CTA sums
 constexpr int kSmMaxVocab = 1 << 18;
 static_assert(2 * kSmThreads == kSmBins, "two bins per thread");
 
@@ -86,12 +87,15 @@ struct SmShared {
   double target;
   u64 lo, hi;     // the range that is split, as (order, id)
   u64 border;     // the last kept (order, id)
+  u64 edge;       // the weight of the border's value
   int listed;     // the first CTA's: tokens in its list
   int pick;
   // the borders of top_k and top_p among values: place in the list of values (-1:
   // none), how many of its tokens are kept, of how many
   int place_of[2], ties_of[2], held_of[2];
   double sum_k;
+  int near;                 // logits nearer to zero than the window
+  unsigned short near_of[kSmNear];
   double warp_d[kSmWarps];
   u64 warp_lo[kSmWarps], warp_hi[kSmWarps];
   int warp_n[kSmWarps];
@@ -155,6 +159,12 @@ __device__ __forceinline__ uint32_t min_bf16x2(uint32_t a, uint32_t b) {
   asm("min.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+// All bits of the halves that are equal.
+__device__ __forceinline__ uint32_t equal_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("set.eq.u32.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -171,9 +181,12 @@ struct SmRow {
   // what is kept so far: logits above `least`, and equal ones up to an id
   float least;
   int last_id;
+  bool cut;  // not all equal ones: how many of this warp's vectors' are kept
+  int ties;
 
   __device__ __forceinline__ bool keeps(float x, int id) const { return x > least || (x == least && id <= last_id); }
   __device__ __forceinline__ void keep_all() {
+    cut = false;
     least = -INFINITY;  // and no equal one: what lies before the row has negative ids
     last_id = -0x7fffffff - 1;
   }
@@ -199,6 +212,7 @@ __device__ __forceinline__ N sm_sum(N v) {
 template <typename T, bool kWhole>
 struct SmSlice {
   static constexpr int VE = 16 / sizeof(T);
+  static constexpr bool kAlone = kWhole;  // a cluster of one CTA
   static constexpr int kAhead = kWhole ? 4 : 1;  // vectors in flight per thread
   const uint4* data;
   int vecs;
@@ -314,8 +328,8 @@ __device__ __forceinline__ bool sm_passes(const SmSums<double>& s, double need, 
 // same way through it.
 template <bool kMass, typename Slice>
 __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const Slice& sl, SmRow& row, double limit) {
-  const int tid = threadIdx.x, ranks = cl.num_blocks();
-  const bool first = cl.block_rank() == 0;
+  const int tid = threadIdx.x, ranks = Slice::kAlone ? 1 : cl.num_blocks();
+  const bool first = Slice::kAlone || cl.block_rank() == 0;
   SmShared& lead = *cl.map_shared_rank(&sh, 0);
   bool split = false;  // the range is [lo, hi], not yet: one bin of distances
   u64 lo = 0, hi = 0, width = 0;
@@ -535,11 +549,11 @@ constexpr int kSmZone = 2 * kSmValues;  // the place of what is nearer to zero t
 template <typename Slice>
 __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice& sl, SmRow& row, const SmWindow& win,
                           int top_k, double top_p) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ranks = cl.num_blocks(), rank = cl.block_rank();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int ranks = Slice::kAlone ? 1 : cl.num_blocks(), rank = Slice::kAlone ? 0 : cl.block_rank();
   for (int i = tid; i < 2 * kSmValues / 4; i += kSmThreads) reinterpret_cast<uint4*>(sh.values)[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (tid == 0) sh.near = 0;
   __syncthreads();
-  double zone = 0.0;
-  int zones = 0;
   sl.vectors(0, sl.vecs, tid, kSmThreads, [&](const uint4& u, int) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
     unsigned at[8];
@@ -560,33 +574,37 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
         if (place >= 0) {
           atomicAdd(&sh.values[win.bin(b, min(place, kSmValues - 1))], 1u);
         } else {
-          zone += pow2(row.exponent(__uint_as_float(b << 16)));
-          ++zones;
+          const int k = atomicAdd(&sh.near, 1);
+          if (k < kSmNear) sh.near_of[k] = static_cast<unsigned short>(b);
         }
       }
     }
   });
-  zones = __reduce_add_sync(0xffffffffu, zones);
-  if (zones > 0) zone = sm_sum(zone);
-  if (lane == 0) {
-    sh.warp_d[warp] = zone;
-    sh.warp_n[warp] = zones;
-  }
+  __syncthreads();
+  const int zones = sh.near;
+  // (their sum is the same whatever order they were listed in: whole numbers of 2^-52)
+  u64 near = 0;
+  for (int k = tid; k < min(zones, kSmNear); k += kSmThreads)
+    near += static_cast<u64>(pow2(row.exponent(__uint_as_float(static_cast<unsigned>(sh.near_of[k]) << 16))) * 0x1p52);
+  near = sm_sum(near);
+  if (lane == 0) sh.warp_lo[warp] = near;
   if (tid < 2) sh.place_of[tid] = -1;
   __syncthreads();
   if (warp == 0) {
-    zones = __reduce_add_sync(0xffffffffu, lane < kSmWarps ? sh.warp_n[lane] : 0);
-    zone = zones > 0 ? sm_sum(lane < kSmWarps ? sh.warp_d[lane] : 0.0) : 0.0;
+    near = sm_sum(lane < kSmWarps ? sh.warp_lo[lane] : 0ull);
     if (lane < ranks) {
       SmShared& o = *cl.map_shared_rank(&sh, lane);
-      o.zone_of[rank] = zone;
+      o.zone_of[rank] = static_cast<double>(near) * 0x1p-52;
       o.zones_of[rank] = zones;
     }
   }
   cl.sync();
+  for (int r = 0; r < ranks; ++r)
+    if (sh.zones_of[r] > kSmNear) return false;  // more than were listed
   // ---- this CTA's share of the bins: a thread's are neighbours in the order
   constexpr int kMost = 2 * kSmValues / kSmThreads;  // bins per thread of a whole row's CTA
-  const int shift = __ffs(kMost / ranks) - 1, each = 1 << shift, share = 2 * kSmValues / ranks;  // (1, 2, 4 or 8 CTAs)
+  const int shift = Slice::kAlone ? 3 : __ffs(kMost / ranks) - 1, each = 1 << shift, share = 2 * kSmValues / ranks;  // (1, 2, 4 or 8 CTAs)
+  static_assert(kMost == 8, "shift");
   const int place0 = rank * share + tid * each;
   int n[kMost + 1];
   double w[kMost + 1], mass[kMost + 1];
@@ -623,10 +641,17 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
   double sum = 0.0;
 #pragma unroll
   for (int e = 0; e < kMost; ++e) {
-    w[e] = pow2(row.exponent(fminf(win.value(sm_bin_at(place0 + (e < each ? e : 0))), row.maxf)));
-    mass[e] = n[e] * w[e];
+    w[e] = mass[e] = 0.0;
     count += n[e];
-    sum += mass[e];
+  }
+  if (__any_sync(0xffffffffu, count != 0)) {  // most warps' bins are empty
+#pragma unroll
+    for (int e = 0; e < kMost; ++e) {
+      if (e >= each) break;
+      w[e] = pow2(row.exponent(fminf(win.value(sm_bin_at(place0 + e)), row.maxf)));
+      mass[e] = n[e] * w[e];
+      sum += mass[e];
+    }
   }
   w[kMost] = mass[kMost] = 0.0;
   if (place0 + each == kSmValues) {  // the zone follows the last positive bin
@@ -729,9 +754,15 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
     for (int i = 0; i < 8; ++i) c += x[i] == edge;
     return c;
   };
-  int c = 0;
-  sl.vectors(v_lo, v_hi, lane, 32, [&](const uint4& u, int) { c += equal(u); });
-  c = __reduce_add_sync(0xffffffffu, c);
+  // two counts of 16 bits: a lane has at most 2^18 / 512 logits
+  const uint32_t edge2 = pack_bf16x2(edge, edge);
+  uint32_t pairs = 0;
+  sl.vectors(v_lo, v_hi, lane, 32, [&](const uint4& u, int) {
+    pairs += (equal_bf16x2(u.x, edge2) & 0x00010001u) + (equal_bf16x2(u.y, edge2) & 0x00010001u) +
+             (equal_bf16x2(u.z, edge2) & 0x00010001u) + (equal_bf16x2(u.w, edge2) & 0x00010001u);
+  });
+  const int own = __reduce_add_sync(0xffffffffu, static_cast<int>((pairs & 0xffffu) + (pairs >> 16)));
+  int c = own;
   __syncthreads();
   if (lane == 0) sh.warp_n[warp] = c;
   __syncthreads();
@@ -742,6 +773,11 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
   cl.sync();
   int before = 0;
   for (int r = 0; r < rank; ++r) before += sh.zones_of[r];
+  {  // how many of this warp's are kept
+    const int others = __reduce_add_sync(0xffffffffu, lane < warp ? sh.warp_n[lane] : 0);
+    row.ties = min(max(ties - before - others, 0), own);
+    row.cut = true;
+  }
   if (before < ties && before + sh.zones_of[rank] >= ties) {  // in this CTA's slice
     int from = 0;
     while (before + sh.warp_n[from] < ties) before += sh.warp_n[from++];
@@ -809,7 +845,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   extern __shared__ __align__(16) uint8_t sm_raw[];
   __shared__ __align__(16) SmShared sh;
   const cg::cluster_group cl = cg::this_cluster();
-  const int ranks = cl.num_blocks(), rank = cl.block_rank();
+  const int ranks = kWhole ? 1 : cl.num_blocks(), rank = kWhole ? 0 : cl.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long r = blockIdx.x / ranks;
   cl.barrier_arrive();  // no CTA is written to before it runs
@@ -959,9 +995,11 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   if constexpr (sizeof(T) == 2) {
     __syncthreads();
 #pragma unroll 4
-    for (int i = tid; i < 2 * kSmValues; i += kSmThreads) {
+    for (int i = tid; i < 2 * kSmValues; i += kSmThreads) {  // (a warp's bins are neighbours: mostly all or none)
       const float x = win.value(i);
-      sh.weights[i] = x >= row.least && x <= mx && i != 2 * kSmValues - 1 ? sm_fixed(pow2(row.exponent(fminf(x, mx))), row.min_weight) : 0ull;
+      u64 w = 0;
+      if (x >= row.least && x <= mx && i != 2 * kSmValues - 1) w = sm_fixed(pow2(row.exponent(x)), row.min_weight);
+      sh.weights[i] = w;
     }
     __syncthreads();
   }
@@ -1010,8 +1048,41 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   const int per = (sl.vecs + kSmWarps - 1) / kSmWarps;
   const int v_lo = min(sl.vecs, warp * per), v_hi = min(sl.vecs, v_lo + per);
   u64 sum = 0;
-  sl.vectors(v_lo, v_hi, lane, 32, [&](const uint4& d, int v) { sum += sum_of(d, v); });
-  sum = sm_sum(sum);
+  const int edge_place = win.place(__float_as_uint(row.least) >> 16);
+  if (sizeof(T) == 2 && plain && row.least > 0.f && edge_place > 0 && (row.cut || row.last_id == 0x7fffffff)) {
+    // only positive logits of the window are kept: as signed numbers, what is below
+    // them reads the one bin before the border's, which holds 0, so lanes that keep
+    // nothing share an access; equal logits that are cut are counted already
+    if (row.cut) {
+      __syncthreads();
+      if (tid == 0) {
+        const u64 w = sh.weights[edge_place];
+        sh.weights[edge_place] = 0;
+        sh.edge = w;
+      }
+      __syncthreads();
+    }
+    const int low = (win.lo + edge_place - 1) * 8;
+    const char* const table = reinterpret_cast<const char*>(sh.weights) - win.lo * 8;
+    u64 odd = 0;
+    sl.vectors(v_lo, v_hi, lane, 32, [&](const uint4& d, int) {
+      const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sum += *reinterpret_cast<const u64*>(table + max(static_cast<int>(w[i] << 16) >> 13, low));
+        odd += *reinterpret_cast<const u64*>(table + max(static_cast<int>(w[i]) >> 13 & ~7, low));
+      }
+    });
+    sum = sm_sum(sum + odd);
+    if (row.cut) {
+      sum += sh.edge * static_cast<u64>(row.ties);
+      __syncthreads();
+      if (tid == 0) sh.weights[edge_place] = sh.edge;
+    }
+  } else {
+    sl.vectors(v_lo, v_hi, lane, 32, [&](const uint4& d, int v) { sum += sum_of(d, v); });
+    sum = sm_sum(sum);
+  }
   __syncthreads();
   if (lane == 0) sh.warp_lo[warp] = sum;
   __syncthreads();

@@ -23,7 +23,11 @@ lengths, shared prompts, windows): :meth:`Qwen3MoEStack.prefill_paged`,
 :meth:`~Qwen3MoEStack.decode_paged`, :meth:`~Qwen3MoEStack.generate_paged` and
 :meth:`~Qwen3MoEStack.score` run the library's own attention for prompts too
 (``nkimoe_qk_norm_rope_store``, ``nkimoe_paged_prefill_attention``,
-``nkimoe_paged_decode_attention``, ``nkimoe_token_logprobs``).
+``nkimoe_paged_decode_attention``, ``nkimoe_token_logprobs``), draw from
+restricted distributions (``nkimoe_sample_tokens``), and check trees of drafted
+tokens in one step (:meth:`~Qwen3MoEStack.draft_paged`,
+:meth:`~Qwen3MoEStack.accept_paged`: ``nkimoe_paged_tree_attention``,
+``nkimoe_accept_drafts``).
 
 Decode keeps every shape static (a KV cache of ``max_seq`` positions, the
 current position in a device tensor that the attention kernel reads), so one
@@ -43,7 +47,8 @@ import torch
 import torch.nn.functional as F
 
 from . import ops
-from .paged import PagedKVCache
+from .drafts import LookupDrafts
+from .paged import CacheFull, PagedKVCache
 
 
 @contextlib.contextmanager
@@ -68,6 +73,20 @@ def _token_ids(t: torch.Tensor, vocab: int) -> torch.Tensor:
     if not t.is_cuda and t.numel() and not (0 <= int(t.min()) and int(t.max()) < vocab):
         raise ValueError(f"token ids must be in [0, {vocab})")
     return t
+
+
+@dataclass
+class DraftStep:
+    """A step with drafted tokens that waits for :meth:`Qwen3MoEStack.accept_paged`."""
+
+    seqs: list
+    lengths: list  # of the sequences before it
+    nodes: list  # of each tree
+    tokens: torch.Tensor  # packed, as ops.accept_drafts takes them
+    parents: torch.Tensor
+    cu_seqlens: torch.Tensor
+    kv_lens: torch.Tensor
+    table: torch.Tensor
 
 
 @dataclass
@@ -549,16 +568,132 @@ class Qwen3MoEStack:
         self._paged_last = (weakref.ref(cache), B)
         return out
 
+    # ------------------------------------------------------------ drafted tokens
+    @torch.inference_mode()
+    def draft_paged(self, cache: PagedKVCache, seqs, tokens, parents=None) -> tuple[torch.Tensor, DraftStep]:
+        """One step for a tree of tokens per sequence: ``tokens[i]`` (at most 64
+        token ids, the first being what comes next in sequence ``seqs[i]``, the
+        others drafts of what may follow) and ``parents[i]`` (for each the index
+        of its parent, below its own, -1 for the first; None: each follows the one
+        before).  Returns the logits after every node ``[sum of nodes, V]``, packed,
+        and the step, which :meth:`accept_paged` ends: until then the sequences
+        hold all nodes.  Where the call fails, they keep their lengths."""
+        if any(lyr.ep is not None for lyr in self.layers):
+            raise ValueError("drafted tokens are for stacks on one GPU: ranks would take different numbers of steps")
+        seqs, c = list(seqs), self.cfg
+        nodes = self._prompt_lengths(seqs, tokens)
+        if max(nodes) > 64:
+            raise ValueError(f"trees of at most 64 nodes, not {max(nodes)}")
+        if parents is None:
+            parents = [range(-1, n - 1) for n in nodes]
+        parents = [[int(x) for x in p] for p in parents]
+        if len(parents) != len(seqs) or [len(p) for p in parents] != nodes:
+            raise ValueError("one parent for each node")
+        for p in parents:
+            if p[0] != -1 or any(not 0 <= x < i for i, x in enumerate(p) if i):
+                raise ValueError("the first node's parent is -1, the others' are nodes before them")
+        lengths = [cache.length(q) for q in seqs]
+        with _appending(cache, seqs, nodes):
+            cu = torch.zeros(len(seqs) + 1, dtype=torch.int32)
+            cu[1:] = torch.tensor(nodes).cumsum(0)
+            step = DraftStep(seqs, lengths, nodes,
+                             torch.cat([t.reshape(-1).to(self.device, torch.int64) for t in tokens]),
+                             torch.tensor([x for p in parents for x in p], dtype=torch.int32).to(self.device),
+                             cu.to(self.device),
+                             torch.tensor([n + m for n, m in zip(lengths, nodes)], dtype=torch.int32).to(self.device),
+                             cache.table(seqs).to(self.device))
+            T = step.tokens.numel()
+            linear = ops.skinny_linear if T <= 16 and self._skinny_ok else F.linear
+
+            def attention(li, lyr, xn):
+                k, v = cache.layer(li)
+                return ops.paged_tree_attention(linear(xn, lyr.qkv_w), lyr.q_norm, lyr.k_norm, step.parents,
+                                                step.cu_seqlens, step.kv_lens, k, v, step.table, c.num_attention_heads,
+                                                c.num_key_value_heads, c.rope_theta, c.rms_norm_eps,
+                                                window=cache.window, sinks=cache.sinks)
+
+            hn = self._layers(F.embedding(step.tokens, self.embed), attention, linear, decode=True)
+            return linear(hn, self.lm_head), step
+
+    @torch.inference_mode()
+    def accept_paged(self, cache: PagedKVCache, step: DraftStep, sampled: torch.Tensor) -> list[torch.Tensor]:
+        """Ends a step with drafted tokens: ``sampled`` (int64 on the device) is the
+        token drawn after each of its nodes, from the logits of :meth:`draft_paged`.
+        Of each tree the path that the drawn tokens agree with stays in the
+        sequence, the other nodes leave it.  Returns for each sequence the rows of
+        its path: ``sampled[rows[i]]`` are its new tokens, of which the last is not
+        in the cache yet."""
+        if any(q not in cache or cache.length(q) != n + m for q, n, m in zip(step.seqs, step.lengths, step.nodes)):
+            raise ValueError("the sequences are not as the step left them")
+        counts, path, _ = ops.accept_drafts(step.tokens, sampled, step.parents, step.cu_seqlens, step.kv_lens, cache.pool,
+                                            step.table)
+        counts = counts.tolist()
+        cache.take_back(step.seqs, [n + k for n, k in zip(step.lengths, counts)])
+        for q in step.seqs:
+            cache.trim(q)
+        starts = torch.tensor(step.nodes).cumsum(0) - torch.tensor(step.nodes)
+        return [path[a:a + k].long() + a for a, k in zip(starts.tolist(), counts)]
+
+    def _draw(self, logits, temperature, top_k, top_p, min_p, generator):
+        """Tokens from rows of logits, by a random number each."""
+        if temperature == 0:
+            return logits.argmax(-1)
+        u = torch.rand(logits.shape[0], dtype=torch.float64, device=self.device, generator=generator)
+        return ops.sample_tokens(logits, u, temperature, top_k, top_p, min_p)[0]
+
+    def _generate_drafted(self, cache, seqs, tok, prompts, max_new, drafts, draw, top_logprobs, scores):
+        """The loop of :meth:`generate_paged` with drafts, from each sequence's first
+        new token on; appends to ``scores`` (one list per sequence)."""
+        new = [[int(t)] for t in tok.tolist()]
+        texts = [LookupDrafts(p + n) for p, n in zip(prompts, new)]
+        live = [i for i in range(len(seqs)) if max_new > 1]
+        while live:
+            trees = []
+            for i in live:
+                room = cache.max_pages * cache.page_size - cache.length(seqs[i])
+                most = max(0, min(drafts, max_new - len(new[i]) - 1, 63, room - 1))
+                tokens, parents = texts[i].tree(most)
+                trees.append(([new[i][-1]] + tokens, [-1] + [x + 1 for x in parents]))
+            for attempt in (trees, [(t[:1], p[:1]) for t, p in trees]):  # pages may be short of drafts
+                try:
+                    logits, step = self.draft_paged(cache, [seqs[i] for i in live], [torch.tensor(t) for t, _ in attempt],
+                                                    [p for _, p in attempt])
+                    break
+                except CacheFull:
+                    if attempt is not trees:
+                        raise
+            sampled = draw(logits)
+            rows = self.accept_paged(cache, step, sampled)
+            kept = torch.cat(rows)
+            if top_logprobs is not None:
+                parts = ops.token_logprobs(logits[kept], sampled[kept], top_logprobs)
+                at = 0
+                for i, r in zip(live, rows):
+                    scores[i].append(tuple(x[at:at + len(r)] for x in parts))
+                    at += len(r)
+            drawn = sampled[kept].tolist()
+            for i, r in zip(live, rows):
+                new[i] += drawn[:len(r)]
+                texts[i].extend(drawn[:len(r)])
+                drawn = drawn[len(r):]
+            live = [i for i in live if len(new[i]) < max_new]
+        return new
+
     @torch.inference_mode()
     def generate_paged(self, prompts, max_new_tokens: int, samples: int = 1, temperature: float = 0.0,
                        top_logprobs: int | None = None, page_size: int = 64, window: int = 0, sinks: int = 0,
                        generator: torch.Generator | None = None, cache: PagedKVCache | None = None,
-                       graph: bool = True):
+                       graph: bool = True, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, drafts: int = 0):
         """Generation for prompts of any lengths, ``samples`` continuations of
         each from one prefill (the prompt's pages are shared).
 
         Greedy with ``temperature`` 0, else sampled (``generator`` on the
-        stack's device).  With ``window`` the model attends to the last
+        stack's device), with ``top_k``, ``top_p`` and ``min_p`` from the
+        distribution that they restrict (:func:`nki_moe_b200.ops.sample_tokens`).
+        With ``drafts`` each step checks up to so many tokens (at most 63) that the
+        text itself suggests (:class:`nki_moe_b200.drafts.LookupDrafts`) and keeps
+        those that the model agrees with: the tokens are the model's own, in fewer
+        steps where texts repeat; steps are not captured then.  With ``window`` the model attends to the last
         ``window`` tokens and the first ``sinks`` ones; a ``cache`` that is given
         brings its own page size and window.  Returns ``(tokens
         [len(prompts), samples, max_new_tokens], scores)``; ``scores`` is None
@@ -567,7 +702,14 @@ class Qwen3MoEStack:
         ``[.., max_new_tokens, top_logprobs]``."""
         if samples < 1 or max_new_tokens < 1:
             raise ValueError("samples and max_new_tokens must be positive")
-        n, ends, own = len(prompts), [int(p.numel()) + max_new_tokens for p in prompts], cache is None
+        if not (0 <= top_p <= 1 and 0 <= min_p <= 1 and top_k >= 0 and 0 <= drafts <= 63):
+            raise ValueError("top_k must not be negative, top_p and min_p must be in [0, 1], drafts in [0, 63]")
+        if drafts and any(lyr.ep is not None for lyr in self.layers):
+            raise ValueError("drafts are for stacks on one GPU")
+        restricted = top_k > 0 or top_p < 1 or min_p > 0
+        if (restricted or drafts) and not temperature >= 0:
+            raise ValueError("temperature must not be negative")
+        n, ends, own = len(prompts), [int(p.numel()) + max_new_tokens + drafts for p in prompts], cache is None
         if n == 0:
             raise ValueError("no prompts")
         if cache is None:
@@ -581,8 +723,21 @@ class Qwen3MoEStack:
             seqs = [q for first in seqs for q in [first] + [cache.fork(first) for _ in range(samples - 1)]]
             logits = logits.repeat_interleave(samples, 0)
             out, scores = [], []
-            for i in range(max_new_tokens):
-                if temperature > 0:
+
+            def draw(rows):
+                return self._draw(rows, temperature, top_k, top_p, min_p, generator)
+
+            if drafts:
+                tok = draw(logits)
+                if top_logprobs is not None:
+                    scores = [[tuple(x[i:i + 1] for x in ops.token_logprobs(logits, tok, top_logprobs))]
+                              for i in range(len(seqs))]
+                texts = [p.reshape(-1).tolist() for p in prompts for _ in range(samples)]
+                out = self._generate_drafted(cache, seqs, tok, texts, max_new_tokens, drafts, draw, top_logprobs, scores)
+            for i in range(0 if drafts else max_new_tokens):
+                if temperature > 0 and restricted:
+                    tok = draw(logits)
+                elif temperature > 0:
                     # the largest of logits + Gumbel noise is a sample of the softmax
                     noise = torch.empty_like(logits, dtype=torch.float32).exponential_(generator=generator).log()
                     tok = (logits.float() / temperature - noise).argmax(-1)
@@ -599,10 +754,15 @@ class Qwen3MoEStack:
                     cache.free(q)
             if own:
                 self._drop_steps(cache)  # nobody else can use this cache
-        tokens = torch.stack(out, 1).view(n, samples, max_new_tokens)
+        tokens = torch.tensor(out, device=self.device) if drafts else torch.stack(out, 1)
+        tokens = tokens.view(n, samples, max_new_tokens)
         if top_logprobs is None:
             return tokens, None
-        lp, ent, tlp, tid = (torch.stack(x, 1) for x in zip(*scores))
+        if drafts:
+            lp, ent, tlp, tid = (torch.stack([torch.cat(x) for x in part]) for part in
+                                 zip(*([[s[k] for s in seq] for k in range(4)] for seq in scores)))
+        else:
+            lp, ent, tlp, tid = (torch.stack(x, 1) for x in zip(*scores))
         shape = (n, samples, max_new_tokens)
         return tokens, {"logprob": lp.view(shape), "entropy": ent.view(shape), "top_logprobs": tlp.view(*shape, -1),
                         "top_ids": tid.view(*shape, -1)}

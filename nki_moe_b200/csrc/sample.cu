@@ -96,6 +96,7 @@ struct SmShared {
   double sum_k;
   int near;                 // logits nearer to zero than the window
   unsigned short near_of[kSmNear];
+  double powers[64];  // 2^(j / 64)
   double warp_d[kSmWarps];
   u64 warp_lo[kSmWarps], warp_hi[kSmWarps];
   int warp_n[kSmWarps];
@@ -145,8 +146,23 @@ __device__ __forceinline__ double pow2(double t) {
   return t < -1022.0 ? 0.0 : __hiloint2double(__double2hiint(y) + (n << 20), __double2loint(y));
 }
 
-__device__ __forceinline__ float sm_float(float v) { return v; }
-__device__ __forceinline__ float sm_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+// The same for many: t = n / 64 + f with |f| <= 1/128, 2^(n / 64) from a table of 64
+// (2^(j / 64)) and the exponent, 2^f by four terms (the first left out is
+// (0.0054)^5 / 120 = 2^-44.5); 0 below 2^-60.  11 operations in 64 bits, not 21 (an
+// SM does 64 a cycle).
+__device__ __forceinline__ double pow2_by(const double* table, double t) {
+  const double big = 105553116266496.0;  // 1.5 * 2^46: the sum's low word is rint(64 t)
+  const double s = t + big;
+  const int n = __double2loint(s);
+  const double f = t - (s - big);
+  double y = 0.0096181291076284771619790715736589;  // ln(2)^k / k!
+  y = fma(y, f, 0.055504108664821579953142263768622);
+  y = fma(y, f, 0.24022650695910071233355126316333);
+  y = fma(y, f, 0.69314718055994530941723212145818);
+  const double w = table[n & 63];
+  y = fma(w * y, f, w);
+  return t < -60.0 ? 0.0 : __hiloint2double(__double2hiint(y) + ((n >> 6) << 20), __double2loint(y));
+}
 
 // Maxima that let a NaN through, and minima that pass one over.
 __device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
@@ -357,7 +373,7 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const Slice
       }
       if constexpr (kMass) {
         // in units of 2^-31, at most 2^32 - 1; the halves of 65536 weights add up in 32 bits
-        const double q = pow2(y) * 2147483648.0;
+        const double q = pow2_by(sh.powers, y) * 2147483648.0;
         const unsigned w = q >= 4294967295.0 ? 0xffffffffu : __double2uint_rn(q);
         atomicAdd(&sh.hist.a[at], w >> 16);
         atomicAdd(&sh.hist.b[at], w & 0xffffu);
@@ -450,7 +466,7 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const Slice
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
           const int i = tid * kEach + e;
-          v[e] = i >= n ? 0.0 : kMass ? pow2(row.exponent(falling_value(static_cast<unsigned>(sh.list[i] >> 32)))) : 1.0;
+          v[e] = i >= n ? 0.0 : kMass ? pow2_by(sh.powers, row.exponent(falling_value(static_cast<unsigned>(sh.list[i] >> 32)))) : 1.0;
           sum += v[e];
         }
         double total;
@@ -585,7 +601,7 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
   // (their sum is the same whatever order they were listed in: whole numbers of 2^-52)
   u64 near = 0;
   for (int k = tid; k < min(zones, kSmNear); k += kSmThreads)
-    near += static_cast<u64>(pow2(row.exponent(__uint_as_float(static_cast<unsigned>(sh.near_of[k]) << 16))) * 0x1p52);
+    near += static_cast<u64>(pow2_by(sh.powers, row.exponent(__uint_as_float(static_cast<unsigned>(sh.near_of[k]) << 16))) * 0x1p52);
   near = sm_sum(near);
   if (lane == 0) sh.warp_lo[warp] = near;
   if (tid < 2) sh.place_of[tid] = -1;
@@ -648,7 +664,7 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
 #pragma unroll
     for (int e = 0; e < kMost; ++e) {
       if (e >= each) break;
-      w[e] = pow2(row.exponent(fminf(win.value(sm_bin_at(place0 + e)), row.maxf)));
+      w[e] = pow2_by(sh.powers, row.exponent(fminf(win.value(sm_bin_at(place0 + e)), row.maxf)));
       mass[e] = n[e] * w[e];
       sum += mass[e];
     }
@@ -818,23 +834,25 @@ __device__ __forceinline__ u64 sm_fixed(double w, double min_weight) {
 
 // The sum of a vector's kept weights, each formed for itself; id: of its first.
 template <typename T>
-__device__ __forceinline__ u64 sm_weigh_here(const uint4& d, int id, const SmRow& row) {
+__device__ __forceinline__ u64 sm_weigh_here(const uint4& d, int id, const SmRow& row, const double* powers) {
   constexpr int VE = 16 / sizeof(T);
   float e[VE];
   SmSlice<T, false>::unpack(d, e);
   u64 sum = 0;
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
-    const u64 x = sm_fixed(pow2(row.exponent(e[i])), row.min_weight);
+    const u64 x = sm_fixed(pow2_by(powers, row.exponent(e[i])), row.min_weight);
     sum += row.keeps(e[i], id + i) ? x : 0ull;
   }
   return sum;
 }
-__device__ __noinline__ u64 sm_weigh_rare(uint4 d, int id, SmRow row) { return sm_weigh_here<__nv_bfloat16>(d, id, row); }
+__device__ __noinline__ u64 sm_weigh_rare(uint4 d, int id, SmRow row, const double* powers) {
+  return sm_weigh_here<__nv_bfloat16>(d, id, row, powers);
+}
 template <typename T>
-__device__ __forceinline__ u64 sm_weigh(const uint4& d, int id, const SmRow& row) {
-  if constexpr (sizeof(T) == 2) return sm_weigh_rare(d, id, row);  // near zero, or equal logits that are cut
-  else return sm_weigh_here<T>(d, id, row);
+__device__ __forceinline__ u64 sm_weigh(const uint4& d, int id, const SmRow& row, const double* powers) {
+  if constexpr (sizeof(T) == 2) return sm_weigh_rare(d, id, row, powers);  // near zero, or equal logits that are cut
+  else return sm_weigh_here<T>(d, id, row, powers);
 }
 
 // Grid: kWhole a CTA per row, else a cluster per row.
@@ -849,6 +867,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long r = blockIdx.x / ranks;
   cl.barrier_arrive();  // no CTA is written to before it runs
+  if (tid < 64) sh.powers[tid] = pow2(tid * (1.0 / 64));
   pdl_launch_dependents();
   pdl_wait();
 
@@ -989,6 +1008,19 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     if (by_p) sm_select<true>(cl, sh, sl, row, top_p);
   }
 
+  // what weighs less than min_p need not be looked at: a bound a little below it
+  // (the weights themselves decide)
+  if (row.min_weight > 0.0) {
+    float bound = static_cast<float>(row.max + log2(row.min_weight) / row.c);
+    bound -= fabsf(bound) * 0x1p-22f + 1e-30f;
+    if (bound > row.least) {
+      row.least = bound;
+      row.last_id = 0x7fffffff;
+      row.cut = false;
+      if (sizeof(T) == 2 && bound > 0.f) row.least = __uint_as_float(__float_as_uint(bound) & 0xffff0000u);
+    }
+  }
+
   // ---- the kept weights' sums, a warp's vectors being neighbours: whole numbers
   // of 2^-44 of the largest weight, so 2^18 of them fit 64 bits and add up alike
   // in any order.  bf16 weights come from a table.
@@ -998,7 +1030,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     for (int i = tid; i < 2 * kSmValues; i += kSmThreads) {  // (a warp's bins are neighbours: mostly all or none)
       const float x = win.value(i);
       u64 w = 0;
-      if (x >= row.least && x <= mx && i != 2 * kSmValues - 1) w = sm_fixed(pow2(row.exponent(x)), row.min_weight);
+      if (x >= row.least && x <= mx && i != 2 * kSmValues - 1) w = sm_fixed(pow2_by(sh.powers, row.exponent(x)), row.min_weight);
       sh.weights[i] = w;
     }
     __syncthreads();
@@ -1043,7 +1075,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
         return sum + even;
       }
     }
-    return sm_weigh<T>(d, sl.id0 + v * VE, row);
+    return sm_weigh<T>(d, sl.id0 + v * VE, row, sh.powers);
   };
   const int per = (sl.vecs + kSmWarps - 1) / kSmWarps;
   const int v_lo = min(sl.vecs, warp * per), v_hi = min(sl.vecs, v_lo + per);
@@ -1150,7 +1182,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
 #pragma unroll
         for (int j = 1; j < VE; ++j) y = i == j ? e[j] : y;
         const int id = sl.id0 + v * VE + i;
-        const u64 w = row.keeps(y, id) ? sm_fixed(pow2(row.exponent(y)), row.min_weight) : 0ull;
+        const u64 w = row.keeps(y, id) ? sm_fixed(pow2_by(sh.powers, row.exponent(y)), row.min_weight) : 0ull;
         // the first that passes, or the last
         if (w > 0 && (token < 0 || !passed || s <= goal)) {
           token = id;

@@ -87,7 +87,6 @@ struct SmShared {
   double target;
   u64 lo, hi;     // the range that is split, as (order, id)
   u64 border;     // the last kept (order, id)
-  u64 edge;       // the weight of the border's value
   int listed;     // the first CTA's: tokens in its list
   int pick;
   // the borders of top_k and top_p among values: place in the list of values (-1:
@@ -197,7 +196,7 @@ struct SmRow {
   // what is kept so far: logits above `least`, and equal ones up to an id
   float least;
   int last_id;
-  bool cut;  // not all equal ones: how many of this warp's vectors' are kept
+  bool cut;  // of equal ones the first `ties` in the order of their ids
   int ties;
 
   __device__ __forceinline__ bool keeps(float x, int id) const { return x > least || (x == least && id <= last_id); }
@@ -557,45 +556,55 @@ struct SmWindow {
 __device__ __forceinline__ int sm_bin_at(int place) { return place < kSmValues ? kSmValues - 1 - place : place; }
 constexpr int kSmZone = 2 * kSmValues;  // the place of what is nearer to zero than the window
 
+// Counts the values of a vector.
+__device__ __forceinline__ void sm_count(SmShared& sh, const SmWindow& win, const uint4& u) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  unsigned at[8];
+  int below = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) win.offsets<4>(w[i], at[2 * i], at[2 * i + 1], below);
+  if (below >= 0) {
+    // -inf, and what is too far below the maximum to weigh anything, add to the
+    // last negative bin, which no other logit is in
+#pragma unroll
+    for (int i = 0; i < 8; ++i) atomicAdd(reinterpret_cast<unsigned*>(reinterpret_cast<char*>(sh.values) + at[i]), 1u);
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t x = i < 2 ? u.x : i < 4 ? u.y : i < 6 ? u.z : u.w;
+      const unsigned b = i & 1 ? x >> 16 : x & 0xffffu;
+      const int place = win.place(b);
+      if (place >= 0) {
+        atomicAdd(&sh.values[win.bin(b, min(place, kSmValues - 1))], 1u);
+      } else {
+        const int k = atomicAdd(&sh.near, 1);
+        if (k < kSmNear) sh.near_of[k] = static_cast<unsigned short>(b);
+      }
+    }
+  }
+}
+__device__ __forceinline__ void sm_clear(SmShared& sh) {
+  for (int i = threadIdx.x; i < 2 * kSmValues / 4; i += kSmThreads)
+    reinterpret_cast<uint4*>(sh.values)[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (threadIdx.x == 0) sh.near = 0;
+  __syncthreads();
+}
+
 // The border of top_k (0: none) and top_p (1: none) among bf16 logits, into what
 // row keeps.  In order stand the positive values, the zone (what is nearer to zero
 // than the window), the negative ones; each CTA of the cluster has a share of the
-// bins.  Weights below 2^-64 count as 0.  All CTAs of the cluster call it and take
-// the same way through it; false: the border lies in the zone and has to be searched.
+// bins.  Weights below 2^-64 count as 0.  `counted`: sh.values holds the counts
+// already.  All CTAs of the cluster call it and take the same way through it; false:
+// the border lies in the zone and has to be searched.
 template <typename Slice>
 __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice& sl, SmRow& row, const SmWindow& win,
-                          int top_k, double top_p) {
+                          bool counted, int top_k, double top_p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int ranks = Slice::kAlone ? 1 : cl.num_blocks(), rank = Slice::kAlone ? 0 : cl.block_rank();
-  for (int i = tid; i < 2 * kSmValues / 4; i += kSmThreads) reinterpret_cast<uint4*>(sh.values)[i] = make_uint4(0u, 0u, 0u, 0u);
-  if (tid == 0) sh.near = 0;
-  __syncthreads();
-  sl.vectors(0, sl.vecs, tid, kSmThreads, [&](const uint4& u, int) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    unsigned at[8];
-    int below = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) win.offsets<4>(w[i], at[2 * i], at[2 * i + 1], below);
-    if (below >= 0) {
-      // -inf, and what is too far below the maximum to weigh anything, add to the
-      // last negative bin, which no other logit is in
-#pragma unroll
-      for (int i = 0; i < 8; ++i) atomicAdd(reinterpret_cast<unsigned*>(reinterpret_cast<char*>(sh.values) + at[i]), 1u);
-    } else {
-#pragma unroll 1
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t x = i < 2 ? u.x : i < 4 ? u.y : i < 6 ? u.z : u.w;
-        const unsigned b = i & 1 ? x >> 16 : x & 0xffffu;
-        const int place = win.place(b);
-        if (place >= 0) {
-          atomicAdd(&sh.values[win.bin(b, min(place, kSmValues - 1))], 1u);
-        } else {
-          const int k = atomicAdd(&sh.near, 1);
-          if (k < kSmNear) sh.near_of[k] = static_cast<unsigned short>(b);
-        }
-      }
-    }
-  });
+  if (!counted) {
+    sm_clear(sh);
+    sl.vectors(0, sl.vecs, tid, kSmThreads, [&](const uint4& u, int) { sm_count(sh, win, u); });
+  }
   __syncthreads();
   const int zones = sh.near;
   // (their sum is the same whatever order they were listed in: whole numbers of 2^-52)
@@ -757,71 +766,9 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
   const int ties = pk == pp ? min(sh.ties_of[0], sh.ties_of[1]) : sh.ties_of[i];
   const float edge = win.value(sm_bin_at(sh.place_of[i]));
   row.least = edge;
-  row.last_id = 0x7fffffff;
-  if (ties == sh.held_of[i]) return true;
-  // ---- equal logits at the border: the id of the last that is kept
-  const int per = (sl.vecs + kSmWarps - 1) / kSmWarps;
-  const int v_lo = min(sl.vecs, warp * per), v_hi = min(sl.vecs, v_lo + per);
-  auto equal = [&](const uint4& u) {
-    float x[8];
-    Slice::unpack(u, x);
-    int c = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c += x[i] == edge;
-    return c;
-  };
-  // two counts of 16 bits: a lane has at most 2^18 / 512 logits
-  const uint32_t edge2 = pack_bf16x2(edge, edge);
-  uint32_t pairs = 0;
-  sl.vectors(v_lo, v_hi, lane, 32, [&](const uint4& u, int) {
-    pairs += (equal_bf16x2(u.x, edge2) & 0x00010001u) + (equal_bf16x2(u.y, edge2) & 0x00010001u) +
-             (equal_bf16x2(u.z, edge2) & 0x00010001u) + (equal_bf16x2(u.w, edge2) & 0x00010001u);
-  });
-  const int own = __reduce_add_sync(0xffffffffu, static_cast<int>((pairs & 0xffffu) + (pairs >> 16)));
-  int c = own;
-  __syncthreads();
-  if (lane == 0) sh.warp_n[warp] = c;
-  __syncthreads();
-  if (warp == 0) {
-    c = __reduce_add_sync(0xffffffffu, lane < kSmWarps ? sh.warp_n[lane] : 0);
-    if (lane < ranks) cl.map_shared_rank(&sh, lane)->zones_of[rank] = c;
-  }
-  cl.sync();
-  int before = 0;
-  for (int r = 0; r < rank; ++r) before += sh.zones_of[r];
-  {  // how many of this warp's are kept
-    const int others = __reduce_add_sync(0xffffffffu, lane < warp ? sh.warp_n[lane] : 0);
-    row.ties = min(max(ties - before - others, 0), own);
-    row.cut = true;
-  }
-  if (before < ties && before + sh.zones_of[rank] >= ties) {  // in this CTA's slice
-    int from = 0;
-    while (before + sh.warp_n[from] < ties) before += sh.warp_n[from++];
-    // that warp's vectors, neighbours for each thread
-    const int most = (per + kSmThreads - 1) / kSmThreads;
-    const int first = min(sl.vecs, from * per) + most * tid, end = min(sl.vecs, from * per + per);
-    int mine = 0;
-    for (int v = first; v < min(end, first + most); ++v) mine += equal(sl.raw(v));
-    int sum_all;
-    const SmSums<int> sums = sm_scan(mine, sh.warp_n, sum_all);
-    const int need = ties - before;
-    if (mine > 0 && sums.before < need && need <= sums.upto) {
-      int left = need - sums.before, id = 0;
-      for (int v = first; v < min(end, first + most); ++v) {
-        float x[8];
-        Slice::unpack(sl.raw(v), x);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (x[i] == edge && left > 0) {
-            id = sl.id0 + v * 8 + i;
-            --left;
-          }
-      }
-      for (int r = 0; r < ranks; ++r) cl.map_shared_rank(&sh, r)->border = composite(edge, id);
-    }
-  }
-  cl.sync();
-  row.keep_to(sh.border);
+  row.cut = ties < sh.held_of[i];
+  row.ties = ties;
+  row.last_id = row.cut ? -0x7fffffff - 1 : 0x7fffffff;
   return true;
 }
 
@@ -901,12 +848,39 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
 
   // ---- the largest logit (a NaN comes through), and of bf16 the smallest
   float mx = -INFINITY, mn = INFINITY;
+  const bool by_k = top_k > 0 && top_k < p.V, by_p = top_p < 1.0;
+  SmWindow win{0};
+  bool counted = false;
   if constexpr (sizeof(T) == 2) {
     uint32_t high = 0xff80ff80u, low = 0x7f807f80u;
-    sl.vectors(0, sl.vecs, tid, kSmThreads, [&](const uint4& d, int) {  // what this thread copied
+    auto look = [&](const uint4& d) {
       high = max_nan_bf16x2(high, max_nan_bf16x2(max_nan_bf16x2(d.x, d.y), max_nan_bf16x2(d.z, d.w)));
       low = min_bf16x2(low, min_bf16x2(min_bf16x2(d.x, d.y), min_bf16x2(d.z, d.w)));
-    });
+    };
+    if (kWhole && (by_k || by_p) && temperature > 0.0 && top_k != 1) {
+      // counts in the same pass, for magnitudes up to four times what a sample shows;
+      // where that was too little they are counted again
+      const uint4 d = sl.raw(static_cast<int>(static_cast<long long>(sl.vecs) * tid / kSmThreads));
+      unsigned most = 0;
+      const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned a = w[i] & 0x7fffu, c = w[i] >> 16 & 0x7fffu;
+        most = max(most, max(a < 0x7f80u ? a : 0u, c < 0x7f80u ? c : 0u));
+      }
+      most = __reduce_max_sync(0xffffffffu, most);
+      if (lane == 0) sh.warp_n[warp] = static_cast<int>(most);
+      sm_clear(sh);
+      most = __reduce_max_sync(0xffffffffu, lane < kSmWarps ? static_cast<unsigned>(sh.warp_n[lane]) : 0u);
+      win.lo = max(0, min(static_cast<int>(most) + 256, 0x7f7f) - kSmValues + 1);
+      sl.vectors(0, sl.vecs, tid, kSmThreads, [&](const uint4& u, int) {
+        look(u);
+        sm_count(sh, win, u);
+      });
+      counted = true;
+    } else {
+      sl.vectors(0, sl.vecs, tid, kSmThreads, [&](const uint4& u, int) { look(u); });  // what this thread copied
+    }
     const float2 f = unpack_bf16x2(high), g = unpack_bf16x2(low);
     mx = max_nan(f.x, f.y);
     mn = fminf(g.x, g.y);
@@ -989,8 +963,6 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   row.bins = static_cast<float>(fmin(row.c * kSmBinsPerOctave, 1e30));
   row.min_weight = min_p > 0.0 ? fmin(min_p, 1.0) : 0.0;
   row.keep_all();
-  const bool by_k = top_k > 0 && top_k < p.V, by_p = top_p < 1.0;
-  SmWindow win{0};
   bool search = by_k || by_p, plain = true;  // plain: the table holds all weights but the zone's
   if constexpr (sizeof(T) == 2) {
     // magnitudes up to beyond the largest of a negative logit that weighs 2^-64 or
@@ -999,8 +971,11 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     const int top = static_cast<int>((__float_as_uint(mx) & 0x7fffffffu) >> 16);
     const int down = low < 0.f ? static_cast<int>((__float_as_uint(low) & 0x7fffffffu) >> 16) + 1 : 0;
     plain = down <= 0x7f7f && 64.0 / row.c < 1e38;
-    win.lo = max(0, min(max(top, down), 0x7f7f) - kSmValues + 1);
-    if (search && plain && sm_values(cl, sh, sl, row, win, by_k ? static_cast<int>(top_k) : 0, top_p)) search = false;
+    const int hi = min(max(top, down), 0x7f7f);
+    counted = counted && hi <= win.lo + kSmValues - 1;
+    if (!counted) win.lo = max(0, hi - kSmValues + 1);
+    if (search && plain && sm_values(cl, sh, sl, row, win, counted, by_k ? static_cast<int>(top_k) : 0, top_p))
+      search = false;
   }
   if (search) {
     row.keep_all();
@@ -1030,7 +1005,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     for (int i = tid; i < 2 * kSmValues; i += kSmThreads) {  // (a warp's bins are neighbours: mostly all or none)
       const float x = win.value(i);
       u64 w = 0;
-      if (x >= row.least && x <= mx && i != 2 * kSmValues - 1) w = sm_fixed(pow2_by(sh.powers, row.exponent(x)), row.min_weight);
+      if (x >= row.least && x <= mx && i != 2 * kSmValues - 1 && !(row.cut && x == row.least)) w = sm_fixed(pow2_by(sh.powers, row.exponent(x)), row.min_weight);
       sh.weights[i] = w;
     }
     __syncthreads();
@@ -1055,7 +1030,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
       for (int i = 0; i < 4; ++i) win.offsets<8>(x[i], at[2 * i], at[2 * i + 1], below);
       const int id = sl.id0 + v * VE;
       bool ties = false;  // cut within this vector
-      if (id + VE - 1 > row.last_id && row.least > -INFINITY) {  // behind the last equal logit that is kept, if not before its vector's end
+      if (!row.cut && id + VE - 1 > row.last_id && row.least > -INFINITY) {  // behind the last equal logit that is kept, if not before its vector's end
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -1080,82 +1055,110 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   const int per = (sl.vecs + kSmWarps - 1) / kSmWarps;
   const int v_lo = min(sl.vecs, warp * per), v_hi = min(sl.vecs, v_lo + per);
   u64 sum = 0;
+  // equal logits that are cut weigh nothing there and are counted (two counts of 16
+  // bits: a lane has at most 2^18 / 512 of a row)
+  const u64 edge = row.cut ? sm_fixed(pow2_by(sh.powers, row.exponent(row.least)), row.min_weight) : 0ull;
+  uint32_t pairs = 0;
+  auto equal = [&](const uint4& d) {
+    return (equal_bf16x2(d.x, edge2) & 0x00010001u) + (equal_bf16x2(d.y, edge2) & 0x00010001u) +
+           (equal_bf16x2(d.z, edge2) & 0x00010001u) + (equal_bf16x2(d.w, edge2) & 0x00010001u);
+  };
   const int edge_place = win.place(__float_as_uint(row.least) >> 16);
   if (sizeof(T) == 2 && plain && row.least > 0.f && edge_place > 0 && (row.cut || row.last_id == 0x7fffffff)) {
     // only positive logits of the window are kept: as signed numbers, what is below
     // them reads the one bin before the border's, which holds 0, so lanes that keep
-    // nothing share an access; equal logits that are cut are counted already
-    if (row.cut) {
-      __syncthreads();
-      if (tid == 0) {
-        const u64 w = sh.weights[edge_place];
-        sh.weights[edge_place] = 0;
-        sh.edge = w;
-      }
-      __syncthreads();
-    }
+    // nothing share an access
     const int low = (win.lo + edge_place - 1) * 8;
     const char* const table = reinterpret_cast<const char*>(sh.weights) - win.lo * 8;
     u64 odd = 0;
     sl.vectors(v_lo, v_hi, lane, 32, [&](const uint4& d, int) {
       const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+      if (row.cut) pairs += equal(d);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         sum += *reinterpret_cast<const u64*>(table + max(static_cast<int>(w[i] << 16) >> 13, low));
         odd += *reinterpret_cast<const u64*>(table + max(static_cast<int>(w[i]) >> 13 & ~7, low));
       }
     });
-    sum = sm_sum(sum + odd);
-    if (row.cut) {
-      sum += sh.edge * static_cast<u64>(row.ties);
-      __syncthreads();
-      if (tid == 0) sh.weights[edge_place] = sh.edge;
-    }
+    sum += odd;
   } else {
-    sl.vectors(v_lo, v_hi, lane, 32, [&](const uint4& d, int v) { sum += sum_of(d, v); });
-    sum = sm_sum(sum);
+    sl.vectors(v_lo, v_hi, lane, 32, [&](const uint4& d, int v) {
+      sum += sum_of(d, v);
+      if (sizeof(T) == 2 && row.cut) pairs += equal(d);
+    });
   }
+  sum = sm_sum(sum);
+  int ties = __reduce_add_sync(0xffffffffu, static_cast<int>((pairs & 0xffffu) + (pairs >> 16)));
   __syncthreads();
-  if (lane == 0) sh.warp_lo[warp] = sum;
+  if (lane == 0) {
+    sh.warp_lo[warp] = sum;
+    sh.warp_n[warp] = ties;
+  }
   __syncthreads();
   if (warp == 0) {
     const u64 all = sm_sum(lane < kSmWarps ? sh.warp_lo[lane] : 0ull);
-    if (lane < ranks) cl.map_shared_rank(&sh, lane)->sum_of[rank] = all;
+    ties = __reduce_add_sync(0xffffffffu, lane < kSmWarps ? sh.warp_n[lane] : 0);
+    if (lane < ranks) {
+      SmShared& o = *cl.map_shared_rank(&sh, lane);
+      o.sum_of[rank] = all;
+      o.zones_of[rank] = ties;
+    }
   }
   cl.sync();
 
   // ---- the CTA, the warp and the token where the running sum passes u S; outside
   // of [0, 1) there may be none: the last that is kept
+  int left = row.cut ? row.ties : 0;  // equal logits that are still to come
+  auto with_ties = [&](u64 sum, int n) {  // a part's sum, of the n equal logits in it those that are kept
+    const int k = min(n, left);
+    left -= k;
+    return sum + edge * static_cast<u64>(k);
+  };
   u64 whole = 0;
-  for (int q = 0; q < ranks; ++q) whole += sh.sum_of[q];
+  for (int q = 0; q < ranks; ++q) whole += with_ties(sh.sum_of[q], sh.zones_of[q]);
   const double part = u * static_cast<double>(whole);
   const u64 goal = part >= static_cast<double>(whole) || part != part ? whole : part > 0.0 ? static_cast<u64>(part) : 0ull;
-  u64 before = 0, at = 0;
-  int here = -1;
-  for (int q = 0; q < ranks; ++q) {
-    if (sh.sum_of[q] > 0) {
-      here = q;
-      before = at;
-      if (at + sh.sum_of[q] > goal) break;
+  u64 before = 0;
+  int here = -1, left_here = 0;
+  auto pick = [&](int n, const u64* sums, const int* counts) {  // the first part that passes, or the last that holds any
+    u64 at = before;
+    here = -1;
+    for (int q = 0; q < n; ++q) {
+      const int had = left;
+      const u64 s = with_ties(sums[q], counts[q]);
+      if (s > 0) {
+        here = q;
+        before = at;
+        left_here = had;
+        if (at + s > goal) break;
+      }
+      at += s;
     }
-    at += sh.sum_of[q];
-  }
+    left = left_here;
+  };
+  left = row.cut ? row.ties : 0;
+  pick(ranks, sh.sum_of, sh.zones_of);
   if (here != rank) return;
-  at = before;
-  here = -1;
-  for (int w = 0; w < kSmWarps; ++w) {
-    if (sh.warp_lo[w] > 0) {
-      here = w;
-      before = at;
-      if (at + sh.warp_lo[w] > goal) break;
-    }
-    at += sh.warp_lo[w];
-  }
+  pick(kSmWarps, sh.warp_lo, sh.warp_n);
   // that warp's vectors, neighbours for each thread
   const int most = (per + kSmThreads - 1) / kSmThreads;
   const int first = min(sl.vecs, here * per) + most * tid, end = min(sl.vecs, here * per + per);
   u64 mine = 0;
-  for (int v = first; v < min(end, first + most); ++v) mine += sum_of(sl.raw(v), v);
+  int own = 0;
+  for (int v = first; v < min(end, first + most); ++v) {
+    const uint4 d = sl.raw(v);
+    mine += sum_of(d, v);
+    if (sizeof(T) == 2 && row.cut) {
+      const uint32_t c = equal(d);
+      own += static_cast<int>((c & 0xffffu) + (c >> 16));
+    }
+  }
+  if (row.cut) {
+    int none;
+    const SmSums<int> counts = sm_scan(own, sh.warp_n, none);
+    left = max(0, left - counts.before);
+    mine += edge * static_cast<u64>(min(own, left));
+  }
   u64 all;
   const SmSums<u64> sums = sm_scan(mine, sh.warp_hi, all);
   if (tid == 0) {
@@ -1182,7 +1185,11 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
 #pragma unroll
         for (int j = 1; j < VE; ++j) y = i == j ? e[j] : y;
         const int id = sl.id0 + v * VE + i;
-        const u64 w = row.keeps(y, id) ? sm_fixed(pow2_by(sh.powers, row.exponent(y)), row.min_weight) : 0ull;
+        u64 w = row.keeps(y, id) ? sm_fixed(pow2_by(sh.powers, row.exponent(y)), row.min_weight) : 0ull;
+        if (row.cut && y == row.least && left > 0) {
+          w = edge;
+          --left;
+        }
         // the first that passes, or the last
         if (w > 0 && (token < 0 || !passed || s <= goal)) {
           token = id;

@@ -161,6 +161,32 @@ def test_masked_and_broken_rows(dtype):
         assert tok[0] == 3000 and tok[1] == tok[2] == tok[3] == -1
 
 
+def test_rows_whose_sample_misses_what_matters():
+    """Whole rows are counted with a window that a sample of them suggests: largest and smallest
+    logits far outside of it, all zeros but a few, all tiny, many near zero."""
+    rows, vocab = 150, 20011
+    x, u = logits_of(rows, vocab, 21)
+    x[0:30, 777] = 300.0
+    x[30:60, 15001] = -3000.0
+    x[60:90] *= 2.0 ** -60
+    x[90:100] = 0.0
+    x[90:100, ::100] = torch.randn(10, 201, generator=torch.Generator().manual_seed(1)).bfloat16()
+    x[100:110, 1::2] *= 2.0 ** -20
+    x[110:120] = -x[110:120].abs() - 4
+    x[120:130, 5] = -0.0
+    x[130:140] = torch.where(torch.arange(vocab) % 3 == 0, -0.0, 0.0).bfloat16()
+    x, u = x.cuda(), u.cuda()
+    for s in (dict(temperature=0.9, top_p=0.9), dict(top_k=3000), dict(temperature=200.0, top_p=0.6, top_k=15000),
+              dict(temperature=3.0, top_p=0.999), dict(top_k=7, top_p=0.5)):
+        tok, lp = ops.sample_tokens(x, u, **s)
+        for i in [*range(0, rows, 6), 90, 91, 130, 131]:
+            want, want_lp, margin = drawn(x[i].cpu(), u[i].item(), s.get("temperature", 1.0), s.get("top_k", 0),
+                                          s.get("top_p", 1.0))
+            if margin > 2 ** -31:
+                assert int(tok[i]) == want, (s, i)
+                assert abs(float(lp[i]) - want_lp) <= 2 ** -24 * abs(want_lp) + vocab * 2 ** -45 + 1e-12
+
+
 def test_settings_per_row():
     g = torch.Generator().manual_seed(3)
     x, u = logits_of(64, 5003, 12)

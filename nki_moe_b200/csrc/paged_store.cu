@@ -92,15 +92,29 @@ __global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_stor
   }
   wtab[threadIdx.x >> 7][threadIdx.x & 127] = head_wload(threadIdx.x < D ? p.qw : p.kw, p.w_dtype, threadIdx.x & 127);
   __syncthreads();
-  if (t >= p.T || t >= p.cu[p.B]) return;  // behind the last sequence
-  const int b = sequence_of(p.cu, p.B, static_cast<int>(t), lane);
-  const int start = p.cu[b], end = p.cu[b + 1];
-  const int place = p.kv_lens[b] - end + static_cast<int>(t);
+  if (t >= p.T) return;
+  int b, start, end, kv;
+  if (kTree && p.B <= 32) {  // a step's sequences: one look at all of them, a chain of loads less
+    const int c = lane < p.B ? p.cu[lane] : 0, next = lane < p.B ? p.cu[lane + 1] : 0, len = lane < p.B ? p.kv_lens[lane] : 0;
+    if (t >= __shfl_sync(0xffffffffu, next, p.B - 1)) return;  // behind the last sequence
+    b = 31 - __clz(__ballot_sync(0xffffffffu, lane == 0 || (lane < p.B && c <= t)));
+    start = __shfl_sync(0xffffffffu, c, b);
+    end = __shfl_sync(0xffffffffu, next, b);
+    kv = __shfl_sync(0xffffffffu, len, b);
+  } else {
+    if (t >= p.cu[p.B]) return;  // behind the last sequence
+    b = sequence_of(p.cu, p.B, static_cast<int>(t), lane);
+    start = p.cu[b];
+    end = p.cu[b + 1];
+    kv = p.kv_lens[b];
+  }
+  const int place = kv - end + static_cast<int>(t);
   const int slot = place >> p.c.page_shift;
   if (t < start || t >= end || place < 0 || slot >= p.c.max_pages) {
     if (lane == 0) atomicOr(p.status, kDevErrBadIndex);
     return;
   }
+  const int page = p.c.table[b * p.c.table_stride + slot];
   int pos = place;
   if constexpr (kTree) {
     const int n = end - start, i = static_cast<int>(t) - start;
@@ -112,7 +126,6 @@ __global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_stor
     pos = line.pos;
     if (lane == 0 && warp % kWarps == 0) p.tree.rows[t] = line;
   }
-  const int page = p.c.table[b * p.c.table_stride + slot];
   const bool held = page >= 0 && page < p.c.num_pages;
   if (!held && page != -1 && lane == 0) atomicOr(p.status, kDevErrBadIndex);
   tab[warp][lane] = rope_cos_sin(p.turns.f[lane], pos);

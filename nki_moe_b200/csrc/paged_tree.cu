@@ -42,8 +42,9 @@ namespace {
 
 constexpr int kTrThreads = 384;
 constexpr int kTrK = 3, kTrV = 2;  // stages of 32 KB: K blocks, V blocks
-constexpr int kTrItem = 2;         // key blocks that beginning and ending an item (sequence, kv head, tile) costs
-constexpr int kTrMinRun = 3;       // places of a CTA's run at least: a block for each warpgroup
+constexpr int kTrItem = 2;         // key blocks that beginning and ending an item (sequence, kv head, tile) costs:
+                                   // 40 ragged sequences 114 us at 0, 80 at 1, 71 at 2, 72 at 3, 73 at 4
+constexpr int kTrMinRun = 3;       // places of a CTA's run at least
 // A part of a cut item: o four columns at a time [32][128 rows][4], then the
 // rows' m, then their l (a warp's rows are neighbours: coalesced)
 constexpr int kTrPart = (kHeadDim + 2) * kPfRows;
@@ -124,8 +125,11 @@ __device__ __forceinline__ TrSeq tr_sequence(const TrParams& p, int b, bool flag
 }
 
 // The run of one CTA through the list of blocks (sequence, kv head, tile, block),
-// each item preceded by kTrItem places for its own cost; a warp walks it.
+// each item preceded by places for its own cost; a warp walks it.  Where two blocks
+// a CTA are enough for all, items begin at even places instead, so that no CTA
+// has a block each of two items.
 struct TrRun {
+  bool pairs;
   int share, run_lo, run_hi;
   int at;    // place in the list
   int base;  // place of the first of sequence b
@@ -133,8 +137,12 @@ struct TrRun {
   TrSeq mine;  // of sequence 32 * (b / 32) + lane
 
   __device__ __forceinline__ int tiles(const TrParams& p, const TrSeq& s) const { return (s.n + p.tpt - 1) / p.tpt; }
+  __device__ __forceinline__ int cost() const { return pairs ? 0 : kTrItem; }
+  __device__ __forceinline__ int span(const TrSeq& s) const {  // places of an item
+    return pairs ? (s.blocks + 1) & ~1 : s.blocks + kTrItem;
+  }
   __device__ __forceinline__ int places(const TrParams& p, const TrSeq& s) const {
-    return tiles(p, s) * p.c.nkv * (s.blocks + kTrItem);
+    return tiles(p, s) * p.c.nkv * span(s);
   }
   __device__ __forceinline__ TrSeq of(int b) const {
     const int l = b & 31;
@@ -143,12 +151,18 @@ struct TrRun {
   }
 
   __device__ __forceinline__ void begin(const TrParams& p, int lane) {
-    int total = 0;
+    int total = 0, even = 0;
     for (int c = 0; c < p.B; c += 32) {
       mine = tr_sequence(p, c + lane, blockIdx.x == 0);
+      pairs = true;
+      even += __reduce_add_sync(0xffffffffu, places(p, mine));
+      pairs = false;
       total += __reduce_add_sync(0xffffffffu, places(p, mine));
     }
-    share = max(kTrMinRun, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+    const int ctas = gridDim.x;
+    pairs = even <= 2 * ctas;
+    if (pairs) total = even;
+    share = pairs ? 2 : max(kTrMinRun, (total + ctas - 1) / ctas);
     run_lo = min(total, static_cast<int>(blockIdx.x) * share);
     run_hi = min(total, run_lo + share);
     at = run_lo;
@@ -188,12 +202,12 @@ struct TrRun {
       s = of(b);
     }
     const int n = s.blocks, tls = tiles(p, s);
-    const int q = (at - base) / (n + kTrItem);
-    const int item = base + q * (n + kTrItem) + kTrItem;  // the list's first block of the item
+    const int q = (at - base) / span(s);
+    const int item = base + q * span(s) + cost();  // the list's first block of the item
     const int tile = q % tls;
     w.lo = max(at - item, 0);
     w.hi = min(n, run_hi - item);
-    at = item + n;
+    at = base + (q + 1) * span(s);
     if (w.hi <= 0) return TrWork{};  // the run ends before the item's blocks
     w.row0 = s.row0 + tile * p.tpt;
     w.tokens = min(p.tpt, s.n - tile * p.tpt);
@@ -666,14 +680,13 @@ __global__ void __launch_bounds__(kTrThreads, 1)
 }
 
 // Joins the parts of a cut item, in order: a CTA per (item, 8 rows), a thread per
-// row and four columns, eight parts in flight once their factors are known.
-// (One sequence over all SMs, 37 parts each: 8.4 us with a running maximum over
-// the parts; with a few CTAs that take slices in turn the ragged batch takes 6 us
-// more.)
+// row and four columns, 13 parts in flight.  (With a few CTAs that take slices in
+// turn the ragged batch takes 6 us more.)
 __global__ void __launch_bounds__(32 * kTrJoinRows) paged_tree_join_kernel(const __grid_constant__ TrParams p) {
-  constexpr int kSlices = kPfRows / kTrJoinRows, kAhead = 8, kFew = 4;
+  constexpr int kSlices = kPfRows / kTrJoinRows, kAhead = 13, kFew = 4;
   extern __shared__ float2 factor[];  // [parts][rows]: maximum and sum, then the weight and the sum's share
   __shared__ float whole[kTrJoinRows];
+  __shared__ unsigned most[kTrJoinRows];
   const int cta = blockIdx.x / kSlices, row0 = (blockIdx.x % kSlices) * kTrJoinRows;
   const int r = threadIdx.x % kTrJoinRows, col4 = threadIdx.x / kTrJoinRows, row = row0 + r;
   pdl_launch_dependents();
@@ -714,10 +727,7 @@ __global__ void __launch_bounds__(32 * kTrJoinRows) paged_tree_join_kernel(const
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
     return;
   }
-  for (int s = col4; s < sp.parts; s += 32) {
-    const float* from = part_of(s) + kHeadDim * kPfRows + row;
-    factor[s * kTrJoinRows + r] = make_float2(__ldcg(from), __ldcg(from + kPfRows));
-  }
+  if (threadIdx.x < kTrJoinRows) most[threadIdx.x] = 0u;
   // the first parts, long before their factors are known
   float4 v[kAhead];
   auto load = [&](int s0) {
@@ -727,15 +737,19 @@ __global__ void __launch_bounds__(32 * kTrJoinRows) paged_tree_join_kernel(const
   };
   load(0);
   __syncthreads();
-  if (col4 == 0) {
-    float m = -INFINITY, l = 0.f;
-    for (int s = 0; s < sp.parts; ++s) m = fmaxf(m, factor[s * kTrJoinRows + r].x);
-    for (int s = 0; s < sp.parts; ++s) {
-      float2& f = factor[s * kTrJoinRows + r];
-      f.x = f.x == -INFINITY ? 0.f : exp2f(f.x - m);
-      l = fmaf(f.x, f.y, l);
-    }
-    whole[r] = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+  for (int s = col4; s < sp.parts; s += 32) {
+    const float* from = part_of(s) + kHeadDim * kPfRows + row;
+    const float2 ml = make_float2(__ldcg(from), __ldcg(from + kPfRows));
+    factor[s * kTrJoinRows + r] = ml;
+    const unsigned b = __float_as_uint(ml.x);  // integers that rise as the maxima do
+    atomicMax(&most[r], b & 0x80000000u ? ~b : b | 0x80000000u);
+  }
+  __syncthreads();
+  const float m = __uint_as_float(most[r] & 0x80000000u ? most[r] & 0x7fffffffu : ~most[r]);
+  for (int s = col4; s < sp.parts; s += 32) {
+    float2& f = factor[s * kTrJoinRows + r];
+    f.x = f.x == -INFINITY ? 0.f : exp2f(f.x - m);
+    f.y *= f.x;
   }
   __syncthreads();
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -751,6 +765,12 @@ __global__ void __launch_bounds__(32 * kTrJoinRows) paged_tree_join_kernel(const
       o.w = fmaf(f, v[e].w, o.w);
     }
   }
+  if (col4 == 0) {
+    float l = 0.f;
+    for (int s = 0; s < sp.parts; ++s) l += factor[s * kTrJoinRows + r].y;
+    whole[r] = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+  }
+  __syncthreads();
   if (token >= sp.tokens) return;
   const float inv = whole[r];
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
@@ -767,8 +787,8 @@ TrLayout tr_layout(long long T, long long B, int nq, int nkv, long long max_page
   const int tpt = kPfRows / (nq / nkv);
   const long long tiles = T / tpt + (B < T ? B : T);
   const long long blocks = (max_pages * page_size + kPfBlock - 1) / kPfBlock;
-  // places at most, and so runs at most
-  const long long most = (tiles * nkv * (blocks + 1 + kTrItem) + kTrMinRun - 1) / kTrMinRun;
+  // pairs of blocks at most
+  const long long most = tiles * nkv * ((blocks + 2) / 2);
   L.grid = device_sm_count();
   if (most < L.grid) L.grid = most;
   auto round = [](size_t n) { return (n + 255) & ~static_cast<size_t>(255); };

@@ -591,12 +591,12 @@ def paged_tree_attention(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: to
     if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != row or not qkv.is_contiguous():
         raise ValueError(f"qkv must be a contiguous bf16 [T, {row}] tensor")
     T, dev = qkv.shape[0], qkv.device
-    _node_ids(parents, "parents", torch.int32, T)
+    _node_ids(parents, "parents", torch.int32, T, dev.index)
     B = _lengths(cu_seqlens, kv_lens)
     qw, kw, wdt = _norm_weights(q_weight, k_weight)
     cache = _paged_cache(k_pages, v_pages, page_table, n_kv_heads, B)
-    _same_device(dev.index, "q_weight k_weight parents cu_seqlens kv_lens k_pages v_pages page_table", qw, kw, parents,
-                 cu_seqlens, kv_lens, k_pages, v_pages, page_table)
+    _same_device(dev.index, "q_weight k_weight cu_seqlens kv_lens k_pages v_pages page_table", qw, kw, cu_seqlens,
+                 kv_lens, k_pages, v_pages, page_table)
     out = _rows_out(out, (T, n_heads * 128), qkv)
     s = _raw_stream(dev.index)
     nbytes = _paged_ws_bytes(dev.index, "nkimoe_paged_tree_attention_workspace_bytes", T, B, n_heads, n_kv_heads,
@@ -720,30 +720,31 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
     or with a negative or NaN temperature, has no distribution and gives -1 and
     NaN."""
     _cuda(logits, "logits")
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
+    shape, dt, udt, dev = logits.shape, logits.dtype, uniforms.dtype, logits.get_device()
+    if len(shape) != 2 or (dt != torch.bfloat16 and dt != torch.float32):
         raise ValueError("logits must be fp32 or bf16 [T, V]")
-    T, V = logits.shape
-    if V == 0 or (V > 1 and logits.stride(1) != 1):
+    T, V = shape
+    row, step = logits.stride()
+    if V == 0 or (V > 1 and step != 1):
         raise ValueError("logits must have contiguous, non-empty rows")
-    dev = logits.get_device()
-    if not uniforms.is_cuda or uniforms.dtype not in (torch.float32, torch.float64) or uniforms.shape != (T,) \
+    if uniforms.get_device() != dev or (udt != torch.float32 and udt != torch.float64) or uniforms.shape != (T,) \
             or not uniforms.is_contiguous():
-        raise ValueError(f"uniforms must be a contiguous CUDA fp32 or fp64 [{T}] tensor")
-    _same_device(dev, "uniforms", uniforms)
-    settings = (*_setting(temperature, "temperature", torch.float32, T, dev),
-                *_setting(top_k, "top_k", torch.int32, T, dev), *_setting(top_p, "top_p", torch.float32, T, dev),
-                *_setting(min_p, "min_p", torch.float32, T, dev))
-    tokens = torch.empty(T, dtype=torch.int64, device=logits.device)
-    lp = torch.empty(T, dtype=torch.float32, device=logits.device)
-    call("nkimoe_sample_tokens", logits.data_ptr(), _DT[logits.dtype], logits.stride(0) if T > 1 else V,
-         uniforms.data_ptr(), F32 if uniforms.dtype == torch.float32 else F64, *settings, T, V, tokens.data_ptr(),
-         lp.data_ptr(), _raw_stream(dev))
+        raise ValueError(f"uniforms must be a contiguous fp32 or fp64 [{T}] tensor on cuda:{dev}")
+    t_rows, t_all = _setting(temperature, "temperature", torch.float32, T, dev)
+    k_rows, k_all = _setting(top_k, "top_k", torch.int32, T, dev)
+    p_rows, p_all = _setting(top_p, "top_p", torch.float32, T, dev)
+    m_rows, m_all = _setting(min_p, "min_p", torch.float32, T, dev)
+    tokens = uniforms.new_empty((T,), dtype=torch.int64)
+    lp = torch.empty_like(uniforms) if udt == torch.float32 else uniforms.new_empty((T,), dtype=torch.float32)
+    call("nkimoe_sample_tokens", logits.data_ptr(), _DT[dt], row if T > 1 else V, uniforms.data_ptr(),
+         F32 if udt == torch.float32 else F64, t_rows, t_all, k_rows, k_all, p_rows, p_all, m_rows, m_all, T, V,
+         tokens.data_ptr(), lp.data_ptr(), _raw_stream(dev))
     return tokens, lp
 
 
-def _node_ids(t: torch.Tensor, name: str, dtype: torch.dtype, T: int) -> None:
-    if not t.is_cuda or t.dtype != dtype or t.shape != (T,) or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous CUDA {dtype} [{T}] tensor")
+def _node_ids(t: torch.Tensor, name: str, dtype: torch.dtype, T: int, dev: int) -> None:
+    if t.get_device() != dev or t.dtype != dtype or t.shape != (T,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} [{T}] tensor on cuda:{dev}")
 
 
 @_on_its_device
@@ -763,33 +764,31 @@ def accept_drafts(tokens: torch.Tensor, sampled: torch.Tensor, parents: torch.Te
     places right behind what the cache held before, so that the sequence goes on
     from ``kv_len - n + counts[b]`` positions."""
     _cuda(tokens, "tokens")
-    T, dev = tokens.numel(), tokens.device
-    _node_ids(tokens, "tokens", torch.int64, T)
-    _node_ids(sampled, "sampled", torch.int64, T)
-    _node_ids(parents, "parents", torch.int32, T)
-    B = _lengths(cu_seqlens, kv_lens)
-    shape = pages.shape
-    if not pages.is_cuda or len(shape) < 4 or not pages.is_contiguous() or pages.numel() == 0:
-        raise ValueError("pages must be contiguous CUDA [..., pages, n_kv_heads, page_size, head_dim]")
-    if not page_table.is_cuda or page_table.dtype != torch.int32 or page_table.dim() != 2:
-        raise ValueError("page_table must be CUDA int32 [sequences, pages per sequence]")
-    rows, width = page_table.shape
-    if rows < B or width == 0 or (width > 1 and page_table.stride(1) != 1):
+    T, dev = tokens.numel(), tokens.get_device()
+    _node_ids(tokens, "tokens", torch.int64, T, dev)
+    _node_ids(sampled, "sampled", torch.int64, T, dev)
+    _node_ids(parents, "parents", torch.int32, T, dev)
+    B, width, shape = _lengths(cu_seqlens, kv_lens), page_table.shape, pages.shape
+    if pages.get_device() != dev or len(shape) < 4 or not pages.is_contiguous() or 0 in shape:
+        raise ValueError(f"pages must be contiguous [..., pages, n_kv_heads, page_size, head_dim] on cuda:{dev}")
+    if page_table.get_device() != dev or page_table.dtype != torch.int32 or len(width) != 2:
+        raise ValueError(f"page_table must be int32 [sequences, pages per sequence] on cuda:{dev}")
+    rows, width = width
+    row_step, step = page_table.stride()
+    if rows < B or width == 0 or (width > 1 and step != 1):
         raise ValueError(f"page_table must have contiguous rows for {B} sequences")
-    _same_device(dev.index, "sampled parents cu_seqlens kv_lens pages page_table", sampled, parents, cu_seqlens, kv_lens,
-                 pages, page_table)
-    counts = torch.empty(B, dtype=torch.int32, device=dev)
-    path = torch.empty(T, dtype=torch.int32, device=dev)
-    new = torch.empty(T, dtype=torch.int64, device=dev)
+    if cu_seqlens.get_device() != dev or kv_lens.get_device() != dev:
+        raise ValueError(f"cu_seqlens and kv_lens must be on cuda:{dev}")
+    counts, path, new = torch.empty_like(kv_lens), torch.empty_like(parents), torch.empty_like(tokens)
     if B == 0 or T == 0:
         return counts.zero_(), path.fill_(-1), new.fill_(-1)
-    s = _raw_stream(dev.index)
-    ws = _paged_workspace(dev, s, 0)
+    s = _raw_stream(dev)
+    ws = _paged_workspace(tokens.device, s, 0)
+    n_pages, heads, size, dim = shape[-4:]
     call("nkimoe_accept_drafts", tokens.data_ptr(), sampled.data_ptr(), parents.data_ptr(), cu_seqlens.data_ptr(),
-         kv_lens.data_ptr(), pages.data_ptr(), pages.numel() // (shape[-1] * shape[-2] * shape[-3] * shape[-4]),
-         shape[-4], shape[-3], shape[-2], shape[-1] * pages.element_size(), page_table.data_ptr(),
-         page_table.stride(0) if rows > 1 else width, width, counts.data_ptr(), path.data_ptr(), new.data_ptr(), T, B,
-         ws.data_ptr(), s)
+         kv_lens.data_ptr(), pages.data_ptr(), pages.numel() // (n_pages * heads * size * dim), n_pages, heads, size,
+         dim * pages.element_size(), page_table.data_ptr(), row_step if rows > 1 else width, width, counts.data_ptr(),
+         path.data_ptr(), new.data_ptr(), T, B, ws.data_ptr(), s)
     if "NKIMOE_SYNC_CHECK" in os.environ and sync_check_enabled():
         read_status(ws)
     return counts, path, new

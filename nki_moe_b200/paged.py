@@ -146,6 +146,10 @@ class PageTables:
                 s.pages.append(self._take())
         return copies
 
+    def alone(self, seq: int, start: int) -> bool:
+        """Whether ``seq`` shares none of its pages from position ``start`` on."""
+        return all(p < 0 or self._refs[p] == 1 for p in self._seq(seq).pages[start // self.page_size:])
+
     def take_back(self, seqs, lengths) -> None:
         """Puts ``seqs[i]`` back to ``lengths[i]`` positions, as it had before an
         :meth:`extend` whose positions were not written after all.  The pages

@@ -86,7 +86,6 @@ class DraftStep:
     parents: torch.Tensor
     cu_seqlens: torch.Tensor
     kv_lens: torch.Tensor
-    table: torch.Tensor
 
 
 @dataclass
@@ -577,7 +576,8 @@ class Qwen3MoEStack:
         of its parent, below its own, -1 for the first; None: each follows the one
         before).  Returns the logits after every node ``[sum of nodes, V]``, packed,
         and the step, which :meth:`accept_paged` ends: until then the sequences
-        hold all nodes.  Where the call fails, they keep their lengths."""
+        hold all nodes and are not forked.  Where the call fails, they keep their
+        lengths."""
         if any(lyr.ep is not None for lyr in self.layers):
             raise ValueError("drafted tokens are for stacks on one GPU: ranks would take different numbers of steps")
         seqs, c = list(seqs), self.cfg
@@ -600,15 +600,15 @@ class Qwen3MoEStack:
                              torch.cat([t.reshape(-1).to(self.device, torch.int64) for t in tokens]),
                              torch.tensor([x for p in parents for x in p], dtype=torch.int32).to(self.device),
                              cu.to(self.device),
-                             torch.tensor([n + m for n, m in zip(lengths, nodes)], dtype=torch.int32).to(self.device),
-                             cache.table(seqs).to(self.device))
+                             torch.tensor([n + m for n, m in zip(lengths, nodes)], dtype=torch.int32).to(self.device))
+            table = cache.table(seqs).to(self.device)
             T = step.tokens.numel()
             linear = ops.skinny_linear if T <= 16 and self._skinny_ok else F.linear
 
             def attention(li, lyr, xn):
                 k, v = cache.layer(li)
                 return ops.paged_tree_attention(linear(xn, lyr.qkv_w), lyr.q_norm, lyr.k_norm, step.parents,
-                                                step.cu_seqlens, step.kv_lens, k, v, step.table, c.num_attention_heads,
+                                                step.cu_seqlens, step.kv_lens, k, v, table, c.num_attention_heads,
                                                 c.num_key_value_heads, c.rope_theta, c.rms_norm_eps,
                                                 window=cache.window, sinks=cache.sinks)
 
@@ -625,8 +625,10 @@ class Qwen3MoEStack:
         in the cache yet."""
         if any(q not in cache or cache.length(q) != n + m for q, n, m in zip(step.seqs, step.lengths, step.nodes)):
             raise ValueError("the sequences are not as the step left them")
+        if not all(cache.alone(q, n) for q, n in zip(step.seqs, step.lengths)):
+            raise ValueError("a sequence was forked between its step and the step's end")
         counts, path, _ = ops.accept_drafts(step.tokens, sampled, step.parents, step.cu_seqlens, step.kv_lens, cache.pool,
-                                            step.table)
+                                            cache.table(step.seqs).to(self.device))
         counts = counts.tolist()
         cache.take_back(step.seqs, [n + k for n, k in zip(step.lengths, counts)])
         for q in step.seqs:

@@ -9,6 +9,7 @@ import torch
 
 from nki_moe_b200 import _lib, ops
 from nki_moe_b200.drafts import LookupDrafts
+from nki_moe_b200.paged import PageTables
 
 
 def paths(tokens, parents):
@@ -47,6 +48,17 @@ def test_every_path_has_followed_the_text_before(seed):
             assert any(text[i:i + len(whole)] == whole for i in range(len(text) - len(path)))
         if text[-1] in text[:-1]:
             assert tokens
+
+
+def test_sequences_know_which_pages_are_their_own():
+    t = PageTables(10, 16, 6)
+    a = t.add()
+    t.extend([a], [40])
+    assert t.alone(a, 0)
+    b = t.fork(a)
+    assert not t.alone(a, 0) and not t.alone(a, 39) and t.alone(a, 48)
+    t.extend([a], [4])  # the last page becomes its own
+    assert t.alone(a, 40) and t.alone(b, 40) and not t.alone(b, 16)
 
 
 def refused(name, *args):

@@ -92,6 +92,29 @@ def test_chains_are_the_default_and_a_step_may_be_taken_back(pair):
     assert cache.length(a) == 44 and cache.length(b) == 60
 
 
+def test_pages_may_move_but_not_be_shared_within_a_step(pair):
+    hf, st = pair
+    text = ids(70, 4)
+    cache = st.paged_cache(20, page_size=16)
+    hole = cache.add()
+    cache.extend([hole], [64])
+    seq = cache.add()
+    st.prefill_paged(cache, [seq], [text[:40]])
+    parents = [-1, 0, 0, 2, 3]
+    tokens = torch.stack([text[40], text[0], text[41], text[42], text[43]])
+    logits, step = st.draft_paged(cache, [seq], [tokens], [parents])
+    cache.free(hole)
+    assert cache.compact()
+    sampled = torch.stack([text[41], text[0], text[42], text[43], text[44]]).cuda()
+    other = cache.fork(seq)
+    with pytest.raises(ValueError, match="forked"):
+        st.accept_paged(cache, step, sampled)
+    cache.free(other)
+    rows = st.accept_paged(cache, step, sampled)
+    assert rows[0].tolist() == [0, 2, 3, 4] and cache.length(seq) == 44
+    _check(st.prefill_paged(cache, [seq], [text[44:]]), hf_logits(hf, text)[-1:])
+
+
 def own_choice(hf, text, tokens):
     """How far each token's HF logit lies below the largest, relative to the largest logit."""
     logits = hf_logits(hf, torch.cat([text, tokens]))[len(text) - 1:-1]

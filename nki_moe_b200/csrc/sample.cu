@@ -102,8 +102,8 @@ struct SmShared {
   float warp_f[kSmWarps], warp_g[kSmWarps];
   union __align__(16) {
     struct {
-      unsigned a[kSmBins];  // counts, or the upper halves of weights
-      unsigned b[kSmBins];  // the lower halves
+      unsigned a[kSmBins];  // counts, or the lower words of weights
+      unsigned b[kSmBins];  // the upper words
     } hist;
     u64 list[kSmList];
     unsigned values[2 * kSmValues];  // counts by magnitude, then of negative values
@@ -371,11 +371,10 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const Slice
         if (kMass) y = row.exponent(x) + at * (1.0 / kSmBinsPerOctave);
       }
       if constexpr (kMass) {
-        // in units of 2^-31, at most 2^32 - 1; the halves of 65536 weights add up in 32 bits
+        // in units of 2^-31, at most 2^32 - 1; whoever makes the lower word wrap carries
         const double q = pow2_by(sh.powers, y) * 2147483648.0;
         const unsigned w = q >= 4294967295.0 ? 0xffffffffu : __double2uint_rn(q);
-        atomicAdd(&sh.hist.a[at], w >> 16);
-        atomicAdd(&sh.hist.b[at], w & 0xffffu);
+        if (atomicAdd(&sh.hist.a[at], w) > 0xffffffffu - w) atomicAdd(&sh.hist.b[at], 1u);
       } else {
         atomicAdd(&sh.hist.a[at], 1u);
       }
@@ -389,7 +388,7 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const Slice
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int i = 2 * tid + e;
-          v[e] += kMass ? fma(static_cast<double>(o.hist.a[i]), 65536.0, static_cast<double>(o.hist.b[i]))
+          v[e] += kMass ? fma(static_cast<double>(o.hist.b[i]), 4294967296.0, static_cast<double>(o.hist.a[i]))
                         : static_cast<double>(o.hist.a[i]);
         }
       }
@@ -957,7 +956,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   }
 
   SmRow row;
-  row.c = 1.4426950408889634074 / temperature;
+  row.c = fmin(1.4426950408889634074 / temperature, 1e300);
   row.max = static_cast<double>(mx);
   row.maxf = mx;
   row.bins = static_cast<float>(fmin(row.c * kSmBinsPerOctave, 1e30));

@@ -732,6 +732,8 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
         raise ValueError(f"uniforms must be a contiguous fp32 or fp64 [{T}] tensor on cuda:{dev}")
     t_rows, t_all = _setting(temperature, "temperature", torch.float32, T, dev)
     k_rows, k_all = _setting(top_k, "top_k", torch.int32, T, dev)
+    if k_all > V:  # any number, as all
+        k_all = 0
     p_rows, p_all = _setting(top_p, "top_p", torch.float32, T, dev)
     m_rows, m_all = _setting(min_p, "min_p", torch.float32, T, dev)
     tokens = uniforms.new_empty((T,), dtype=torch.int64)

@@ -124,6 +124,28 @@ def test_equal_logits_go_by_id(values, dtype, s):
     check(x, torch.tensor([0.318309886, 0.9990234], dtype=torch.float64), exact_margin=False, **s)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [151936, 262144])
+def test_equal_logits_of_whole_rows(vocab, dtype):
+    """A CTA adds up a whole row's weights in one bin: 2^18 of 2^31 units each."""
+    x = torch.full((1, vocab), 0.75, dtype=dtype, device="cuda").expand(150, -1)
+    u = torch.full((150,), 0.318309886, dtype=torch.float64, device="cuda")
+    near = (torch.arange(vocab) % 3 * 2.0 ** -100).to(dtype)[None].cuda().expand(150, -1)
+    for logits, t, k, p in ((x, 1.0, 0, 0.9), (x, 1e30, 0, 0.4), (x, math.inf, 150001, 0.7), (near, 2.0, 0, 0.45)):
+        tok, lp = ops.sample_tokens(logits, u, torch.full((150,), t, device="cuda"), k, p)
+        want, want_lp, margin = drawn(logits[0].cpu(), u[0].item(), t, k, p)
+        assert margin > 2 ** -31
+        assert (tok == want).all()
+        assert (lp.double() - want_lp).abs().max() <= 2 ** -24 * abs(want_lp) + vocab * 2 ** -45 + 1e-12
+
+
+def test_the_smallest_temperatures():
+    x, u = logits_of(3, 5003, 23)
+    for t in (5e-324, 1e-310, 1e-200):
+        check(x, u, t)
+        check(x.float(), u, t, 40, 0.9)
+
+
 def test_signed_zeros_are_equal():
     x = torch.full((1, 40), -0.0)
     x[0, ::2] = 0.0

@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kStoreThreads, kWarps == 1 ? 4 : 3) paged_stor
   int pos = place;
   if constexpr (kTree) {
     const int n = end - start, i = static_cast<int>(t) - start;
-    if (n > kTreeNodes || place < i) {  // the attention leaves such a sequence out
+    if (start < 0 || end > p.T || n > kTreeNodes || place < i) {  // the attention leaves such a sequence out
       if (lane == 0) atomicOr(p.status, kDevErrBadIndex);
       return;
     }

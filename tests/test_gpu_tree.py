@@ -271,6 +271,11 @@ def test_bad_data_is_reported(monkeypatch):
     got = run(4, torch.tensor([0, 6, 6 - 2, 18], dtype=torch.int32, device="cuda"))
     got = run(4, torch.tensor([0, 6, 11, 400], dtype=torch.int32, device="cuda"))
     assert torch.equal(got[:11], good[:11])
+    # rows that the call does not have, within what a tree may hold
+    got = run(4, torch.tensor([0, 6, 11, 18 + 40], dtype=torch.int32, device="cuda"))
+    assert torch.equal(got[:11], good[:11]) and (got[11:] == 3.0).all()
+    got = run(4, torch.tensor([-30, 6, 11, 18], dtype=torch.int32, device="cuda"))
+    assert torch.equal(got[6:], good[6:]) and (got[:6] == 3.0).all()
     # a page that the tree needs
     for bad in (-1, 10 ** 6):
         table = args[8].clone()

@@ -86,6 +86,7 @@ class DraftStep:
     parents: torch.Tensor
     cu_seqlens: torch.Tensor
     kv_lens: torch.Tensor
+    ended: bool = False
 
 
 @dataclass
@@ -623,13 +624,14 @@ class Qwen3MoEStack:
         sequence, the other nodes leave it.  Returns for each sequence the rows of
         its path: ``sampled[rows[i]]`` are its new tokens, of which the last is not
         in the cache yet."""
-        if any(q not in cache or cache.length(q) != n + m for q, n, m in zip(step.seqs, step.lengths, step.nodes)):
+        if step.ended or any(q not in cache or cache.length(q) != n + m for q, n, m in zip(step.seqs, step.lengths, step.nodes)):
             raise ValueError("the sequences are not as the step left them")
         if not all(cache.alone(q, n) for q, n in zip(step.seqs, step.lengths)):
             raise ValueError("a sequence was forked between its step and the step's end")
         counts, path, _ = ops.accept_drafts(step.tokens, sampled, step.parents, step.cu_seqlens, step.kv_lens, cache.pool,
                                             cache.table(step.seqs).to(self.device))
         counts = counts.tolist()
+        step.ended = True
         cache.take_back(step.seqs, [n + k for n, k in zip(step.lengths, counts)])
         for q in step.seqs:
             cache.trim(q)
@@ -637,7 +639,8 @@ class Qwen3MoEStack:
         return [path[a:a + k].long() + a for a, k in zip(starts.tolist(), counts)]
 
     def _draw(self, logits, temperature, top_k, top_p, min_p, generator):
-        """Tokens from rows of logits, by a random number each."""
+        """Tokens from rows of logits, by a random number each; -1 for a row that has no
+        distribution (a NaN, or nothing that is finite)."""
         if temperature == 0:
             return logits.argmax(-1)
         u = torch.rand(logits.shape[0], dtype=torch.float64, device=self.device, generator=generator)
@@ -674,6 +677,8 @@ class Qwen3MoEStack:
                     scores[i].append(tuple(x[at:at + len(r)] for x in parts))
                     at += len(r)
             drawn = sampled[kept].tolist()
+            if min(drawn) < 0:
+                raise RuntimeError("logits without a distribution")
             for i, r in zip(live, rows):
                 new[i] += drawn[:len(r)]
                 texts[i].extend(drawn[:len(r)])
@@ -731,6 +736,8 @@ class Qwen3MoEStack:
 
             if drafts:
                 tok = draw(logits)
+                if int(tok.min()) < 0:
+                    raise RuntimeError("logits without a distribution")
                 if top_logprobs is not None:
                     scores = [[tuple(x[i:i + 1] for x in ops.token_logprobs(logits, tok, top_logprobs))]
                               for i in range(len(seqs))]
@@ -749,7 +756,8 @@ class Qwen3MoEStack:
                 if top_logprobs is not None:
                     scores.append(ops.token_logprobs(logits, tok, top_logprobs))
                 if i + 1 < max_new_tokens:
-                    logits = self.decode_paged(cache, seqs, tok, graph)
+                    # (a row without a distribution goes on with any token: it is refused at the end)
+                    logits = self.decode_paged(cache, seqs, tok.clamp(min=0) if restricted else tok, graph)
         finally:
             for q in seqs:
                 if q in cache:
@@ -758,6 +766,8 @@ class Qwen3MoEStack:
                 self._drop_steps(cache)  # nobody else can use this cache
         tokens = torch.tensor(out, device=self.device) if drafts else torch.stack(out, 1)
         tokens = tokens.view(n, samples, max_new_tokens)
+        if restricted and not drafts and int(tokens.min()) < 0:
+            raise RuntimeError("logits without a distribution")
         if top_logprobs is None:
             return tokens, None
         if drafts:

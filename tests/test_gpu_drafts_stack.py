@@ -1,6 +1,8 @@
 """Drafted tokens in the decoder stack: steps with trees against HF (bars: see
 ``test_gpu_stack.py``), generation with drafts and with restricted sampling."""
 
+import math
+
 import pytest
 import torch
 
@@ -112,6 +114,12 @@ def test_pages_may_move_but_not_be_shared_within_a_step(pair):
     cache.free(other)
     rows = st.accept_paged(cache, step, sampled)
     assert rows[0].tolist() == [0, 2, 3, 4] and cache.length(seq) == 44
+    logits, step = st.draft_paged(cache, [seq], [text[44:47]])
+    rows = st.accept_paged(cache, step, text[45:48].cuda())
+    assert rows[0].tolist() == [0, 1, 2] and cache.length(seq) == 47
+    with pytest.raises(ValueError):  # it has ended, with all of its nodes
+        st.accept_paged(cache, step, text[:3].cuda())
+    cache.take_back([seq], [44])
     _check(st.prefill_paged(cache, [seq], [text[44:]]), hf_logits(hf, text)[-1:])
 
 
@@ -204,3 +212,18 @@ def test_refusals(pair):
                dict(temperature=-1.0, top_k=3), dict(temperature=float("nan"), drafts=3)):
         with pytest.raises(ValueError):
             st.generate_paged([ids(4, 1)], 4, **kw)
+
+
+def test_logits_without_a_distribution_are_refused(pair):
+    _, st = pair
+    head = st.lm_head
+    try:
+        st.lm_head = torch.full_like(head, math.nan)
+        for kw in (dict(drafts=4), dict(), dict(graph=False)):
+            with pytest.raises(RuntimeError, match="distribution"):
+                st.generate_paged([ids(9, 1), ids(20, 2)], 3, temperature=1.0, top_k=5, **kw)
+    finally:
+        st.lm_head = head
+        st.release_graph()
+    tokens, _ = st.generate_paged([ids(9, 1), ids(20, 2)], 3, temperature=1.0, top_k=10 ** 30)
+    assert int(tokens.min()) >= 0

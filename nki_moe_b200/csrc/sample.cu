@@ -107,7 +107,7 @@ struct SmShared {
     } hist;
     u64 list[kSmList];
     unsigned values[2 * kSmValues];  // counts by magnitude, then of negative values
-    u64 weights[2 * kSmValues];      // as the counts
+    uint2 weights[2 * kSmValues];    // as the counts: a weight's low 22 bits, and the others
   };
 };
 
@@ -233,6 +233,7 @@ struct SmSlice {
   int vecs;
   int id0;  // of the first element (a vector may begin before the row: -inf there)
   int V;
+  int in_lo, in_n;  // the vectors [in_lo, in_lo + in_n) lie inside the row
 
   // A vector of the row in global memory; what lies outside of the row is -inf.
   static __device__ __forceinline__ uint4 fetch(const uint4* at, int id, int V) {
@@ -247,7 +248,10 @@ struct SmSlice {
     return x.u;
   }
   __device__ __forceinline__ uint4 raw(int v) const {
-    if constexpr (kWhole) return fetch(data + v, id0 + v * VE, V);
+    if constexpr (kWhole) {
+      if (static_cast<unsigned>(v - in_lo) < static_cast<unsigned>(in_n)) return __ldg(data + v);
+      return fetch(data + v, id0 + v * VE, V);
+    }
     return data[v];
   }
   static __device__ __forceinline__ void unpack(const uint4& u, float (&x)[VE]) {
@@ -263,7 +267,17 @@ struct SmSlice {
   // f(vector, its number) for the vectors lo + at, lo + at + step, ... below hi
   template <typename F>
   __device__ __forceinline__ void vectors(int lo, int hi, int at, int step, F f) const {
-    for (int v = lo + at; v < hi; v += kAhead * step) {
+    int v = lo + at;
+    if constexpr (kAhead > 1) {
+      for (; v + (kAhead - 1) * step < hi; v += kAhead * step) {
+        uint4 u[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) u[a] = raw(v + a * step);
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) f(u[a], v + a * step);
+      }
+    }
+    for (; v < hi; v += kAhead * step) {
       uint4 u[kAhead];
 #pragma unroll
       for (int a = 0; a < kAhead; ++a)
@@ -531,51 +545,47 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const Slice
 struct SmWindow {
   int lo;
   __device__ __forceinline__ int place(unsigned b) const { return static_cast<int>(b & 0x7fffu) - lo; }
-  __device__ __forceinline__ bool has(int at) const { return static_cast<unsigned>(at) < kSmValues; }
-  // the bin of bits b whose magnitude has place `at`
-  __device__ __forceinline__ int bin(unsigned b, int at) const { return at | (b >> 4 & kSmValues); }
   __device__ __forceinline__ float value(int bin) const {
     return __uint_as_float(static_cast<unsigned>(lo + (bin & (kSmValues - 1))) << 16 | (bin & kSmValues ? 0x80000000u : 0u));
   }
-  // Byte offsets of the bins (kBytes each) of a word's two logits, the place clamped
-  // from above (what lies behind the window counts as its last bin); `below` gets a
-  // negative number where one lies nearer to zero than the window.
+  // Byte offsets of the bins (kBytes each) of a word's two logits, both halves at a
+  // time.  What lies outside of the window, on either side, goes to its sign's last
+  // bin; `least` takes the smallest magnitudes, for near().
   template <int kBytes>
-  __device__ __forceinline__ void offsets(uint32_t w, unsigned& first, unsigned& second, int& below) const {
-    constexpr int kShift = kBytes == 8 ? 3 : 2;
-    constexpr unsigned kMags = 0x7fffu << kShift, kSign = kSmValues * kBytes;  // the sign's bit: 13 or 14
-    const int a = static_cast<int>(w << kShift & kMags) - (lo << kShift), c = static_cast<int>(w >> (16 - kShift) & kMags) - (lo << kShift);
-    below = min(below, min(a, c));
-    first = static_cast<unsigned>(min(a, (kSmValues - 1) * kBytes)) | (w >> (4 - kShift) & kSign);
-    second = static_cast<unsigned>(min(c, (kSmValues - 1) * kBytes)) | (w >> (20 - kShift) & kSign);
+  __device__ __forceinline__ void offsets(uint32_t w, unsigned& first, unsigned& second, uint32_t& least) const {
+    static_assert(kSmValues * kBytes * 2 <= 1 << 16 && kSmValues == 1 << 11, "halves of 16 bits, the sign above the place");
+    const uint32_t mags = w & 0x7fff7fffu;
+    least = __vminu2(least, mags);
+    const uint32_t minus = static_cast<uint32_t>(-lo & 0xffff) * 0x10001u;
+    const uint32_t q = (__viaddmin_u16x2(mags, minus, (kSmValues - 1) * 0x10001u) | (w >> 4 & 0x08000800u)) * kBytes;
+    first = q & 0xffffu;
+    second = q >> 16;
   }
+  // whether one of them lies nearer to zero than the window
+  __device__ __forceinline__ bool near(uint32_t least) const { return static_cast<int>(min(least & 0xffffu, least >> 16)) < lo; }
 };
 // Bins in falling order of their values: the positive ones by falling magnitude,
 // then the negative ones by rising magnitude.
 __device__ __forceinline__ int sm_bin_at(int place) { return place < kSmValues ? kSmValues - 1 - place : place; }
 constexpr int kSmZone = 2 * kSmValues;  // the place of what is nearer to zero than the window
 
-// Counts the values of a vector.
+// Counts the values of a vector.  -inf, and what is too far below the maximum to
+// weigh anything, add to the last negative bin, which no other logit is in; what is
+// nearer to zero than the window is listed (and counted in its sign's last bin).
 __device__ __forceinline__ void sm_count(SmShared& sh, const SmWindow& win, const uint4& u) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
   unsigned at[8];
-  int below = 0;
+  uint32_t least = 0x7fff7fffu;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) win.offsets<4>(w[i], at[2 * i], at[2 * i + 1], below);
-  if (below >= 0) {
-    // -inf, and what is too far below the maximum to weigh anything, add to the
-    // last negative bin, which no other logit is in
+  for (int i = 0; i < 4; ++i) win.offsets<4>(w[i], at[2 * i], at[2 * i + 1], least);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) atomicAdd(reinterpret_cast<unsigned*>(reinterpret_cast<char*>(sh.values) + at[i]), 1u);
-  } else {
+  for (int i = 0; i < 8; ++i) atomicAdd(reinterpret_cast<unsigned*>(reinterpret_cast<char*>(sh.values) + at[i]), 1u);
+  if (win.near(least)) {
 #pragma unroll 1
     for (int i = 0; i < 8; ++i) {
       const uint32_t x = i < 2 ? u.x : i < 4 ? u.y : i < 6 ? u.z : u.w;
       const unsigned b = i & 1 ? x >> 16 : x & 0xffffu;
-      const int place = win.place(b);
-      if (place >= 0) {
-        atomicAdd(&sh.values[win.bin(b, min(place, kSmValues - 1))], 1u);
-      } else {
+      if (win.place(b) < 0) {
         const int k = atomicAdd(&sh.near, 1);
         if (k < kSmNear) sh.near_of[k] = static_cast<unsigned short>(b);
       }
@@ -608,8 +618,11 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
   const int zones = sh.near;
   // (their sum is the same whatever order they were listed in: whole numbers of 2^-52)
   u64 near = 0;
-  for (int k = tid; k < min(zones, kSmNear); k += kSmThreads)
-    near += static_cast<u64>(pow2_by(sh.powers, row.exponent(__uint_as_float(static_cast<unsigned>(sh.near_of[k]) << 16))) * 0x1p52);
+  for (int k = tid; k < min(zones, kSmNear); k += kSmThreads) {
+    const unsigned b = sh.near_of[k];
+    near += static_cast<u64>(pow2_by(sh.powers, row.exponent(__uint_as_float(b << 16))) * 0x1p52);
+    if (!(b & 0x8000u)) atomicSub(&sh.values[kSmValues - 1], 1u);  // it is not one of the largest
+  }
   near = sm_sum(near);
   if (lane == 0) sh.warp_lo[warp] = near;
   if (tid < 2) sh.place_of[tid] = -1;
@@ -825,6 +838,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   sl.V = p.V;
   sl.id0 = rank * p.slice - mis;
   sl.vecs = min(p.slice, max(0, p.V - sl.id0) + VE - 1) / VE;
+  sl.in_lo = mis > 0;
+  sl.in_n = max(0, (p.V - sl.id0) / VE - sl.in_lo);
   if constexpr (kWhole) {
     sl.data = row0;
   } else {
@@ -1005,7 +1020,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
       const float x = win.value(i);
       u64 w = 0;
       if (x >= row.least && x <= mx && i != 2 * kSmValues - 1 && !(row.cut && x == row.least)) w = sm_fixed(pow2_by(sh.powers, row.exponent(x)), row.min_weight);
-      sh.weights[i] = w;
+      sh.weights[i] = make_uint2(static_cast<unsigned>(w) & 0x3fffffu, static_cast<unsigned>(w >> 22));
     }
     __syncthreads();
   }
@@ -1024,9 +1039,9 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     if constexpr (sizeof(T) == 2) {
       const uint32_t x[4] = {d.x, d.y, d.z, d.w};
       unsigned at[8];
-      int below = plain ? 0 : -1;
+      uint32_t least = 0x7fff7fffu;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) win.offsets<8>(x[i], at[2 * i], at[2 * i + 1], below);
+      for (int i = 0; i < 4; ++i) win.offsets<8>(x[i], at[2 * i], at[2 * i + 1], least);
       const int id = sl.id0 + v * VE;
       bool ties = false;  // cut within this vector
       if (!row.cut && id + VE - 1 > row.last_id && row.least > -INFINITY) {  // behind the last equal logit that is kept, if not before its vector's end
@@ -1039,14 +1054,15 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
         }
         ties = m != 0;
       }
-      if (below >= 0 && !ties) {
-        u64 even = 0;
+      if (plain && !win.near(least) && !ties) {
+        unsigned low = 0, high = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          sum += *reinterpret_cast<const u64*>(reinterpret_cast<const char*>(sh.weights) + at[i]);
-          even += *reinterpret_cast<const u64*>(reinterpret_cast<const char*>(sh.weights) + at[i + 1]);
+        for (int i = 0; i < 8; ++i) {
+          const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(sh.weights) + at[i]);
+          low += w.x;
+          high += w.y;
         }
-        return sum + even;
+        return low + (static_cast<u64>(high) << 22);
       }
     }
     return sm_weigh<T>(d, sl.id0 + v * VE, row, sh.powers);
@@ -1054,40 +1070,46 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   const int per = (sl.vecs + kSmWarps - 1) / kSmWarps;
   const int v_lo = min(sl.vecs, warp * per), v_hi = min(sl.vecs, v_lo + per);
   u64 sum = 0;
-  // equal logits that are cut weigh nothing there and are counted (two counts of 16
-  // bits: a lane has at most 2^18 / 512 of a row)
+  // equal logits that are cut weigh nothing there and are counted
   const u64 edge = row.cut ? sm_fixed(pow2_by(sh.powers, row.exponent(row.least)), row.min_weight) : 0ull;
-  uint32_t pairs = 0;
+  // (masks of 16 bits are added: a equal ones in the words' low halves and c in the high
+  // ones give (a - c) 2^16 - a; a lane has at most 2^18 / 512 of a row)
+  uint32_t masks = 0;
   auto equal = [&](const uint4& d) {
-    return (equal_bf16x2(d.x, edge2) & 0x00010001u) + (equal_bf16x2(d.y, edge2) & 0x00010001u) +
-           (equal_bf16x2(d.z, edge2) & 0x00010001u) + (equal_bf16x2(d.w, edge2) & 0x00010001u);
+    return equal_bf16x2(d.x, edge2) + equal_bf16x2(d.y, edge2) + equal_bf16x2(d.z, edge2) + equal_bf16x2(d.w, edge2);
+  };
+  auto equals = [](uint32_t masks) {
+    const uint32_t a = -masks & 0xffffu;
+    return static_cast<int>(a + ((a - ((masks + a) >> 16)) & 0xffffu));
   };
   const int edge_place = win.place(__float_as_uint(row.least) >> 16);
   if (sizeof(T) == 2 && plain && row.least > 0.f && edge_place > 0 && (row.cut || row.last_id == 0x7fffffff)) {
     // only positive logits of the window are kept: as signed numbers, what is below
     // them reads the one bin before the border's, which holds 0, so lanes that keep
     // nothing share an access
-    const int low = (win.lo + edge_place - 1) * 8;
-    const char* const table = reinterpret_cast<const char*>(sh.weights) - win.lo * 8;
-    u64 odd = 0;
+    const uint32_t low2 = static_cast<uint32_t>(win.lo + edge_place - 1) * 0x10001u, lo2 = static_cast<uint32_t>(win.lo) * 0x10001u;
+    unsigned low = 0, high = 0;  // (at most 2^18 / 512 of 2^22 each)
     sl.vectors(v_lo, v_hi, lane, 32, [&](const uint4& d, int) {
       const uint32_t w[4] = {d.x, d.y, d.z, d.w};
-      if (row.cut) pairs += equal(d);
+      if (row.cut) masks += equal(d);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        sum += *reinterpret_cast<const u64*>(table + max(static_cast<int>(w[i] << 16) >> 13, low));
-        odd += *reinterpret_cast<const u64*>(table + max(static_cast<int>(w[i]) >> 13 & ~7, low));
+        const uint32_t at = (__vmaxs2(w[i], low2) - lo2) * 8u;
+        const uint2 a = *reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(sh.weights) + (at & 0xffffu));
+        const uint2 c = *reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(sh.weights) + (at >> 16));
+        low += a.x + c.x;
+        high += a.y + c.y;
       }
     });
-    sum += odd;
+    sum = low + (static_cast<u64>(high) << 22);
   } else {
     sl.vectors(v_lo, v_hi, lane, 32, [&](const uint4& d, int v) {
       sum += sum_of(d, v);
-      if (sizeof(T) == 2 && row.cut) pairs += equal(d);
+      if (sizeof(T) == 2 && row.cut) masks += equal(d);
     });
   }
   sum = sm_sum(sum);
-  int ties = __reduce_add_sync(0xffffffffu, static_cast<int>((pairs & 0xffffu) + (pairs >> 16)));
+  int ties = __reduce_add_sync(0xffffffffu, equals(masks));
   __syncthreads();
   if (lane == 0) {
     sh.warp_lo[warp] = sum;
@@ -1147,10 +1169,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   for (int v = first; v < min(end, first + most); ++v) {
     const uint4 d = sl.raw(v);
     mine += sum_of(d, v);
-    if (sizeof(T) == 2 && row.cut) {
-      const uint32_t c = equal(d);
-      own += static_cast<int>((c & 0xffffu) + (c >> 16));
-    }
+    if (sizeof(T) == 2 && row.cut) own += equals(equal(d));
   }
   if (row.cut) {
     int none;
@@ -1171,36 +1190,46 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   }
   __syncthreads();
   const bool passed = sh.listed < kSmThreads;
-  if (tid == (passed ? sh.listed : sh.pick)) {
-    u64 s = before + sums.before;
-    int token = -1;
-    float x = 0.f;
-    for (int v = first; v < min(end, first + most); ++v) {
-      float e[VE];
-      Slice::unpack(sl.raw(v), e);
-#pragma unroll 1
-      for (int i = 0; i < VE; ++i) {
-        float y = e[0];
-#pragma unroll
-        for (int j = 1; j < VE; ++j) y = i == j ? e[j] : y;
-        const int id = sl.id0 + v * VE + i;
-        u64 w = row.keeps(y, id) ? sm_fixed(pow2_by(sh.powers, row.exponent(y)), row.min_weight) : 0ull;
-        if (row.cut && y == row.least && left > 0) {
-          w = edge;
-          --left;
-        }
-        // the first that passes, or the last
-        if (w > 0 && (token < 0 || !passed || s <= goal)) {
-          token = id;
-          x = y;
-        }
-        s += w;
-      }
-    }
-    p.tokens[r] = token;
-    // the weight itself, not its whole number
-    p.logprob[r] = static_cast<float>(row.exponent(x) * 0.69314718055994530942 - log(static_cast<double>(whole) * 0x1p-44));
+  const int who = passed ? sh.listed : sh.pick;
+  if (tid == who) {
+    sh.lo = before + sums.before;
+    sh.place_of[0] = left;
   }
+  __syncthreads();
+  // that thread's logits, one a lane
+  if (warp == 1 && lane == 0) sh.warp_d[0] = log(static_cast<double>(whole) * 0x1p-44);
+  if (warp == 0 && who >= 0) {
+    const int v0 = min(sl.vecs, here * per) + most * who;
+    u64 run = sh.lo;
+    int to_come = sh.place_of[0];
+    for (int e = lane; e - lane < most * VE; e += 32) {
+      const int v = v0 + e / VE, id = sl.id0 + v * VE + e % VE;
+      float x = -INFINITY;
+      if (v < min(end, v0 + most) && id >= 0 && id < p.V)
+        x = static_cast<float>(reinterpret_cast<const T*>(sl.data)[v * VE + e % VE]);
+      u64 w = row.keeps(x, id) ? sm_fixed(pow2_by(sh.powers, row.exponent(x)), row.min_weight) : 0ull;
+      const unsigned ties = __ballot_sync(0xffffffffu, row.cut && x == row.least);
+      if ((ties >> lane & 1u) && __popc(ties & ((1u << lane) - 1u)) < to_come) w = edge;
+      u64 upto = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 q = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += q;
+      }
+      // the first that passes, or the last
+      const unsigned kept = __ballot_sync(0xffffffffu, w > 0);
+      const unsigned over = __ballot_sync(0xffffffffu, w > 0 && run + upto > goal);
+      if (lane == (over ? __ffs(over) - 1 : 31 - __clz(kept))) {
+        p.tokens[r] = id;
+        sh.warp_d[1] = row.exponent(x) * 0.69314718055994530942;  // the weight itself, not its whole number
+      }
+      if (over) break;
+      run += __shfl_sync(0xffffffffu, upto, 31);
+      to_come = max(0, to_come - __popc(ties));
+    }
+  }
+  __syncthreads();
+  if (tid == 0 && who >= 0) p.logprob[r] = static_cast<float>(sh.warp_d[1] - sh.warp_d[0]);
 }
 
 template <typename T>

@@ -264,17 +264,23 @@ struct SmSlice {
       x[3] = __uint_as_float(u.w);
     }
   }
-  // f(vector, its number) for the vectors lo + at, lo + at + step, ... below hi
+  // f(vector, its number) for the vectors lo + at, lo + at + step, ... below hi, at
+  // being a thread's number in its warp or CTA.  (The warp comes together after each
+  // vector: lanes that took a rare way would stay apart for many.)
   template <typename F>
   __device__ __forceinline__ void vectors(int lo, int hi, int at, int step, F f) const {
     int v = lo + at;
+    const int lane = threadIdx.x & 31;
     if constexpr (kAhead > 1) {
-      for (; v + (kAhead - 1) * step < hi; v += kAhead * step) {
+      for (; v - lane + 31 + (kAhead - 1) * step < hi; v += kAhead * step) {
         uint4 u[kAhead];
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) u[a] = raw(v + a * step);
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) f(u[a], v + a * step);
+        for (int a = 0; a < kAhead; ++a) {
+          f(u[a], v + a * step);
+          __syncwarp();
+        }
       }
     }
     for (; v < hi; v += kAhead * step) {

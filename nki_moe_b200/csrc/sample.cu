@@ -53,6 +53,7 @@ constexpr int kSmWholeRows = 148;    // rows from which on a CTA takes a whole o
 constexpr int kSmValues = 2048;      // values of a sign that have a bin
 constexpr int kSmNear = 512;         // logits nearer to zero that a CTA sums
 constexpr int kSmMaxVocab = 1 << 18;
+constexpr int kSmGroups = 17;        // groups of vectors in a warp's part
 static_assert(2 * kSmThreads == kSmBins, "two bins per thread");
 
 using u64 = unsigned long long;
@@ -100,6 +101,10 @@ struct SmShared {
   u64 warp_lo[kSmWarps], warp_hi[kSmWarps];
   int warp_n[kSmWarps];
   float warp_f[kSmWarps], warp_g[kSmWarps];
+  u64 group_sum[kSmWarps * kSmGroups];  // of kept weights, without equal logits that are cut
+  int group_ties[kSmWarps * kSmGroups];  // those
+  u64 part_before;
+  int part_ties, part;
   union __align__(16) {
     struct {
       unsigned a[kSmBins];  // counts, or the lower words of weights
@@ -223,6 +228,18 @@ __device__ __forceinline__ N sm_sum(N v) {
   return v;
 }
 
+// The shared memory of CTA r of a row, and their barrier; a whole row's CTA is alone.
+template <bool kAlone>
+__device__ __forceinline__ SmShared& sm_of(const cg::cluster_group& cl, SmShared& sh, int r) {
+  if constexpr (kAlone) return sh;
+  return *cl.map_shared_rank(&sh, r);
+}
+template <bool kAlone>
+__device__ __forceinline__ void sm_sync(const cg::cluster_group& cl) {
+  if constexpr (kAlone) __syncthreads();
+  else cl.sync();
+}
+
 // The CTA's part of the row: a slice in shared memory, or (kWhole) the row itself.
 template <typename T, bool kWhole>
 struct SmSlice {
@@ -271,16 +288,14 @@ struct SmSlice {
   __device__ __forceinline__ void vectors(int lo, int hi, int at, int step, F f) const {
     int v = lo + at;
     const int lane = threadIdx.x & 31;
-    if constexpr (kAhead > 1) {
-      for (; v - lane + 31 + (kAhead - 1) * step < hi; v += kAhead * step) {
-        uint4 u[kAhead];
+    for (; v - lane + 31 + (kAhead - 1) * step < hi; v += kAhead * step) {
+      uint4 u[kAhead];
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) u[a] = raw(v + a * step);
+      for (int a = 0; a < kAhead; ++a) u[a] = raw(v + a * step);
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) {
-          f(u[a], v + a * step);
-          __syncwarp();
-        }
+      for (int a = 0; a < kAhead; ++a) {
+        f(u[a], v + a * step);
+        __syncwarp();
       }
     }
     for (; v < hi; v += kAhead * step) {
@@ -365,7 +380,7 @@ template <bool kMass, typename Slice>
 __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const Slice& sl, SmRow& row, double limit) {
   const int tid = threadIdx.x, ranks = Slice::kAlone ? 1 : cl.num_blocks();
   const bool first = Slice::kAlone || cl.block_rank() == 0;
-  SmShared& lead = *cl.map_shared_rank(&sh, 0);
+  SmShared& lead = sm_of<Slice::kAlone>(cl, sh, 0);
   bool split = false;  // the range is [lo, hi], not yet: one bin of distances
   u64 lo = 0, hi = 0, width = 0;
   double top = 0.0;  // split: exponent of the range's largest weight
@@ -399,12 +414,12 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const Slice
         atomicAdd(&sh.hist.a[at], 1u);
       }
     });
-    cl.sync();
+    sm_sync<Slice::kAlone>(cl);
     // ---- the first CTA joins the histograms and finds the bin
     if (first) {
       double v[2] = {0.0, 0.0};
       for (int r = 0; r < ranks; ++r) {
-        const SmShared& o = *cl.map_shared_rank(&sh, r);
+        const SmShared& o = sm_of<Slice::kAlone>(cl, sh, r);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int i = 2 * tid + e;
@@ -436,15 +451,15 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const Slice
         const int at = 2 * tid + second;
         const double ab = above + sums.before + (second ? v[0] : 0.0);
         for (int r = 0; r < ranks; ++r) {
-          SmShared& o = *cl.map_shared_rank(&sh, r);
+          SmShared& o = sm_of<Slice::kAlone>(cl, sh, r);
           o.bin = at;
           o.above = ab;
         }
       } else if (none && tid == 0) {
-        for (int r = 0; r < ranks; ++r) cl.map_shared_rank(&sh, r)->bin = -1;
+        for (int r = 0; r < ranks; ++r) sm_of<Slice::kAlone>(cl, sh, r).bin = -1;
       }
     }
-    cl.sync();
+    sm_sync<Slice::kAlone>(cl);
     bin = sh.bin;
     if (bin < 0) return;  // fewer than k
     if (split) {
@@ -458,7 +473,7 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const Slice
       const int at = atomicAdd(&lead.listed, 1);
       if (at < kSmList) lead.list[at] = key;
     });
-    cl.sync();
+    sm_sync<Slice::kAlone>(cl);
     const int n = lead.listed;
     if (n <= kSmList) {
       if (first) {
@@ -500,10 +515,10 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const Slice
               ++at;
             }
           const u64 border = sh.list[min(at, n - 1)];
-          for (int r = 0; r < ranks; ++r) cl.map_shared_rank(&sh, r)->border = border;
+          for (int r = 0; r < ranks; ++r) sm_of<Slice::kAlone>(cl, sh, r).border = border;
         }
       }
-      cl.sync();
+      sm_sync<Slice::kAlone>(cl);
       row.keep_to(sh.border);
       return;
     }
@@ -530,11 +545,11 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const Slice
         least = min(least, sh.warp_lo[w]);
         most = max(most, sh.warp_hi[w]);
       }
-      SmShared& o = *cl.map_shared_rank(&sh, tid);
+      SmShared& o = sm_of<Slice::kAlone>(cl, sh, tid);
       o.lo_of[cl.block_rank()] = least;
       o.hi_of[cl.block_rank()] = most;
     }
-    cl.sync();
+    sm_sync<Slice::kAlone>(cl);
     lo = ~0ull;
     hi = 0;
     for (int r = 0; r < ranks; ++r) {
@@ -636,12 +651,12 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
   if (warp == 0) {
     near = sm_sum(lane < kSmWarps ? sh.warp_lo[lane] : 0ull);
     if (lane < ranks) {
-      SmShared& o = *cl.map_shared_rank(&sh, lane);
+      SmShared& o = sm_of<Slice::kAlone>(cl, sh, lane);
       o.zone_of[rank] = static_cast<double>(near) * 0x1p-52;
       o.zones_of[rank] = zones;
     }
   }
-  cl.sync();
+  sm_sync<Slice::kAlone>(cl);
   for (int r = 0; r < ranks; ++r)
     if (sh.zones_of[r] > kSmNear) return false;  // more than were listed
   // ---- this CTA's share of the bins: a thread's are neighbours in the order
@@ -657,7 +672,7 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
     unsigned got[kMost];
 #pragma unroll
     for (int i = 0; i < kMost; ++i)  // all loads in flight
-      got[i] = cl.map_shared_rank(&sh, i >> shift)->values[sm_bin_at(place0 + (i & (each - 1)))];
+      got[i] = sm_of<Slice::kAlone>(cl, sh, i >> shift).values[sm_bin_at(place0 + (i & (each - 1)))];
 #pragma unroll
     for (int e = 0; e < kMost; ++e)
 #pragma unroll
@@ -673,7 +688,7 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
     const bool gets = place0 + each == kSmValues, gives = place0 == kSmValues;
     if (gets)
       for (int r = 0; r < ranks; ++r) {
-        const int more = static_cast<int>(cl.map_shared_rank(&sh, r)->values[kSmValues]);
+        const int more = static_cast<int>(sm_of<Slice::kAlone>(cl, sh, r).values[kSmValues]);
 #pragma unroll
         for (int e = 0; e < kMost; ++e)
           if (e == each - 1) n[e] += more;
@@ -710,11 +725,11 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
   SmSums<int> counts = sm_scan(count, sh.warp_n, held);
   SmSums<double> sums = sm_scan(sum, sh.warp_d, mine);
   if (tid < ranks) {
-    SmShared& o = *cl.map_shared_rank(&sh, tid);
+    SmShared& o = sm_of<Slice::kAlone>(cl, sh, tid);
     o.count_of[rank] = held;
     o.mass_of[rank] = mine;
   }
-  cl.sync();
+  sm_sync<Slice::kAlone>(cl);
   int all = 0, count_before = 0;
   double total = 0.0, mass_before = 0.0;
   for (int r = 0; r < ranks; ++r) {
@@ -733,7 +748,7 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
   // tells all CTAs border i: of a thread's bin e the first `ties` tokens are kept
   auto tell = [&](int i, int e, int ties, int of, double kept) {
     for (int r = 0; r < ranks; ++r) {
-      SmShared& o = *cl.map_shared_rank(&sh, r);
+      SmShared& o = sm_of<Slice::kAlone>(cl, sh, r);
       o.place_of[i] = e == kMost ? kSmZone : place0 + e;
       o.ties_of[i] = ties;
       o.held_of[i] = of;
@@ -755,7 +770,7 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
         m += mass[e];
       }
     }
-    cl.sync();
+    sm_sync<Slice::kAlone>(cl);
     if (sh.place_of[0] == kSmZone) return false;
     kept = sh.sum_k;
   }
@@ -774,7 +789,7 @@ __device__ bool sm_values(const cg::cluster_group& cl, SmShared& sh, const Slice
         m += mass[e];
       }
     }
-    cl.sync();
+    sm_sync<Slice::kAlone>(cl);
     if (sh.place_of[1] == kSmZone) return false;
   }
   // ---- the first of the two
@@ -831,7 +846,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   const int ranks = kWhole ? 1 : cl.num_blocks(), rank = kWhole ? 0 : cl.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long r = blockIdx.x / ranks;
-  cl.barrier_arrive();  // no CTA is written to before it runs
+  if (!kWhole) cl.barrier_arrive();  // no CTA is written to before it runs
   if (tid < 64) sh.powers[tid] = pow2(tid * (1.0 / 64));
   pdl_launch_dependents();
   pdl_wait();
@@ -925,18 +940,18 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     sh.warp_g[warp] = mn;
   }
   __syncthreads();
-  cl.barrier_wait();
+  if (!kWhole) cl.barrier_wait();
   if (warp == 0) {
     mx = lane < kSmWarps ? sh.warp_f[lane] : -INFINITY;
     mn = lane < kSmWarps ? sh.warp_g[lane] : INFINITY;
     join();
     if (lane < ranks) {
-      SmShared& o = *cl.map_shared_rank(&sh, lane);
+      SmShared& o = sm_of<kWhole>(cl, sh, lane);
       o.max_of[rank] = mx;
       o.min_of[rank] = mn;
     }
   }
-  cl.sync();
+  sm_sync<kWhole>(cl);
   mx = -INFINITY;
   mn = INFINITY;
   for (int q = 0; q < ranks; ++q) {
@@ -965,9 +980,9 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     __syncthreads();
     if (warp == 0) {
       id = __reduce_min_sync(0xffffffffu, lane < kSmWarps ? sh.warp_n[lane] : 0x7fffffff);
-      if (lane == 0) cl.map_shared_rank(&sh, 0)->count_of[rank] = id;
+      if (lane == 0) sm_of<kWhole>(cl, sh, 0).count_of[rank] = id;
     }
-    cl.sync();
+    sm_sync<kWhole>(cl);
     if (rank == 0 && tid == 0) {
       for (int q = 0; q < ranks; ++q) id = min(id, sh.count_of[q]);
       p.tokens[r] = id;
@@ -1073,14 +1088,10 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     }
     return sm_weigh<T>(d, sl.id0 + v * VE, row, sh.powers);
   };
-  const int per = (sl.vecs + kSmWarps - 1) / kSmWarps;
-  const int v_lo = min(sl.vecs, warp * per), v_hi = min(sl.vecs, v_lo + per);
-  u64 sum = 0;
-  // equal logits that are cut weigh nothing there and are counted
+  // equal logits that are cut weigh nothing there and are counted (masks of 16 bits
+  // are added: a equal ones in the words' low halves and c in the high ones give
+  // (a - c) 2^16 - a)
   const u64 edge = row.cut ? sm_fixed(pow2_by(sh.powers, row.exponent(row.least)), row.min_weight) : 0ull;
-  // (masks of 16 bits are added: a equal ones in the words' low halves and c in the high
-  // ones give (a - c) 2^16 - a; a lane has at most 2^18 / 512 of a row)
-  uint32_t masks = 0;
   auto equal = [&](const uint4& d) {
     return equal_bf16x2(d.x, edge2) + equal_bf16x2(d.y, edge2) + equal_bf16x2(d.z, edge2) + equal_bf16x2(d.w, edge2);
   };
@@ -1088,154 +1099,163 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     const uint32_t a = -masks & 0xffffu;
     return static_cast<int>(a + ((a - ((masks + a) >> 16)) & 0xffffu));
   };
+  constexpr int kGroup = kWhole ? 32 / VE : 1;  // vectors of a lane in a group
+  constexpr int kAtOnce = kWhole ? 4 : 1;
+  constexpr int kSliceVecs = kSmMaxVocab / VE / kSmCluster + 1 > kSmSlice / 16 ? kSmMaxVocab / VE / kSmCluster + 1 : kSmSlice / 16;
+  constexpr int kMostVecs = kWhole ? kSmMaxVocab / VE + 1 : kSliceVecs;
+  static_assert((kMostVecs + kSmWarps - 1) / kSmWarps <= kSmGroups * 32 * kGroup && kSmWarps * kSmGroups <= kSmThreads, "groups");
+  const int per = (sl.vecs + kSmWarps - 1) / kSmWarps;
+  const int v_lo = min(sl.vecs, warp * per), v_hi = min(sl.vecs, v_lo + per);
+  if (lane < kSmGroups) {
+    sh.group_sum[warp * kSmGroups + lane] = 0;
+    sh.group_ties[warp * kSmGroups + lane] = 0;
+  }
+  __syncwarp();
+  // where only positive logits of the window are kept: as signed numbers, what is below
+  // them reads the one bin before the border's, which holds 0, so lanes that keep
+  // nothing share an access
   const int edge_place = win.place(__float_as_uint(row.least) >> 16);
-  if (sizeof(T) == 2 && plain && row.least > 0.f && edge_place > 0 && (row.cut || row.last_id == 0x7fffffff)) {
-    // only positive logits of the window are kept: as signed numbers, what is below
-    // them reads the one bin before the border's, which holds 0, so lanes that keep
-    // nothing share an access
-    const uint32_t low2 = static_cast<uint32_t>(win.lo + edge_place - 1) * 0x10001u, lo2 = static_cast<uint32_t>(win.lo) * 0x10001u;
-    unsigned low = 0, high = 0;  // (at most 2^18 / 512 of 2^22 each)
-    sl.vectors(v_lo, v_hi, lane, 32, [&](const uint4& d, int) {
-      const uint32_t w[4] = {d.x, d.y, d.z, d.w};
-      if (row.cut) masks += equal(d);
+  const bool high_only =
+      sizeof(T) == 2 && plain && row.least > 0.f && edge_place > 0 && (row.cut || row.last_id == 0x7fffffff);
+  const uint32_t low2 = static_cast<uint32_t>(win.lo + edge_place - 1) * 0x10001u, lo2 = static_cast<uint32_t>(win.lo) * 0x10001u;
+  for (int g = 0, v0 = v_lo; v0 < v_hi; ++g, v0 += 32 * kGroup) {
+    u64 sum = 0;
+    uint32_t masks = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t at = (__vmaxs2(w[i], low2) - lo2) * 8u;
-        const uint2 a = *reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(sh.weights) + (at & 0xffffu));
-        const uint2 c = *reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(sh.weights) + (at >> 16));
-        low += a.x + c.x;
-        high += a.y + c.y;
+    for (int a0 = 0; a0 < kGroup; a0 += kAtOnce) {
+      uint4 d[kAtOnce];
+      const int v = v0 + a0 * 32 + lane;
+      if (v0 + (a0 + kAtOnce) * 32 <= v_hi) {
+#pragma unroll
+        for (int a = 0; a < kAtOnce; ++a) d[a] = sl.raw(v + a * 32);
+      } else {  // -inf behind the part
+        const unsigned none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+#pragma unroll
+        for (int a = 0; a < kAtOnce; ++a) d[a] = v + a * 32 < v_hi ? sl.raw(v + a * 32) : make_uint4(none, none, none, none);
       }
-    });
-    sum = low + (static_cast<u64>(high) << 22);
-  } else {
-    sl.vectors(v_lo, v_hi, lane, 32, [&](const uint4& d, int v) {
-      sum += sum_of(d, v);
-      if (sizeof(T) == 2 && row.cut) masks += equal(d);
-    });
-  }
-  sum = sm_sum(sum);
-  int ties = __reduce_add_sync(0xffffffffu, equals(masks));
-  __syncthreads();
-  if (lane == 0) {
-    sh.warp_lo[warp] = sum;
-    sh.warp_n[warp] = ties;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    const u64 all = sm_sum(lane < kSmWarps ? sh.warp_lo[lane] : 0ull);
-    ties = __reduce_add_sync(0xffffffffu, lane < kSmWarps ? sh.warp_n[lane] : 0);
-    if (lane < ranks) {
-      SmShared& o = *cl.map_shared_rank(&sh, lane);
-      o.sum_of[rank] = all;
-      o.zones_of[rank] = ties;
+      if (high_only) {
+        unsigned low = 0, high = 0;
+#pragma unroll
+        for (int a = 0; a < kAtOnce; ++a) {
+          const uint32_t w[4] = {d[a].x, d[a].y, d[a].z, d[a].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t at = (__vmaxs2(w[i], low2) - lo2) * 8u;
+            const uint2 e = *reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(sh.weights) + (at & 0xffffu));
+            const uint2 f = *reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(sh.weights) + (at >> 16));
+            low += e.x + f.x;
+            high += e.y + f.y;
+          }
+        }
+        sum += low + (static_cast<u64>(high) << 22);
+      } else {
+#pragma unroll
+        for (int a = 0; a < kAtOnce; ++a) {
+          sum += sum_of(d[a], v + a * 32);
+          __syncwarp();
+        }
+      }
+      if (sizeof(T) == 2 && row.cut) {
+#pragma unroll
+        for (int a = 0; a < kAtOnce; ++a) masks += equal(d[a]);
+      }
+    }
+    // (a lane's 32 weights: 49 bits)
+    const u64 low = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(sum) & 0x3ffffffu);
+    const u64 high = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(sum >> 26));
+    if (lane == 0) sh.group_sum[warp * kSmGroups + g] = low + (high << 26);
+    if (sizeof(T) == 2 && row.cut) {
+      const int ties = __reduce_add_sync(0xffffffffu, equals(masks));
+      if (lane == 0) sh.group_ties[warp * kSmGroups + g] = ties;
     }
   }
-  cl.sync();
-
-  // ---- the CTA, the warp and the token where the running sum passes u S; outside
-  // of [0, 1) there may be none: the last that is kept
-  int left = row.cut ? row.ties : 0;  // equal logits that are still to come
-  auto with_ties = [&](u64 sum, int n) {  // a part's sum, of the n equal logits in it those that are kept
-    const int k = min(n, left);
-    left -= k;
-    return sum + edge * static_cast<u64>(k);
-  };
-  u64 whole = 0;
-  for (int q = 0; q < ranks; ++q) whole += with_ties(sh.sum_of[q], sh.zones_of[q]);
-  const double part = u * static_cast<double>(whole);
-  const u64 goal = part >= static_cast<double>(whole) || part != part ? whole : part > 0.0 ? static_cast<u64>(part) : 0ull;
-  u64 before = 0;
-  int here = -1, left_here = 0;
-  auto pick = [&](int n, const u64* sums, const int* counts) {  // the first part that passes, or the last that holds any
-    u64 at = before;
-    here = -1;
-    for (int q = 0; q < n; ++q) {
-      const int had = left;
-      const u64 s = with_ties(sums[q], counts[q]);
-      if (s > 0) {
-        here = q;
-        before = at;
-        left_here = had;
-        if (at + s > goal) break;
-      }
-      at += s;
-    }
-    left = left_here;
-  };
-  left = row.cut ? row.ties : 0;
-  pick(ranks, sh.sum_of, sh.zones_of);
-  if (here != rank) return;
-  pick(kSmWarps, sh.warp_lo, sh.warp_n);
-  // that warp's vectors, neighbours for each thread
-  const int most = (per + kSmThreads - 1) / kSmThreads;
-  const int first = min(sl.vecs, here * per) + most * tid, end = min(sl.vecs, here * per + per);
-  u64 mine = 0;
+  __syncthreads();
+  const u64 group = tid < kSmWarps * kSmGroups ? sh.group_sum[tid] : 0ull;
+  const int group_ties = tid < kSmWarps * kSmGroups ? sh.group_ties[tid] : 0;
+  u64 mine;
   int own = 0;
-  for (int v = first; v < min(end, first + most); ++v) {
-    const uint4 d = sl.raw(v);
-    mine += sum_of(d, v);
-    if (sizeof(T) == 2 && row.cut) own += equals(equal(d));
+  SmSums<u64> sums = sm_scan(group, sh.warp_lo, mine);
+  SmSums<int> ties{0, 0};
+  if (row.cut) ties = sm_scan(group_ties, sh.warp_n, own);
+  if (tid < ranks) {
+    SmShared& o = sm_of<kWhole>(cl, sh, tid);
+    o.sum_of[rank] = mine;
+    o.zones_of[rank] = own;
   }
-  if (row.cut) {
-    int none;
-    const SmSums<int> counts = sm_scan(own, sh.warp_n, none);
-    left = max(0, left - counts.before);
-    mine += edge * static_cast<u64>(min(own, left));
+  sm_sync<kWhole>(cl);
+
+  // ---- the CTA, the group, the vector and the token where the running sum passes
+  // u S; for a u outside of [0, 1) the first or the last that is kept
+  u64 whole = 0;
+  int had = 0;  // equal logits before
+  auto kept_ties = [&](int n, int before) { return row.cut ? max(0, min(n, row.ties - before)) : 0; };
+  u64 before = 0;
+  int before_ties = 0;
+  for (int q = 0; q < ranks; ++q) {
+    if (q == rank) {
+      before = whole;
+      before_ties = had;
+    }
+    whole += sh.sum_of[q] + edge * static_cast<u64>(kept_ties(sh.zones_of[q], had));
+    had += sh.zones_of[q];
+  }
+  const double part = u * static_cast<double>(whole);
+  const u64 goal = part >= static_cast<double>(whole) || part != part ? whole - 1 : part > 0.0 ? min(static_cast<u64>(part), whole - 1) : 0ull;
+  const u64 here = mine + edge * static_cast<u64>(kept_ties(own, before_ties));
+  if (goal < before || goal - before >= here) return;
+  // of the threads' parts, in order, the one that holds the goal
+  auto choose = [&](u64 part, int n, SmSums<u64> sums, SmSums<int> ties) {
+    if (row.cut) {
+      part += edge * static_cast<u64>(kept_ties(n, before_ties + ties.before));
+      u64 all;
+      sums = sm_scan(part, sh.warp_lo, all);
+    }
+    if (before + sums.before <= goal && goal < before + sums.upto) {
+      sh.part = tid;
+      sh.part_before = before + sums.before;
+      sh.part_ties = before_ties + ties.before;
+    }
+    __syncthreads();
+    before = sh.part_before;
+    before_ties = sh.part_ties;
+    return sh.part;
+  };
+  const int at = choose(group, group_ties, sums, ties);
+  const int g_lo = min(sl.vecs, at / kSmGroups * per) + at % kSmGroups * 32 * kGroup;
+  const int g_hi = min(min(sl.vecs, (at / kSmGroups + 1) * per), g_lo + 32 * kGroup);
+  u64 vector = 0;
+  int vector_ties = 0;
+  if (g_lo + tid < g_hi) {
+    const uint4 d = sl.raw(g_lo + tid);
+    vector = sum_of(d, g_lo + tid);
+    if (sizeof(T) == 2 && row.cut) vector_ties = equals(equal(d));
   }
   u64 all;
-  const SmSums<u64> sums = sm_scan(mine, sh.warp_hi, all);
-  if (tid == 0) {
-    sh.pick = -1;
-    sh.listed = kSmThreads;
-  }
-  __syncthreads();
-  if (mine > 0) {
-    atomicMax(&sh.pick, tid);
-    if (before + sums.upto > goal) atomicMin(&sh.listed, tid);
-  }
-  __syncthreads();
-  const bool passed = sh.listed < kSmThreads;
-  const int who = passed ? sh.listed : sh.pick;
-  if (tid == who) {
-    sh.lo = before + sums.before;
-    sh.place_of[0] = left;
-  }
-  __syncthreads();
-  // that thread's logits, one a lane
+  int some_ties;
+  if (row.cut) ties = sm_scan(vector_ties, sh.warp_n, some_ties);
+  else sums = sm_scan(vector, sh.warp_lo, all);
+  const int v = g_lo + choose(vector, vector_ties, sums, ties);
   if (warp == 1 && lane == 0) sh.warp_d[0] = log(static_cast<double>(whole) * 0x1p-44);
-  if (warp == 0 && who >= 0) {
-    const int v0 = min(sl.vecs, here * per) + most * who;
-    u64 run = sh.lo;
-    int to_come = sh.place_of[0];
-    for (int e = lane; e - lane < most * VE; e += 32) {
-      const int v = v0 + e / VE, id = sl.id0 + v * VE + e % VE;
-      float x = -INFINITY;
-      if (v < min(end, v0 + most) && id >= 0 && id < p.V)
-        x = static_cast<float>(reinterpret_cast<const T*>(sl.data)[v * VE + e % VE]);
-      u64 w = row.keeps(x, id) ? sm_fixed(pow2_by(sh.powers, row.exponent(x)), row.min_weight) : 0ull;
-      const unsigned ties = __ballot_sync(0xffffffffu, row.cut && x == row.least);
-      if ((ties >> lane & 1u) && __popc(ties & ((1u << lane) - 1u)) < to_come) w = edge;
-      u64 upto = w;
+  if (warp == 0) {  // its logits, one a lane
+    const int id = sl.id0 + v * VE + lane;
+    float x = -INFINITY;
+    if (lane < VE && id >= 0 && id < p.V) x = static_cast<float>(reinterpret_cast<const T*>(sl.data)[v * VE + lane]);
+    u64 w = row.keeps(x, id) ? sm_fixed(pow2_by(sh.powers, row.exponent(x)), row.min_weight) : 0ull;
+    const unsigned equal_ones = __ballot_sync(0xffffffffu, row.cut && x == row.least);
+    if ((equal_ones >> lane & 1u) && before_ties + __popc(equal_ones & ((1u << lane) - 1u)) < row.ties) w = edge;
+    u64 upto = w;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 q = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += q;
-      }
-      // the first that passes, or the last
-      const unsigned kept = __ballot_sync(0xffffffffu, w > 0);
-      const unsigned over = __ballot_sync(0xffffffffu, w > 0 && run + upto > goal);
-      if (lane == (over ? __ffs(over) - 1 : 31 - __clz(kept))) {
-        p.tokens[r] = id;
-        sh.warp_d[1] = row.exponent(x) * 0.69314718055994530942;  // the weight itself, not its whole number
-      }
-      if (over) break;
-      run += __shfl_sync(0xffffffffu, upto, 31);
-      to_come = max(0, to_come - __popc(ties));
+    for (int o = 1; o < VE; o <<= 1) {
+      const u64 q = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += q;
+    }
+    if (lane < VE && before + upto - w <= goal && goal < before + upto) {
+      p.tokens[r] = id;
+      sh.warp_d[1] = row.exponent(x) * 0.69314718055994530942;  // the weight itself, not its whole number
     }
   }
   __syncthreads();
-  if (tid == 0 && who >= 0) p.logprob[r] = static_cast<float>(sh.warp_d[1] - sh.warp_d[0]);
+  if (tid == 0) p.logprob[r] = static_cast<float>(sh.warp_d[1] - sh.warp_d[0]);
 }
 
 template <typename T>

@@ -240,12 +240,12 @@ __device__ __forceinline__ void sm_sync(const cg::cluster_group& cl) {
   else cl.sync();
 }
 
-// The CTA's part of the row: a slice in shared memory, or (kWhole) the row itself.
-template <typename T, bool kWhole>
+// The CTA's part of the row, in shared memory or (kStream) where it is; kOne: all of it.
+template <typename T, bool kStream, bool kOne>
 struct SmSlice {
   static constexpr int VE = 16 / sizeof(T);
-  static constexpr bool kAlone = kWhole;  // a cluster of one CTA
-  static constexpr int kAhead = kWhole ? 4 : 1;  // vectors in flight per thread
+  static constexpr bool kAlone = kOne;
+  static constexpr int kAhead = kStream ? 4 : 1;  // vectors in flight per thread
   const uint4* data;
   int vecs;
   int id0;  // of the first element (a vector may begin before the row: -inf there)
@@ -265,7 +265,7 @@ struct SmSlice {
     return x.u;
   }
   __device__ __forceinline__ uint4 raw(int v) const {
-    if constexpr (kWhole) {
+    if constexpr (kStream) {
       if (static_cast<unsigned>(v - in_lo) < static_cast<unsigned>(in_n)) return __ldg(data + v);
       return fetch(data + v, id0 + v * VE, V);
     }
@@ -817,7 +817,7 @@ template <typename T>
 __device__ __forceinline__ u64 sm_weigh_here(const uint4& d, int id, const SmRow& row, const double* powers) {
   constexpr int VE = 16 / sizeof(T);
   float e[VE];
-  SmSlice<T, false>::unpack(d, e);
+  SmSlice<T, false, false>::unpack(d, e);
   u64 sum = 0;
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
@@ -835,18 +835,18 @@ __device__ __forceinline__ u64 sm_weigh(const uint4& d, int id, const SmRow& row
   else return sm_weigh_here<T>(d, id, row, powers);
 }
 
-// Grid: kWhole a CTA per row, else a cluster per row.
-template <typename T, bool kWhole>
+// Grid: a CTA (kAlone) or a cluster per row.
+template <typename T, bool kStream, bool kAlone>
 __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __grid_constant__ SmParams p) {
-  using Slice = SmSlice<T, kWhole>;
+  using Slice = SmSlice<T, kStream, kAlone>;
   constexpr int VE = Slice::VE;
   extern __shared__ __align__(16) uint8_t sm_raw[];
   __shared__ __align__(16) SmShared sh;
   const cg::cluster_group cl = cg::this_cluster();
-  const int ranks = kWhole ? 1 : cl.num_blocks(), rank = kWhole ? 0 : cl.block_rank();
+  const int ranks = kAlone ? 1 : cl.num_blocks(), rank = kAlone ? 0 : cl.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long r = blockIdx.x / ranks;
-  if (!kWhole) cl.barrier_arrive();  // no CTA is written to before it runs
+  if (!kAlone) cl.barrier_arrive();  // no CTA is written to before it runs
   if (tid < 64) sh.powers[tid] = pow2(tid * (1.0 / 64));
   pdl_launch_dependents();
   pdl_wait();
@@ -861,12 +861,12 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   sl.vecs = min(p.slice, max(0, p.V - sl.id0) + VE - 1) / VE;
   sl.in_lo = mis > 0;
   sl.in_n = max(0, (p.V - sl.id0) / VE - sl.in_lo);
-  if constexpr (kWhole) {
-    sl.data = row0;
+  const uint4* const from = row0 + rank * (p.slice / VE);
+  if constexpr (kStream) {
+    sl.data = from;
   } else {
     uint4* const data = reinterpret_cast<uint4*>(sm_raw);
     sl.data = data;
-    const uint4* const from = row0 + rank * (p.slice / VE);
     for (int v = tid; v < sl.vecs; v += kSmThreads) {
       const int id = sl.id0 + v * VE;
       if (id >= 0 && id + VE <= p.V) cp_async_16(smem_u32(data + v), from + v, 16);
@@ -879,7 +879,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   const double top_p = p.top_p ? static_cast<double>(p.top_p[r]) : p.top_p_all;
   const double min_p = p.min_p ? static_cast<double>(p.min_p[r]) : p.min_p_all;
   const double u = p.u_f64 ? static_cast<const double*>(p.u)[r] : static_cast<double>(static_cast<const float*>(p.u)[r]);
-  if constexpr (!kWhole) asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if constexpr (!kStream) asm volatile("cp.async.wait_group 0;" ::: "memory");
 
   // ---- the largest logit (a NaN comes through), and of bf16 the smallest
   float mx = -INFINITY, mn = INFINITY;
@@ -892,22 +892,27 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
       high = max_nan_bf16x2(high, max_nan_bf16x2(max_nan_bf16x2(d.x, d.y), max_nan_bf16x2(d.z, d.w)));
       low = min_bf16x2(low, min_bf16x2(min_bf16x2(d.x, d.y), min_bf16x2(d.z, d.w)));
     };
-    if (kWhole && (by_k || by_p) && temperature > 0.0 && top_k != 1) {
-      // counts in the same pass, for magnitudes up to four times what a sample shows;
-      // where that was too little they are counted again
-      const uint4 d = sl.raw(static_cast<int>(static_cast<long long>(sl.vecs) * tid / kSmThreads));
-      unsigned most = 0;
+    if (kStream && (by_k || by_p) && temperature > 0.0 && top_k != 1) {
+      // counts in the same pass, for magnitudes up to four times what a sample of the
+      // row shows, and where it shows -inf for all that weigh something; where that was
+      // too little they are counted again
+      const int v = static_cast<int>(static_cast<long long>((p.V + mis + VE - 1) / VE) * tid / kSmThreads);
+      const uint4 d = Slice::fetch(row0 + v, v * VE - mis, p.V);
+      int most = 0;
+      bool masked = false;
       const uint32_t w[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const unsigned a = w[i] & 0x7fffu, c = w[i] >> 16 & 0x7fffu;
-        most = max(most, max(a < 0x7f80u ? a : 0u, c < 0x7f80u ? c : 0u));
+      for (int i = 0; i < 8; ++i) {
+        const int a = static_cast<int>(w[i >> 1] >> (16 * (i & 1)) & 0x7fffu);
+        masked = masked || a == 0x7f80;
+        if (a < 0x7f80) most = max(most, a);
       }
+      if (masked) most = max(most, static_cast<int>(__float_as_uint(fminf(static_cast<float>(64.0 * temperature) * 0.6932f, 1e38f)) >> 16) - 255);
       most = __reduce_max_sync(0xffffffffu, most);
-      if (lane == 0) sh.warp_n[warp] = static_cast<int>(most);
+      if (lane == 0) sh.warp_n[warp] = most;
       sm_clear(sh);
-      most = __reduce_max_sync(0xffffffffu, lane < kSmWarps ? static_cast<unsigned>(sh.warp_n[lane]) : 0u);
-      win.lo = max(0, min(static_cast<int>(most) + 256, 0x7f7f) - kSmValues + 1);
+      most = __reduce_max_sync(0xffffffffu, lane < kSmWarps ? sh.warp_n[lane] : 0);
+      win.lo = max(0, min(most + 256, 0x7f7f) - kSmValues + 1);
       sl.vectors(0, sl.vecs, tid, kSmThreads, [&](const uint4& u, int) {
         look(u);
         sm_count(sh, win, u);
@@ -940,18 +945,18 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     sh.warp_g[warp] = mn;
   }
   __syncthreads();
-  if (!kWhole) cl.barrier_wait();
+  if (!kAlone) cl.barrier_wait();
   if (warp == 0) {
     mx = lane < kSmWarps ? sh.warp_f[lane] : -INFINITY;
     mn = lane < kSmWarps ? sh.warp_g[lane] : INFINITY;
     join();
     if (lane < ranks) {
-      SmShared& o = sm_of<kWhole>(cl, sh, lane);
+      SmShared& o = sm_of<kAlone>(cl, sh, lane);
       o.max_of[rank] = mx;
       o.min_of[rank] = mn;
     }
   }
-  sm_sync<kWhole>(cl);
+  sm_sync<kAlone>(cl);
   mx = -INFINITY;
   mn = INFINITY;
   for (int q = 0; q < ranks; ++q) {
@@ -980,9 +985,9 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     __syncthreads();
     if (warp == 0) {
       id = __reduce_min_sync(0xffffffffu, lane < kSmWarps ? sh.warp_n[lane] : 0x7fffffff);
-      if (lane == 0) sm_of<kWhole>(cl, sh, 0).count_of[rank] = id;
+      if (lane == 0) sm_of<kAlone>(cl, sh, 0).count_of[rank] = id;
     }
-    sm_sync<kWhole>(cl);
+    sm_sync<kAlone>(cl);
     if (rank == 0 && tid == 0) {
       for (int q = 0; q < ranks; ++q) id = min(id, sh.count_of[q]);
       p.tokens[r] = id;
@@ -1099,10 +1104,10 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     const uint32_t a = -masks & 0xffffu;
     return static_cast<int>(a + ((a - ((masks + a) >> 16)) & 0xffffu));
   };
-  constexpr int kGroup = kWhole ? 32 / VE : 1;  // vectors of a lane in a group
-  constexpr int kAtOnce = kWhole ? 4 : 1;
+  constexpr int kGroup = kStream ? 32 / VE : 1;  // vectors of a lane in a group
+  constexpr int kAtOnce = kStream ? 4 : 1;
   constexpr int kSliceVecs = kSmMaxVocab / VE / kSmCluster + 1 > kSmSlice / 16 ? kSmMaxVocab / VE / kSmCluster + 1 : kSmSlice / 16;
-  constexpr int kMostVecs = kWhole ? kSmMaxVocab / VE + 1 : kSliceVecs;
+  constexpr int kMostVecs = kStream ? kSmMaxVocab / VE + 1 : kSliceVecs;
   static_assert((kMostVecs + kSmWarps - 1) / kSmWarps <= kSmGroups * 32 * kGroup && kSmWarps * kSmGroups <= kSmThreads, "groups");
   const int per = (sl.vecs + kSmWarps - 1) / kSmWarps;
   const int v_lo = min(sl.vecs, warp * per), v_hi = min(sl.vecs, v_lo + per);
@@ -1178,11 +1183,11 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   SmSums<int> ties{0, 0};
   if (row.cut) ties = sm_scan(group_ties, sh.warp_n, own);
   if (tid < ranks) {
-    SmShared& o = sm_of<kWhole>(cl, sh, tid);
+    SmShared& o = sm_of<kAlone>(cl, sh, tid);
     o.sum_of[rank] = mine;
     o.zones_of[rank] = own;
   }
-  sm_sync<kWhole>(cl);
+  sm_sync<kAlone>(cl);
 
   // ---- the CTA, the group, the vector and the token where the running sum passes
   // u S; for a u outside of [0, 1) the first or the last that is kept
@@ -1263,16 +1268,21 @@ cudaError_t sm_launch(const SmParams& params, long long rows, cudaStream_t s) {
   constexpr int VE = 16 / sizeof(T);
   SmParams p = params;
   const long long vecs = (static_cast<long long>(p.V) + VE - 1 + VE - 1) / VE;  // a row may begin inside a vector
-  // rows enough for two on every SM: a CTA each
-  const bool whole = rows >= kSmWholeRows;
-  // else as few CTAs per row as hold it at two per SM; more where rows are few
+  // as few CTAs per row as hold it at two per SM; more where rows are few
   int ranks = 1;
-  while (!whole && ranks < kSmCluster && ((vecs + ranks - 1) / ranks) * 16 > kSmSlice) ranks *= 2;
-  while (!whole && ranks < kSmCluster && rows * ranks < device_sm_count() && vecs > 64 * ranks) ranks *= 2;
+  while (ranks < kSmCluster && ((vecs + ranks - 1) / ranks) * 16 > kSmSlice) ranks *= 2;
+  while (ranks < kSmCluster && rows * ranks < device_sm_count() && vecs > 64 * ranks) ranks *= 2;
+  // where they do not all run at once, rows stay where they are, with as many CTAs as do;
+  // a CTA each where that is all there is room for
+  const long long room = 2 * device_sm_count();
+  const bool stream = rows * ranks > room || rows >= kSmWholeRows;
+  if (stream) ranks = kSmCluster;
+  while (stream && ranks > 1 && rows * ranks > room) ranks /= 2;
+  const bool alone = stream && ranks == 1;
   p.slice = static_cast<int>((vecs + ranks - 1) / ranks) * VE;
-  const size_t smem = whole ? 0 : static_cast<size_t>(p.slice) * sizeof(T);
+  const size_t smem = stream ? 0 : static_cast<size_t>(p.slice) * sizeof(T);
   constexpr int kMost = kSmMaxVocab * sizeof(T) / kSmCluster;
-  cudaError_t e = allow_smem<sample_tokens_kernel<T, false>>((kMost > kSmSlice ? kMost : kSmSlice) + 64);
+  cudaError_t e = allow_smem<sample_tokens_kernel<T, false, false>>((kMost > kSmSlice ? kMost : kSmSlice) + 64);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * ranks));
@@ -1288,8 +1298,9 @@ cudaError_t sm_launch(const SmParams& params, long long rows, cudaStream_t s) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  return whole ? cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T, true>, p)
-               : cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T, false>, p);
+  if (alone) return cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T, true, true>, p);
+  if (stream) return cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T, true, false>, p);
+  return cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T, false, false>, p);
 }
 
 }  // namespace

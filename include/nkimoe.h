@@ -342,7 +342,8 @@ NKIMOE_API int nkimoe_accept_drafts(const int64_t* tokens, const int64_t* sample
  * equal ones, logprob 0.  Each setting is a device array with an entry per row,
  * or, where that is NULL, the one value after it.  In arrays a top_k below 1, a
  * top_p that is not below 1 and a min_p that is not above 0 restrict nothing.
- * Weights and sums are fp64.  A logit of -inf is never drawn; a row with a NaN,
+ * Weights are formed in fp64 and the drawn sum adds whole numbers of 2^-44 of
+ * the largest, in any order the same.  A logit of -inf is never drawn; a row with a NaN,
  * a +inf, nothing but -inf, or a negative or NaN temperature has no
  * distribution: token -1, logprob NaN.
  * No reference counterpart (sampling is its runtime's). */

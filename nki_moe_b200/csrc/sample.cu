@@ -10,13 +10,14 @@
 // The random number u is the caller's.  Which token comes out depends on sums
 // over up to V weights next to a border, so the sums have to be better than
 // fp32: a border lies within 2^-24 S of u S for one row in a hundred when 10^5
-// tokens are kept.  Weights and sums are fp64; where the order of addition
-// would depend on timing (histograms) they are added as integers.
+// tokens are kept.  Weights are formed in fp64.  The draw adds them up as whole
+// numbers of 2^-44 of the largest, histograms of weights as whole numbers too, so
+// that no order of addition, by threads or by atomics, changes a token.
 //
 // Few rows: a cluster of CTAs holds a row in shared memory, each a slice, so that
-// all SMs work on them.  Many rows: a CTA takes a whole row, from the L2 after its
-// first pass, so that nothing waits for other CTAs.  What top_k and top_p keep is
-// found from histograms:
+// all SMs work on them.  Rows whose slices do not all run at once stay in global
+// memory (from the L2 after the first pass), with as many CTAs each as do.  What top_k and
+// top_p keep is found from histograms:
 //
 //   bf16  of the values themselves.  Of each sign the 2048 values of the 16 binary
 //         orders below the largest magnitude that matters have a bin, so counts
@@ -27,6 +28,14 @@
 //         counts or of weights; the border's bin is sorted by the cluster's first
 //         CTA, or, with more tokens than that takes, split further by its own
 //         smallest and largest (logit, id).
+//
+// Bounds and figures (B200, 151936 logits a row, device time): 8 bf16 rows with top-k
+// and top-p 20 us, a chain of some 20 barriers of a cluster; 1024 rows with top-p 209 us
+// (1.5 TB/s of 6.5): an SM has two rows at a time and 3.46 rounds of them, of 60 us a
+// row 25 go to the counting pass (7 operations and a shared atomic a logit, whose banks
+// conflict 3.3 times), 12 to the borders and the table of weights, 16 to the sums and 6
+// to the draw.  fp32 with top-p, 290 rows: 300 us, 14 operations in 64 bits per logit
+// and pass; without filters 113, with min-p alone 74.
 //
 // Reference: the sampling of the reference's runtime is not vendored; no
 // kernel of its own.
@@ -48,13 +57,14 @@ constexpr int kSmBins = 1024;
 constexpr int kSmBinsPerOctave = 32;
 constexpr int kSmList = 2048;        // tokens that the last sort takes
 constexpr int kSmCluster = 8;        // CTAs per row at most
-constexpr int kSmSlice = 76 * 1024;  // bytes of a row per CTA that two CTAs per SM leave room for
+constexpr int kSmSlice = 75 * 1024;  // bytes of a row per CTA that two CTAs per SM leave room for
 constexpr int kSmWholeRows = 148;    // rows from which on a CTA takes a whole one
 constexpr int kSmValues = 2048;      // values of a sign that have a bin
 constexpr int kSmNear = 512;         // logits nearer to zero that a CTA sums
 constexpr int kSmMaxVocab = 1 << 18;
 constexpr int kSmGroups = 17;        // groups of vectors in a warp's part
 static_assert(2 * kSmThreads == kSmBins, "two bins per thread");
+static_assert(2 * (kSmSlice + 39 * 1024) <= 228 * 1024, "two CTAs, with 39 KB of SmShared and the system's each");
 
 using u64 = unsigned long long;
 
@@ -1272,10 +1282,13 @@ cudaError_t sm_launch(const SmParams& params, long long rows, cudaStream_t s) {
   int ranks = 1;
   while (ranks < kSmCluster && ((vecs + ranks - 1) / ranks) * 16 > kSmSlice) ranks *= 2;
   while (ranks < kSmCluster && rows * ranks < device_sm_count() && vecs > 64 * ranks) ranks *= 2;
-  // where they do not all run at once, rows stay where they are, with as many CTAs as do;
-  // a CTA each where that is all there is room for
+  // where they do not all run at once, rows stay where they are, with as many CTAs as do:
+  // 100 rows of 151936 bf16 with top-p take 46 us so, as slices of four CTAs each, in two
+  // rounds, 58; 70 rows, whose slices fit, 33 us as slices
   const long long room = 2 * device_sm_count();
-  const bool stream = rows * ranks > room || rows >= kSmWholeRows;
+  // (bf16 rows of 18000 with filters, 150 of them: 23.1 us, as slices 25.7; fp32 rows of 500: 11.3
+  // and 6.6 us, of 18000 20.2 and 17.3)
+  const bool stream = rows * ranks > room || (sizeof(T) == 2 && rows >= kSmWholeRows);
   if (stream) ranks = kSmCluster;
   while (stream && ranks > 1 && rows * ranks > room) ranks /= 2;
   const bool alone = stream && ranks == 1;

@@ -34,8 +34,8 @@
 // (1.5 TB/s of 6.5): an SM has two rows at a time and 3.46 rounds of them, of 60 us a
 // row 25 go to the counting pass (7 operations and a shared atomic a logit, whose banks
 // conflict 3.3 times), 12 to the borders and the table of weights, 16 to the sums and 6
-// to the draw.  fp32 with top-p, 290 rows: 300 us, 14 operations in 64 bits per logit
-// and pass; without filters 113, with min-p alone 74.
+// to the draw.  fp32 with top-p, 290 rows: 284 us, 14 operations in 64 bits per logit
+// and pass; without filters 119, with min-p alone 62.
 //
 // Reference: the sampling of the reference's runtime is not vendored; no
 // kernel of its own.
@@ -63,6 +63,7 @@ constexpr int kSmValues = 2048;      // values of a sign that have a bin
 constexpr int kSmNear = 512;         // logits nearer to zero that a CTA sums
 constexpr int kSmMaxVocab = 1 << 18;
 constexpr int kSmGroups = 17;        // groups of vectors in a warp's part
+constexpr int kSmFew = 48;           // kept logits of a warp's 32 vectors that are set aside
 static_assert(2 * kSmThreads == kSmBins, "two bins per thread");
 static_assert(2 * (kSmSlice + 39 * 1024) <= 228 * 1024, "two CTAs, with 39 KB of SmShared and the system's each");
 
@@ -123,6 +124,7 @@ struct SmShared {
     u64 list[kSmList];
     unsigned values[2 * kSmValues];  // counts by magnitude, then of negative values
     uint2 weights[2 * kSmValues];    // as the counts: a weight's low 22 bits, and the others
+    float kept[kSmWarps][32 + kSmFew];  // logits of each warp that wait for their weights
   };
 };
 
@@ -1133,6 +1135,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
   const bool high_only =
       sizeof(T) == 2 && plain && row.least > 0.f && edge_place > 0 && (row.cut || row.last_id == 0x7fffffff);
   const uint32_t low2 = static_cast<uint32_t>(win.lo + edge_place - 1) * 0x10001u, lo2 = static_cast<uint32_t>(win.lo) * 0x10001u;
+  auto weigh = [&](float x) { return sm_fixed(pow2_by(sh.powers, row.exponent(x)), row.min_weight); };
+  int waiting = 0;  // of this warp's logits in sh.kept (fp32 only)
   for (int g = 0, v0 = v_lo; v0 < v_hi; ++g, v0 += 32 * kGroup) {
     u64 sum = 0;
     uint32_t masks = 0;
@@ -1163,10 +1167,44 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
           }
         }
         sum += low + (static_cast<u64>(high) << 22);
-      } else {
+      } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int a = 0; a < kAtOnce; ++a) {
           sum += sum_of(d[a], v + a * 32);
+          __syncwarp();
+        }
+      } else {
+        // a weight is a chain of 600 cycles: where a warp's vectors keep few, 32 of
+        // them are weighed at a time (257 rows with min-p 21 us, and 26 one vector at a time, the
+        // row that keeps most being what the others wait for)
+#pragma unroll
+        for (int a = 0; a < kAtOnce; ++a) {
+          if (!__any_sync(0xffffffffu, some(d[a]))) continue;
+          float e[VE];
+          Slice::unpack(d[a], e);
+          unsigned who[VE];
+          int n = row.least > -INFINITY ? 0 : 32 * VE;  // (nothing is cut: hardly few)
+          if (n == 0) {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+              who[i] = __ballot_sync(0xffffffffu, row.keeps(e[i], sl.id0 + (v + a * 32) * VE + i));
+              n += __popc(who[i]);
+            }
+          }
+          if (n > kSmFew) {
+            sum += sm_weigh<T>(d[a], sl.id0 + (v + a * 32) * VE, row, sh.powers);
+            continue;
+          }
+#pragma unroll
+          for (int i = 0; i < VE; ++i) {
+            if (who[i] >> lane & 1u) sh.kept[warp][waiting + __popc(who[i] & ((1u << lane) - 1u))] = e[i];
+            waiting += __popc(who[i]);
+          }
+          __syncwarp();
+          while (waiting >= 32) {
+            waiting -= 32;
+            sum += weigh(sh.kept[warp][waiting + lane]);
+          }
           __syncwarp();
         }
       }
@@ -1175,7 +1213,12 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
         for (int a = 0; a < kAtOnce; ++a) masks += equal(d[a]);
       }
     }
-    // (a lane's 32 weights: 49 bits)
+    if (sizeof(T) == 4 && waiting > 0) {
+      if (lane < waiting) sum += weigh(sh.kept[warp][lane]);
+      waiting = 0;
+      __syncwarp();
+    }
+    // (a lane's weights, 32 or at most 48 in all lanes more: 50 bits)
     const u64 low = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(sum) & 0x3ffffffu);
     const u64 high = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(sum >> 26));
     if (lane == 0) sh.group_sum[warp * kSmGroups + g] = low + (high << 26);

@@ -115,6 +115,24 @@ def test_rows_enough_for_wide_slices(rows, vocab, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", [(300, 50257), (310, 1027), (120, 151937)])
+def test_rows_that_keep_few_or_many(rows, vocab, dtype):
+    """Few kept logits of a warp's vectors are weighed together, many one by one; both in one row."""
+    x, u = logits_of(rows, vocab, 3 * rows, dtype)
+    x[::3, vocab // 2:vocab // 2 + 700] = x[::3].float().amax(1, keepdim=True).to(dtype) - 1.5
+    x[1::3] *= 0.25
+    x, u = x.cuda(), u.cuda()
+    for s in (dict(min_p=0.05), dict(min_p=1e-5, temperature=1.5), dict(top_k=900, min_p=0.01), dict(top_p=0.4)):
+        tok, lp = ops.sample_tokens(x, u, **s)
+        for i in [*range(0, rows, 23), rows - 1]:
+            want, want_lp, margin = drawn(x[i].cpu(), u[i].item(), s.get("temperature", 1.0), s.get("top_k", 0),
+                                          s.get("top_p", 1.0), s.get("min_p", 0.0))
+            if margin > 2 ** -31:
+                assert int(tok[i]) == want, (s, i)
+                assert abs(float(lp[i]) - want_lp) <= 2 ** -24 * abs(want_lp) + vocab * 2 ** -45 + 1e-12
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("values", [[0.0], [1.5, -0.25], [3.0, 2.984375, -40.0]])
 @pytest.mark.parametrize("s", [dict(), dict(k=777), dict(k=70001), dict(p=0.31), dict(k=9000, p=0.77), dict(t=0.2, p=0.999)])
 def test_equal_logits_go_by_id(values, dtype, s):

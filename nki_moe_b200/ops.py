@@ -590,18 +590,20 @@ def paged_tree_attention(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: to
     row = (n_heads + 2 * n_kv_heads) * 128
     if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != row or not qkv.is_contiguous():
         raise ValueError(f"qkv must be a contiguous bf16 [T, {row}] tensor")
-    T, dev = qkv.shape[0], qkv.device
-    _node_ids(parents, "parents", torch.int32, T, dev.index)
+    T, dev = qkv.shape[0], qkv.get_device()
+    _node_ids(parents, "parents", torch.int32, T, dev)
     B = _lengths(cu_seqlens, kv_lens)
     qw, kw, wdt = _norm_weights(q_weight, k_weight)
     cache = _paged_cache(k_pages, v_pages, page_table, n_kv_heads, B)
-    _same_device(dev.index, "q_weight k_weight cu_seqlens kv_lens k_pages v_pages page_table", qw, kw, cu_seqlens,
-                 kv_lens, k_pages, v_pages, page_table)
-    out = _rows_out(out, (T, n_heads * 128), qkv)
-    s = _raw_stream(dev.index)
-    nbytes = _paged_ws_bytes(dev.index, "nkimoe_paged_tree_attention_workspace_bytes", T, B, n_heads, n_kv_heads,
+    if not (dev == qw.get_device() == kw.get_device() == cu_seqlens.get_device() == kv_lens.get_device()
+            == k_pages.get_device() == v_pages.get_device() == page_table.get_device()):
+        _same_device(dev, "q_weight k_weight cu_seqlens kv_lens k_pages v_pages page_table", qw, kw, cu_seqlens,
+                     kv_lens, k_pages, v_pages, page_table)
+    out = qkv.new_empty((T, n_heads * 128)) if out is None else _rows_out(out, (T, n_heads * 128), qkv)
+    s = _raw_stream(dev)
+    nbytes = _paged_ws_bytes(dev, "nkimoe_paged_tree_attention_workspace_bytes", T, B, n_heads, n_kv_heads,
                              cache[8], cache[5])
-    ws = _paged_workspace(dev, s, nbytes)
+    ws = _paged_workspace(qkv.device, s, nbytes)
     call("nkimoe_paged_tree_attention", qkv.data_ptr(), qw.data_ptr(), kw.data_ptr(), wdt, parents.data_ptr(),
          cu_seqlens.data_ptr(), kv_lens.data_ptr(), *cache, out.data_ptr(), T, B, n_heads, n_kv_heads, 128, theta, eps,
          128 ** -0.5 if scale is None else scale, window, sinks, ws.data_ptr(), ws.numel(), s)

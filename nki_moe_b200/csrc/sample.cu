@@ -58,7 +58,7 @@ constexpr int kSmBinsPerOctave = 32;
 constexpr int kSmList = 2048;        // tokens that the last sort takes
 constexpr int kSmCluster = 8;        // CTAs per row at most
 constexpr int kSmSlice = 75 * 1024;  // bytes of a row per CTA that two CTAs per SM leave room for
-constexpr int kSmWholeRows = 148;    // rows from which on a CTA takes a whole one
+constexpr int kSmWholeRows = 148;    // bf16 rows that stay in global memory even where slices would fit
 constexpr int kSmValues = 2048;      // values of a sign that have a bin
 constexpr int kSmNear = 512;         // logits nearer to zero that a CTA sums
 constexpr int kSmMaxVocab = 1 << 18;

@@ -52,9 +52,10 @@ __global__ void __launch_bounds__(kAcThreads) accept_drafts_kernel(const __grid_
   pdl_launch_dependents();
   pdl_wait();
   if (threadIdx.x < 32) {
-    const int lo = p.cu[b], hi = p.cu[b + 1], kv = p.kv_lens[b], n = hi - lo;
-    const bool valid = lo >= 0 && n >= 0 && hi <= p.T && n <= kTreeNodes && kv >= n &&
-                       kv <= static_cast<long long>(p.max_pages) * p.page_size;
+    const int lo = p.cu[b], hi = p.cu[b + 1], kv = p.kv_lens[b];
+    const bool rows = lo >= 0 && hi >= lo && hi <= p.T;
+    const int n = rows ? hi - lo : 0;  // (the difference of two that make no sense may pass 32 bits)
+    const bool valid = rows && n <= kTreeNodes && kv >= n && kv <= static_cast<long long>(p.max_pages) * p.page_size;
     int count = 0;
     if (valid && n > 0) {
       int par[2];

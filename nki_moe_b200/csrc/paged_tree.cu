@@ -117,15 +117,16 @@ __device__ __forceinline__ TrSeq tr_sequence(const TrParams& p, int b, bool flag
   TrSeq s{0, 0, 0, 0};
   if (b >= p.B) return s;
   s.row0 = p.cu[b];
-  s.n = p.cu[b + 1] - s.row0;
   s.kv = p.kv_lens[b];
-  if (s.n == 0) return s;
-  if (s.row0 < 0 || s.n < 0 || s.row0 + s.n > p.T || s.n > kTreeNodes || s.kv < s.n ||
+  const int end = p.cu[b + 1];
+  if (s.row0 == end) return s;
+  // (the order first: the difference of two that make no sense may pass 32 bits)
+  if (s.row0 < 0 || end < s.row0 || end > p.T || end - s.row0 > kTreeNodes || s.kv < end - s.row0 ||
       s.kv > static_cast<long long>(p.c.max_pages) << p.c.page_shift) {
     if (flag) atomicOr(p.status, kDevErrBadIndex);
-    s.n = 0;
     return s;
   }
+  s.n = end - s.row0;
   s.blocks = blocks_of(s.kv - s.n, s.kv - 1, p.window, p.sinks).n;
   return s;
 }

@@ -109,11 +109,17 @@ __global__ void __launch_bounds__(kAcThreads) accept_drafts_kernel(const __grid_
       s_count = count;
       if (blockIdx.x == 0) p.counts[b] = count;
     }
-    if (blockIdx.x == 0 && b == p.B - 1 && hi >= 0)  // rows of no sequence
-      for (long long i = hi + lane; i < p.T; i += 32) {
-        p.path[i] = -1;
-        p.new_tokens[i] = -1;
-      }
+    if (blockIdx.x == 0) {  // rows without a path: of a refused sequence, of none before the first or behind the last
+      auto none = [&](long long from, long long end) {
+        for (long long i = max(from, 0LL) + lane; i < min(end, p.T); i += 32) {
+          p.path[i] = -1;
+          p.new_tokens[i] = -1;
+        }
+      };
+      if (!valid) none(lo, hi);
+      if (b == 0) none(0, lo);
+      if (b == p.B - 1) none(hi, p.T);
+    }
   }
   __syncthreads();
   const int count = s_count;

@@ -1,5 +1,5 @@
-"""Lengths that make no sense at the ends of their type's range, in the calls of drafted
-decoding: they are reported, and nothing outside of what was given is read or written."""
+"""Lengths that make no sense in the calls of drafted decoding: they are reported, nothing outside
+of what was given is read or written, and what is documented for the others holds."""
 
 import pytest
 import torch
@@ -78,3 +78,44 @@ def test_lengths_at_the_ends_of_the_type(length, monkeypatch):
     counts, _, _ = ops.accept_drafts(*dev)
     reported()
     assert counts.tolist() == [0, int(want[0][1])]
+
+
+def recycled(T):
+    """Leaves a block of 7s behind, of the size that the next outputs take."""
+    for dtype in (torch.int32, torch.int64):
+        blocks = [torch.full((T,), 7, dtype=dtype, device="cuda") for _ in range(4)]
+        del blocks
+
+
+@pytest.mark.parametrize("starts,lens,paths", [
+    ([0, 65, 69], [70, 20], {1: [65, 66, 67, 68]}),  # more nodes than a tree has
+    ([0, 4, 8], [3, 20], {1: [4, 5, 6, 7]}),  # a cache shorter than the tree
+    ([0, 4, 8], [20, 10 ** 6], {0: [0, 1, 2, 3]}),
+    ([5, 9, 9, 12], [20, 0, 20], {0: [5, 6, 7, 8], 2: [9, 10, 11]}),  # rows before the first
+    ([-3, 4, 8], [20, 20], {1: [4, 5, 6, 7]}),
+    ([3, 7, 10 ** 9], [20, 20], {0: [3, 4, 5, 6]}),
+    ([6, 2], [20], {}),
+    ([-8, -4], [20], {}),
+    ([100, 104], [20], {}),
+])
+def test_rows_without_a_path_are_minus_one(starts, lens, paths, monkeypatch):
+    """Of refused sequences, and of none."""
+    monkeypatch.setenv("NKIMOE_SYNC_CHECK", "0")
+    T, B = 80, len(lens)
+    token = torch.ones(T, dtype=torch.int64, device="cuda")
+    parents = torch.full((T,), -1, dtype=torch.int32)
+    for rows in paths.values():
+        parents[rows] = torch.arange(-1, len(rows) - 1, dtype=torch.int32)  # chains that are agreed with
+    pages = torch.zeros(2, 5 * B, 1, 16, 8, dtype=torch.bfloat16, device="cuda")
+    table = torch.arange(5 * B, dtype=torch.int32, device="cuda").view(B, 5)
+    want = torch.full((T,), -1, dtype=torch.int32)
+    for rows in paths.values():
+        want[rows] = torch.arange(len(rows), dtype=torch.int32)
+    recycled(T)
+    counts, path, new = ops.accept_drafts(token, token, parents.cuda(), ints(*starts), ints(*lens), pages, table)
+    refused = [b for b in range(B) if b not in paths and starts[b] != starts[b + 1]]
+    if refused:
+        reported()
+    assert counts.tolist() == [len(paths.get(b, [])) for b in range(B)]
+    assert torch.equal(path.cpu(), want)
+    assert torch.equal(new.cpu(), torch.where(want >= 0, 1, -1))

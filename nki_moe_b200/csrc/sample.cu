@@ -505,13 +505,17 @@ __device__ void sm_select(const cg::cluster_group& cl, SmShared& sh, const Slice
             }
             __syncthreads();
           }
-        // in order until the border is reached
+        // in order until the border is reached.  Weights are formed relative to the
+        // list's largest, as the histogram's are to their bin's: pow2_by gives 0 below
+        // 2^-60, where a top_p just below 1 may have its border
         constexpr int kEach = kSmList / kSmThreads;
+        auto listed = [&](int i) { return row.exponent(falling_value(static_cast<unsigned>(sh.list[i] >> 32))); };
+        const double most = kMass ? listed(0) : 0.0, unit = kMass ? pow2(most) : 1.0;
         double v[kEach], sum = 0.0;
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
           const int i = tid * kEach + e;
-          v[e] = i >= n ? 0.0 : kMass ? pow2_by(sh.powers, row.exponent(falling_value(static_cast<unsigned>(sh.list[i] >> 32)))) : 1.0;
+          v[e] = i >= n ? 0.0 : kMass ? pow2_by(sh.powers, listed(i) - most) * unit : 1.0;
           sum += v[e];
         }
         double total;
@@ -635,7 +639,7 @@ __device__ __forceinline__ void sm_clear(SmShared& sh) {
 // The border of top_k (0: none) and top_p (1: none) among bf16 logits, into what
 // row keeps.  In order stand the positive values, the zone (what is nearer to zero
 // than the window), the negative ones; each CTA of the cluster has a share of the
-// bins.  Weights below 2^-64 count as 0.  `counted`: sh.values holds the counts
+// bins.  Weights below 2^-60 count as 0 (pow2_by).  `counted`: sh.values holds the counts
 // already.  All CTAs of the cluster call it and take the same way through it; false:
 // the border lies in the zone and has to be searched.
 template <typename Slice>

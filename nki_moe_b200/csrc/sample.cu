@@ -226,7 +226,9 @@ struct SmRow {
     least = falling_value(static_cast<unsigned>(border >> 32));
     last_id = static_cast<int>(border & 0xffffffffu);
   }
-  __device__ __forceinline__ double exponent(float x) const { return (static_cast<double>(x) - max) * c; }
+  // (rounded by itself: contracted with what follows it, differently where it is inlined,
+  // the sums of a group and of its vectors might not be the same whole number)
+  __device__ __forceinline__ double exponent(float x) const { return __dmul_rn(static_cast<double>(x) - max, c); }
   __device__ __forceinline__ int bin(float x) const {
     return __float2int_rn(fminf(fminf(maxf - x, 3e38f) * bins, kSmBins - 1.f));
   }

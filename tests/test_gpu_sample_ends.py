@@ -61,3 +61,22 @@ def test_top_p_just_below_one(t, dtype):
         assert tok.tolist() == [w[0] for w in want], p
         for a, (_, b, _) in zip(lp.tolist(), want):
             assert abs(a - b) <= 2 ** -24 * abs(b) + 151936 * 2 ** -45 + 1e-12
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("s", [dict(), dict(min_p=1e-4), dict(top_k=3000), dict(top_p=0.97), dict(top_k=900, min_p=0.002)])
+def test_a_token_for_every_random_number(s, dtype):
+    """The sums of groups, of a group's vectors and of a vector's logits, each formed where it is
+    needed, have to be the same whole numbers: else a number between them finds no token."""
+    n = 4096
+    g = torch.Generator().manual_seed(41)
+    x, _ = logits_of(1, 20011, 40, dtype)
+    u = torch.cat([(torch.arange(n, dtype=torch.float64) + 0.5) / n, torch.rand(n, generator=g, dtype=torch.float64)])
+    u = u.sort().values.cuda()
+    for rows in (2, 100, 2 * n):  # slices, parts of rows in global memory, whole rows
+        for at in range(0, 2 * n, rows) if rows > 2 else (0, 17, 5000):
+            part = u[at:at + rows]
+            tok, lp = ops.sample_tokens(x.cuda().expand(len(part), -1), part, 0.9, **s)
+            assert int(tok.min()) >= 0 and int(tok.max()) < 20011 and not lp.isnan().any()
+            assert (tok.diff() >= 0).all()  # as the random numbers rise, so do the ids
+            assert (x[0].cuda()[tok] > -math.inf).all()

@@ -642,7 +642,8 @@ class Qwen3MoEStack:
         """Tokens from rows of logits, by a random number each; -1 for a row that has no
         distribution (a NaN, or nothing that is finite)."""
         if temperature == 0:
-            return logits.argmax(-1)
+            most, tok = logits.max(-1)  # a NaN comes through; the first of equal logits
+            return torch.where(most.abs() < math.inf, tok, -1)
         u = torch.rand(logits.shape[0], dtype=torch.float64, device=self.device, generator=generator)
         return ops.sample_tokens(logits, u, temperature, top_k, top_p, min_p)[0]
 
@@ -744,7 +745,7 @@ class Qwen3MoEStack:
                 texts = [p.reshape(-1).tolist() for p in prompts for _ in range(samples)]
                 out = self._generate_drafted(cache, seqs, tok, texts, max_new_tokens, drafts, draw, top_logprobs, scores)
             for i in range(0 if drafts else max_new_tokens):
-                if temperature > 0 and restricted:
+                if restricted:
                     tok = draw(logits)
                 elif temperature > 0:
                     # the largest of logits + Gumbel noise is a sample of the softmax

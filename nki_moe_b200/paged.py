@@ -34,6 +34,7 @@ class CacheFull(RuntimeError):
 class _Sequence:
     def __init__(self, pages: list[int], length: int):
         self.pages, self.length = pages, length  # a page of -1 is not held (a window has passed it)
+        self.marks: dict[int, int] = {}  # the length that each was made at
 
 
 class PageTables:
@@ -52,7 +53,7 @@ class PageTables:
         self._free = list(range(num_pages))  # a heap: the lowest ids are used first
         self._refs = [0] * num_pages
         self._seqs: dict[int, _Sequence] = {}
-        self._next = 0
+        self._next = self._marks = 0
 
     # ------------------------------------------------------------ reading
     @property
@@ -146,6 +147,22 @@ class PageTables:
                 s.pages.append(self._take())
         return copies
 
+    def mark(self, seq: int) -> int:
+        """A mark of the positions that ``seq`` holds now, for :meth:`kept`."""
+        s, self._marks = self._seq(seq), self._marks + 1
+        s.marks[self._marks] = s.length
+        return self._marks
+
+    def kept(self, seq: int, mark: int) -> bool:
+        """Whether ``seq`` holds the positions of ``mark`` and no others, none of them having been
+        taken back since."""
+        s = self._seqs.get(seq)
+        return s is not None and s.marks.get(mark) == s.length
+
+    def unmark(self, seq: int, mark: int) -> None:
+        """Forgets a mark."""
+        self._seq(seq).marks.pop(mark, None)
+
     def alone(self, seq: int, start: int) -> bool:
         """Whether ``seq`` shares none of its pages from position ``start`` on."""
         return all(p < 0 or self._refs[p] == 1 for p in self._seq(seq).pages[start // self.page_size:])
@@ -162,6 +179,7 @@ class PageTables:
             while len(s.pages) > -(-n // self.page_size):
                 self._drop(s.pages.pop())
             s.length = n
+            s.marks = {m: at for m, at in s.marks.items() if at <= n}
 
     def _take(self) -> int:
         page = heapq.heappop(self._free)

@@ -79,7 +79,9 @@ def _token_ids(t: torch.Tensor, vocab: int) -> torch.Tensor:
 class DraftStep:
     """A step with drafted tokens that waits for :meth:`Qwen3MoEStack.accept_paged`."""
 
+    cache: PagedKVCache
     seqs: list
+    marks: list  # of the sequences with its nodes
     lengths: list  # of the sequences before it
     nodes: list  # of each tree
     tokens: torch.Tensor  # packed, as ops.accept_drafts takes them
@@ -597,7 +599,7 @@ class Qwen3MoEStack:
         with _appending(cache, seqs, nodes):
             cu = torch.zeros(len(seqs) + 1, dtype=torch.int32)
             cu[1:] = torch.tensor(nodes).cumsum(0)
-            step = DraftStep(seqs, lengths, nodes,
+            step = DraftStep(cache, seqs, [cache.mark(q) for q in seqs], lengths, nodes,
                              torch.cat([t.reshape(-1).to(self.device, torch.int64) for t in tokens]),
                              torch.tensor([x for p in parents for x in p], dtype=torch.int32).to(self.device),
                              cu.to(self.device),
@@ -624,7 +626,9 @@ class Qwen3MoEStack:
         sequence, the other nodes leave it.  Returns for each sequence the rows of
         its path: ``sampled[rows[i]]`` are its new tokens, of which the last is not
         in the cache yet."""
-        if step.ended or any(q not in cache or cache.length(q) != n + m for q, n, m in zip(step.seqs, step.lengths, step.nodes)):
+        if cache is not step.cache:
+            raise ValueError("the step is of another cache")
+        if step.ended or not all(cache.kept(q, m) for q, m in zip(step.seqs, step.marks)):
             raise ValueError("the sequences are not as the step left them")
         if not all(cache.alone(q, n) for q, n in zip(step.seqs, step.lengths)):
             raise ValueError("a sequence was forked between its step and the step's end")
@@ -632,6 +636,8 @@ class Qwen3MoEStack:
                                             cache.table(step.seqs).to(self.device))
         counts = counts.tolist()
         step.ended = True
+        for q, m in zip(step.seqs, step.marks):
+            cache.unmark(q, m)
         cache.take_back(step.seqs, [n + k for n, k in zip(step.lengths, counts)])
         for q in step.seqs:
             cache.trim(q)

@@ -117,3 +117,34 @@ def test_the_python_calls_refuse_host_tensors():
         ops.accept_drafts(i.long(), i.long(), i, i, i[:3], z.view(1, 1, 4, 10), i.view(1, 4))
     with pytest.raises(ValueError):
         ops.paged_tree_attention(z.bfloat16(), z, z, i, i, i[:3], z, z, i.view(1, 4), 1, 1)
+
+
+def test_marks_end_with_the_positions_they_are_of():
+    t = PageTables(10, 16, 6)
+    a = t.add()
+    t.extend([a], [20])
+    m = t.mark(a)
+    assert t.kept(a, m) and not t.kept(a, m + 1) and not t.kept(7, m)
+    t.extend([a], [5])
+    assert not t.kept(a, m)
+    b = t.fork(a)
+    t.take_back([a], [20])  # what came behind is gone, the marked ones never were
+    assert t.kept(a, m) and not t.kept(b, m)
+    t.compact()
+    t.trim(a)
+    with pytest.raises(RuntimeError):
+        t.extend([a, b], [70, 70])  # nothing was changed
+    assert t.kept(a, m)
+    n = t.mark(a)
+    t.take_back([a], [19])
+    t.extend([a], [1])  # as long as before
+    assert not t.kept(a, m) and not t.kept(a, n)
+    k = t.mark(a)
+    assert t.kept(a, k)
+    t.unmark(a, k)
+    assert not t.kept(a, k)
+    k = t.mark(a)
+    t.free(a)
+    assert not t.kept(a, k)
+    with pytest.raises(ValueError):
+        t.mark(a)

@@ -55,3 +55,39 @@ def test_greedy_draws_name_the_first_of_equal_logits(pair):
     x[3, 9] = math.nan
     x[4, 11:] = -math.inf
     assert st._draw(x, 0.0, 0, 1.0, 0.0, None).tolist() == [0, 300, -1, -1, 0]
+
+
+def test_a_step_that_others_have_overtaken_is_refused(pair):
+    """Its nodes' rows are not in the cache any more, or not in this one."""
+    _, st = pair
+    text = ids(60, 3)
+    cache, other = (st.paged_cache(20, page_size=16) for _ in range(2))
+    a, b = cache.add(), other.add()
+    for c, q in ((cache, a), (other, b)):
+        st.prefill_paged(c, [q], [text[:40]])
+    assert a == b
+    sampled = text[41:46].cuda()
+    _, old = st.draft_paged(cache, [a], [ids(5, 1)])
+    st.draft_paged(other, [b], [text[40:45]])
+    with pytest.raises(ValueError, match="cache"):
+        st.accept_paged(other, old, sampled)
+    cache.take_back([a], [40])
+    _, new = st.draft_paged(cache, [a], [text[40:45]])  # as many nodes
+    with pytest.raises(ValueError, match="left"):
+        st.accept_paged(cache, old, sampled)
+    rows = st.accept_paged(cache, new, sampled)
+    assert rows[0].tolist() == [0, 1, 2, 3, 4] and cache.length(a) == 45
+    # ended, put back, and grown to the same length by other calls
+    _, old = st.draft_paged(cache, [a], [text[45:48]])
+    cache.take_back([a], [45])
+    st.prefill_paged(cache, [a], [text[45:48]])
+    with pytest.raises(ValueError, match="left"):
+        st.accept_paged(cache, old, text[46:49].cuda())
+    assert cache.length(a) == 48
+    # a call behind its nodes that was put back does not touch them
+    _, step = st.draft_paged(cache, [a], [text[48:51]])
+    st.decode_paged(cache, [a], text[:1], graph=False)
+    with pytest.raises(ValueError, match="left"):
+        st.accept_paged(cache, step, text[49:52].cuda())
+    cache.take_back([a], [51])
+    assert st.accept_paged(cache, step, text[49:52].cuda())[0].tolist() == [0, 1, 2] and cache.length(a) == 51

@@ -15,7 +15,6 @@ namespace nkimoe {
 namespace {
 
 constexpr int kStoreThreads = 256;
-constexpr int kStoreFew = 4 * 148;  // rows that get a CTA each
 
 struct StoreParams {
   const __nv_bfloat16* qkv;  // [T, (nq + 2 nkv) * 128]
@@ -219,6 +218,9 @@ RopeTurns rope_turns(float theta) {
   return r;
 }
 
+// Rows that get a CTA each.
+static int store_few() { return 4 * device_sm_count(); }
+
 static StoreParams store_params(const __nv_bfloat16* qkv, const void* qw, const void* kw, int w_dtype,
                                 const int* cu_seqlens, const int* kv_lens, const PagedCache& cache,
                                 __nv_bfloat16* q_out, long long T, int B, int nq, float theta, float eps, int* status) {
@@ -249,7 +251,7 @@ cudaError_t paged_store_launch(const __nv_bfloat16* qkv, const void* qw, const v
   // few rows: a CTA's eight warps on each; many: a warp each, so that the lookups
   // and the sines of a row are done once (8192 rows of 32 + 2 * 4 heads, before keys
   // were formed again: 37 us, with two warps 46, with eight 42)
-  if (T <= kStoreFew)
+  if (T <= store_few())
     return launch_pdl(paged_store_kernel<8, StoreParams>, dim3(static_cast<unsigned>(T)), dim3(kStoreThreads), 0, s, p);
   return launch_pdl(paged_store_kernel<1, StoreParams>, dim3(static_cast<unsigned>((T + 7) / 8)), dim3(kStoreThreads), 0, s,
                     p);
@@ -266,9 +268,9 @@ cudaError_t paged_tree_store_launch(const __nv_bfloat16* qkv, const void* qw, co
   // steps are hundreds of rows: eight warps on each as long as all CTAs run at
   // once, then four (the whole step, 16 trees of 49 to 64 nodes = 913 rows: with
   // four 115 us, two 122, eight 120, one 127; 8 trees of 8: 20, 23, 19 us)
-  if (T <= kStoreFew / 2)
+  if (T <= store_few() / 2)
     return launch_pdl(paged_store_kernel<8, TreeStoreParams>, dim3(static_cast<unsigned>(T)), dim3(kStoreThreads), 0, s, p);
-  if (T <= 4 * kStoreFew)
+  if (T <= 4 * store_few())
     return launch_pdl(paged_store_kernel<4, TreeStoreParams>, dim3(static_cast<unsigned>((T + 1) / 2)), dim3(kStoreThreads), 0,
                       s, p);
   return launch_pdl(paged_store_kernel<1, TreeStoreParams>, dim3(static_cast<unsigned>((T + 7) / 8)), dim3(kStoreThreads), 0,

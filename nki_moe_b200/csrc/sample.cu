@@ -58,7 +58,6 @@ constexpr int kSmBinsPerOctave = 32;
 constexpr int kSmList = 2048;        // tokens that the last sort takes
 constexpr int kSmCluster = 8;        // CTAs per row at most
 constexpr int kSmSlice = 75 * 1024;  // bytes of a row per CTA that two CTAs per SM leave room for
-constexpr int kSmWholeRows = 148;    // bf16 rows that stay in global memory even where slices would fit
 constexpr int kSmValues = 2048;      // values of a sign that have a bin
 constexpr int kSmNear = 512;         // logits nearer to zero that a CTA sums
 constexpr int kSmMaxVocab = 1 << 18;
@@ -1335,9 +1334,9 @@ cudaError_t sm_launch(const SmParams& params, long long rows, cudaStream_t s) {
   // 100 rows of 151936 bf16 with top-p take 46 us so, as slices of four CTAs each, in two
   // rounds, 58; 70 rows, whose slices fit, 33 us as slices
   const long long room = 2 * device_sm_count();
-  // (bf16 rows of 18000 with filters, 150 of them: 23.1 us, as slices 25.7; fp32 rows of 500: 11.3
-  // and 6.6 us, of 18000 20.2 and 17.3)
-  const bool stream = rows * ranks > room || (sizeof(T) == 2 && rows >= kSmWholeRows);
+  // (bf16 rows do from one per SM on even where slices would fit: of 18000 with filters, 150 of
+  // them: 23.1 us, as slices 25.7; fp32 rows of 500: 11.3 and 6.6 us, of 18000 20.2 and 17.3)
+  const bool stream = rows * ranks > room || (sizeof(T) == 2 && rows >= device_sm_count());
   if (stream) ranks = kSmCluster;
   while (stream && ranks > 1 && rows * ranks > room) ranks /= 2;
   const bool alone = stream && ranks == 1;

@@ -28,6 +28,13 @@ constexpr long long kWaitBudgetCycles = 4000000000LL;
 // it before its first global-memory access (so completion stays transitive
 // along the stream).  pdl_launch_dependents() lets the stream's next kernel be
 // launched early; that kernel still waits in its own pdl_wait().
+//
+// One kernel touches global memory before its wait: paged_tree_kernel, what its
+// own store kernel (paged_store_kernel of trees) does not write, but for the
+// status word, which both change by atomics.  That store calls
+// pdl_launch_dependents() only after its pdl_wait(), so all that came before it
+// has completed when the attention starts.  The two are launched one directly
+// behind the other; a kernel between them would have to keep that order.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

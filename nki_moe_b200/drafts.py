@@ -4,8 +4,9 @@ A draft is a tree of token ids, given in an order in which every node comes
 after its parent: ``(tokens, parents)``, ``parents[i]`` being the index of node
 ``i``'s parent or -1 for one that follows the sequence's last token.  Whoever
 checks it (:meth:`nki_moe_b200.qwen_stack.Qwen3MoEStack.generate_paged`) keeps the
-path that the model itself would have taken, so a draft changes how many steps a
-text takes and nothing else about it.
+path that the model itself takes, so a wrong draft never gets into a text; a draft
+changes how many steps it takes.  (To the arithmetic: a step with drafts rounds in
+other places than one without, so among nearly equal logits the choice may differ.)
 
 The reference decodes one token a step; nothing there corresponds to this module.
 """

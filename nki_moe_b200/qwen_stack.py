@@ -706,8 +706,10 @@ class Qwen3MoEStack:
         distribution that they restrict (:func:`nki_moe_b200.ops.sample_tokens`).
         With ``drafts`` each step checks up to so many tokens (at most 63) that the
         text itself suggests (:class:`nki_moe_b200.drafts.LookupDrafts`) and keeps
-        those that the model agrees with: the tokens are the model's own, in fewer
-        steps where texts repeat; steps are not captured then.  With ``window`` the model attends to the last
+        those that the model agrees with: every token is drawn from the model's own
+        logits for the text before it, in fewer steps where texts repeat (near ties
+        between logits may fall the other way than without drafts, whose steps round
+        elsewhere); steps are not captured then.  With ``window`` the model attends to the last
         ``window`` tokens and the first ``sinks`` ones; a ``cache`` that is given
         brings its own page size and window.  Returns ``(tokens
         [len(prompts), samples, max_new_tokens], scores)``; ``scores`` is None

@@ -11,8 +11,9 @@
 // thread that writes it: the moves need no second buffer.
 //
 // What bounds it: bytes where many rows move (64 trees of 31 nodes, 44 MB in 96 planes
-// of 4 heads: 9.9 us, 4.5 TB/s of a measured copy's 6.5), else the chain lengths ->
-// parents and tokens -> page ids -> rows (8 trees of 8: 3.3 us).  A sequence's tree is
+// of 4 heads: 10 us from the L2, 19 from HBM, a kernel's start and the chain among it),
+// else the chain lengths -> parents and tokens -> page ids -> rows (8 trees of 8: 3.5 us,
+// cold 6).  A sequence's tree is
 // walked by every CTA that moves its rows, as a path that another CTA would hand over
 // takes a launch or a wait, which cost as much as the whole.
 //

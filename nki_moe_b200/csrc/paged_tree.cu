@@ -26,7 +26,9 @@
 // queries rounded too the output's error against 64 bits is 1.8 times that of its
 // own rounding, so 1.4 times; weights as hi + lo bring it to 1.0, but take 2500
 // cycles more per block (37 sequences of 16 nodes over 16 K: 290 us, so 228, and
-// with rounded queries 201).
+// with rounded queries 201).  The attention of prompts rounds its weights the same way;
+// the decode step, whose MMAs have idle rows for it, keeps them to 2^-17, so logits
+// after a node are not bit for bit those of a decode step.
 //
 // Work: the blocks of all (sequence, kv head, tile) form one list, and every CTA
 // takes an equal run of it, so sequences of any mix of lengths load all SMs alike
@@ -35,11 +37,12 @@
 // store lets this kernel start only once all that came before it has ended, so
 // what the store does not write may be read at once.
 //
-// Bounds and figures (B200, 32 heads over 4, all three kernels): trees of 13 over 30011
-// places 28.6 us, 40 ragged ones over 1 to 32768 71 us (4.1 TB/s of 6.5): 1.6 us per
+// Bounds and figures (B200, 32 heads over 4, all three kernels; replays, so from the L2
+// as far as the cache fits, in brackets from HBM): trees of 13 over 30011
+// places 29 us (36), 40 ragged ones over 1 to 32768 72 us (77, 3.8 TB/s of 6.5): 1.6 us per
 // block of a CTA, beginnings and ends of items, and 2 to 2.5 us for each kernel's
-// start.  8 trees of 8 over 512 to 639: 17.4 us, that chain with two blocks.  16 trees
-// of 49 to 64 nodes: 112 us, two chains of scores, softmax and products per SM.
+// start.  8 trees of 8 over 512 to 639: 18 us (24), that chain with two blocks.  16 trees
+// of 49 to 64 nodes: 111 us (119), two chains of scores, softmax and products per SM.
 #include "paged_tree.cuh"
 
 namespace nkimoe {

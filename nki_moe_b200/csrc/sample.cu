@@ -29,13 +29,18 @@
 //         CTA, or, with more tokens than that takes, split further by its own
 //         smallest and largest (logit, id).
 //
-// Bounds and figures (B200, 151936 logits a row, device time): 8 bf16 rows with top-k
-// and top-p 20 us, a chain of some 20 barriers of a cluster; 1024 rows with top-p 209 us
-// (1.5 TB/s of 6.5): an SM has two rows at a time and 3.46 rounds of them, of 60 us a
+// Bounds and figures (B200, 151936 logits a row, device time of replays, so from the L2
+// as far as the rows fit; where they come from HBM 6 to 12 us more, a kernel's start and
+// its instructions among it): 8 bf16 rows with top-k
+// and top-p 20 us (cold 33), a chain of some 20 barriers of a cluster; 1024 rows with top-p 208 us
+// (215; 1.5 TB/s of 6.5): an SM has two rows at a time and 3.46 rounds of them, of 60 us a
 // row 25 go to the counting pass (7 operations and a shared atomic a logit, whose banks
 // conflict 3.3 times), 12 to the borders and the table of weights, 16 to the sums and 6
-// to the draw.  fp32 with top-p, 290 rows: 284 us, 14 operations in 64 bits per logit
-// and pass; without filters 119, with min-p alone 62.
+// to the draw.  fp32 with top-p, 290 rows: 265 to 284 us, 14 operations in 64 bits per logit
+// and pass; without filters 120, with min-p alone 62.
+// At two CTAs per SM a thread has 64 registers, and the instances spill, of bytes of
+// stack: bf16 slices 88, bf16 in global memory 288 (a whole row per CTA 216), fp32 in
+// global memory 184 (128), fp32 slices 0; sm_values' bins of a thread are most of it.
 //
 // Reference: the sampling of the reference's runtime is not vendored; no
 // kernel of its own.

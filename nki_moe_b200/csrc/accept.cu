@@ -44,6 +44,32 @@ struct AcParams {
   int B, planes, per_cta, num_pages, max_pages, page_size, row16, units;  // units: 16-byte columns of a plane's row
 };
 
+// Nodes of sequence b, -1 where its lengths make no sense.
+__device__ __forceinline__ int ac_nodes(const AcParams& p, int b) {
+  const int lo = p.cu[b], hi = p.cu[b + 1], kv = p.kv_lens[b];
+  if (lo < 0 || hi < lo || hi > p.T) return -1;  // (the difference of two that make no sense may pass 32 bits)
+  const int n = hi - lo;
+  return n <= kTreeNodes && kv >= n && kv <= static_cast<long long>(p.max_pages) * p.page_size ? n : -1;
+}
+
+// A warp: -1 for the rows [from, end), which no path is in.  Where starts do not rise they
+// may lie in another sequence, whose own they are then.
+__device__ __noinline__ void ac_none(const AcParams& p, long long from, long long end, int lane) {
+  from = max(from, 0LL);
+  end = min(end, p.T);
+  if (from >= end) return;
+  bool rise = true;
+  for (int q = lane; q < p.B; q += 32) rise = rise && p.cu[q] <= p.cu[q + 1];
+  rise = __all_sync(0xffffffffu, rise);
+  for (long long i = from + lane; i < end; i += 32) {
+    bool owned = false;
+    for (int q = 0; !rise && q < p.B; ++q) owned = owned || (ac_nodes(p, q) > 0 && p.cu[q] <= i && i < p.cu[q + 1]);
+    if (owned) continue;
+    p.path[i] = -1;
+    p.new_tokens[i] = -1;
+  }
+}
+
 // CTA (group of planes, sequence); every CTA walks its sequence's tree itself,
 // two nodes a lane, and then moves the path's rows, a thread a column of 16 bytes.
 __global__ void __launch_bounds__(kAcThreads) accept_drafts_kernel(const __grid_constant__ AcParams p) {
@@ -53,12 +79,9 @@ __global__ void __launch_bounds__(kAcThreads) accept_drafts_kernel(const __grid_
   pdl_launch_dependents();
   pdl_wait();
   if (threadIdx.x < 32) {
-    const int lo = p.cu[b], hi = p.cu[b + 1], kv = p.kv_lens[b];
-    const bool rows = lo >= 0 && hi >= lo && hi <= p.T;
-    const int n = rows ? hi - lo : 0;  // (the difference of two that make no sense may pass 32 bits)
-    const bool valid = rows && n <= kTreeNodes && kv >= n && kv <= static_cast<long long>(p.max_pages) * p.page_size;
+    const int lo = p.cu[b], hi = p.cu[b + 1], kv = p.kv_lens[b], n = ac_nodes(p, b);
     int count = 0;
-    if (valid && n > 0) {
+    if (n > 0) {
       int par[2];
       long long tok[2], sam[2];
 #pragma unroll
@@ -103,24 +126,18 @@ __global__ void __launch_bounds__(kAcThreads) accept_drafts_kernel(const __grid_
           p.new_tokens[lo + k] = i >= 0 ? p.sampled[lo + i] : -1;
         }
       }
-    } else if (!valid && lane == 0) {
+    } else if (n < 0 && lane == 0) {
       atomicOr(p.status, kDevErrBadIndex);
     }
     if (lane == 0) {
       s_count = count;
       if (blockIdx.x == 0) p.counts[b] = count;
     }
-    if (blockIdx.x == 0) {  // rows without a path: of a refused sequence, of none before the first or behind the last
-      auto none = [&](long long from, long long end) {
-        for (long long i = max(from, 0LL) + lane; i < min(end, p.T); i += 32) {
-          p.path[i] = -1;
-          p.new_tokens[i] = -1;
-        }
-      };
-      if (!valid) none(lo, hi);
-      if (b == 0) none(0, lo);
-      if (b == p.B - 1) none(hi, p.T);
-    }
+  } else if (blockIdx.x == 0 && threadIdx.x < 64) {
+    // rows without a path: of a refused sequence, of none before the first or behind the last
+    if (ac_nodes(p, b) < 0) ac_none(p, p.cu[b], p.cu[b + 1], lane);
+    if (b == 0) ac_none(p, 0, p.cu[0], lane);
+    if (b == p.B - 1) ac_none(p, p.cu[p.B], p.T, lane);
   }
   __syncthreads();
   const int count = s_count;

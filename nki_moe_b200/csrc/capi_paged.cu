@@ -390,7 +390,13 @@ int nkimoe_accept_drafts(const int64_t* tokens, const int64_t* sampled, const in
               NKIMOE_ERR_UNSUPPORTED, "shape too large");
   NKI_REQUIRE(max_pages <= (1LL << 30) / page_size, NKIMOE_ERR_UNSUPPORTED, "sequences over 2^30 positions");
   NKI_REQUIRE(table_stride >= max_pages, NKIMOE_ERR_INVALID_ARG, "page table rows overlap");
-  if (T == 0 || batch == 0) return NKIMOE_OK;
+  if (T == 0 || batch == 0) {  // no paths; rows of no sequence
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (batch > 0 && counts) NKI_CUDA(cudaMemsetAsync(counts, 0, sizeof(int32_t) * batch, s));
+    if (T > 0 && path) NKI_CUDA(cudaMemsetAsync(path, 0xff, sizeof(int32_t) * T, s));
+    if (T > 0 && new_tokens) NKI_CUDA(cudaMemsetAsync(new_tokens, 0xff, sizeof(int64_t) * T, s));
+    return NKIMOE_OK;
+  }
   NKI_REQUIRE(tokens && sampled && parents && cu_seqlens && kv_lens && pages && page_table && counts && path &&
                   new_tokens && status,
               NKIMOE_ERR_INVALID_ARG, "null pointer");

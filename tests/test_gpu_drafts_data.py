@@ -119,3 +119,31 @@ def test_rows_without_a_path_are_minus_one(starts, lens, paths, monkeypatch):
     assert counts.tolist() == [len(paths.get(b, [])) for b in range(B)]
     assert torch.equal(path.cpu(), want)
     assert torch.equal(new.cpu(), torch.where(want >= 0, 1, -1))
+
+
+@pytest.mark.parametrize("starts,paths", [
+    ([0, 70, 4, 8], {2: [4, 5, 6, 7]}),  # the first would have what the third has
+    ([0, 4, 8, 2], {0: [0, 1, 2, 3], 1: [4, 5, 6, 7]}),  # and what lies behind the last
+    ([6, 2, 9, 9], {1: [2, 3, 4, 5, 6, 7, 8]}),  # and before the first
+])
+def test_rows_of_others_are_left_to_them(starts, paths, monkeypatch):
+    """Where starts do not rise, a refused sequence's rows may be another's."""
+    monkeypatch.setenv("NKIMOE_SYNC_CHECK", "0")
+    for _ in range(5):
+        test_rows_without_a_path_are_minus_one(starts, [70] * 3, paths, monkeypatch)
+
+
+def test_calls_of_no_sequences_and_of_no_rows():
+    """Through the C entry: the outputs are written all the same."""
+    from nki_moe_b200 import _lib
+
+    tok = torch.ones(9, dtype=torch.int64, device="cuda")
+    pages = torch.zeros(1, 2, 1, 16, 8, dtype=torch.bfloat16, device="cuda")
+    table, status = ints(0, 1).view(1, 2), torch.zeros(64, dtype=torch.int32, device="cuda")
+    for T, B in ((9, 0), (0, 1)):
+        counts, path, new = ints(7), ints(*[7] * 9), torch.full((9,), 7, dtype=torch.int64, device="cuda")
+        _lib.call("nkimoe_accept_drafts", tok.data_ptr(), tok.data_ptr(), path.data_ptr(), ints(0, 0).data_ptr(),
+                  ints(0).data_ptr(), pages.data_ptr(), 1, 2, 1, 16, 16, table.data_ptr(), 2, 2, counts.data_ptr(),
+                  path.data_ptr(), new.data_ptr(), T, B, status.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert (path.tolist(), new.tolist()) == (([-1] * 9,) * 2 if B == 0 else ([7] * 9,) * 2)
+        assert counts.tolist() == [7 if B == 0 else 0]

@@ -1045,10 +1045,10 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_tokens_kernel(const __gr
     if (by_p) sm_select<true>(cl, sh, sl, row, top_p);
   }
 
-  // what weighs less than min_p need not be looked at: a bound a little below it
-  // (the weights themselves decide)
+  // what weighs less than min_p need not be looked at: a bound a little below it, by
+  // 2^-30 of a binary order and the rounding of the logit (the weights themselves decide)
   if (row.min_weight > 0.0) {
-    float bound = static_cast<float>(row.max + log2(row.min_weight) / row.c);
+    float bound = static_cast<float>(row.max + (log2(row.min_weight) - 0x1p-30) / row.c);
     bound -= fabsf(bound) * 0x1p-22f + 1e-30f;
     if (bound > row.least) {
       row.least = bound;

@@ -80,3 +80,22 @@ def test_a_token_for_every_random_number(s, dtype):
             assert int(tok.min()) >= 0 and int(tok.max()) < 20011 and not lp.isnan().any()
             assert (tok.diff() >= 0).all()  # as the random numbers rise, so do the ids
             assert (x[0].cuda()[tok] > -math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 200])
+def test_weights_that_round_to_the_largest_are_at_least_as_large(rows, dtype):
+    """Near zero logits may differ by less than their weights can."""
+    g = torch.Generator().manual_seed(51)
+    x = -torch.rand(rows, 2011, generator=g) * 10.0 ** -torch.randint(17, 30, (rows, 2011), generator=g)
+    x[:, 1000:] -= 1.0
+    x[:, 7] = 0.0
+    x = x.to(dtype)
+    u = torch.rand(rows, generator=g, dtype=torch.float64)
+    for t in (1.0, 3.0, math.inf):
+        temperature = torch.full((rows,), t, device="cuda")
+        tok, lp = ops.sample_tokens(x.cuda(), u.cuda(), temperature, 0, 1.0, 1.0)
+        for i in range(0, rows, 11):
+            want, want_lp, _ = drawn(x[i], u[i].item(), t, 0, 1.0, 1.0)
+            assert int(tok[i]) == want
+            assert abs(float(lp[i]) - want_lp) <= 2 ** -24 * abs(want_lp) + 2011 * 2 ** -45 + 1e-12
